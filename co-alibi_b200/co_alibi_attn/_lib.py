@@ -15,6 +15,7 @@ ERR_TIMEOUT = 10
 
 c_int, c_uint, c_float, c_void_p, c_size_t = (ctypes.c_int, ctypes.c_uint, ctypes.c_float,
                                               ctypes.c_void_p, ctypes.c_size_t)
+c_int64 = ctypes.c_longlong
 
 
 class CoalibiFwdArgs(ctypes.Structure):
@@ -39,10 +40,39 @@ class CoalibiBwdArgs(ctypes.Structure):
     ]
 
 
+class CoalibiPagedAppendArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("k", "v", "q", "q_out", "k_pages", "v_pages", "page_table", "start", "count",
+                                        "positions", "cos", "sin", "status")]
+    _fields_ += [(n, c_int64 * 3) for n in ("k_stride", "v_stride", "q_stride", "q_out_stride", "k_page_stride",
+                                            "v_page_stride")]
+    _fields_ += [("table_stride", c_int64)]
+    _fields_ += [(n, c_int) for n in ("B", "Hq", "Hkv", "S", "D", "page_size", "max_pages", "n_pages", "rot", "n_pos",
+                                      "interleaved", "dtype")]
+
+
+class CoalibiPagedAttentionArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("q", "o", "k_pages", "v_pages", "slopes", "page_table", "ctx_lens",
+                                        "tree_mask", "status")]
+    _fields_ += [(n, c_int64 * 3) for n in ("q_stride", "o_stride", "k_page_stride", "v_page_stride")]
+    _fields_ += [("table_stride", c_int64), ("mask_stride", c_int64)]
+    _fields_ += [(n, c_int) for n in ("B", "Hq", "Hkv", "Sq", "D", "page_size", "max_pages", "n_pages", "dtype",
+                                      "slopes_dtype")]
+    _fields_ += [("sm_scale", c_float)]
+
+
+class CoalibiSampleArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("logits", "noise", "temperature", "top_k", "top_p", "min_p", "tokens",
+                                        "logprobs")]
+    _fields_ += [("logits_stride", c_int64), ("noise_stride", c_int64)]
+    _fields_ += [("B", c_int), ("V", c_int), ("dtype", c_int), ("temperature_all", c_float), ("top_k_all", c_int),
+                 ("top_p_all", c_float), ("min_p_all", c_float)]
+
+
 EXPORTS = ("coalibi_fwd", "coalibi_fwd_decode", "coalibi_fwd_decode_workspace_bytes", "coalibi_bwd",
            "coalibi_bwd_carry", "coalibi_bwd_phases", "coalibi_bwd_noalloc", "coalibi_bwd_workspace_size",
            "coalibi_bwd_workspace_bytes", "coalibi_bwd_workspace_min_bytes", "coalibi_selftest_wait_timeout",
-           "coalibi_strerror",
+           "coalibi_paged_append", "coalibi_paged_attention", "coalibi_paged_attention_workspace_bytes",
+           "coalibi_sample", "coalibi_strerror",
            "coalibi_abi_version", "coalibi_last_error", "coalibi_describe_launch")
 
 NOALLOC_SCRATCH_BYTES = 64 << 20  # COALIBI_NOALLOC_SCRATCH_BYTES
@@ -83,6 +113,15 @@ def load():
             lib.coalibi_bwd_workspace_min_bytes.restype = c_size_t
             lib.coalibi_bwd_workspace_size.argtypes = [ctypes.POINTER(CoalibiBwdArgs)]
             lib.coalibi_bwd_workspace_size.restype = c_size_t
+            # these take the argument structs as packed bytes (serving.py) or by ctypes.byref
+            lib.coalibi_paged_append.argtypes = [c_void_p, c_void_p]
+            lib.coalibi_paged_append.restype = c_int
+            lib.coalibi_paged_attention.argtypes = [c_void_p, c_void_p, c_size_t, c_void_p]
+            lib.coalibi_paged_attention.restype = c_int
+            lib.coalibi_paged_attention_workspace_bytes.argtypes = [c_int] * 5
+            lib.coalibi_paged_attention_workspace_bytes.restype = c_size_t
+            lib.coalibi_sample.argtypes = [c_void_p, c_void_p]
+            lib.coalibi_sample.restype = c_int
             lib.coalibi_selftest_wait_timeout.argtypes = [ctypes.c_uint, c_void_p, c_void_p]
             lib.coalibi_selftest_wait_timeout.restype = c_int
             lib.coalibi_strerror.argtypes = [c_int]

@@ -223,6 +223,12 @@ int enter_device(const void* ptr, void* stream) {
   if (int rc = device_setup(ptr)) return rc;
   int dev = -1, sdev = -1;
   cudaGetDevice(&dev);
+  // A capturing stream cannot be asked for its device (the query would end the
+  // capture); one of another device fails at the launch instead.
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (stream != nullptr && cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture) == cudaSuccess &&
+      capture == cudaStreamCaptureStatusActive)
+    return COALIBI_OK;
   if (cudaStreamGetDevice(static_cast<cudaStream_t>(stream), &sdev) != cudaSuccess) {
     cudaGetLastError();
     snprintf(g_last_error, sizeof(g_last_error), "cudaStreamGetDevice failed for stream %p", stream);
@@ -579,6 +585,7 @@ extern "C" const char* coalibi_strerror(int code) {
     case COALIBI_ERR_WORKSPACE: return "backward workspace missing or too small";
     case COALIBI_ERR_DEVICE: return "current CUDA device is not an sm_100 (B200) GPU";
     case COALIBI_ERR_TIMEOUT: return "a bounded in-kernel wait timed out";
+    case COALIBI_ERR_PAGE: return "a token or page outside the paged cache was skipped";
     default: return "unknown error";
   }
 }

@@ -1,0 +1,220 @@
+// C-ABI entry points of the serving operators (declared in include/coalibi.h): paged
+// append, attention of drafted trees over a paged cache, and sampling.  Arguments are
+// checked before any device use; nothing here allocates or synchronises.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <cstdio>
+
+#include "coalibi.h"
+#include "ctx_guard.h"
+#include "paged.cuh"
+#include "sample.cuh"
+
+namespace coalibi {
+
+void set_last_error_detail(const char* msg);
+
+namespace {
+
+bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// strides of 16-byte rows: multiples of 8 elements, not negative
+bool row_strides(const long long* s) {
+  for (int i = 0; i < 3; ++i)
+    if (s[i] < 0 || s[i] % 8 != 0) return false;
+  return true;
+}
+
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return COALIBI_OK;
+  char msg[160];
+  snprintf(msg, sizeof(msg), "%s: %s", what, cudaGetErrorString(e));
+  set_last_error_detail(msg);
+  return COALIBI_ERR_LAUNCH;
+}
+
+void copy3(long long* dst, const long long* src) {
+  for (int i = 0; i < 3; ++i) dst[i] = src[i];
+}
+
+int check_cache(int B, int Hkv, int D, int page_size, int max_pages, int n_pages, int dtype,
+                const long long* k_page_stride, const long long* v_page_stride, long long table_stride) {
+  if (D != 64 && D != 128) return COALIBI_ERR_HEAD_DIM;
+  if (dtype != COALIBI_F16 && dtype != COALIBI_BF16) return COALIBI_ERR_DTYPE;
+  if (B <= 0 || Hkv <= 0 || page_size <= 0 || page_size % 16 != 0 || max_pages <= 0 || n_pages <= 0)
+    return COALIBI_ERR_SHAPE;
+  // token numbers and lengths are 32-bit on the device
+  if ((long long)max_pages * page_size > 0x7fffff00LL || table_stride < 0 || B > 65535 || Hkv > 65535)
+    return COALIBI_ERR_SHAPE;
+  if (!row_strides(k_page_stride) || !row_strides(v_page_stride)) return COALIBI_ERR_ALIGNMENT;
+  return COALIBI_OK;
+}
+
+}  // namespace
+}  // namespace coalibi
+
+using namespace coalibi;
+
+extern "C" int coalibi_paged_append(const CoalibiPagedAppendArgs* a, void* stream) {
+  if (a == nullptr || !a->k || !a->v || !a->k_pages || !a->v_pages || !a->page_table || !a->start)
+    return COALIBI_ERR_NULL_POINTER;
+  if ((a->q != nullptr) != (a->q_out != nullptr)) return COALIBI_ERR_NULL_POINTER;
+  int rc = check_cache(a->B, a->Hkv, a->D, a->page_size, a->max_pages, a->n_pages, a->dtype, a->k_page_stride,
+                       a->v_page_stride, a->table_stride);
+  if (rc) return rc;
+  if (a->S <= 0 || (long long)a->B * a->S > 0x7fffffffLL || (a->q && (a->Hq <= 0 || a->Hq > 65535)))
+    return COALIBI_ERR_SHAPE;
+  if (a->rot < 0 || a->rot > a->D || a->rot % 16 != 0 || (a->rot > 0 && a->n_pos <= 0)) return COALIBI_ERR_SHAPE;
+  if (a->rot > 0 && (!a->cos || !a->sin)) return COALIBI_ERR_NULL_POINTER;
+  if (!row_strides(a->k_stride) || !row_strides(a->v_stride) ||
+      (a->q && (!row_strides(a->q_stride) || !row_strides(a->q_out_stride))))
+    return COALIBI_ERR_ALIGNMENT;
+  if (!aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->q, 16) || !aligned(a->q_out, 16) ||
+      !aligned(a->k_pages, 16) || !aligned(a->v_pages, 16) || !aligned(a->cos, 16) || !aligned(a->sin, 16))
+    return COALIBI_ERR_ALIGNMENT;
+  CtxGuard guard;
+  if ((rc = enter_device(a->k_pages, stream))) return rc;
+  AppendParams p{};
+  p.k = a->k;
+  p.v = a->v;
+  p.q = a->q;
+  p.q_out = a->q_out;
+  p.k_pages = a->k_pages;
+  p.v_pages = a->v_pages;
+  p.page_table = a->page_table;
+  p.start = a->start;
+  p.count = a->count;
+  p.positions = a->positions;
+  p.cos = a->cos;
+  p.sin = a->sin;
+  p.status = a->status;
+  copy3(p.ks, a->k_stride);
+  copy3(p.vs, a->v_stride);
+  copy3(p.qs, a->q_stride);
+  copy3(p.qos, a->q_out_stride);
+  copy3(p.kps, a->k_page_stride);
+  copy3(p.vps, a->v_page_stride);
+  p.table_stride = a->table_stride;
+  p.Hq = a->Hq;
+  p.Hkv = a->Hkv;
+  p.S = a->S;
+  p.D = a->D;
+  p.page_size = a->page_size;
+  p.max_pages = a->max_pages;
+  p.n_pages = a->n_pages;
+  p.rot = a->rot;
+  p.n_pos = a->n_pos;
+  p.interleaved = a->interleaved;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->dtype == COALIBI_BF16)
+    coalibi_paged_append_kernel<true><<<a->B * a->S, kAppendThreads, 0, s>>>(p);
+  else
+    coalibi_paged_append_kernel<false><<<a->B * a->S, kAppendThreads, 0, s>>>(p);
+  return launched("paged append launch");
+}
+
+extern "C" size_t coalibi_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int Sq, int D) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Sq > kTreeMaxSq || Hq % Hkv != 0 || (D != 64 && D != 128)) return 0;
+  return 16;
+}
+
+extern "C" int coalibi_paged_attention(const CoalibiPagedAttentionArgs* a, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+  if (a == nullptr || !a->q || !a->o || !a->k_pages || !a->v_pages || !a->slopes || !a->page_table || !a->ctx_lens)
+    return COALIBI_ERR_NULL_POINTER;
+  int rc = check_cache(a->B, a->Hkv, a->D, a->page_size, a->max_pages, a->n_pages, a->dtype, a->k_page_stride,
+                       a->v_page_stride, a->table_stride);
+  if (rc) return rc;
+  if (a->slopes_dtype != COALIBI_F16 && a->slopes_dtype != COALIBI_BF16 && a->slopes_dtype != COALIBI_F32)
+    return COALIBI_ERR_DTYPE;
+  if (a->Hq <= 0 || a->Hq % a->Hkv != 0 || a->Hq > 65535 || a->Sq <= 0 || a->Sq > kTreeMaxSq || a->mask_stride < 0)
+    return COALIBI_ERR_SHAPE;
+  if (!row_strides(a->q_stride) || !row_strides(a->o_stride)) return COALIBI_ERR_ALIGNMENT;
+  if (!aligned(a->q, 16) || !aligned(a->o, 16) || !aligned(a->k_pages, 16) || !aligned(a->v_pages, 16) ||
+      !aligned(a->tree_mask, 8))
+    return COALIBI_ERR_ALIGNMENT;
+  if (workspace == nullptr || !aligned(workspace, 16) ||
+      workspace_bytes < coalibi_paged_attention_workspace_bytes(a->B, a->Hq, a->Hkv, a->Sq, a->D))
+    return COALIBI_ERR_WORKSPACE;
+  CtxGuard guard;
+  if ((rc = enter_device(a->k_pages, stream))) return rc;
+  PagedAttnParams p{};
+  p.q = a->q;
+  p.o = a->o;
+  p.k_pages = a->k_pages;
+  p.v_pages = a->v_pages;
+  p.slopes = a->slopes;
+  p.page_table = a->page_table;
+  p.ctx_lens = a->ctx_lens;
+  p.tree_mask = a->tree_mask;
+  p.status = a->status;
+  copy3(p.qs, a->q_stride);
+  copy3(p.os, a->o_stride);
+  copy3(p.kps, a->k_page_stride);
+  copy3(p.vps, a->v_page_stride);
+  p.table_stride = a->table_stride;
+  p.mask_stride = a->mask_stride;
+  p.B = a->B;
+  p.Hq = a->Hq;
+  p.Hkv = a->Hkv;
+  p.Sq = a->Sq;
+  p.page_size = a->page_size;
+  p.max_pages = a->max_pages;
+  p.n_pages = a->n_pages;
+  p.slopes_dtype = a->slopes_dtype;
+  p.sm_scale = a->sm_scale;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const dim3 grid(a->Sq, a->Hq, a->B);
+  const bool bf16 = a->dtype == COALIBI_BF16;
+  if (a->D == 128) {
+    if (bf16)
+      coalibi_paged_attn_kernel<128, true><<<grid, 128, 0, s>>>(p);
+    else
+      coalibi_paged_attn_kernel<128, false><<<grid, 128, 0, s>>>(p);
+  } else {
+    if (bf16)
+      coalibi_paged_attn_kernel<64, true><<<grid, 128, 0, s>>>(p);
+    else
+      coalibi_paged_attn_kernel<64, false><<<grid, 128, 0, s>>>(p);
+  }
+  return launched("paged attention launch");
+}
+
+extern "C" int coalibi_sample(const CoalibiSampleArgs* a, void* stream) {
+  if (a == nullptr || !a->logits || !a->noise || !a->tokens || !a->logprobs) return COALIBI_ERR_NULL_POINTER;
+  if (a->dtype != COALIBI_F16 && a->dtype != COALIBI_BF16 && a->dtype != COALIBI_F32) return COALIBI_ERR_DTYPE;
+  if (a->B <= 0 || a->V <= 0 || a->V > COALIBI_SAMPLE_MAX_VOCAB || a->logits_stride < 0 || a->noise_stride < 0)
+    return COALIBI_ERR_SHAPE;
+  if (!aligned(a->logits, a->dtype == COALIBI_F32 ? 4 : 2) || !aligned(a->noise, 4) || !aligned(a->tokens, 8) ||
+      !aligned(a->logprobs, 4))
+    return COALIBI_ERR_ALIGNMENT;
+  CtxGuard guard;
+  if (int rc = enter_device(a->logits, stream)) return rc;
+  SampleParams p{};
+  p.logits = a->logits;
+  p.noise = a->noise;
+  p.temperature = a->temperature;
+  p.top_k = a->top_k;
+  p.top_p = a->top_p;
+  p.min_p = a->min_p;
+  p.tokens = a->tokens;
+  p.logprobs = a->logprobs;
+  p.logits_stride = a->logits_stride;
+  p.noise_stride = a->noise_stride;
+  p.B = a->B;
+  p.V = a->V;
+  p.temperature_all = a->temperature_all;
+  p.top_k_all = a->top_k_all;
+  p.top_p_all = a->top_p_all;
+  p.min_p_all = a->min_p_all;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->dtype == COALIBI_F32)
+    coalibi_sample_kernel<2><<<a->B, kSampleThreads, 0, s>>>(p);
+  else if (a->dtype == COALIBI_BF16)
+    coalibi_sample_kernel<1><<<a->B, kSampleThreads, 0, s>>>(p);
+  else
+    coalibi_sample_kernel<0><<<a->B, kSampleThreads, 0, s>>>(p);
+  return launched("sampling launch");
+}

@@ -57,7 +57,9 @@ enum coalibi_error {
   COALIBI_ERR_TENSOR_MAP = 7,   /* cuTensorMapEncodeTiled failed or unavailable */
   COALIBI_ERR_WORKSPACE = 8,    /* workspace missing or smaller than coalibi_bwd_workspace_bytes() */
   COALIBI_ERR_DEVICE = 9,       /* device is not sm_100, or the stream is on another device */
-  COALIBI_ERR_TIMEOUT = 10      /* device status only: a bounded wait expired */
+  COALIBI_ERR_TIMEOUT = 10,     /* device status only: a bounded wait expired */
+  COALIBI_ERR_PAGE = 11         /* device status only: a token outside its page table, a page outside the
+                                   pool, or a position outside the rotary table; the access was skipped */
 };
 
 /* Forward.  Replaces the Triton launch in co_alibi_attn/co_alibi_attn.py:44-57
@@ -201,6 +203,114 @@ int coalibi_selftest_wait_timeout(unsigned int timeout_ms, int* status, void* st
  * buf_len bytes.  Launches nothing and changes no CUDA state. */
 int coalibi_describe_launch(int which, int B, int Hq, int Hkv, int Sq, int Skv, int D, int causal, int device,
                             char* buf, size_t buf_len);
+
+/* ---------------------------------------------------------------------------
+ * Serving: a decoding step of a Co-ALiBi model over a paged key/value cache.
+ * The reference has no counterpart of these.
+ *
+ * A cache is a pool of pages: k_pages and v_pages hold n_pages pages of page_size
+ * tokens (a multiple of 16) for each of Hkv heads, element (page, head, slot, d) at
+ * page * stride[0] + head * stride[1] + slot * stride[2] + d; strides in elements,
+ * multiples of 8, bases 16-byte aligned.  Token t of request b lives in page
+ * page_table[b * table_stride + t / page_size], slot t % page_size.  Lengths and
+ * tables are read on the device, so a captured graph can replay as they change;
+ * entries past a request's tokens are never used.  A token outside the table or a
+ * page outside the pool is skipped and reported as COALIBI_ERR_PAGE in *status.
+ * ------------------------------------------------------------------------- */
+
+/* Append the S new tokens (count[b] of them when count is given) of each request at
+ * tokens start[b], start[b] + 1, ... of its cache.  With rot > 0 the first rot
+ * elements of each key, and of each query when q is given, are rotated by the angle
+ * of the token's position (positions[b, i], default start[b] + i): pairs
+ * (x[i], x[i + rot / 2]), or (x[2i], x[2i + 1]) when interleaved, become
+ * (a cos - b sin, b cos + a sin) in float32, rounded once.  q_out rows past count[b]
+ * are zero.  Strides of k, v, q, q_out: batch, head, token; multiples of 8. */
+typedef struct CoalibiPagedAppendArgs {
+  const void* k;
+  const void* v;
+  const void* q;          /* optional: queries to rotate */
+  void* q_out;
+  void* k_pages;
+  void* v_pages;
+  const int* page_table;  /* [B, max_pages] */
+  const int* start;       /* [B] */
+  const int* count;       /* [B]; NULL: S */
+  const int* positions;   /* [B, S] contiguous; NULL: start[b] + i */
+  const float* cos;       /* [n_pos, rot / 2]; NULL with rot = 0 */
+  const float* sin;
+  int* status;            /* optional device int */
+  long long k_stride[3], v_stride[3], q_stride[3], q_out_stride[3];
+  long long k_page_stride[3], v_page_stride[3]; /* page, head, slot */
+  long long table_stride;
+  int B, Hq, Hkv, S, D;   /* Hq read only with q */
+  int page_size, max_pages, n_pages;
+  int rot, n_pos, interleaved; /* rot: a multiple of 16, at most D */
+  int dtype;
+} CoalibiPagedAppendArgs;
+
+int coalibi_paged_append(const CoalibiPagedAppendArgs* args, void* stream);
+
+/* Co-ALiBi attention of Sq query rows per request over its paged cache: the
+ * ctx_lens[b] context tokens, which every row sees, and the up to Sq drafted tokens
+ * after them, of which row i sees token ctx_lens[b] + t where bit t of
+ * tree_mask[b * mask_stride + i] is set (tree_mask NULL: bits 0 .. i, a chain; Sq = 1
+ * is one decoding step).  z sums the sigmoids of the keys the row sees, in cache order;
+ * a row that sees nothing gives 0.  Drafted tokens that no row of a request sees are
+ * not read.  workspace: coalibi_paged_attention_workspace_bytes() bytes, 16-byte
+ * aligned, contents on entry irrelevant, not shared by calls that may overlap. */
+#define COALIBI_TREE_MAX_SQ 64
+typedef struct CoalibiPagedAttentionArgs {
+  const void* q;          /* [B, Hq, Sq, D] by stride */
+  void* o;
+  const void* k_pages;
+  const void* v_pages;
+  const void* slopes;     /* [Hq], slopes_dtype */
+  const int* page_table;
+  const int* ctx_lens;    /* [B] */
+  const long long* tree_mask;
+  int* status;
+  long long q_stride[3], o_stride[3]; /* batch, head, row; multiples of 8 */
+  long long k_page_stride[3], v_page_stride[3];
+  long long table_stride, mask_stride; /* mask_stride 0: one mask for all requests */
+  int B, Hq, Hkv, Sq, D;
+  int page_size, max_pages, n_pages;
+  int dtype, slopes_dtype;
+  float sm_scale;
+} CoalibiPagedAttentionArgs;
+
+size_t coalibi_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int Sq, int D);
+int coalibi_paged_attention(const CoalibiPagedAttentionArgs* args, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* Draw one token for each row of logits.  Tokens are ranked by (logit descending,
+ * index ascending) and weighted w = exp((logit - max) / temperature); kept are the
+ * first top_k (0: all), of those the shortest prefix whose weights reach top_p of
+ * their sum (>= 1: all, at least one stays), of those w >= min_p.  The token is the
+ * kept one with the largest w / noise: with noise drawn from Exp(1) that samples the
+ * renormalised distribution.  temperature <= 0: the first of the ranking.  Logits of
+ * -inf or NaN are never drawn; +inf logits share all the weight.  logprobs[b] is the
+ * drawn token's log-probability among the kept.  A row with nothing to draw gives
+ * token -1, logprob -inf.  Sums are exact in 64-bit fixed point: results repeat bit
+ * for bit. */
+#define COALIBI_SAMPLE_MAX_VOCAB (1 << 21)
+typedef struct CoalibiSampleArgs {
+  const void* logits;       /* [B, V], row stride logits_stride elements */
+  const float* noise;       /* [B, V], row stride noise_stride */
+  const float* temperature; /* [B], or NULL: temperature_all; the same for the next three */
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  long long* tokens;        /* [B] */
+  float* logprobs;          /* [B] */
+  long long logits_stride, noise_stride;
+  int B, V;
+  int dtype;                /* float16, bfloat16 or float32 */
+  float temperature_all;
+  int top_k_all;
+  float top_p_all, min_p_all;
+} CoalibiSampleArgs;
+
+int coalibi_sample(const CoalibiSampleArgs* args, void* stream);
 
 /* Static name of an error code. */
 const char* coalibi_strerror(int code);
