@@ -242,14 +242,13 @@ int enter_device(const void* ptr, void* stream) {
   return COALIBI_OK;
 }
 
-namespace {
-
-// SM count of the current device (device_setup has run for it)
-int current_sm_count() {
+int device_sm_count() {
   int dev = 0;
   cudaGetDevice(&dev);
   return g_dev[dev].sm_count;
 }
+
+namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -283,7 +282,7 @@ int launch_fwd_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensor
   // end, so each CTA then takes one item and the hardware balances (measured:
   // B = 1, 2 at H16 S4096 one-item 25% faster; B = 4, 8 persistent 2-4% faster).
   const int n_items = p.B * p.Hq * p.n_qtiles;
-  const int sms = current_sm_count();
+  const int sms = device_sm_count();
   const int grid = (n_items >= 12 * sms) ? sms : n_items;
   cudaError_t e = launch_pdl(coalibi_fwd_kernel<D, BF16>, dim3(grid), dim3(FwdLayout<D>::THREADS), FwdLayout<D>::ALLOC,
                              stream, tq, tk, tv, p);

@@ -29,4 +29,7 @@ class CtxGuard {
 // that device.  Returns COALIBI_OK or an error code (detail in coalibi_last_error).
 int enter_device(const void* ptr, void* stream);
 
+// SM count of the current device, after enter_device has run for it.
+int device_sm_count();
+
 }  // namespace coalibi

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "sm100.cuh"
+#include "decode.cuh"
 #include "fwd.cuh"
 
 namespace coalibi {
@@ -123,9 +124,24 @@ __global__ void __launch_bounds__(kAppendThreads) coalibi_paged_append_kernel(co
 }
 
 // ---------------------------------------------------------------------------
-// Attention.  One CTA per (request, query head, row): the keys right to left in
-// blocks of 128, one key per thread; a block-wide suffix sum of the sigmoids gives z,
-// then an online softmax and, one column per thread, the weighted sum of V.
+// Attention.  Per row i and key j, keys in cache order:
+//   x_j = scale q.k_j,  s_j = 1 / (1 + e^-x_j),  z_j = sum of s over the seen keys >= j,
+//   o = sum_j e^(x_j - slope z_j) v_j / sum_j e^(x_j - slope z_j).
+// A piece [lo, hi) of the keys, walked right to left with z restarted at 0, gives
+// (T, m, l, O): its sigmoid total, largest logit, weight sum and weighted V.  The keys
+// right of it add the constant R (their total) to every z in it, that is -slope R to
+// every logit, so pieces join exactly: m' = m - slope R, then the usual log-sum-exp merge.
+//
+// What must move is K and V, once per kv head: the G * Sq rows that share them go
+// through the tensor cores together, 16 to a warp.  A CTA has four warps: RW of them
+// side by side over the rows and KG = 4 / RW over the keys.  Up to 64 rows the kernel
+// is bound by the reads; the warp-level MMA is enough for that, and its fragments can be
+// scanned in registers.
+//
+// The work is cut evenly, whatever the lengths: items (request, kv head, block of RW *
+// 16 rows) are laid end to end in units of 32 * KG keys, and each of a grid of resident
+// CTAs takes an equal run of units.  An item inside one run is finished there; the
+// pieces of one that spans runs go to the workspace and a second kernel joins them.
 // ---------------------------------------------------------------------------
 struct PagedAttnParams {
   const void* q;
@@ -137,111 +153,574 @@ struct PagedAttnParams {
   const int* ctx_lens;
   const long long* tree_mask;
   int* status;
+  float* ws;
   long long qs[3], os[3], kps[3], vps[3];
   long long table_stride, mask_stride;
   int B, Hq, Hkv, Sq;
-  int page_size, max_pages, n_pages;
+  int page_size, page_shift, max_pages, n_pages;  // page_shift: log2(page_size), or -1
   int slopes_dtype;
+  int row_blocks;  // blocks of RW * 16 rows per kv head
+  int n_ctas;      // of the attention kernel
   float sm_scale;
 };
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(128) coalibi_paged_attn_kernel(const PagedAttnParams p) {
-  __shared__ float s_q[D], s_p[128], s_red[8];
-  __shared__ long long s_v[128];
-  const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z, g = h / (p.Hq / p.Hkv);
+constexpr int kPagedStep = 32;  // keys per step of a warp
+
+template <int D, int RW>
+struct PagedLayout {
+  static constexpr int KG = 4 / RW;
+  static constexpr int UNIT = kPagedStep * KG;
+  static constexpr int ROWS = 16 * RW;
+  static constexpr int TILE = kPagedStep * D * 2;  // K or V of one step
+  static constexpr int NBUF = 3;                   // two steps in flight while one is computed
+  static constexpr int RING = NBUF * 2 * TILE;     // per key group
+  static constexpr int BYTES = KG * RING;
+  static constexpr int CTAS = D == 128 ? (RW == 1 ? 1 : 2) : 2;  // resident per SM
+  static constexpr int RECORD = ROWS * (4 + D);    // floats of one piece: stats, then O
+  // the joining of the key groups reuses the ring
+  static_assert(KG * 16 * RW * (D + 4) * 4 <= BYTES || KG == 1, "exchange fits the ring");
+};
+
+constexpr int kPagedMaxSms = 160;
+
+// Workspace: B + 2 ints (unit prefix of each request, units per run), then two records per CTA.
+template <int D, int RW>
+inline size_t paged_ws_bytes(int B) {
+  using L = PagedLayout<D, RW>;
+  const size_t head = ((size_t)(B + 2) * 4 + 255) / 256 * 256;
+  return head + (size_t)kPagedMaxSms * L::CTAS * 2 * L::RECORD * 4;
+}
+__host__ __device__ inline size_t paged_ws_head(int B) { return ((size_t)(B + 2) * 4 + 255) / 256 * 64; }  // in floats
+
+// Row warps for `rows` query rows per kv head.
+inline int paged_row_warps(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+__device__ __forceinline__ int paged_keys(const PagedAttnParams& p, int b) {
+  const int room = p.max_pages * p.page_size;  // at most 2^31 - 256
+  return min(min(max(p.ctx_lens[b], 0), room) + p.Sq, room);
+}
+
+// One thread per request range: exclusive prefix sums of the requests' units.  Returns
+// the total; s_pre[t] is the prefix at the first request of thread t's range.
+template <int UNIT>
+__device__ __forceinline__ int paged_prefix(const PagedAttnParams& p, int* s_pre, int* s_warp, int per, int* out) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint16_t* kp = static_cast<const uint16_t*>(p.k_pages) + g * p.kps[1];
-  const uint16_t* vp = static_cast<const uint16_t*>(p.v_pages) + g * p.vps[1];
-  if (tid < D / 2) {
-    const float2 f = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.q) + b * p.qs[0] +
-                                                                      h * p.qs[1] + i * p.qs[2] + 2 * tid));
-    s_q[2 * tid] = f.x;
-    s_q[2 * tid + 1] = f.y;
-  }
-  const unsigned long long bits = p.tree_mask != nullptr ? (unsigned long long)p.tree_mask[b * p.mask_stride + i]
-                                                         : (2ull << i) - 1;
-  const long long room = (long long)p.max_pages * p.page_size;
-  const int ctx = max(p.ctx_lens[b], 0);
-  const unsigned long long mine = p.Sq < 64 ? bits & ((1ull << p.Sq) - 1) : bits;
-  long long end = (long long)ctx + (64 - __clzll((long long)mine));
-  if (end > room) {
-    end = room;
-    if (tid == 0) report_page(p.status);
-  }
-  const float slope = load_slope(p.slopes, p.slopes_dtype, h);
-  float m = -INFINITY, l = 0.f, carry = 0.f, o = 0.f;
-  __syncthreads();
-  for (long long hi = end; hi > 0; hi -= 128) {
-    // thread tid takes key hi - 1 - tid: the block's prefix sums are sums over the keys to the right
-    const long long key = hi - 1 - tid;
-    bool seen = key >= 0 && (key < ctx || (mine >> (key - ctx) & 1));
-    long long ko = 0;
-    s_v[tid] = -1;
-    if (seen) {
-      const int at = (int)(key / p.page_size), slot = (int)(key - (long long)at * p.page_size);
-      const int page = p.page_table[(size_t)b * p.table_stride + at];
-      seen = page >= 0 && page < p.n_pages;
-      if (!seen) report_page(p.status);
-      if (seen) {
-        ko = page * p.kps[0] + slot * p.kps[2];
-        s_v[tid] = page * p.vps[0] + slot * p.vps[2];
-      }
-    }
-    float dot = 0.f;
-    if (seen) {
-      for (int c = 0; c < D; c += 8) {
-        const uint4 u = *reinterpret_cast<const uint4*>(kp + ko + c);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  int sum = 0;
+  for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) sum += (paged_keys(p, b) + UNIT - 1) / UNIT;
+  int inc = sum;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = unpack2<BF16>(w[j]);
-          dot = fmaf(f.x, s_q[c + 2 * j], dot);
-          dot = fmaf(f.y, s_q[c + 2 * j + 1], dot);
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += y;
+  }
+  if (lane == 31) s_warp[warp] = inc;
+  __syncthreads();
+  int left = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < warp) left += s_warp[w];
+    total += s_warp[w];
+  }
+  int at = left + inc - sum;
+  s_pre[tid] = at;
+  if (out != nullptr) {
+    for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) {
+      out[b] = at;
+      at += (paged_keys(p, b) + UNIT - 1) / UNIT;
+    }
+    if (tid == 0) out[p.B] = total;
+  }
+  __syncthreads();
+  return total;
+}
+
+// smem row of a step's key: a warp's score fragment then has keys 8 t .. 8 t + 7 of the
+// step in the lanes t of a quad, so the suffix sum over a row is 8 additions in a lane and
+// one scan over the quad.  Row r of the tile holds key:
+__device__ __forceinline__ int paged_row_key(int r) { return 8 * ((r & 7) >> 1) + 2 * (r >> 3) + (r & 1); }
+
+template <int D, bool BF16, int RW, int XR>
+__global__ void __launch_bounds__(128) coalibi_paged_attn_kernel(const PagedAttnParams p) {
+  using L = PagedLayout<D, RW>;
+  constexpr int KG = L::KG, KK = D / 16, CH = D / 8;
+  constexpr int THREADS = 32 * RW;  // per key group
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int s_pre[128], s_warp[4], s_find;
+  __shared__ float4 s_stat[KG > 1 ? KG * L::ROWS : 1];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int gq = lane >> 2, tig = lane & 3;
+  const int rwarp = warp % RW, kg = warp / RW, gtid = tid % THREADS;
+  const int G = p.Hq / p.Hkv, rows = G * p.Sq;
+  const int heads = p.Hkv * p.row_blocks;  // items per request
+  uint8_t* ring = smem + kg * L::RING;
+  grid_dep_wait();
+
+  // ---- this CTA's run of units
+  int* head = reinterpret_cast<int*>(p.ws);
+  const int per = (p.B + 127) / 128;
+  const long long total = (long long)paged_prefix<L::UNIT>(p, s_pre, s_warp, per, blockIdx.x == 0 ? head : nullptr) * heads;
+  const long long quota = (total + p.n_ctas - 1) / p.n_ctas;
+  if (blockIdx.x == 0 && tid == 0) head[p.B + 1] = (int)quota;
+  long long at = quota * blockIdx.x;
+  const long long stop = min(total, at + quota);
+  if (at >= stop) return;
+  // the request that holds unit `at`
+  if ((long long)s_pre[tid] * heads <= at && (tid == 127 || (long long)s_pre[tid + 1] * heads > at)) s_find = tid;
+  __syncthreads();
+  int b = s_find * per, pre = s_pre[s_find];
+  int units = (paged_keys(p, b) + L::UNIT - 1) / L::UNIT;
+  while ((long long)(pre + units) * heads <= at) {
+    pre += units;
+    ++b;
+    units = (paged_keys(p, b) + L::UNIT - 1) / L::UNIT;
+  }
+  int item = (int)((at - (long long)pre * heads) / units);
+  int u0 = (int)((at - (long long)pre * heads) - (long long)item * units);
+
+  for (bool first = true; at < stop; first = false) {
+    const int u1 = (int)min((long long)units, u0 + (stop - at));
+    const int g = item / p.row_blocks, r0 = (item - g * p.row_blocks) * L::ROWS + rwarp * 16;
+    const int len = p.ctx_lens[b], room = p.max_pages * p.page_size, ctx = min(max(len, 0), room);
+
+    // ---- the rows: visibility words, slopes, queries as A fragments
+    unsigned long long word[XR];
+    unsigned long long seen_by_any = 0;  // over all rows of the request
+    float slope2[XR];
+    const uint16_t* qrow[XR];
+    bool rok[XR];
+#pragma unroll
+    for (int x = 0; x < XR; ++x) {
+      const int r = r0 + gq + 8 * x;
+      rok[x] = r < rows;
+      const int rr = rok[x] ? r : 0;
+      const int h = g * G + rr / p.Sq, i = rr % p.Sq;
+      word[x] = p.tree_mask != nullptr ? (unsigned long long)p.tree_mask[b * p.mask_stride + i] : (2ull << i) - 1;
+      slope2[x] = load_slope(p.slopes, p.slopes_dtype, h) * kLog2e;
+      qrow[x] = static_cast<const uint16_t*>(p.q) + b * p.qs[0] + h * p.qs[1] + i * p.qs[2];
+    }
+    if (p.tree_mask == nullptr) {
+      seen_by_any = (2ull << (p.Sq - 1)) - 1;
+    } else {
+      for (int i = lane; i < p.Sq; i += 32) seen_by_any |= (unsigned long long)p.tree_mask[b * p.mask_stride + i];
+#pragma unroll
+      for (int d = 16; d; d >>= 1) seen_by_any |= __shfl_xor_sync(0xffffffffu, seen_by_any, d);
+      if (p.Sq < 64) seen_by_any &= (1ull << p.Sq) - 1;
+    }
+    const int drafts = 64 - __clzll((long long)seen_by_any);
+    if ((len > room || ctx + drafts > room) && tid == 0) report_page(p.status);
+    uint32_t qa[KK][4];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          qa[kk][2 * hf + x] = x < XR && rok[x % XR]
+                                   ? *reinterpret_cast<const uint32_t*>(qrow[x % XR] + 16 * kk + 8 * hf + 2 * tig)
+                                   : 0u;
+
+    // ---- this key group's keys: [lo, hi), lo a multiple of 16 (so a half step lies in one page)
+    const int s_lo = u0 * L::UNIT, s_hi = min(min(u1 * L::UNIT, room), ctx + drafts);
+    const int sub = ((s_hi - s_lo + KG - 1) / KG + 15) & ~15;
+    const int lo = s_lo + kg * sub, hi = min(s_hi, lo + sub);
+    const int nsteps = hi > lo ? (hi - lo + kPagedStep - 1) / kPagedStep : 0;
+
+    float o[2 * KK][4];
+#pragma unroll
+    for (int dn = 0; dn < 2 * KK; ++dn) o[dn][0] = o[dn][1] = o[dn][2] = o[dn][3] = 0.f;
+    float m_run[XR], l_part[XR], carry[XR];
+#pragma unroll
+    for (int x = 0; x < XR; ++x) m_run[x] = -INFINITY, l_part[x] = 0.f, carry[x] = 0.f;
+
+    const int* table = p.page_table + (size_t)b * p.table_stride;
+    const uint16_t* kbase = static_cast<const uint16_t*>(p.k_pages) + g * p.kps[1];
+    const uint16_t* vbase = static_cast<const uint16_t*>(p.v_pages) + g * p.vps[1];
+    int page_id[2];    // of the next step to be staged, per half
+    uint32_t lost = 0;  // two bits per ring slot: halves whose page is outside the pool
+    auto lookup = [&](int st) {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int key = lo + st * kPagedStep + 16 * hf;
+        page_id[hf] = 0;
+        if (st >= 0 && key < hi) page_id[hf] = table[p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size];
+      }
+    };
+    auto stage = [&](int st) {
+      const int kb = lo + st * kPagedStep, slot = st % L::NBUF;
+      uint8_t* kt = ring + slot * 2 * L::TILE;
+      uint8_t* vt = kt + L::TILE;
+      const uint16_t* kr[2];
+      const uint16_t* vr[2];
+      bool in[2];
+      lost &= ~(3u << (2 * slot));
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int key = kb + 16 * hf;
+        const int first_slot = p.page_shift >= 0 ? key & (p.page_size - 1) : key % p.page_size;
+        in[hf] = (unsigned)page_id[hf] < (unsigned)p.n_pages;
+        if (!in[hf]) {
+          lost |= 1u << (2 * slot + hf);
+          report_page(p.status);
+        }
+        const long long pg = in[hf] ? page_id[hf] : 0;
+        kr[hf] = kbase + pg * p.kps[0] + first_slot * p.kps[2];
+        vr[hf] = vbase + pg * p.vps[0] + first_slot * p.vps[2];
+      }
+#pragma unroll
+      for (int it = 0; it < kPagedStep * CH / THREADS; ++it) {
+        const int idx = it * THREADS + gtid;
+        const int row = idx / CH, c = idx % CH;
+        const int off = paged_row_key(row), hf = off >> 4, key = kb + off;
+        const bool ok = key < hi && in[hf] && (key < ctx || (seen_by_any >> (key - ctx) & 1));
+        const int dst = row * (D * 2) + ((c ^ (row & 7)) << 4);
+        cp_async16(kt + dst, kr[hf] + (ok ? (off & 15) * p.kps[2] + c * 8 : 0), ok);
+        cp_async16(vt + dst, vr[hf] + (ok ? (off & 15) * p.vps[2] + c * 8 : 0), ok);
+      }
+    };
+    auto group_sync = [&]() {
+      if (RW == 1)
+        __syncwarp();
+      else
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + kg), "n"(THREADS) : "memory");
+    };
+
+    lookup(nsteps - 1);
+#pragma unroll
+    for (int a = 1; a < L::NBUF; ++a) {
+      if (nsteps - a >= 0) stage(nsteps - a);
+      cp_async_commit();
+      lookup(nsteps - a - 1);
+    }
+    const float c_a = p.sm_scale * kLog2e;
+    const int mat = lane >> 3, row8 = lane & 7;
+    for (int st = nsteps - 1; st >= 0; --st) {
+      cp_async_wait_pending<L::NBUF - 2>();  // this thread's part of step st has landed
+      group_sync();                          // the others' too, and all are done with step st + 1
+      if (st - (L::NBUF - 1) >= 0) stage(st - (L::NBUF - 1));
+      cp_async_commit();
+      lookup(st - L::NBUF);
+      const int slot = st % L::NBUF, kb = lo + st * kPagedStep;
+      const uint32_t kt = smem_u32(ring + slot * 2 * L::TILE), vt = kt + L::TILE;
+      // ---- S = Q K^T
+      float sc[4][4];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+        for (int np = 0; np < 2; ++np) {
+          uint32_t b0, b1, b2, b3;
+          const int row = 16 * np + (mat >> 1) * 8 + row8, c = 2 * kk + (mat & 1);
+          ldsm_x4(kt + row * (D * 2) + ((c ^ row8) << 4), b0, b1, b2, b3);
+          mma16816<BF16>(sc[2 * np], qa[kk], b0, b1);
+          mma16816<BF16>(sc[2 * np + 1], qa[kk], b2, b3);
+        }
+      }
+      // ---- which of this lane's 8 keys (kb + 8 tig + j) each row sees
+      const bool all = kb + kPagedStep <= min(hi, ctx) && (lost >> (2 * slot) & 3) == 0;
+      uint32_t vis[XR];
+#pragma unroll
+      for (int x = 0; x < XR; ++x) vis[x] = 0xffu;
+      if (!all) {
+        const int k0 = kb + 8 * tig;
+        const bool gone = lost >> (2 * slot + (tig >> 1)) & 1;
+#pragma unroll
+        for (int x = 0; x < XR; ++x) {
+          uint32_t v = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int key = k0 + j;
+            if (!gone && key < hi && (key < ctx || (word[x] >> (key - ctx) & 1))) v |= 1u << j;
+          }
+          vis[x] = v;
+        }
+      }
+      // ---- sigmoids, suffix sums, logits (in log2 units), online softmax
+#pragma unroll
+      for (int x = 0; x < XR; ++x) {
+        float suf[8];
+        float run = 0.f;
+#pragma unroll
+        for (int j = 7; j >= 0; --j) {
+          float& v = sc[j >> 1][2 * x + (j & 1)];
+          v *= c_a;
+          float sg = rcp_approx(1.f + ex2_approx(-v));
+          if (!all) sg = vis[x] >> j & 1 ? sg : 0.f;
+          run += sg;
+          suf[j] = run;
+        }
+        float inc = run;
+        float y = __shfl_down_sync(0xffffffffu, inc, 1);
+        if (tig < 3) inc += y;
+        y = __shfl_down_sync(0xffffffffu, inc, 2);
+        if (tig < 2) inc += y;
+        const float base = carry[x] + (inc - run);
+        carry[x] += __shfl_sync(0xffffffffu, inc, lane & ~3);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float& v = sc[j >> 1][2 * x + (j & 1)];
+          v = fmaf(-slope2[x], suf[j] + base, v);
+          if (!all) v = vis[x] >> j & 1 ? v : -INFINITY;
+          mx = fmaxf(mx, v);
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // the newest keys weigh most, so the maximum seldom moves after the first steps
+        if (__any_sync(0xffffffffu, mx > m_run[x])) {
+          const float m_new = fmaxf(m_run[x], mx);
+          const float fac = m_run[x] == -INFINITY ? 0.f : ex2_approx(m_run[x] - m_new);
+          m_run[x] = m_new;
+          l_part[x] *= fac;
+#pragma unroll
+          for (int dn = 0; dn < 2 * KK; ++dn) {
+            o[dn][2 * x] *= fac;
+            o[dn][2 * x + 1] *= fac;
+          }
+        }
+        const float m_use = m_run[x] == -INFINITY ? 0.f : m_run[x];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float& v = sc[j >> 1][2 * x + (j & 1)];
+          v = ex2_approx(v - m_use);
+          l_part[x] += v;
+        }
+      }
+      // ---- a drafted token's V that is not finite must not reach the rows that do not see
+      // it through 0 * V: such rows of the tile are added by hand and then zeroed
+      if (!all && p.Sq > 1 && kb + kPagedStep > ctx) {
+        uint8_t* vrow = ring + slot * 2 * L::TILE + L::TILE + lane * (D * 2);
+        bool bad = false;
+        if (kb + paged_row_key(lane) >= ctx) {
+#pragma unroll 4
+          for (int c = 0; c < CH; ++c) {
+            const uint4 u = *reinterpret_cast<const uint4*>(vrow + (c << 4));
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = unpack2<BF16>(w[j]);
+              bad |= !(fabsf(f.x) <= 3.4e38f) || !(fabsf(f.y) <= 3.4e38f);
+            }
+          }
+        }
+        uint32_t bads = __ballot_sync(0xffffffffu, bad);
+        if (bads != 0) {
+          for (uint32_t left = bads; left != 0; left &= left - 1) {
+            const int row = __ffs(left) - 1, off = paged_row_key(row);
+            const uint8_t* vb = ring + slot * 2 * L::TILE + L::TILE + row * (D * 2);
+#pragma unroll
+            for (int x = 0; x < XR; ++x) {
+              float w = 0.f;
+              uint32_t see = 0;
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if ((off & 7) == j) w = sc[j >> 1][2 * x + (j & 1)];
+              see = vis[x] >> (off & 7) & 1;
+              w = __shfl_sync(0xffffffffu, w, (lane & ~3) | (off >> 3));
+              see = __shfl_sync(0xffffffffu, see, (lane & ~3) | (off >> 3));
+              if (see) {
+#pragma unroll
+                for (int dn = 0; dn < 2 * KK; ++dn) {
+                  const float2 f =
+                      unpack2<BF16>(*reinterpret_cast<const uint32_t*>(vb + ((dn ^ (row & 7)) << 4) + 4 * tig));
+                  o[dn][2 * x] = fmaf(w, f.x, o[dn][2 * x]);
+                  o[dn][2 * x + 1] = fmaf(w, f.y, o[dn][2 * x + 1]);
+                }
+              }
+            }
+          }
+          group_sync();
+          if (rwarp == 0 && bad)
+            for (int c = 0; c < CH; ++c) *reinterpret_cast<uint4*>(vrow + (c << 4)) = make_uint4(0u, 0u, 0u, 0u);
+          group_sync();
+        }
+      }
+      // ---- O += P V: the C fragments of two key tiles are the A fragment of one k-step.
+      // P is rounded to the inputs' type for the product; l sums it unrounded.
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
+        uint32_t pa[4];
+        pa[0] = pack2<BF16>(sc[2 * k2][0], sc[2 * k2][1]);
+        pa[1] = XR > 1 ? pack2<BF16>(sc[2 * k2][2], sc[2 * k2][3]) : 0u;
+        pa[2] = pack2<BF16>(sc[2 * k2 + 1][0], sc[2 * k2 + 1][1]);
+        pa[3] = XR > 1 ? pack2<BF16>(sc[2 * k2 + 1][2], sc[2 * k2 + 1][3]) : 0u;
+#pragma unroll
+        for (int dp = 0; dp < KK; ++dp) {
+          uint32_t b0, b1, b2, b3;
+          const int row = 16 * k2 + (mat & 1) * 8 + row8, c = 2 * dp + (mat >> 1);
+          ldsm_x4_t(vt + row * (D * 2) + ((c ^ row8) << 4), b0, b1, b2, b3);
+          mma16816<BF16>(o[2 * dp], pa, b0, b1);
+          mma16816<BF16>(o[2 * dp + 1], pa, b2, b3);
         }
       }
     }
-    const float x = dot * p.sm_scale;
-    const float sg = seen ? 1.f / (1.f + expf(-x)) : 0.f;
-    float inc = sg;
+    cp_async_wait_all();
+#pragma unroll
+    for (int x = 0; x < XR; ++x) {
+      l_part[x] += __shfl_xor_sync(0xffffffffu, l_part[x], 1);
+      l_part[x] += __shfl_xor_sync(0xffffffffu, l_part[x], 2);
+    }
+
+    // ---- the piece's result: the output if the item is whole, else a record
+    const bool whole = u0 == 0 && u1 == units;
+    float* rec = p.ws + paged_ws_head(p.B) + ((size_t)blockIdx.x * 2 + (first && u0 > 0 ? 0 : 1)) * L::RECORD;
+    float4* stats = reinterpret_cast<float4*>(rec);
+    float* orec = rec + 4 * L::ROWS;
+    if (KG == 1) {
+#pragma unroll
+      for (int x = 0; x < XR; ++x) {
+        const int r = rwarp * 16 + gq + 8 * x;
+        if (!rok[x]) continue;
+        if (whole) {
+          const int rr = r0 + gq + 8 * x;
+          uint16_t* y = static_cast<uint16_t*>(p.o) + b * p.os[0] + (g * G + rr / p.Sq) * p.os[1] + (rr % p.Sq) * p.os[2];
+          const float inv = l_part[x] > 0.f ? 1.f / l_part[x] : (l_part[x] == 0.f ? 0.f : l_part[x]);
+#pragma unroll
+          for (int dn = 0; dn < 2 * KK; ++dn)
+            *reinterpret_cast<uint32_t*>(y + 8 * dn + 2 * tig) = pack2<BF16>(o[dn][2 * x] * inv, o[dn][2 * x + 1] * inv);
+        } else {
+          if (tig == 0) stats[r] = make_float4(carry[x], m_run[x], l_part[x], 0.f);
+#pragma unroll
+          for (int dn = 0; dn < 2 * KK; ++dn)
+            *reinterpret_cast<float2*>(orec + r * D + 8 * dn + 2 * tig) = make_float2(o[dn][2 * x], o[dn][2 * x + 1]);
+        }
+      }
+    } else {
+      // key groups join through shared memory (the rings are idle now)
+      float* xo = reinterpret_cast<float*>(smem);  // [KG][ROWS][D]
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < XR; ++x) {
+        const int r = rwarp * 16 + gq + 8 * x;
+        if (tig == 0) s_stat[kg * L::ROWS + r] = make_float4(carry[x], m_run[x], l_part[x], slope2[x]);
+#pragma unroll
+        for (int dn = 0; dn < 2 * KK; ++dn)
+          *reinterpret_cast<float2*>(xo + ((size_t)kg * L::ROWS + r) * D + 8 * dn + 2 * tig) =
+              make_float2(o[dn][2 * x], o[dn][2 * x + 1]);
+      }
+      __syncthreads();
+      const int rb = (item - g * p.row_blocks) * L::ROWS;
+      const int n = min(XR == 1 ? 8 : L::ROWS, rows - rb);
+      for (int e = tid; e < n * (D / 4); e += 128) {
+        const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+        float right = 0.f, M = -INFINITY, w[KG];
+#pragma unroll
+        for (int c = KG - 1; c >= 0; --c) {
+          const float4 s = s_stat[c * L::ROWS + r];
+          w[c] = s.y == -INFINITY ? -INFINITY : s.y - s.w * right;
+          M = fmaxf(M, w[c]);
+          right += s.x;
+        }
+        const float m_use = M == -INFINITY ? 0.f : M;
+        float l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int c = KG - 1; c >= 0; --c) {
+          const float f = ex2_approx(w[c] - m_use);
+          l = fmaf(s_stat[c * L::ROWS + r].z, f, l);
+          const float4 v = *reinterpret_cast<const float4*>(xo + ((size_t)c * L::ROWS + r) * D + d);
+          acc.x = fmaf(v.x, f, acc.x);
+          acc.y = fmaf(v.y, f, acc.y);
+          acc.z = fmaf(v.z, f, acc.z);
+          acc.w = fmaf(v.w, f, acc.w);
+        }
+        if (whole) {
+          const int rr = rb + r;
+          uint16_t* y = static_cast<uint16_t*>(p.o) + b * p.os[0] + (g * G + rr / p.Sq) * p.os[1] + (rr % p.Sq) * p.os[2];
+          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+          *reinterpret_cast<uint2*>(y + d) =
+              make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+        } else {
+          if (d == 0) stats[r] = make_float4(right, M, l, 0.f);
+          *reinterpret_cast<float4*>(orec + r * D + d) = acc;
+        }
+      }
+    }
+    __syncthreads();  // the rings are free for the next item
+
+    // ---- next item of the run
+    at += u1 - u0;
+    u0 = 0;
+    if (++item == heads) {
+      item = 0;
+      pre += units;
+      if (++b < p.B) units = (paged_keys(p, b) + L::UNIT - 1) / L::UNIT;
+    }
+  }
+}
+
+// Joins the pieces of the items that span runs.  One warp per query row; lanes hold the
+// statistics of up to 32 pieces at a time, rightmost first.
+template <int D, bool BF16, int RW>
+__global__ void __launch_bounds__(128) coalibi_paged_join_kernel(const PagedAttnParams p) {
+  using L = PagedLayout<D, RW>;
+  constexpr int V = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int G = p.Hq / p.Hkv, rows = G * p.Sq;
+  const int r = blockIdx.y * 4 + (threadIdx.x >> 5);
+  const int b = blockIdx.x / p.Hkv, g = blockIdx.x - b * p.Hkv;
+  grid_dep_wait();
+  if (r >= rows) return;
+  const int* head = reinterpret_cast<const int*>(p.ws);
+  const int heads = p.Hkv * p.row_blocks, item = g * p.row_blocks + r / L::ROWS, rr = r % L::ROWS;
+  const int units = head[b + 1] - head[b];
+  const long long quota = head[p.B + 1];
+  const long long t0 = (long long)head[b] * heads + (long long)item * units, t1 = t0 + units;
+  const int c0 = (int)(t0 / quota), c1 = (int)((t1 - 1) / quota);
+  if (c0 == c1) return;  // finished by the attention kernel
+  const int h = g * G + r / p.Sq, i = r % p.Sq;
+  const float slope2 = load_slope(p.slopes, p.slopes_dtype, h) * kLog2e;
+  const float* recs = p.ws + paged_ws_head(p.B);
+  auto record = [&](int c) { return recs + ((size_t)c * 2 + (t0 < c * quota ? 0 : 1)) * L::RECORD; };
+  float M = -INFINITY, l = 0.f, right = 0.f, acc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = 0.f;
+  for (int top = c1; top >= c0; top -= 32) {
+    const int n = min(32, top - c0 + 1);
+    float4 s = make_float4(0.f, -INFINITY, 0.f, 0.f);
+    if (lane < n) s = reinterpret_cast<const float4*>(record(top - lane))[rr];
+    float inc = s.x;
+#pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const float y = __shfl_up_sync(0xffffffffu, inc, d);
       if (lane >= d) inc += y;
     }
-    if (lane == 31) s_red[warp] = inc;
-    __syncthreads();
-    float left = carry;
-    for (int w = 0; w < 4; ++w) {
-      if (w < warp) left += s_red[w];
-      carry += s_red[w];
-    }
-    const float a = seen ? x - slope * (inc + left) : -INFINITY;
-    float mx = a;
+    float m = s.y == -INFINITY ? -INFINITY : s.y - slope2 * (right + (inc - s.x));
+    right += __shfl_sync(0xffffffffu, inc, 31);
+    float mx = m;
+#pragma unroll
     for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    if (lane == 0) s_red[4 + warp] = mx;
-    __syncthreads();
-    const float m_new = fmaxf(fmaxf(fmaxf(s_red[4], s_red[5]), fmaxf(s_red[6], s_red[7])), m);
-    const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float fac = m == -INFINITY ? 0.f : expf(m - m_use);
-    s_p[tid] = a == -INFINITY ? 0.f : expf(a - m_use);
-    m = m_new;
-    l *= fac;
-    o *= fac;
-    __syncthreads();
-    for (int j = 0; j < 128; ++j) {
-      const float w = s_p[j];
-      l += w;
-      if (s_v[j] < 0 || tid >= D) continue;
-      const uint16_t e = vp[s_v[j] + tid];
-      o = fmaf(w, BF16 ? __bfloat162float(__ushort_as_bfloat16(e)) : __half2float(__ushort_as_half(e)), o);
+    const float m_new = fmaxf(M, mx), m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float fac = M == -INFINITY ? 0.f : ex2_approx(M - m_use);
+    M = m_new;
+    const float f = ex2_approx(m - m_use);
+    float lw = f * s.z;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, d);
+    l = l * fac + lw;
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] *= fac;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const float w = __shfl_sync(0xffffffffu, f, j);
+      const float* y = record(top - j) + 4 * L::ROWS + rr * D + lane * V;
+      if (V == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(y);
+        acc[0] = fmaf(w, u.x, acc[0]);
+        acc[1] = fmaf(w, u.y, acc[1]);
+        acc[V - 2] = fmaf(w, u.z, acc[V - 2]);
+        acc[V - 1] = fmaf(w, u.w, acc[V - 1]);
+      } else {
+        const float2 u = *reinterpret_cast<const float2*>(y);
+        acc[0] = fmaf(w, u.x, acc[0]);
+        acc[1] = fmaf(w, u.y, acc[1]);
+      }
     }
-    __syncthreads();
   }
-  if (tid < D) {
-    const float r = l > 0.f ? o / l : 0.f;
-    uint16_t* y = static_cast<uint16_t*>(p.o) + b * p.os[0] + h * p.os[1] + i * p.os[2];
-    y[tid] = BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(r)) : __half_as_ushort(__float2half_rn(r));
-  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  uint16_t* y = static_cast<uint16_t*>(p.o) + b * p.os[0] + h * p.os[1] + i * p.os[2] + lane * V;
+#pragma unroll
+  for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t*>(y + v) = pack2<BF16>(acc[v] * inv, acc[v + 1] * inv);
 }
 
 }  // namespace coalibi

@@ -115,9 +115,56 @@ extern "C" int coalibi_paged_append(const CoalibiPagedAppendArgs* a, void* strea
   return launched("paged append launch");
 }
 
+namespace coalibi {
+namespace {
+
+template <int D, bool BF16, int RW, int XR>
+int launch_paged(PagedAttnParams& p, int sms, cudaStream_t s) {
+  using L = PagedLayout<D, RW>;
+  // once per device would do; the call is a few hundred nanoseconds and needs no state
+  cudaError_t e = cudaFuncSetAttribute(coalibi_paged_attn_kernel<D, BF16, RW, XR>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
+  const int rows = p.Hq / p.Hkv * p.Sq;
+  p.row_blocks = (rows + L::ROWS - 1) / L::ROWS;
+  p.n_ctas = (sms < kPagedMaxSms ? sms : kPagedMaxSms) * L::CTAS;
+  const long long most = ((long long)p.max_pages * p.page_size + L::UNIT - 1) / L::UNIT;
+  const long long bound = most * p.B * p.Hkv * p.row_blocks;  // units, if every table row were full
+  if (bound > 0x7fffffffLL) return COALIBI_ERR_SHAPE;
+  if (bound < p.n_ctas) p.n_ctas = (int)bound;
+  if (e == cudaSuccess)
+    e = launch_pdl(coalibi_paged_attn_kernel<D, BF16, RW, XR>, dim3(p.n_ctas), dim3(128), L::BYTES, s, p);
+  // an item of one unit is never split
+  if (e == cudaSuccess && most > 1)
+    e = launch_pdl(coalibi_paged_join_kernel<D, BF16, RW>, dim3(p.B * p.Hkv, (rows + 3) / 4), dim3(128), 0, s, p);
+  if (e != cudaSuccess) set_last_error_detail(cudaGetErrorString(e));
+  return e == cudaSuccess ? launched("paged attention launch") : COALIBI_ERR_LAUNCH;
+}
+
+template <int D, bool BF16>
+int launch_paged_rows(PagedAttnParams& p, int sms, cudaStream_t s) {
+  const int rows = p.Hq / p.Hkv * p.Sq;
+  switch (paged_row_warps(rows)) {
+    case 1: return rows <= 8 ? launch_paged<D, BF16, 1, 1>(p, sms, s) : launch_paged<D, BF16, 1, 2>(p, sms, s);
+    case 2: return launch_paged<D, BF16, 2, 2>(p, sms, s);
+    default: return launch_paged<D, BF16, 4, 2>(p, sms, s);
+  }
+}
+
+template <int D>
+size_t paged_ws_rows(int B, int rows) {
+  switch (paged_row_warps(rows)) {
+    case 1: return paged_ws_bytes<D, 1>(B);
+    case 2: return paged_ws_bytes<D, 2>(B);
+    default: return paged_ws_bytes<D, 4>(B);
+  }
+}
+
+}  // namespace
+}  // namespace coalibi
+
 extern "C" size_t coalibi_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int Sq, int D) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Sq > kTreeMaxSq || Hq % Hkv != 0 || (D != 64 && D != 128)) return 0;
-  return 16;
+  return D == 128 ? paged_ws_rows<128>(B, Hq / Hkv * Sq) : paged_ws_rows<64>(B, Hq / Hkv * Sq);
 }
 
 extern "C" int coalibi_paged_attention(const CoalibiPagedAttentionArgs* a, void* workspace, size_t workspace_bytes,
@@ -166,20 +213,14 @@ extern "C" int coalibi_paged_attention(const CoalibiPagedAttentionArgs* a, void*
   p.slopes_dtype = a->slopes_dtype;
   p.sm_scale = a->sm_scale;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(a->Sq, a->Hq, a->B);
+  p.ws = static_cast<float*>(workspace);
+  p.page_shift = -1;
+  for (int k = 4; k < 31; ++k)
+    if (a->page_size == 1 << k) p.page_shift = k;
   const bool bf16 = a->dtype == COALIBI_BF16;
-  if (a->D == 128) {
-    if (bf16)
-      coalibi_paged_attn_kernel<128, true><<<grid, 128, 0, s>>>(p);
-    else
-      coalibi_paged_attn_kernel<128, false><<<grid, 128, 0, s>>>(p);
-  } else {
-    if (bf16)
-      coalibi_paged_attn_kernel<64, true><<<grid, 128, 0, s>>>(p);
-    else
-      coalibi_paged_attn_kernel<64, false><<<grid, 128, 0, s>>>(p);
-  }
-  return launched("paged attention launch");
+  const int sms = device_sm_count();
+  if (a->D == 128) return bf16 ? launch_paged_rows<128, true>(p, sms, s) : launch_paged_rows<128, false>(p, sms, s);
+  return bf16 ? launch_paged_rows<64, true>(p, sms, s) : launch_paged_rows<64, false>(p, sms, s);
 }
 
 extern "C" int coalibi_sample(const CoalibiSampleArgs* a, void* stream) {
