@@ -50,6 +50,8 @@ def _check_cache(what, k_pages, v_pages, page_table, B, D, dtype, device):
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
         if not _rows16(t):
             raise ValueError(f"co_alibi_attn: {what}: {name} must have contiguous, 16-byte aligned rows")
+        if 0 in (s for s, n in zip(t.stride(), t.shape) if n > 1):
+            raise ValueError(f"co_alibi_attn: {what}: {name} must not be an expanded tensor")
     if page_table.dtype != torch.int32:
         raise TypeError(f"co_alibi_attn: {what}: page_table must be int32, got {page_table.dtype}")
     if page_table.dim() != 2 or page_table.shape[0] != B or page_table.shape[1] == 0 or page_table.stride(1) != 1:
@@ -68,8 +70,14 @@ def _on(what, device, *tensors):
 
 def _rows16(t):
     """Whether every row of t [., ., ., D] is contiguous and 16-byte aligned."""
-    s = t.stride()
-    return s[3] == 1 and not (s[0] | s[1] | s[2]) & 7 and t.data_ptr() % 16 == 0
+    s = _strides(t)
+    return t.stride(3) == 1 and not (s[0] | s[1] | s[2]) & 7 and t.data_ptr() % 16 == 0
+
+
+def _strides(t):
+    """The first three strides of t, 0 for a dimension of one entry (PyTorch may report any there)."""
+    n, s = t.shape, t.stride()
+    return s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0
 
 
 def _aligned_rows(t):
@@ -148,7 +156,7 @@ def append_paged_kv(k, v, k_pages, v_pages, page_table, start, count=None, q=Non
         _on(what, device, q)
         q = _aligned_rows(q)
         Hq, q_out = q.shape[1], torch.empty_like(q)
-        qs, qos = q.stride()[:3], q_out.stride()[:3]
+        qs, qos = _strides(q), _strides(q_out)
     cos = sin = None
     rot = n_pos = 0
     if rotary is not None:
@@ -168,7 +176,7 @@ def append_paged_kv(k, v, k_pages, v_pages, page_table, start, count=None, q=Non
         k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), start.data_ptr(),
         count.data_ptr() if count is not None else 0, positions.data_ptr() if positions is not None else 0,
         cos.data_ptr() if rot else 0, sin.data_ptr() if rot else 0, _status_word(device).data_ptr(),
-        *k.stride()[:3], *v.stride()[:3], *qs, *qos, *k_pages.stride()[:3], *v_pages.stride()[:3],
+        *_strides(k), *_strides(v), *qs, *qos, *_strides(k_pages), *_strides(v_pages),
         page_table.stride(0), B, Hq, Hkv, S, D, k_pages.shape[2], page_table.shape[1], k_pages.shape[0],
         rot, n_pos, 1 if interleaved else 0, _DTYPES[dtype])
     _call(device, _lib.load().coalibi_paged_append, "coalibi_paged_append", args)
@@ -232,7 +240,7 @@ def paged_tree_attention(q, k_pages, v_pages, page_table, ctx_lens, tree_mask=No
     args = _ATTN.pack(
         q.data_ptr(), o.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), slopes.data_ptr(), page_table.data_ptr(),
         ctx_lens.data_ptr(), tree_mask.data_ptr() if tree_mask is not None else 0, _status_word(device).data_ptr(),
-        *q.stride()[:3], *o.stride()[:3], *k_pages.stride()[:3], *v_pages.stride()[:3], page_table.stride(0),
+        *_strides(q), *_strides(o), *_strides(k_pages), *_strides(v_pages), page_table.stride(0),
         mask_stride, B, Hq, Hkv, Sq, D, k_pages.shape[2], page_table.shape[1], k_pages.shape[0], _DTYPES[dtype],
         _SLOPE_DTYPES[slopes.dtype], sm_scale if sm_scale is not None else D ** -0.5)
     _call(device, lib.coalibi_paged_attention, "coalibi_paged_attention", args, ws.data_ptr(), nbytes)

@@ -62,6 +62,34 @@ int make_tmap(CUtensorMap* map, const void* base, int D, int rows, int heads, in
   return COALIBI_OK;
 }
 
+// 4-D view (D, slot, head, page) of a page pool of any strides (in elements; that of a
+// dimension of one entry is never used), loaded as boxes of 64 columns x 16 slots with the
+// 128-byte swizzle.
+int make_page_tmap(CUtensorMap* map, const void* base, int D, int page_size, int heads, int pages,
+                   const long long* stride, bool bf16) {
+  auto fn = encode_fn();
+  if (fn == nullptr) {
+    snprintf(g_last_error, sizeof(g_last_error), "cuTensorMapEncodeTiled unavailable from the driver");
+    return COALIBI_ERR_TENSOR_MAP;
+  }
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)page_size, (cuuint64_t)heads, (cuuint64_t)pages};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] > 1 ? (cuuint64_t)stride[2 - i] * 2 : (cuuint64_t)D * 2;
+  cuuint32_t box[4] = {64, 16, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    snprintf(g_last_error, sizeof(g_last_error),
+             "cuTensorMapEncodeTiled -> %d (base=%p D=%d page_size=%d heads=%d pages=%d)", (int)r, base, D, page_size,
+             heads, pages);
+    return COALIBI_ERR_TENSOR_MAP;
+  }
+  return COALIBI_OK;
+}
+
 // Driver entry points used to bind and restore contexts.  Binding goes through
 // the driver API so that the runtime's per-thread device selection (what
 // cudaSetDevice changes) is never touched: a thread that had no context current

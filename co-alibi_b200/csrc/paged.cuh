@@ -171,17 +171,18 @@ struct PagedLayout {
   static constexpr int KG = 4 / RW;
   static constexpr int UNIT = kPagedStep * KG;
   static constexpr int ROWS = 16 * RW;
-  static constexpr int TILE = kPagedStep * D * 2;  // K or V of one step
-  static constexpr int NBUF = 3;                   // two steps in flight while one is computed
+  static constexpr int TILE = kPagedStep * D * 2;  // K or V of one step: [D / 64][32 keys][128 bytes], swizzled
+  static constexpr int NBUF = RW == 4 ? 4 : 3;     // all but one of the steps in flight
   static constexpr int RING = NBUF * 2 * TILE;     // per key group
-  static constexpr int BYTES = KG * RING;
-  static constexpr int CTAS = D == 128 ? (RW == 1 ? 1 : 2) : 2;  // resident per SM
+  static constexpr int BYTES = KG * RING + 1024;   // (the ring starts at a multiple of 1024)
+  static constexpr int CTAS = D == 128 ? (RW == 1 ? 1 : 2) : RW == 1 ? 2 : RW == 2 ? 3 : 4;  // resident per SM
   static constexpr int RECORD = ROWS * (4 + D);    // floats of one piece: stats, then O
   // the joining of the key groups reuses the ring
-  static_assert(KG * 16 * RW * (D + 4) * 4 <= BYTES || KG == 1, "exchange fits the ring");
+  static_assert(KG * 16 * RW * D * 4 <= KG * RING || KG == 1, "exchange fits the ring");
 };
 
 constexpr int kPagedMaxSms = 160;
+constexpr uint64_t kPagedTimeoutNs = 2000000000ull;  // bound on every wait for a load
 
 // Workspace: B + 2 ints (unit prefix of each request, units per run), then two records per CTA.
 template <int D, int RW>
@@ -234,25 +235,57 @@ __device__ __forceinline__ int paged_prefix(const PagedAttnParams& p, int* s_pre
   return total;
 }
 
-// smem row of a step's key: a warp's score fragment then has keys 8 t .. 8 t + 7 of the
-// step in the lanes t of a quad, so the suffix sum over a row is 8 additions in a lane and
-// one scan over the quad.  Row r of the tile holds key:
-__device__ __forceinline__ int paged_row_key(int r) { return 8 * ((r & 7) >> 1) + 2 * (r >> 3) + (r & 1); }
+// A 4-D tile load (column, slot, head, page) of the page pool.
+__device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const void* tmap, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(smem_dst),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// Order of a step's 32 keys in the score fragments.  Lane t of a quad holds keys
+// 8 t .. 8 t + 7, so a row's suffix sum is additions in a lane and one scan over the
+// quad; key tile n of the MMA takes the pair (n + t) % 4 of them, which spreads the
+// eight rows of a tile over all eight phases of the 128-byte swizzle (no bank conflicts).
+// Key of row j (0 .. 7) of tile n:
+__device__ __forceinline__ int paged_tile_key(int n, int j) {
+  const int t = j >> 1;
+  return 8 * t + 2 * ((n + t) & 3) + (j & 1);
+}
 
 template <int D, bool BF16, int RW, int XR>
-__global__ void __launch_bounds__(128) coalibi_paged_attn_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(128)
+    coalibi_paged_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                              const PagedAttnParams p) {
   using L = PagedLayout<D, RW>;
-  constexpr int KG = L::KG, KK = D / 16, CH = D / 8;
+  constexpr int KG = L::KG, KK = D / 16;
   constexpr int THREADS = 32 * RW;  // per key group
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ uint64_t s_full[KG * L::NBUF];
+  __shared__ int s_abort;
+  __shared__ volatile int s_fail[KG];
   __shared__ int s_pre[128], s_warp[4], s_find;
   __shared__ float4 s_stat[KG > 1 ? KG * L::ROWS : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gq = lane >> 2, tig = lane & 3;
-  const int rwarp = warp % RW, kg = warp / RW, gtid = tid % THREADS;
+  const int rwarp = warp % RW, kg = warp / RW;
+  const bool issuer = rwarp == 0 && lane == 0;  // of the group's loads
   const int G = p.Hq / p.Hkv, rows = G * p.Sq;
   const int heads = p.Hkv * p.row_blocks;  // items per request
   uint8_t* ring = smem + kg * L::RING;
+  uint64_t* full = s_full + kg * L::NBUF;
+  const CtaGuard guard{&s_abort, p.status, kPagedTimeoutNs};
+  if (tid == 0) {
+    for (int i = 0; i < KG * L::NBUF; ++i) mbar_init(&s_full[i], 1);
+    s_abort = 0;
+    for (int i = 0; i < KG; ++i) s_fail[i] = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
   grid_dep_wait();
 
   // ---- this CTA's run of units
@@ -276,6 +309,18 @@ __global__ void __launch_bounds__(128) coalibi_paged_attn_kernel(const PagedAttn
   }
   int item = (int)((at - (long long)pre * heads) / units);
   int u0 = (int)((at - (long long)pre * heads) - (long long)item * units);
+
+  // shared-memory offsets (within a tile) of this lane's ldmatrix rows; the k-step and the
+  // tile pair only flip bits of them: columns 32 * (kk % 4), pair 1 moves the key by 4
+  const int mat = lane >> 3, row8 = lane & 7;
+  const int key_k = paged_tile_key(mat >> 1, row8), key_v = paged_tile_key(mat & 1, row8);
+  const uint32_t off_k = key_k * 128 + (((mat & 1) ^ (key_k & 7)) << 4);
+  const uint32_t off_v = key_v * 128 + (((mat >> 1) ^ (key_v & 7)) << 4);
+  constexpr uint32_t kPair = 4 * 128 | 4 << 4;
+  int fill = 0, drain = 0;            // ring slots of the next load and of the next step
+  uint32_t fill_n = 0, drain_n = 0;   // loads issued, steps awaited
+  uint32_t phase = 0;                 // parity of the next step's barrier
+  bool ok = true;                     // no wait has run out
 
   for (bool first = true; at < stop; first = false) {
     const int u1 = (int)min((long long)units, u0 + (stop - at));
@@ -333,49 +378,45 @@ __global__ void __launch_bounds__(128) coalibi_paged_attn_kernel(const PagedAttn
     for (int x = 0; x < XR; ++x) m_run[x] = -INFINITY, l_part[x] = 0.f, carry[x] = 0.f;
 
     const int* table = p.page_table + (size_t)b * p.table_stride;
-    const uint16_t* kbase = static_cast<const uint16_t*>(p.k_pages) + g * p.kps[1];
-    const uint16_t* vbase = static_cast<const uint16_t*>(p.v_pages) + g * p.vps[1];
-    int page_id[2];    // of the next step to be staged, per half
-    uint32_t lost = 0;  // two bits per ring slot: halves whose page is outside the pool
+    int page_id[2], page_slot[2];  // of the next step to be loaded, per half; id -1: nothing there
+    uint32_t gone_q = 0;           // two bits per ring slot: halves that were not loaded
     auto lookup = [&](int st) {
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const int key = lo + st * kPagedStep + 16 * hf;
-        page_id[hf] = 0;
-        if (st >= 0 && key < hi) page_id[hf] = table[p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size];
+        page_id[hf] = -1;
+        page_slot[hf] = 0;
+        if (st >= 0 && key < hi) {
+          const int n = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+          page_id[hf] = table[n];
+          page_slot[hf] = key - n * p.page_size;
+          if ((unsigned)page_id[hf] >= (unsigned)p.n_pages) {
+            page_id[hf] = -1;
+            report_page(p.status);
+          }
+        }
       }
     };
-    auto stage = [&](int st) {
-      const int kb = lo + st * kPagedStep, slot = st % L::NBUF;
-      uint8_t* kt = ring + slot * 2 * L::TILE;
-      uint8_t* vt = kt + L::TILE;
-      const uint16_t* kr[2];
-      const uint16_t* vr[2];
-      bool in[2];
-      lost &= ~(3u << (2 * slot));
+    // the half steps are 16 keys of one page: a box of 64 columns x 16 slots each
+    auto load = [&]() {
+      gone_q &= ~(3u << (2 * fill));
+      gone_q |= ((page_id[0] < 0 ? 1u : 0u) | (page_id[1] < 0 ? 2u : 0u)) << (2 * fill);
+      if (issuer) {
+        const uint32_t dst = smem_u32(ring + fill * 2 * L::TILE);
+        const int halves = (page_id[0] >= 0) + (page_id[1] >= 0);
+        mbar_arrive_expect_tx(&full[fill], halves * L::TILE);
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int key = kb + 16 * hf;
-        const int first_slot = p.page_shift >= 0 ? key & (p.page_size - 1) : key % p.page_size;
-        in[hf] = (unsigned)page_id[hf] < (unsigned)p.n_pages;
-        if (!in[hf]) {
-          lost |= 1u << (2 * slot + hf);
-          report_page(p.status);
+        for (int hf = 0; hf < 2; ++hf) {
+          if (page_id[hf] < 0) continue;
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            tma_load_4d(dst + c * 4096 + hf * 2048, &tk, &full[fill], 64 * c, page_slot[hf], g, page_id[hf]);
+            tma_load_4d(dst + L::TILE + c * 4096 + hf * 2048, &tv, &full[fill], 64 * c, page_slot[hf], g, page_id[hf]);
+          }
         }
-        const long long pg = in[hf] ? page_id[hf] : 0;
-        kr[hf] = kbase + pg * p.kps[0] + first_slot * p.kps[2];
-        vr[hf] = vbase + pg * p.vps[0] + first_slot * p.vps[2];
       }
-#pragma unroll
-      for (int it = 0; it < kPagedStep * CH / THREADS; ++it) {
-        const int idx = it * THREADS + gtid;
-        const int row = idx / CH, c = idx % CH;
-        const int off = paged_row_key(row), hf = off >> 4, key = kb + off;
-        const bool ok = key < hi && in[hf] && (key < ctx || (seen_by_any >> (key - ctx) & 1));
-        const int dst = row * (D * 2) + ((c ^ (row & 7)) << 4);
-        cp_async16(kt + dst, kr[hf] + (ok ? (off & 15) * p.kps[2] + c * 8 : 0), ok);
-        cp_async16(vt + dst, vr[hf] + (ok ? (off & 15) * p.vps[2] + c * 8 : 0), ok);
-      }
+      fill = fill + 1 == L::NBUF ? 0 : fill + 1;
+      ++fill_n;
     };
     auto group_sync = [&]() {
       if (RW == 1)
@@ -387,19 +428,22 @@ __global__ void __launch_bounds__(128) coalibi_paged_attn_kernel(const PagedAttn
     lookup(nsteps - 1);
 #pragma unroll
     for (int a = 1; a < L::NBUF; ++a) {
-      if (nsteps - a >= 0) stage(nsteps - a);
-      cp_async_commit();
+      if (nsteps - a >= 0) load();
       lookup(nsteps - a - 1);
     }
     const float c_a = p.sm_scale * kLog2e;
-    const int mat = lane >> 3, row8 = lane & 7;
     for (int st = nsteps - 1; st >= 0; --st) {
-      cp_async_wait_pending<L::NBUF - 2>();  // this thread's part of step st has landed
-      group_sync();                          // the others' too, and all are done with step st + 1
-      if (st - (L::NBUF - 1) >= 0) stage(st - (L::NBUF - 1));
-      cp_async_commit();
+      if (ok && !mbar_wait(&full[drain], phase, guard)) s_fail[kg] = 1;
+      group_sync();  // all are done with step st + 1, whose slot is loaded next
+      ok = s_fail[kg] == 0;  // the same for the group's warps, which meet again in the masked steps
+      const int slot = drain;
+      drain = drain + 1 == L::NBUF ? 0 : drain + 1;
+      if (drain == 0) phase ^= 1;
+      ++drain_n;
+      if (!ok) continue;
+      if (st - (L::NBUF - 1) >= 0) load();
       lookup(st - L::NBUF);
-      const int slot = st % L::NBUF, kb = lo + st * kPagedStep;
+      const int kb = lo + st * kPagedStep;
       const uint32_t kt = smem_u32(ring + slot * 2 * L::TILE), vt = kt + L::TILE;
       // ---- S = Q K^T
       float sc[4][4];
@@ -410,27 +454,25 @@ __global__ void __launch_bounds__(128) coalibi_paged_attn_kernel(const PagedAttn
 #pragma unroll
         for (int np = 0; np < 2; ++np) {
           uint32_t b0, b1, b2, b3;
-          const int row = 16 * np + (mat >> 1) * 8 + row8, c = 2 * kk + (mat & 1);
-          ldsm_x4(kt + row * (D * 2) + ((c ^ row8) << 4), b0, b1, b2, b3);
+          ldsm_x4(kt + (off_k ^ (32 * (kk & 3)) ^ (np * kPair)) + (kk >> 2) * 4096, b0, b1, b2, b3);
           mma16816<BF16>(sc[2 * np], qa[kk], b0, b1);
           mma16816<BF16>(sc[2 * np + 1], qa[kk], b2, b3);
         }
       }
-      // ---- which of this lane's 8 keys (kb + 8 tig + j) each row sees
-      const bool all = kb + kPagedStep <= min(hi, ctx) && (lost >> (2 * slot) & 3) == 0;
+      // ---- which of this lane's 8 keys each row sees: bit 2 n + e for element e of tile n
+      const uint32_t gone = gone_q >> (2 * slot) & 3;
+      const bool all = kb + kPagedStep <= min(hi, ctx) && gone == 0;
       uint32_t vis[XR];
 #pragma unroll
       for (int x = 0; x < XR; ++x) vis[x] = 0xffu;
       if (!all) {
-        const int k0 = kb + 8 * tig;
-        const bool gone = lost >> (2 * slot + (tig >> 1)) & 1;
 #pragma unroll
         for (int x = 0; x < XR; ++x) {
           uint32_t v = 0;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const int key = k0 + j;
-            if (!gone && key < hi && (key < ctx || (word[x] >> (key - ctx) & 1))) v |= 1u << j;
+            const int key = kb + 8 * tig + 2 * (((j >> 1) + tig) & 3) + (j & 1);
+            if (!(gone >> (tig >> 1) & 1) && key < hi && (key < ctx || (word[x] >> (key - ctx) & 1))) v |= 1u << j;
           }
           vis[x] = v;
         }
@@ -438,31 +480,44 @@ __global__ void __launch_bounds__(128) coalibi_paged_attn_kernel(const PagedAttn
       // ---- sigmoids, suffix sums, logits (in log2 units), online softmax
 #pragma unroll
       for (int x = 0; x < XR; ++x) {
-        float suf[8];
-        float run = 0.f;
+        float sg[4], pr[4];  // sigmoid of a pair's second key, and of the pair
 #pragma unroll
-        for (int j = 7; j >= 0; --j) {
-          float& v = sc[j >> 1][2 * x + (j & 1)];
-          v *= c_a;
-          float sg = rcp_approx(1.f + ex2_approx(-v));
-          if (!all) sg = vis[x] >> j & 1 ? sg : 0.f;
-          run += sg;
-          suf[j] = run;
+        for (int n = 0; n < 4; ++n) {
+          float s2[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& v = sc[n][2 * x + e];
+            v *= c_a;
+            s2[e] = rcp_approx(1.f + ex2_approx(-v));
+            if (!all) s2[e] = vis[x] >> (2 * n + e) & 1 ? s2[e] : 0.f;
+          }
+          sg[n] = s2[1];
+          pr[n] = s2[0] + s2[1];
         }
-        float inc = run;
+        // tiles n >= 4 - t hold the lane's first pairs: their suffix also takes in all the
+        // others, whose own suffix stops at tile 3 - t
+        const float r2 = pr[3], r1 = r2 + pr[2], r0 = r1 + pr[1], tot = r0 + pr[0];
+        const float wrapped = tig == 0 ? 0.f : tig == 1 ? r2 : tig == 2 ? r1 : r0;
+        float inc = tot;
         float y = __shfl_down_sync(0xffffffffu, inc, 1);
         if (tig < 3) inc += y;
         y = __shfl_down_sync(0xffffffffu, inc, 2);
         if (tig < 2) inc += y;
-        const float base = carry[x] + (inc - run);
+        const float base = carry[x] + (inc - tot);
         carry[x] += __shfl_sync(0xffffffffu, inc, lane & ~3);
+        const float b_last = base - wrapped, b_first = b_last + tot;
+        const float after[4] = {b_last + r0, (tig == 3 ? b_first : b_last) + r1, (tig >= 2 ? b_first : b_last) + r2,
+                                tig >= 1 ? b_first : b_last};
         float mx = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float& v = sc[j >> 1][2 * x + (j & 1)];
-          v = fmaf(-slope2[x], suf[j] + base, v);
-          if (!all) v = vis[x] >> j & 1 ? v : -INFINITY;
-          mx = fmaxf(mx, v);
+        for (int n = 0; n < 4; ++n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& v = sc[n][2 * x + e];
+            v = fmaf(-slope2[x], after[n] + (e ? sg[n] : pr[n]), v);
+            if (!all) v = vis[x] >> (2 * n + e) & 1 ? v : -INFINITY;
+            mx = fmaxf(mx, v);
+          }
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -486,54 +541,58 @@ __global__ void __launch_bounds__(128) coalibi_paged_attn_kernel(const PagedAttn
           l_part[x] += v;
         }
       }
-      // ---- a drafted token's V that is not finite must not reach the rows that do not see
-      // it through 0 * V: such rows of the tile are added by hand and then zeroed
-      if (!all && p.Sq > 1 && kb + kPagedStep > ctx) {
-        uint8_t* vrow = ring + slot * 2 * L::TILE + L::TILE + lane * (D * 2);
+      // ---- V rows that no row sees (past the end, of no page, unseen drafts) may hold
+      // anything: zero them, 0 * NaN is not 0.  A drafted token's V that is not finite must
+      // not reach the rows that do not see it either: it is added by hand, then zeroed.
+      if (!all) {
+        const int key = kb + lane;
+        uint8_t* vrow = ring + slot * 2 * L::TILE + L::TILE + lane * 128;
+        const bool used = !(gone >> (lane >> 4) & 1) && key < hi && (key < ctx || (seen_by_any >> (key - ctx) & 1));
         bool bad = false;
-        if (kb + paged_row_key(lane) >= ctx) {
+        if (used && key >= ctx && p.Sq > 1) {
 #pragma unroll 4
-          for (int c = 0; c < CH; ++c) {
-            const uint4 u = *reinterpret_cast<const uint4*>(vrow + (c << 4));
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 u = *reinterpret_cast<const uint4*>(vrow + (c >> 3) * 4096 + ((c & 7) << 4));
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float2 f = unpack2<BF16>(w[j]);
-              bad |= !(fabsf(f.x) <= 3.4e38f) || !(fabsf(f.y) <= 3.4e38f);
+              bad |= !(fabsf(f.x) < INFINITY) || !(fabsf(f.y) < INFINITY);
             }
           }
         }
-        uint32_t bads = __ballot_sync(0xffffffffu, bad);
-        if (bads != 0) {
-          for (uint32_t left = bads; left != 0; left &= left - 1) {
-            const int row = __ffs(left) - 1, off = paged_row_key(row);
-            const uint8_t* vb = ring + slot * 2 * L::TILE + L::TILE + row * (D * 2);
+        for (uint32_t left = __ballot_sync(0xffffffffu, bad); left != 0; left &= left - 1) {
+          const int off = __ffs(left) - 1, t = off >> 3;
+          const int el = 2 * ((((off & 7) >> 1) - t) & 3) + (off & 1);  // 2 n + e in the lanes t
+          const uint8_t* vb = ring + slot * 2 * L::TILE + L::TILE + off * 128;
 #pragma unroll
-            for (int x = 0; x < XR; ++x) {
-              float w = 0.f;
-              uint32_t see = 0;
+          for (int x = 0; x < XR; ++x) {
+            float w = 0.f;
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if ((off & 7) == j) w = sc[j >> 1][2 * x + (j & 1)];
-              see = vis[x] >> (off & 7) & 1;
-              w = __shfl_sync(0xffffffffu, w, (lane & ~3) | (off >> 3));
-              see = __shfl_sync(0xffffffffu, see, (lane & ~3) | (off >> 3));
-              if (see) {
+            for (int j = 0; j < 8; ++j)
+              if (el == j) w = sc[j >> 1][2 * x + (j & 1)];
+            uint32_t see = vis[x] >> el & 1;
+            w = __shfl_sync(0xffffffffu, w, (lane & ~3) | t);
+            see = __shfl_sync(0xffffffffu, see, (lane & ~3) | t);
+            if (see) {
 #pragma unroll
-                for (int dn = 0; dn < 2 * KK; ++dn) {
-                  const float2 f =
-                      unpack2<BF16>(*reinterpret_cast<const uint32_t*>(vb + ((dn ^ (row & 7)) << 4) + 4 * tig));
-                  o[dn][2 * x] = fmaf(w, f.x, o[dn][2 * x]);
-                  o[dn][2 * x + 1] = fmaf(w, f.y, o[dn][2 * x + 1]);
-                }
+              for (int dn = 0; dn < 2 * KK; ++dn) {
+                const float2 f = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(
+                    vb + (dn >> 3) * 4096 + (((dn & 7) ^ (off & 7)) << 4) + 4 * tig));
+                o[dn][2 * x] = fmaf(w, f.x, o[dn][2 * x]);
+                o[dn][2 * x + 1] = fmaf(w, f.y, o[dn][2 * x + 1]);
               }
             }
           }
-          group_sync();
-          if (rwarp == 0 && bad)
-            for (int c = 0; c < CH; ++c) *reinterpret_cast<uint4*>(vrow + (c << 4)) = make_uint4(0u, 0u, 0u, 0u);
-          group_sync();
         }
+        group_sync();
+        if (rwarp == 0 && (!used || bad)) {
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            *reinterpret_cast<uint4*>(vrow + (c >> 3) * 4096 + ((c & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+          fence_async_smem();  // ordered before the load that refills the slot
+        }
+        group_sync();
       }
       // ---- O += P V: the C fragments of two key tiles are the A fragment of one k-step.
       // P is rounded to the inputs' type for the product; l sums it unrounded.
@@ -547,14 +606,20 @@ __global__ void __launch_bounds__(128) coalibi_paged_attn_kernel(const PagedAttn
 #pragma unroll
         for (int dp = 0; dp < KK; ++dp) {
           uint32_t b0, b1, b2, b3;
-          const int row = 16 * k2 + (mat & 1) * 8 + row8, c = 2 * dp + (mat >> 1);
-          ldsm_x4_t(vt + row * (D * 2) + ((c ^ row8) << 4), b0, b1, b2, b3);
+          ldsm_x4_t(vt + (off_v ^ (32 * (dp & 3)) ^ (k2 * kPair)) + (dp >> 2) * 4096, b0, b1, b2, b3);
           mma16816<BF16>(o[2 * dp], pa, b0, b1);
           mma16816<BF16>(o[2 * dp + 1], pa, b2, b3);
         }
       }
     }
-    cp_async_wait_all();
+    if (!ok && issuer) {  // a wait ran out: let the loads already issued land before leaving
+      for (; drain_n < fill_n; ++drain_n) {
+        mbar_drain(&full[drain], phase, kPagedTimeoutNs);
+        drain = drain + 1 == L::NBUF ? 0 : drain + 1;
+        if (drain == 0) phase ^= 1;
+      }
+    }
+    if (!ok) drain_n = fill_n;
 #pragma unroll
     for (int x = 0; x < XR; ++x) {
       l_part[x] += __shfl_xor_sync(0xffffffffu, l_part[x], 1);
@@ -636,7 +701,9 @@ __global__ void __launch_bounds__(128) coalibi_paged_attn_kernel(const PagedAttn
         }
       }
     }
+    if (KG > 1) fence_async_smem();
     __syncthreads();  // the rings are free for the next item
+    if (s_abort != 0) return;
 
     // ---- next item of the run
     at += u1 - u0;

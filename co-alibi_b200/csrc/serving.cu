@@ -3,6 +3,7 @@
 // checked before any device use; nothing here allocates or synchronises.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 
@@ -14,6 +15,8 @@
 namespace coalibi {
 
 void set_last_error_detail(const char* msg);
+int make_page_tmap(CUtensorMap* map, const void* base, int D, int page_size, int heads, int pages,
+                   const long long* stride, bool bf16);
 
 namespace {
 
@@ -49,6 +52,12 @@ int check_cache(int B, int Hkv, int D, int page_size, int max_pages, int n_pages
   if ((long long)max_pages * page_size > 0x7fffff00LL || table_stride < 0 || B > 65535 || Hkv > 65535)
     return COALIBI_ERR_SHAPE;
   if (!row_strides(k_page_stride) || !row_strides(v_page_stride)) return COALIBI_ERR_ALIGNMENT;
+  const int sizes[3] = {n_pages, Hkv, page_size};
+  for (int i = 0; i < 3; ++i) {
+    const long long k = k_page_stride[i], v = v_page_stride[i];
+    if (sizes[i] > 1 && (k == 0 || v == 0)) return COALIBI_ERR_SHAPE;  // entries on top of each other
+    if (k >= 1LL << 39 || v >= 1LL << 39) return COALIBI_ERR_SHAPE;
+  }
   return COALIBI_OK;
 }
 
@@ -119,11 +128,17 @@ namespace coalibi {
 namespace {
 
 template <int D, bool BF16, int RW, int XR>
-int launch_paged(PagedAttnParams& p, int sms, cudaStream_t s) {
+int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& p, int sms, cudaStream_t s) {
   using L = PagedLayout<D, RW>;
-  // once per device would do; the call is a few hundred nanoseconds and needs no state
-  cudaError_t e = cudaFuncSetAttribute(coalibi_paged_attn_kernel<D, BF16, RW, XR>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
+  cudaError_t e = cudaSuccess;
+  static std::atomic<unsigned long long> ready{0};  // bit per device (the library knows at most 64)
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    e = cudaFuncSetAttribute(coalibi_paged_attn_kernel<D, BF16, RW, XR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             L::BYTES);
+    if (e == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   const int rows = p.Hq / p.Hkv * p.Sq;
   p.row_blocks = (rows + L::ROWS - 1) / L::ROWS;
   p.n_ctas = (sms < kPagedMaxSms ? sms : kPagedMaxSms) * L::CTAS;
@@ -132,7 +147,7 @@ int launch_paged(PagedAttnParams& p, int sms, cudaStream_t s) {
   if (bound > 0x7fffffffLL) return COALIBI_ERR_SHAPE;
   if (bound < p.n_ctas) p.n_ctas = (int)bound;
   if (e == cudaSuccess)
-    e = launch_pdl(coalibi_paged_attn_kernel<D, BF16, RW, XR>, dim3(p.n_ctas), dim3(128), L::BYTES, s, p);
+    e = launch_pdl(coalibi_paged_attn_kernel<D, BF16, RW, XR>, dim3(p.n_ctas), dim3(128), L::BYTES, s, tk, tv, p);
   // an item of one unit is never split
   if (e == cudaSuccess && most > 1)
     e = launch_pdl(coalibi_paged_join_kernel<D, BF16, RW>, dim3(p.B * p.Hkv, (rows + 3) / 4), dim3(128), 0, s, p);
@@ -141,12 +156,12 @@ int launch_paged(PagedAttnParams& p, int sms, cudaStream_t s) {
 }
 
 template <int D, bool BF16>
-int launch_paged_rows(PagedAttnParams& p, int sms, cudaStream_t s) {
+int launch_paged_rows(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& p, int sms, cudaStream_t s) {
   const int rows = p.Hq / p.Hkv * p.Sq;
   switch (paged_row_warps(rows)) {
-    case 1: return rows <= 8 ? launch_paged<D, BF16, 1, 1>(p, sms, s) : launch_paged<D, BF16, 1, 2>(p, sms, s);
-    case 2: return launch_paged<D, BF16, 2, 2>(p, sms, s);
-    default: return launch_paged<D, BF16, 4, 2>(p, sms, s);
+    case 1: return rows <= 8 ? launch_paged<D, BF16, 1, 1>(tk, tv, p, sms, s) : launch_paged<D, BF16, 1, 2>(tk, tv, p, sms, s);
+    case 2: return launch_paged<D, BF16, 2, 2>(tk, tv, p, sms, s);
+    default: return launch_paged<D, BF16, 4, 2>(tk, tv, p, sms, s);
   }
 }
 
@@ -219,8 +234,11 @@ extern "C" int coalibi_paged_attention(const CoalibiPagedAttentionArgs* a, void*
     if (a->page_size == 1 << k) p.page_shift = k;
   const bool bf16 = a->dtype == COALIBI_BF16;
   const int sms = device_sm_count();
-  if (a->D == 128) return bf16 ? launch_paged_rows<128, true>(p, sms, s) : launch_paged_rows<128, false>(p, sms, s);
-  return bf16 ? launch_paged_rows<64, true>(p, sms, s) : launch_paged_rows<64, false>(p, sms, s);
+  CUtensorMap tk, tv;
+  if ((rc = make_page_tmap(&tk, a->k_pages, a->D, a->page_size, a->Hkv, a->n_pages, a->k_page_stride, bf16))) return rc;
+  if ((rc = make_page_tmap(&tv, a->v_pages, a->D, a->page_size, a->Hkv, a->n_pages, a->v_page_stride, bf16))) return rc;
+  if (a->D == 128) return bf16 ? launch_paged_rows<128, true>(tk, tv, p, sms, s) : launch_paged_rows<128, false>(tk, tv, p, sms, s);
+  return bf16 ? launch_paged_rows<64, true>(tk, tv, p, sms, s) : launch_paged_rows<64, false>(tk, tv, p, sms, s);
 }
 
 extern "C" int coalibi_sample(const CoalibiSampleArgs* a, void* stream) {
