@@ -2,6 +2,8 @@
 // way) and Co-ALiBi attention of one token or of a tree of drafted tokens over it.
 #pragma once
 
+#include <type_traits>
+
 #include "sm100.cuh"
 #include "decode.cuh"
 #include "fwd.cuh"
@@ -165,6 +167,9 @@ struct PagedAttnParams {
 };
 
 constexpr int kPagedStep = 32;  // keys per step of a warp
+// What starting and finishing an item costs, in units: lengths, queries and the first
+// load's latency before its keys, the join of the key groups after them.
+constexpr int kPagedItemCost = 3;
 
 template <int D, int RW>
 struct PagedLayout {
@@ -184,7 +189,7 @@ struct PagedLayout {
 constexpr int kPagedMaxSms = 160;
 constexpr uint64_t kPagedTimeoutNs = 2000000000ull;  // bound on every wait for a load
 
-// Workspace: B + 2 ints (unit prefix of each request, units per run), then two records per CTA.
+// Workspace: B + 2 ints (prefix of the requests' spans, units per run), then two records per CTA.
 template <int D, int RW>
 inline size_t paged_ws_bytes(int B) {
   using L = PagedLayout<D, RW>;
@@ -201,13 +206,19 @@ __device__ __forceinline__ int paged_keys(const PagedAttnParams& p, int b) {
   return min(min(max(p.ctx_lens[b], 0), room) + p.Sq, room);
 }
 
-// One thread per request range: exclusive prefix sums of the requests' units.  Returns
+// Units of an item of request b, with its overhead.
+template <int UNIT>
+__device__ __forceinline__ int paged_span(const PagedAttnParams& p, int b) {
+  return (paged_keys(p, b) + UNIT - 1) / UNIT + kPagedItemCost;
+}
+
+// One thread per request range: exclusive prefix sums of the requests' spans.  Returns
 // the total; s_pre[t] is the prefix at the first request of thread t's range.
 template <int UNIT>
 __device__ __forceinline__ int paged_prefix(const PagedAttnParams& p, int* s_pre, int* s_warp, int per, int* out) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int sum = 0;
-  for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) sum += (paged_keys(p, b) + UNIT - 1) / UNIT;
+  for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) sum += paged_span<UNIT>(p, b);
   int inc = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -227,7 +238,7 @@ __device__ __forceinline__ int paged_prefix(const PagedAttnParams& p, int* s_pre
   if (out != nullptr) {
     for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) {
       out[b] = at;
-      at += (paged_keys(p, b) + UNIT - 1) / UNIT;
+      at += paged_span<UNIT>(p, b);
     }
     if (tid == 0) out[p.B] = total;
   }
@@ -287,6 +298,7 @@ __global__ void __launch_bounds__(128)
     tma_prefetch_desc(&tv);
   }
   grid_dep_wait();
+  grid_dep_launch();  // the joining kernel may set up; it waits for this grid's end
 
   // ---- this CTA's run of units
   int* head = reinterpret_cast<int*>(p.ws);
@@ -301,14 +313,14 @@ __global__ void __launch_bounds__(128)
   if ((long long)s_pre[tid] * heads <= at && (tid == 127 || (long long)s_pre[tid + 1] * heads > at)) s_find = tid;
   __syncthreads();
   int b = s_find * per, pre = s_pre[s_find];
-  int units = (paged_keys(p, b) + L::UNIT - 1) / L::UNIT;
-  while ((long long)(pre + units) * heads <= at) {
-    pre += units;
+  int span = paged_span<L::UNIT>(p, b);
+  while ((long long)(pre + span) * heads <= at) {
+    pre += span;
     ++b;
-    units = (paged_keys(p, b) + L::UNIT - 1) / L::UNIT;
+    span = paged_span<L::UNIT>(p, b);
   }
-  int item = (int)((at - (long long)pre * heads) / units);
-  int u0 = (int)((at - (long long)pre * heads) - (long long)item * units);
+  int item = (int)((at - (long long)pre * heads) / span);
+  int v0 = (int)((at - (long long)pre * heads) - (long long)item * span);
 
   // shared-memory offsets (within a tile) of this lane's ldmatrix rows; the k-step and the
   // tile pair only flip bits of them: columns 32 * (kk % 4), pair 1 moves the key by 4
@@ -322,8 +334,11 @@ __global__ void __launch_bounds__(128)
   uint32_t phase = 0;                 // parity of the next step's barrier
   bool ok = true;                     // no wait has run out
 
-  for (bool first = true; at < stop; first = false) {
-    const int u1 = (int)min((long long)units, u0 + (stop - at));
+  while (at < stop) {
+    // units [u0, u1) of the item; none if the run ends within its overhead
+    const int v1 = (int)min((long long)span, v0 + (stop - at));
+    const int u0 = max(v0 - kPagedItemCost, 0), u1 = v1 - kPagedItemCost, units = span - kPagedItemCost;
+    if (u1 <= 0) break;
     const int g = item / p.row_blocks, r0 = (item - g * p.row_blocks) * L::ROWS + rwarp * 16;
     const int len = p.ctx_lens[b], room = p.max_pages * p.page_size, ctx = min(max(len, 0), room);
 
@@ -465,7 +480,106 @@ __global__ void __launch_bounds__(128)
       uint32_t vis[XR];
 #pragma unroll
       for (int x = 0; x < XR; ++x) vis[x] = 0xffu;
-      if (!all) {
+      // ---- sigmoids, suffix sums, logits (in log2 units), online softmax.  The rows go
+      // through each stage together (their chains overlap), pairs of keys as float2.
+      auto softmax = [&](auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        float2 sg[XR][4];                 // sigmoids of a pair: x first key, y second
+        float pr[XR][4], tot[XR], inc[XR];
+#pragma unroll
+        for (int x = 0; x < XR; ++x) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            float2 v = __fmul2_rn(make_float2(sc[n][2 * x], sc[n][2 * x + 1]), make_float2(c_a, c_a));
+            sc[n][2 * x] = v.x;
+            sc[n][2 * x + 1] = v.y;
+            v = __fadd2_rn(make_float2(ex2_approx(-v.x), ex2_approx(-v.y)), make_float2(1.f, 1.f));
+            sg[x][n] = make_float2(rcp_approx(v.x), rcp_approx(v.y));
+            if (MASKED) {
+              sg[x][n].x = vis[x] >> (2 * n) & 1 ? sg[x][n].x : 0.f;
+              sg[x][n].y = vis[x] >> (2 * n + 1) & 1 ? sg[x][n].y : 0.f;
+            }
+            pr[x][n] = sg[x][n].x + sg[x][n].y;
+          }
+          tot[x] = ((pr[x][0] + pr[x][1]) + (pr[x][2] + pr[x][3]));
+          inc[x] = tot[x];
+        }
+#pragma unroll
+        for (int d = 1; d <= 2; ++d) {
+#pragma unroll
+          for (int x = 0; x < XR; ++x) {
+            const float y = __shfl_down_sync(0xffffffffu, inc[x], d);
+            if (tig + d < 4) inc[x] += y;
+          }
+        }
+        float mx[XR];
+#pragma unroll
+        for (int x = 0; x < XR; ++x) {
+          // tiles n >= 4 - t hold the lane's first pairs: their suffix also takes in all the
+          // others, whose own suffix stops at tile 3 - t
+          const float r2 = pr[x][3], r1 = r2 + pr[x][2], r0 = r1 + pr[x][1];
+          const float wrapped = tig == 0 ? 0.f : tig == 1 ? r2 : tig == 2 ? r1 : r0;
+          const float b_last = carry[x] + ((inc[x] - tot[x]) - wrapped), b_first = b_last + tot[x];
+          carry[x] += __shfl_sync(0xffffffffu, inc[x], lane & ~3);
+          const float after[4] = {b_last + r0, (tig == 3 ? b_first : b_last) + r1,
+                                  (tig >= 2 ? b_first : b_last) + r2, tig >= 1 ? b_first : b_last};
+          float m4[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float2 z = __fadd2_rn(make_float2(pr[x][n], sg[x][n].y), make_float2(after[n], after[n]));
+            float2 v = __ffma2_rn(make_float2(-slope2[x], -slope2[x]), z,
+                                  make_float2(sc[n][2 * x], sc[n][2 * x + 1]));
+            if (MASKED) {
+              v.x = vis[x] >> (2 * n) & 1 ? v.x : -INFINITY;
+              v.y = vis[x] >> (2 * n + 1) & 1 ? v.y : -INFINITY;
+            }
+            sc[n][2 * x] = v.x;
+            sc[n][2 * x + 1] = v.y;
+            m4[n] = fmaxf(v.x, v.y);
+          }
+          mx[x] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        }
+#pragma unroll
+        for (int d = 1; d <= 2; ++d) {
+#pragma unroll
+          for (int x = 0; x < XR; ++x) mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], d));
+        }
+        // the newest keys weigh most, so the maximum seldom moves after the first steps
+        bool up = mx[0] > m_run[0];
+        if (XR > 1) up |= mx[XR - 1] > m_run[XR - 1];
+        if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+          for (int x = 0; x < XR; ++x) {
+            const float m_new = fmaxf(m_run[x], mx[x]);
+            const float fac = m_run[x] == -INFINITY ? 0.f : ex2_approx(m_run[x] - m_new);
+            m_run[x] = m_new;
+            l_part[x] *= fac;
+#pragma unroll
+            for (int dn = 0; dn < 2 * KK; ++dn) {
+              o[dn][2 * x] *= fac;
+              o[dn][2 * x + 1] *= fac;
+            }
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < XR; ++x) {
+          const float m_use = m_run[x] == -INFINITY ? 0.f : m_run[x];
+          float2 l2 = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float2 v =
+                __fadd2_rn(make_float2(sc[n][2 * x], sc[n][2 * x + 1]), make_float2(-m_use, -m_use));
+            const float2 w = make_float2(ex2_approx(v.x), ex2_approx(v.y));
+            l2 = __fadd2_rn(l2, w);
+            sc[n][2 * x] = w.x;
+            sc[n][2 * x + 1] = w.y;
+          }
+          l_part[x] += l2.x + l2.y;
+        }
+      };
+      if (all) {
+        softmax(std::false_type{});
+      } else {
 #pragma unroll
         for (int x = 0; x < XR; ++x) {
           uint32_t v = 0;
@@ -476,70 +590,7 @@ __global__ void __launch_bounds__(128)
           }
           vis[x] = v;
         }
-      }
-      // ---- sigmoids, suffix sums, logits (in log2 units), online softmax
-#pragma unroll
-      for (int x = 0; x < XR; ++x) {
-        float sg[4], pr[4];  // sigmoid of a pair's second key, and of the pair
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          float s2[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& v = sc[n][2 * x + e];
-            v *= c_a;
-            s2[e] = rcp_approx(1.f + ex2_approx(-v));
-            if (!all) s2[e] = vis[x] >> (2 * n + e) & 1 ? s2[e] : 0.f;
-          }
-          sg[n] = s2[1];
-          pr[n] = s2[0] + s2[1];
-        }
-        // tiles n >= 4 - t hold the lane's first pairs: their suffix also takes in all the
-        // others, whose own suffix stops at tile 3 - t
-        const float r2 = pr[3], r1 = r2 + pr[2], r0 = r1 + pr[1], tot = r0 + pr[0];
-        const float wrapped = tig == 0 ? 0.f : tig == 1 ? r2 : tig == 2 ? r1 : r0;
-        float inc = tot;
-        float y = __shfl_down_sync(0xffffffffu, inc, 1);
-        if (tig < 3) inc += y;
-        y = __shfl_down_sync(0xffffffffu, inc, 2);
-        if (tig < 2) inc += y;
-        const float base = carry[x] + (inc - tot);
-        carry[x] += __shfl_sync(0xffffffffu, inc, lane & ~3);
-        const float b_last = base - wrapped, b_first = b_last + tot;
-        const float after[4] = {b_last + r0, (tig == 3 ? b_first : b_last) + r1, (tig >= 2 ? b_first : b_last) + r2,
-                                tig >= 1 ? b_first : b_last};
-        float mx = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& v = sc[n][2 * x + e];
-            v = fmaf(-slope2[x], after[n] + (e ? sg[n] : pr[n]), v);
-            if (!all) v = vis[x] >> (2 * n + e) & 1 ? v : -INFINITY;
-            mx = fmaxf(mx, v);
-          }
-        }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        // the newest keys weigh most, so the maximum seldom moves after the first steps
-        if (__any_sync(0xffffffffu, mx > m_run[x])) {
-          const float m_new = fmaxf(m_run[x], mx);
-          const float fac = m_run[x] == -INFINITY ? 0.f : ex2_approx(m_run[x] - m_new);
-          m_run[x] = m_new;
-          l_part[x] *= fac;
-#pragma unroll
-          for (int dn = 0; dn < 2 * KK; ++dn) {
-            o[dn][2 * x] *= fac;
-            o[dn][2 * x + 1] *= fac;
-          }
-        }
-        const float m_use = m_run[x] == -INFINITY ? 0.f : m_run[x];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float& v = sc[j >> 1][2 * x + (j & 1)];
-          v = ex2_approx(v - m_use);
-          l_part[x] += v;
-        }
+        softmax(std::true_type{});
       }
       // ---- V rows that no row sees (past the end, of no page, unseen drafts) may hold
       // anything: zero them, 0 * NaN is not 0.  A drafted token's V that is not finite must
@@ -628,7 +679,7 @@ __global__ void __launch_bounds__(128)
 
     // ---- the piece's result: the output if the item is whole, else a record
     const bool whole = u0 == 0 && u1 == units;
-    float* rec = p.ws + paged_ws_head(p.B) + ((size_t)blockIdx.x * 2 + (first && u0 > 0 ? 0 : 1)) * L::RECORD;
+    float* rec = p.ws + paged_ws_head(p.B) + ((size_t)blockIdx.x * 2 + (u0 > 0 ? 0 : 1)) * L::RECORD;
     float4* stats = reinterpret_cast<float4*>(rec);
     float* orec = rec + 4 * L::ROWS;
     if (KG == 1) {
@@ -706,12 +757,11 @@ __global__ void __launch_bounds__(128)
     if (s_abort != 0) return;
 
     // ---- next item of the run
-    at += u1 - u0;
-    u0 = 0;
+    at += v1 - v0;
+    v0 = 0;
     if (++item == heads) {
       item = 0;
-      pre += units;
-      if (++b < p.B) units = (paged_keys(p, b) + L::UNIT - 1) / L::UNIT;
+      if (++b < p.B) span = paged_span<L::UNIT>(p, b);
     }
   }
 }
@@ -730,9 +780,10 @@ __global__ void __launch_bounds__(128) coalibi_paged_join_kernel(const PagedAttn
   if (r >= rows) return;
   const int* head = reinterpret_cast<const int*>(p.ws);
   const int heads = p.Hkv * p.row_blocks, item = g * p.row_blocks + r / L::ROWS, rr = r % L::ROWS;
-  const int units = head[b + 1] - head[b];
+  const int span = head[b + 1] - head[b];
   const long long quota = head[p.B + 1];
-  const long long t0 = (long long)head[b] * heads + (long long)item * units, t1 = t0 + units;
+  const long long start = (long long)head[b] * heads + (long long)item * span;
+  const long long t0 = start + kPagedItemCost, t1 = start + span;
   const int c0 = (int)(t0 / quota), c1 = (int)((t1 - 1) / quota);
   if (c0 == c1) return;  // finished by the attention kernel
   const int h = g * G + r / p.Sq, i = r % p.Sq;

@@ -143,7 +143,7 @@ int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& 
   p.row_blocks = (rows + L::ROWS - 1) / L::ROWS;
   p.n_ctas = (sms < kPagedMaxSms ? sms : kPagedMaxSms) * L::CTAS;
   const long long most = ((long long)p.max_pages * p.page_size + L::UNIT - 1) / L::UNIT;
-  const long long bound = most * p.B * p.Hkv * p.row_blocks;  // units, if every table row were full
+  const long long bound = (most + kPagedItemCost) * p.B * p.Hkv * p.row_blocks;  // if every table row were full
   if (bound > 0x7fffffffLL) return COALIBI_ERR_SHAPE;
   if (bound < p.n_ctas) p.n_ctas = (int)bound;
   if (e == cudaSuccess)
