@@ -167,14 +167,17 @@ struct PagedAttnParams {
 };
 
 constexpr int kPagedStep = 32;  // keys per step of a warp
-// What starting and finishing an item costs, in units: lengths, queries and the first
-// load's latency before its keys, the join of the key groups after them.
-constexpr int kPagedItemCost = 3;
 
 template <int D, int RW>
 struct PagedLayout {
   static constexpr int KG = 4 / RW;
   static constexpr int UNIT = kPagedStep * KG;
+  // What starting and finishing an item costs, in units (256 keys' worth): lengths,
+  // queries and the first load's latency before its keys, the results after them.  Ragged
+  // decoding of 16 requests of 0 .. 8191 keys: 81 us without, 60 / 62 / 65 / 69 us with 2 / 3
+  // / 5 / 8 units of 128 keys; trees of 16 over 127 .. 16383: 166 us, with 2 / 3 / 5 / 8 units
+  // of 32 keys 135 / 123 / 121 / 120 us.
+  static constexpr int COST = 256 / UNIT;
   static constexpr int ROWS = 16 * RW;
   static constexpr int TILE = kPagedStep * D * 2;  // K or V of one step: [D / 64][32 keys][128 bytes], swizzled
   static constexpr int NBUF = RW == 4 ? 4 : 3;     // all but one of the steps in flight
@@ -207,18 +210,18 @@ __device__ __forceinline__ int paged_keys(const PagedAttnParams& p, int b) {
 }
 
 // Units of an item of request b, with its overhead.
-template <int UNIT>
+template <typename L>
 __device__ __forceinline__ int paged_span(const PagedAttnParams& p, int b) {
-  return (paged_keys(p, b) + UNIT - 1) / UNIT + kPagedItemCost;
+  return (paged_keys(p, b) + L::UNIT - 1) / L::UNIT + L::COST;
 }
 
 // One thread per request range: exclusive prefix sums of the requests' spans.  Returns
 // the total; s_pre[t] is the prefix at the first request of thread t's range.
-template <int UNIT>
+template <typename L>
 __device__ __forceinline__ int paged_prefix(const PagedAttnParams& p, int* s_pre, int* s_warp, int per, int* out) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int sum = 0;
-  for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) sum += paged_span<UNIT>(p, b);
+  for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) sum += paged_span<L>(p, b);
   int inc = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -238,7 +241,7 @@ __device__ __forceinline__ int paged_prefix(const PagedAttnParams& p, int* s_pre
   if (out != nullptr) {
     for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) {
       out[b] = at;
-      at += paged_span<UNIT>(p, b);
+      at += paged_span<L>(p, b);
     }
     if (tid == 0) out[p.B] = total;
   }
@@ -298,12 +301,11 @@ __global__ void __launch_bounds__(128)
     tma_prefetch_desc(&tv);
   }
   grid_dep_wait();
-  grid_dep_launch();  // the joining kernel may set up; it waits for this grid's end
 
   // ---- this CTA's run of units
   int* head = reinterpret_cast<int*>(p.ws);
   const int per = (p.B + 127) / 128;
-  const long long total = (long long)paged_prefix<L::UNIT>(p, s_pre, s_warp, per, blockIdx.x == 0 ? head : nullptr) * heads;
+  const long long total = (long long)paged_prefix<L>(p, s_pre, s_warp, per, blockIdx.x == 0 ? head : nullptr) * heads;
   const long long quota = (total + p.n_ctas - 1) / p.n_ctas;
   if (blockIdx.x == 0 && tid == 0) head[p.B + 1] = (int)quota;
   long long at = quota * blockIdx.x;
@@ -313,11 +315,11 @@ __global__ void __launch_bounds__(128)
   if ((long long)s_pre[tid] * heads <= at && (tid == 127 || (long long)s_pre[tid + 1] * heads > at)) s_find = tid;
   __syncthreads();
   int b = s_find * per, pre = s_pre[s_find];
-  int span = paged_span<L::UNIT>(p, b);
+  int span = paged_span<L>(p, b);
   while ((long long)(pre + span) * heads <= at) {
     pre += span;
     ++b;
-    span = paged_span<L::UNIT>(p, b);
+    span = paged_span<L>(p, b);
   }
   int item = (int)((at - (long long)pre * heads) / span);
   int v0 = (int)((at - (long long)pre * heads) - (long long)item * span);
@@ -337,27 +339,13 @@ __global__ void __launch_bounds__(128)
   while (at < stop) {
     // units [u0, u1) of the item; none if the run ends within its overhead
     const int v1 = (int)min((long long)span, v0 + (stop - at));
-    const int u0 = max(v0 - kPagedItemCost, 0), u1 = v1 - kPagedItemCost, units = span - kPagedItemCost;
+    const int u0 = max(v0 - L::COST, 0), u1 = v1 - L::COST, units = span - L::COST;
     if (u1 <= 0) break;
     const int g = item / p.row_blocks, r0 = (item - g * p.row_blocks) * L::ROWS + rwarp * 16;
     const int len = p.ctx_lens[b], room = p.max_pages * p.page_size, ctx = min(max(len, 0), room);
 
-    // ---- the rows: visibility words, slopes, queries as A fragments
-    unsigned long long word[XR];
-    unsigned long long seen_by_any = 0;  // over all rows of the request
-    float slope2[XR];
-    const uint16_t* qrow[XR];
-    bool rok[XR];
-#pragma unroll
-    for (int x = 0; x < XR; ++x) {
-      const int r = r0 + gq + 8 * x;
-      rok[x] = r < rows;
-      const int rr = rok[x] ? r : 0;
-      const int h = g * G + rr / p.Sq, i = rr % p.Sq;
-      word[x] = p.tree_mask != nullptr ? (unsigned long long)p.tree_mask[b * p.mask_stride + i] : (2ull << i) - 1;
-      slope2[x] = load_slope(p.slopes, p.slopes_dtype, h) * kLog2e;
-      qrow[x] = static_cast<const uint16_t*>(p.q) + b * p.qs[0] + h * p.qs[1] + i * p.qs[2];
-    }
+    // ---- drafted tokens that any row of the request sees
+    unsigned long long seen_by_any = 0;
     if (p.tree_mask == nullptr) {
       seen_by_any = (2ull << (p.Sq - 1)) - 1;
     } else {
@@ -368,29 +356,12 @@ __global__ void __launch_bounds__(128)
     }
     const int drafts = 64 - __clzll((long long)seen_by_any);
     if ((len > room || ctx + drafts > room) && tid == 0) report_page(p.status);
-    uint32_t qa[KK][4];
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          qa[kk][2 * hf + x] = x < XR && rok[x % XR]
-                                   ? *reinterpret_cast<const uint32_t*>(qrow[x % XR] + 16 * kk + 8 * hf + 2 * tig)
-                                   : 0u;
 
     // ---- this key group's keys: [lo, hi), lo a multiple of 16 (so a half step lies in one page)
     const int s_lo = u0 * L::UNIT, s_hi = min(min(u1 * L::UNIT, room), ctx + drafts);
     const int sub = ((s_hi - s_lo + KG - 1) / KG + 15) & ~15;
     const int lo = s_lo + kg * sub, hi = min(s_hi, lo + sub);
     const int nsteps = hi > lo ? (hi - lo + kPagedStep - 1) / kPagedStep : 0;
-
-    float o[2 * KK][4];
-#pragma unroll
-    for (int dn = 0; dn < 2 * KK; ++dn) o[dn][0] = o[dn][1] = o[dn][2] = o[dn][3] = 0.f;
-    float m_run[XR], l_part[XR], carry[XR];
-#pragma unroll
-    for (int x = 0; x < XR; ++x) m_run[x] = -INFINITY, l_part[x] = 0.f, carry[x] = 0.f;
 
     const int* table = p.page_table + (size_t)b * p.table_stride;
     int page_id[2], page_slot[2];  // of the next step to be loaded, per half; id -1: nothing there
@@ -446,6 +417,40 @@ __global__ void __launch_bounds__(128)
       if (nsteps - a >= 0) load();
       lookup(nsteps - a - 1);
     }
+
+    // ---- the rows: visibility words, slopes, queries as A fragments
+    unsigned long long word[XR];
+    float slope2[XR];
+    const uint16_t* qrow[XR];
+    bool rok[XR];
+#pragma unroll
+    for (int x = 0; x < XR; ++x) {
+      const int r = r0 + gq + 8 * x;
+      rok[x] = r < rows;
+      const int rr = rok[x] ? r : 0;
+      const int h = g * G + rr / p.Sq, i = rr % p.Sq;
+      word[x] = p.tree_mask != nullptr ? (unsigned long long)p.tree_mask[b * p.mask_stride + i] : (2ull << i) - 1;
+      slope2[x] = load_slope(p.slopes, p.slopes_dtype, h) * kLog2e;
+      qrow[x] = static_cast<const uint16_t*>(p.q) + b * p.qs[0] + h * p.qs[1] + i * p.qs[2];
+    }
+    uint32_t qa[KK][4];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          qa[kk][2 * hf + x] = x < XR && rok[x % XR]
+                                   ? *reinterpret_cast<const uint32_t*>(qrow[x % XR] + 16 * kk + 8 * hf + 2 * tig)
+                                   : 0u;
+
+    float o[2 * KK][4];
+#pragma unroll
+    for (int dn = 0; dn < 2 * KK; ++dn) o[dn][0] = o[dn][1] = o[dn][2] = o[dn][3] = 0.f;
+    float m_run[XR], l_part[XR], carry[XR];
+#pragma unroll
+    for (int x = 0; x < XR; ++x) m_run[x] = -INFINITY, l_part[x] = 0.f, carry[x] = 0.f;
+
     const float c_a = p.sm_scale * kLog2e;
     for (int st = nsteps - 1; st >= 0; --st) {
       if (ok && !mbar_wait(&full[drain], phase, guard)) s_fail[kg] = 1;
@@ -761,7 +766,7 @@ __global__ void __launch_bounds__(128)
     v0 = 0;
     if (++item == heads) {
       item = 0;
-      if (++b < p.B) span = paged_span<L::UNIT>(p, b);
+      if (++b < p.B) span = paged_span<L>(p, b);
     }
   }
 }
@@ -783,7 +788,7 @@ __global__ void __launch_bounds__(128) coalibi_paged_join_kernel(const PagedAttn
   const int span = head[b + 1] - head[b];
   const long long quota = head[p.B + 1];
   const long long start = (long long)head[b] * heads + (long long)item * span;
-  const long long t0 = start + kPagedItemCost, t1 = start + span;
+  const long long t0 = start + L::COST, t1 = start + span;
   const int c0 = (int)(t0 / quota), c1 = (int)((t1 - 1) / quota);
   if (c0 == c1) return;  // finished by the attention kernel
   const int h = g * G + r / p.Sq, i = r % p.Sq;

@@ -1,15 +1,31 @@
 // Drawing tokens from logits: temperature, top-k, top-p, min-p and a race of given
-// exponential random numbers, one CTA per row.
+// exponential random numbers.
 //
 // With the tokens ranked by (logit descending, index ascending) every filter keeps a
-// prefix of the ranking, so a row needs one threshold: the lowest ranked key kept.
-// It is found without sorting, by radix descent: 8 bits of the key per level, a
-// histogram of the counts (top-k) or of the weights (top-p) of the keys that share
-// the prefix so far, and the bin in which the wanted count or mass is reached.  The
-// key is 64 bits, the logit mapped to an ordered integer and the inverted index
-// below it, so equal logits are told apart by the same descent.
+// prefix of the ranking, so a row needs one threshold, and no sort of the vocabulary.
+// What must move is the logits, once (and the random numbers of the kept tokens); the
+// rest is latency.  A cluster of CTAs takes a row, each CTA a slice that it holds in
+// shared memory, so that the passes after the first read no memory:
+//
+//   maximum    of the slice, then of the row;
+//   top-k      (k <= kSampleMaxK) each CTA counts its slice in 2048 bins of the logit below its
+//              maximum, and sends the bins that hold its k largest to the first CTA,
+//              which sorts the few hundred that arrive and works on the sorted list;
+//   top-p      2048 bins of the weight's logarithm collect the weights; the tokens of
+//              the one bin in which the sum crosses top_p are compared one by one;
+//   the race   over the tokens at or above the threshold.
+//
+// Histograms use 32-bit shared-memory atomics alone: they run at the rate of plain
+// stores, 64-bit and float ones are loops of compare-and-swap (48 adds of 1024 threads:
+// 11 thousand cycles against 41 to 340 thousand).  Weights are 2^-31 fixed point in two
+// 16-bit halves there, so sums are exact integers and the order of atomics is irrelevant.
+// Rows that the bins do not separate (masses of equal logits, infinite ones, k above
+// kSampleMaxK, slices over 65536 tokens) take a radix descent in one CTA.
 #pragma once
 
+#include <cooperative_groups.h>
+
+#include "fwd.cuh"
 #include "sm100.cuh"
 
 namespace coalibi {
@@ -28,13 +44,20 @@ struct SampleParams {
   float temperature_all;
   int top_k_all;
   float top_p_all, min_p_all;
+  int cluster;       // CTAs per row
+  int slice_chunks;  // 16-byte chunks per CTA; 0: the slices stay in global memory
 };
 
-constexpr int kSampleThreads = 1024;
-// Weights are summed as integers of 2^-42: the sum of up to 2^21 of them (each at most
-// 1) fits 64 bits, integer addition makes the order of the atomics irrelevant, and
-// the resolution is below float32's for every weight above 2^-18 of the largest.
-constexpr float kWeightOne = 4398046511104.f;  // 2^42
+constexpr int kSampleThreads = 512;
+constexpr int kSampleMaxCluster = 8;
+constexpr int kSampleWarps = kSampleThreads / 32;
+constexpr int kSampleBins = 2048;
+constexpr int kSampleMaxK = 1024;
+constexpr int kSampleRegion = 1280;       // candidates a CTA may send: the k largest and their bin
+constexpr int kSampleTies = 1024;         // tokens of the crossing bin that are compared one by one
+constexpr int kSampleMaxSlice = 65536;    // 16-bit halves of the weights then sum within 32 bits
+constexpr float kSampleBinsPerLogit = 64.f;
+constexpr float kSampleBinsPerLog2 = 44.f;  // 2048 bins reach down to 2^-46, below half of 2^-31
 
 template <int DT>
 __device__ __forceinline__ float load_logit(const void* base, long long i) {
@@ -43,161 +66,642 @@ __device__ __forceinline__ float load_logit(const void* base, long long i) {
   return __half2float(static_cast<const __half*>(base)[i]);
 }
 
-// Logit -> integer of the same order; NaN ranks with -inf, -0 with +0.
+// NaN counts as -inf, -0 as +0.
+__device__ __forceinline__ float clean_logit(float x) { return x != x ? -INFINITY : x + 0.f; }
+
+// Integer of the same order as a clean logit, and back.
 __device__ __forceinline__ uint32_t order_key(float x) {
-  if (x != x) x = -INFINITY;
-  const uint32_t u = __float_as_uint(x + 0.f);
+  const uint32_t u = __float_as_uint(x);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+__device__ __forceinline__ float key_logit(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+// Rank of a token: larger is earlier.
+__device__ __forceinline__ unsigned long long rank_key(float x, int i) {
+  return ((unsigned long long)order_key(x) << 32) | (uint32_t)~i;
+}
 
-template <int DT>
-__global__ void __launch_bounds__(kSampleThreads) coalibi_sample_kernel(const SampleParams p) {
-  __shared__ unsigned int h_cnt[256];
-  __shared__ unsigned long long h_mass[256];
-  __shared__ float red_f[32];
-  __shared__ int red_i[32];
-  __shared__ unsigned long long red_u[32];
-  __shared__ unsigned long long s_prefix, s_acc;
-  __shared__ int s_done;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const char* lrow = static_cast<const char*>(p.logits) + (size_t)b * p.logits_stride * (DT == 2 ? 4 : 2);
-  const float* nrow = p.noise + (size_t)b * p.noise_stride;
-  const float t = p.temperature ? p.temperature[b] : p.temperature_all;
-  const float top_p = p.top_p ? p.top_p[b] : p.top_p_all;
-  const float min_p = p.min_p ? p.min_p[b] : p.min_p_all;
-  const int top_k = p.top_k ? p.top_k[b] : p.top_k_all;
-  const bool greedy = !(t > 0.f);
-  const float inv_t = greedy ? 0.f : 1.f / t;
+struct SampleShared {
+  unsigned int hist[2][kSampleBins];
+  unsigned int warp_u[kSampleWarps];
+  unsigned long long warp_ull[kSampleWarps];
+  float warp_f[kSampleWarps];
+  double warp_d[kSampleWarps];
+  int warp_i[kSampleWarps];
+  // results that all threads, or the other CTAs of the cluster, read
+  unsigned long long best_key;  // of this CTA's slice
+  unsigned long long floor_key, target, base;
+  unsigned int found_bin, found_count, n_list;
+  int overflow;
+  // in the first CTA, an entry from each
+  unsigned int sent[kSampleMaxCluster];
+  float score[kSampleMaxCluster];
+  int token[kSampleMaxCluster];
+  double rest[kSampleMaxCluster];
+};
 
-  // the first of the ranking: largest key, lowest index
-  unsigned long long best = 0;
-  for (int i = tid; i < p.V; i += kSampleThreads) {
-    const unsigned long long ck = ((unsigned long long)order_key(load_logit<DT>(lrow, i)) << 32) | (uint32_t)~i;
-    best = ck > best ? ck : best;
-  }
-  for (int o = 16; o; o >>= 1) {
-    const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
-    best = y > best ? y : best;
-  }
-  if (lane == 0) red_u[warp] = best;
+__device__ __forceinline__ unsigned long long block_max(unsigned long long v, SampleShared& s) {
+  // the high words' maximum, then the low words' among the threads that hold it
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto warp_max = [](unsigned long long x) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(x >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(x >> 32) == hi ? (uint32_t)x : 0u);
+    return ((unsigned long long)hi << 32) | lo;
+  };
+  v = warp_max(v);
+  if (lane == 0) s.warp_ull[warp] = v;
   __syncthreads();
-  for (int w = 0; w < 32; ++w) best = red_u[w] > best ? red_u[w] : best;
+  v = warp_max(lane < kSampleWarps ? s.warp_ull[lane] : 0ull);
   __syncthreads();
-  const int first = (int)~(uint32_t)best;
-  const float mx = load_logit<DT>(lrow, first);
-  if ((uint32_t)(best >> 32) == order_key(-INFINITY)) {
-    if (tid == 0) {
-      p.tokens[b] = -1;
-      p.logprobs[b] = -INFINITY;
-    }
-    return;
-  }
-  if (greedy) {
-    if (tid == 0) {
-      p.tokens[b] = first;
-      p.logprobs[b] = 0.f;
-    }
-    return;
-  }
-  auto dist = [&](float x) { return x == mx ? 0.f : (x != x ? -INFINITY : (x - mx) * inv_t); };
+  return v;
+}
 
-  // lowest key kept; the histogram descent below raises it
-  unsigned long long floor_key = ((unsigned long long)(order_key(-INFINITY) + 1)) << 32;
-  for (int filter = 0; filter < 2; ++filter) {
-    const bool by_mass = filter == 1;
-    if (by_mass ? top_p >= 1.f : (top_k <= 0 || top_k >= p.V)) continue;
-    unsigned long long target;
-    if (by_mass) {
-      unsigned long long s = 0;
-      for (int i = tid; i < p.V; i += kSampleThreads) {
-        const float x = load_logit<DT>(lrow, i);
-        const unsigned long long ck = ((unsigned long long)order_key(x) << 32) | (uint32_t)~i;
-        if (ck >= floor_key) s += (unsigned long long)(expf(dist(x)) * kWeightOne);
-      }
-      for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) red_u[warp] = s;
-      __syncthreads();
-      s = 0;
-      for (int w = 0; w < 32; ++w) s += red_u[w];
-      __syncthreads();
-      const double want = (double)fmaxf(top_p, 0.f) * (double)s;
-      target = want < 1.0 ? 1ull : (unsigned long long)ceil(want);
-    } else {
-      target = top_k;
-    }
-    if (tid == 0) {
-      s_prefix = 0;
-      s_acc = 0;
-      s_done = 0;
-    }
-    for (int shift = 56; shift >= 0; shift -= 8) {
-      if (tid < 256) {
-        h_cnt[tid] = 0;
-        h_mass[tid] = 0;
-      }
-      __syncthreads();
-      const unsigned long long prefix = s_prefix;
-      for (int i = tid; i < p.V; i += kSampleThreads) {
-        const float x = load_logit<DT>(lrow, i);
-        const unsigned long long ck = ((unsigned long long)order_key(x) << 32) | (uint32_t)~i;
-        if (ck < floor_key || (shift < 56 && (ck >> (shift + 8)) != (prefix >> (shift + 8)))) continue;
-        const int bin = (int)(ck >> shift) & 255;
-        atomicAdd(&h_cnt[bin], 1u);
-        if (by_mass) atomicAdd(&h_mass[bin], (unsigned long long)(expf(dist(x)) * kWeightOne));
-      }
-      __syncthreads();
-      if (tid == 0) {
-        unsigned long long acc = s_acc;
-        int bin = 255, last = -1;
-        for (; bin >= 0; --bin) {
-          if (h_cnt[bin] == 0) continue;
-          last = bin;
-          const unsigned long long v = by_mass ? h_mass[bin] : h_cnt[bin];
-          if (acc + v >= target) break;
-          acc += v;
-        }
-        if (bin < 0) bin = last, acc = 0, s_done = 2;  // fewer than the target: all stay
-        s_acc = acc;
-        s_prefix = prefix | ((unsigned long long)bin << shift);
-        if (s_done == 0 && (h_cnt[bin] == 1 || (!by_mass && acc + h_cnt[bin] == target))) s_done = 1;
-      }
-      __syncthreads();
-      if (s_done) break;
-    }
-    if (s_done != 2 && s_prefix > floor_key) floor_key = s_prefix;
-    __syncthreads();
+template <typename T>
+__device__ __forceinline__ T block_exclusive(T v, T* warp_sums, T& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  T inc = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const T y = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += y;
   }
+  if (lane == 31) warp_sums[warp] = inc;
+  __syncthreads();
+  T left = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kSampleWarps; ++w) {
+    const T y = warp_sums[w];
+    if (w < warp) left += y;
+    total += y;
+  }
+  __syncthreads();
+  return left + inc - v;
+}
 
-  // the race among the kept, and the sum of their weights without the first's (exactly 1)
-  float score = -1.f;
-  int token = first;
-  unsigned long long rest = 0;
-  for (int i = tid; i < p.V; i += kSampleThreads) {
-    const float x = load_logit<DT>(lrow, i);
-    const unsigned long long ck = ((unsigned long long)order_key(x) << 32) | (uint32_t)~i;
-    const float w = expf(dist(x));
-    if (ck < floor_key || w < min_p || w == 0.f) {
-      if (i != first) continue;
-    }
-    if (i != first) rest += (unsigned long long)(w * kWeightOne);
-    const float sc = w / nrow[i];
-    if (sc > score || (sc == score && i < token)) score = sc, token = i;
+// Weights and distances of a row.
+struct SampleScale {
+  float mx, inv_t, k2;
+  __device__ __forceinline__ float dist(float x) const { return x == mx ? 0.f : (x - mx) * inv_t; }
+  // of a finite maximum only; the float32 weight the passes over a slice use
+  __device__ __forceinline__ float log2w(float x) const { return (x - mx) * k2; }
+  __device__ __forceinline__ unsigned fixed(float l2) const { return __float2uint_rn(ex2_approx(l2) * 2147483648.f); }
+  __device__ __forceinline__ int bin(float l2) const {
+    return min(kSampleBins - 1, __float2int_rz(l2 * -kSampleBinsPerLog2));
   }
+};
+
+// The winner of the block's race and the weights beside the first token's, in thread 0.
+__device__ __forceinline__ void block_race(float& score, int& token, double& rest, SampleShared& s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
   for (int o = 16; o; o >>= 1) {
     const float ys = __shfl_xor_sync(0xffffffffu, score, o);
     const int yi = __shfl_xor_sync(0xffffffffu, token, o);
     if (ys > score || (ys == score && yi < token)) score = ys, token = yi;
     rest += __shfl_xor_sync(0xffffffffu, rest, o);
   }
-  if (lane == 0) red_f[warp] = score, red_i[warp] = token, red_u[warp] = rest;
+  if (lane == 0) s.warp_f[warp] = score, s.warp_i[warp] = token, s.warp_d[warp] = rest;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < 32; ++w) {
-      if (red_f[w] > score || (red_f[w] == score && red_i[w] < token)) score = red_f[w], token = red_i[w];
-      rest += red_u[w];
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kSampleWarps; ++w) {
+      if (s.warp_f[w] > score || (s.warp_f[w] == score && s.warp_i[w] < token)) score = s.warp_f[w], token = s.warp_i[w];
+      rest += s.warp_d[w];
     }
+  }
+}
+
+// The radix descent, by one CTA over the whole row: 8 bits of the rank key per level, a
+// histogram of the counts or of the weights (three parts of 11 bits: 2^21 of them fit 32
+// bits) of the keys that share the prefix, and the bin in which the target is reached.
+template <int DT>
+__device__ void sample_general(const SampleParams& p, SampleShared& s, int b, const void* lrow, const float* nrow,
+                               const SampleScale& sc, int first, int top_k, float top_p, float min_p) {
+  const int tid = threadIdx.x;
+  auto weight = [&](float x) { return expf(sc.dist(x)); };
+  auto fixed = [&](float x) { return (unsigned)__float2uint_rn(weight(x) * 2147483648.f); };
+  unsigned long long floor_key = ((unsigned long long)(order_key(-INFINITY) + 1)) << 32;
+  unsigned int* h = s.hist[0];  // [4][256]: counts, then the parts of the weights
+  for (int filter = 0; filter < 2; ++filter) {
+    const bool by_mass = filter == 1;
+    if (by_mass ? top_p >= 1.f : (top_k <= 0 || top_k >= p.V)) continue;
+    unsigned long long target = top_k;
+    if (by_mass) {
+      unsigned long long sum = 0, total;
+      for (int i = tid; i < p.V; i += kSampleThreads) {
+        const float x = clean_logit(load_logit<DT>(lrow, i));
+        if (rank_key(x, i) >= floor_key) sum += fixed(x);
+      }
+      block_exclusive(sum, s.warp_ull, total);
+      target = (unsigned long long)fmax(1.0, ceil((double)fmaxf(top_p, 0.f) * (double)total));
+    }
+    unsigned long long prefix = 0, acc = 0;
+    int done = 0;
+    for (int shift = 56; shift >= 0 && done == 0; shift -= 8) {
+      for (int i = tid; i < 1024; i += kSampleThreads) h[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < p.V; i += kSampleThreads) {
+        const float x = clean_logit(load_logit<DT>(lrow, i));
+        const unsigned long long ck = rank_key(x, i);
+        if (ck < floor_key || (shift < 56 && (ck >> (shift + 8)) != (prefix >> (shift + 8)))) continue;
+        const int bin = (int)(ck >> shift) & 255;
+        atomicAdd(&h[bin], 1u);
+        if (by_mass) {
+          const unsigned w = fixed(x);
+          atomicAdd(&h[256 + bin], w & 2047u);
+          atomicAdd(&h[512 + bin], w >> 11 & 2047u);
+          atomicAdd(&h[768 + bin], w >> 22);
+        }
+      }
+      __syncthreads();
+      if (tid == 0) {
+        int bin = 255, last = -1;
+        for (; bin >= 0; --bin) {
+          if (h[bin] == 0) continue;
+          last = bin;
+          const unsigned long long v =
+              by_mass ? h[256 + bin] + ((unsigned long long)h[512 + bin] << 11) + ((unsigned long long)h[768 + bin] << 22)
+                      : h[bin];
+          if (acc + v >= target) break;
+          acc += v;
+        }
+        s.overflow = 0;
+        if (bin < 0) s.overflow = 2, bin = last;  // fewer than the target: all stay
+        s.base = acc;
+        s.floor_key = prefix | ((unsigned long long)bin << shift);
+        if (s.overflow == 0 && (h[bin] == 1 || (!by_mass && acc + h[bin] == target))) s.overflow = 1;
+      }
+      __syncthreads();
+      done = s.overflow;
+      acc = s.base;
+      prefix = s.floor_key;
+      __syncthreads();
+    }
+    if (done != 2 && prefix > floor_key) floor_key = prefix;
+  }
+  float score = -1.f;
+  int token = first;
+  double rest = 0.0;
+  for (int i = tid; i < p.V; i += kSampleThreads) {
+    const float x = clean_logit(load_logit<DT>(lrow, i));
+    const float w = weight(x);
+    if (i != first) {
+      if (rank_key(x, i) < floor_key || w < min_p || w == 0.f) continue;
+      rest += (double)w;
+    }
+    const float y = w / nrow[i];
+    if (y > score || (y == score && i < token)) score = y, token = i;
+  }
+  block_race(score, token, rest, s);
+  if (tid == 0) {
     p.tokens[b] = token;
-    p.logprobs[b] = dist(load_logit<DT>(lrow, token)) - log1pf((float)((double)rest * (1.0 / (double)kWeightOne)));
+    p.logprobs[b] = sc.dist(clean_logit(load_logit<DT>(lrow, token))) - log1pf((float)rest);
+  }
+}
+
+// Top-k, in the first CTA: the candidates that the CTAs sent (rank keys, region r of the list
+// holds s.sent[r] of them) sorted as far as rank k, then the other filters and the race on
+// the sorted list.  `binned` and `sorted` are scratch.  Returns false if the bins do not
+// separate the candidates.
+__device__ bool sample_topk(const SampleParams& p, SampleShared& s, int b, const float* nrow, SampleScale sc,
+                            const unsigned long long* list, unsigned long long* binned, unsigned long long* sorted,
+                            int k, float top_p, float min_p) {
+  const int tid = threadIdx.x;
+  unsigned int* hist = s.hist[0];
+  unsigned int* off = s.hist[1];
+  constexpr int PER = kSampleBins / kSampleThreads;
+  unsigned long long best = 0;
+  for (int i = tid; i < kSampleBins; i += kSampleThreads) hist[i] = 0;
+  for (int r = 0; r < p.cluster; ++r)
+    for (int i = tid; i < (int)s.sent[r]; i += kSampleThreads) {
+      const unsigned long long key = list[r * kSampleRegion + i];
+      best = key > best ? key : best;
+    }
+  if (tid == 0) s.found_count = 0;
+  best = block_max(best, s);
+  if (best == 0) {  // nothing but -inf
+    if (tid == 0) p.tokens[b] = -1, p.logprobs[b] = -INFINITY;
+    return true;
+  }
+  sc.mx = key_logit((uint32_t)(best >> 32));
+  auto bin_of = [&](unsigned long long key) {
+    return min(kSampleBins - 1, __float2int_rz((sc.mx - key_logit((uint32_t)(key >> 32))) * kSampleBinsPerLogit));
+  };
+  for (int r = 0; r < p.cluster; ++r)
+    for (int i = tid; i < (int)s.sent[r]; i += kSampleThreads) atomicAdd(&hist[bin_of(list[r * kSampleRegion + i])], 1u);
+  __syncthreads();
+  unsigned v[PER], sum = 0, total;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) v[j] = hist[tid * PER + j], sum += v[j];
+  unsigned at = block_exclusive(sum, s.warp_u, total);
+  const int kk = min(k, (int)total);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    off[tid * PER + j] = at;
+    hist[tid * PER + j] = at;  // where the bin's next key goes
+    at += v[j];
+    if (v[j] > 0 && (int)(at - v[j]) < kk && (int)at >= kk) s.found_count = at;  // keys of the bins down to rank kk - 1
+  }
+  __syncthreads();
+  const int m = s.found_count;
+  if (m > 2 * kSampleMaxK) return false;
+  for (int r = 0; r < p.cluster; ++r)
+    for (int i = tid; i < (int)s.sent[r]; i += kSampleThreads) {
+      const unsigned long long key = list[r * kSampleRegion + i];
+      const int bin = bin_of(key);
+      if ((int)off[bin] < kk) binned[atomicAdd(&hist[bin], 1u)] = key;
+    }
+  __syncthreads();
+  for (int i = tid; i < m; i += kSampleThreads) {
+    const unsigned long long key = binned[i];
+    const int bin = bin_of(key), from = off[bin], to = hist[bin];
+    int place = from;
+    for (int j = from; j < to; ++j) place += binned[j] > key;
+    if (place < kk) sorted[place] = key;
+  }
+  __syncthreads();
+  // ranks 2 tid and 2 tid + 1
+  float w[2] = {0.f, 0.f};
+  int index[2] = {0, 0};
+  unsigned long long f[2] = {0, 0}, mass;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = 2 * tid + j;
+    if (r < kk) {
+      w[j] = expf(sc.dist(key_logit((uint32_t)(sorted[r] >> 32))));
+      index[j] = (int)~(uint32_t)sorted[r];
+      f[j] = __float2uint_rn(w[j] * 2147483648.f);
+    }
+  }
+  const unsigned long long before = block_exclusive(f[0] + f[1], s.warp_ull, mass);
+  const unsigned long long target =
+      top_p >= 1.f ? ~0ull : (unsigned long long)fmax(1.0, ceil((double)fmaxf(top_p, 0.f) * (double)mass));
+  float score = -1.f;
+  int token = 2 * tid < kk ? index[0] : 0x7fffffff;
+  double rest = 0.0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = 2 * tid + j;
+    if (r >= kk || before + (j ? f[0] : 0) >= target) continue;
+    if (r > 0) {
+      if (w[j] < min_p || w[j] == 0.f) continue;
+      rest += (double)w[j];
+    }
+    const float y = w[j] / nrow[index[j]];
+    if (y > score || (y == score && index[j] < token)) score = y, token = index[j];
+  }
+  block_race(score, token, rest, s);
+  if (tid == 0) {
+    if (score < 0.f) token = (int)~(uint32_t)best;  // no number won: the first of the ranking
+    s.token[0] = token;
+    s.rest[0] = rest;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = 2 * tid + j;
+    if (r < kk && index[j] == s.token[0]) {
+      p.tokens[b] = index[j];
+      p.logprobs[b] = sc.dist(key_logit((uint32_t)(sorted[r] >> 32))) - log1pf((float)s.rest[0]);
+    }
+  }
+  return true;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kSampleThreads) coalibi_sample_kernel(const SampleParams p) {
+  namespace cg = cooperative_groups;
+  constexpr int SIZE = DT == 2 ? 4 : 2, EPC = 16 / SIZE;  // elements per 16-byte chunk
+  __shared__ SampleShared s;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  // [cluster][kSampleRegion] candidates (or the row's bin masses), then the slice
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(smem_raw);
+  uint4* data = reinterpret_cast<uint4*>(smem_raw + (size_t)p.cluster * kSampleRegion * 8);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = p.cluster, rank = C > 1 ? (int)cluster.block_rank() : 0, b = blockIdx.x / C;
+  const int tid = threadIdx.x;
+  SampleShared& s0 = C > 1 ? *cluster.map_shared_rank(&s, 0) : s;  // the first CTA's
+  unsigned long long* list0 = C > 1 ? cluster.map_shared_rank(list, 0) : list;
+  auto meet = [&]() {
+    if (C > 1)
+      cluster.sync();
+    else
+      __syncthreads();
+  };
+  const char* lrow = static_cast<const char*>(p.logits) + (size_t)b * p.logits_stride * SIZE;
+  const float* nrow = p.noise + (size_t)b * p.noise_stride;
+  const float t = p.temperature ? p.temperature[b] : p.temperature_all;
+  const float top_p = p.top_p ? p.top_p[b] : p.top_p_all;
+  const float min_p = p.min_p ? p.min_p[b] : p.min_p_all;
+  const int top_k = p.top_k ? p.top_k[b] : p.top_k_all;
+  const bool greedy = !(t > 0.f), by_k = top_k > 0 && top_k < p.V;
+  SampleScale sc;
+  sc.inv_t = greedy ? 0.f : 1.f / t;
+  sc.k2 = sc.inv_t * kLog2e;
+
+  for (int i = tid; i < kSampleBins; i += kSampleThreads) s.hist[0][i] = s.hist[1][i] = 0;
+  if (tid == 0) s.n_list = 0, s.overflow = 0, s.found_bin = kSampleBins - 1, s.found_count = 0;
+
+  // ---- the slice: chunks [c0, c1) of the 16-byte chunks that the row touches.  Elements of a
+  // chunk outside the row, and NaN, become -inf.
+  const int skip = (int)(reinterpret_cast<uintptr_t>(lrow) & 15) / SIZE;
+  const char* base = lrow - (size_t)skip * SIZE;
+  const int chunks = (p.V + skip + EPC - 1) / EPC, per = (chunks + C - 1) / C;
+  const int c0 = min(rank * per, chunks), c1 = min(c0 + per, chunks);
+  const bool cached = p.slice_chunks > 0;
+  auto unpack = [](uint4 u, float* x) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (DT == 2) {
+        x[j] = __uint_as_float(w[j]);
+      } else {
+        const float2 f = unpack2<DT == 1>(w[j]);
+        x[2 * j % EPC] = f.x;
+        x[(2 * j + 1) % EPC] = f.y;
+      }
+    }
+  };
+  auto fetch = [&](int c) {
+    const int i0 = c * EPC - skip;
+    if (i0 >= 0 && i0 + EPC <= p.V) return *reinterpret_cast<const uint4*>(base + (size_t)c * 16);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (DT == 2) {
+        w[j] = i0 + j >= 0 && i0 + j < p.V ? reinterpret_cast<const uint32_t*>(lrow)[i0 + j] : 0xff800000u;
+      } else {
+        const uint32_t none = DT == 1 ? 0xff80u : 0xfc00u;
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(lrow);
+        const int a = i0 + 2 * j;
+        const uint32_t lo = a >= 0 && a < p.V ? h[a] : none, hi = a + 1 >= 0 && a + 1 < p.V ? h[a + 1] : none;
+        w[j] = lo | hi << 16;
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  // calls f(first index, EPC clean logits) for the chunks of this thread
+  auto each = [&](auto&& f) {
+    for (int c = c0 + tid; c < c1; c += kSampleThreads) {
+      float x[EPC];
+      unpack(cached ? data[c - c0] : fetch(c), x);
+#pragma unroll
+      for (int e = 0; e < EPC; ++e) x[e] = clean_logit(x[e]);
+      f(c * EPC - skip, x);
+    }
+  };
+  float mx = -INFINITY;
+  int arg = 0x7fffffff;
+#pragma unroll 4
+  for (int c = c0 + tid; c < c1; c += kSampleThreads) {
+    const uint4 u = fetch(c);
+    if (cached) data[c - c0] = u;
+    float x[EPC];
+    unpack(u, x);
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) {
+      const float y = clean_logit(x[e]);
+      if (y > mx) mx = y, arg = c * EPC - skip + e;  // a thread's indices grow: the first of equals
+    }
+  }
+  const unsigned long long mine = block_max(mx > -INFINITY ? rank_key(mx, arg) : 0ull, s);
+  sc.mx = mine != 0 ? key_logit((uint32_t)(mine >> 32)) : -INFINITY;
+  if (tid == 0) s.best_key = mine;
+  meet();  // (and every CTA of the cluster has started)
+
+  if (by_k && !greedy && top_k <= kSampleMaxK) {
+    // ---- top-k: this slice's k largest, and what shares the last one's bin, go to the first CTA
+    if (mine != 0 && sc.mx < INFINITY) {
+      each([&](int, const float* x) {
+#pragma unroll
+        for (int e = 0; e < EPC; ++e)
+          if (x[e] > -INFINITY)
+            atomicAdd(&s.hist[0][min(kSampleBins - 1, __float2int_rz((sc.mx - x[e]) * kSampleBinsPerLogit))], 1u);
+      });
+      __syncthreads();
+      constexpr int PER = kSampleBins / kSampleThreads;
+      unsigned v[PER], sum = 0, total;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) v[j] = s.hist[0][tid * PER + j], sum += v[j];
+      unsigned at = block_exclusive(sum, s.warp_u, total);
+      const unsigned want = min((unsigned)top_k, total);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        if (at < want && at + v[j] >= want) s.found_bin = tid * PER + j, s.found_count = at + v[j];
+        at += v[j];
+      }
+      __syncthreads();
+      const int last = s.found_bin;
+      if (s.found_count <= kSampleRegion) {
+        each([&](int i0, const float* x) {
+#pragma unroll
+          for (int e = 0; e < EPC; ++e)
+            if (x[e] > -INFINITY && min(kSampleBins - 1, __float2int_rz((sc.mx - x[e]) * kSampleBinsPerLogit)) <= last)
+              list0[rank * kSampleRegion + atomicAdd(&s.n_list, 1u)] = rank_key(x[e], i0 + e);
+        });
+      }
+    }
+    if (tid == 0) {
+      s0.sent[rank] = s.found_count <= kSampleRegion ? s.found_count : 0u;
+      if (s.found_count > kSampleRegion || sc.mx == INFINITY) s0.overflow = 1;
+    }
+    meet();
+    if (rank != 0) return;
+    if (s.overflow == 0 &&
+        sample_topk(p, s, b, nrow, sc, list, reinterpret_cast<unsigned long long*>(data),
+                    reinterpret_cast<unsigned long long*>(data) + 2 * kSampleMaxK, top_k, top_p, min_p))
+      return;
+    __syncthreads();
+    if (tid == 0) s.best_key = 0;
+    unsigned long long best = 0;
+    for (int i = tid; i < p.V; i += kSampleThreads) {
+      const unsigned long long key = rank_key(clean_logit(load_logit<DT>(lrow, i)), i);
+      best = key > best ? key : best;
+    }
+    best = block_max(best, s);
+    sc.mx = key_logit((uint32_t)(best >> 32));
+    sample_general<DT>(p, s, b, lrow, nrow, sc, (int)~(uint32_t)best, top_k, top_p, min_p);
+    return;
+  }
+
+  unsigned long long best = mine;
+  for (int r = 0; r < C && C > 1; ++r) {
+    const unsigned long long y = cluster.map_shared_rank(&s, r)->best_key;
+    best = y > best ? y : best;
+  }
+  const int first = (int)~(uint32_t)best;
+  sc.mx = best != 0 ? key_logit((uint32_t)(best >> 32)) : -INFINITY;
+  const bool general = by_k || sc.mx == INFINITY || (top_p < 1.f && per * EPC > kSampleMaxSlice);
+  if (best == 0 || greedy || general) {
+    meet();  // the others have read this CTA's best_key
+    if (rank != 0) return;
+    if (best == 0 || greedy) {
+      if (tid == 0) p.tokens[b] = best == 0 ? -1 : first, p.logprobs[b] = best == 0 ? -INFINITY : 0.f;
+    } else {
+      sample_general<DT>(p, s, b, lrow, nrow, sc, first, top_k, top_p, min_p);
+    }
+    return;
+  }
+
+  unsigned long long floor_key = 1;  // of nothing but -inf
+  if (top_p < 1.f) {
+    // ---- top-p: bins of the weights' logarithm
+    each([&](int, const float* x) {
+#pragma unroll
+      for (int e = 0; e < EPC; ++e) {
+        const float l2 = sc.log2w(x[e]);
+        const unsigned w = sc.fixed(l2);
+        if (w == 0) continue;
+        const int bin = sc.bin(l2);
+        atomicAdd(&s.hist[0][bin], w & 0xffffu);
+        if (w >> 16) atomicAdd(&s.hist[1][bin], w >> 16);
+      }
+    });
+    meet();
+    constexpr int PER = kSampleBins / kSampleThreads;
+    if (C > 1) {  // a stripe of the bins each, summed over the cluster
+      for (int i = rank * kSampleThreads + tid; i < kSampleBins; i += C * kSampleThreads) {
+        unsigned long long sum = 0;
+        for (int r = 0; r < C; ++r) {
+          const SampleShared* o = cluster.map_shared_rank(&s, r);
+          sum += o->hist[0][i] + ((unsigned long long)o->hist[1][i] << 16);
+        }
+        list0[i] = sum;
+      }
+      meet();
+    }
+    if (rank == 0) {
+      unsigned long long v[PER], sum = 0, total;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int i = tid * PER + j;
+        v[j] = C > 1 ? list[i] : s.hist[0][i] + ((unsigned long long)s.hist[1][i] << 16);
+        sum += v[j];
+      }
+      unsigned long long at = block_exclusive(sum, s.warp_ull, total);
+      const unsigned long long target = (unsigned long long)fmax(1.0, ceil((double)fmaxf(top_p, 0.f) * (double)total));
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        if (at < target && at + v[j] >= target) s.found_bin = tid * PER + j, s.base = at, s.target = target;
+        at += v[j];
+      }
+    }
+    meet();
+    const int cross = s0.found_bin;
+    // ---- the tokens of the bin in which the sum crosses the target, one by one
+    each([&](int i0, const float* x) {
+#pragma unroll
+      for (int e = 0; e < EPC; ++e)
+        if (x[e] > -INFINITY && sc.bin(sc.log2w(x[e])) == cross) {
+          const unsigned at = atomicAdd(&s0.n_list, 1u);
+          if (at < kSampleTies) list0[at] = rank_key(x[e], i0 + e);
+        }
+    });
+    meet();
+    if (rank == 0) {
+      const int n = s.n_list;
+      unsigned long long low = ~0ull;
+      if (n <= kSampleTies) {
+        unsigned* weight = s.hist[0];
+        for (int i = tid; i < n; i += kSampleThreads) weight[i] = sc.fixed(sc.log2w(key_logit((uint32_t)(list[i] >> 32))));
+        __syncthreads();
+        for (int i = tid; i < n; i += kSampleThreads) {
+          unsigned long long before = s.base;
+          const unsigned long long key = list[i];
+          for (int j = 0; j < n; ++j) before += list[j] > key ? weight[j] : 0u;
+          if (before < s.target) low = key < low ? key : low;
+        }
+      }
+      low = ~block_max(~low, s);
+      if (tid == 0) s.floor_key = low, s.overflow = n > kSampleTies;
+    }
+    meet();
+    floor_key = s0.floor_key;
+    const bool lost = s0.overflow != 0;
+    if (lost) {
+      meet();  // all have read it
+      if (rank == 0) sample_general<DT>(p, s, b, lrow, nrow, sc, first, top_k, top_p, min_p);
+      return;
+    }
+  }
+
+  // ---- the race.  Only a token whose quick weight comes within 1e-4 of beating the best so
+  // far (its error is below 2e-5) gets an exact weight and division.
+  const float floor_x = key_logit((uint32_t)(floor_key >> 32));
+  const int floor_i = (int)~(uint32_t)floor_key;
+  const bool whole = floor_key == 1;
+  float score = -1.f;
+  int token = 0x7fffffff;
+  double rest = 0.0;
+  auto enter = [&](int i, float x, float w, float e) {
+    if (w * 1.0001f >= score * e) {
+      const float y = expf(sc.dist(x)) / e;
+      if (y > score || (y == score && i < token)) score = y, token = i;
+    }
+  };
+  if (whole && min_p <= 0.f) {
+    // every token: the random numbers stream in beside the logits
+    const bool wide = (reinterpret_cast<uintptr_t>(nrow - skip) & 15) == 0;
+    constexpr int AHEAD = 16 / EPC;  // chunks whose numbers are in flight
+    for (int c = c0 + tid; c < c1; c += AHEAD * kSampleThreads) {
+      float e[AHEAD][EPC];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const int cc = c + a * kSampleThreads, i0 = cc * EPC - skip;
+        if (cc < c1 && wide && i0 >= 0 && i0 + EPC <= p.V) {
+#pragma unroll
+          for (int q = 0; q < EPC / 4; ++q)
+            *reinterpret_cast<float4*>(&e[a][4 * q]) = *reinterpret_cast<const float4*>(nrow + i0 + 4 * q);
+        } else {
+#pragma unroll
+          for (int q = 0; q < EPC; ++q) e[a][q] = cc < c1 && i0 + q >= 0 && i0 + q < p.V ? nrow[i0 + q] : 1.f;
+        }
+      }
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const int cc = c + a * kSampleThreads, i0 = cc * EPC - skip;
+        if (cc >= c1) break;
+        float x[EPC], sum = 0.f;
+        unpack(cached ? data[cc - c0] : fetch(cc), x);
+#pragma unroll
+        for (int q = 0; q < EPC; ++q) {
+          x[q] = clean_logit(x[q]);
+          const float w = ex2_approx(sc.log2w(x[q]));
+          if (i0 + q != first) sum += w;
+          if (x[q] > -INFINITY) enter(i0 + q, x[q], w, e[a][q]);
+        }
+        rest += (double)sum;
+      }
+    }
+  } else {
+    each([&](int i0, const float* x) {
+      float sum = 0.f;
+#pragma unroll
+      for (int q = 0; q < EPC; ++q) {
+        const int i = i0 + q;
+        const float w = ex2_approx(sc.log2w(x[q]));
+        if (i != first) {
+          if (!(x[q] > -INFINITY) || w < min_p || w == 0.f) continue;
+          if (!whole && (x[q] < floor_x || (x[q] == floor_x && i > floor_i))) continue;
+          sum += w;
+        }
+        enter(i, x[q], w, nrow[i]);
+      }
+      rest += (double)sum;
+    });
+  }
+  block_race(score, token, rest, s);
+  if (tid == 0) s0.score[rank] = score, s0.token[rank] = token, s0.rest[rank] = rest;
+  meet();
+  if (rank == 0 && tid == 0) {
+    for (int r = 1; r < C; ++r) {
+      if (s.score[r] > score || (s.score[r] == score && s.token[r] < token)) score = s.score[r], token = s.token[r];
+      rest += s.rest[r];
+    }
+    if (score < 0.f) token = first;  // no number won
+    p.tokens[b] = token;
+    p.logprobs[b] = sc.dist(clean_logit(load_logit<DT>(lrow, token))) - log1pf((float)rest);
   }
 }
 

@@ -143,7 +143,7 @@ int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& 
   p.row_blocks = (rows + L::ROWS - 1) / L::ROWS;
   p.n_ctas = (sms < kPagedMaxSms ? sms : kPagedMaxSms) * L::CTAS;
   const long long most = ((long long)p.max_pages * p.page_size + L::UNIT - 1) / L::UNIT;
-  const long long bound = (most + kPagedItemCost) * p.B * p.Hkv * p.row_blocks;  // if every table row were full
+  const long long bound = (most + L::COST) * p.B * p.Hkv * p.row_blocks;  // if every table row were full
   if (bound > 0x7fffffffLL) return COALIBI_ERR_SHAPE;
   if (bound < p.n_ctas) p.n_ctas = (int)bound;
   if (e == cudaSuccess)
@@ -241,10 +241,58 @@ extern "C" int coalibi_paged_attention(const CoalibiPagedAttentionArgs* a, void*
   return bf16 ? launch_paged_rows<64, true>(tk, tv, p, sms, s) : launch_paged_rows<64, false>(tk, tv, p, sms, s);
 }
 
+namespace coalibi {
+namespace {
+
+template <int DT>
+int launch_sample(SampleParams& p, cudaStream_t s) {
+  constexpr int kSize = DT == 2 ? 4 : 2, kChunk = 16 / kSize;
+  constexpr int kMostBytes = 200 << 10, kRowBytes = 64 << 10;
+  const int sms = device_sm_count();
+  const long long chunks = (p.V + kChunk - 2) / kChunk + 1;  // of a row at any alignment, at most
+  // CTAs per row: enough for slices of about 64 KB, and more while the SMs outnumber them
+  int c = 1;
+  while (c < kSampleMaxCluster && (chunks * 16 > (long long)c * kRowBytes || (long long)p.B * c * 2 <= sms) &&
+         chunks >= 256LL * c)
+    c *= 2;
+  p.cluster = c;
+  const long long per = (chunks + c - 1) / c;
+  const size_t list = (size_t)c * kSampleRegion * 8, scratch = 3 * kSampleMaxK * 8;
+  size_t slice = (size_t)per * 16;
+  p.slice_chunks = slice + list <= kMostBytes ? (int)per : 0;
+  if (p.slice_chunks == 0) slice = 0;
+  const size_t bytes = list + (slice > scratch ? slice : scratch);
+  cudaError_t e = cudaSuccess;
+  static std::atomic<unsigned long long> ready{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    e = cudaFuncSetAttribute(coalibi_sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes + 4096);
+    if (e == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.B * c));
+  cfg.blockDim = dim3(kSampleThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = c;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, coalibi_sample_kernel<DT>, static_cast<const SampleParams&>(p));
+  if (e != cudaSuccess) set_last_error_detail(cudaGetErrorString(e));
+  return e == cudaSuccess ? COALIBI_OK : COALIBI_ERR_LAUNCH;
+}
+
+}  // namespace
+}  // namespace coalibi
+
 extern "C" int coalibi_sample(const CoalibiSampleArgs* a, void* stream) {
   if (a == nullptr || !a->logits || !a->noise || !a->tokens || !a->logprobs) return COALIBI_ERR_NULL_POINTER;
   if (a->dtype != COALIBI_F16 && a->dtype != COALIBI_BF16 && a->dtype != COALIBI_F32) return COALIBI_ERR_DTYPE;
-  if (a->B <= 0 || a->V <= 0 || a->V > COALIBI_SAMPLE_MAX_VOCAB || a->logits_stride < 0 || a->noise_stride < 0)
+  if (a->B <= 0 || a->B > 0x7fffffff / kSampleMaxCluster || a->V <= 0 || a->V > COALIBI_SAMPLE_MAX_VOCAB || a->logits_stride < 0 || a->noise_stride < 0)
     return COALIBI_ERR_SHAPE;
   if (!aligned(a->logits, a->dtype == COALIBI_F32 ? 4 : 2) || !aligned(a->noise, 4) || !aligned(a->tokens, 8) ||
       !aligned(a->logprobs, 4))
@@ -269,11 +317,8 @@ extern "C" int coalibi_sample(const CoalibiSampleArgs* a, void* stream) {
   p.top_p_all = a->top_p_all;
   p.min_p_all = a->min_p_all;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a->dtype == COALIBI_F32)
-    coalibi_sample_kernel<2><<<a->B, kSampleThreads, 0, s>>>(p);
-  else if (a->dtype == COALIBI_BF16)
-    coalibi_sample_kernel<1><<<a->B, kSampleThreads, 0, s>>>(p);
-  else
-    coalibi_sample_kernel<0><<<a->B, kSampleThreads, 0, s>>>(p);
-  return launched("sampling launch");
+  const int rc = a->dtype == COALIBI_F32    ? launch_sample<2>(p, s)
+                 : a->dtype == COALIBI_BF16 ? launch_sample<1>(p, s)
+                                            : launch_sample<0>(p, s);
+  return rc ? rc : launched("sampling launch");
 }
