@@ -8,12 +8,12 @@
 // shared memory, so that the passes after the first read no memory:
 //
 //   maximum    of the slice, then of the row;
-//   top-k      (k <= kSampleMaxK) each CTA counts its slice in 2048 bins of the logit below its
-//              maximum, and sends the bins that hold its k largest to the first CTA,
-//              which sorts the few hundred that arrive and works on the sorted list;
-//   top-p      2048 bins of the weight's logarithm collect the weights; the tokens of
-//              the one bin in which the sum crosses top_p are compared one by one;
-//   the race   over the tokens at or above the threshold.
+//   top-k      (k <= kSampleMaxK) each CTA lists what can be among its k largest: what is not
+//              below the k-th largest of its threads' maxima, or the bins of a histogram
+//              down to rank k; the first CTA sorts the few hundred listed and works on those;
+//   top-p      2048 bins of the weight's logarithm collect the weights; tokens above the bin
+//              in which their sum crosses top_p race at once, its own are compared one by one;
+//   the race   largest w / noise.
 //
 // Histograms use 32-bit shared-memory atomics alone: they run at the rate of plain
 // stores, 64-bit and float ones are loops of compare-and-swap (48 adds of 1024 threads:
@@ -46,6 +46,7 @@ struct SampleParams {
   float top_p_all, min_p_all;
   int cluster;       // CTAs per row
   int slice_chunks;  // 16-byte chunks per CTA; 0: the slices stay in global memory
+  int filters;       // whether any row may ask for top-k or top-p
 };
 
 constexpr int kSampleThreads = 512;
@@ -53,7 +54,8 @@ constexpr int kSampleMaxCluster = 8;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 2048;
 constexpr int kSampleMaxK = 1024;
-constexpr int kSampleRegion = 1280;       // candidates a CTA may send: the k largest and their bin
+constexpr int kSampleListed = 2048;       // tokens a CTA may list
+constexpr int kSampleQuickK = 384;        // of 512 threads: the bound by their maxima stays tight
 constexpr int kSampleTies = 1024;         // tokens of the crossing bin that are compared one by one
 constexpr int kSampleMaxSlice = 65536;    // 16-bit halves of the weights then sum within 32 bits
 constexpr float kSampleBinsPerLogit = 64.f;
@@ -69,6 +71,29 @@ __device__ __forceinline__ float load_logit(const void* base, long long i) {
 // NaN counts as -inf, -0 as +0.
 __device__ __forceinline__ float clean_logit(float x) { return x != x ? -INFINITY : x + 0.f; }
 
+// The same for a 32-bit word of logits, and the larger of two clean words' elements.
+template <int DT>
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
+  if (DT == 2) return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  uint32_t r;
+  if (DT == 1)
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t clean_word(uint32_t a) {
+  if (DT == 2) return __float_as_uint(fmaxf(__uint_as_float(a), -INFINITY) + 0.f);
+  a = max_word<DT>(a, DT == 1 ? 0xff80ff80u : 0xfc00fc00u);  // the operand that is a number
+  if (DT == 1) {
+    const __nv_bfloat162 y = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&a), __floats2bfloat162_rn(0.f, 0.f));
+    return *reinterpret_cast<const uint32_t*>(&y);
+  }
+  const __half2 y = __hadd2(*reinterpret_cast<__half2*>(&a), __floats2half2_rn(0.f, 0.f));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
 // Integer of the same order as a clean logit, and back.
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(x);
@@ -83,7 +108,7 @@ __device__ __forceinline__ unsigned long long rank_key(float x, int i) {
 }
 
 struct SampleShared {
-  unsigned int hist[2][kSampleBins];
+  unsigned int* hist;  // [2][kSampleBins], dynamic shared memory
   unsigned int warp_u[kSampleWarps];
   unsigned long long warp_ull[kSampleWarps];
   float warp_f[kSampleWarps];
@@ -93,9 +118,9 @@ struct SampleShared {
   unsigned long long best_key;  // of this CTA's slice
   unsigned long long floor_key, target, base;
   unsigned int found_bin, found_count, n_list;
-  int overflow;
+  int first, overflow;
   // in the first CTA, an entry from each
-  unsigned int sent[kSampleMaxCluster];
+  unsigned int sent[kSampleMaxCluster];  // listed tokens; ~0: more than fit, or +inf among them
   float score[kSampleMaxCluster];
   int token[kSampleMaxCluster];
   double rest[kSampleMaxCluster];
@@ -113,6 +138,16 @@ __device__ __forceinline__ unsigned long long block_max(unsigned long long v, Sa
   if (lane == 0) s.warp_ull[warp] = v;
   __syncthreads();
   v = warp_max(lane < kSampleWarps ? s.warp_ull[lane] : 0ull);
+  __syncthreads();
+  return v;
+}
+
+__device__ __forceinline__ uint32_t block_max(uint32_t v, SampleShared& s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = __reduce_max_sync(0xffffffffu, v);
+  if (lane == 0) s.warp_u[warp] = v;
+  __syncthreads();
+  v = __reduce_max_sync(0xffffffffu, lane < kSampleWarps ? s.warp_u[lane] : 0u);
   __syncthreads();
   return v;
 }
@@ -147,9 +182,6 @@ struct SampleScale {
   // of a finite maximum only; the float32 weight the passes over a slice use
   __device__ __forceinline__ float log2w(float x) const { return (x - mx) * k2; }
   __device__ __forceinline__ unsigned fixed(float l2) const { return __float2uint_rn(ex2_approx(l2) * 2147483648.f); }
-  __device__ __forceinline__ int bin(float l2) const {
-    return min(kSampleBins - 1, __float2int_rz(l2 * -kSampleBinsPerLog2));
-  }
 };
 
 // The winner of the block's race and the weights beside the first token's, in thread 0.
@@ -182,7 +214,7 @@ __device__ void sample_general(const SampleParams& p, SampleShared& s, int b, co
   auto weight = [&](float x) { return expf(sc.dist(x)); };
   auto fixed = [&](float x) { return (unsigned)__float2uint_rn(weight(x) * 2147483648.f); };
   unsigned long long floor_key = ((unsigned long long)(order_key(-INFINITY) + 1)) << 32;
-  unsigned int* h = s.hist[0];  // [4][256]: counts, then the parts of the weights
+  unsigned int* h = s.hist;  // [4][256]: counts, then the parts of the weights
   for (int filter = 0; filter < 2; ++filter) {
     const bool by_mass = filter == 1;
     if (by_mass ? top_p >= 1.f : (top_k <= 0 || top_k >= p.V)) continue;
@@ -260,27 +292,28 @@ __device__ void sample_general(const SampleParams& p, SampleShared& s, int b, co
   }
 }
 
-// Top-k, in the first CTA: the candidates that the CTAs sent (rank keys, region r of the list
-// holds s.sent[r] of them) sorted as far as rank k, then the other filters and the race on
-// the sorted list.  `binned` and `sorted` are scratch.  Returns false if the bins do not
-// separate the candidates.
-__device__ bool sample_topk(const SampleParams& p, SampleShared& s, int b, const float* nrow, SampleScale sc,
-                            const unsigned long long* list, unsigned long long* binned, unsigned long long* sorted,
-                            int k, float top_p, float min_p) {
+// Top-k, in the first CTA: the n listed tokens of the cluster (rank keys, key_at(i)) sorted
+// as far as rank k, then the other filters and the race on the sorted list.  `binned` and
+// `sorted` are scratch; done_reading() follows the last key_at.  Returns false if the bins
+// do not separate the tokens.
+template <typename KeyAt, typename Done>
+__device__ bool sample_topk(const SampleParams& p, SampleShared& s, int b, const float* nrow, SampleScale sc, int n,
+                            KeyAt&& key_at, Done&& done_reading, unsigned long long* binned,
+                            unsigned long long* sorted, int k, float top_p, float min_p) {
   const int tid = threadIdx.x;
-  unsigned int* hist = s.hist[0];
-  unsigned int* off = s.hist[1];
+  unsigned int* hist = s.hist;
+  unsigned int* off = s.hist + kSampleBins;
   constexpr int PER = kSampleBins / kSampleThreads;
   unsigned long long best = 0;
   for (int i = tid; i < kSampleBins; i += kSampleThreads) hist[i] = 0;
-  for (int r = 0; r < p.cluster; ++r)
-    for (int i = tid; i < (int)s.sent[r]; i += kSampleThreads) {
-      const unsigned long long key = list[r * kSampleRegion + i];
-      best = key > best ? key : best;
-    }
+  for (int i = tid; i < n; i += kSampleThreads) {
+    const unsigned long long key = key_at(i);
+    best = key > best ? key : best;
+  }
   if (tid == 0) s.found_count = 0;
   best = block_max(best, s);
   if (best == 0) {  // nothing but -inf
+    done_reading();
     if (tid == 0) p.tokens[b] = -1, p.logprobs[b] = -INFINITY;
     return true;
   }
@@ -288,8 +321,7 @@ __device__ bool sample_topk(const SampleParams& p, SampleShared& s, int b, const
   auto bin_of = [&](unsigned long long key) {
     return min(kSampleBins - 1, __float2int_rz((sc.mx - key_logit((uint32_t)(key >> 32))) * kSampleBinsPerLogit));
   };
-  for (int r = 0; r < p.cluster; ++r)
-    for (int i = tid; i < (int)s.sent[r]; i += kSampleThreads) atomicAdd(&hist[bin_of(list[r * kSampleRegion + i])], 1u);
+  for (int i = tid; i < n; i += kSampleThreads) atomicAdd(&hist[bin_of(key_at(i))], 1u);
   __syncthreads();
   unsigned v[PER], sum = 0, total;
 #pragma unroll
@@ -305,14 +337,16 @@ __device__ bool sample_topk(const SampleParams& p, SampleShared& s, int b, const
   }
   __syncthreads();
   const int m = s.found_count;
-  if (m > 2 * kSampleMaxK) return false;
-  for (int r = 0; r < p.cluster; ++r)
-    for (int i = tid; i < (int)s.sent[r]; i += kSampleThreads) {
-      const unsigned long long key = list[r * kSampleRegion + i];
-      const int bin = bin_of(key);
-      if ((int)off[bin] < kk) binned[atomicAdd(&hist[bin], 1u)] = key;
-    }
-  __syncthreads();
+  if (m > 2 * kSampleMaxK) {
+    done_reading();
+    return false;
+  }
+  for (int i = tid; i < n; i += kSampleThreads) {
+    const unsigned long long key = key_at(i);
+    const int bin = bin_of(key);
+    if ((int)off[bin] < kk) binned[atomicAdd(&hist[bin], 1u)] = key;
+  }
+  done_reading();  // (a barrier)
   for (int i = tid; i < m; i += kSampleThreads) {
     const unsigned long long key = binned[i];
     const int bin = bin_of(key), from = off[bin], to = hist[bin];
@@ -370,14 +404,17 @@ __device__ bool sample_topk(const SampleParams& p, SampleShared& s, int b, const
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kSampleThreads) coalibi_sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const SampleParams p) {
   namespace cg = cooperative_groups;
   constexpr int SIZE = DT == 2 ? 4 : 2, EPC = 16 / SIZE;  // elements per 16-byte chunk
+  constexpr int PER = kSampleBins / kSampleThreads;
   __shared__ SampleShared s;
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  // [cluster][kSampleRegion] candidates (or the row's bin masses), then the slice
-  unsigned long long* list = reinterpret_cast<unsigned long long*>(smem_raw);
-  uint4* data = reinterpret_cast<uint4*>(smem_raw + (size_t)p.cluster * kSampleRegion * 8);
+  // histograms, listed tokens (or the row's bin masses), the slice; without filters the
+  // first are 4 KB for the descent and there is no list
+  unsigned int* hist = reinterpret_cast<unsigned int*>(smem_raw);
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(smem_raw + 8 * kSampleBins);
+  uint4* data = reinterpret_cast<uint4*>(smem_raw + (p.filters ? 8 * kSampleBins + 8 * kSampleListed : 4096));
   cg::cluster_group cluster = cg::this_cluster();
   const int C = p.cluster, rank = C > 1 ? (int)cluster.block_rank() : 0, b = blockIdx.x / C;
   const int tid = threadIdx.x;
@@ -400,16 +437,49 @@ __global__ void __launch_bounds__(kSampleThreads) coalibi_sample_kernel(const Sa
   sc.inv_t = greedy ? 0.f : 1.f / t;
   sc.k2 = sc.inv_t * kLog2e;
 
-  for (int i = tid; i < kSampleBins; i += kSampleThreads) s.hist[0][i] = s.hist[1][i] = 0;
-  if (tid == 0) s.n_list = 0, s.overflow = 0, s.found_bin = kSampleBins - 1, s.found_count = 0;
+  if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  // before the first access to another CTA's memory: all of the cluster have started
+  auto started = [&]() {
+    if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  };
+  if (p.filters)
+    for (int i = tid; i < 2 * kSampleBins; i += kSampleThreads) hist[i] = 0;
+  if (tid == 0) {
+    s.hist = hist;
+    s.n_list = 0, s.overflow = 0, s.found_bin = kSampleBins - 1, s.found_count = 0, s.first = 0x7fffffff;
+  }
 
   // ---- the slice: chunks [c0, c1) of the 16-byte chunks that the row touches.  Elements of a
-  // chunk outside the row, and NaN, become -inf.
+  // chunk outside the row, and NaN, become -inf; -0 becomes +0.
   const int skip = (int)(reinterpret_cast<uintptr_t>(lrow) & 15) / SIZE;
   const char* base = lrow - (size_t)skip * SIZE;
   const int chunks = (p.V + skip + EPC - 1) / EPC, per = (chunks + C - 1) / C;
   const int c0 = min(rank * per, chunks), c1 = min(c0 + per, chunks);
   const bool cached = p.slice_chunks > 0;
+  auto fetch = [&](int c) {
+    const int i0 = c * EPC - skip;
+    uint32_t w[4];
+    if (i0 >= 0 && i0 + EPC <= p.V) {
+      const uint4 u = *reinterpret_cast<const uint4*>(base + (size_t)c * 16);
+      w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (DT == 2) {
+          w[j] = i0 + j >= 0 && i0 + j < p.V ? reinterpret_cast<const uint32_t*>(lrow)[i0 + j] : 0xff800000u;
+        } else {
+          const uint32_t none = DT == 1 ? 0xff80u : 0xfc00u;
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(lrow);
+          const int a = i0 + 2 * j;
+          const uint32_t lo = a >= 0 && a < p.V ? h[a] : none, hi = a + 1 >= 0 && a + 1 < p.V ? h[a + 1] : none;
+          w[j] = lo | hi << 16;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = clean_word<DT>(w[j]);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
   auto unpack = [](uint4 u, float* x) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -423,97 +493,131 @@ __global__ void __launch_bounds__(kSampleThreads) coalibi_sample_kernel(const Sa
       }
     }
   };
-  auto fetch = [&](int c) {
-    const int i0 = c * EPC - skip;
-    if (i0 >= 0 && i0 + EPC <= p.V) return *reinterpret_cast<const uint4*>(base + (size_t)c * 16);
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (DT == 2) {
-        w[j] = i0 + j >= 0 && i0 + j < p.V ? reinterpret_cast<const uint32_t*>(lrow)[i0 + j] : 0xff800000u;
-      } else {
-        const uint32_t none = DT == 1 ? 0xff80u : 0xfc00u;
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(lrow);
-        const int a = i0 + 2 * j;
-        const uint32_t lo = a >= 0 && a < p.V ? h[a] : none, hi = a + 1 >= 0 && a + 1 < p.V ? h[a + 1] : none;
-        w[j] = lo | hi << 16;
-      }
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  };
-  // calls f(first index, EPC clean logits) for the chunks of this thread
+  // calls f(first index, EPC logits) for the chunks of this thread
   auto each = [&](auto&& f) {
     for (int c = c0 + tid; c < c1; c += kSampleThreads) {
       float x[EPC];
       unpack(cached ? data[c - c0] : fetch(c), x);
-#pragma unroll
-      for (int e = 0; e < EPC; ++e) x[e] = clean_logit(x[e]);
       f(c * EPC - skip, x);
     }
   };
-  float mx = -INFINITY;
-  int arg = 0x7fffffff;
+  float tmax = -INFINITY;  // of this thread's elements
+  {
+    uint32_t m = DT == 2 ? 0xff800000u : DT == 1 ? 0xff80ff80u : 0xfc00fc00u;
 #pragma unroll 4
-  for (int c = c0 + tid; c < c1; c += kSampleThreads) {
-    const uint4 u = fetch(c);
-    if (cached) data[c - c0] = u;
-    float x[EPC];
-    unpack(u, x);
-#pragma unroll
-    for (int e = 0; e < EPC; ++e) {
-      const float y = clean_logit(x[e]);
-      if (y > mx) mx = y, arg = c * EPC - skip + e;  // a thread's indices grow: the first of equals
+    for (int c = c0 + tid; c < c1; c += kSampleThreads) {
+      const uint4 u = fetch(c);
+      if (cached) data[c - c0] = u;
+      m = max_word<DT>(max_word<DT>(max_word<DT>(m, u.x), max_word<DT>(u.y, u.z)), u.w);
+    }
+    if (DT == 2) {
+      tmax = __uint_as_float(m);
+    } else {
+      const float2 f = unpack2<DT == 1>(m);
+      tmax = fmaxf(f.x, f.y);
     }
   }
-  const unsigned long long mine = block_max(mx > -INFINITY ? rank_key(mx, arg) : 0ull, s);
-  sc.mx = mine != 0 ? key_logit((uint32_t)(mine >> 32)) : -INFINITY;
-  if (tid == 0) s.best_key = mine;
-  meet();  // (and every CTA of the cluster has started)
+  sc.mx = key_logit(block_max(order_key(tmax), s));
 
   if (by_k && !greedy && top_k <= kSampleMaxK) {
-    // ---- top-k: this slice's k largest, and what shares the last one's bin, go to the first CTA
-    if (mine != 0 && sc.mx < INFINITY) {
-      each([&](int, const float* x) {
-#pragma unroll
-        for (int e = 0; e < EPC; ++e)
-          if (x[e] > -INFINITY)
-            atomicAdd(&s.hist[0][min(kSampleBins - 1, __float2int_rz((sc.mx - x[e]) * kSampleBinsPerLogit))], 1u);
-      });
+    // ---- top-k: list what can be among this slice's k largest
+    const float mx = sc.mx;
+    auto bin_of = [&](float x) { return min(kSampleBins - 1, __float2int_rz((mx - x) * kSampleBinsPerLogit)); };
+    // the bin of rank `want` - 1 of the histogram, and the count down to its end
+    auto find = [&](unsigned want) {
       __syncthreads();
-      constexpr int PER = kSampleBins / kSampleThreads;
       unsigned v[PER], sum = 0, total;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) v[j] = s.hist[0][tid * PER + j], sum += v[j];
+      for (int j = 0; j < PER; ++j) v[j] = hist[tid * PER + j], sum += v[j];
       unsigned at = block_exclusive(sum, s.warp_u, total);
-      const unsigned want = min((unsigned)top_k, total);
+      want = min(want, total);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         if (at < want && at + v[j] >= want) s.found_bin = tid * PER + j, s.found_count = at + v[j];
         at += v[j];
       }
       __syncthreads();
-      const int last = s.found_bin;
-      if (s.found_count <= kSampleRegion) {
-        each([&](int i0, const float* x) {
+      return total;
+    };
+    unsigned n = 0;
+    if (mx == INFINITY) {
+      n = ~0u;
+    } else if (mx > -INFINITY) {
+      bool listed = false;
+      if (top_k <= kSampleQuickK) {
+        if (tmax > -INFINITY) atomicAdd(&hist[bin_of(tmax)], 1u);
+        if (find(top_k) >= (unsigned)top_k) {
+          // k threads have a maximum of at least this, so the k-th largest token is no less
+          const bool in = tmax > -INFINITY && bin_of(tmax) <= (int)s.found_bin;
+          const float least = key_logit(~block_max(in ? ~order_key(tmax) : 0u, s));
+          each([&](int i0, const float* x) {
+#pragma unroll
+            for (int e = 0; e < EPC; ++e)
+              if (x[e] >= least) {
+                const unsigned at = atomicAdd(&s.n_list, 1u);
+                if (at < kSampleListed) list[at] = rank_key(x[e], i0 + e);
+              }
+          });
+          __syncthreads();
+          n = s.n_list;
+          listed = n <= kSampleListed;
+        }
+      }
+      if (!listed) {
+        __syncthreads();
+        for (int i = tid; i < kSampleBins; i += kSampleThreads) hist[i] = 0;
+        if (tid == 0) s.n_list = 0;
+        __syncthreads();
+        each([&](int, const float* x) {
 #pragma unroll
           for (int e = 0; e < EPC; ++e)
-            if (x[e] > -INFINITY && min(kSampleBins - 1, __float2int_rz((sc.mx - x[e]) * kSampleBinsPerLogit)) <= last)
-              list0[rank * kSampleRegion + atomicAdd(&s.n_list, 1u)] = rank_key(x[e], i0 + e);
+            if (x[e] > -INFINITY) atomicAdd(&hist[bin_of(x[e])], 1u);
         });
+        find(top_k);
+        const int last = s.found_bin;
+        n = s.found_count <= kSampleListed ? s.found_count : ~0u;
+        if (n != ~0u) {
+          each([&](int i0, const float* x) {
+#pragma unroll
+            for (int e = 0; e < EPC; ++e)
+              if (x[e] > -INFINITY && bin_of(x[e]) <= last) list[atomicAdd(&s.n_list, 1u)] = rank_key(x[e], i0 + e);
+          });
+        }
       }
     }
-    if (tid == 0) {
-      s0.sent[rank] = s.found_count <= kSampleRegion ? s.found_count : 0u;
-      if (s.found_count > kSampleRegion || sc.mx == INFINITY) s0.overflow = 1;
-    }
+    started();
+    if (tid == 0) s0.sent[rank] = n;
     meet();
-    if (rank != 0) return;
-    if (s.overflow == 0 &&
-        sample_topk(p, s, b, nrow, sc, list, reinterpret_cast<unsigned long long*>(data),
-                    reinterpret_cast<unsigned long long*>(data) + 2 * kSampleMaxK, top_k, top_p, min_p))
+    if (rank != 0) {
+      meet();  // the first CTA has read the list
       return;
+    }
+    int start[kSampleMaxCluster + 1], total = 0;
+    bool fits = true;
+#pragma unroll
+    for (int r = 0; r < kSampleMaxCluster; ++r) {
+      start[r] = total;
+      if (r < C) {
+        fits = fits && s.sent[r] != ~0u;
+        total += (int)s.sent[r];
+      }
+    }
+    if (fits) {
+      auto key_at = [&](int i) {
+        if (C == 1) return list[i];
+        int r = 0, from = 0;
+#pragma unroll
+        for (int q = 1; q < kSampleMaxCluster; ++q)
+          if (q < C && i >= start[q]) r = q, from = start[q];
+        return cluster.map_shared_rank(list, r)[i - from];
+      };
+      unsigned long long* scratch = reinterpret_cast<unsigned long long*>(data);
+      if (sample_topk(p, s, b, nrow, sc, total, key_at, meet, scratch, scratch + 2 * kSampleMaxK, top_k, top_p, min_p))
+        return;
+    } else {
+      meet();
+    }
     __syncthreads();
-    if (tid == 0) s.best_key = 0;
     unsigned long long best = 0;
     for (int i = tid; i < p.V; i += kSampleThreads) {
       const unsigned long long key = rank_key(clean_logit(load_logit<DT>(lrow, i)), i);
@@ -525,10 +629,26 @@ __global__ void __launch_bounds__(kSampleThreads) coalibi_sample_kernel(const Sa
     return;
   }
 
-  unsigned long long best = mine;
-  for (int r = 0; r < C && C > 1; ++r) {
-    const unsigned long long y = cluster.map_shared_rank(&s, r)->best_key;
-    best = y > best ? y : best;
+  // ---- the row's first: the threads that hold the slice's maximum look for its lowest index
+  if (sc.mx > -INFINITY && tmax == sc.mx) {
+    int arg = 0x7fffffff;
+    each([&](int i0, const float* x) {
+#pragma unroll
+      for (int e = EPC - 1; e >= 0; --e)
+        if (x[e] == tmax && i0 + e < arg) arg = i0 + e;
+    });
+    atomicMin(&s.first, arg);
+  }
+  started();
+  __syncthreads();
+  unsigned long long best = sc.mx > -INFINITY ? rank_key(sc.mx, s.first) : 0ull;
+  if (C > 1) {
+    if (tid == 0) s.best_key = best;
+    meet();
+    for (int r = 0; r < C; ++r) {
+      const unsigned long long y = cluster.map_shared_rank(&s, r)->best_key;
+      best = y > best ? y : best;
+    }
   }
   const int first = (int)~(uint32_t)best;
   sc.mx = best != 0 ? key_logit((uint32_t)(best >> 32)) : -INFINITY;
@@ -544,28 +664,67 @@ __global__ void __launch_bounds__(kSampleThreads) coalibi_sample_kernel(const Sa
     return;
   }
 
-  unsigned long long floor_key = 1;  // of nothing but -inf
+  // ---- the race.  Only a token whose quick weight comes within 1e-4 of beating `bound`, the best
+  // that its warp has seen (the quick weight's error is below 2e-5), gets an exact weight and
+  // division; the first token's own score is the bound to start from.
+  float score = 0.f;
+  int token = 0x7fffffff;
+  double rest = 0.0;
+  const float e_first = nrow[first];
+  float bound = e_first > 0.f ? 1.f / e_first : 0.f;
+  auto enter = [&](int i, float x, float w, float e) {
+    if (w * 1.0001f > bound * e) {
+      const float y = expf(sc.dist(x)) / e;
+      if (y > score || (y == score && i < token)) score = y, token = i;
+    }
+  };
+  // the tokens of one chunk per thread that `keep` names, with weights w and random numbers e
+  auto race = [&](int i0, const float* x, const float* w, const float* e, unsigned keep) {
+    float sum = 0.f;
+    bool any = false;
+#pragma unroll
+    for (int q = 0; q < EPC; ++q) {
+      const float wq = keep >> q & 1 ? w[q] : 0.f;
+      sum += wq;
+      any |= wq * 1.0001f > bound * e[q];
+    }
+    if ((unsigned)(first - i0) < (unsigned)EPC) {  // `rest` is without the first's own 1
+      sum = 0.f;
+#pragma unroll
+      for (int q = 0; q < EPC; ++q) sum += keep >> q & 1 && i0 + q != first ? w[q] : 0.f;
+    }
+    rest += (double)sum;
+    if (__any_sync(0xffffffffu, any)) {
+      if (any) {
+#pragma unroll
+        for (int q = 0; q < EPC; ++q)
+          if (keep >> q & 1) enter(i0 + q, x[q], w[q], e[q]);
+      }
+      bound = fmaxf(bound, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(score))));
+    }
+  };
+  constexpr unsigned kAll = (1u << EPC) - 1;
   if (top_p < 1.f) {
     // ---- top-p: bins of the weights' logarithm
+    const float to_bin = -kSampleBinsPerLog2;
     each([&](int, const float* x) {
 #pragma unroll
       for (int e = 0; e < EPC; ++e) {
         const float l2 = sc.log2w(x[e]);
         const unsigned w = sc.fixed(l2);
         if (w == 0) continue;
-        const int bin = sc.bin(l2);
-        atomicAdd(&s.hist[0][bin], w & 0xffffu);
-        if (w >> 16) atomicAdd(&s.hist[1][bin], w >> 16);
+        const int bin = min(kSampleBins - 1, __float2int_rz(l2 * to_bin));
+        atomicAdd(&hist[bin], w & 0xffffu);
+        if (w >> 16) atomicAdd(&hist[kSampleBins + bin], w >> 16);
       }
     });
     meet();
-    constexpr int PER = kSampleBins / kSampleThreads;
     if (C > 1) {  // a stripe of the bins each, summed over the cluster
       for (int i = rank * kSampleThreads + tid; i < kSampleBins; i += C * kSampleThreads) {
         unsigned long long sum = 0;
         for (int r = 0; r < C; ++r) {
-          const SampleShared* o = cluster.map_shared_rank(&s, r);
-          sum += o->hist[0][i] + ((unsigned long long)o->hist[1][i] << 16);
+          const unsigned int* h = cluster.map_shared_rank(hist, r);
+          sum += h[i] + ((unsigned long long)h[kSampleBins + i] << 16);
         }
         list0[i] = sum;
       }
@@ -576,7 +735,7 @@ __global__ void __launch_bounds__(kSampleThreads) coalibi_sample_kernel(const Sa
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         const int i = tid * PER + j;
-        v[j] = C > 1 ? list[i] : s.hist[0][i] + ((unsigned long long)s.hist[1][i] << 16);
+        v[j] = C > 1 ? list[i] : hist[i] + ((unsigned long long)hist[kSampleBins + i] << 16);
         sum += v[j];
       }
       unsigned long long at = block_exclusive(sum, s.warp_ull, total);
@@ -588,118 +747,121 @@ __global__ void __launch_bounds__(kSampleThreads) coalibi_sample_kernel(const Sa
       }
     }
     meet();
-    const int cross = s0.found_bin;
-    // ---- the tokens of the bin in which the sum crosses the target, one by one
-    each([&](int i0, const float* x) {
+    // ---- the tokens of the bins above the crossing one race, its own are listed
+    const float cross = (float)s0.found_bin;
+    for (int cb = c0; cb < c1; cb += kSampleThreads) {  // (the warps stay together)
+      const int c = cb + tid, i0 = c * EPC - skip;
+      float x[EPC], w[EPC], e[EPC];
+      unsigned keep = 0;
+      if (c < c1) {
+        unpack(cached ? data[c - c0] : fetch(c), x);
 #pragma unroll
-      for (int e = 0; e < EPC; ++e)
-        if (x[e] > -INFINITY && sc.bin(sc.log2w(x[e])) == cross) {
-          const unsigned at = atomicAdd(&s0.n_list, 1u);
-          if (at < kSampleTies) list0[at] = rank_key(x[e], i0 + e);
-        }
-    });
-    meet();
-    if (rank == 0) {
-      const int n = s.n_list;
-      unsigned long long low = ~0ull;
-      if (n <= kSampleTies) {
-        unsigned* weight = s.hist[0];
-        for (int i = tid; i < n; i += kSampleThreads) weight[i] = sc.fixed(sc.log2w(key_logit((uint32_t)(list[i] >> 32))));
-        __syncthreads();
-        for (int i = tid; i < n; i += kSampleThreads) {
-          unsigned long long before = s.base;
-          const unsigned long long key = list[i];
-          for (int j = 0; j < n; ++j) before += list[j] > key ? weight[j] : 0u;
-          if (before < s.target) low = key < low ? key : low;
+        for (int q = 0; q < EPC; ++q) {
+          const float l2 = sc.log2w(x[q]), at = l2 * to_bin;
+          w[q] = ex2_approx(l2);
+          if (at < cross) {
+            if (w[q] >= min_p || i0 + q == first) keep |= 1u << q;
+          } else if (at < cross + 1.f) {
+            const unsigned n = atomicAdd(&s0.n_list, 1u);
+            if (n < kSampleTies) list0[n] = rank_key(x[q], i0 + q);
+          }
         }
       }
-      low = ~block_max(~low, s);
-      if (tid == 0) s.floor_key = low, s.overflow = n > kSampleTies;
+#pragma unroll
+      for (int q = 0; q < EPC; ++q) e[q] = keep >> q & 1 ? nrow[i0 + q] : 1.f;
+      race(i0, x, w, e, keep);
     }
+    block_race(score, token, rest, s);
+    if (tid == 0) s0.score[rank] = score, s0.token[rank] = token, s0.rest[rank] = rest;
     meet();
-    floor_key = s0.floor_key;
-    const bool lost = s0.overflow != 0;
-    if (lost) {
-      meet();  // all have read it
-      if (rank == 0) sample_general<DT>(p, s, b, lrow, nrow, sc, first, top_k, top_p, min_p);
+    if (rank != 0) return;
+    const int n = s.n_list;
+    if (n > kSampleTies) {
+      __syncthreads();
+      sample_general<DT>(p, s, b, lrow, nrow, sc, first, top_k, top_p, min_p);
       return;
     }
-  }
-
-  // ---- the race.  Only a token whose quick weight comes within 1e-4 of beating the best so
-  // far (its error is below 2e-5) gets an exact weight and division.
-  const float floor_x = key_logit((uint32_t)(floor_key >> 32));
-  const int floor_i = (int)~(uint32_t)floor_key;
-  const bool whole = floor_key == 1;
-  float score = -1.f;
-  int token = 0x7fffffff;
-  double rest = 0.0;
-  auto enter = [&](int i, float x, float w, float e) {
-    if (w * 1.0001f >= score * e) {
-      const float y = expf(sc.dist(x)) / e;
-      if (y > score || (y == score && i < token)) score = y, token = i;
+    for (int i = tid; i < n; i += kSampleThreads) hist[i] = sc.fixed(sc.log2w(key_logit((uint32_t)(list[i] >> 32))));
+    score = 0.f, token = 0x7fffffff, rest = 0.0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kSampleThreads) {
+      unsigned long long before = s.base;
+      const unsigned long long key = list[i];
+      for (int j = 0; j < n; ++j) before += list[j] > key ? hist[j] : 0u;
+      if (before >= s.target) continue;
+      const int at = (int)~(uint32_t)key;
+      const float x = key_logit((uint32_t)(key >> 32)), w = ex2_approx(sc.log2w(x));
+      if (at != first) {
+        if (w < min_p) continue;
+        rest += (double)w;
+      }
+      enter(at, x, w, nrow[at]);
     }
-  };
-  if (whole && min_p <= 0.f) {
-    // every token: the random numbers stream in beside the logits
+    block_race(score, token, rest, s);
+  } else if (min_p <= 0.f) {
+    // ---- every token: the random numbers stream in beside the logits
     const bool wide = (reinterpret_cast<uintptr_t>(nrow - skip) & 15) == 0;
     constexpr int AHEAD = 16 / EPC;  // chunks whose numbers are in flight
-    for (int c = c0 + tid; c < c1; c += AHEAD * kSampleThreads) {
+    for (int cb = c0; cb < c1; cb += AHEAD * kSampleThreads) {
       float e[AHEAD][EPC];
 #pragma unroll
       for (int a = 0; a < AHEAD; ++a) {
-        const int cc = c + a * kSampleThreads, i0 = cc * EPC - skip;
-        if (cc < c1 && wide && i0 >= 0 && i0 + EPC <= p.V) {
+        const int c = cb + a * kSampleThreads + tid, i0 = c * EPC - skip;
+        if (c < c1 && wide && i0 >= 0 && i0 + EPC <= p.V) {
 #pragma unroll
           for (int q = 0; q < EPC / 4; ++q)
-            *reinterpret_cast<float4*>(&e[a][4 * q]) = *reinterpret_cast<const float4*>(nrow + i0 + 4 * q);
+            *reinterpret_cast<float4*>(&e[a][4 * q]) = __ldcs(reinterpret_cast<const float4*>(nrow + i0 + 4 * q));
         } else {
 #pragma unroll
-          for (int q = 0; q < EPC; ++q) e[a][q] = cc < c1 && i0 + q >= 0 && i0 + q < p.V ? nrow[i0 + q] : 1.f;
+          for (int q = 0; q < EPC; ++q) e[a][q] = c < c1 && i0 + q >= 0 && i0 + q < p.V ? nrow[i0 + q] : 1.f;
         }
       }
 #pragma unroll
       for (int a = 0; a < AHEAD; ++a) {
-        const int cc = c + a * kSampleThreads, i0 = cc * EPC - skip;
-        if (cc >= c1) break;
-        float x[EPC], sum = 0.f;
-        unpack(cached ? data[cc - c0] : fetch(cc), x);
+        const int c = cb + a * kSampleThreads + tid;
+        float x[EPC], w[EPC];
+        if (c < c1) {
+          unpack(cached ? data[c - c0] : fetch(c), x);
 #pragma unroll
-        for (int q = 0; q < EPC; ++q) {
-          x[q] = clean_logit(x[q]);
-          const float w = ex2_approx(sc.log2w(x[q]));
-          if (i0 + q != first) sum += w;
-          if (x[q] > -INFINITY) enter(i0 + q, x[q], w, e[a][q]);
+          for (int q = 0; q < EPC; ++q) w[q] = ex2_approx(sc.log2w(x[q]));
         }
-        rest += (double)sum;
+        race(c * EPC - skip, x, w, e[a], c < c1 ? kAll : 0u);
       }
     }
+    block_race(score, token, rest, s);
   } else {
-    each([&](int i0, const float* x) {
-      float sum = 0.f;
+    // ---- min-p alone
+    for (int cb = c0; cb < c1; cb += kSampleThreads) {
+      const int c = cb + tid, i0 = c * EPC - skip;
+      float x[EPC], w[EPC], e[EPC];
+      unsigned keep = 0;
+      if (c < c1) {
+        unpack(cached ? data[c - c0] : fetch(c), x);
 #pragma unroll
-      for (int q = 0; q < EPC; ++q) {
-        const int i = i0 + q;
-        const float w = ex2_approx(sc.log2w(x[q]));
-        if (i != first) {
-          if (!(x[q] > -INFINITY) || w < min_p || w == 0.f) continue;
-          if (!whole && (x[q] < floor_x || (x[q] == floor_x && i > floor_i))) continue;
-          sum += w;
+        for (int q = 0; q < EPC; ++q) {
+          w[q] = ex2_approx(sc.log2w(x[q]));
+          if (w[q] >= min_p || i0 + q == first) keep |= 1u << q;
         }
-        enter(i, x[q], w, nrow[i]);
       }
-      rest += (double)sum;
-    });
+#pragma unroll
+      for (int q = 0; q < EPC; ++q) e[q] = keep >> q & 1 ? nrow[i0 + q] : 1.f;
+      race(i0, x, w, e, keep);
+    }
+    block_race(score, token, rest, s);
   }
-  block_race(score, token, rest, s);
-  if (tid == 0) s0.score[rank] = score, s0.token[rank] = token, s0.rest[rank] = rest;
-  meet();
+
+  // ---- the first CTA joins the results of all (after top-p its own last one is a further part)
+  const bool more = top_p < 1.f;
+  if (!more) {
+    if (tid == 0) s0.score[rank] = score, s0.token[rank] = token, s0.rest[rank] = rest;
+    meet();
+  }
   if (rank == 0 && tid == 0) {
-    for (int r = 1; r < C; ++r) {
+    for (int r = more ? 0 : 1; r < C; ++r) {
       if (s.score[r] > score || (s.score[r] == score && s.token[r] < token)) score = s.score[r], token = s.token[r];
       rest += s.rest[r];
     }
-    if (score < 0.f) token = first;  // no number won
+    if (token == 0x7fffffff) token = first;  // no number won
     p.tokens[b] = token;
     p.logprobs[b] = sc.dist(clean_logit(load_logit<DT>(lrow, token))) - log1pf((float)rest);
   }

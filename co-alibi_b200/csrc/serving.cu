@@ -257,17 +257,19 @@ int launch_sample(SampleParams& p, cudaStream_t s) {
     c *= 2;
   p.cluster = c;
   const long long per = (chunks + c - 1) / c;
-  const size_t list = (size_t)c * kSampleRegion * 8, scratch = 3 * kSampleMaxK * 8;
+  p.filters = p.top_k || p.top_p || (p.top_k_all > 0 && p.top_k_all < p.V) || !(p.top_p_all >= 1.f);
+  const size_t fixed = p.filters ? 8 * kSampleBins + 8 * kSampleListed : 4096;
+  const size_t scratch = p.filters ? 3 * kSampleMaxK * 8 : 0;
   size_t slice = (size_t)per * 16;
-  p.slice_chunks = slice + list <= kMostBytes ? (int)per : 0;
+  p.slice_chunks = slice + fixed <= kMostBytes ? (int)per : 0;
   if (p.slice_chunks == 0) slice = 0;
-  const size_t bytes = list + (slice > scratch ? slice : scratch);
+  const size_t bytes = fixed + (slice > scratch ? slice : scratch);
   cudaError_t e = cudaSuccess;
   static std::atomic<unsigned long long> ready{0};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    e = cudaFuncSetAttribute(coalibi_sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes + 4096);
+    e = cudaFuncSetAttribute(coalibi_sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes);
     if (e == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg = {};
