@@ -68,8 +68,8 @@ __device__ __forceinline__ float load_logit(const void* base, long long i) {
   return __half2float(static_cast<const __half*>(base)[i]);
 }
 
-// NaN counts as -inf, -0 as +0.
-__device__ __forceinline__ float clean_logit(float x) { return x != x ? -INFINITY : x + 0.f; }
+// NaN counts as -inf.
+__device__ __forceinline__ float clean_logit(float x) { return fmaxf(x, -INFINITY); }
 
 // The same for a 32-bit word of logits, and the larger of two clean words' elements.
 template <int DT>
@@ -83,20 +83,13 @@ __device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
   return r;
 }
 template <int DT>
-__device__ __forceinline__ uint32_t clean_word(uint32_t a) {
-  if (DT == 2) return __float_as_uint(fmaxf(__uint_as_float(a), -INFINITY) + 0.f);
-  a = max_word<DT>(a, DT == 1 ? 0xff80ff80u : 0xfc00fc00u);  // the operand that is a number
-  if (DT == 1) {
-    const __nv_bfloat162 y = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&a), __floats2bfloat162_rn(0.f, 0.f));
-    return *reinterpret_cast<const uint32_t*>(&y);
-  }
-  const __half2 y = __hadd2(*reinterpret_cast<__half2*>(&a), __floats2half2_rn(0.f, 0.f));
-  return *reinterpret_cast<const uint32_t*>(&y);
+__device__ __forceinline__ uint32_t clean_word(uint32_t a) {  // (max takes the operand that is a number)
+  return max_word<DT>(a, DT == 2 ? 0xff800000u : DT == 1 ? 0xff80ff80u : 0xfc00fc00u);
 }
 
-// Integer of the same order as a clean logit, and back.
+// Integer of the same order as a clean logit (-0 as +0), and back.
 __device__ __forceinline__ uint32_t order_key(float x) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float key_logit(uint32_t k) {
@@ -179,9 +172,9 @@ __device__ __forceinline__ T block_exclusive(T v, T* warp_sums, T& total) {
 struct SampleScale {
   float mx, inv_t, k2;
   __device__ __forceinline__ float dist(float x) const { return x == mx ? 0.f : (x - mx) * inv_t; }
-  // of a finite maximum only; the float32 weight the passes over a slice use
+  // of a finite maximum only; the passes over a slice use it with an approximate 2^x
   __device__ __forceinline__ float log2w(float x) const { return (x - mx) * k2; }
-  __device__ __forceinline__ unsigned fixed(float l2) const { return __float2uint_rn(ex2_approx(l2) * 2147483648.f); }
+  __device__ __forceinline__ unsigned fixed(float l2) const { return __float2uint_rn(ex2_approx(l2 + 31.f)); }
 };
 
 // The winner of the block's race and the weights beside the first token's, in thread 0.
@@ -450,7 +443,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
   }
 
   // ---- the slice: chunks [c0, c1) of the 16-byte chunks that the row touches.  Elements of a
-  // chunk outside the row, and NaN, become -inf; -0 becomes +0.
+  // chunk outside the row, and NaN, become -inf.
   const int skip = (int)(reinterpret_cast<uintptr_t>(lrow) & 15) / SIZE;
   const char* base = lrow - (size_t)skip * SIZE;
   const int chunks = (p.V + skip + EPC - 1) / EPC, per = (chunks + C - 1) / C;
@@ -671,51 +664,63 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
   int token = 0x7fffffff;
   double rest = 0.0;
   const float e_first = nrow[first];
-  float bound = e_first > 0.f ? 1.f / e_first : 0.f;
+  float bound = e_first > 0.f ? 1.f / e_first : 0.f, near = bound * 0.9999f;
   auto enter = [&](int i, float x, float w, float e) {
-    if (w * 1.0001f > bound * e) {
+    if (w > near * e) {
       const float y = expf(sc.dist(x)) / e;
       if (y > score || (y == score && i < token)) score = y, token = i;
     }
   };
-  // the tokens of one chunk per thread that `keep` names, with weights w and random numbers e
-  auto race = [&](int i0, const float* x, const float* w, const float* e, unsigned keep) {
-    float sum = 0.f;
+  // one chunk per thread, with random numbers e and weights w, 0 for the tokens that stay out;
+  // returns the weights' sum without the first token's own 1
+  auto race = [&](int i0, const float* x, const float* w, const float* e) {
+    float2 sum2 = make_float2(w[0], w[1]);
     bool any = false;
 #pragma unroll
-    for (int q = 0; q < EPC; ++q) {
-      const float wq = keep >> q & 1 ? w[q] : 0.f;
-      sum += wq;
-      any |= wq * 1.0001f > bound * e[q];
+    for (int q = 0; q < EPC; q += 2) {
+      if (q > 0) sum2 = __fadd2_rn(sum2, make_float2(w[q], w[q + 1]));
+      const float2 lim = __fmul2_rn(make_float2(e[q], e[q + 1]), make_float2(near, near));
+      any |= w[q] > lim.x || w[q + 1] > lim.y;
     }
-    if ((unsigned)(first - i0) < (unsigned)EPC) {  // `rest` is without the first's own 1
+    float sum = sum2.x + sum2.y;
+    if ((unsigned)(first - i0) < (unsigned)EPC) {
       sum = 0.f;
 #pragma unroll
-      for (int q = 0; q < EPC; ++q) sum += keep >> q & 1 && i0 + q != first ? w[q] : 0.f;
+      for (int q = 0; q < EPC; ++q) sum += i0 + q != first ? w[q] : 0.f;
     }
-    rest += (double)sum;
     if (__any_sync(0xffffffffu, any)) {
-      if (any) {
+#pragma unroll 1
+      for (int q = 0; q < EPC && any; ++q) {
+        float xq = x[0], wq = w[0], eq = e[0];  // (a loop, not EPC copies of the rare path)
 #pragma unroll
-        for (int q = 0; q < EPC; ++q)
-          if (keep >> q & 1) enter(i0 + q, x[q], w[q], e[q]);
+        for (int j = 1; j < EPC; ++j)
+          if (q == j) xq = x[j], wq = w[j], eq = e[j];
+        enter(i0 + q, xq, wq, eq);
       }
+      __syncwarp();
       bound = fmaxf(bound, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(score))));
+      near = bound * 0.9999f;
     }
+    return sum;
   };
-  constexpr unsigned kAll = (1u << EPC) - 1;
+  auto log2w2 = [&](float x0, float x1) {
+    return __fmul2_rn(__fadd2_rn(make_float2(x0, x1), make_float2(-sc.mx, -sc.mx)), make_float2(sc.k2, sc.k2));
+  };
   if (top_p < 1.f) {
     // ---- top-p: bins of the weights' logarithm
     const float to_bin = -kSampleBinsPerLog2;
     each([&](int, const float* x) {
 #pragma unroll
-      for (int e = 0; e < EPC; ++e) {
-        const float l2 = sc.log2w(x[e]);
-        const unsigned w = sc.fixed(l2);
-        if (w == 0) continue;
-        const int bin = min(kSampleBins - 1, __float2int_rz(l2 * to_bin));
-        atomicAdd(&hist[bin], w & 0xffffu);
-        if (w >> 16) atomicAdd(&hist[kSampleBins + bin], w >> 16);
+      for (int q = 0; q < EPC; q += 2) {
+        const float2 l2 = log2w2(x[q], x[q + 1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const unsigned w = sc.fixed(j ? l2.y : l2.x);
+          if (w == 0) continue;
+          const int bin = min(kSampleBins - 1, __float2int_rz((j ? l2.y : l2.x) * to_bin));
+          atomicAdd(&hist[bin], w & 0xffffu);
+          if (w >> 16) atomicAdd(&hist[kSampleBins + bin], w >> 16);
+        }
       }
     });
     meet();
@@ -752,24 +757,29 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
     for (int cb = c0; cb < c1; cb += kSampleThreads) {  // (the warps stay together)
       const int c = cb + tid, i0 = c * EPC - skip;
       float x[EPC], w[EPC], e[EPC];
-      unsigned keep = 0;
+#pragma unroll
+      for (int q = 0; q < EPC; ++q) w[q] = 0.f;
       if (c < c1) {
         unpack(cached ? data[c - c0] : fetch(c), x);
 #pragma unroll
-        for (int q = 0; q < EPC; ++q) {
-          const float l2 = sc.log2w(x[q]), at = l2 * to_bin;
-          w[q] = ex2_approx(l2);
-          if (at < cross) {
-            if (w[q] >= min_p || i0 + q == first) keep |= 1u << q;
-          } else if (at < cross + 1.f) {
-            const unsigned n = atomicAdd(&s0.n_list, 1u);
-            if (n < kSampleTies) list0[n] = rank_key(x[q], i0 + q);
+        for (int q = 0; q < EPC; q += 2) {
+          const float2 l2 = log2w2(x[q], x[q + 1]), at = __fmul2_rn(l2, make_float2(to_bin, to_bin));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float a = j ? at.y : at.x;
+            if (a < cross) {
+              const float y = ex2_approx(j ? l2.y : l2.x);
+              w[q + j] = y >= min_p || i0 + q + j == first ? y : 0.f;
+            } else if (a < cross + 1.f) {
+              const unsigned n = atomicAdd(&s0.n_list, 1u);
+              if (n < kSampleTies) list0[n] = rank_key(x[q + j], i0 + q + j);
+            }
           }
         }
       }
 #pragma unroll
-      for (int q = 0; q < EPC; ++q) e[q] = keep >> q & 1 ? nrow[i0 + q] : 1.f;
-      race(i0, x, w, e, keep);
+      for (int q = 0; q < EPC; ++q) e[q] = w[q] > 0.f ? nrow[i0 + q] : 1.f;
+      rest += (double)race(i0, x, w, e);
     }
     block_race(score, token, rest, s);
     if (tid == 0) s0.score[rank] = score, s0.token[rank] = token, s0.rest[rank] = rest;
@@ -816,17 +826,25 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
           for (int q = 0; q < EPC; ++q) e[a][q] = c < c1 && i0 + q >= 0 && i0 + q < p.V ? nrow[i0 + q] : 1.f;
         }
       }
+      float sum = 0.f;
 #pragma unroll
       for (int a = 0; a < AHEAD; ++a) {
         const int c = cb + a * kSampleThreads + tid;
         float x[EPC], w[EPC];
+#pragma unroll
+        for (int q = 0; q < EPC; ++q) w[q] = 0.f;
         if (c < c1) {
           unpack(cached ? data[c - c0] : fetch(c), x);
 #pragma unroll
-          for (int q = 0; q < EPC; ++q) w[q] = ex2_approx(sc.log2w(x[q]));
+          for (int q = 0; q < EPC; q += 2) {
+            const float2 l2 = log2w2(x[q], x[q + 1]);
+            w[q] = ex2_approx(l2.x);
+            w[q + 1] = ex2_approx(l2.y);
+          }
         }
-        race(c * EPC - skip, x, w, e[a], c < c1 ? kAll : 0u);
+        sum += race(c * EPC - skip, x, w, e[a]);
       }
+      rest += (double)sum;
     }
     block_race(score, token, rest, s);
   } else {
@@ -834,18 +852,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
     for (int cb = c0; cb < c1; cb += kSampleThreads) {
       const int c = cb + tid, i0 = c * EPC - skip;
       float x[EPC], w[EPC], e[EPC];
-      unsigned keep = 0;
+#pragma unroll
+      for (int q = 0; q < EPC; ++q) w[q] = 0.f;
       if (c < c1) {
         unpack(cached ? data[c - c0] : fetch(c), x);
 #pragma unroll
         for (int q = 0; q < EPC; ++q) {
-          w[q] = ex2_approx(sc.log2w(x[q]));
-          if (w[q] >= min_p || i0 + q == first) keep |= 1u << q;
+          const float y = ex2_approx(sc.log2w(x[q]));
+          w[q] = y >= min_p || i0 + q == first ? y : 0.f;
         }
       }
 #pragma unroll
-      for (int q = 0; q < EPC; ++q) e[q] = keep >> q & 1 ? nrow[i0 + q] : 1.f;
-      race(i0, x, w, e, keep);
+      for (int q = 0; q < EPC; ++q) e[q] = w[q] > 0.f ? nrow[i0 + q] : 1.f;
+      rest += (double)race(i0, x, w, e);
     }
     block_race(score, token, rest, s);
   }
