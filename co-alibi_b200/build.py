@@ -1,9 +1,10 @@
-"""Build libcoalibi_sm100.so in-tree with nvcc for sm_100a.
+"""Build libcoalibi_sm100.so in-tree with nvcc for sm_100a, and the Python binding of the
+serving operators (_serving, C++ over PyTorch's headers) that links it.
 
     python co-alibi_b200/build.py [--force] [--verbose]
 
-The library lands in co-alibi_b200/co_alibi_attn/ next to the Python package
-that loads it.  Rebuilds only when a source is newer than the library.
+Both land in co-alibi_b200/co_alibi_attn/ next to the Python package that loads
+them.  Each is rebuilt only when a source is newer than it.
 """
 import argparse
 import glob
@@ -11,12 +12,16 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
-OUT = os.path.join(HERE, "co_alibi_attn", "libcoalibi_sm100.so")
+PKG = os.path.join(HERE, "co_alibi_attn")
+OUT = os.path.join(PKG, "libcoalibi_sm100.so")
+BINDING_SRC = os.path.join(CSRC, "binding.cpp")
+BINDING = os.path.join(PKG, "_serving" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -48,21 +53,50 @@ def needs_build():
 
 
 def build(force=False, verbose=False):
-    if not force and not needs_build():
-        return OUT
-    cu = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
-    tmp = OUT + ".tmp"
-    cmd = [nvcc_path(), *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, *cu, "-o", tmp]
+    build_library(force, verbose)
+    build_binding(force, verbose)
+    return OUT
+
+
+def _run(cmd, verbose, what):
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
     if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + res.stderr[-4000:])
+        raise RuntimeError(f"{what} failed:\n" + res.stderr[-4000:])
+    return res
+
+
+def build_library(force=False, verbose=False):
+    if not force and not needs_build():
+        return
+    cu = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
+    tmp = OUT + ".tmp"
+    res = _run([nvcc_path(), *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, *cu, "-o", tmp], verbose, "nvcc")
     os.replace(tmp, OUT)
     with open(OUT + ".ptxas.txt", "w") as f:
         f.write("\n".join(l for l in res.stderr.splitlines() if "ptxas" in l or "registers" in l
                           or "spill" in l or "smem" in l))
-    return OUT
+
+
+def build_binding(force=False, verbose=False):
+    header = os.path.join(INCLUDE, "coalibi.h")
+    if not force and os.path.exists(BINDING) and all(
+            os.path.getmtime(s) <= os.path.getmtime(BINDING) for s in (BINDING_SRC, header)):
+        return
+    import torch  # for its headers and libraries; nothing of it runs
+    home = os.path.dirname(torch.__file__)
+    inc = [sysconfig.get_paths()["include"], os.path.join(home, "include"),
+           os.path.join(home, "include", "torch", "csrc", "api", "include"),
+           os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include"), INCLUDE]
+    lib = os.path.join(home, "lib")
+    tmp = BINDING + ".tmp"
+    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *sum((["-isystem", i] for i in inc), []),
+          BINDING_SRC, "-o", tmp, "-L", PKG, "-l:libcoalibi_sm100.so", "-Wl,-rpath,$ORIGIN", "-L", lib,
+          f"-Wl,-rpath,{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"],
+         verbose, "g++")
+    os.replace(tmp, BINDING)
 
 
 if __name__ == "__main__":

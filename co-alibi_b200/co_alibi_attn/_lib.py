@@ -113,7 +113,7 @@ def load():
             lib.coalibi_bwd_workspace_min_bytes.restype = c_size_t
             lib.coalibi_bwd_workspace_size.argtypes = [ctypes.POINTER(CoalibiBwdArgs)]
             lib.coalibi_bwd_workspace_size.restype = c_size_t
-            # these take the argument structs as packed bytes (serving.py) or by ctypes.byref
+            # (the serving operators are called through the compiled binding, serving.py)
             lib.coalibi_paged_append.argtypes = [c_void_p, c_void_p]
             lib.coalibi_paged_append.restype = c_int
             lib.coalibi_paged_attention.argtypes = [c_void_p, c_void_p, c_size_t, c_void_p]

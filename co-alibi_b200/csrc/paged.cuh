@@ -18,8 +18,11 @@ __device__ __forceinline__ void report_page(int* status) {
 }
 
 // ---------------------------------------------------------------------------
-// Append.  One CTA per (request, new token); a thread moves 16-byte pieces (8
-// elements) of its heads.  A rotated piece also needs its partner's 8 elements (half
+// Append: key (a, b) of a rotated pair becomes (a cos - b sin, b cos + a sin), everything
+// else is moved.  Bound by the bytes (each read and written once) for prompts and by latency
+// (start -> page table -> store) for single tokens.  A CTA takes `group` consecutive tokens of
+// the batch; its first threads look up where they go, then all threads move 16-byte pieces (8
+// elements), two in flight each.  A rotated piece also needs its partner's 8 elements (half
 // layout) or none (interleaved); the partner is in the same row, so the second load hits L1.
 // ---------------------------------------------------------------------------
 struct AppendParams {
@@ -38,17 +41,20 @@ struct AppendParams {
   int* status;
   long long ks[3], vs[3], qs[3], qos[3], kps[3], vps[3];
   long long table_stride;
-  int Hq, Hkv, S, D;
+  int Hq, Hkv, S;  // Hq 0: no queries
+  long long tokens;  // B * S
+  int group;         // tokens per CTA
   int page_size, max_pages, n_pages;
   int rot, n_pos, interleaved;
 };
 
 constexpr int kAppendThreads = 256;
+constexpr int kAppendGroup = 8;  // most tokens of a CTA
 
-// Rotate the 8 elements at column c of row x (rot columns take part).
+// Rotate the 8 elements `own` at column c < rot; `other` is the partner piece of the half layout.
 template <bool BF16>
-__device__ __forceinline__ uint4 rotate8(const uint16_t* x, int c, uint4 own, const float* cos, const float* sin,
-                                         int rot, int interleaved) {
+__device__ __forceinline__ uint4 rotate8(int c, uint4 own, uint4 other, const float* cos, const float* sin, int rot,
+                                         int interleaved) {
   uint32_t a[4] = {own.x, own.y, own.z, own.w};
   if (interleaved) {
     const float4 cs = *reinterpret_cast<const float4*>(cos + c / 2);
@@ -60,16 +66,14 @@ __device__ __forceinline__ uint4 rotate8(const uint16_t* x, int c, uint4 own, co
       a[i] = pack2<BF16>(f.x * cc[i] - f.y * ss[i], f.y * cc[i] + f.x * ss[i]);
     }
   } else {
-    const int half = rot / 2;
-    const bool low = c < half;
-    const int j = low ? c : c - half;
-    const uint4 other = *reinterpret_cast<const uint4*>(x + (low ? c + half : j));
+    const bool low = c < rot / 2;
+    const int j = low ? c : c - rot / 2;
     const uint32_t o[4] = {other.x, other.y, other.z, other.w};
+    const float sg = low ? -1.f : 1.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float4 cs = *reinterpret_cast<const float4*>(cos + j + 4 * h);
       const float4 sn = *reinterpret_cast<const float4*>(sin + j + 4 * h);
-      const float sg = low ? -1.f : 1.f;
       const float2 f0 = unpack2<BF16>(a[2 * h]), f1 = unpack2<BF16>(a[2 * h + 1]);
       const float2 g0 = unpack2<BF16>(o[2 * h]), g1 = unpack2<BF16>(o[2 * h + 1]);
       a[2 * h] = pack2<BF16>(f0.x * cs.x + sg * g0.x * sn.x, f0.y * cs.y + sg * g0.y * sn.y);
@@ -79,49 +83,90 @@ __device__ __forceinline__ uint4 rotate8(const uint16_t* x, int c, uint4 own, co
   return make_uint4(a[0], a[1], a[2], a[3]);
 }
 
-template <bool BF16>
+template <bool BF16, int D>
 __global__ void __launch_bounds__(kAppendThreads) coalibi_paged_append_kernel(const AppendParams p) {
-  const int b = blockIdx.x / p.S, i = blockIdx.x - b * p.S;
-  const int start = p.start[b];
-  const bool fresh = i < (p.count != nullptr ? min(p.count[b], p.S) : p.S);
-  const long long tok = (long long)start + i;
-  const int pieces = p.D / 8, Hq = p.q != nullptr ? p.Hq : 0;
-  bool stored = false;
-  long long slot_k = 0, slot_v = 0;
-  int pos = 0;
-  bool turn = false;
-  if (fresh) {
-    int page = -1;
-    const int at = (int)(tok / p.page_size);
-    if (start >= 0 && tok < (long long)p.max_pages * p.page_size) page = p.page_table[(size_t)b * p.table_stride + at];
-    stored = page >= 0 && page < p.n_pages;
-    const int s = (int)(tok - (long long)at * p.page_size);
-    slot_k = page * p.kps[0] + s * p.kps[2];
-    slot_v = page * p.vps[0] + s * p.vps[2];
-    pos = p.positions != nullptr ? p.positions[(size_t)b * p.S + i] : (int)tok;
-    turn = p.rot > 0 && pos >= 0 && pos < p.n_pos;
-    if (threadIdx.x == 0 && (!stored || (p.rot > 0 && !turn))) report_page(p.status);
-  }
-  const float* cos = turn ? p.cos + (size_t)pos * (p.rot / 2) : nullptr;
-  const float* sin = turn ? p.sin + (size_t)pos * (p.rot / 2) : nullptr;
-  const int items = (2 * p.Hkv + Hq) * pieces;
-  for (int it = threadIdx.x; it < items; it += kAppendThreads) {
-    const int row = it / pieces, c = (it - row * pieces) * 8;
-    const int kind = row < Hq ? 0 : (row < Hq + p.Hkv ? 1 : 2);
-    const int h = kind == 0 ? row : (kind == 1 ? row - Hq : row - Hq - p.Hkv);
-    if (kind != 0 && !stored) continue;
-    const long long* st = kind == 0 ? p.qs : (kind == 1 ? p.ks : p.vs);
-    const void* src = kind == 0 ? p.q : (kind == 1 ? p.k : p.v);
-    const uint16_t* x = static_cast<const uint16_t*>(src) + b * st[0] + h * st[1] + i * st[2];
-    uint4 val = make_uint4(0u, 0u, 0u, 0u);
-    if (fresh) {
-      val = *reinterpret_cast<const uint4*>(x + c);
-      if (kind != 2 && turn && c < p.rot) val = rotate8<BF16>(x, c, val, cos, sin, p.rot, p.interleaved);
+  struct Token {
+    long long slot_k, slot_v;
+    int b, i, angle;  // angle: row of the tables, or -1
+    bool fresh, stored;
+  };
+  __shared__ Token s_tok[kAppendGroup];
+  constexpr int PIECES = D / 8;
+  const long long first = (long long)blockIdx.x * p.group;
+  const int n = (int)min((long long)p.group, p.tokens - first);
+  grid_dep_wait();
+  if (threadIdx.x < n) {
+    Token t;
+    t.b = (int)((first + threadIdx.x) / p.S);
+    t.i = (int)(first + threadIdx.x - (long long)t.b * p.S);
+    const int start = p.start[t.b];
+    const long long tok = (long long)start + t.i;
+    t.fresh = t.i < (p.count != nullptr ? p.count[t.b] : p.S);
+    t.stored = false;
+    t.slot_k = t.slot_v = 0;
+    t.angle = -1;
+    if (t.fresh) {
+      int page = -1;
+      const int at = (int)(tok / p.page_size), slot = (int)(tok - (long long)at * p.page_size);
+      if (start >= 0 && tok < (long long)p.max_pages * p.page_size)
+        page = p.page_table[(size_t)t.b * p.table_stride + at];
+      t.stored = page >= 0 && page < p.n_pages;
+      t.slot_k = page * p.kps[0] + slot * p.kps[2];
+      t.slot_v = page * p.vps[0] + slot * p.vps[2];
+      if (p.rot > 0) {
+        const long long pos = p.positions != nullptr ? p.positions[(size_t)t.b * p.S + t.i] : tok;
+        if (pos >= 0 && pos < p.n_pos) t.angle = (int)pos;
+      }
+      if (!t.stored || (p.rot > 0 && t.angle < 0)) report_page(p.status);
     }
-    uint16_t* y = kind == 0 ? static_cast<uint16_t*>(p.q_out) + b * p.qos[0] + h * p.qos[1] + i * p.qos[2]
-                  : kind == 1 ? static_cast<uint16_t*>(p.k_pages) + slot_k + h * p.kps[1]
-                              : static_cast<uint16_t*>(p.v_pages) + slot_v + h * p.vps[1];
-    *reinterpret_cast<uint4*>(y + c) = val;
+    s_tok[threadIdx.x] = t;
+  }
+  __syncthreads();
+  const int rows = p.Hq + 2 * p.Hkv, items = n * rows * PIECES;
+  for (int it0 = threadIdx.x; it0 < items; it0 += 2 * kAppendThreads) {
+    uint4 val[2], other[2];
+    int kind[2], head[2], tok[2], col[2];  // kind: 0 query, 1 key, 2 value, -1 nothing to write
+    bool turn[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int it = it0 + u * kAppendThreads;
+      kind[u] = -1;
+      turn[u] = false;
+      if (it >= items) continue;
+      const int r = it / PIECES, row = r % rows;
+      col[u] = (it % PIECES) * 8;
+      tok[u] = r / rows;
+      const Token& t = s_tok[tok[u]];
+      const int k = row < p.Hq ? 0 : (row < p.Hq + p.Hkv ? 1 : 2);
+      head[u] = k == 0 ? row : (k == 1 ? row - p.Hq : row - p.Hq - p.Hkv);
+      if (k != 0 && !t.stored) continue;
+      kind[u] = k;
+      val[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (!t.fresh) continue;
+      const long long* st = k == 0 ? p.qs : (k == 1 ? p.ks : p.vs);
+      const void* src = k == 0 ? p.q : (k == 1 ? p.k : p.v);
+      const uint16_t* x = static_cast<const uint16_t*>(src) + t.b * st[0] + head[u] * st[1] + t.i * st[2];
+      val[u] = *reinterpret_cast<const uint4*>(x + col[u]);
+      turn[u] = k != 2 && t.angle >= 0 && col[u] < p.rot;
+      if (turn[u] && !p.interleaved) {
+        const int half = p.rot / 2;
+        other[u] = *reinterpret_cast<const uint4*>(x + (col[u] < half ? col[u] + half : col[u] - half));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (kind[u] < 0) continue;
+      const Token& t = s_tok[tok[u]];
+      if (turn[u]) {
+        const size_t at = (size_t)t.angle * (p.rot / 2);
+        val[u] = rotate8<BF16>(col[u], val[u], other[u], p.cos + at, p.sin + at, p.rot, p.interleaved);
+      }
+      uint16_t* y =
+          kind[u] == 0   ? static_cast<uint16_t*>(p.q_out) + t.b * p.qos[0] + head[u] * p.qos[1] + t.i * p.qos[2]
+          : kind[u] == 1 ? static_cast<uint16_t*>(p.k_pages) + t.slot_k + head[u] * p.kps[1]
+                         : static_cast<uint16_t*>(p.v_pages) + t.slot_v + head[u] * p.vps[1];
+      *reinterpret_cast<uint4*>(y + col[u]) = val[u];
+    }
   }
 }
 

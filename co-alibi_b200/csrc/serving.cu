@@ -106,10 +106,10 @@ extern "C" int coalibi_paged_append(const CoalibiPagedAppendArgs* a, void* strea
   copy3(p.kps, a->k_page_stride);
   copy3(p.vps, a->v_page_stride);
   p.table_stride = a->table_stride;
-  p.Hq = a->Hq;
+  p.Hq = a->q != nullptr ? a->Hq : 0;
   p.Hkv = a->Hkv;
   p.S = a->S;
-  p.D = a->D;
+  p.tokens = (long long)a->B * a->S;
   p.page_size = a->page_size;
   p.max_pages = a->max_pages;
   p.n_pages = a->n_pages;
@@ -117,10 +117,17 @@ extern "C" int coalibi_paged_append(const CoalibiPagedAppendArgs* a, void* strea
   p.n_pos = a->n_pos;
   p.interleaved = a->interleaved;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a->dtype == COALIBI_BF16)
-    coalibi_paged_append_kernel<true><<<a->B * a->S, kAppendThreads, 0, s>>>(p);
-  else
-    coalibi_paged_append_kernel<false><<<a->B * a->S, kAppendThreads, 0, s>>>(p);
+  // Few tokens spread over the SMs, one to a CTA; a prompt's go in groups, whose lookups then
+  // overlap the moving (16,000 ragged prompt tokens of 48 heads: AP1 us with 1, AP8 with 8).
+  p.group = p.tokens >= 8LL * kAppendGroup * device_sm_count() ? kAppendGroup : 1;
+  const dim3 grid((unsigned)((p.tokens + p.group - 1) / p.group));
+  const bool bf16 = a->dtype == COALIBI_BF16;
+  auto kernel = a->D == 128 ? (bf16 ? coalibi_paged_append_kernel<true, 128> : coalibi_paged_append_kernel<false, 128>)
+                            : (bf16 ? coalibi_paged_append_kernel<true, 64> : coalibi_paged_append_kernel<false, 64>);
+  if (const cudaError_t e = launch_pdl(kernel, grid, dim3(kAppendThreads), 0, s, p); e != cudaSuccess) {
+    set_last_error_detail(cudaGetErrorString(e));
+    return COALIBI_ERR_LAUNCH;
+  }
   return launched("paged append launch");
 }
 
