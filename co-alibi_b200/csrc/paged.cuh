@@ -91,7 +91,7 @@ struct Angles {
 };
 
 template <bool BF16, int D, int TURN>
-__global__ void __launch_bounds__(kAppendThreads, 8) coalibi_paged_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, TURN == kTurnHalves ? 6 : 8) coalibi_paged_append_kernel(const AppendParams p) {
   struct Token {
     long long slot_k, slot_v;
     int b, i, angle;  // angle: row of the tables, or -1

@@ -111,6 +111,7 @@ struct SampleShared {
   unsigned long long best_key;  // of this CTA's slice
   unsigned long long floor_key, target, base;
   unsigned int found_bin, found_count, n_list;
+  unsigned int bound;  // bits of the best score so far
   int first, overflow;
   // in the first CTA, an entry from each
   unsigned int sent[kSampleMaxCluster];  // listed tokens; ~0: more than fit, or +inf among them
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
     for (int i = tid; i < 2 * kSampleBins; i += kSampleThreads) hist[i] = 0;
   if (tid == 0) {
     s.hist = hist;
-    s.n_list = 0, s.overflow = 0, s.found_bin = kSampleBins - 1, s.found_count = 0, s.first = 0x7fffffff;
+    s.n_list = 0, s.overflow = 0, s.found_bin = kSampleBins - 1, s.found_count = 0, s.first = 0x7fffffff, s.bound = 0;
   }
 
   // ---- the slice: chunks [c0, c1) of the 16-byte chunks that the row touches.  Elements of a
@@ -658,7 +659,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
   }
 
   // ---- the race.  Only a token whose quick weight comes within 1e-4 of beating `bound`, the best
-  // that its warp has seen (the quick weight's error is below 2e-5), gets an exact weight and
+  // that its CTA has seen (the quick weight's error is below 2e-5), gets an exact weight and
   // division; the first token's own score is the bound to start from.
   float score = 0.f;
   int token = 0x7fffffff;
@@ -676,6 +677,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
   auto race = [&](int i0, const float* x, const float* w, const float* e) {
     float2 sum2 = make_float2(w[0], w[1]);
     bool any = false;
+    bound = fmaxf(bound, __uint_as_float(*const_cast<volatile unsigned int*>(&s.bound)));
+    near = bound * 0.9999f;
 #pragma unroll
     for (int q = 0; q < EPC; q += 2) {
       if (q > 0) sum2 = __fadd2_rn(sum2, make_float2(w[q], w[q + 1]));
@@ -689,16 +692,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
       for (int q = 0; q < EPC; ++q) sum += i0 + q != first ? w[q] : 0.f;
     }
     if (__any_sync(0xffffffffu, any)) {
-#pragma unroll 1
-      for (int q = 0; q < EPC && any; ++q) {
-        float xq = x[0], wq = w[0], eq = e[0];  // (a loop, not EPC copies of the rare path)
+      if (any) {
 #pragma unroll
-        for (int j = 1; j < EPC; ++j)
-          if (q == j) xq = x[j], wq = w[j], eq = e[j];
-        enter(i0 + q, xq, wq, eq);
+        for (int q = 0; q < EPC; ++q) enter(i0 + q, x[q], w[q], e[q]);
       }
       __syncwarp();
       bound = fmaxf(bound, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(score))));
+      if ((tid & 31) == 0) atomicMax(&s.bound, __float_as_uint(bound));
       near = bound * 0.9999f;
     }
     return sum;
@@ -883,6 +883,203 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
     if (token == 0x7fffffff) token = first;  // no number won
     p.tokens[b] = token;
     p.logprobs[b] = sc.dist(clean_logit(load_logit<DT>(lrow, token))) - log1pf((float)rest);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// No filter at all: the race in one pass over logits and random numbers.  Weights are taken
+// relative to the largest logit that the warp has met, sums are rescaled when that grows, and
+// two tokens are compared by e^(x1 - x2) e2 / e1, which needs no maximum; so nothing waits
+// before the last loads have been issued.  Bound by the bytes of the two arrays.
+// ---------------------------------------------------------------------------
+struct StreamPart {
+  float m;      // largest logit (FLT_MAX for +inf, -FLT_MAX if there is none above)
+  double rest;  // sum of the weights relative to m, without that of one token of logit m
+  float x, e;   // the race's leader
+  int i;        // its index, or INT_MAX: nothing yet
+  int first;    // lowest index of logit m (greedy rows)
+};
+
+// e^((x1 - x2) / T) / e1 > 1 / e2, ties to the lower index
+__device__ __forceinline__ bool stream_beats(float x1, float e1, int i1, float x2, float e2, int i2, float inv_t) {
+  if (i2 == 0x7fffffff) return true;
+  if (i1 == 0x7fffffff) return false;
+  const float a = expf((x1 - x2) * inv_t) * e2;
+  return a > e1 || (a == e1 && i1 < i2);
+}
+
+__device__ __forceinline__ StreamPart stream_join(StreamPart a, const StreamPart& b, float inv_t, float k2, bool greedy) {
+  const bool none_a = a.first == 0x7fffffff, none_b = b.first == 0x7fffffff;
+  if (b.m > a.m || (b.m == a.m && b.first < a.first)) a.first = b.first;
+  const float m = fmaxf(a.m, b.m);
+  // each part's own token of weight 1 is left out of its rest: that of the smaller maximum comes
+  // back in; a part that has met nothing (m = -FLT_MAX) has none
+  const double fa = a.m == m ? 1.0 : (double)exp2f((a.m - m) * k2), fb = b.m == m ? 1.0 : (double)exp2f((b.m - m) * k2);
+  a.rest = a.rest * fa + b.rest * fb;
+  if (!none_a && !none_b) a.rest += a.m == m ? fb : fa;
+  a.m = m;
+  if (!greedy && stream_beats(b.x, b.e, b.i, a.x, a.e, a.i, inv_t)) a.x = b.x, a.e = b.e, a.i = b.i;
+  return a;
+}
+
+constexpr int kStreamThreads = 256;
+
+template <int DT>
+__global__ void __launch_bounds__(kStreamThreads, 4) coalibi_sample_stream_kernel(const SampleParams p) {
+  namespace cg = cooperative_groups;
+  constexpr int SIZE = DT == 2 ? 4 : 2, EPC = 16 / SIZE;
+  constexpr int AHEAD = 16 / EPC, N = AHEAD * EPC;  // chunks and tokens of a thread in flight
+  constexpr int WARPS = kStreamThreads / 32;
+  __shared__ StreamPart s_part[WARPS], s_row[kSampleMaxCluster];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = p.cluster, rank = C > 1 ? (int)cluster.block_rank() : 0, b = blockIdx.x / C;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  const char* lrow = static_cast<const char*>(p.logits) + (size_t)b * p.logits_stride * SIZE;
+  const float* nrow = p.noise + (size_t)b * p.noise_stride;
+  const float t = p.temperature ? p.temperature[b] : p.temperature_all;
+  const bool greedy = !(t > 0.f);
+  const float inv_t = greedy ? 1.f : 1.f / t, k2 = inv_t * kLog2e;
+  const int skip = (int)(reinterpret_cast<uintptr_t>(lrow) & 15) / SIZE;
+  const char* base = lrow - (size_t)skip * SIZE;
+  const int chunks = (p.V + skip + EPC - 1) / EPC, per = (chunks + C - 1) / C;
+  const int c0 = min(rank * per, chunks), c1 = min(c0 + per, chunks);
+  const bool wide = (reinterpret_cast<uintptr_t>(nrow - skip) & 15) == 0;
+
+  float m = -INFINITY, near = 0.f;  // of the warp
+  bool inf = false;
+  double rest = 0.0;                // of the lane
+  float lx = 0.f, le = 1.f;
+  int li = 0x7fffffff, first = 0x7fffffff;
+  for (int cb = c0; cb < c1; cb += AHEAD * kStreamThreads) {
+    float x[N], e[N];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int c = cb + a * kStreamThreads + tid, i0 = c * EPC - skip;
+      if (c < c1 && wide && i0 >= 0 && i0 + EPC <= p.V) {
+        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(base + (size_t)c * 16));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int q = 0; q < EPC / 4; ++q)
+          *reinterpret_cast<float4*>(&e[a * EPC + 4 * q]) = __ldcs(reinterpret_cast<const float4*>(nrow + i0 + 4 * q));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (DT == 2) {
+            x[a * EPC + j] = __uint_as_float(clean_word<DT>(w[j]));
+          } else {
+            const float2 f = unpack2<DT == 1>(clean_word<DT>(w[j]));
+            x[a * EPC + 2 * j % EPC] = f.x;
+            x[a * EPC + (2 * j + 1) % EPC] = f.y;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < EPC; ++q) {
+          const bool in = c < c1 && i0 + q >= 0 && i0 + q < p.V;
+          x[a * EPC + q] = in ? clean_logit(load_logit<DT>(lrow, i0 + q)) : -INFINITY;
+          e[a * EPC + q] = in ? nrow[i0 + q] : 1.f;
+        }
+      }
+    }
+    auto index = [&](int n) { return (cb + n / EPC * kStreamThreads + tid) * EPC - skip + n % EPC; };
+    float top = x[0];
+#pragma unroll
+    for (int n = 1; n < N; ++n) top = fmaxf(top, x[n]);
+    if (!inf && __any_sync(0xffffffffu, top == INFINITY)) {  // all the weight is theirs
+      inf = true;
+      m = -INFINITY, near = 0.f, rest = 0.0, li = 0x7fffffff, first = 0x7fffffff;
+    }
+    if (inf) {
+      top = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        x[n] = x[n] == INFINITY ? 3.402823466e38f : -INFINITY;
+        top = fmaxf(top, x[n]);
+      }
+    }
+    bool mine = false;  // whether the token left out of `rest` is one of this lane's here
+    if (__any_sync(0xffffffffu, top > m)) {
+      const float up = key_logit(__reduce_max_sync(0xffffffffu, order_key(top)));
+      const float f = m > -INFINITY ? ex2_approx((m - up) * k2) : 0.f;
+      rest = rest * (double)f + (lane == 0 ? (double)f : 0.0);
+      near *= f;
+      m = up;
+      mine = lane == __ffs(__ballot_sync(0xffffffffu, top == m)) - 1;
+      int at = 0x7fffffff;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (x[n] == m) at = min(at, index(n));
+      first = __reduce_min_sync(0xffffffffu, at);
+    }
+    const float mc = fmaxf(m, -3.402823466e38f);
+    float w[N];
+    float2 sum2 = make_float2(0.f, 0.f);
+    bool any = false;
+#pragma unroll
+    for (int n = 0; n < N; n += 2) {
+      const float2 l2 = __fmul2_rn(__fadd2_rn(make_float2(x[n], x[n + 1]), make_float2(-mc, -mc)), make_float2(k2, k2));
+      w[n] = ex2_approx(l2.x);
+      w[n + 1] = ex2_approx(l2.y);
+      sum2 = __fadd2_rn(sum2, make_float2(w[n], w[n + 1]));
+      const float2 lim = __fmul2_rn(make_float2(e[n], e[n + 1]), make_float2(near, near));
+      any |= w[n] > lim.x || w[n + 1] > lim.y;
+    }
+    float sum = sum2.x + sum2.y;
+    if (mine) {
+      bool out = false;
+      sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const bool skip_it = !out && x[n] == m;
+        out |= skip_it;
+        sum += skip_it ? 0.f : w[n];
+      }
+    }
+    rest += (double)sum;
+    if (__any_sync(0xffffffffu, any)) {
+      if (any) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          if (w[n] > near * e[n] && stream_beats(x[n], e[n], index(n), lx, le, li, inv_t))
+            lx = x[n], le = e[n], li = index(n);
+      }
+      __syncwarp();
+      const float v = li == 0x7fffffff ? 0.f : ex2_approx((lx - mc) * k2) / le;
+      near = 0.9999f * __uint_as_float(__reduce_max_sync(0xffffffffu, v > 0.f ? __float_as_uint(v) : 0u));
+    }
+  }
+  // ---- lanes, warps, CTAs
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const float ox = __shfl_xor_sync(0xffffffffu, lx, o), oe = __shfl_xor_sync(0xffffffffu, le, o);
+    const int oi = __shfl_xor_sync(0xffffffffu, li, o);
+    if (stream_beats(ox, oe, oi, lx, le, li, inv_t)) lx = ox, le = oe, li = oi;
+    rest += __shfl_xor_sync(0xffffffffu, rest, o);
+  }
+  if (lane == 0) {
+    s_part[warp] = StreamPart{m, rest, lx, le, li, first};
+  }
+  __syncthreads();
+  if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (tid == 0) {
+    StreamPart a = s_part[0];
+    for (int w = 1; w < WARPS; ++w) a = stream_join(a, s_part[w], inv_t, k2, greedy);
+    (C > 1 ? cluster.map_shared_rank(s_row, 0) : s_row)[rank] = a;
+  }
+  if (C > 1) cluster.sync();
+  if (rank == 0 && tid == 0) {
+    StreamPart a = s_row[0];
+    for (int r = 1; r < C; ++r) a = stream_join(a, s_row[r], inv_t, k2, greedy);
+    if (a.first == 0x7fffffff) {
+      p.tokens[b] = -1;
+      p.logprobs[b] = -INFINITY;
+    } else if (greedy || a.i == 0x7fffffff) {  // (no number won: the first of the ranking)
+      p.tokens[b] = a.first;
+      p.logprobs[b] = greedy ? 0.f : -log1pf((float)a.rest);
+    } else {
+      p.tokens[b] = a.i;
+      p.logprobs[b] = (a.x == a.m ? 0.f : (a.x - a.m) * inv_t) - log1pf((float)a.rest);
+    }
   }
 }
 

@@ -263,12 +263,40 @@ extern "C" int coalibi_paged_attention(const CoalibiPagedAttentionArgs* a, void*
 namespace coalibi {
 namespace {
 
+// A launch with clusters of p.cluster CTAs, one cluster per row.
+template <typename K>
+cudaError_t launch_rows(K kernel, int threads, size_t smem, const SampleParams& p, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.B * p.cluster));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 template <int DT>
 int launch_sample(SampleParams& p, cudaStream_t s) {
   constexpr int kSize = DT == 2 ? 4 : 2, kChunk = 16 / kSize;
   constexpr int kMostBytes = 200 << 10, kRowBytes = 64 << 10;
   const int sms = device_sm_count();
   const long long chunks = (p.V + kChunk - 2) / kChunk + 1;  // of a row at any alignment, at most
+  p.filters = p.top_k || p.top_p || (p.top_k_all > 0 && p.top_k_all < p.V) || !(p.top_p_all >= 1.f);
+  if (!p.filters && !p.min_p && !(p.min_p_all > 0.f)) {
+    // as many CTAs as run at once (four to an SM), while slices keep two rounds of loads: 256 rows
+    // of 131072 tokens take 57 us with 2 per row (512 CTAs), 68 with 4, 83 with 8, 81 with 1
+    int c = 1;
+    while (c < kSampleMaxCluster && (long long)p.B * c * 2 <= 4LL * sms && chunks >= 4LL * c * kStreamThreads) c *= 2;
+    p.cluster = c;
+    const cudaError_t e = launch_rows(coalibi_sample_stream_kernel<DT>, kStreamThreads, 0, p, s);
+    if (e != cudaSuccess) set_last_error_detail(cudaGetErrorString(e));
+    return e == cudaSuccess ? COALIBI_OK : COALIBI_ERR_LAUNCH;
+  }
   // CTAs per row: enough for slices of about 64 KB, and more while the SMs outnumber them
   int c = 1;
   while (c < kSampleMaxCluster && (chunks * 16 > (long long)c * kRowBytes || (long long)p.B * c * 2 <= sms) &&
@@ -276,7 +304,6 @@ int launch_sample(SampleParams& p, cudaStream_t s) {
     c *= 2;
   p.cluster = c;
   const long long per = (chunks + c - 1) / c;
-  p.filters = p.top_k || p.top_p || (p.top_k_all > 0 && p.top_k_all < p.V) || !(p.top_p_all >= 1.f);
   const size_t fixed = p.filters ? 8 * kSampleBins + 8 * kSampleListed : 4096;
   const size_t scratch = p.filters ? 3 * kSampleMaxK * 8 : 0;
   size_t slice = (size_t)per * 16;
@@ -291,18 +318,7 @@ int launch_sample(SampleParams& p, cudaStream_t s) {
     e = cudaFuncSetAttribute(coalibi_sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes);
     if (e == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.B * c));
-  cfg.blockDim = dim3(kSampleThreads);
-  cfg.dynamicSmemBytes = bytes;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = c;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, coalibi_sample_kernel<DT>, static_cast<const SampleParams&>(p));
+  if (e == cudaSuccess) e = launch_rows(coalibi_sample_kernel<DT>, kSampleThreads, bytes, p, s);
   if (e != cudaSuccess) set_last_error_detail(cudaGetErrorString(e));
   return e == cudaSuccess ? COALIBI_OK : COALIBI_ERR_LAUNCH;
 }
