@@ -26,6 +26,15 @@ class GPTConfig:
     mlp_ratio: int = 4
     bias_max: float = 8.0
     init_std: float = 0.02
+    rotary_dim: int = 0  # first elements of each query and key head rotated by position (0: none)
+
+
+def rotate_heads(x, cos, sin):
+    """x [B, H, S, D] with its first R elements rotated in halves by tables [S, R / 2]
+    (``co_alibi_attn.serving.rotary_tables``), in float32; differentiable."""
+    r = cos.shape[-1]
+    a, b = x[..., :r].float(), x[..., r:2 * r].float()
+    return torch.cat(((a * cos - b * sin).to(x.dtype), (b * cos + a * sin).to(x.dtype), x[..., 2 * r:]), -1)
 
 
 class CoALiBiSelfAttention(nn.Module):
@@ -40,12 +49,22 @@ class CoALiBiSelfAttention(nn.Module):
         self.proj = nn.Linear(cfg.d_model, cfg.d_model)
         self.attn_fn = attn_fn
         self.bias_max = cfg.bias_max
+        self.rotary_dim = cfg.rotary_dim
+
+    def heads(self, x):
+        """Queries, keys and values of x [B, S, C] as [B, H, S, D] views of the fused projection."""
+        B, S, _ = x.shape
+        qkv = self.qkv(x).view(B, S, 3, self.n_head, self.head_dim)
+        return [t.transpose(1, 2) for t in qkv.unbind(dim=2)]
 
     def forward(self, x):
         B, S, C = x.shape
-        qkv = self.qkv(x).view(B, S, 3, self.n_head, self.head_dim)
-        # [B, S, 3, H, D] -> three [B, H, S, D] tensors (contiguous: the kernels take row-major heads)
-        q, k, v = (t.transpose(1, 2).contiguous() for t in qkv.unbind(dim=2))
+        # contiguous: the kernels take row-major heads
+        q, k, v = (t.contiguous() for t in self.heads(x))
+        if self.rotary_dim:
+            from co_alibi_attn.serving import rotary_tables
+            cos, sin = rotary_tables(self.rotary_dim, S, device=x.device)
+            q, k = rotate_heads(q, cos, sin), rotate_heads(k, cos, sin)
         y = self.attn_fn(q, k, v, causal=True, bias_max=self.bias_max)
         return self.proj(y.transpose(1, 2).reshape(B, S, C))
 
