@@ -181,10 +181,11 @@ __global__ void __launch_bounds__(kAppendThreads, TURN == kTurnHalves ? 6 : 8) c
 // every logit, so pieces join exactly: m' = m - slope R, then the usual log-sum-exp merge.
 //
 // What must move is K and V, once per kv head: the G * Sq rows that share them go
-// through the tensor cores together, 16 to a warp.  A CTA has four warps: RW of them
-// side by side over the rows and KG = 4 / RW over the keys.  Up to 64 rows the kernel
-// is bound by the reads; the warp-level MMA is enough for that, and its fragments can be
-// scanned in registers.
+// through the tensor cores together.  Up to 32 rows, 16 to a warp with warp-level MMAs (a
+// 128-lane tcgen05 tile would be mostly empty); a CTA has four warps, RW of them side by side
+// over the rows and KG = 4 / RW over the keys.  Bound by the reads: 4 requests of 65 to 131
+// thousand keys, 4 rows each, 1.61 GB, take 266 us, 6.05 TB/s or 0.92 of the measured copy
+// rate, plus 5 us of joining.
 //
 // The work is cut evenly, whatever the lengths: items (request, kv head, block of RW *
 // 16 rows) are laid end to end in units of 32 * KG keys, and each of a grid of resident
@@ -221,34 +222,29 @@ struct PagedLayout {
   // What starting and finishing an item costs, in units (256 keys' worth): lengths,
   // queries and the first load's latency before its keys, the results after them.  Ragged
   // decoding of 16 requests of 0 .. 8191 keys: 81 us without, 60 / 62 / 65 / 69 us with 2 / 3
-  // / 5 / 8 units of 128 keys; trees of 16 over 127 .. 16383: 166 us, with 2 / 3 / 5 / 8 units
-  // of 32 keys 135 / 123 / 121 / 120 us.
+  // / 5 / 8 units of 128 keys.
   static constexpr int COST = 256 / UNIT;
   static constexpr int ROWS = 16 * RW;
   static constexpr int TILE = kPagedStep * D * 2;  // K or V of one step: [D / 64][32 keys][128 bytes], swizzled
-  static constexpr int NBUF = RW == 4 ? 4 : 3;     // all but one of the steps in flight
+  static constexpr int NBUF = 3;                   // two steps in flight while one is computed
   static constexpr int RING = NBUF * 2 * TILE;     // per key group
   static constexpr int BYTES = KG * RING + 1024;   // (the ring starts at a multiple of 1024)
-  static constexpr int CTAS = D == 128 ? (RW == 1 ? 1 : 2) : RW == 1 ? 2 : RW == 2 ? 3 : 4;  // resident per SM
+  static constexpr int CTAS = D == 128 ? (RW == 1 ? 1 : 2) : (RW == 1 ? 2 : 3);  // resident per SM
   static constexpr int RECORD = ROWS * (4 + D);    // floats of one piece: stats, then O
   // the joining of the key groups reuses the ring
-  static_assert(KG * 16 * RW * D * 4 <= KG * RING || KG == 1, "exchange fits the ring");
+  static_assert(16 * RW * D * 4 <= RING, "exchange fits the ring");
 };
 
 constexpr int kPagedMaxSms = 160;
 constexpr uint64_t kPagedTimeoutNs = 2000000000ull;  // bound on every wait for a load
 
 // Workspace: B + 2 ints (prefix of the requests' spans, units per run), then two records per CTA.
-template <int D, int RW>
+template <typename L>
 inline size_t paged_ws_bytes(int B) {
-  using L = PagedLayout<D, RW>;
   const size_t head = ((size_t)(B + 2) * 4 + 255) / 256 * 256;
   return head + (size_t)kPagedMaxSms * L::CTAS * 2 * L::RECORD * 4;
 }
 __host__ __device__ inline size_t paged_ws_head(int B) { return ((size_t)(B + 2) * 4 + 255) / 256 * 64; }  // in floats
-
-// Row warps for `rows` query rows per kv head.
-inline int paged_row_warps(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
 __device__ __forceinline__ int paged_keys(const PagedAttnParams& p, int b) {
   const int room = p.max_pages * p.page_size;  // at most 2^31 - 256
@@ -266,15 +262,17 @@ __device__ __forceinline__ int paged_span(const PagedAttnParams& p, int b) {
 template <typename L>
 __device__ __forceinline__ int paged_prefix(const PagedAttnParams& p, int* s_pre, int* s_warp, int per, int* out) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool takes = tid < 128;  // (a larger block's other threads only meet at the barriers)
   int sum = 0;
-  for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) sum += paged_span<L>(p, b);
+  if (takes)
+    for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) sum += paged_span<L>(p, b);
   int inc = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += y;
   }
-  if (lane == 31) s_warp[warp] = inc;
+  if (takes && lane == 31) s_warp[warp] = inc;
   __syncthreads();
   int left = 0, total = 0;
 #pragma unroll
@@ -283,16 +281,38 @@ __device__ __forceinline__ int paged_prefix(const PagedAttnParams& p, int* s_pre
     total += s_warp[w];
   }
   int at = left + inc - sum;
-  s_pre[tid] = at;
-  if (out != nullptr) {
-    for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) {
-      out[b] = at;
-      at += paged_span<L>(p, b);
+  if (takes) {
+    s_pre[tid] = at;
+    if (out != nullptr) {
+      for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) {
+        out[b] = at;
+        at += paged_span<L>(p, b);
+      }
+      if (tid == 0) out[p.B] = total;
     }
-    if (tid == 0) out[p.B] = total;
   }
   __syncthreads();
   return total;
+}
+
+// The request, item and unit of it (after its overhead's) that stand at `at`.  All threads.
+template <typename L>
+__device__ __forceinline__ void paged_find(const PagedAttnParams& p, const int* s_pre, int* s_find, int per, int heads,
+                                           unsigned at, int& b, int& span, int& item, int& v0) {
+  const int tid = threadIdx.x;
+  if (tid < 128 && (unsigned)s_pre[tid] * heads <= at && (tid == 127 || (unsigned)s_pre[tid + 1] * heads > at))
+    *s_find = tid;
+  __syncthreads();
+  b = *s_find * per;
+  int pre = s_pre[*s_find];
+  span = paged_span<L>(p, b);
+  while ((unsigned)(pre + span) * heads <= at) {
+    pre += span;
+    ++b;
+    span = paged_span<L>(p, b);
+  }
+  item = (int)((at - (unsigned)pre * heads) / (unsigned)span);
+  v0 = (int)((at - (unsigned)pre * heads) - (unsigned)item * span);
 }
 
 // A 4-D tile load (column, slot, head, page) of the page pool.
@@ -328,7 +348,7 @@ __global__ void __launch_bounds__(128)
   __shared__ int s_abort;
   __shared__ volatile int s_fail[KG];
   __shared__ int s_pre[128], s_warp[4], s_find;
-  __shared__ float4 s_stat[KG > 1 ? KG * L::ROWS : 1];
+  __shared__ float4 s_stat[KG * L::ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gq = lane >> 2, tig = lane & 3;
   const int rwarp = warp % RW, kg = warp / RW;
@@ -351,24 +371,14 @@ __global__ void __launch_bounds__(128)
   // ---- this CTA's run of units
   int* head = reinterpret_cast<int*>(p.ws);
   const int per = (p.B + 127) / 128;
-  const long long total = (long long)paged_prefix<L>(p, s_pre, s_warp, per, blockIdx.x == 0 ? head : nullptr) * heads;
-  const long long quota = (total + p.n_ctas - 1) / p.n_ctas;
+  const unsigned total = (unsigned)paged_prefix<L>(p, s_pre, s_warp, per, blockIdx.x == 0 ? head : nullptr) * heads;
+  const unsigned quota = (total + p.n_ctas - 1) / p.n_ctas;  // (the host bounds the total below 2^31)
   if (blockIdx.x == 0 && tid == 0) head[p.B + 1] = (int)quota;
-  long long at = quota * blockIdx.x;
-  const long long stop = min(total, at + quota);
+  unsigned at = quota * blockIdx.x;
+  const unsigned stop = min(total, at + quota);
   if (at >= stop) return;
-  // the request that holds unit `at`
-  if ((long long)s_pre[tid] * heads <= at && (tid == 127 || (long long)s_pre[tid + 1] * heads > at)) s_find = tid;
-  __syncthreads();
-  int b = s_find * per, pre = s_pre[s_find];
-  int span = paged_span<L>(p, b);
-  while ((long long)(pre + span) * heads <= at) {
-    pre += span;
-    ++b;
-    span = paged_span<L>(p, b);
-  }
-  int item = (int)((at - (long long)pre * heads) / span);
-  int v0 = (int)((at - (long long)pre * heads) - (long long)item * span);
+  int b, span, item, v0;
+  paged_find<L>(p, s_pre, &s_find, per, heads, at, b, span, item, v0);
 
   // shared-memory offsets (within a tile) of this lane's ldmatrix rows; the k-step and the
   // tile pair only flip bits of them: columns 32 * (kk % 4), pair 1 moves the key by 4
@@ -384,7 +394,7 @@ __global__ void __launch_bounds__(128)
 
   while (at < stop) {
     // units [u0, u1) of the item; none if the run ends within its overhead
-    const int v1 = (int)min((long long)span, v0 + (stop - at));
+    const int v1 = (int)min((unsigned)span, v0 + (stop - at));
     const int u0 = max(v0 - L::COST, 0), u1 = v1 - L::COST, units = span - L::COST;
     if (u1 <= 0) break;
     const int g = item / p.row_blocks, r0 = (item - g * p.row_blocks) * L::ROWS + rwarp * 16;
@@ -733,26 +743,7 @@ __global__ void __launch_bounds__(128)
     float* rec = p.ws + paged_ws_head(p.B) + ((size_t)blockIdx.x * 2 + (u0 > 0 ? 0 : 1)) * L::RECORD;
     float4* stats = reinterpret_cast<float4*>(rec);
     float* orec = rec + 4 * L::ROWS;
-    if (KG == 1) {
-#pragma unroll
-      for (int x = 0; x < XR; ++x) {
-        const int r = rwarp * 16 + gq + 8 * x;
-        if (!rok[x]) continue;
-        if (whole) {
-          const int rr = r0 + gq + 8 * x;
-          uint16_t* y = static_cast<uint16_t*>(p.o) + b * p.os[0] + (g * G + rr / p.Sq) * p.os[1] + (rr % p.Sq) * p.os[2];
-          const float inv = l_part[x] > 0.f ? 1.f / l_part[x] : (l_part[x] == 0.f ? 0.f : l_part[x]);
-#pragma unroll
-          for (int dn = 0; dn < 2 * KK; ++dn)
-            *reinterpret_cast<uint32_t*>(y + 8 * dn + 2 * tig) = pack2<BF16>(o[dn][2 * x] * inv, o[dn][2 * x + 1] * inv);
-        } else {
-          if (tig == 0) stats[r] = make_float4(carry[x], m_run[x], l_part[x], 0.f);
-#pragma unroll
-          for (int dn = 0; dn < 2 * KK; ++dn)
-            *reinterpret_cast<float2*>(orec + r * D + 8 * dn + 2 * tig) = make_float2(o[dn][2 * x], o[dn][2 * x + 1]);
-        }
-      }
-    } else {
+    {
       // key groups join through shared memory (the rings are idle now)
       float* xo = reinterpret_cast<float*>(smem);  // [KG][ROWS][D]
       __syncthreads();
@@ -803,7 +794,7 @@ __global__ void __launch_bounds__(128)
         }
       }
     }
-    if (KG > 1) fence_async_smem();
+    fence_async_smem();
     __syncthreads();  // the rings are free for the next item
     if (s_abort != 0) return;
 
@@ -817,11 +808,611 @@ __global__ void __launch_bounds__(128)
   }
 }
 
+// ---------------------------------------------------------------------------
+// More than 32 rows per kv head (trees): tcgen05.  64 or 128 rows as the 128 lanes of TMEM,
+// one row to a thread, so a row's scan over its keys is additions in a register file and
+// needs no shuffles, fragments or ldmatrix (per score about a third of the instructions of
+// the warp-level kernel above, which stays for fewer rows: there a 128-lane tile would be
+// mostly empty).  Two groups of four softmax warps work on their own keys, each with a
+// warp that issues its MMAs and one that issues its loads; per step of a group
+//   S [128 x 64 keys] = Q K^T into one of two TMEM buffers, P = softmax weights written over
+//   it as 16-bit, O [128 x D] += P V.
+// With at most 64 rows (DUP) the rows stand twice in the tile: lanes 0 .. 63 take the first 32
+// keys of a step, lanes 64 .. 127 the other 32, with zeros in P for each other's, so all four
+// warps of a group are busy; those 32 keys come from two separate pieces of the item, and no
+// step needs an exchange between threads.  Pieces join at the item's end as above.
+// ---------------------------------------------------------------------------
+template <int D, bool DUP>
+struct WideLayout {
+  static constexpr int PIECES = DUP ? 4 : 2;       // of an item, per CTA
+  static constexpr int STEP = DUP ? 32 : 64;       // keys of a piece per step
+  static constexpr int UNIT = 128;
+  // As above: trees of 16 drafts over 127 .. 16383 keys take 132 us with 3 units, 79 with 7, 70 with
+  // 9 to 11, 71 with 14 (an item's queries, first loads, exchange and joining take about 10 us).
+  static constexpr int COST = 10;
+  static constexpr int ROWS = DUP ? 64 : 128;
+  static constexpr int TILE = 64 * D * 2;          // K or V of a group's step: [D / 64][64 keys][128 bytes]
+  static constexpr int BOX = 64 * 128;
+  static constexpr int NBUF = 3;
+  static constexpr int RING = NBUF * 2 * TILE;     // per group
+  static constexpr int QBYTES = 128 * D * 2;       // [D / 64][128 rows][128 bytes]
+  static constexpr int BYTES = QBYTES + 2 * RING + 1024;
+  static constexpr int CTAS = 1;
+  static constexpr int RECORD = ROWS * (4 + D);
+  static constexpr int TM_S = 64, TM_O = 256;      // columns of an S buffer; O of group w at TM_O + w * D
+  static constexpr int THREADS = 384;
+  // a group's part of the exchange (O in float, then statistics) reuses its ring
+  static_assert(128 * D * 4 + 128 * 16 <= RING, "exchange fits the ring");
+};
+
+template <int D, bool BF16, bool DUP>
+__global__ void __launch_bounds__(384, 1)
+    coalibi_paged_wide_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                              const PagedAttnParams p) {
+  using L = WideLayout<D, DUP>;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ uint64_t s_full[2][L::NBUF], s_empty[2][L::NBUF], s_scores[2][2], s_probs[2][2], s_pv[2], s_idle[2];
+  // four bits: 16-key quarters of the step that were not loaded; 16: some key of it is not of the context
+  __shared__ int s_gone[2][L::NBUF];
+  __shared__ int s_pre[128], s_warp[4], s_find, s_abort;
+  __shared__ uint32_t s_tmem;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool softmax = warp < 8, issues = warp == 8 || warp == 9;
+  const int w = softmax ? warp >> 2 : warp & 1;  // group
+  const int G = p.Hq / p.Hkv, rows = G * p.Sq;
+  const int heads = p.Hkv * p.row_blocks;
+  const CtaGuard guard{&s_abort, p.status, kPagedTimeoutNs};
+  if (tid == 0) {
+    for (int g = 0; g < 2; ++g) {
+      for (int i = 0; i < L::NBUF; ++i) {
+        mbar_init(&s_full[g][i], 1);
+        mbar_init(&s_empty[g][i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_scores[g][i], 1);
+        mbar_init(&s_probs[g][i], 4);
+      }
+      mbar_init(&s_pv[g], 1);
+      mbar_init(&s_idle[g], 1);
+    }
+    s_abort = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
+  if (warp == 8) {
+    tmem_alloc(&s_tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  grid_dep_wait();
+
+  int* head = reinterpret_cast<int*>(p.ws);
+  const int per = (p.B + 127) / 128;
+  const unsigned total = (unsigned)paged_prefix<L>(p, s_pre, s_warp, per, blockIdx.x == 0 ? head : nullptr) * heads;
+  const unsigned quota = (total + p.n_ctas - 1) / p.n_ctas;  // (the host bounds the total below 2^31)
+  if (blockIdx.x == 0 && tid == 0) head[p.B + 1] = (int)quota;
+  unsigned at = quota * blockIdx.x;
+  const unsigned stop = min(total, at + quota);
+  int b = 0, span = 1, item = 0, v0 = 0;
+  if (at < stop) paged_find<L>(p, s_pre, &s_find, per, heads, at, b, span, item, v0);
+
+  uint8_t* ring = smem + L::QBYTES + w * L::RING;
+  uint32_t seq = 0;  // steps of this group in earlier items: the barriers' phases go on
+  bool ok = true;
+  while (at < stop) {
+    const int v1 = (int)min((unsigned)span, v0 + (stop - at));
+    const int u0 = max(v0 - L::COST, 0), u1 = v1 - L::COST, units = span - L::COST;
+    if (u1 <= 0) break;
+    const int g = item / p.row_blocks, rb = (item - g * p.row_blocks) * L::ROWS;
+    const int len = p.ctx_lens[b], room = p.max_pages * p.page_size, ctx = min(max(len, 0), room);
+    unsigned long long seen_by_any = 0;
+    if (p.tree_mask == nullptr) {
+      seen_by_any = (2ull << (p.Sq - 1)) - 1;
+    } else {
+      for (int i = lane; i < p.Sq; i += 32) seen_by_any |= (unsigned long long)p.tree_mask[b * p.mask_stride + i];
+#pragma unroll
+      for (int d = 16; d; d >>= 1) seen_by_any |= __shfl_xor_sync(0xffffffffu, seen_by_any, d);
+      if (p.Sq < 64) seen_by_any &= (1ull << p.Sq) - 1;
+    }
+    const int drafts = 64 - __clzll((long long)seen_by_any);
+    if ((len > room || ctx + drafts > room) && tid == 0) report_page(p.status);
+    // the pieces: `sub` keys each, the group's first at piece PIECES / 2 * w
+    const int s_lo = u0 * L::UNIT, s_hi = min(min(u1 * L::UNIT, room), ctx + drafts);
+    const int sub = ((max(s_hi - s_lo, 0) + L::PIECES - 1) / L::PIECES + 15) & ~15;
+    auto piece_lo = [&](int q) { return s_lo + q * sub; };
+    auto piece_hi = [&](int q) { return min(s_hi, s_lo + (q + 1) * sub); };
+    auto piece_steps = [&](int q) { return max(0, (piece_hi(q) - piece_lo(q) + L::STEP - 1) / L::STEP); };
+    const int q0 = L::PIECES / 2 * w;
+    const int nsteps = DUP ? max(piece_steps(q0), piece_steps(q0 + 1)) : piece_steps(q0);
+    // first key of half hf of step n (counted from the right); its piece's end
+    auto half_base = [&](int n, int hf) {
+      if (DUP) return piece_lo(q0 + hf) + (piece_steps(q0 + hf) - 1 - n) * 32;
+      return piece_lo(q0) + (nsteps - 1 - n) * 64 + 32 * hf;
+    };
+    auto half_hi = [&](int hf) { return piece_hi(DUP ? q0 + hf : q0); };
+    auto half_lo = [&](int hf) { return piece_lo(DUP ? q0 + hf : q0); };
+
+    // whether some row sees key `lane` of half hf of step n; whether it is a drafted one of those
+    auto used = [&](int n, int hf, int gone) {
+      const int base = half_base(n, hf), key = base + lane;
+      return base >= half_lo(hf) && !(gone >> (2 * hf + (lane >> 4)) & 1) && key < half_hi(hf) &&
+             (key < ctx || (seen_by_any >> (key - ctx) & 1));
+    };
+    auto drafted = [&](int n, int hf, int gone) { return used(n, hf, gone) && half_base(n, hf) + lane >= ctx; };
+    auto not_finite = [&](const uint8_t* vrow) {  // a row of V in shared memory
+      bool bad = false;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 u = *reinterpret_cast<const uint4*>(vrow + (c >> 3) * L::BOX + ((c & 7) << 4));
+        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpack2<BF16>(x[j]);
+          bad |= !(fabsf(f.x) < INFINITY) || !(fabsf(f.y) < INFINITY);
+        }
+      }
+      return bad;
+    };
+    auto is_plain = [&](int n, int gone) {  // all 64 keys loaded and of the context
+      bool plain = gone == 0;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) plain = plain && half_base(n, hf) + 32 <= min(half_hi(hf), ctx);
+      return plain;
+    };
+    int loaded = 0;
+    auto load = [&](int n) {  // step n of the group (one lane of its loading warp)
+      const uint32_t k = seq + n;
+      const int slot = k % L::NBUF;
+      const int* table = p.page_table + (size_t)b * p.table_stride;
+      int page[4], at_slot[4], gone = 0, bytes = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = half_base(n, i >> 1) + 16 * (i & 1);
+        page[i] = -1;
+        at_slot[i] = 0;
+        if (key >= half_lo(i >> 1) && key < half_hi(i >> 1)) {
+          const int t = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+          page[i] = table[t];
+          at_slot[i] = key - t * p.page_size;
+          if ((unsigned)page[i] >= (unsigned)p.n_pages) {
+            page[i] = -1;
+            report_page(p.status);
+          }
+        }
+        if (page[i] < 0)
+          gone |= 1 << i;
+        else
+          bytes += 16 * D * 2 * 2;
+      }
+      if (!mbar_wait(&s_empty[w][slot], ((k / L::NBUF) & 1) ^ 1, guard)) return false;
+      s_gone[w][slot] = is_plain(n, gone) ? 0 : gone | 16;
+      mbar_arrive_expect_tx(&s_full[w][slot], bytes);
+      const uint32_t dst = smem_u32(ring + slot * 2 * L::TILE);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (page[i] < 0) continue;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          tma_load_4d(dst + c * L::BOX + i * 2048, &tk, &s_full[w][slot], 64 * c, at_slot[i], g, page[i]);
+          tma_load_4d(dst + L::TILE + c * L::BOX + i * 2048, &tv, &s_full[w][slot], 64 * c, at_slot[i], g, page[i]);
+        }
+      }
+      ++loaded;
+      return true;
+    };
+    const int ahead = min(nsteps, L::NBUF);  // the rings are free: these start beside the queries
+    if (warp >= 10) {
+      if (lane == 0)
+        for (int n = 0; n < ahead && ok; ++n) ok = load(n);
+      __syncwarp();
+    }
+    if (softmax) {
+      // ---- the queries, in the K-major 128-byte-swizzled form the MMA reads
+      for (int c = tid; c < 128 * (D / 8); c += 256) {
+        const int r = c / (D / 8), ch = c % (D / 8), row = rb + (DUP ? r & 63 : r);
+        uint4 val = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows)
+          val = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + b * p.qs[0] +
+                                                (g * G + row / p.Sq) * p.qs[1] + (row % p.Sq) * p.qs[2] + ch * 8);
+        *reinterpret_cast<uint4*>(smem + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = val;
+      }
+      // O starts at zero; so do the columns of P that this thread's lane never fills
+      const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+      uint32_t zero[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) zero[j] = 0u;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) tmem_st32(mine + L::TM_O + w * D + c, zero);
+      tmem_st_wait();
+      fence_async_smem();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+
+    if (warp >= 10) {
+      // ---------------------------------------------------------- loads
+      if (lane == 0) {
+        for (int n = ahead; n < nsteps && ok; ++n) ok = load(n);
+        const int n_issued = loaded;
+        // every issued copy lands before the item (and the CTA) ends
+        for (int n = max(n_issued - L::NBUF, 0); n < n_issued; ++n)
+          mbar_drain(&s_full[w][(seq + n) % L::NBUF], ((seq + n) / L::NBUF) & 1, guard.timeout_ns);
+      }
+      __syncwarp();
+    } else if (issues) {
+      // ---------------------------------------------------------- MMAs (lane 0 issues)
+      constexpr uint32_t idS = make_idesc_f16(BF16, 128, 64, false, false);
+      constexpr uint32_t idPV = make_idesc_f16(BF16, 128, D, false, true);
+      const uint32_t q_addr = smem_u32(smem), ring_addr = smem_u32(ring);
+      auto issue_scores = [&](int n) {
+        const uint32_t k = seq + n;
+        const int slot = k % L::NBUF;
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[w][slot], (k / L::NBUF) & 1, guard))) return false;
+        if (lane == 0) {
+          tc_fence_after();
+          const uint32_t d = tmem + (2 * w + (k & 1)) * L::TM_S, k_addr = ring_addr + slot * 2 * L::TILE;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_ss(d, make_sdesc_sw128(q_addr + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024),
+                    make_sdesc_sw128(k_addr + (kk >> 2) * L::BOX + (kk & 3) * 32, 16, 1024), idS, kk > 0 ? 1u : 0u);
+          umma_commit(&s_scores[w][k & 1]);
+        }
+        __syncwarp();
+        return true;
+      };
+      // S(0), S(1), PV(0), S(2), PV(1), ...: S(n + 2) overwrites the buffer that PV(n), issued
+      // before it by this thread, has read P from
+      for (int n = 0; n < 2 && n < nsteps && ok; ++n) ok = issue_scores(n);
+      for (int n = 0; n < nsteps && ok; ++n) {
+        const uint32_t k = seq + n;
+        const int slot = k % L::NBUF;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&s_probs[w][k & 1], (k >> 1) & 1, guard)))) break;
+        const int gone = s_gone[w][slot];
+        if (gone != 0) {
+          // V rows that no row sees (past the end, of no page, unseen drafts) may hold anything: zero
+          // them, 0 * NaN is not 0; the drafts that the softmax warps have added by hand too
+#pragma unroll 1
+          for (int hf = 0; hf < 2; ++hf) {
+            uint8_t* vrow = ring + slot * 2 * L::TILE + L::TILE + (32 * hf + lane) * 128;
+            const bool mine = used(n, hf, gone);
+            if (!mine || (p.Sq > 1 && half_base(n, hf) + lane >= ctx && not_finite(vrow))) {
+#pragma unroll
+              for (int c = 0; c < D / 8; ++c)
+                *reinterpret_cast<uint4*>(vrow + (c >> 3) * L::BOX + ((c & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          fence_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) {
+          tc_fence_after();
+          const uint32_t pa = tmem + (2 * w + (k & 1)) * L::TM_S, v_addr = ring_addr + slot * 2 * L::TILE + L::TILE;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_ts(tmem + L::TM_O + w * D, pa + kk * 8, make_sdesc_sw128(v_addr + kk * 16 * 128, L::BOX, 1024), idPV, 1u);
+          umma_commit(&s_pv[w]);
+          umma_commit(&s_empty[w][slot]);
+        }
+        __syncwarp();
+        if (n + 2 < nsteps) ok = issue_scores(n + 2);
+      }
+      if (!ok && lane == 0) {  // what was issued must have finished before TMEM is released
+        umma_commit(&s_idle[w]);
+        mbar_drain(&s_idle[w], 0, guard.timeout_ns);
+      }
+      __syncwarp();
+    } else {
+      // ---------------------------------------------------------- softmax: one row to a thread
+      const int t = (warp & 3) * 32 + lane, r = DUP ? t & 63 : t, my_half = t >> 6;
+      const bool rok = rb + r < rows;
+      const float slope2 = load_slope(p.slopes, p.slopes_dtype, g * G + (rok ? rb + r : rb) / p.Sq) * kLog2e, c_a = p.sm_scale * kLog2e;
+      const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+      const uint32_t o_base = lane_base + L::TM_O + w * D;
+      float m = -INFINITY, l = 0.f, carry = 0.f;
+      bool left = false;
+      for (int n = 0; n < nsteps; ++n) {
+        const uint32_t k = seq + n;
+        const int slot = k % L::NBUF;
+        const uint32_t s_base = lane_base + (2 * w + (k & 1)) * L::TM_S;
+        if (ok) ok = mbar_wait(&s_full[w][slot], (k / L::NBUF) & 1, guard);
+        if (ok) ok = mbar_wait(&s_scores[w][k & 1], (k >> 1) & 1, guard);
+        ok = __all_sync(0xffffffffu, ok);
+        const int gone = s_gone[w][slot];
+        const bool plain = gone == 0;
+        uint32_t pk[DUP ? 1 : 2][16];
+        float alpha = 1.f;
+        bool rescale = false;
+        uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
+        if (!plain) {
+          const int row_of = (rok ? rb + r : rb) % p.Sq;
+          const unsigned long long word =
+              p.tree_mask != nullptr ? (unsigned long long)p.tree_mask[b * p.mask_stride + row_of] : (2ull << row_of) - 1;
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const int base = half_base(n, hf), in = min(half_hi(hf), ctx) - base, end = half_hi(hf) - base;
+            uint32_t v = in >= 32 ? 0xffffffffu : in > 0 ? (1u << in) - 1u : 0u;  // of the context
+            if (end > in && end > 0) {  // drafted tokens, up to `end`
+              const int d = base - ctx;
+              const uint32_t bits = d >= 0 ? (d < 64 ? (uint32_t)(word >> d) : 0u) : d > -32 ? (uint32_t)word << -d : 0u;
+              const uint32_t upto = end >= 32 ? 0xffffffffu : (1u << end) - 1u;
+              v |= bits & upto & ~(in > 0 ? (in >= 32 ? 0xffffffffu : (1u << in) - 1u) : 0u);
+            }
+            if (base < half_lo(hf)) v = 0u;  // this piece has ended
+            if (gone >> (2 * hf) & 1) v &= 0xffff0000u;
+            if (gone >> (2 * hf + 1) & 1) v &= 0x0000ffffu;
+            vis[hf] = v;
+          }
+        }
+        if (ok) {
+          tc_fence_after();
+#pragma unroll
+          for (int x = 0; x < (DUP ? 1 : 2); ++x) {  // (the right half first)
+            const int hf = DUP ? my_half : 1 - x;
+            uint32_t s[32];
+            tmem_ld32_sync(s_base + 32 * hf, s);
+            const uint32_t seen = hf ? vis[1] : vis[0];
+            auto scan = [&](auto masked) {
+              constexpr bool MASKED = decltype(masked)::value;
+              // sub-chunks of 8 keys: short chains of additions that overlap
+              float tot[4];
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                float run = 0.f;
+#pragma unroll
+                for (int j = 7; j >= 0; j -= 2) {
+                  const int e = 8 * c + j - 1;  // the pair (e, e + 1)
+                  const float2 y = __fmul2_rn(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
+                                              make_float2(c_a, c_a));
+                  const float2 dn = __fadd2_rn(make_float2(ex2_approx(-y.x), ex2_approx(-y.y)), make_float2(1.f, 1.f));
+                  float2 sg = make_float2(rcp_approx(dn.x), rcp_approx(dn.y));
+                  if (MASKED) {
+                    sg.x = seen >> e & 1 ? sg.x : 0.f;
+                    sg.y = seen >> (e + 1) & 1 ? sg.y : 0.f;
+                  }
+                  const float z1 = run + sg.y, z0 = z1 + sg.x;
+                  run = z0;
+                  const float2 v = __ffma2_rn(make_float2(-slope2, -slope2), make_float2(z0, z1), y);
+                  s[e] = __float_as_uint(v.x);
+                  s[e + 1] = __float_as_uint(v.y);
+                }
+                tot[c] = run;
+              }
+              // sums right of each sub-chunk shift its logits
+              float off[4];
+              off[3] = carry;
+              off[2] = off[3] + tot[3];
+              off[1] = off[2] + tot[2];
+              off[0] = off[1] + tot[1];
+              carry = off[0] + tot[0];
+              float mx = -INFINITY;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const float sh = -slope2 * off[c];
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                  const int e = 8 * c + j;
+                  float2 v = __fadd2_rn(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), make_float2(sh, sh));
+                  if (MASKED) {
+                    v.x = seen >> e & 1 ? v.x : -INFINITY;
+                    v.y = seen >> (e + 1) & 1 ? v.y : -INFINITY;
+                  }
+                  s[e] = __float_as_uint(v.x);
+                  s[e + 1] = __float_as_uint(v.y);
+                  mx = fmaxf(mx, fmaxf(v.x, v.y));
+                }
+              }
+              return mx;
+            };
+            const float mx = plain ? scan(std::false_type{}) : scan(std::true_type{});
+            // the reference moves only when a logit passes it by 2^8: weights stay below 256, and
+            // O needs rescaling rarely
+            if (mx > m + 8.f || (m == -INFINITY && mx > -INFINITY)) {
+              const float f = m == -INFINITY ? 0.f : ex2_approx(m - mx);
+              if (m != -INFINITY) {
+                rescale = true;
+                alpha *= f;
+                if (!DUP && x == 1) {  // the right half's weights of this step move too
+                  const float2 f2 = make_float2(f, f);
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) {
+                    const float2 u = __fmul2_rn(unpack2<BF16>(pk[0][j]), f2);
+                    pk[0][j] = pack2<BF16>(u.x, u.y);
+                  }
+                }
+              }
+              l *= f;
+              m = mx;
+            }
+            const float m_use = m == -INFINITY ? 0.f : m;
+            float2 ls = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float2 v = __fadd2_rn(make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])),
+                                          make_float2(-m_use, -m_use));
+              const float2 e = make_float2(ex2_approx(v.x), ex2_approx(v.y));
+              ls = __fadd2_rn(ls, e);
+              pk[DUP ? 0 : x][j] = pack2<BF16>(e.x, e.y);
+            }
+            l += ls.x + ls.y;
+          }
+          if (__any_sync(0xffffffffu, rescale)) {
+            // every PV before this step's must have added its part
+            if (k > 0) ok = mbar_wait(&s_pv[w], (k - 1) & 1, guard);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+              tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_ld32_sync(o_base + c, o);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                tmem_st32(o_base + c, o);
+              }
+            }
+          }
+        }
+        // ---- P over this step's scores
+        if (!ok) {
+          left = true;
+          break;
+        }
+        if (DUP) {
+          const uint32_t none[16] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+          tmem_st16(s_base + 16 * my_half, pk[0]);
+          tmem_st16(s_base + 16 * (1 - my_half), none);
+        } else {
+          tmem_st16(s_base + 16, pk[0]);
+          tmem_st16(s_base, pk[DUP ? 0 : 1]);
+        }
+        tmem_st_wait();
+        if (!plain && p.Sq > 1) {
+          // ---- a drafted token's V that is not finite must not reach the rows that do not see it
+          // through 0 * V: it is added by hand, and the issuing warp zeroes it
+#pragma unroll 1
+          for (int hf = 0; hf < 2; ++hf) {
+            const uint8_t* vt = ring + slot * 2 * L::TILE + L::TILE + 32 * hf * 128;
+            const bool bad = drafted(n, hf, gone) && not_finite(vt + lane * 128);
+            const uint32_t bads = __ballot_sync(0xffffffffu, bad);
+            if (bads != 0 && (!DUP || hf == my_half)) {
+              if (k > 0) ok = mbar_wait(&s_pv[w], (k - 1) & 1, guard);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              tc_fence_after();
+              for (uint32_t rest = bads; rest != 0; rest &= rest - 1) {
+                const int j = __ffs(rest) - 1;
+                const float2 w2 = unpack2<BF16>(__float_as_uint(tmem_ld1_sync(s_base + 16 * hf + (j >> 1))));
+                const float wj = j & 1 ? w2.y : w2.x;
+                const bool see = (hf ? vis[1] : vis[0]) >> j & 1;
+                const uint8_t* vj = vt + j * 128;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 16) {
+                  uint32_t o[16];
+                  tmem_ld16_sync(o_base + c, o);
+#pragma unroll
+                  for (int q = 0; q < 8; ++q) {
+                    const int ch = (c + 2 * q) >> 3;
+                    const float2 f = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(
+                        vj + (ch >> 3) * L::BOX + (((ch & 7) ^ (j & 7)) << 4) + ((2 * q) & 7) * 2));
+                    if (see) {
+                      o[2 * q] = __float_as_uint(fmaf(wj, f.x, __uint_as_float(o[2 * q])));
+                      o[2 * q + 1] = __float_as_uint(fmaf(wj, f.y, __uint_as_float(o[2 * q + 1])));
+                    }
+                  }
+                  tmem_st16(o_base + c, o);
+                  tmem_st_wait();
+                }
+              }
+            }
+          }
+        }
+        if (!ok) {
+          left = true;
+          break;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_probs[w][k & 1]);
+      }
+      // ---- this group's pieces to the exchange: O, swizzled by row, and the statistics
+      // (the last scores imply every PV but the last two: a wait on the last one's parity alone would
+      // pass while the one before it is under way)
+      if (!left && nsteps > 1) ok = mbar_wait(&s_pv[w], (seq + nsteps - 2) & 1, guard);
+      if (ok && !left && nsteps > 0) ok = mbar_wait(&s_pv[w], (seq + nsteps - 1) & 1, guard);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        tc_fence_after();
+        float* xo = reinterpret_cast<float*>(ring);
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld32_sync(o_base + c, o);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const int ch = (c + j) >> 2;
+            *reinterpret_cast<uint4*>(xo + t * D + ((ch ^ (t & (D / 4 - 1))) << 2)) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          }
+        }
+        reinterpret_cast<float4*>(xo + 128 * D)[t] = make_float4(carry, m, l, slope2);
+      }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (*static_cast<volatile int*>(&s_abort) != 0) break;
+
+    // ---- pieces join, right to left
+    const bool whole = u0 == 0 && u1 == units;
+    float* rec = p.ws + paged_ws_head(p.B) + ((size_t)blockIdx.x * 2 + (u0 > 0 ? 0 : 1)) * L::RECORD;
+    const int n_rows = min(L::ROWS, rows - rb);
+    for (int e = tid; e < n_rows * (D / 4); e += L::THREADS) {
+      const int r = e / (D / 4), ch = e % (D / 4);
+      float right = 0.f, M = -INFINITY, wt[L::PIECES];
+#pragma unroll
+      for (int q = L::PIECES - 1; q >= 0; --q) {
+        const int lane_row = DUP ? r + 64 * (q & 1) : r, grp = DUP ? q >> 1 : q;
+        const float* xo = reinterpret_cast<const float*>(smem + L::QBYTES + grp * L::RING);
+        const float4 st = reinterpret_cast<const float4*>(xo + 128 * D)[lane_row];
+        wt[q] = st.y == -INFINITY ? -INFINITY : st.y - st.w * right;
+        M = fmaxf(M, wt[q]);
+        right += st.x;
+      }
+      const float m_use = M == -INFINITY ? 0.f : M;
+      float l = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int q = L::PIECES - 1; q >= 0; --q) {
+        const int lane_row = DUP ? r + 64 * (q & 1) : r, grp = DUP ? q >> 1 : q;
+        const float* xo = reinterpret_cast<const float*>(smem + L::QBYTES + grp * L::RING);
+        const float f = ex2_approx(wt[q] - m_use);
+        l = fmaf(reinterpret_cast<const float4*>(xo + 128 * D)[lane_row].z, f, l);
+        const float4 v = *reinterpret_cast<const float4*>(xo + lane_row * D + ((ch ^ (lane_row & (D / 4 - 1))) << 2));
+        acc.x = fmaf(v.x, f, acc.x);
+        acc.y = fmaf(v.y, f, acc.y);
+        acc.z = fmaf(v.z, f, acc.z);
+        acc.w = fmaf(v.w, f, acc.w);
+      }
+      if (whole) {
+        const int rr = rb + r;
+        uint16_t* y = static_cast<uint16_t*>(p.o) + b * p.os[0] + (g * G + rr / p.Sq) * p.os[1] + (rr % p.Sq) * p.os[2];
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        *reinterpret_cast<uint2*>(y + 4 * ch) =
+            make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+      } else {
+        if (ch == 0) reinterpret_cast<float4*>(rec)[r] = make_float4(right, M, l, 0.f);
+        *reinterpret_cast<float4*>(rec + 4 * L::ROWS + r * D + 4 * ch) = acc;
+      }
+    }
+    fence_async_smem();  // the exchange before the loads that refill the rings
+    __syncthreads();
+
+    seq += nsteps;
+    at += v1 - v0;
+    v0 = 0;
+    if (++item == heads) {
+      item = 0;
+      if (++b < p.B) span = paged_span<L>(p, b);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 // Joins the pieces of the items that span runs.  One warp per query row; lanes hold the
 // statistics of up to 32 pieces at a time, rightmost first.
-template <int D, bool BF16, int RW>
+template <int D, bool BF16, typename L>
 __global__ void __launch_bounds__(128) coalibi_paged_join_kernel(const PagedAttnParams p) {
-  using L = PagedLayout<D, RW>;
   constexpr int V = D / 32;
   const int lane = threadIdx.x & 31;
   const int G = p.Hq / p.Hkv, rows = G * p.Sq;

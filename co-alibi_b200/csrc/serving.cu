@@ -146,16 +146,15 @@ extern "C" int coalibi_paged_append(const CoalibiPagedAppendArgs* a, void* strea
 namespace coalibi {
 namespace {
 
-template <int D, bool BF16, int RW, int XR>
-int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& p, int sms, cudaStream_t s) {
-  using L = PagedLayout<D, RW>;
+// The attention kernel of layout L and the kernel that joins its pieces.
+template <int D, bool BF16, typename L, typename K>
+int launch_paged(K kernel, std::atomic<unsigned long long>& ready, int threads, const CUtensorMap& tk,
+                 const CUtensorMap& tv, PagedAttnParams& p, int sms, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
-  static std::atomic<unsigned long long> ready{0};  // bit per device (the library knows at most 64)
   int dev = 0;
   cudaGetDevice(&dev);
-  if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    e = cudaFuncSetAttribute(coalibi_paged_attn_kernel<D, BF16, RW, XR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             L::BYTES);
+  if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {  // bit per device (the library knows at most 64)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
     if (e == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   const int rows = p.Hq / p.Hkv * p.Sq;
@@ -165,32 +164,48 @@ int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& 
   const long long bound = (most + L::COST) * p.B * p.Hkv * p.row_blocks;  // if every table row were full
   if (bound > 0x7fffffffLL) return COALIBI_ERR_SHAPE;
   if (bound < p.n_ctas) p.n_ctas = (int)bound;
-  if (e == cudaSuccess)
-    e = launch_pdl(coalibi_paged_attn_kernel<D, BF16, RW, XR>, dim3(p.n_ctas), dim3(128), L::BYTES, s, tk, tv, p);
+  if (e == cudaSuccess) e = launch_pdl(kernel, dim3(p.n_ctas), dim3(threads), L::BYTES, s, tk, tv, p);
   // an item of one unit is never split
   if (e == cudaSuccess && most > 1)
-    e = launch_pdl(coalibi_paged_join_kernel<D, BF16, RW>, dim3(p.B * p.Hkv, (rows + 3) / 4), dim3(128), 0, s, p);
+    e = launch_pdl(coalibi_paged_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, (rows + 3) / 4), dim3(128), 0, s, p);
   if (e != cudaSuccess) set_last_error_detail(cudaGetErrorString(e));
   return e == cudaSuccess ? launched("paged attention launch") : COALIBI_ERR_LAUNCH;
+}
+
+template <int D, bool BF16, int RW, int XR>
+int launch_narrow(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& p, int sms, cudaStream_t s) {
+  static std::atomic<unsigned long long> ready{0};
+  return launch_paged<D, BF16, PagedLayout<D, RW>>(coalibi_paged_attn_kernel<D, BF16, RW, XR>, ready, 128, tk, tv, p,
+                                                   sms, s);
+}
+
+template <int D, bool BF16, bool DUP>
+int launch_wide(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& p, int sms, cudaStream_t s) {
+  static std::atomic<unsigned long long> ready{0};
+  using L = WideLayout<D, DUP>;
+  return launch_paged<D, BF16, L>(coalibi_paged_wide_kernel<D, BF16, DUP>, ready, L::THREADS, tk, tv, p, sms, s);
 }
 
 template <int D, bool BF16>
 int launch_paged_rows(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& p, int sms, cudaStream_t s) {
   const int rows = p.Hq / p.Hkv * p.Sq;
-  switch (paged_row_warps(rows)) {
-    case 1: return rows <= 8 ? launch_paged<D, BF16, 1, 1>(tk, tv, p, sms, s) : launch_paged<D, BF16, 1, 2>(tk, tv, p, sms, s);
-    case 2: return launch_paged<D, BF16, 2, 2>(tk, tv, p, sms, s);
-    default: return launch_paged<D, BF16, 4, 2>(tk, tv, p, sms, s);
-  }
+  // Warp-level MMAs up to 32 rows, tcgen05 from there, measured (warp level / tcgen05, us a call):
+  // 32 rows, 8 requests of 8192 keys, 8 kv heads 68 / 67; 32 rows, 32 requests of 500 keys 33 / 37;
+  // 24 rows of D = 64, 8 requests of 4000 keys, 12 heads 38 / 53; 16 rows, 8 of 8192 62 / 66;
+  // 64 rows, 8 requests of 127 to 16383 keys 120 / 70.
+  if (rows <= 8) return launch_narrow<D, BF16, 1, 1>(tk, tv, p, sms, s);
+  if (rows <= 16) return launch_narrow<D, BF16, 1, 2>(tk, tv, p, sms, s);
+  if (rows <= 32) return launch_narrow<D, BF16, 2, 2>(tk, tv, p, sms, s);
+  if (rows <= 64) return launch_wide<D, BF16, true>(tk, tv, p, sms, s);
+  return launch_wide<D, BF16, false>(tk, tv, p, sms, s);
 }
 
 template <int D>
 size_t paged_ws_rows(int B, int rows) {
-  switch (paged_row_warps(rows)) {
-    case 1: return paged_ws_bytes<D, 1>(B);
-    case 2: return paged_ws_bytes<D, 2>(B);
-    default: return paged_ws_bytes<D, 4>(B);
-  }
+  if (rows <= 16) return paged_ws_bytes<PagedLayout<D, 1>>(B);
+  if (rows <= 32) return paged_ws_bytes<PagedLayout<D, 2>>(B);
+  if (rows <= 64) return paged_ws_bytes<WideLayout<D, true>>(B);
+  return paged_ws_bytes<WideLayout<D, false>>(B);
 }
 
 }  // namespace

@@ -25,7 +25,7 @@ def pool(lens, Hkv, D, page, dtype, seed, token_major=False, spare=2):
 def gather(pages, table, b, n):
     """The first n tokens of request b: [Hkv, n, D]."""
     page = pages.shape[2]
-    t = torch.arange(n)
+    t = torch.arange(n, device=pages.device)
     return pages[table[b].long()[t // page], :, t % page].transpose(0, 1)
 
 

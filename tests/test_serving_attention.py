@@ -103,6 +103,30 @@ def test_long_context_with_spread_weights(Hq, Hkv, D, L, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv,D,Sq", [(24, 8, 128, 1), (32, 8, 64, 5), (32, 8, 128, 16), (16, 4, 64, 12), (24, 4, 128, 20)])
+def test_many_ragged_requests(Hq, Hkv, D, Sq):
+    """More items than CTAs, of every length modulo the steps: items that end and begin within
+    one CTA's run, pieces of unequal steps, masked steps before plain ones.  Float64 on the GPU."""
+    dt, page = bf16, 16
+    ctx = [0, 1, 15, 16, 31, 33] + list(range(40, 620, 13)) + [1500, 2047]
+    B = len(ctx)
+    k, v, table = (x.cuda() for x in ref.pool([c + Sq for c in ctx], Hkv, D, page, dt, seed=24))
+    q = _q(B, Hq, Sq, D, dt, 25).cuda()
+    words = [ref.tree(Sq, 26 + b) for b in range(B)]
+    slopes = _slopes(Hq)(dt).cuda()
+    o = _run(q, k, v, table, ctx, words)
+    for b, c in enumerate(ctx):
+        kb, vb = (ref.gather(x, table, b, c + Sq).double() for x in (k, v))
+        hidden = torch.zeros(Sq, c + Sq, dtype=torch.bool, device="cuda")
+        hidden[:, c:] = torch.tensor([[not w >> t & 1 for t in range(Sq)] for w in words[b]], device="cuda")
+        p = q[b].double() @ kb.repeat_interleave(Hq // Hkv, 0).transpose(1, 2) / math.sqrt(D)
+        z = torch.sigmoid(p).masked_fill(hidden, 0).flip(-1).cumsum(-1).flip(-1)
+        w = torch.softmax((p - slopes.double()[:, None, None] * z).masked_fill(hidden, -math.inf), -1)
+        vv = vb.repeat_interleave(Hq // Hkv, 0)
+        _check(o[b], (w @ vv).cpu(), (w @ vv.abs()).cpu(), dt)
+
+
+@pytest.mark.gpu
 def test_rows_that_see_nothing_and_unseen_drafts():
     """Words of 0 with an empty context give zero rows; drafts no word names are not read,
     so their slots may hold NaN, and their pages need not exist."""
