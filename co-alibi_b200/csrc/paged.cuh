@@ -638,21 +638,29 @@ __global__ void __launch_bounds__(128)
           l_part[x] += l2.x + l2.y;
         }
       };
-      if (all) {
-        softmax(std::false_type{});
-      } else {
-#pragma unroll
+      if (!all) {
+#pragma unroll 1
         for (int x = 0; x < XR; ++x) {
           uint32_t v = 0;
-#pragma unroll
+#pragma unroll 1
           for (int j = 0; j < 8; ++j) {
             const int key = kb + 8 * tig + 2 * (((j >> 1) + tig) & 3) + (j & 1);
-            if (!(gone >> (tig >> 1) & 1) && key < hi && (key < ctx || (word[x] >> (key - ctx) & 1))) v |= 1u << j;
+            if (!(gone >> (tig >> 1) & 1) && key < hi && (key < ctx || ((x ? word[XR - 1] : word[0]) >> (key - ctx) & 1)))
+              v |= 1u << j;
           }
-          vis[x] = v;
+          if (x)
+            vis[XR - 1] = v;
+          else
+            vis[0] = v;
         }
-        softmax(std::true_type{});
       }
+      // with one row to a lane a second copy for the steps without masks costs more in
+      // instruction fetches than it saves (long contexts 281 us with, 269 without); with two
+      // rows it pays (16 rows, 8 requests of 8192 keys 62 us with, 65 without)
+      if (XR == 1 || !all)
+        softmax(std::true_type{});
+      else
+        softmax(std::false_type{});
       // ---- V rows that no row sees (past the end, of no page, unseen drafts) may hold
       // anything: zero them, 0 * NaN is not 0.  A drafted token's V that is not finite must
       // not reach the rows that do not see it either: it is added by hand, then zeroed.
