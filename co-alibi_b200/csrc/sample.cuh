@@ -422,6 +422,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
   };
   const char* lrow = static_cast<const char*>(p.logits) + (size_t)b * p.logits_stride * SIZE;
   const float* nrow = p.noise + (size_t)b * p.noise_stride;
+  grid_dep_wait();
   const float t = p.temperature ? p.temperature[b] : p.temperature_all;
   const float top_p = p.top_p ? p.top_p[b] : p.top_p_all;
   const float min_p = p.min_p ? p.min_p[b] : p.min_p_all;
@@ -597,17 +598,31 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
       }
     }
     if (fits) {
-      auto key_at = [&](int i) {
-        if (C == 1) return list[i];
+      auto remote = [&](int i) {
         int r = 0, from = 0;
 #pragma unroll
         for (int q = 1; q < kSampleMaxCluster; ++q)
           if (q < C && i >= start[q]) r = q, from = start[q];
         return cluster.map_shared_rank(list, r)[i - from];
       };
+      // scratch over the slice: [2048] binned, [1024] sorted, [2048] the cluster's listed tokens
       unsigned long long* scratch = reinterpret_cast<unsigned long long*>(data);
-      if (sample_topk(p, s, b, nrow, sc, total, key_at, meet, scratch, scratch + 2 * kSampleMaxK, top_k, top_p, min_p))
-        return;
+      unsigned long long* sorted = scratch + 2 * kSampleMaxK;
+      unsigned long long* near_list = scratch + 3 * kSampleMaxK;
+      bool done;
+      if (C == 1 || total <= 2 * kSampleMaxK) {  // brought here once, the other CTAs leave
+        if (C > 1) {
+          for (int i = tid; i < total; i += kSampleThreads) near_list[i] = remote(i);
+          meet();
+        } else {
+          near_list = list;
+        }
+        done = sample_topk(p, s, b, nrow, sc, total, [&](int i) { return near_list[i]; }, [] { __syncthreads(); },
+                           scratch, sorted, top_k, top_p, min_p);
+      } else {
+        done = sample_topk(p, s, b, nrow, sc, total, remote, meet, scratch, sorted, top_k, top_p, min_p);
+      }
+      if (done) return;
     } else {
       meet();
     }
@@ -937,6 +952,7 @@ __global__ void __launch_bounds__(kStreamThreads, 4) coalibi_sample_stream_kerne
   if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const char* lrow = static_cast<const char*>(p.logits) + (size_t)b * p.logits_stride * SIZE;
   const float* nrow = p.noise + (size_t)b * p.noise_stride;
+  grid_dep_wait();
   const float t = p.temperature ? p.temperature[b] : p.temperature_all;
   const bool greedy = !(t > 0.f);
   const float inv_t = greedy ? 1.f : 1.f / t, k2 = inv_t * kLog2e;

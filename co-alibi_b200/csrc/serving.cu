@@ -278,7 +278,8 @@ extern "C" int coalibi_paged_attention(const CoalibiPagedAttentionArgs* a, void*
 namespace coalibi {
 namespace {
 
-// A launch with clusters of p.cluster CTAs, one cluster per row.
+// A launch with clusters of p.cluster CTAs, one cluster per row, its set-up beside the end of the
+// kernel before it on the stream.
 template <typename K>
 cudaError_t launch_rows(K kernel, int threads, size_t smem, const SampleParams& p, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
@@ -286,12 +287,14 @@ cudaError_t launch_rows(K kernel, int threads, size_t smem, const SampleParams& 
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = p.cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // (the kernels wait before global memory)
+  attr[1].val.programmaticStreamSerializationAllowed = COALIBI_PDL ? 1 : 0;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
@@ -320,7 +323,7 @@ int launch_sample(SampleParams& p, cudaStream_t s) {
   p.cluster = c;
   const long long per = (chunks + c - 1) / c;
   const size_t fixed = p.filters ? 8 * kSampleBins + 8 * kSampleListed : 4096;
-  const size_t scratch = p.filters ? 3 * kSampleMaxK * 8 : 0;
+  const size_t scratch = p.filters ? 5 * kSampleMaxK * 8 : 0;  // see coalibi_sample_kernel's top-k
   size_t slice = (size_t)per * 16;
   p.slice_chunks = slice + fixed <= kMostBytes ? (int)per : 0;
   if (p.slice_chunks == 0) slice = 0;

@@ -115,6 +115,14 @@ def test_many_ragged_requests(Hq, Hkv, D, Sq):
     words = [ref.tree(Sq, 26 + b) for b in range(B)]
     slopes = _slopes(Hq)(dt).cuda()
     o = _run(q, k, v, table, ctx, words)
+    if Sq == 1:  # more requests than threads that sum the lengths; tables as views of wider ones
+        many = torch.randint(0, B, (300,), generator=torch.Generator().manual_seed(27))
+        wide = torch.full((300, table.shape[1] + 5), -7, dtype=torch.int32, device="cuda")
+        wide[:, 2:-3] = table[many.cuda()]
+        import co_alibi_attn
+        got = co_alibi_attn.paged_tree_attention(q[many.cuda()], k, v, wide[:, 2:-3],
+                                                 torch.tensor(ctx, dtype=torch.int32)[many].cuda())
+        assert torch.allclose(got.float(), o[many.cuda()].float(), atol=2e-2, rtol=2e-2)  # split elsewhere
     for b, c in enumerate(ctx):
         kb, vb = (ref.gather(x, table, b, c + Sq).double() for x in (k, v))
         hidden = torch.zeros(Sq, c + Sq, dtype=torch.bool, device="cuda")

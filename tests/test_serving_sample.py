@@ -46,6 +46,18 @@ def test_matches_definition(dt, B, V, top_k, top_p, min_p):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("B,V,top_k,top_p", [(2, 50304, 1025, 1.0), (2, 4099, 3000, 0.9), (1, 1_000_003, 50, 1.0),
+                                             (2, 1_000_003, 0, 0.9), (1, 600_001, 1024, 0.5), (150, 2500, 1024, 0.99),
+                                             (40, 9000, 385, 1.0), (1, 2 ** 21, 3, 1.0), (75, 33333, 0, 0.5)])
+def test_large_k_and_vocabularies(dt, B, V, top_k, top_p):
+    """k past the lists, slices that stay in global memory or exceed the bins' 16-bit halves, and
+    row counts on either side of the cluster sizes."""
+    x, e = _inputs(B, V, DT[dt], seed=V % 1000 + top_k)
+    _check(x, e, 0.9, top_k, top_p)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [50304, 333])
 def test_each_row_its_own_parameters(V):
     B = 24
