@@ -724,19 +724,23 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
   if (top_p < 1.f) {
     // ---- top-p: bins of the weights' logarithm
     const float to_bin = -kSampleBinsPerLog2;
-    each([&](int, const float* x) {
+    each([&](int i0, const float* x) {
+      unsigned most = 0;
 #pragma unroll
       for (int q = 0; q < EPC; q += 2) {
         const float2 l2 = log2w2(x[q], x[q + 1]);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const unsigned w = sc.fixed(j ? l2.y : l2.x);
+          most = max(most, w);
           if (w == 0) continue;
           const int bin = min(kSampleBins - 1, __float2int_rz((j ? l2.y : l2.x) * to_bin));
           atomicAdd(&hist[bin], w & 0xffffu);
           if (w >> 16) atomicAdd(&hist[kSampleBins + bin], w >> 16);
         }
       }
+      // the random numbers of tokens that are likely to stay, on their way while the bins are summed
+      if (most >= 1u << 19) asm volatile("prefetch.global.L2 [%0];" ::"l"(nrow + max(i0, 0)));
     });
     meet();
     if (C > 1) {  // a stripe of the bins each, summed over the cluster
@@ -809,11 +813,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
     for (int i = tid; i < n; i += kSampleThreads) hist[i] = sc.fixed(sc.log2w(key_logit((uint32_t)(list[i] >> 32))));
     score = 0.f, token = 0x7fffffff, rest = 0.0;
     __syncthreads();
-    for (int i = tid; i < n; i += kSampleThreads) {
-      unsigned long long before = s.base;
-      const unsigned long long key = list[i];
-      for (int j = 0; j < n; ++j) before += list[j] > key ? hist[j] : 0u;
-      if (before >= s.target) continue;
+    for (int i0 = 0; i0 < n; i0 += kSampleThreads / 4) {  // four lanes to a token
+      const int i = i0 + tid / 4;
+      unsigned long long before = 0;
+      const unsigned long long key = i < n ? list[i] : 0ull;
+      for (int j = tid & 3; j < n; j += 4) before += list[j] > key ? hist[j] : 0u;
+      before += __shfl_xor_sync(0xffffffffu, before, 1);
+      before += __shfl_xor_sync(0xffffffffu, before, 2);
+      if (i >= n || (tid & 3) != 0 || s.base + before >= s.target) continue;
       const int at = (int)~(uint32_t)key;
       const float x = key_logit((uint32_t)(key >> 32)), w = ex2_approx(sc.log2w(x));
       if (at != first) {
