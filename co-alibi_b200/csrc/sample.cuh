@@ -19,6 +19,11 @@
 // stores, 64-bit and float ones are loops of compare-and-swap (48 adds of 1024 threads:
 // 11 thousand cycles against 41 to 340 thousand).  Weights are 2^-31 fixed point in two
 // 16-bit halves there, so sums are exact integers and the order of atomics is irrelevant.
+// Measured, us a call: one row of 50304 with top-k 50 9.8; 64 rows of 50304, each with its own
+// parameters, 22.7 (floor of the reads 2); 300 rows of 32001 with top-p 60 (floor 3: per row 7 us
+// are the bins' atomics, 5 the random numbers' latency, and 300 rows are four more than run at
+// once); 256 rows of 131072 without filters 55 (floor 41, the streaming kernel below).
+//
 // Rows that the bins do not separate (masses of equal logits, infinite ones, k above
 // kSampleMaxK, slices over 65536 tokens) take a radix descent in one CTA.
 #pragma once
@@ -912,7 +917,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
 // No filter at all: the race in one pass over logits and random numbers.  Weights are taken
 // relative to the largest logit that the warp has met, sums are rescaled when that grows, and
 // two tokens are compared by e^(x1 - x2) e2 / e1, which needs no maximum; so nothing waits
-// before the last loads have been issued.  Bound by the bytes of the two arrays.
+// before the last loads have been issued.  Bound by the bytes of the two arrays: 256 rows of
+// 131072 float32 logits, 268 MB, take 55 us, 4.9 TB/s or 0.74 of the measured copy rate.
 // ---------------------------------------------------------------------------
 struct StreamPart {
   float m;      // largest logit (FLT_MAX for +inf, -FLT_MAX if there is none above)
