@@ -182,8 +182,9 @@ __global__ void __launch_bounds__(kAppendThreads, TURN == kTurnHalves ? 6 : 8) c
 //
 // What must move is K and V, once per kv head: the G * Sq rows that share them go
 // through the tensor cores together.  Up to 32 rows, 16 to a warp with warp-level MMAs (a
-// 128-lane tcgen05 tile would be mostly empty); a CTA has four warps, RW of them side by side
-// over the rows and KG = 4 / RW over the keys.  Bound by the reads: 4 requests of 65 to 131
+// 128-lane tcgen05 tile would be mostly empty); a CTA has WARPS warps, RW of them side by side
+// over the rows and KG = WARPS / RW over the keys.  With few items four warps share one, with
+// many each RW warps are a CTA of their own, whose starts and ends overlap the others' reads.  Bound by the reads: 4 requests of 65 to 131
 // thousand keys, 4 rows each, 1.61 GB, take 266 us, 6.05 TB/s or 0.92 of the measured copy
 // rate, plus 5 us of joining.
 //
@@ -210,26 +211,29 @@ struct PagedAttnParams {
   int slopes_dtype;
   int row_blocks;  // blocks of RW * 16 rows per kv head
   int n_ctas;      // of the attention kernel
+  int whole;       // one item to a CTA, none split
   float sm_scale;
 };
 
 constexpr int kPagedStep = 32;  // keys per step of a warp
 
-template <int D, int RW>
+template <int D, int RW, int WARPS>
 struct PagedLayout {
-  static constexpr int KG = 4 / RW;
+  static constexpr int THREADS = 32 * WARPS, KG = WARPS / RW;
   static constexpr int UNIT = kPagedStep * KG;
-  // What starting and finishing an item costs, in units (256 keys' worth): lengths,
-  // queries and the first load's latency before its keys, the results after them.  Ragged
-  // decoding of 16 requests of 0 .. 8191 keys: 81 us without, 60 / 62 / 65 / 69 us with 2 / 3
-  // / 5 / 8 units of 128 keys.
-  static constexpr int COST = 256 / UNIT;
+  // What starting and finishing an item costs, in units: lengths, queries and the first load's
+  // latency before its keys, the results after them.  Ragged decoding of 16 requests of 0 .. 8191
+  // keys with four warps: 81 us without, 60 / 62 / 65 / 69 us with 2 / 3 / 5 / 8 units of 128
+  // keys; with one warp, beside others on its SM, 57.7 / 58.2 us with 4 / 8 of 32.
+  static constexpr int COST = KG == 1 ? 4 : 256 / UNIT;
+  // Up to this many keys an item is not worth splitting: the joining costs a launch.
+  static constexpr int WHOLE = 512;
   static constexpr int ROWS = 16 * RW;
   static constexpr int TILE = kPagedStep * D * 2;  // K or V of one step: [D / 64][32 keys][128 bytes], swizzled
   static constexpr int NBUF = 3;                   // two steps in flight while one is computed
   static constexpr int RING = NBUF * 2 * TILE;     // per key group
   static constexpr int BYTES = KG * RING + 1024;   // (the ring starts at a multiple of 1024)
-  static constexpr int CTAS = D == 128 ? (RW == 1 ? 1 : 2) : (RW == 1 ? 2 : 3);  // resident per SM
+  static constexpr int CTAS = 200 * 1024 / BYTES < 8 ? 200 * 1024 / BYTES : 8;  // resident per SM
   static constexpr int RECORD = ROWS * (4 + D);    // floats of one piece: stats, then O
   // the joining of the key groups reuses the ring
   static_assert(16 * RW * D * 4 <= RING, "exchange fits the ring");
@@ -261,8 +265,9 @@ __device__ __forceinline__ int paged_span(const PagedAttnParams& p, int b) {
 // the total; s_pre[t] is the prefix at the first request of thread t's range.
 template <typename L>
 __device__ __forceinline__ int paged_prefix(const PagedAttnParams& p, int* s_pre, int* s_warp, int per, int* out) {
+  constexpr int NT = L::THREADS < 128 ? L::THREADS : 128;  // (the others only meet at the barriers)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const bool takes = tid < 128;  // (a larger block's other threads only meet at the barriers)
+  const bool takes = tid < NT;
   int sum = 0;
   if (takes)
     for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) sum += paged_span<L>(p, b);
@@ -276,7 +281,7 @@ __device__ __forceinline__ int paged_prefix(const PagedAttnParams& p, int* s_pre
   __syncthreads();
   int left = 0, total = 0;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < NT / 32; ++w) {
     if (w < warp) left += s_warp[w];
     total += s_warp[w];
   }
@@ -299,8 +304,9 @@ __device__ __forceinline__ int paged_prefix(const PagedAttnParams& p, int* s_pre
 template <typename L>
 __device__ __forceinline__ void paged_find(const PagedAttnParams& p, const int* s_pre, int* s_find, int per, int heads,
                                            unsigned at, int& b, int& span, int& item, int& v0) {
+  constexpr int NT = L::THREADS < 128 ? L::THREADS : 128;
   const int tid = threadIdx.x;
-  if (tid < 128 && (unsigned)s_pre[tid] * heads <= at && (tid == 127 || (unsigned)s_pre[tid + 1] * heads > at))
+  if (tid < NT && (unsigned)s_pre[tid] * heads <= at && (tid == NT - 1 || (unsigned)s_pre[tid + 1] * heads > at))
     *s_find = tid;
   __syncthreads();
   b = *s_find * per;
@@ -335,11 +341,11 @@ __device__ __forceinline__ int paged_tile_key(int n, int j) {
   return 8 * t + 2 * ((n + t) & 3) + (j & 1);
 }
 
-template <int D, bool BF16, int RW, int XR>
-__global__ void __launch_bounds__(128)
+template <int D, bool BF16, int RW, int XR, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS)
     coalibi_paged_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                               const PagedAttnParams p) {
-  using L = PagedLayout<D, RW>;
+  using L = PagedLayout<D, RW, WARPS>;
   constexpr int KG = L::KG, KK = D / 16;
   constexpr int THREADS = 32 * RW;  // per key group
   extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -348,7 +354,7 @@ __global__ void __launch_bounds__(128)
   __shared__ int s_abort;
   __shared__ volatile int s_fail[KG];
   __shared__ int s_pre[128], s_warp[4], s_find;
-  __shared__ float4 s_stat[KG * L::ROWS];
+  __shared__ float4 s_stat[KG > 1 ? KG * L::ROWS : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gq = lane >> 2, tig = lane & 3;
   const int rwarp = warp % RW, kg = warp / RW;
@@ -366,19 +372,29 @@ __global__ void __launch_bounds__(128)
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
   }
+  __syncthreads();
   grid_dep_wait();
 
   // ---- this CTA's run of units
-  int* head = reinterpret_cast<int*>(p.ws);
-  const int per = (p.B + 127) / 128;
-  const unsigned total = (unsigned)paged_prefix<L>(p, s_pre, s_warp, per, blockIdx.x == 0 ? head : nullptr) * heads;
-  const unsigned quota = (total + p.n_ctas - 1) / p.n_ctas;  // (the host bounds the total below 2^31)
-  if (blockIdx.x == 0 && tid == 0) head[p.B + 1] = (int)quota;
-  unsigned at = quota * blockIdx.x;
-  const unsigned stop = min(total, at + quota);
-  if (at >= stop) return;
-  int b, span, item, v0;
-  paged_find<L>(p, s_pre, &s_find, per, heads, at, b, span, item, v0);
+  unsigned at = 0, stop;
+  int b, span, item, v0 = 0;
+  if (p.whole) {
+    b = blockIdx.x / heads;
+    item = blockIdx.x - b * heads;
+    span = paged_span<L>(p, b);
+    stop = span;
+  } else {
+    int* head = reinterpret_cast<int*>(p.ws);
+    constexpr int NT = L::THREADS < 128 ? L::THREADS : 128;
+    const int per = (p.B + NT - 1) / NT;
+    const unsigned total = (unsigned)paged_prefix<L>(p, s_pre, s_warp, per, blockIdx.x == 0 ? head : nullptr) * heads;
+    const unsigned quota = (total + p.n_ctas - 1) / p.n_ctas;  // (the host bounds the total below 2^31)
+    if (blockIdx.x == 0 && tid == 0) head[p.B + 1] = (int)quota;
+    at = quota * blockIdx.x;
+    stop = min(total, at + quota);
+    if (at >= stop) return;
+    paged_find<L>(p, s_pre, &s_find, per, heads, at, b, span, item, v0);
+  }
 
   // shared-memory offsets (within a tile) of this lane's ldmatrix rows; the k-step and the
   // tile pair only flip bits of them: columns 32 * (kk % 4), pair 1 moves the key by 4
@@ -751,7 +767,25 @@ __global__ void __launch_bounds__(128)
     float* rec = p.ws + paged_ws_head(p.B) + ((size_t)blockIdx.x * 2 + (u0 > 0 ? 0 : 1)) * L::RECORD;
     float4* stats = reinterpret_cast<float4*>(rec);
     float* orec = rec + 4 * L::ROWS;
-    {
+    if (KG == 1) {
+#pragma unroll
+      for (int x = 0; x < XR; ++x) {
+        const int r = rwarp * 16 + gq + 8 * x, rr = r0 + gq + 8 * x;
+        if (!rok[x]) continue;
+        if (whole) {
+          uint16_t* y = static_cast<uint16_t*>(p.o) + b * p.os[0] + (g * G + rr / p.Sq) * p.os[1] + (rr % p.Sq) * p.os[2];
+          const float inv = l_part[x] > 0.f ? 1.f / l_part[x] : (l_part[x] == 0.f ? 0.f : l_part[x]);
+#pragma unroll
+          for (int dn = 0; dn < 2 * KK; ++dn)
+            *reinterpret_cast<uint32_t*>(y + 8 * dn + 2 * tig) = pack2<BF16>(o[dn][2 * x] * inv, o[dn][2 * x + 1] * inv);
+        } else {
+          if (tig == 0) stats[r] = make_float4(carry[x], m_run[x], l_part[x], 0.f);
+#pragma unroll
+          for (int dn = 0; dn < 2 * KK; ++dn)
+            *reinterpret_cast<float2*>(orec + r * D + 8 * dn + 2 * tig) = make_float2(o[dn][2 * x], o[dn][2 * x + 1]);
+        }
+      }
+    } else {
       // key groups join through shared memory (the rings are idle now)
       float* xo = reinterpret_cast<float*>(smem);  // [KG][ROWS][D]
       __syncthreads();
@@ -767,7 +801,7 @@ __global__ void __launch_bounds__(128)
       __syncthreads();
       const int rb = (item - g * p.row_blocks) * L::ROWS;
       const int n = min(XR == 1 ? 8 : L::ROWS, rows - rb);
-      for (int e = tid; e < n * (D / 4); e += 128) {
+      for (int e = tid; e < n * (D / 4); e += L::THREADS) {
         const int r = e / (D / 4), d = (e % (D / 4)) * 4;
         float right = 0.f, M = -INFINITY, w[KG];
 #pragma unroll
@@ -802,7 +836,7 @@ __global__ void __launch_bounds__(128)
         }
       }
     }
-    fence_async_smem();
+    if (KG > 1) fence_async_smem();
     __syncthreads();  // the rings are free for the next item
     if (s_abort != 0) return;
 
@@ -840,6 +874,7 @@ struct WideLayout {
   // As above: trees of 16 drafts over 127 .. 16383 keys take 132 us with 3 units, 79 with 7, 70 with
   // 9 to 11, 71 with 14 (an item's queries, first loads, exchange and joining take about 10 us).
   static constexpr int COST = 10;
+  static constexpr int WHOLE = 1024;  // 32 requests of 500 / 1000 keys, 8 kv heads: 43 / 52 us, split 50 / 59
   static constexpr int ROWS = DUP ? 64 : 128;
   static constexpr int TILE = 64 * D * 2;          // K or V of a group's step: [D / 64][64 keys][128 bytes]
   static constexpr int BOX = 64 * 128;
@@ -901,15 +936,24 @@ __global__ void __launch_bounds__(384, 1)
   const uint32_t tmem = s_tmem;
   grid_dep_wait();
 
-  int* head = reinterpret_cast<int*>(p.ws);
-  const int per = (p.B + 127) / 128;
-  const unsigned total = (unsigned)paged_prefix<L>(p, s_pre, s_warp, per, blockIdx.x == 0 ? head : nullptr) * heads;
-  const unsigned quota = (total + p.n_ctas - 1) / p.n_ctas;  // (the host bounds the total below 2^31)
-  if (blockIdx.x == 0 && tid == 0) head[p.B + 1] = (int)quota;
-  unsigned at = quota * blockIdx.x;
-  const unsigned stop = min(total, at + quota);
+  unsigned at = 0, stop;
   int b = 0, span = 1, item = 0, v0 = 0;
-  if (at < stop) paged_find<L>(p, s_pre, &s_find, per, heads, at, b, span, item, v0);
+  if (p.whole) {
+    b = blockIdx.x / heads;
+    item = blockIdx.x - b * heads;
+    span = paged_span<L>(p, b);
+    stop = span;
+  } else {
+    int* head = reinterpret_cast<int*>(p.ws);
+    constexpr int NT = L::THREADS < 128 ? L::THREADS : 128;
+    const int per = (p.B + NT - 1) / NT;
+    const unsigned total = (unsigned)paged_prefix<L>(p, s_pre, s_warp, per, blockIdx.x == 0 ? head : nullptr) * heads;
+    const unsigned quota = (total + p.n_ctas - 1) / p.n_ctas;
+    if (blockIdx.x == 0 && tid == 0) head[p.B + 1] = (int)quota;
+    at = quota * blockIdx.x;
+    stop = min(total, at + quota);
+    if (at < stop) paged_find<L>(p, s_pre, &s_find, per, heads, at, b, span, item, v0);
+  }
 
   uint8_t* ring = smem + L::QBYTES + w * L::RING;
   uint32_t seq = 0;  // steps of this group in earlier items: the barriers' phases go on

@@ -3,6 +3,7 @@
 // checked before any device use; nothing here allocates or synchronises.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
 #include <cstdio>
@@ -163,20 +164,35 @@ int launch_paged(K kernel, std::atomic<unsigned long long>& ready, int threads, 
   const long long most = ((long long)p.max_pages * p.page_size + L::UNIT - 1) / L::UNIT;
   const long long bound = (most + L::COST) * p.B * p.Hkv * p.row_blocks;  // if every table row were full
   if (bound > 0x7fffffffLL) return COALIBI_ERR_SHAPE;
-  if (bound < p.n_ctas) p.n_ctas = (int)bound;
+  const long long items = (long long)p.B * p.Hkv * p.row_blocks;
+  p.whole = most * L::UNIT <= L::WHOLE;
+  if (p.whole)
+    p.n_ctas = (int)items;
+  else if (bound < p.n_ctas)
+    p.n_ctas = (int)bound;
   if (e == cudaSuccess) e = launch_pdl(kernel, dim3(p.n_ctas), dim3(threads), L::BYTES, s, tk, tv, p);
-  // an item of one unit is never split
-  if (e == cudaSuccess && most > 1)
+  if (e == cudaSuccess && !p.whole)
     e = launch_pdl(coalibi_paged_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, (rows + 3) / 4), dim3(128), 0, s, p);
   if (e != cudaSuccess) set_last_error_detail(cudaGetErrorString(e));
   return e == cudaSuccess ? launched("paged attention launch") : COALIBI_ERR_LAUNCH;
 }
 
+template <int D, bool BF16, int RW, int XR, int WARPS>
+int launch_narrow_of(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& p, int sms, cudaStream_t s) {
+  static std::atomic<unsigned long long> ready{0};
+  return launch_paged<D, BF16, PagedLayout<D, RW, WARPS>>(coalibi_paged_attn_kernel<D, BF16, RW, XR, WARPS>, ready,
+                                                          32 * WARPS, tk, tv, p, sms, s);
+}
+
 template <int D, bool BF16, int RW, int XR>
 int launch_narrow(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& p, int sms, cudaStream_t s) {
-  static std::atomic<unsigned long long> ready{0};
-  return launch_paged<D, BF16, PagedLayout<D, RW>>(coalibi_paged_attn_kernel<D, BF16, RW, XR>, ready, 128, tk, tv, p,
-                                                   sms, s);
+  // Four warps to an item, or RW where items are plenty, measured (four / one, us a call, 8 kv heads,
+  // 4 rows): 16 requests of 500 keys 11 / 17, 32 of 500 21 / 23, 64 of 500 46 / 31, 256 of 200 92 / 63,
+  // 64 of 1000 67 / 61, 256 of 1000 230 / 195, 8 of 8192 56 / 57.
+  const int rows = p.Hq / p.Hkv * p.Sq;
+  const long long items = (long long)p.B * p.Hkv * ((rows + 16 * RW - 1) / (16 * RW));
+  if (items > 2LL * sms) return launch_narrow_of<D, BF16, RW, XR, RW>(tk, tv, p, sms, s);
+  return launch_narrow_of<D, BF16, RW, XR, 4>(tk, tv, p, sms, s);
 }
 
 template <int D, bool BF16, bool DUP>
@@ -202,8 +218,8 @@ int launch_paged_rows(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnPar
 
 template <int D>
 size_t paged_ws_rows(int B, int rows) {
-  if (rows <= 16) return paged_ws_bytes<PagedLayout<D, 1>>(B);
-  if (rows <= 32) return paged_ws_bytes<PagedLayout<D, 2>>(B);
+  if (rows <= 16) return std::max(paged_ws_bytes<PagedLayout<D, 1, 1>>(B), paged_ws_bytes<PagedLayout<D, 1, 4>>(B));
+  if (rows <= 32) return std::max(paged_ws_bytes<PagedLayout<D, 2, 2>>(B), paged_ws_bytes<PagedLayout<D, 2, 4>>(B));
   if (rows <= 64) return paged_ws_bytes<WideLayout<D, true>>(B);
   return paged_ws_bytes<WideLayout<D, false>>(B);
 }
