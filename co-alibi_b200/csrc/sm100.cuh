@@ -352,8 +352,8 @@ __device__ __forceinline__ void tmem_ld_fence32(uint32_t* r) {
   asm volatile("" : COALIBI_W8(0), COALIBI_W8(8), COALIBI_W8(16), COALIBI_W8(24) : : "memory");
 }
 
-// Load and wait in one statement: between the two forms above the compiler may move or spill
-// a destination register before its value has arrived, which it does under register pressure.
+// Load and wait in one statement: between the two statements of the forms above the compiler
+// is free to move or spill a destination register before its value has arrived.
 __device__ __forceinline__ void tmem_ld32_sync(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
