@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kAppendThreads, TURN == kTurnHalves ? 6 : 8) c
 // over the rows and KG = WARPS / RW over the keys.  With few items four warps share one, with
 // many each RW warps are a CTA of their own, whose starts and ends overlap the others' reads.  Bound by the reads: 4 requests of 65 to 131
 // thousand keys, 4 rows each, 1.61 GB, take 266 us, 6.05 TB/s or 0.92 of the measured copy
-// rate, plus 5 us of joining.
+// rate, plus 4 us of joining.
 //
 // The work is cut evenly, whatever the lengths: items (request, kv head, block of RW *
 // 16 rows) are laid end to end in units of 32 * KG keys, and each of a grid of resident
@@ -1489,10 +1489,28 @@ __global__ void __launch_bounds__(128) coalibi_paged_join_kernel(const PagedAttn
   float M = -INFINITY, l = 0.f, right = 0.f, acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.f;
+  constexpr int EARLY = 4;  // pieces whose O is on its way beside the statistics
   for (int top = c1; top >= c0; top -= 32) {
     const int n = min(32, top - c0 + 1);
+    auto o_of = [&](int j, float* u) {
+      const float* y = record(top - j) + 4 * L::ROWS + rr * D + lane * V;
+      if (V == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(y);
+        u[0] = f.x, u[1] = f.y, u[V - 2] = f.z, u[V - 1] = f.w;
+      } else {
+        const float2 f = *reinterpret_cast<const float2*>(y);
+        u[0] = f.x, u[1] = f.y;
+      }
+    };
     float4 s = make_float4(0.f, -INFINITY, 0.f, 0.f);
     if (lane < n) s = reinterpret_cast<const float4*>(record(top - lane))[rr];
+    float early[EARLY][V];
+#pragma unroll
+    for (int j = 0; j < EARLY; ++j) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) early[j][v] = 0.f;
+      if (j < n) o_of(j, early[j]);
+    }
     float inc = s.x;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -1514,21 +1532,19 @@ __global__ void __launch_bounds__(128) coalibi_paged_join_kernel(const PagedAttn
     l = l * fac + lw;
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] *= fac;
+#pragma unroll
+    for (int j = 0; j < EARLY; ++j) {
+      const float w = __shfl_sync(0xffffffffu, f, j);  // 0 past the last piece
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = fmaf(w, early[j][v], acc[v]);
+    }
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) {
+    for (int j = EARLY; j < n; ++j) {
       const float w = __shfl_sync(0xffffffffu, f, j);
-      const float* y = record(top - j) + 4 * L::ROWS + rr * D + lane * V;
-      if (V == 4) {
-        const float4 u = *reinterpret_cast<const float4*>(y);
-        acc[0] = fmaf(w, u.x, acc[0]);
-        acc[1] = fmaf(w, u.y, acc[1]);
-        acc[V - 2] = fmaf(w, u.z, acc[V - 2]);
-        acc[V - 1] = fmaf(w, u.w, acc[V - 1]);
-      } else {
-        const float2 u = *reinterpret_cast<const float2*>(y);
-        acc[0] = fmaf(w, u.x, acc[0]);
-        acc[1] = fmaf(w, u.y, acc[1]);
-      }
+      float u[V];
+      o_of(j, u);
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = fmaf(w, u[v], acc[v]);
     }
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
