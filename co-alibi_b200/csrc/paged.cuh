@@ -183,10 +183,10 @@ __global__ void __launch_bounds__(kAppendThreads, TURN == kTurnHalves ? 6 : 8) c
 // What must move is K and V, once per kv head: the G * Sq rows that share them go
 // through the tensor cores together.  Up to 32 rows, 16 to a warp with warp-level MMAs (a
 // 128-lane tcgen05 tile would be mostly empty); a CTA has WARPS warps, RW of them side by side
-// over the rows and KG = WARPS / RW over the keys.  With few items four warps share one, with
-// many each RW warps are a CTA of their own, whose starts and ends overlap the others' reads.  Bound by the reads: 4 requests of 65 to 131
-// thousand keys, 4 rows each, 1.61 GB, take 266 us, 6.05 TB/s or 0.92 of the measured copy
-// rate, plus 4 us of joining.
+// over the rows and KG = WARPS / RW over the keys.  Each RW warps are a CTA of their own, whose
+// starts and ends overlap the others' reads; four warps share an item where there is little
+// work.  Bound by the reads: 4 requests of 65 to 131 thousand keys, 4 rows each, 1.61 GB, take
+// 254 us, 0.97 of the measured copy rate (237 of them here, 10 the joining).
 //
 // The work is cut evenly, whatever the lengths: items (request, kv head, block of RW *
 // 16 rows) are laid end to end in units of 32 * KG keys, and each of a grid of resident
@@ -224,16 +224,19 @@ struct PagedLayout {
   // What starting and finishing an item costs, in units: lengths, queries and the first load's
   // latency before its keys, the results after them.  Ragged decoding of 16 requests of 0 .. 8191
   // keys with four warps: 81 us without, 60 / 62 / 65 / 69 us with 2 / 3 / 5 / 8 units of 128
-  // keys; with one warp, beside others on its SM, 57.7 / 58.2 us with 4 / 8 of 32.
+  // keys; with one warp, beside others on its SM, 4 units of 32 do (8: 1% slower).
   static constexpr int COST = KG == 1 ? 4 : 256 / UNIT;
   // Up to this many keys an item is not worth splitting: the joining costs a launch.
   static constexpr int WHOLE = 512;
   static constexpr int ROWS = 16 * RW;
   static constexpr int TILE = kPagedStep * D * 2;  // K or V of one step: [D / 64][32 keys][128 bytes], swizzled
-  static constexpr int NBUF = 3;                   // two steps in flight while one is computed
+  // Ring of steps.  Six CTAs of one warp with one step in flight each read faster than four with
+  // two: long contexts 254 / 280 us, a ragged decode batch 52 / 56 us.
+  static constexpr int NBUF = KG == 1 ? 2 : 3;
   static constexpr int RING = NBUF * 2 * TILE;     // per key group
   static constexpr int BYTES = KG * RING + 1024;   // (the ring starts at a multiple of 1024)
-  static constexpr int CTAS = 200 * 1024 / BYTES < 8 ? 200 * 1024 / BYTES : 8;  // resident per SM
+  // resident per SM: by shared memory, and by 256 registers a thread
+  static constexpr int FIT = 200 * 1024 / BYTES, CTAS = FIT < 256 / THREADS ? FIT : 256 / THREADS;
   static constexpr int RECORD = ROWS * (4 + D);    // floats of one piece: stats, then O
   // the joining of the key groups reuses the ring
   static_assert(16 * RW * D * 4 <= RING, "exchange fits the ring");

@@ -186,12 +186,15 @@ int launch_narrow_of(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnPara
 
 template <int D, bool BF16, int RW, int XR>
 int launch_narrow(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& p, int sms, cudaStream_t s) {
-  // Four warps to an item, or RW where items are plenty, measured (four / one, us a call, 8 kv heads,
-  // 4 rows): 16 requests of 500 keys 11 / 17, 32 of 500 21 / 23, 64 of 500 46 / 31, 256 of 200 92 / 63,
-  // 64 of 1000 67 / 61, 256 of 1000 230 / 195, 8 of 8192 56 / 57.
+  // Four warps to an item where the tables hold little work, else RW to a CTA, measured (four / one,
+  // us a call, 8 kv heads, 4 rows): 1 request of 500 keys 11 / 28, 32 of 500 21 / 29, 1 of 1000 11 / 15,
+  // 8 of 1000 16 / 15, 8 of 1900 21 / 19, 8 of 8192 55 / 52, 64 of 500 46 / 31, 256 of 200 92 / 52,
+  // 256 of 1000 230 / 170; 16 rows, 8 of 8192 63 / 55.
   const int rows = p.Hq / p.Hkv * p.Sq;
   const long long items = (long long)p.B * p.Hkv * ((rows + 16 * RW - 1) / (16 * RW));
-  if (items > 2LL * sms) return launch_narrow_of<D, BF16, RW, XR, RW>(tk, tv, p, sms, s);
+  const long long width = (long long)p.max_pages * p.page_size;
+  if (items > 2LL * sms || (width > 512 && items * width > 32768))
+    return launch_narrow_of<D, BF16, RW, XR, RW>(tk, tv, p, sms, s);
   return launch_narrow_of<D, BF16, RW, XR, 4>(tk, tv, p, sms, s);
 }
 
