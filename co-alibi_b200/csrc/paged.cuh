@@ -1492,7 +1492,7 @@ __global__ void __launch_bounds__(128) coalibi_paged_join_kernel(const PagedAttn
   float M = -INFINITY, l = 0.f, right = 0.f, acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.f;
-  constexpr int EARLY = 4;  // pieces whose O is on its way beside the statistics
+  constexpr int EARLY = 8;  // pieces whose O is on its way beside the statistics (4: 1% slower)
   for (int top = c1; top >= c0; top -= 32) {
     const int n = min(32, top - c0 + 1);
     auto o_of = [&](int j, float* u) {
