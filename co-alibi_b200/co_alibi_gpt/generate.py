@@ -5,6 +5,8 @@ cache; every further step appends its tokens, attends over the cache and samples
 (``generate``), or verifies a tree of drafted tokens at once and keeps the path that
 the samples confirm (``tree_step``).  The reference has no counterpart.
 """
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -18,21 +20,33 @@ __all__ = ["PagedCache", "extend", "generate", "prefill", "tree_step", "tree_wor
 
 class PagedCache:
     """Keys and values of every layer for ``batch`` requests of up to ``max_len`` tokens:
-    pools [n_pages, H, page_size, D], one page table for all layers, and the lengths."""
+    pools [n_pages, H, page_size, D], one page table for all layers, and the lengths.
+    ``spare`` further slots take the drafts of a step that starts near the end: a tree's
+    slots run ahead of its depths, so they may be needed though few are accepted.  In all a
+    request has ``capacity`` slots, every one with its row of the rotary tables."""
 
-    def __init__(self, model, batch, max_len, page_size=64):
+    def __init__(self, model, batch, max_len, page_size=64, spare=TREE_MAX_SQ):
         cfg, weight = model.cfg, model.emb.weight
-        per = -(-max_len // page_size)
+        per = -(-(max_len + spare) // page_size)
+        self.capacity = per * page_size
         shape = (batch * per, cfg.n_head, page_size, cfg.d_model // cfg.n_head)
         self.k = [torch.empty(shape, dtype=weight.dtype, device=weight.device) for _ in range(cfg.n_layer)]
         self.v = [torch.empty_like(k) for k in self.k]
         self.table = torch.arange(batch * per, dtype=torch.int32, device=weight.device).view(batch, per)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=weight.device)
-        self.rotary = rotary_tables(cfg.rotary_dim, max_len, device=weight.device) if cfg.rotary_dim else None
+        self.rotary = rotary_tables(cfg.rotary_dim, self.capacity, device=weight.device) if cfg.rotary_dim else None
+        self.steps = torch.arange(TREE_MAX_SQ, dtype=torch.int32, device=weight.device)
+
+    def missing(self, S):
+        """Which of S tokens behind each request's end have no slot: bool [B, S]."""
+        if S > TREE_MAX_SQ:
+            raise ValueError(f"at most {TREE_MAX_SQ} tokens of a request at once, got {S}")
+        return self.lens[:, None] + self.steps[:S] >= self.capacity
 
     def rows(self, pages, at):
-        """The cached rows of tokens at [B, n] of each request: [B, H, n, D]."""
-        size = pages.shape[2]
+        """The cached rows of tokens at [B, n] of each request: [B, H, n, D]; past the capacity, of
+        its last token (an index outside the table would be a fault on the device)."""
+        size, at = pages.shape[2], at.clamp(max=self.capacity - 1)
         page = self.table.gather(1, (at // size).long()).long()
         return pages[page, :, (at % size).long()].transpose(1, 2)
 
@@ -52,6 +66,8 @@ def prefill(model, cache, tokens, counts=None):
     each prompt's last token, [B, V]."""
     x = model.emb(tokens)
     B, S, C = x.shape
+    if S > cache.capacity and (counts is None or cache.rotary is not None):
+        raise ValueError(f"prompts of {S} tokens, but the cache holds {cache.capacity} of each request")
     for layer, blk in enumerate(model.blocks):
         q, k, v = blk.attn.heads(blk.ln1(x))
         if cache.rotary is not None:
@@ -68,11 +84,14 @@ def prefill(model, cache, tokens, counts=None):
 
 
 @torch.no_grad()
-def extend(model, cache, tokens, words=None, depths=None):
+def extend(model, cache, tokens, words=None, depths=None, counts=None):
     """Logits [B, S, V] of S <= 64 further tokens of each request, appended behind the cache
     (whose lengths stay: the caller says how many of them count).  ``words`` [B, S] int64:
     which of the new tokens each sees (default: those before it and itself);
-    ``depths`` [B, S] int32: their distance from the cache's end, for the rotation."""
+    ``depths`` [B, S] int32: their distance from the cache's end, for the rotation; ``counts``
+    [B] int32: how many enter the cache (default: all).  A token behind the cache's capacity
+    has no key to see itself by: its logits are NaN (``sample_tokens`` draws -1 from them),
+    and the operators report it by ``device_status()`` unless ``counts`` left it out."""
     x = model.emb(tokens)
     B, S, C = x.shape
     positions = None if depths is None else cache.lens[:, None] + depths
@@ -80,12 +99,12 @@ def extend(model, cache, tokens, words=None, depths=None):
         q, k, v = blk.attn.heads(blk.ln1(x))
         where = (cache.k[layer], cache.v[layer], cache.table, cache.lens)
         if cache.rotary is None:
-            append_paged_kv(k, v, *where)
+            append_paged_kv(k, v, *where, count=counts)
         else:
-            q = append_paged_kv(k, v, *where, q=q, rotary=cache.rotary, positions=positions)
+            q = append_paged_kv(k, v, *where, count=counts, q=q, rotary=cache.rotary, positions=positions)
         y = paged_tree_attention(q, *where, tree_mask=words, bias_max=model.cfg.bias_max)
         x = _mlp(blk, x + blk.attn.proj(y.transpose(1, 2).reshape(B, S, C)))
-    return _logits(model, x)
+    return _logits(model, x.masked_fill(cache.missing(S)[..., None], math.nan))
 
 
 def _noise(logits, generator):
@@ -96,7 +115,7 @@ def _noise(logits, generator):
 def generate(model, prompts, max_new_tokens, counts=None, generator=None, page_size=64, **sampling):
     """``max_new_tokens`` tokens for each prompt [B, S], [B, max_new_tokens].  ``sampling``:
     temperature, top_k, top_p and min_p of ``sample_tokens``."""
-    cache = PagedCache(model, prompts.shape[0], prompts.shape[1] + max_new_tokens, page_size)
+    cache = PagedCache(model, prompts.shape[0], prompts.shape[1] + max_new_tokens, page_size, spare=0)
     logits = prefill(model, cache, prompts, counts)
     out = []
     for _ in range(max_new_tokens):
@@ -133,14 +152,18 @@ def tree_step(model, cache, last, drafts, parents, generator=None, **sampling):
     the cache), ``drafts`` [B, T] and ``parents`` [B, T] as in ``tree_words``.  A token is
     sampled after every row; from row 0 on, a draft that equals its parent's sample is
     accepted, and the first sample that no draft matches ends the step.  That draws from the
-    model's own distribution whatever the drafts are.
+    model's own distribution whatever the drafts are.  Drafts behind the cache's capacity count
+    as none: the step ends before them.
 
     Returns (tokens [B, T + 1], n [B] int32): the first n[b] of tokens[b] are new, the last of
-    them becomes ``last``.  The cache then holds every token before it."""
+    them becomes ``last``.  The cache then holds every token before it.  A request whose cache is
+    full already gets n = 0 and tokens of -1, and ``device_status()`` reports it."""
     B, T = drafts.shape
+    missing = cache.missing(T + 1)
+    parents = parents.masked_fill(missing[:, 1:], -1)
     words, depths = tree_words(parents)
     rows = torch.cat((last[:, None], drafts), 1)
-    logits = extend(model, cache, rows, words, depths)
+    logits = extend(model, cache, rows, words, depths, counts=cache.capacity - cache.lens)
     flat = logits.flatten(0, 1)
     per_row = {k: v.repeat_interleave(T + 1) if isinstance(v, torch.Tensor) else v for k, v in sampling.items()}
     sampled = sample_tokens(flat, _noise(flat, generator), **per_row)[0].view(B, T + 1)
@@ -156,6 +179,7 @@ def tree_step(model, cache, last, drafts, parents, generator=None, **sampling):
         path[:, j:j + 1] = at
         tokens[:, j:j + 1] = sampled.gather(1, at)
         n += alive[:, 0].int()
+    n.masked_fill_(missing[:, 0], 0)
     # the accepted rows move together behind the context; they are rotated already, by their depth
     keep = cache.lens[:, None] + path.int()
     for k, v in zip(cache.k, cache.v):
