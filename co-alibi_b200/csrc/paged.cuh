@@ -7,6 +7,7 @@
 #include "sm100.cuh"
 #include "decode.cuh"
 #include "fwd.cuh"
+#include "load_ring.h"
 
 namespace coalibi {
 
@@ -406,10 +407,8 @@ __global__ void __launch_bounds__(32 * WARPS)
   const uint32_t off_k = key_k * 128 + (((mat & 1) ^ (key_k & 7)) << 4);
   const uint32_t off_v = key_v * 128 + (((mat >> 1) ^ (key_v & 7)) << 4);
   constexpr uint32_t kPair = 4 * 128 | 4 << 4;
-  int fill = 0, drain = 0;            // ring slots of the next load and of the next step
-  uint32_t fill_n = 0, drain_n = 0;   // loads issued, steps awaited
-  uint32_t phase = 0;                 // parity of the next step's barrier
-  bool ok = true;                     // no wait has run out
+  LoadRing<L::NBUF> loads;
+  bool ok = true;  // no wait has run out
 
   while (at < stop) {
     // units [u0, u1) of the item; none if the run ends within its overhead
@@ -460,24 +459,24 @@ __global__ void __launch_bounds__(32 * WARPS)
     };
     // the half steps are 16 keys of one page: a box of 64 columns x 16 slots each
     auto load = [&]() {
-      gone_q &= ~(3u << (2 * fill));
-      gone_q |= ((page_id[0] < 0 ? 1u : 0u) | (page_id[1] < 0 ? 2u : 0u)) << (2 * fill);
+      const int slot = loads.fill;
+      gone_q &= ~(3u << (2 * slot));
+      gone_q |= ((page_id[0] < 0 ? 1u : 0u) | (page_id[1] < 0 ? 2u : 0u)) << (2 * slot);
       if (issuer) {
-        const uint32_t dst = smem_u32(ring + fill * 2 * L::TILE);
+        const uint32_t dst = smem_u32(ring + slot * 2 * L::TILE);
         const int halves = (page_id[0] >= 0) + (page_id[1] >= 0);
-        mbar_arrive_expect_tx(&full[fill], halves * L::TILE);
+        mbar_arrive_expect_tx(&full[slot], halves * L::TILE);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           if (page_id[hf] < 0) continue;
 #pragma unroll
           for (int c = 0; c < D / 64; ++c) {
-            tma_load_4d(dst + c * 4096 + hf * 2048, &tk, &full[fill], 64 * c, page_slot[hf], g, page_id[hf]);
-            tma_load_4d(dst + L::TILE + c * 4096 + hf * 2048, &tv, &full[fill], 64 * c, page_slot[hf], g, page_id[hf]);
+            tma_load_4d(dst + c * 4096 + hf * 2048, &tk, &full[slot], 64 * c, page_slot[hf], g, page_id[hf]);
+            tma_load_4d(dst + L::TILE + c * 4096 + hf * 2048, &tv, &full[slot], 64 * c, page_slot[hf], g, page_id[hf]);
           }
         }
       }
-      fill = fill + 1 == L::NBUF ? 0 : fill + 1;
-      ++fill_n;
+      loads.issue();
     };
     auto group_sync = [&]() {
       if (RW == 1)
@@ -528,14 +527,14 @@ __global__ void __launch_bounds__(32 * WARPS)
 
     const float c_a = p.sm_scale * kLog2e;
     for (int st = nsteps - 1; st >= 0; --st) {
-      if (ok && !mbar_wait(&full[drain], phase, guard)) s_fail[kg] = 1;
+      if (ok && !mbar_wait(&full[loads.drain], loads.phase, guard)) s_fail[kg] = st + 1;
       group_sync();  // all are done with step st + 1, whose slot is loaded next
-      ok = s_fail[kg] == 0;  // the same for the group's warps, which meet again in the masked steps
-      const int slot = drain;
-      drain = drain + 1 == L::NBUF ? 0 : drain + 1;
-      if (drain == 0) phase ^= 1;
-      ++drain_n;
+      // the same for the group's warps, which meet again in the masked steps: a wait of this step or
+      // of one before it ran out (one that a faster warp already meets in the next step counts there)
+      ok = s_fail[kg] <= st;
       if (!ok) continue;
+      const int slot = loads.drain;
+      loads.landed();
       if (st - (L::NBUF - 1) >= 0) load();
       lookup(st - L::NBUF);
       const int kb = lo + st * kPagedStep;
@@ -751,14 +750,8 @@ __global__ void __launch_bounds__(32 * WARPS)
         }
       }
     }
-    if (!ok && issuer) {  // a wait ran out: let the loads already issued land before leaving
-      for (; drain_n < fill_n; ++drain_n) {
-        mbar_drain(&full[drain], phase, kPagedTimeoutNs);
-        drain = drain + 1 == L::NBUF ? 0 : drain + 1;
-        if (drain == 0) phase ^= 1;
-      }
-    }
-    if (!ok) drain_n = fill_n;
+    if (!ok && issuer)  // a wait ran out: the loads already issued land before the CTA leaves, below
+      for (; loads.in_flight(); loads.landed()) mbar_drain(&full[loads.drain], loads.phase, kPagedTimeoutNs);
 #pragma unroll
     for (int x = 0; x < XR; ++x) {
       l_part[x] += __shfl_xor_sync(0xffffffffu, l_part[x], 1);
