@@ -55,6 +55,12 @@ def _mlp(blk, x):
     return x + blk.out(F.gelu(blk.fc(blk.ln2(x)), approximate="tanh"))
 
 
+def _embed(model, tokens):
+    """Embeddings; a token below 0 (padding, an absent draft, nothing drawn) takes those of token
+    0, since looking it up would be a fault on the device."""
+    return model.emb(tokens.clamp(min=0))
+
+
 def _logits(model, x):
     return F.linear(model.ln_f(x), model.emb.weight)
 
@@ -64,7 +70,7 @@ def prefill(model, cache, tokens, counts=None):
     """Run prompts [B, S] (``counts`` [B] int32 real tokens each; the rest is padding, which
     causality keeps away from them) and fill the empty cache.  Returns the logits after
     each prompt's last token, [B, V]."""
-    x = model.emb(tokens)
+    x = _embed(model, tokens)
     B, S, C = x.shape
     if S > cache.capacity and (counts is None or cache.rotary is not None):
         raise ValueError(f"prompts of {S} tokens, but the cache holds {cache.capacity} of each request")
@@ -91,8 +97,9 @@ def extend(model, cache, tokens, words=None, depths=None, counts=None):
     ``depths`` [B, S] int32: their distance from the cache's end, for the rotation; ``counts``
     [B] int32: how many enter the cache (default: all).  A token behind the cache's capacity
     has no key to see itself by: its logits are NaN (``sample_tokens`` draws -1 from them),
-    and the operators report it by ``device_status()`` unless ``counts`` left it out."""
-    x = model.emb(tokens)
+    and the operators report it by ``device_status()`` unless ``counts`` left it out.  The
+    logits after a token below 0 are NaN too."""
+    x = _embed(model, tokens)
     B, S, C = x.shape
     positions = None if depths is None else cache.lens[:, None] + depths
     for layer, blk in enumerate(model.blocks):
@@ -104,7 +111,7 @@ def extend(model, cache, tokens, words=None, depths=None, counts=None):
             q = append_paged_kv(k, v, *where, count=counts, q=q, rotary=cache.rotary, positions=positions)
         y = paged_tree_attention(q, *where, tree_mask=words, bias_max=model.cfg.bias_max)
         x = _mlp(blk, x + blk.attn.proj(y.transpose(1, 2).reshape(B, S, C)))
-    return _logits(model, x.masked_fill(cache.missing(S)[..., None], math.nan))
+    return _logits(model, x.masked_fill((cache.missing(S) | (tokens < 0))[..., None], math.nan))
 
 
 def _noise(logits, generator):

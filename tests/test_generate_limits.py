@@ -147,3 +147,29 @@ def test_more_drafts_than_a_word_has_bits_are_refused(monkeypatch):
     cache = gen.PagedCache(model, 1, 16, page_size=16)
     with pytest.raises(ValueError):
         gen.tree_step(model, cache, _tokens(1, 1, "cpu")[:, 0], _tokens(1, 64, "cpu"), torch.arange(64)[None])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_padding_of_minus_one_is_not_looked_up(device, monkeypatch):
+    """Prompts and drafts padded with -1, which no embedding has a row for."""
+    gen = _generate(device, monkeypatch)
+    model = _model(device)
+    counts = torch.tensor([11, 4], dtype=torch.int32, device=device)
+    prompt = _tokens(2, 11, device)
+    prompt[1, 4:] = -1
+    plain = torch.stack([_greedy(model, prompt[b:b + 1, :counts[b]], 4)[0][0] for b in range(2)])
+    cache = gen.PagedCache(model, 2, 32, page_size=16)
+    last = gen.prefill(model, cache, prompt, counts).argmax(-1)
+    drafts = torch.cat((plain[:, 1:3], torch.full_like(plain[:, :2], -1)), 1)
+    parents = torch.tensor([[0, 1, -1, -1]] * 2, device=device)
+    tokens, n = gen.tree_step(model, cache, last, drafts, parents, temperature=0.0)
+    assert n.tolist() == [3, 3] and torch.equal(tokens[:, :3], plain[:, 1:]) and _status(device) == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_model_without_a_token_to_draw_ends_in_minus_one(device, monkeypatch):
+    gen = _generate(device, monkeypatch)
+    model = _model(device)
+    with torch.no_grad():
+        model.ln_f.weight.fill_(float("nan"))
+    assert (gen.generate(model, _tokens(2, 5, device), 3, page_size=16) == -1).all()
