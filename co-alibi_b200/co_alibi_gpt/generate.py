@@ -69,7 +69,8 @@ def _logits(model, x):
 def prefill(model, cache, tokens, counts=None):
     """Run prompts [B, S] (``counts`` [B] int32 real tokens each; the rest is padding, which
     causality keeps away from them) and fill the empty cache.  Returns the logits after
-    each prompt's last token, [B, V]."""
+    each prompt's last token, [B, V]: NaN for a request of no tokens, or of more than the
+    cache holds (of which ``lens`` then counts those that entered)."""
     x = _embed(model, tokens)
     B, S, C = x.shape
     if S > cache.capacity and (counts is None or cache.rotary is not None):
@@ -85,8 +86,11 @@ def prefill(model, cache, tokens, counts=None):
     if counts is None:
         cache.lens += S
         return _logits(model, x[:, -1])
-    cache.lens += counts
-    return _logits(model, x[torch.arange(B, device=x.device), (counts - 1).long()])
+    counts = counts.clamp(0, S)
+    none = (counts == 0) | (counts > cache.capacity)
+    cache.lens += counts.clamp(max=cache.capacity)
+    x = x[torch.arange(B, device=x.device), (counts - 1).clamp(min=0).long()]
+    return _logits(model, x.masked_fill(none[:, None], math.nan))
 
 
 @torch.no_grad()

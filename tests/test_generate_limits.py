@@ -173,3 +173,22 @@ def test_a_model_without_a_token_to_draw_ends_in_minus_one(device, monkeypatch):
     with torch.no_grad():
         model.ln_f.weight.fill_(float("nan"))
     assert (gen.generate(model, _tokens(2, 5, device), 3, page_size=16) == -1).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_counts_outside_the_prompt(device, monkeypatch):
+    """A count past the prompt's width means all of it; a request without tokens has no logits."""
+    gen = _generate(device, monkeypatch)
+    model = _model(device)
+    prompt = _tokens(4, 9, device)
+    counts = torch.tensor([9, 12, 0, -3], dtype=torch.int32, device=device)
+    cache = gen.PagedCache(model, 4, 16, page_size=16)
+    logits = gen.prefill(model, cache, prompt, counts)
+    assert cache.lens.tolist() == [9, 9, 0, 0] and logits[2:].isnan().all() and _status(device) == 0
+    assert torch.equal(logits[:2].argmax(-1), _greedy(model, prompt[:2], 1)[0][:, 0])
+    # with fewer slots than prompt: what entered counts, the rest leaves no logits
+    cache = gen.PagedCache(model, 4, 5, page_size=16, spare=0)
+    wide = _tokens(4, 20, device)
+    logits = gen.prefill(model, cache, wide, torch.tensor([16, 17, 3, 20], dtype=torch.int32, device=device))
+    assert cache.lens.tolist() == [16, 16, 3, 16]
+    assert logits.isnan().any(1).tolist() == [False, True, False, True] and _status(device) != 0
