@@ -126,6 +126,8 @@ def _noise(logits, generator):
 def generate(model, prompts, max_new_tokens, counts=None, generator=None, page_size=64, **sampling):
     """``max_new_tokens`` tokens for each prompt [B, S], [B, max_new_tokens].  ``sampling``:
     temperature, top_k, top_p and min_p of ``sample_tokens``."""
+    if max_new_tokens <= 0:
+        return torch.empty(prompts.shape[0], 0, dtype=torch.int64, device=prompts.device)
     cache = PagedCache(model, prompts.shape[0], prompts.shape[1] + max_new_tokens, page_size, spare=0)
     logits = prefill(model, cache, prompts, counts)
     out = []

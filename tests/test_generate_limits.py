@@ -192,3 +192,9 @@ def test_counts_outside_the_prompt(device, monkeypatch):
     logits = gen.prefill(model, cache, wide, torch.tensor([16, 17, 3, 20], dtype=torch.int32, device=device))
     assert cache.lens.tolist() == [16, 16, 3, 16]
     assert logits.isnan().any(1).tolist() == [False, True, False, True] and _status(device) != 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_no_new_tokens(device, monkeypatch):
+    out = _generate(device, monkeypatch).generate(_model(device), _tokens(3, 5, device), 0)
+    assert out.shape == (3, 0) and out.dtype == torch.int64
