@@ -142,8 +142,8 @@ def generate(model, prompts, max_new_tokens, counts=None, generator=None, page_s
 
 def tree_words(parents):
     """Visibility words [B, T + 1] and depths [B, T + 1] of drafted trees: row 0 is the last
-    accepted token, row 1 + t draft t, hung below row ``parents[b, t]`` <= t (-1: no draft,
-    its word is 0 and nothing of it is read)."""
+    accepted token, row 1 + t draft t, hung below row ``parents[b, t]`` of 0 .. t (else, -1
+    say: no draft, its word is 0 and nothing of it is read)."""
     B, T = parents.shape
     if T + 1 > TREE_MAX_SQ:
         raise ValueError(f"at most {TREE_MAX_SQ - 1} drafted tokens, got {T}")
@@ -153,9 +153,9 @@ def tree_words(parents):
     for t in range(T):
         up = parents[:, t:t + 1].long()
         bit = (1 << (t + 1)) if t + 1 < 63 else -(1 << 63)
-        here = up >= 0
-        words[:, t + 1:t + 2] = torch.where(here, words.gather(1, up.clamp(min=0)) | bit, 0)
-        depths[:, t + 1:t + 2] = torch.where(here, depths.gather(1, up.clamp(min=0)) + 1, 0)
+        here, up = (up >= 0) & (up <= t), up.clamp(0, t)
+        words[:, t + 1:t + 2] = torch.where(here, words.gather(1, up) | bit, 0)
+        depths[:, t + 1:t + 2] = torch.where(here, depths.gather(1, up) + 1, 0)
     return words, depths
 
 
@@ -173,7 +173,7 @@ def tree_step(model, cache, last, drafts, parents, generator=None, **sampling):
     full already gets n = 0 and tokens of -1, and ``device_status()`` reports it."""
     B, T = drafts.shape
     missing = cache.missing(T + 1)
-    parents = parents.masked_fill(missing[:, 1:], -1)
+    parents = parents.masked_fill(missing[:, 1:] | (parents > cache.steps[:T]), -1)
     words, depths = tree_words(parents)
     rows = torch.cat((last[:, None], drafts), 1)
     logits = extend(model, cache, rows, words, depths, counts=cache.capacity - cache.lens)

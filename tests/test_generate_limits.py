@@ -198,3 +198,22 @@ def test_counts_outside_the_prompt(device, monkeypatch):
 def test_no_new_tokens(device, monkeypatch):
     out = _generate(device, monkeypatch).generate(_model(device), _tokens(3, 5, device), 0)
     assert out.shape == (3, 0) and out.dtype == torch.int64
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_parent_that_does_not_come_before_its_draft_is_none(device, monkeypatch):
+    """Row numbers of parents past the draft's own, past the tree, or of an absent draft: such a
+    draft sees nothing and is not accepted, and no index leaves the tree."""
+    gen = _generate(device, monkeypatch)
+    words, depths = gen.tree_words(torch.tensor([[1, 0, 99, 2, -7]]))
+    assert words.tolist() == [[1, 0, 0b101, 0, 0b10101, 0]] and depths.tolist() == [[0, 0, 1, 0, 2, 0]]
+    model = _model(device)
+    prompt = _tokens(1, 12, device)
+    plain, _ = _greedy(model, prompt, 5)
+    cache = gen.PagedCache(model, 1, 32, page_size=16)
+    last = gen.prefill(model, cache, prompt).argmax(-1)
+    drafts = plain[:, [1, 1, 2, 2, 3]]
+    for parents, accepted in (([2, 0, 99, 2, 4], 3), ([2, 99, 0, 3, 1], 0), ([5, 1, 1, 1, 1], 0)):
+        cache.lens.fill_(12)
+        tokens, n = gen.tree_step(model, cache, last, drafts, torch.tensor([parents], device=device), temperature=0.0)
+        assert n.tolist() == [accepted + 1] and torch.equal(tokens[0, :accepted + 1], plain[0, 1:accepted + 2])
