@@ -17,6 +17,10 @@ pool works too; page_size a multiple of 16) and an int32 ``page_table``
 there: calls launch on the current stream, never synchronise, and can be captured in a
 CUDA graph.  A token whose page is outside the pool, or past the table, is skipped and
 reported by ``device_status()`` as code 11.
+
+There is no backward: where gradients are enabled, keys, values, queries and pools that
+require one are refused (call under ``torch.no_grad()``), and log-probabilities of sampled
+tokens carry none.  Appending counts as an in-place write of the pools for autograd.
 """
 import torch
 

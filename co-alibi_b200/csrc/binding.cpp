@@ -7,6 +7,7 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -55,6 +56,18 @@ int dtype_any(const Tensor& t) { return t.scalar_type() == at::kFloat ? COALIBI_
 
 void on(const char* what, const char* name, const Tensor& t, c10::Device device) {
   if (t.device() != device) refuse(PyExc_ValueError, what, name, " is on ", t.device().str(), ", not ", device.str());
+}
+
+// The operators have no backward: a result that silently dropped its graph would train wrongly.
+void no_grad(const char* what, const char* name, const Tensor& t) {
+  if (c10::GradMode::is_enabled() && t.requires_grad())
+    refuse(PyExc_RuntimeError, what, name, " requires grad, but there is no backward: call this under torch.no_grad()");
+}
+
+// As after torch's own in-place operations, a backward over a saved t fails instead of reading the
+// new values.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 // The first three strides of [., ., ., D], 0 for a dimension of one entry.
@@ -145,12 +158,14 @@ PyObject* append_paged_kv(PyObject* const* a) {
   check_cache(what, kp, vp, table, B, D, dtype, device);
   if (kp.size(1) != Hkv) refuse(PyExc_ValueError, what, "the cache has ", kp.size(1), " kv heads, k ", Hkv);
   on(what, "v", v0, device);
+  no_grad(what, "k", k0), no_grad(what, "v", v0), no_grad(what, "k_pages", kp), no_grad(what, "v_pages", vp);
   Tensor q, q_out, start, count, positions, cos, sin;
   if (with_q) {
     q = THPVariable_Unpack(a[7]);
     if (q.dim() != 4 || q.size(0) != B || q.size(2) != S || q.size(3) != D)
       refuse(PyExc_ValueError, what, "q must be [", B, ", Hq, ", S, ", ", D, "], got ", shape_of(q));
     on(what, "q", q, device);
+    no_grad(what, "q", q);
     q = aligned_rows(q.detach());
     q_out = at::empty_like(q);
     p.Hq = (int)q.size(1);
@@ -210,6 +225,7 @@ PyObject* append_paged_kv(PyObject* const* a) {
     p.interleaved = truth;
     if (with_q && p.Hq == 0) p.q = nullptr, p.q_out = nullptr;
     check(coalibi_paged_append(&p, stream_of(device)), "coalibi_paged_append");
+    written(kp), written(vp);
   }
   if (!with_q) Py_RETURN_NONE;
   return THPVariable_Wrap(q_out);
@@ -249,6 +265,8 @@ PyObject* paged_tree_attention(PyObject* const* a) {
   if (slopes0.dim() != 1 || slopes0.size(0) != Hq)
     refuse(PyExc_ValueError, what, "slopes must have shape [", Hq, "], got ", shape_of(slopes0));
   on(what, "slopes", slopes0, device);
+  no_grad(what, "q", q0), no_grad(what, "k_pages", kp), no_grad(what, "v_pages", vp);
+  no_grad(what, "slopes", slopes0);
   p.sm_scale = (float)(1.0 / std::sqrt((double)D));
   if (a[6] != Py_None) {
     const double s = PyFloat_AsDouble(a[6]);
