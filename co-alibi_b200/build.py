@@ -4,7 +4,9 @@ serving operators (_serving, C++ over PyTorch's headers) that links it.
     python co-alibi_b200/build.py [--force] [--verbose]
 
 Both land in co-alibi_b200/co_alibi_attn/ next to the Python package that loads
-them.  Each is rebuilt only when a source is newer than it.
+them.  Each is rebuilt only when a source is newer than it.  The library needs nvcc alone;
+where PyTorch (with CUDA), Python's headers or a C++ compiler are missing, the binding is
+left out with a note, and the serving operators' Python calls say so.
 """
 import argparse
 import glob
@@ -52,10 +54,36 @@ def needs_build():
     return any(os.path.getmtime(s) > t for s in sources())
 
 
-def build(force=False, verbose=False):
+def build(force=False, verbose=False, binding=None):
+    """Returns the library's path.  ``binding``: True to fail where it cannot be built."""
     build_library(force, verbose)
-    build_binding(force, verbose)
+    missing = binding_lacks()
+    if not missing:
+        build_binding(force, verbose)
+    elif binding:
+        raise RuntimeError(f"the binding of the serving operators needs {missing}")
+    else:
+        sys.stderr.write(f"build.py: the binding of the serving operators is left out: it needs {missing}\n")
     return OUT
+
+
+def binding_lacks():
+    """What the binding needs and this machine has not, or None."""
+    try:
+        import torch
+    except ImportError as e:
+        return f"PyTorch ({e})"
+    if not glob.glob(os.path.join(os.path.dirname(torch.__file__), "lib", "*c10_cuda*")):
+        return "PyTorch with CUDA"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python's headers (Python.h)"
+    if shutil.which(cxx_path()) is None:
+        return f"a C++ compiler ({cxx_path()} not found)"
+    return None
+
+
+def cxx_path():
+    return os.environ.get("CXX", "g++")
 
 
 def _run(cmd, verbose, what):
@@ -91,7 +119,7 @@ def build_binding(force=False, verbose=False):
            os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include"), INCLUDE]
     lib = os.path.join(home, "lib")
     tmp = BINDING + ".tmp"
-    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+    _run([cxx_path(), "-O2", "-std=c++17", "-fPIC", "-shared",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *sum((["-isystem", i] for i in inc), []),
           BINDING_SRC, "-o", tmp, "-L", PKG, "-l:libcoalibi_sm100.so", "-Wl,-rpath,$ORIGIN", "-L", lib,
           f"-Wl,-rpath,{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"],
