@@ -37,6 +37,22 @@ def rotate_heads(x, cos, sin):
     return torch.cat(((a * cos - b * sin).to(x.dtype), (b * cos + a * sin).to(x.dtype), x[..., 2 * r:]), -1)
 
 
+_rotary_cache = {}
+
+
+def _rotary(rotary_dim, seq_len, S, device):
+    """cos and sin of the first S positions, of tables that are built once per device for
+    ``seq_len`` positions and again when a longer input comes: building them copies from
+    the host, which stalls the stream and cannot be captured in a CUDA graph."""
+    key = (rotary_dim, device)
+    tables = _rotary_cache.get(key)
+    if tables is None or tables[0].shape[0] < S:
+        from co_alibi_attn import serving
+        tables = serving.rotary_tables(rotary_dim, max(S, seq_len), device=device)
+        _rotary_cache[key] = tables
+    return tables[0][:S], tables[1][:S]
+
+
 class CoALiBiSelfAttention(nn.Module):
     """QKV projection, Co-ALiBi causal attention over [B, H, S, D] heads, output projection."""
 
@@ -50,6 +66,7 @@ class CoALiBiSelfAttention(nn.Module):
         self.attn_fn = attn_fn
         self.bias_max = cfg.bias_max
         self.rotary_dim = cfg.rotary_dim
+        self.seq_len = cfg.seq_len
 
     def heads(self, x):
         """Queries, keys and values of x [B, S, C] as [B, H, S, D] views of the fused projection."""
@@ -62,8 +79,7 @@ class CoALiBiSelfAttention(nn.Module):
         # contiguous: the kernels take row-major heads
         q, k, v = (t.contiguous() for t in self.heads(x))
         if self.rotary_dim:
-            from co_alibi_attn.serving import rotary_tables
-            cos, sin = rotary_tables(self.rotary_dim, S, device=x.device)
+            cos, sin = _rotary(self.rotary_dim, self.seq_len, S, x.device)
             q, k = rotate_heads(q, cos, sin), rotate_heads(k, cos, sin)
         y = self.attn_fn(q, k, v, causal=True, bias_max=self.bias_max)
         return self.proj(y.transpose(1, 2).reshape(B, S, C))
