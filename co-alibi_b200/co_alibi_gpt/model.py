@@ -26,7 +26,7 @@ class GPTConfig:
     mlp_ratio: int = 4
     bias_max: float = 8.0
     init_std: float = 0.02
-    rotary_dim: int = 0  # first elements of each query and key head rotated by position (0: none)
+    rotary_dim: int = 0  # first elements of each query and key head rotated by position (0: none); a multiple of 16
 
 
 def rotate_heads(x, cos, sin):
@@ -61,6 +61,8 @@ class CoALiBiSelfAttention(nn.Module):
         assert cfg.d_model % cfg.n_head == 0
         self.n_head = cfg.n_head
         self.head_dim = cfg.d_model // cfg.n_head
+        if not 0 <= cfg.rotary_dim <= self.head_dim or cfg.rotary_dim % 16:  # as append_paged_kv takes it
+            raise ValueError(f"rotary_dim must be a multiple of 16 up to the head width {self.head_dim}, got {cfg.rotary_dim}")
         self.qkv = nn.Linear(cfg.d_model, 3 * cfg.d_model)
         self.proj = nn.Linear(cfg.d_model, cfg.d_model)
         self.attn_fn = attn_fn

@@ -52,3 +52,11 @@ def test_a_training_step_can_be_captured():
     assert (loss - want[0]).abs() <= 2e-3
     for g, w in zip(grads, want[1]):
         assert (g.float() - w.float()).abs().max() <= 1e-2 * w.float().abs().max() + 1e-6
+
+
+@pytest.mark.parametrize("rotary_dim", [-16, 8, 24, 33, 80])
+def test_widths_that_the_cache_does_not_take_are_refused(rotary_dim):
+    from co_alibi_gpt import CoALiBiGPT
+    with pytest.raises(ValueError):
+        CoALiBiGPT(_cfg(rotary_dim=rotary_dim), oracle_attention)
+    CoALiBiGPT(_cfg(rotary_dim=64), oracle_attention)
