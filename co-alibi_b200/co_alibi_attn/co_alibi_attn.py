@@ -58,7 +58,8 @@ def _api_slopes(n_heads, bias_max, dtype, device):
     key = (n_heads, float(bias_max), dtype, device)
     t = _slope_cache.get(key)
     if t is None:
-        t = (2.0 * _get_coalibi_slopes(n_heads, bias_max)).to(device, dtype=dtype)
+        with torch.inference_mode(False):  # an inference tensor could not be saved for a backward later
+            t = (2.0 * _get_coalibi_slopes(n_heads, bias_max)).to(device, dtype=dtype)
         with _cache_lock:
             _slope_cache[key] = t
     return t
@@ -78,7 +79,8 @@ def device_status(device=None, reset=False) -> int:
 def _status_word(device):
     t = _status_cache.get(device)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # (device_status() resets it in any mode)
+            t = torch.zeros(1, dtype=torch.int32, device=device)
         with _cache_lock:
             _status_cache[device] = t
     return t
