@@ -54,10 +54,19 @@ def _ev():
     return torch.cuda.Event(enable_timing=True)
 
 
+def _not_capturing(device, what):
+    """What is built on first use and kept must not be built inside a CUDA graph capture: the
+    values would be written by each replay, or copied from the host, which cannot be captured."""
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"co_alibi_attn: {what} is built by the first call on {device}, which a CUDA graph cannot "
+                           "capture; run the call once before the capture")
+
+
 def _api_slopes(n_heads, bias_max, dtype, device):
     key = (n_heads, float(bias_max), dtype, device)
     t = _slope_cache.get(key)
     if t is None:
+        _not_capturing(device, f"the slope table of {n_heads} heads")
         with torch.inference_mode(False):  # an inference tensor could not be saved for a backward later
             t = (2.0 * _get_coalibi_slopes(n_heads, bias_max)).to(device, dtype=dtype)
         with _cache_lock:
@@ -79,6 +88,7 @@ def device_status(device=None, reset=False) -> int:
 def _status_word(device):
     t = _status_cache.get(device)
     if t is None:
+        _not_capturing(device, "the status word")
         with torch.inference_mode(False):  # (device_status() resets it in any mode)
             t = torch.zeros(1, dtype=torch.int32, device=device)
         with _cache_lock:

@@ -15,7 +15,8 @@ pool works too; page_size a multiple of 16) and an int32 ``page_table``
 [B, max_pages]: token t of request b is slot ``t % page_size`` of page
 ``page_table[b, t // page_size]``.  Lengths and tables live on the device and are read
 there: calls launch on the current stream, never synchronise, and can be captured in a
-CUDA graph.  A token whose page is outside the pool, or past the table, is skipped and
+CUDA graph, after one call outside (the first on a device, or of a number of heads, builds
+what is kept, and a capture refuses it).  A token whose page is outside the pool, or past the table, is skipped and
 reported by ``device_status()`` as code 11.
 
 There is no backward: where gradients are enabled, keys, values, queries and pools that

@@ -48,6 +48,8 @@ def _rotary(rotary_dim, seq_len, S, device):
     tables = _rotary_cache.get(key)
     if tables is None or tables[0].shape[0] < S:
         from co_alibi_attn import serving
+        from co_alibi_attn.co_alibi_attn import _not_capturing
+        _not_capturing(device, f"the rotary table of {S} positions")
         with torch.inference_mode(False):  # kept for training too
             tables = serving.rotary_tables(rotary_dim, max(S, seq_len), device=device)
         _rotary_cache[key] = tables

@@ -37,3 +37,28 @@ def test_first_calls_in_inference_mode(monkeypatch):
     out = co_alibi_attn.co_alibi_attention(q2, k, v)
     out.sum().backward()
     assert torch.equal(out, o) and torch.isfinite(q2.grad).all()
+
+
+@pytest.mark.gpu
+def test_first_calls_inside_a_capture_are_refused(monkeypatch):
+    import co_alibi_attn
+    from co_alibi_attn import append_paged_kv, co_alibi_attention, paged_tree_attention
+    z = lambda *s, dt=torch.float16: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    k, pages, table, lens = z(1, 2, 1, 64), z(3, 2, 16, 64), z(1, 1, dt=torch.int32), z(1, dt=torch.int32)
+    x = z(1, 2, 40, 64)
+    calls = (lambda: append_paged_kv(k, k, pages, pages.clone(), table, lens),
+             lambda: paged_tree_attention(k, pages, pages, table, lens, slopes=z(2)),
+             lambda: paged_tree_attention(k, pages, pages, table, lens),
+             lambda: co_alibi_attention(x, x, x))
+    for call in calls:
+        core, _ = _fresh(monkeypatch)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        assert not core._status_cache and not core._slope_cache
+        call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        graph.replay()
+        assert co_alibi_attn.device_status(reset=True) == 0
