@@ -174,6 +174,10 @@ __device__ __forceinline__ T block_exclusive(T v, T* warp_sums, T& total) {
   return left + inc - v;
 }
 
+// 1 / T, held to normal numbers: 0 * infinity would be NaN, for the largest logit at the smallest
+// temperatures and for masked ones at an infinite one.
+__device__ __forceinline__ float inverse_temperature(float t) { return fminf(fmaxf(1.f / t, 0x1p-126f), 0x1p126f); }
+
 // Weights and distances of a row.
 struct SampleScale {
   float mx, inv_t, k2;
@@ -434,7 +438,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
   const int top_k = p.top_k ? p.top_k[b] : p.top_k_all;
   const bool greedy = !(t > 0.f), by_k = top_k > 0 && top_k < p.V;
   SampleScale sc;
-  sc.inv_t = greedy ? 0.f : 1.f / t;
+  sc.inv_t = greedy ? 0.f : inverse_temperature(t);
   sc.k2 = sc.inv_t * kLog2e;
 
   if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -968,7 +972,7 @@ __global__ void __launch_bounds__(kStreamThreads, 4) coalibi_sample_stream_kerne
   grid_dep_wait();
   const float t = p.temperature ? p.temperature[b] : p.temperature_all;
   const bool greedy = !(t > 0.f);
-  const float inv_t = greedy ? 1.f : 1.f / t, k2 = inv_t * kLog2e;
+  const float inv_t = greedy ? 1.f : inverse_temperature(t), k2 = inv_t * kLog2e;
   const int skip = (int)(reinterpret_cast<uintptr_t>(lrow) & 15) / SIZE;
   const char* base = lrow - (size_t)skip * SIZE;
   const int chunks = (p.V + skip + EPC - 1) / EPC, per = (chunks + C - 1) / C;
