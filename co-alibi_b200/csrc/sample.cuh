@@ -684,12 +684,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
 
   // ---- the race.  Only a token whose quick weight comes within 1e-4 of beating `bound`, the best
   // that its CTA has seen (the quick weight's error is below 2e-5), gets an exact weight and
-  // division; the first token's own score is the bound to start from.
+  // division; the first token's own score is the bound to start from.  The bound stays finite: after
+  // a random number of 0, tokens of another such number still enter, and the lowest index wins.
   float score = 0.f;
   int token = 0x7fffffff;
   double rest = 0.0;
   const float e_first = nrow[first];
-  float bound = e_first > 0.f ? 1.f / e_first : 0.f, near = bound * 0.9999f;
+  constexpr float kMost = 3.402823466e38f;
+  float bound = e_first > 0.f ? fminf(1.f / e_first, kMost) : 0.f, near = bound * 0.9999f;
   auto enter = [&](int i, float x, float w, float e) {
     if (w > near * e) {
       const float y = expf(sc.dist(x)) / e;
@@ -721,7 +723,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) coalibi_sample_kernel(const
         for (int q = 0; q < EPC; ++q) enter(i0 + q, x[q], w[q], e[q]);
       }
       __syncwarp();
-      bound = fmaxf(bound, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(score))));
+      bound = fmaxf(bound, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fminf(score, kMost)))));
       if ((tid & 31) == 0) atomicMax(&s.bound, __float_as_uint(bound));
       near = bound * 0.9999f;
     }
