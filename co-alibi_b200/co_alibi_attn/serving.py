@@ -73,7 +73,7 @@ def append_paged_kv(k, v, k_pages, v_pages, page_table, start, count=None, q=Non
     tables at the token's position, or at ``positions`` (int32 [B, S]; a drafted tree's
     tokens sit at their depth, not at their slot).  With ``q`` [B, Hq, S, D] the queries
     are rotated in the same launch and returned (rows past ``count`` are zero); without,
-    None is returned."""
+    None is returned.  Rotations are float32, rounded once; all else is moved as it is."""
     assert k.is_cuda, "Inputs must be CUDA tensors"
     return _native().append_paged_kv(k, v, k_pages, v_pages, page_table, start, count, q, rotary, interleaved,
                                      positions, _status_word(k.device))
@@ -94,7 +94,11 @@ def paged_tree_attention(q, k_pages, v_pages, page_table, ctx_lens, tree_mask=No
     Per row: p = sm_scale * q.k, z_j = the sum of sigmoid(p) over the keys the row sees at
     j and after it in cache order, o = softmax(p - slope * z) V; scale, slopes and
     ``bias_max`` as in ``co_alibi_attention`` (``slopes`` [Hq] replaces its table, e.g. for
-    a head shard).  Returns [B, Hq, Sq, D]; a row that sees nothing is zero."""
+    a head shard).  Returns [B, Hq, Sq, D]; a row that sees nothing is zero.
+
+    Scores, sigmoid sums, softmax statistics and the result's sums are float32 (with the
+    hardware's approximate exponential and reciprocal); the weights are rounded to the
+    inputs' type for the product with V, as in ``co_alibi_attention``."""
     assert q.is_cuda, "Inputs must be CUDA tensors"
     if slopes is None:
         slopes = _api_slopes(q.shape[1], bias_max, q.dtype, q.device)
@@ -116,6 +120,7 @@ def sample_tokens(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
     int32).  Logits of -inf or NaN are never drawn; a row of nothing else gives token -1.
 
     Returns (tokens int64 [B], logprobs float32 [B]: the drawn token's log-probability
-    among the kept)."""
+    among the kept).  Weights are float32 with a relative error of up to 2e-5: a token whose
+    weight, or the mass before it, lies that close to a limit may fall on either side of it."""
     assert logits.is_cuda, "Inputs must be CUDA tensors"
     return _native().sample_tokens(logits, noise, temperature, top_k, top_p, min_p)

@@ -27,7 +27,9 @@ __device__ __forceinline__ void report_page(int* status) {
 // pieces (8 elements).  A thread keeps its column, so it loads a token's angles once for all
 // heads and needs no division per piece (with one the same prompts took 77 us); 32 registers
 // leave 8 CTAs to an SM (at 4: 60 us).  A rotated piece also needs its partner's 8 elements
-// (half layout) or none (interleaved); the partner is in the same row and hits L1.
+// (half layout) or none (interleaved); the partner is in the same row and hits L1.  The half
+// layout's partners and second set of angles take 40 registers and leave 6: prompts whose whole
+// heads turn so take 55 us (floor 41), the same without rotation, keys and values alone, 17.
 // ---------------------------------------------------------------------------
 struct AppendParams {
   const void* k;
@@ -733,7 +735,8 @@ __global__ void __launch_bounds__(32 * WARPS)
         group_sync();
       }
       // ---- O += P V: the C fragments of two key tiles are the A fragment of one k-step.
-      // P is rounded to the inputs' type for the product; l sums it unrounded.
+      // P is rounded to the inputs' type, which the MMA takes; l sums it unrounded (half an ulp of
+      // each weight, averaging out over the keys).
 #pragma unroll
       for (int k2 = 0; k2 < 2; ++k2) {
         uint32_t pa[4];
@@ -861,14 +864,23 @@ __global__ void __launch_bounds__(32 * WARPS)
 // step needs an exchange between threads.  Pieces join at the item's end as above.  Bound by
 // the reads in long items (8 requests of 8192 keys, 64 rows, 268 MB: 63 us, 4.3 TB/s; each
 // further 1000 keys per SM cost 13 us, 5.8 TB/s) and by an item's start and end, about 10 us.
+// More rows share the reads but not the exponentials: 8 requests of 127 to 16383 keys, 8 kv heads,
+// take 76 us with 64 rows, 104 with 128 and 184 with 256 (two blocks of rows, each reading all keys).
+//
+// P is 16-bit, as the MMA takes it, while l sums the weights unrounded: an error of half an ulp of
+// each weight that averages out over the keys, at half the bytes of TMEM and of the instruction's
+// operands.  Where the reference moves between the halves of a step, the right half's weights, rounded
+// already, are scaled and rounded again (only when a logit passes it by 8 in log2 units, and the other way is to hold
+// 32 floats more); the drafts that are added by hand take the weight as rounded, like the others of their row.
 // ---------------------------------------------------------------------------
 template <int D, bool DUP>
 struct WideLayout {
   static constexpr int PIECES = DUP ? 4 : 2;       // of an item, per CTA
   static constexpr int STEP = DUP ? 32 : 64;       // keys of a piece per step
   static constexpr int UNIT = 128;
-  // As above: trees of 16 drafts over 127 .. 16383 keys take 132 us with 3 units, 79 with 7, 70 with
-  // 9 to 11, 71 with 14 (an item's queries, first loads, exchange and joining take about 10 us).
+  // As above: trees of 16 drafts over 127 .. 16383 keys took 132 us with 3 units, 79 with 7, 70 with
+  // 9 to 11, 71 with 14, in one run on one GPU (an item's queries, first loads, exchange and joining take
+  // about 10 us; 75 to 76 is usual).
   static constexpr int COST = 10;
   static constexpr int WHOLE = 1024;  // 32 requests of 500 / 1000 keys, 8 kv heads: 43 / 52 us, split 50 / 59
   static constexpr int ROWS = DUP ? 64 : 128;
@@ -1071,7 +1083,7 @@ __global__ void __launch_bounds__(384, 1)
                                                 (g * G + row / p.Sq) * p.qs[1] + (row % p.Sq) * p.qs[2] + ch * 8);
         *reinterpret_cast<uint4*>(smem + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = val;
       }
-      // O starts at zero; so do the columns of P that this thread's lane never fills
+      // O starts at zero
       const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
       uint32_t zero[32];
 #pragma unroll

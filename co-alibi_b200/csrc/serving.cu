@@ -189,7 +189,9 @@ int launch_narrow(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams&
   // Four warps to an item where the tables hold little work, else RW to a CTA, measured (four / one,
   // us a call, 8 kv heads, 4 rows): 1 request of 500 keys 11 / 28, 32 of 500 21 / 29, 1 of 1000 11 / 15,
   // 8 of 1000 16 / 15, 8 of 1900 21 / 19, 8 of 8192 55 / 52, 64 of 500 46 / 31, 256 of 200 92 / 52,
-  // 256 of 1000 230 / 170; 16 rows, 8 of 8192 63 / 55.
+  // 256 of 1000 230 / 170; 16 rows, 8 of 8192 63 / 55.  The host sees the tables' width alone, which
+  // was the longest request's in all of these: under a table of 2048 or 8192 keys 1 request of 37
+  // (12 heads of 64) takes 12.1 us a call, 9.4 under one of 48; 16 of 0 .. 8191 under one of 32768 the same 52.
   const int rows = p.Hq / p.Hkv * p.Sq;
   const long long items = (long long)p.B * p.Hkv * ((rows + 16 * RW - 1) / (16 * RW));
   const long long width = (long long)p.max_pages * p.page_size;
@@ -211,7 +213,7 @@ int launch_paged_rows(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnPar
   // Warp-level MMAs up to 32 rows, tcgen05 from there, measured (warp level / tcgen05, us a call):
   // 32 rows, 8 requests of 8192 keys, 8 kv heads 68 / 67; 32 rows, 32 requests of 500 keys 33 / 37;
   // 24 rows of D = 64, 8 requests of 4000 keys, 12 heads 38 / 53; 16 rows, 8 of 8192 62 / 66;
-  // 64 rows, 8 requests of 127 to 16383 keys 120 / 70.
+  // 64 rows, 8 requests of 127 to 16383 keys 120 / 75.
   if (rows <= 8) return launch_narrow<D, BF16, 1, 1>(tk, tv, p, sms, s);
   if (rows <= 16) return launch_narrow<D, BF16, 1, 2>(tk, tv, p, sms, s);
   if (rows <= 32) return launch_narrow<D, BF16, 2, 2>(tk, tv, p, sms, s);

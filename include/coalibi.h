@@ -290,8 +290,10 @@ int coalibi_paged_attention(const CoalibiPagedAttentionArgs* args, void* workspa
  * renormalised distribution.  temperature <= 0: the first of the ranking.  Logits of
  * -inf or NaN are never drawn; +inf logits share all the weight.  logprobs[b] is the
  * drawn token's log-probability among the kept.  A row with nothing to draw gives
- * token -1, logprob -inf.  Sums are exact in 64-bit fixed point: results repeat bit
- * for bit. */
+ * token -1, logprob -inf.  The masses that top_p cuts are 64-bit fixed point (weights
+ * in units of 2^-31, so that the order of atomics does not matter); the sum behind logprobs
+ * adds float32 weights, in double across chunks and in a fixed order.  Results repeat bit for
+ * bit. */
 #define COALIBI_SAMPLE_MAX_VOCAB (1 << 21)
 typedef struct CoalibiSampleArgs {
   const void* logits;       /* [B, V], row stride logits_stride elements */
