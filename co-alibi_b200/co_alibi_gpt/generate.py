@@ -36,19 +36,24 @@ class PagedCache:
         self.lens = torch.zeros(batch, dtype=torch.int32, device=weight.device)
         self.rotary = rotary_tables(cfg.rotary_dim, self.capacity, device=weight.device) if cfg.rotary_dim else None
         self.steps = torch.arange(TREE_MAX_SQ, dtype=torch.int32, device=weight.device)
+        self.limits = self.capacity - self.steps
 
     def missing(self, S):
         """Which of S tokens behind each request's end have no slot: bool [B, S]."""
         if S > TREE_MAX_SQ:
             raise ValueError(f"at most {TREE_MAX_SQ} tokens of a request at once, got {S}")
-        return self.lens[:, None] + self.steps[:S] >= self.capacity
+        return self.lens[:, None] >= self.limits[:S]
+
+    def where(self, at):
+        """Page and slot of the tokens at [B, n] of each request; past the capacity, of its last one
+        (an index outside the table would be a fault on the device)."""
+        size, at = self.k[0].shape[2], at.clamp(max=self.capacity - 1)
+        return self.table.gather(1, (at // size).long()).long(), (at % size).long()
 
     def rows(self, pages, at):
-        """The cached rows of tokens at [B, n] of each request: [B, H, n, D]; past the capacity, of
-        its last token (an index outside the table would be a fault on the device)."""
-        size, at = pages.shape[2], at.clamp(max=self.capacity - 1)
-        page = self.table.gather(1, (at // size).long()).long()
-        return pages[page, :, (at % size).long()].transpose(1, 2)
+        """The cached rows of tokens at [B, n] of each request: [B, H, n, D]."""
+        page, slot = self.where(at)
+        return pages[page, :, slot].transpose(1, 2)
 
 
 def _mlp(blk, x):
@@ -94,7 +99,7 @@ def prefill(model, cache, tokens, counts=None):
 
 
 @torch.no_grad()
-def extend(model, cache, tokens, words=None, depths=None, counts=None):
+def extend(model, cache, tokens, words=None, depths=None, counts=None, missing=None):
     """Logits [B, S, V] of S <= 64 further tokens of each request, appended behind the cache
     (whose lengths stay: the caller says how many of them count).  ``words`` [B, S] int64:
     which of the new tokens each sees (default: those before it and itself);
@@ -102,7 +107,16 @@ def extend(model, cache, tokens, words=None, depths=None, counts=None):
     [B] int32: how many enter the cache (default: all).  A token behind the cache's capacity
     has no key to see itself by: its logits are NaN (``sample_tokens`` draws -1 from them),
     and the operators report it by ``device_status()`` unless ``counts`` left it out.  The
-    logits after a token below 0 are NaN too."""
+    logits after a token below 0 are NaN too.  ``missing``: ``cache.missing(S)`` where the
+    caller has it."""
+    if missing is None:
+        missing = cache.missing(tokens.shape[1])
+    x = _extend(model, cache, tokens, words, depths, counts)
+    return _logits(model, x.masked_fill((missing | (tokens < 0))[..., None], math.nan))
+
+
+def _extend(model, cache, tokens, words=None, depths=None, counts=None):
+    """The last layer's output of ``extend``."""
     x = _embed(model, tokens)
     B, S, C = x.shape
     positions = None if depths is None else cache.lens[:, None] + depths
@@ -115,7 +129,7 @@ def extend(model, cache, tokens, words=None, depths=None, counts=None):
             q = append_paged_kv(k, v, *where, count=counts, q=q, rotary=cache.rotary, positions=positions)
         y = paged_tree_attention(q, *where, tree_mask=words, bias_max=model.cfg.bias_max)
         x = _mlp(blk, x + blk.attn.proj(y.transpose(1, 2).reshape(B, S, C)))
-    return _logits(model, x.masked_fill((cache.missing(S) | (tokens < 0))[..., None], math.nan))
+    return x
 
 
 def _noise(logits, generator):
@@ -135,9 +149,10 @@ def generate(model, prompts, max_new_tokens, counts=None, generator=None, page_s
         token, _ = sample_tokens(logits, _noise(logits, generator), **sampling)
         out.append(token)
         if len(out) < max_new_tokens:
-            logits = extend(model, cache, token[:, None])[:, 0]
+            logits = _logits(model, _extend(model, cache, token[:, None])[:, 0])  # (the cache has room for all)
             cache.lens += 1
-    return torch.stack(out, 1)
+    out = torch.stack(out, 1)
+    return out.masked_fill((out < 0).cummax(1)[0], -1)  # nothing follows where nothing could be drawn
 
 
 def tree_words(parents):
@@ -176,7 +191,7 @@ def tree_step(model, cache, last, drafts, parents, generator=None, **sampling):
     parents = parents.masked_fill(missing[:, 1:] | (parents > cache.steps[:T]), -1)
     words, depths = tree_words(parents)
     rows = torch.cat((last[:, None], drafts), 1)
-    logits = extend(model, cache, rows, words, depths, counts=cache.capacity - cache.lens)
+    logits = extend(model, cache, rows, words, depths, cache.capacity - cache.lens, missing)
     flat = logits.flatten(0, 1)
     per_row = {k: v.repeat_interleave(T + 1) if isinstance(v, torch.Tensor) else v for k, v in sampling.items()}
     sampled = sample_tokens(flat, _noise(flat, generator), **per_row)[0].view(B, T + 1)
@@ -194,8 +209,8 @@ def tree_step(model, cache, last, drafts, parents, generator=None, **sampling):
         n += alive[:, 0].int()
     n.masked_fill_(missing[:, 0], 0)
     # the accepted rows move together behind the context; they are rotated already, by their depth
-    keep = cache.lens[:, None] + path.int()
+    page, slot = cache.where(cache.lens[:, None] + path.int())
     for k, v in zip(cache.k, cache.v):
-        append_paged_kv(cache.rows(k, keep), cache.rows(v, keep), k, v, cache.table, cache.lens, count=n)
+        append_paged_kv(*(x[page, :, slot].transpose(1, 2) for x in (k, v)), k, v, cache.table, cache.lens, count=n)
     cache.lens += n
     return tokens, n
