@@ -17,7 +17,8 @@ pool works too; page_size a multiple of 16) and an int32 ``page_table``
 there: calls launch on the current stream, never synchronise, and can be captured in a
 CUDA graph, after one call outside (the first on a device, or of a number of heads, builds
 what is kept, and a capture refuses it).  A token whose page is outside the pool, or past the table, is skipped and
-reported by ``device_status()`` as code 11.
+reported by ``device_status()`` as code 11; one whose position has no row in the rotary
+tables is stored unrotated and reported too.
 
 There is no backward: where gradients are enabled, keys, values, queries and pools that
 require one are refused (call under ``torch.no_grad()``), and log-probabilities of sampled

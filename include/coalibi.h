@@ -215,7 +215,8 @@ int coalibi_describe_launch(int which, int B, int Hq, int Hkv, int Sq, int Skv, 
  * page_table[b * table_stride + t / page_size], slot t % page_size.  Lengths and
  * tables are read on the device, so a captured graph can replay as they change;
  * entries past a request's tokens are never used.  A token outside the table or a
- * page outside the pool is skipped and reported as COALIBI_ERR_PAGE in *status.
+ * page outside the pool is skipped and reported as COALIBI_ERR_PAGE in *status; a token
+ * whose position has no row in the rotary table is appended unrotated and reported too.
  * ------------------------------------------------------------------------- */
 
 /* Append the S new tokens (count[b] of them when count is given) of each request at
