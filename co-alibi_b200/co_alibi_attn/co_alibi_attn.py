@@ -57,7 +57,7 @@ def _ev():
 def _not_capturing(device, what):
     """What is built on first use and kept must not be built inside a CUDA graph capture: the
     values would be written by each replay, or copied from the host, which cannot be captured."""
-    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+    if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"co_alibi_attn: {what} is built by the first call on {device}, which a CUDA graph cannot "
                            "capture; run the call once before the capture")
 
