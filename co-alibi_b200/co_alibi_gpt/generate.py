@@ -180,15 +180,15 @@ def tree_step(model, cache, last, drafts, parents, generator=None, **sampling):
     the cache), ``drafts`` [B, T] and ``parents`` [B, T] as in ``tree_words``.  A token is
     sampled after every row; from row 0 on, a draft that equals its parent's sample is
     accepted, and the first sample that no draft matches ends the step.  That draws from the
-    model's own distribution whatever the drafts are.  Drafts behind the cache's capacity count
-    as none: the step ends before them.
+    model's own distribution whatever the drafts are.  Drafts behind the cache's capacity, and
+    tokens below 0, count as none: the step ends before them.
 
     Returns (tokens [B, T + 1], n [B] int32): the first n[b] of tokens[b] are new, the last of
     them becomes ``last``.  The cache then holds every token before it.  A request whose cache is
     full already gets n = 0 and tokens of -1, and ``device_status()`` reports it."""
     B, T = drafts.shape
     missing = cache.missing(T + 1)
-    parents = parents.masked_fill(missing[:, 1:] | (parents > cache.steps[:T]), -1)
+    parents = parents.masked_fill(missing[:, 1:] | (parents > cache.steps[:T]) | (drafts < 0), -1)
     words, depths = tree_words(parents)
     rows = torch.cat((last[:, None], drafts), 1)
     logits = extend(model, cache, rows, words, depths, cache.capacity - cache.lens, missing)

@@ -217,3 +217,17 @@ def test_a_parent_that_does_not_come_before_its_draft_is_none(device, monkeypatc
         cache.lens.fill_(12)
         tokens, n = gen.tree_step(model, cache, last, drafts, torch.tensor([parents], device=device), temperature=0.0)
         assert n.tolist() == [accepted + 1] and torch.equal(tokens[0, :accepted + 1], plain[0, 1:accepted + 2])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_absent_token_confirms_nothing(device, monkeypatch):
+    """Where nothing can be drawn the step ends, also before drafts of -1 that name a parent."""
+    gen = _generate(device, monkeypatch)
+    model = _model(device)
+    cache = gen.PagedCache(model, 2, 32, page_size=16)
+    last = gen.prefill(model, cache, _tokens(2, 5, device)).argmax(-1)
+    with torch.no_grad():
+        model.ln_f.weight.fill_(float("nan"))
+    drafts = torch.full((2, 3), -1, device=device)
+    tokens, n = gen.tree_step(model, cache, last, drafts, torch.arange(3, device=device).expand(2, 3))
+    assert (tokens == -1).all() and n.tolist() == [1, 1] and cache.lens.tolist() == [6, 6]
