@@ -29,7 +29,7 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
     "-Xcompiler", "-fPIC", "-shared",
-    "--expt-relaxed-constexpr",
+    "--expt-relaxed-constexpr", "--threads", "0",
     "-Xptxas", "-v",
 ]
 

@@ -68,10 +68,30 @@ class CoalibiSampleArgs(ctypes.Structure):
                  ("top_p_all", c_float), ("min_p_all", c_float)]
 
 
+class CoalibiCacheScales(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_stride", c_int64 * 2), ("v_stride", c_int64 * 2)]
+
+
+class CoalibiPagedReadArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("k_pages", "v_pages", "page_table", "positions", "k", "v", "status")]
+    _fields_ += [("k_page_stride", c_int64 * 3), ("v_page_stride", c_int64 * 3), ("table_stride", c_int64)]
+    _fields_ += [(n, c_int) for n in ("B", "Hkv", "S", "D", "page_size", "max_pages", "n_pages", "dtype")]
+
+
+class CoalibiHeadsArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("qkv", "q", "k", "v", "q_weight", "k_weight", "cos", "sin", "start", "positions",
+                                        "status", "dqkv", "dq_weight", "dk_weight")]
+    _fields_ += [(n, c_int64 * 3) for n in ("qkv_stride", "q_stride", "k_stride", "v_stride")]
+    _fields_ += [(n, c_int) for n in ("B", "S", "Hq", "Hkv", "D", "rot", "n_pos", "interleaved", "dtype", "weight_dtype")]
+    _fields_ += [("eps", c_float)]
+
+
 EXPORTS = ("coalibi_fwd", "coalibi_fwd_decode", "coalibi_fwd_decode_workspace_bytes", "coalibi_bwd",
            "coalibi_bwd_carry", "coalibi_bwd_phases", "coalibi_bwd_noalloc", "coalibi_bwd_workspace_size",
            "coalibi_bwd_workspace_bytes", "coalibi_bwd_workspace_min_bytes", "coalibi_selftest_wait_timeout",
            "coalibi_paged_append", "coalibi_paged_attention", "coalibi_paged_attention_workspace_bytes",
+           "coalibi_paged_append8", "coalibi_paged_attention8", "coalibi_paged_attention8_workspace_bytes",
+           "coalibi_paged_read8", "coalibi_heads_fwd", "coalibi_heads_bwd", "coalibi_heads_bwd_workspace_bytes",
            "coalibi_sample", "coalibi_strerror",
            "coalibi_abi_version", "coalibi_last_error", "coalibi_describe_launch")
 
@@ -120,6 +140,20 @@ def load():
             lib.coalibi_paged_attention.restype = c_int
             lib.coalibi_paged_attention_workspace_bytes.argtypes = [c_int] * 5
             lib.coalibi_paged_attention_workspace_bytes.restype = c_size_t
+            lib.coalibi_paged_append8.argtypes = [c_void_p] * 3
+            lib.coalibi_paged_append8.restype = c_int
+            lib.coalibi_paged_attention8.argtypes = [c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+            lib.coalibi_paged_attention8.restype = c_int
+            lib.coalibi_paged_attention8_workspace_bytes.argtypes = [c_int] * 5
+            lib.coalibi_paged_attention8_workspace_bytes.restype = c_size_t
+            lib.coalibi_paged_read8.argtypes = [c_void_p] * 3
+            lib.coalibi_paged_read8.restype = c_int
+            lib.coalibi_heads_fwd.argtypes = [c_void_p] * 2
+            lib.coalibi_heads_fwd.restype = c_int
+            lib.coalibi_heads_bwd.argtypes = [c_void_p, c_void_p, c_size_t, c_void_p]
+            lib.coalibi_heads_bwd.restype = c_int
+            lib.coalibi_heads_bwd_workspace_bytes.argtypes = [c_int]
+            lib.coalibi_heads_bwd_workspace_bytes.restype = c_size_t
             lib.coalibi_sample.argtypes = [c_void_p, c_void_p]
             lib.coalibi_sample.restype = c_int
             lib.coalibi_selftest_wait_timeout.argtypes = [ctypes.c_uint, c_void_p, c_void_p]

@@ -6,6 +6,7 @@ cache.  The reference ships the attention operator alone
   queries on the way for models that add rotary positions to the Co-ALiBi bias.
 * ``paged_tree_attention``: Co-ALiBi attention of one token, or of a tree of drafted
   tokens, per request over that cache.
+* ``read_paged_kv``: tokens of a cache that is held in 8 bits, in 16 bits again.
 * ``sample_tokens``: temperature, top-k, top-p and min-p, and a draw by given random
   numbers.
 
@@ -20,6 +21,15 @@ what is kept, and a capture refuses it).  A token whose page is outside the pool
 reported by ``device_status()`` as code 11; one whose position has no row in the rotary
 tables is stored unrotated and reported too.
 
+A cache may be held in 8 bits: pools of ``torch.float8_e4m3fn`` (D a multiple of 16, strides
+too) with ``scales`` = (k_scales, v_scales), float32 [n_pages, Hkv, page_size / 16], one for each
+block of 16 tokens of a page and head.  A value is its code times the scale of its block.
+``append_paged_kv`` writes scales that are powers of two, the least by which a block's largest
+value is at most 448 (and at least 2^-100): a code's relative error is at most 2^-4 then, or 2^-10 of the scale, that is
+2^-18 to 2^-17 of the block's largest, for what is smaller.  A block that already holds tokens keeps its scale unless
+a new one is too large for it, and if so the old codes move to the new scale, which changes none but
+those that fall below 2^-6 of it.  Slots behind a request's tokens hold nothing.
+
 There is no backward: where gradients are enabled, keys, values, queries and pools that
 require one are refused (call under ``torch.no_grad()``), and log-probabilities of sampled
 tokens carry none.  Appending counts as an in-place write of the pools for autograd.
@@ -28,9 +38,11 @@ import torch
 
 from .co_alibi_attn import _api_slopes, _status_word
 
-__all__ = ["append_paged_kv", "paged_tree_attention", "sample_tokens", "rotary_tables", "TREE_MAX_SQ"]
+__all__ = ["append_paged_kv", "paged_tree_attention", "read_paged_kv", "sample_tokens", "rotary_tables", "TREE_MAX_SQ",
+           "QUANT_BLOCK"]
 
 TREE_MAX_SQ = 64  # COALIBI_TREE_MAX_SQ in coalibi.h
+QUANT_BLOCK = 16  # COALIBI_QUANT_BLOCK: tokens that share a scale in a cache of 8 bits
 
 _binding = None
 
@@ -60,7 +72,7 @@ def rotary_tables(rotary_dim, max_pos, base=10000.0, scale=1.0, device=None):
 
 
 def append_paged_kv(k, v, k_pages, v_pages, page_table, start, count=None, q=None, rotary=None, interleaved=False,
-                    positions=None):
+                    positions=None, scales=None):
     """Write the new tokens' keys and values into the cache, in place.
 
     k, v: [B, Hkv, S, D] (any strides with contiguous rows, e.g. views of a fused
@@ -74,14 +86,17 @@ def append_paged_kv(k, v, k_pages, v_pages, page_table, start, count=None, q=Non
     tables at the token's position, or at ``positions`` (int32 [B, S]; a drafted tree's
     tokens sit at their depth, not at their slot).  With ``q`` [B, Hq, S, D] the queries
     are rotated in the same launch and returned (rows past ``count`` are zero); without,
-    None is returned.  Rotations are float32, rounded once; all else is moved as it is."""
+    None is returned.  Rotations are float32, rounded once; all else is moved as it is.
+
+    ``scales``: those of a cache in 8 bits, written with it.  Keys (rotated in float32) and values
+    are rounded once, to the nearest code of their block, ties to the even one; infinities become NaN."""
     assert k.is_cuda, "Inputs must be CUDA tensors"
     return _native().append_paged_kv(k, v, k_pages, v_pages, page_table, start, count, q, rotary, interleaved,
-                                     positions, _status_word(k.device))
+                                     positions, _status_word(k.device), scales)
 
 
 def paged_tree_attention(q, k_pages, v_pages, page_table, ctx_lens, tree_mask=None, sm_scale=None, bias_max=8.0,
-                         slopes=None):
+                         slopes=None, scales=None):
     """Co-ALiBi attention of each request's Sq query rows over its cache (forward only).
 
     q: [B, Hq, Sq, D], Sq <= 64, Hq a multiple of the cache's Hkv.  Every row sees the
@@ -99,12 +114,33 @@ def paged_tree_attention(q, k_pages, v_pages, page_table, ctx_lens, tree_mask=No
 
     Scores, sigmoid sums, softmax statistics and the result's sums are float32 (with the
     hardware's approximate exponential and reciprocal); the weights are rounded to the
-    inputs' type for the product with V, as in ``co_alibi_attention``."""
+    inputs' type for the product with V, as in ``co_alibi_attention``.
+
+    ``scales``: those of a cache in 8 bits.  Its products take the codes as float16, which holds them
+    whole (bfloat16 queries too, each row by a power of two), and the weights as float16."""
     assert q.is_cuda, "Inputs must be CUDA tensors"
     if slopes is None:
         slopes = _api_slopes(q.shape[1], bias_max, q.dtype, q.device)
     return _native().paged_tree_attention(q, k_pages, v_pages, page_table, ctx_lens, tree_mask, sm_scale, slopes,
-                                          _status_word(q.device))
+                                          _status_word(q.device), scales)
+
+
+_READ_DTYPES = {torch.float16: False, torch.bfloat16: True}
+
+
+def read_paged_kv(k_pages, v_pages, page_table, positions, scales, dtype=torch.bfloat16):
+    """Tokens of a cache in 8 bits, as (k, v) [B, Hkv, S, D] of ``dtype`` (float16 or bfloat16).
+
+    ``positions`` int32 [B, S]: which tokens of each request, in any order, the same one as often
+    as asked for; a negative one gives a row of zeros, and so does one without a page, which is
+    reported.  Values are rounded once (bfloat16 holds every one whose scale is a power of two whole);
+    one past the type's largest is that.  What is read and appended again, with a scale not below
+    its block's, gets the same codes."""
+    assert k_pages.is_cuda, "Inputs must be CUDA tensors"
+    if dtype not in _READ_DTYPES:
+        raise TypeError(f"co_alibi_attn: read_paged_kv: dtype must be float16 or bfloat16, got {dtype}")
+    return _native().read_paged_kv(k_pages, v_pages, page_table, positions, scales, _READ_DTYPES[dtype],
+                                   _status_word(k_pages.device))
 
 
 def sample_tokens(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):

@@ -7,6 +7,7 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <ATen/ops/zeros_like.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -79,18 +80,59 @@ void strides(const Tensor& t, long long* s) {
 bool rows16(const Tensor& t) {
   long long s[3];
   strides(t, s);
-  return (t.stride(3) == 1 || t.size(3) == 1) && ((s[0] | s[1] | s[2]) & 7) == 0 &&
+  return (t.stride(3) == 1 || t.size(3) == 1) && ((s[0] | s[1] | s[2]) & (16 / t.element_size() - 1)) == 0 &&
          (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
 }
 
 Tensor aligned_rows(const Tensor& t) { return rows16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
+// The scales of a cache in 8 bits.
+struct Scales {
+  Tensor k, v;
+  CoalibiCacheScales c{};
+  bool given = false;
+};
+
+Scales scales_of(PyObject* o, const char* what) {
+  Scales s;
+  if (o == Py_None) return s;
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2) refuse(PyExc_TypeError, what, "scales must be a tuple (k_scales, v_scales)");
+  s.k = tensor(PyTuple_GET_ITEM(o, 0), what, "k_scales");
+  s.v = tensor(PyTuple_GET_ITEM(o, 1), what, "v_scales");
+  s.given = true;
+  return s;
+}
+
+void check_scales(const char* what, Scales& s, const Tensor& pages, c10::Device device) {
+  const int64_t blocks = pages.size(2) / COALIBI_QUANT_BLOCK;
+  const char* names[2] = {"k_scales", "v_scales"};
+  for (int i = 0; i < 2; ++i) {
+    const Tensor& t = i ? s.v : s.k;
+    if (t.scalar_type() != at::kFloat) refuse(PyExc_TypeError, what, names[i], " must be float32, got ", c10::toString(t.scalar_type()));
+    if (t.dim() != 3 || t.size(0) != pages.size(0) || t.size(1) != pages.size(1) || t.size(2) != blocks)
+      refuse(PyExc_ValueError, what, names[i], " must be [", pages.size(0), ", ", pages.size(1), ", ", blocks, "], got ", shape_of(t));
+    if (blocks > 1 && t.stride(2) != 1) refuse(PyExc_ValueError, what, names[i], " must have contiguous rows");
+    on(what, names[i], t, device);
+    for (int d = 0; d < 2; ++d) {
+      if (t.size(d) > 1 && t.stride(d) == 0) refuse(PyExc_ValueError, what, names[i], " must not be an expanded tensor");
+      (i ? s.c.v_stride : s.c.k_stride)[d] = t.size(d) > 1 ? t.stride(d) : 0;
+    }
+  }
+  s.c.k = s.k.data_ptr<float>();
+  s.c.v = s.v.data_ptr<float>();
+}
+
+// dtype: of the values that go in or come out; the pools' own, unless they hold codes.
 void check_cache(const char* what, const Tensor& k, const Tensor& v, const Tensor& table, int64_t B, int64_t D,
-                 at::ScalarType dtype, c10::Device device) {
+                 at::ScalarType dtype, c10::Device device, Scales& scales) {
+  const bool codes = k.scalar_type() == at::kFloat8_e4m3fn && v.scalar_type() == at::kFloat8_e4m3fn;
+  if (codes != scales.given)
+    refuse(PyExc_TypeError, what, codes ? "a cache of float8_e4m3fn needs scales" : "scales are for a cache of float8_e4m3fn, got ",
+           codes ? "" : c10::toString(k.scalar_type()));
   if (k.dim() != 4 || v.sizes() != k.sizes())
     refuse(PyExc_ValueError, what, "k_pages and v_pages must both be [n_pages, Hkv, page_size, D], got ", shape_of(k),
            " and ", shape_of(v));
-  if (k.scalar_type() != dtype || v.scalar_type() != dtype)
+  if (!codes && (k.scalar_type() != dtype || v.scalar_type() != dtype))
     refuse(PyExc_TypeError, what, "the cache holds ", c10::toString(k.scalar_type()), " and ",
            c10::toString(v.scalar_type()), ", the inputs ", c10::toString(dtype));
   if (k.size(3) != D) refuse(PyExc_ValueError, what, "the cache has head_dim ", k.size(3), ", the inputs ", D);
@@ -113,6 +155,7 @@ void check_cache(const char* what, const Tensor& k, const Tensor& v, const Tenso
   on(what, "k_pages", k, device);
   on(what, "v_pages", v, device);
   on(what, "page_table", table, device);
+  if (codes) check_scales(what, scales, k, device);
 }
 
 // An index tensor of the given shape (one or two dimensions), contiguous.
@@ -124,6 +167,25 @@ Tensor indices(PyObject* o, const char* what, const char* name, at::IntArrayRef 
   if (t.sizes() != shape) refuse(PyExc_ValueError, what, name, " must have shape ", shape_of(shape), ", got ", shape_of(t));
   on(what, name, t, device);
   return t.contiguous();
+}
+
+// The rotary tables (cos, sin), contiguous and aligned.
+void rotary_of(PyObject* o, const char* what, int64_t D, c10::Device device, Tensor& cos, Tensor& sin) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2)
+    refuse(PyExc_TypeError, what, "rotary must be a tuple (cos, sin)");
+  cos = tensor(PyTuple_GET_ITEM(o, 0), what, "cos");
+  sin = tensor(PyTuple_GET_ITEM(o, 1), what, "sin");
+  if (cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat)
+    refuse(PyExc_TypeError, what, "the rotary tables must be float32");
+  if (cos.dim() != 2 || sin.sizes() != cos.sizes() || cos.size(0) == 0 || cos.size(0) > 0x7fffffff ||
+      cos.size(1) % 8 != 0 || cos.size(1) == 0 || 2 * cos.size(1) > D)
+    refuse(PyExc_ValueError, what, "the rotary tables must be [n_pos, R / 2] with R a multiple of 16 up to ", D,
+           ", got ", shape_of(cos), " and ", shape_of(sin));
+  on(what, "cos", cos, device);
+  on(what, "sin", sin, device);
+  for (Tensor* t : {&cos, &sin})
+    if (!t->is_contiguous() || (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15))
+      *t = t->clone(at::MemoryFormat::Contiguous);
 }
 
 void* status_ptr(PyObject* o, const char* what) { return tensor(o, what, "status").data_ptr(); }
@@ -138,7 +200,7 @@ void check(int code, const char* fn) {
 
 void* stream_of(c10::Device device) { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
 
-// (k, v, k_pages, v_pages, page_table, start, count, q, rotary, interleaved, positions, status)
+// (k, v, k_pages, v_pages, page_table, start, count, q, rotary, interleaved, positions, status, scales)
 PyObject* append_paged_kv(PyObject* const* a) {
   const char* what = "append_paged_kv";
   const Tensor &k0 = tensor(a[0], what, "k"), &v0 = tensor(a[1], what, "v");
@@ -155,7 +217,9 @@ PyObject* append_paged_kv(PyObject* const* a) {
   if (p.dtype < 0 || v0.scalar_type() != dtype || (with_q && tensor(a[7], what, "q").scalar_type() != dtype))
     refuse(PyExc_TypeError, what, "k, v and q must all be float16 or bfloat16");
   if (D != 64 && D != 128) refuse(PyExc_ValueError, what, "head_dim must be 64 or 128, got ", D);
-  check_cache(what, kp, vp, table, B, D, dtype, device);
+  Scales scales = scales_of(a[12], what);
+  check_cache(what, kp, vp, table, B, D, dtype, device, scales);
+  if (scales.given) no_grad(what, "k_scales", scales.k), no_grad(what, "v_scales", scales.v);
   if (kp.size(1) != Hkv) refuse(PyExc_ValueError, what, "the cache has ", kp.size(1), " kv heads, k ", Hkv);
   on(what, "v", v0, device);
   no_grad(what, "k", k0), no_grad(what, "v", v0), no_grad(what, "k_pages", kp), no_grad(what, "v_pages", vp);
@@ -185,21 +249,7 @@ PyObject* append_paged_kv(PyObject* const* a) {
     p.positions = positions.data_ptr<int>();
   }
   if (a[8] != Py_None) {
-    if (!PyTuple_Check(a[8]) || PyTuple_GET_SIZE(a[8]) != 2)
-      refuse(PyExc_TypeError, what, "rotary must be a tuple (cos, sin)");
-    cos = tensor(PyTuple_GET_ITEM(a[8], 0), what, "cos");
-    sin = tensor(PyTuple_GET_ITEM(a[8], 1), what, "sin");
-    if (cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat)
-      refuse(PyExc_TypeError, what, "the rotary tables must be float32");
-    if (cos.dim() != 2 || sin.sizes() != cos.sizes() || cos.size(0) == 0 || cos.size(0) > 0x7fffffff ||
-        cos.size(1) % 8 != 0 || cos.size(1) == 0 || 2 * cos.size(1) > D)
-      refuse(PyExc_ValueError, what, "the rotary tables must be [n_pos, R / 2] with R a multiple of 16 up to ", D,
-             ", got ", shape_of(cos), " and ", shape_of(sin));
-    on(what, "cos", cos, device);
-    on(what, "sin", sin, device);
-    for (Tensor* t : {&cos, &sin})
-      if (!t->is_contiguous() || (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15))
-        *t = t->clone(at::MemoryFormat::Contiguous);
+    rotary_of(a[8], what, D, device, cos, sin);
     p.cos = cos.data_ptr<float>();
     p.sin = sin.data_ptr<float>();
     p.n_pos = (int)cos.size(0);
@@ -224,14 +274,19 @@ PyObject* append_paged_kv(PyObject* const* a) {
     if (truth < 0) return nullptr;
     p.interleaved = truth;
     if (with_q && p.Hq == 0) p.q = nullptr, p.q_out = nullptr;
-    check(coalibi_paged_append(&p, stream_of(device)), "coalibi_paged_append");
+    if (scales.given) {
+      check(coalibi_paged_append8(&p, &scales.c, stream_of(device)), "coalibi_paged_append8");
+      written(scales.k), written(scales.v);
+    } else {
+      check(coalibi_paged_append(&p, stream_of(device)), "coalibi_paged_append");
+    }
     written(kp), written(vp);
   }
   if (!with_q) Py_RETURN_NONE;
   return THPVariable_Wrap(q_out);
 }
 
-// (q, k_pages, v_pages, page_table, ctx_lens, tree_mask, sm_scale, slopes, status)
+// (q, k_pages, v_pages, page_table, ctx_lens, tree_mask, sm_scale, slopes, status, scales)
 PyObject* paged_tree_attention(PyObject* const* a) {
   const char* what = "paged_tree_attention";
   const Tensor& q0 = tensor(a[0], what, "q");
@@ -246,7 +301,9 @@ PyObject* paged_tree_attention(PyObject* const* a) {
   if (D != 64 && D != 128) refuse(PyExc_ValueError, what, "head_dim must be 64 or 128, got ", D);
   if (Sq > COALIBI_TREE_MAX_SQ)
     refuse(PyExc_ValueError, what, "at most ", COALIBI_TREE_MAX_SQ, " rows per request, got ", Sq);
-  check_cache(what, kp, vp, table, B, D, q0.scalar_type(), device);
+  Scales scales = scales_of(a[9], what);
+  check_cache(what, kp, vp, table, B, D, q0.scalar_type(), device, scales);
+  if (scales.given) no_grad(what, "k_scales", scales.k), no_grad(what, "v_scales", scales.v);
   const int64_t Hkv = kp.size(1);
   if (Hq % Hkv != 0) refuse(PyExc_ValueError, what, "num_heads ", Hq, " must be a multiple of num_kv_heads ", Hkv);
   const Tensor ctx = indices(a[4], what, "ctx_lens", {B}, at::kInt, device);
@@ -276,7 +333,8 @@ PyObject* paged_tree_attention(PyObject* const* a) {
   const Tensor q = aligned_rows(q0.detach()), slopes = slopes0.contiguous();
   Tensor o = at::empty_like(q);
   if (q.numel() > 0) {
-    const size_t bytes = coalibi_paged_attention_workspace_bytes((int)B, (int)Hq, (int)Hkv, (int)Sq, (int)D);
+    const size_t bytes = (scales.given ? coalibi_paged_attention8_workspace_bytes : coalibi_paged_attention_workspace_bytes)(
+        (int)B, (int)Hq, (int)Hkv, (int)Sq, (int)D);
     const Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
     p.q = q.data_ptr();
     p.o = o.data_ptr();
@@ -293,9 +351,197 @@ PyObject* paged_tree_attention(PyObject* const* a) {
     p.table_stride = table.stride(0);
     p.B = (int)B, p.Hq = (int)Hq, p.Hkv = (int)Hkv, p.Sq = (int)Sq, p.D = (int)D;
     p.page_size = (int)kp.size(2), p.max_pages = (int)table.size(1), p.n_pages = (int)kp.size(0);
-    check(coalibi_paged_attention(&p, ws.data_ptr(), bytes, stream_of(device)), "coalibi_paged_attention");
+    if (scales.given)
+      check(coalibi_paged_attention8(&p, &scales.c, ws.data_ptr(), bytes, stream_of(device)), "coalibi_paged_attention8");
+    else
+      check(coalibi_paged_attention(&p, ws.data_ptr(), bytes, stream_of(device)), "coalibi_paged_attention");
   }
   return THPVariable_Wrap(o);
+}
+
+// (k_pages, v_pages, page_table, positions, scales, bf16, status)
+PyObject* read_paged_kv(PyObject* const* a) {
+  const char* what = "read_paged_kv";
+  const Tensor &kp = tensor(a[0], what, "k_pages"), &vp = tensor(a[1], what, "v_pages");
+  const Tensor &table = tensor(a[2], what, "page_table"), &positions0 = tensor(a[3], what, "positions");
+  if (positions0.dim() != 2) refuse(PyExc_ValueError, what, "positions must be [B, S], got ", shape_of(positions0));
+  const int64_t B = positions0.size(0), S = positions0.size(1);
+  const auto device = kp.device();
+  const bool bf16 = PyObject_IsTrue(a[5]);
+  const auto dtype = bf16 ? at::kBFloat16 : at::kHalf;
+  Scales scales = scales_of(a[4], what);
+  if (!scales.given) refuse(PyExc_TypeError, what, "scales must be a tuple (k_scales, v_scales)");
+  if (kp.dim() == 4 && kp.size(3) != 64 && kp.size(3) != 128) refuse(PyExc_ValueError, what, "head_dim must be 64 or 128, got ", kp.size(3));
+  check_cache(what, kp, vp, table, B, kp.dim() == 4 ? kp.size(3) : 0, dtype, device, scales);
+  no_grad(what, "k_scales", scales.k), no_grad(what, "v_scales", scales.v);
+  const int64_t Hkv = kp.size(1), D = kp.size(3);
+  if (S > 0x7fffffff) refuse(PyExc_ValueError, what, "too many tokens");
+  const Tensor positions = indices(a[3], what, "positions", {B, S}, at::kInt, device);
+  Tensor k = at::empty({B, Hkv, S, D}, kp.options().dtype(dtype)), v = at::empty_like(k);
+  if (k.numel() > 0) {
+    CoalibiPagedReadArgs p{};
+    p.k_pages = kp.data_ptr();
+    p.v_pages = vp.data_ptr();
+    p.page_table = table.data_ptr<int>();
+    p.positions = positions.data_ptr<int>();
+    p.k = k.data_ptr();
+    p.v = v.data_ptr();
+    p.status = static_cast<int*>(status_ptr(a[6], what));
+    strides(kp, p.k_page_stride);
+    strides(vp, p.v_page_stride);
+    p.table_stride = table.stride(0);
+    p.B = (int)B, p.Hkv = (int)Hkv, p.S = (int)S, p.D = (int)D;
+    p.page_size = (int)kp.size(2), p.max_pages = (int)table.size(1), p.n_pages = (int)kp.size(0);
+    p.dtype = bf16 ? COALIBI_BF16 : COALIBI_F16;
+    check(coalibi_paged_read8(&p, &scales.c, stream_of(device)), "coalibi_paged_read8");
+  }
+  PyObject* pair = PyTuple_New(2);
+  if (pair == nullptr) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(k));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(v));
+  return pair;
+}
+
+// What the forward and the backward of the heads take alike, and the tensors it points at.
+struct Heads {
+  CoalibiHeadsArgs p{};
+  Tensor qkv, weight[2], cos, sin, start, positions;
+  int64_t B, S, Hq, Hkv, D;
+};
+
+int64_t whole(PyObject* o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw Refused{nullptr, ""};
+  return v;
+}
+
+// a: qkv, num_heads, num_kv_heads, q_weight, k_weight, eps, rotary, start, positions, interleaved, status
+Heads heads_of(PyObject* const* a) {
+  const char* what = "norm_rotate_qkv";
+  Heads h;
+  const Tensor& x = tensor(a[0], what, "qkv");
+  h.Hq = whole(a[1]), h.Hkv = whole(a[2]);
+  if (x.dim() != 4) refuse(PyExc_ValueError, what, "qkv must be [B, S, num_heads + 2 num_kv_heads, D], got ", shape_of(x));
+  h.B = x.size(0), h.S = x.size(1), h.D = x.size(3);
+  if (h.Hq <= 0 || h.Hkv <= 0 || h.Hq > 65535 || h.Hkv > 65535 || x.size(2) != h.Hq + 2 * h.Hkv)
+    refuse(PyExc_ValueError, what, "qkv must hold num_heads + 2 num_kv_heads heads, got ", shape_of(x), " with ", h.Hq, " and ", h.Hkv);
+  CoalibiHeadsArgs& p = h.p;
+  p.dtype = p.weight_dtype = dtype16(x);
+  if (p.dtype < 0) refuse(PyExc_TypeError, what, "qkv must be float16 or bfloat16, got ", c10::toString(x.scalar_type()));
+  if (h.D != 64 && h.D != 128) refuse(PyExc_ValueError, what, "head_dim must be 64 or 128, got ", h.D);
+  if (h.B > 0x7fffffff || h.S > 0x7fffffff || h.B * h.S > 0x7fffffff) refuse(PyExc_ValueError, what, "too many tokens");
+  const auto device = x.device();
+  if (!device.is_cuda()) refuse(PyExc_ValueError, what, "qkv is on ", device.str());
+  h.qkv = aligned_rows(x.detach());
+  strides(h.qkv, p.qkv_stride);
+  const char* names[2] = {"q_weight", "k_weight"};
+  at::ScalarType type = x.scalar_type();
+  bool seen = false;
+  for (int i = 0; i < 2; ++i) {
+    if (a[3 + i] == Py_None) continue;
+    const Tensor& w = tensor(a[3 + i], what, names[i]);
+    if ((w.scalar_type() != x.scalar_type() && w.scalar_type() != at::kFloat) || (seen && w.scalar_type() != type))
+      refuse(PyExc_TypeError, what, "the weights must both be ", c10::toString(x.scalar_type()), " or float32, got ", c10::toString(w.scalar_type()));
+    if (w.dim() != 1 || w.size(0) != h.D) refuse(PyExc_ValueError, what, names[i], " must have shape [", h.D, "], got ", shape_of(w));
+    on(what, names[i], w, device);
+    h.weight[i] = w.detach().contiguous();
+    if (reinterpret_cast<uintptr_t>(h.weight[i].data_ptr()) & 3) h.weight[i] = h.weight[i].clone();
+    type = w.scalar_type();
+    seen = true;
+  }
+  if (seen && type == at::kFloat) p.weight_dtype = COALIBI_F32;
+  p.q_weight = h.weight[0].defined() ? h.weight[0].data_ptr() : nullptr;
+  p.k_weight = h.weight[1].defined() ? h.weight[1].data_ptr() : nullptr;
+  const double eps = PyFloat_AsDouble(a[5]);
+  if (eps == -1.0 && PyErr_Occurred()) throw Refused{nullptr, ""};
+  if (!(eps >= 0)) refuse(PyExc_ValueError, what, "eps must not be negative");
+  p.eps = (float)eps;
+  if (a[6] != Py_None) {
+    rotary_of(a[6], what, h.D, device, h.cos, h.sin);
+    p.cos = h.cos.data_ptr<float>();
+    p.sin = h.sin.data_ptr<float>();
+    p.n_pos = (int)h.cos.size(0);
+    p.rot = 2 * (int)h.cos.size(1);
+  }
+  if (a[7] != Py_None) {
+    h.start = indices(a[7], what, "start", {h.B}, at::kInt, device);
+    p.start = h.start.data_ptr<int>();
+  }
+  if (a[8] != Py_None) {
+    h.positions = indices(a[8], what, "positions", {h.B, h.S}, at::kInt, device);
+    p.positions = h.positions.data_ptr<int>();
+  }
+  const int truth = PyObject_IsTrue(a[9]);
+  if (truth < 0) throw Refused{nullptr, ""};
+  p.interleaved = truth;
+  p.status = static_cast<int*>(status_ptr(a[10], what));
+  p.qkv = h.qkv.data_ptr();
+  p.B = (int)h.B, p.S = (int)h.S, p.Hq = (int)h.Hq, p.Hkv = (int)h.Hkv, p.D = (int)h.D;
+  return h;
+}
+
+PyObject* triple(const Tensor& x, const Tensor& y, const Tensor& z) {
+  PyObject* t = PyTuple_New(3);
+  if (t == nullptr) return nullptr;
+  const Tensor* of[3] = {&x, &y, &z};
+  for (int i = 0; i < 3; ++i) {
+    if (of[i]->defined()) {
+      PyTuple_SET_ITEM(t, i, THPVariable_Wrap(*of[i]));
+    } else {
+      Py_INCREF(Py_None);
+      PyTuple_SET_ITEM(t, i, Py_None);
+    }
+  }
+  return t;
+}
+
+// (the eleven of heads_of) -> (q, k, v)
+PyObject* heads_fwd(PyObject* const* a) {
+  Heads h = heads_of(a);
+  CoalibiHeadsArgs& p = h.p;
+  Tensor q = at::empty({h.B, h.Hq, h.S, h.D}, h.qkv.options()), k = at::empty({h.B, h.Hkv, h.S, h.D}, h.qkv.options());
+  Tensor v = at::empty_like(k);
+  if (h.qkv.numel() > 0) {
+    p.q = q.data_ptr();
+    p.k = k.data_ptr();
+    p.v = v.data_ptr();
+    strides(q, p.q_stride), strides(k, p.k_stride), strides(v, p.v_stride);
+    check(coalibi_heads_fwd(&p, stream_of(h.qkv.device())), "coalibi_heads_fwd");
+  }
+  return triple(q, k, v);
+}
+
+// (the eleven of heads_of, dq, dk, dv) -> (dqkv, dq_weight or None, dk_weight or None)
+PyObject* heads_bwd(PyObject* const* a) {
+  const char* what = "norm_rotate_qkv's backward";
+  Heads h = heads_of(a);
+  CoalibiHeadsArgs& p = h.p;
+  Tensor d[3];
+  const char* names[3] = {"the gradient of q", "the gradient of k", "the gradient of v"};
+  for (int i = 0; i < 3; ++i) {
+    const Tensor& t = tensor(a[11 + i], what, names[i]);
+    const int64_t H = i ? h.Hkv : h.Hq;
+    if (t.sizes() != at::IntArrayRef{h.B, H, h.S, h.D} || t.scalar_type() != h.qkv.scalar_type())
+      refuse(PyExc_ValueError, what, names[i], " has shape ", shape_of(t), " and type ", c10::toString(t.scalar_type()));
+    on(what, names[i], t, h.qkv.device());
+    d[i] = aligned_rows(t.detach());
+  }
+  Tensor dqkv = at::empty({h.B, h.S, h.Hq + 2 * h.Hkv, h.D}, h.qkv.options()), dw[2];
+  for (int i = 0; i < 2; ++i)
+    if (h.weight[i].defined()) dw[i] = h.qkv.numel() > 0 ? at::empty_like(h.weight[i]) : at::zeros_like(h.weight[i]);
+  if (h.qkv.numel() > 0) {
+    const size_t bytes = coalibi_heads_bwd_workspace_bytes((int)h.D);
+    const Tensor ws = at::empty({(int64_t)bytes}, h.qkv.options().dtype(at::kByte));
+    p.q = d[0].data_ptr();
+    p.k = d[1].data_ptr();
+    p.v = d[2].data_ptr();
+    strides(d[0], p.q_stride), strides(d[1], p.k_stride), strides(d[2], p.v_stride);
+    p.dqkv = dqkv.data_ptr();
+    p.dq_weight = dw[0].defined() ? dw[0].data_ptr() : nullptr;
+    p.dk_weight = dw[1].defined() ? dw[1].data_ptr() : nullptr;
+    check(coalibi_heads_bwd(&p, ws.data_ptr(), bytes, stream_of(h.qkv.device())), "coalibi_heads_bwd");
+  }
+  return triple(dqkv, dw[0], dw[1]);
 }
 
 // A sampling parameter: a number, or a tensor [B] (kept alive in `keep`).
@@ -384,7 +630,8 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define METHOD(name, n) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<name, n>)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(append_paged_kv, 12), METHOD(paged_tree_attention, 9), METHOD(sample_tokens, 6),
+PyMethodDef methods[] = {METHOD(append_paged_kv, 13), METHOD(paged_tree_attention, 10), METHOD(sample_tokens, 6),
+                         METHOD(read_paged_kv, 7), METHOD(heads_fwd, 11), METHOD(heads_bwd, 14),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serving", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -63,23 +63,29 @@ int make_tmap(CUtensorMap* map, const void* base, int D, int rows, int heads, in
 }
 
 // 4-D view (D, slot, head, page) of a page pool of any strides (in elements; that of a
-// dimension of one entry is never used), loaded as boxes of 64 columns x 16 slots with the
-// 128-byte swizzle.
+// dimension of one entry is never used), loaded as boxes of 16 slots: of 64 columns of 16 bits
+// with the 128-byte swizzle, or of whole rows of 8-bit codes with the swizzle of their width.
 int make_page_tmap(CUtensorMap* map, const void* base, int D, int page_size, int heads, int pages,
-                   const long long* stride, bool bf16) {
+                   const long long* stride, int dtype) {
   auto fn = encode_fn();
   if (fn == nullptr) {
     snprintf(g_last_error, sizeof(g_last_error), "cuTensorMapEncodeTiled unavailable from the driver");
     return COALIBI_ERR_TENSOR_MAP;
   }
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)page_size, (cuuint64_t)heads, (cuuint64_t)pages};
+  const bool codes = dtype == COALIBI_E4M3;
+  const cuuint64_t size = codes ? 1 : 2;
   cuuint64_t strides[3];
-  for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] > 1 ? (cuuint64_t)stride[2 - i] * 2 : (cuuint64_t)D * 2;
-  cuuint32_t box[4] = {64, 16, 1, 1};
+  for (int i = 0; i < 3; ++i) strides[i] = (dims[i + 1] > 1 ? (cuuint64_t)stride[2 - i] : (cuuint64_t)D) * size;
+  cuuint32_t box[4] = {codes ? (cuuint32_t)D : 64u, 16, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  CUresult r = fn(map,
+                  codes                   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                  : dtype == COALIBI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                  4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  codes && D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     snprintf(g_last_error, sizeof(g_last_error),

@@ -1,0 +1,128 @@
+// C-ABI entry points of the normed and rotated heads (declared in include/coalibi.h).  Arguments
+// are checked before any device use; nothing here allocates or synchronises.
+#include "heads.cuh"
+
+#include "serving_host.cuh"
+
+using namespace coalibi;
+
+namespace coalibi {
+namespace {
+
+int heads_passes(int H, int pieces) {
+  const int most = kHeadsThreads / pieces;
+  return (H + most - 1) / most;
+}
+
+constexpr int kHeadsCtas = 16;  // to an SM, at most
+
+int heads_ctas(long long tokens) {
+  const long long most = (long long)device_sm_count() * kHeadsCtas;
+  return (int)(tokens < most ? tokens : most);
+}
+
+int check_heads(const CoalibiHeadsArgs* a, bool backward) {
+  if (a == nullptr || !a->qkv || !a->q || !a->k || !a->v) return COALIBI_ERR_NULL_POINTER;
+  if (backward && !a->dqkv) return COALIBI_ERR_NULL_POINTER;
+  if (a->D != 64 && a->D != 128) return COALIBI_ERR_HEAD_DIM;
+  if (a->dtype != COALIBI_F16 && a->dtype != COALIBI_BF16) return COALIBI_ERR_DTYPE;
+  if (a->weight_dtype != a->dtype && a->weight_dtype != COALIBI_F32) return COALIBI_ERR_DTYPE;
+  if (a->B <= 0 || a->S <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->Hq > 65535 || a->Hkv > 65535 ||
+      (long long)a->B * a->S > 0x7fffffffLL)
+    return COALIBI_ERR_SHAPE;
+  if (a->rot < 0 || a->rot > a->D || a->rot % 16 != 0 || (a->rot > 0 && a->n_pos <= 0)) return COALIBI_ERR_SHAPE;
+  if (a->rot > 0 && (!a->cos || !a->sin)) return COALIBI_ERR_NULL_POINTER;
+  if (!row_strides(a->qkv_stride) || !row_strides(a->q_stride) || !row_strides(a->k_stride) || !row_strides(a->v_stride))
+    return COALIBI_ERR_ALIGNMENT;
+  if (!aligned(a->qkv, 16) || !aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->cos, 16) ||
+      !aligned(a->sin, 16) || !aligned(a->dqkv, 16) || !aligned(a->q_weight, 4) || !aligned(a->k_weight, 4) ||
+      !aligned(a->start, 4) || !aligned(a->positions, 4))
+    return COALIBI_ERR_ALIGNMENT;
+  return COALIBI_OK;
+}
+
+HeadsParams heads_params(const CoalibiHeadsArgs* a) {
+  HeadsParams p{};
+  p.qkv = a->qkv;
+  p.weight[0] = a->q_weight;
+  p.weight[1] = a->k_weight;
+  p.cos = a->cos;
+  p.sin = a->sin;
+  p.start = a->start;
+  p.positions = a->positions;
+  p.status = a->status;
+  copy3(p.xs, a->qkv_stride);
+  copy3(p.hs[0], a->q_stride);
+  copy3(p.hs[1], a->k_stride);
+  copy3(p.hs[2], a->v_stride);
+  p.tokens = (long long)a->B * a->S;
+  p.Hq = a->Hq;
+  p.Hkv = a->Hkv;
+  p.S = a->S;
+  const int H = a->Hq + 2 * a->Hkv, passes = heads_passes(H, a->D / 8);
+  p.rows = (H + passes - 1) / passes;
+  p.rot = a->rot;
+  p.n_pos = a->n_pos;
+  p.interleaved = a->interleaved;
+  p.weight_f32 = a->weight_dtype == COALIBI_F32;
+  p.eps = a->eps;
+  return p;
+}
+
+int heads_threads(const HeadsParams& p, int D) { return (p.rows * (D / 8) + 31) / 32 * 32; }
+
+int heads_result(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return launched(what);
+  set_last_error_detail(cudaGetErrorString(e));
+  return COALIBI_ERR_LAUNCH;
+}
+
+}  // namespace
+}  // namespace coalibi
+
+extern "C" int coalibi_heads_fwd(const CoalibiHeadsArgs* a, void* stream) {
+  if (int rc = check_heads(a, false)) return rc;
+  CtxGuard guard;
+  if (int rc = enter_device(a->qkv, stream)) return rc;
+  HeadsParams p = heads_params(a);
+  p.out[0] = a->q;
+  p.out[1] = a->k;
+  p.out[2] = a->v;
+  const bool bf16 = a->dtype == COALIBI_BF16;
+  auto kernel = a->D == 128 ? (bf16 ? coalibi_heads_fwd_kernel<true, 128> : coalibi_heads_fwd_kernel<false, 128>)
+                            : (bf16 ? coalibi_heads_fwd_kernel<true, 64> : coalibi_heads_fwd_kernel<false, 64>);
+  return heads_result(launch_pdl(kernel, dim3(heads_ctas(p.tokens)), dim3(heads_threads(p, a->D)), 0,
+                                 static_cast<cudaStream_t>(stream), p),
+                      "heads launch");
+}
+
+extern "C" size_t coalibi_heads_bwd_workspace_bytes(int D) {
+  return D == 64 || D == 128 ? (size_t)kPagedMaxSms * kHeadsCtas * 2 * D * 4 : 0;
+}
+
+extern "C" int coalibi_heads_bwd(const CoalibiHeadsArgs* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_heads(a, true)) return rc;
+  if (!aligned(a->dq_weight, 4) || !aligned(a->dk_weight, 4)) return COALIBI_ERR_ALIGNMENT;
+  if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < coalibi_heads_bwd_workspace_bytes(a->D))
+    return COALIBI_ERR_WORKSPACE;
+  CtxGuard guard;
+  if (int rc = enter_device(a->qkv, stream)) return rc;
+  HeadsParams p = heads_params(a);
+  p.in[0] = a->q;
+  p.in[1] = a->k;
+  p.in[2] = a->v;
+  p.dqkv = a->dqkv;
+  p.partial = static_cast<float*>(workspace);
+  p.dweight[0] = a->dq_weight;
+  p.dweight[1] = a->dk_weight;
+  const bool bf16 = a->dtype == COALIBI_BF16;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int ctas = std::min(heads_ctas(p.tokens), kPagedMaxSms * kHeadsCtas);
+  auto kernel = a->D == 128 ? (bf16 ? coalibi_heads_bwd_kernel<true, 128> : coalibi_heads_bwd_kernel<false, 128>)
+                            : (bf16 ? coalibi_heads_bwd_kernel<true, 64> : coalibi_heads_bwd_kernel<false, 64>);
+  auto sum = a->D == 128 ? (bf16 ? coalibi_heads_sum_kernel<true, 128> : coalibi_heads_sum_kernel<false, 128>)
+                         : (bf16 ? coalibi_heads_sum_kernel<true, 64> : coalibi_heads_sum_kernel<false, 64>);
+  cudaError_t e = launch_pdl(kernel, dim3(ctas), dim3(heads_threads(p, a->D)), 0, s, p);
+  if (e == cudaSuccess && (a->dq_weight || a->dk_weight)) e = launch_pdl(sum, dim3(2 * a->D / 8), dim3(256), 0, s, p, ctas);
+  return heads_result(e, "heads backward launch");
+}

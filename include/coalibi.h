@@ -43,7 +43,8 @@ extern "C" {
 enum coalibi_dtype {
   COALIBI_F16 = 0,
   COALIBI_BF16 = 1,
-  COALIBI_F32 = 2 /* only valid for slopes_dtype */
+  COALIBI_F32 = 2, /* only valid for slopes_dtype and weight_dtype */
+  COALIBI_E4M3 = 3 /* the codes of an 8-bit cache; no argument takes it */
 };
 
 enum coalibi_error {
@@ -282,6 +283,85 @@ typedef struct CoalibiPagedAttentionArgs {
 size_t coalibi_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int Sq, int D);
 int coalibi_paged_attention(const CoalibiPagedAttentionArgs* args, void* workspace, size_t workspace_bytes,
                             void* stream);
+
+/* The same cache in 8 bits.  k_pages and v_pages hold e4m3 codes (strides multiples of 16), and each
+ * block of 16 tokens of a page and head has a float32 scale, a power of two, at page * stride[0] +
+ * head * stride[1] + slot / 16: a value is its code times the scale of its block. */
+#define COALIBI_QUANT_BLOCK 16
+typedef struct CoalibiCacheScales {
+  float* k; /* [n_pages, Hkv, page_size / 16] */
+  float* v;
+  long long k_stride[2], v_stride[2]; /* page, head */
+} CoalibiCacheScales;
+
+/* coalibi_paged_append into such a cache.  A block that the new tokens begin takes the least power of
+ * two, and at least 2^-100, by which its largest finite value is at most 448; one that held tokens before
+ * them keeps its scale unless that is smaller, and if not its old codes move to the new scale.  Values are
+ * rounded once, rotated keys from float32; infinities become NaN. */
+int coalibi_paged_append8(const CoalibiPagedAppendArgs* args, const CoalibiCacheScales* scales, void* stream);
+
+/* coalibi_paged_attention over such a cache; the workspace is that of
+ * coalibi_paged_attention8_workspace_bytes(). */
+size_t coalibi_paged_attention8_workspace_bytes(int B, int Hq, int Hkv, int Sq, int D);
+int coalibi_paged_attention8(const CoalibiPagedAttentionArgs* args, const CoalibiCacheScales* scales, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Tokens of such a cache in 16 bits: token positions[b, i] of request b becomes row i of k and v.
+ * Rows of a negative position are zero, and so are those outside the table or the pool, which are
+ * reported.  Values are rounded once; one past the type's largest is that. */
+typedef struct CoalibiPagedReadArgs {
+  const void* k_pages;
+  const void* v_pages;
+  const int* page_table;  /* [B, max_pages] */
+  const int* positions;   /* [B, S] contiguous */
+  void* k;                /* [B, Hkv, S, D] contiguous, dtype */
+  void* v;
+  int* status;
+  long long k_page_stride[3], v_page_stride[3]; /* page, head, slot */
+  long long table_stride;
+  int B, Hkv, S, D;
+  int page_size, max_pages, n_pages;
+  int dtype;
+} CoalibiPagedReadArgs;
+
+int coalibi_paged_read8(const CoalibiPagedReadArgs* args, const CoalibiCacheScales* scales, void* stream);
+
+/* Heads of a fused projection.  qkv [B, S, Hq + 2 Hkv, D]: query, key and value heads of each token.
+ * Forward: q [B, Hq, S, D], k and v [B, Hkv, S, D] by stride; with x a row of a query or key head,
+ *   y = R(x / sqrt(mean(x^2) + eps) * weight),
+ * R the rotation of coalibi_paged_append by the angles of position positions[b, i], else start[b] + i,
+ * else i (rot = 0: none; a position outside the table leaves the row unrotated and is reported as
+ * COALIBI_ERR_PAGE); values are moved.  Arithmetic is float32, rounded once.
+ * Backward: q, k and v are the gradients of the three (read); dqkv [B, S, Hq + 2 Hkv, D] contiguous, and
+ * dq_weight, dk_weight [D] (weight_dtype; NULL: not wanted) are written.  Sums are float32, in a fixed
+ * order: results repeat bit for bit.  workspace: coalibi_heads_bwd_workspace_bytes(), 16-byte aligned,
+ * contents on entry irrelevant, not shared by calls that may overlap. */
+typedef struct CoalibiHeadsArgs {
+  const void* qkv;
+  void* q;
+  void* k;
+  void* v;
+  const void* q_weight;  /* [D]; NULL: ones */
+  const void* k_weight;
+  const float* cos;      /* [n_pos, rot / 2]; NULL with rot = 0 */
+  const float* sin;
+  const int* start;      /* [B]; NULL: 0 */
+  const int* positions;  /* [B, S] contiguous; NULL: start[b] + i */
+  int* status;           /* optional device int */
+  void* dqkv;
+  void* dq_weight;
+  void* dk_weight;
+  long long qkv_stride[3];                        /* batch, token, head; multiples of 8 */
+  long long q_stride[3], k_stride[3], v_stride[3]; /* batch, head, token; multiples of 8 */
+  int B, S, Hq, Hkv, D;
+  int rot, n_pos, interleaved; /* rot: a multiple of 16, at most D */
+  int dtype, weight_dtype;     /* weight_dtype: dtype or COALIBI_F32 */
+  float eps;
+} CoalibiHeadsArgs;
+
+int coalibi_heads_fwd(const CoalibiHeadsArgs* args, void* stream);
+size_t coalibi_heads_bwd_workspace_bytes(int D);
+int coalibi_heads_bwd(const CoalibiHeadsArgs* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Draw one token for each row of logits.  Tokens are ranked by (logit descending,
  * index ascending) and weighted w = exp((logit - max) / temperature); kept are the
