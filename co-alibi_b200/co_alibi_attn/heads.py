@@ -11,6 +11,10 @@ from .serving import _native
 __all__ = ["norm_rotate_qkv"]
 
 
+def _requires_grad(t):
+    return isinstance(t, torch.Tensor) and t.requires_grad
+
+
 class _NormRotateQKV(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, q_weight, k_weight, num_heads, num_kv_heads, eps, rotary, start, positions, interleaved):
@@ -47,10 +51,13 @@ def norm_rotate_qkv(qkv, num_heads, num_kv_heads, q_weight=None, k_weight=None, 
     tables leaves the row unrotated and is reported by ``device_status()`` as code 11.  Values are
     moved as they are.  Arithmetic is float32, rounded once.
 
-    Gradients reach ``qkv`` and the weights (their sums are float32, added in a fixed order: results
-    repeat bit for bit), not the tables; there is no second derivative."""
+    Gradients reach ``qkv`` and the weights (the weights' sums are float32, added in a fixed order: results
+    repeat bit for bit); tables that require one are refused, and there is no second derivative."""
     assert qkv.is_cuda, "Inputs must be CUDA tensors"
-    if rotary is not None and any(isinstance(t, torch.Tensor) and t.requires_grad for t in rotary) and torch.is_grad_enabled():
-        raise RuntimeError("co_alibi_attn: norm_rotate_qkv: the rotary tables require grad, but get none: detach them")
+    if not torch.is_grad_enabled() or not (qkv.requires_grad or _requires_grad(q_weight) or _requires_grad(k_weight)):
+        return _native().heads_fwd(qkv, num_heads, num_kv_heads, q_weight, k_weight, eps, rotary, start, positions,
+                                   interleaved, _status_word(qkv.device))
+    if rotary is not None and any(_requires_grad(t) for t in rotary):
+        raise RuntimeError("co_alibi_attn: norm_rotate_qkv: the rotary tables require grad, but get none")
     return _NormRotateQKV.apply(qkv, q_weight, k_weight, num_heads, num_kv_heads, eps, rotary, start, positions,
                                 interleaved)

@@ -458,6 +458,7 @@ Heads heads_of(PyObject* const* a) {
   p.eps = (float)eps;
   if (a[6] != Py_None) {
     rotary_of(a[6], what, h.D, device, h.cos, h.sin);
+    no_grad(what, "cos", h.cos), no_grad(what, "sin", h.sin);
     p.cos = h.cos.data_ptr<float>();
     p.sin = h.sin.data_ptr<float>();
     p.n_pos = (int)h.cos.size(0);

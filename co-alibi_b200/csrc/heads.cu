@@ -2,6 +2,8 @@
 // are checked before any device use; nothing here allocates or synchronises.
 #include "heads.cuh"
 
+#include <algorithm>
+
 #include "serving_host.cuh"
 
 using namespace coalibi;
@@ -9,17 +11,9 @@ using namespace coalibi;
 namespace coalibi {
 namespace {
 
-int heads_passes(int H, int pieces) {
-  const int most = kHeadsThreads / pieces;
-  return (H + most - 1) / most;
-}
-
-constexpr int kHeadsCtas = 16;  // to an SM, at most
-
-int heads_ctas(long long tokens) {
-  const long long most = (long long)device_sm_count() * kHeadsCtas;
-  return (int)(tokens < most ? tokens : most);
-}
+constexpr int kHeadsWaves = 12;  // CTAs to an SM in all, about
+// Of CTAs, at most: the above, or one for each chunk.
+constexpr size_t kHeadsMostCtas = std::max(kHeadsWaves * kPagedMaxSms, 3 * (65535 / kHeadsChunk + 1));
 
 int check_heads(const CoalibiHeadsArgs* a, bool backward) {
   if (a == nullptr || !a->qkv || !a->q || !a->k || !a->v) return COALIBI_ERR_NULL_POINTER;
@@ -55,21 +49,42 @@ HeadsParams heads_params(const CoalibiHeadsArgs* a) {
   copy3(p.hs[0], a->q_stride);
   copy3(p.hs[1], a->k_stride);
   copy3(p.hs[2], a->v_stride);
-  p.tokens = (long long)a->B * a->S;
+  p.tokens = a->B * a->S;
   p.Hq = a->Hq;
   p.Hkv = a->Hkv;
   p.S = a->S;
-  const int H = a->Hq + 2 * a->Hkv, passes = heads_passes(H, a->D / 8);
-  p.rows = (H + passes - 1) / passes;
+  for (int i = 0; i < 2; ++i) {
+    const int H = i ? a->Hkv : a->Hq;
+    p.chunks[i] = (H + kHeadsChunk - 1) / kHeadsChunk;
+    p.per[i] = (H + p.chunks[i] - 1) / p.chunks[i];
+    p.chunks[i] = (H + p.per[i] - 1) / p.per[i];
+  }
+  const int slots = kHeadsThreads / (a->D / 16), chunks = p.chunks[0] + 2 * p.chunks[1];
+  p.groups = (p.tokens - 1) / slots + 1;
+  p.ctas = std::min(p.groups, std::max(1, kHeadsWaves * std::min(device_sm_count(), kPagedMaxSms) / chunks));
+  p.per_cta = (p.groups - 1) / p.ctas + 1;
+  p.ctas = (p.groups - 1) / p.per_cta + 1;
   p.rot = a->rot;
   p.n_pos = a->n_pos;
-  p.interleaved = a->interleaved;
   p.weight_f32 = a->weight_dtype == COALIBI_F32;
   p.eps = a->eps;
   return p;
 }
 
-int heads_threads(const HeadsParams& p, int D) { return (p.rows * (D / 8) + 31) / 32 * 32; }
+unsigned heads_grid(const HeadsParams& p) { return (unsigned)(p.ctas * (p.chunks[0] + 2 * p.chunks[1])); }
+
+template <bool PAIRS>
+auto heads_fwd_kernel(const CoalibiHeadsArgs* a) {
+  const bool bf16 = a->dtype == COALIBI_BF16;
+  return a->D == 128 ? (bf16 ? coalibi_heads_fwd_kernel<true, 128, PAIRS> : coalibi_heads_fwd_kernel<false, 128, PAIRS>)
+                     : (bf16 ? coalibi_heads_fwd_kernel<true, 64, PAIRS> : coalibi_heads_fwd_kernel<false, 64, PAIRS>);
+}
+template <bool PAIRS>
+auto heads_bwd_kernel(const CoalibiHeadsArgs* a) {
+  const bool bf16 = a->dtype == COALIBI_BF16;
+  return a->D == 128 ? (bf16 ? coalibi_heads_bwd_kernel<true, 128, PAIRS> : coalibi_heads_bwd_kernel<false, 128, PAIRS>)
+                     : (bf16 ? coalibi_heads_bwd_kernel<true, 64, PAIRS> : coalibi_heads_bwd_kernel<false, 64, PAIRS>);
+}
 
 int heads_result(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return launched(what);
@@ -88,16 +103,13 @@ extern "C" int coalibi_heads_fwd(const CoalibiHeadsArgs* a, void* stream) {
   p.out[0] = a->q;
   p.out[1] = a->k;
   p.out[2] = a->v;
-  const bool bf16 = a->dtype == COALIBI_BF16;
-  auto kernel = a->D == 128 ? (bf16 ? coalibi_heads_fwd_kernel<true, 128> : coalibi_heads_fwd_kernel<false, 128>)
-                            : (bf16 ? coalibi_heads_fwd_kernel<true, 64> : coalibi_heads_fwd_kernel<false, 64>);
-  return heads_result(launch_pdl(kernel, dim3(heads_ctas(p.tokens)), dim3(heads_threads(p, a->D)), 0,
-                                 static_cast<cudaStream_t>(stream), p),
-                      "heads launch");
+  auto kernel = a->interleaved ? heads_fwd_kernel<true>(a) : heads_fwd_kernel<false>(a);
+  return heads_result(
+      launch_pdl(kernel, dim3(heads_grid(p)), dim3(kHeadsThreads), 0, static_cast<cudaStream_t>(stream), p), "heads launch");
 }
 
 extern "C" size_t coalibi_heads_bwd_workspace_bytes(int D) {
-  return D == 64 || D == 128 ? (size_t)kPagedMaxSms * kHeadsCtas * 2 * D * 4 : 0;
+  return D == 64 || D == 128 ? kHeadsMostCtas * D * 4 : 0;
 }
 
 extern "C" int coalibi_heads_bwd(const CoalibiHeadsArgs* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -115,14 +127,12 @@ extern "C" int coalibi_heads_bwd(const CoalibiHeadsArgs* a, void* workspace, siz
   p.partial = static_cast<float*>(workspace);
   p.dweight[0] = a->dq_weight;
   p.dweight[1] = a->dk_weight;
-  const bool bf16 = a->dtype == COALIBI_BF16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int ctas = std::min(heads_ctas(p.tokens), kPagedMaxSms * kHeadsCtas);
-  auto kernel = a->D == 128 ? (bf16 ? coalibi_heads_bwd_kernel<true, 128> : coalibi_heads_bwd_kernel<false, 128>)
-                            : (bf16 ? coalibi_heads_bwd_kernel<true, 64> : coalibi_heads_bwd_kernel<false, 64>);
+  const bool bf16 = a->dtype == COALIBI_BF16;
+  auto kernel = a->interleaved ? heads_bwd_kernel<true>(a) : heads_bwd_kernel<false>(a);
   auto sum = a->D == 128 ? (bf16 ? coalibi_heads_sum_kernel<true, 128> : coalibi_heads_sum_kernel<false, 128>)
                          : (bf16 ? coalibi_heads_sum_kernel<true, 64> : coalibi_heads_sum_kernel<false, 64>);
-  cudaError_t e = launch_pdl(kernel, dim3(ctas), dim3(heads_threads(p, a->D)), 0, s, p);
-  if (e == cudaSuccess && (a->dq_weight || a->dk_weight)) e = launch_pdl(sum, dim3(2 * a->D / 8), dim3(256), 0, s, p, ctas);
+  cudaError_t e = launch_pdl(kernel, dim3(heads_grid(p)), dim3(kHeadsThreads), 0, s, p);
+  if (e == cudaSuccess && (a->dq_weight || a->dk_weight)) e = launch_pdl(sum, dim3(2 * a->D / 32), dim3(1024), 0, s, p);
   return heads_result(e, "heads backward launch");
 }

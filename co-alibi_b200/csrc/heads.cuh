@@ -6,9 +6,10 @@
 //
 // Bound by the bytes: the projection read once and the heads written once (forward); the projection and
 // the heads' gradients read, the projection's gradient written (backward; r is computed again rather than
-// kept).  D / 8 lanes take a row, each two pieces of 4 columns: those of a lane that rotates are the
-// two partners of each pair, so a rotation needs no exchange and half the angles.  A CTA takes a token at a
-// time and its threads several heads of it by the same angles.
+// kept).  D / 16 lanes take a row, 16 columns each: those of a lane that rotates are both partners of its 8
+// pairs, so a rotation needs no exchange.  A lane keeps its token and goes over a chunk of heads of one kind,
+// with the token's angles and the kind's weights in registers; the sums of a weight's gradient are a lane's own
+// until the end.
 #pragma once
 
 #include "sm100.cuh"
@@ -26,19 +27,24 @@ struct HeadsParams {
   const int* start;
   const int* positions;
   int* status;
-  float* partial;         // backward: [gridDim][2][D]
+  float* partial;         // backward: [2][most CTAs of a kind][D]
   void* dweight[2];
   long long xs[3];        // batch, token, head
   long long hs[3][3];     // of q, k, v: batch, head, token
-  long long tokens;       // B * S
+  int tokens;             // B * S
   int Hq, Hkv, S;
-  int rows;               // heads that a pass of the CTA covers
-  int rot, n_pos, interleaved;
+  int per[2];             // heads of a chunk: of queries, of keys and values
+  int chunks[2];          // chunks of queries, of keys (and as many of values)
+  int groups;             // token groups, one token to a slot of a CTA
+  int per_cta;            // groups that a CTA goes over
+  int ctas;               // for a chunk
+  int rot, n_pos;
   int weight_f32;
   float eps;
 };
 
-constexpr int kHeadsThreads = 128;  // at most
+constexpr int kHeadsThreads = 256;
+constexpr int kHeadsChunk = 8;  // heads, at most
 
 // A weight of column c, as float.
 template <bool BF16>
@@ -49,19 +55,74 @@ __device__ __forceinline__ float load_weight(const void* w, int f32, int c) {
   return unpack2<BF16>(u).x;
 }
 
-// Where a lane's columns and angles are.  Piece l of a row: partners 4 l .. and R / 2 + 4 l .. of a rotation
-// in halves, else columns 8 l .. 8 l + 7.
+// A lane's 16 columns as the partners a and b of 8 pairs.  In halves (and where nothing turns) the pairs
+// are (c0 + e, c1 + e), of two pieces of 8 columns; interleaved, neighbours.
+struct HeadsRow {
+  float2 a[4], b[4];
+};
+template <bool BF16, bool PAIRS>
+__device__ __forceinline__ void heads_unpack(const uint4& p0, const uint4& p1, HeadsRow& x) {
+  const uint32_t w0[4] = {p0.x, p0.y, p0.z, p0.w}, w1[4] = {p1.x, p1.y, p1.z, p1.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (PAIRS) {
+      const float2 u = unpack2<BF16>(e < 2 ? w0[2 * e] : w1[2 * e - 4]), v = unpack2<BF16>(e < 2 ? w0[2 * e + 1] : w1[2 * e - 3]);
+      x.a[e] = make_float2(u.x, v.x);
+      x.b[e] = make_float2(u.y, v.y);
+    } else {
+      x.a[e] = unpack2<BF16>(w0[e]);
+      x.b[e] = unpack2<BF16>(w1[e]);
+    }
+  }
+}
+template <bool BF16, bool PAIRS>
+__device__ __forceinline__ void heads_pack(const HeadsRow& x, uint4& p0, uint4& p1) {
+  uint32_t w0[4], w1[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (PAIRS) {
+      (e < 2 ? w0[2 * e & 3] : w1[2 * e & 3]) = pack2<BF16>(x.a[e].x, x.b[e].x);
+      (e < 2 ? w0[(2 * e & 3) + 1] : w1[(2 * e & 3) + 1]) = pack2<BF16>(x.a[e].y, x.b[e].y);
+    } else {
+      w0[e] = pack2<BF16>(x.a[e].x, x.a[e].y);
+      w1[e] = pack2<BF16>(x.b[e].x, x.b[e].y);
+    }
+  }
+  p0 = make_uint4(w0[0], w0[1], w0[2], w0[3]);
+  p1 = make_uint4(w1[0], w1[1], w1[2], w1[3]);
+}
+__device__ __forceinline__ float2 splat(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 neg2(float2 x) { return make_float2(-x.x, -x.y); }
+
+// Where a lane's columns and angles are (row l of D / 16 in a row).
 struct HeadsLane {
   int c0, c1;
   bool turns;
 };
-__device__ __forceinline__ HeadsLane heads_lane(int l, int rot, int interleaved) {
+template <bool PAIRS>
+__device__ __forceinline__ HeadsLane heads_lane(int l, int rot) {
   HeadsLane t;
-  t.turns = 8 * l < rot;
-  const bool halves = t.turns && !interleaved;
-  t.c0 = halves ? 4 * l : 8 * l;
-  t.c1 = halves ? rot / 2 + 4 * l : 8 * l + 4;
+  t.turns = 16 * l < rot;
+  const bool halves = t.turns && !PAIRS;
+  t.c0 = halves ? 8 * l : 16 * l;
+  t.c1 = halves ? rot / 2 + 8 * l : 16 * l + 8;
   return t;
+}
+// The weights of a kind in shared memory, in the order of each lane's pairs: piece e (a's first and last four,
+// b's) of lane l at (e * LANES + l) * 4, so that a load takes every bank once.
+template <bool BF16, bool PAIRS, int D>
+__device__ __forceinline__ void heads_weights(const HeadsParams& p, int kind, float* s_w) {
+  constexpr int LANES = D / 16;
+  for (int at = threadIdx.x; at < D; at += kHeadsThreads) {
+    const int e = at / (4 * LANES), l = at / 4 % LANES, i = e % 2 * 4 + at % 4;  // pair i, a or b of it
+    const HeadsLane t = heads_lane<PAIRS>(l, p.rot);
+    const int c = PAIRS ? (i < 4 ? t.c0 + 2 * i : t.c1 + 2 * i - 8) + e / 2 : (e < 2 ? t.c0 : t.c1) + i;
+    s_w[at] = load_weight<BF16>(p.weight[kind], p.weight_f32, c);
+  }
+}
+template <int LANES>
+__device__ __forceinline__ float4 heads_weight(const float* s_w, int l, int e) {
+  return *reinterpret_cast<const float4*>(s_w + (e * LANES + l) * 4);
 }
 
 // The row of the angles of token i of request b, or -1.
@@ -73,223 +134,283 @@ __device__ __forceinline__ int heads_angle(const HeadsParams& p, int b, int i, b
   if (reports && p.status != nullptr) atomicCAS(p.status, 0, 11 /* COALIBI_ERR_PAGE */);
   return -1;
 }
-
-template <bool BF16>
-__device__ __forceinline__ void heads_unpack(uint2 a, uint2 b, float* f) {
-  const uint32_t w[4] = {a.x, a.y, b.x, b.y};
+struct HeadsAngles {
+  float2 c[4], s[4];
+};
+// Whether the lane turns its pairs; if so, their angles.
+__device__ __forceinline__ bool heads_angles(const HeadsParams& p, const HeadsLane& t, int l, int b, int i, bool valid, HeadsAngles& g) {
+  if (!valid || !t.turns) return false;
+  const int row = heads_angle(p, b, i, l == 0);
+  if (row < 0) return false;
+  const float4* c = reinterpret_cast<const float4*>(p.cos + (size_t)row * (p.rot / 2) + 8 * l);
+  const float4* s = reinterpret_cast<const float4*>(p.sin + (size_t)row * (p.rot / 2) + 8 * l);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const float4 u = c[e], v = s[e];
+    g.c[2 * e] = make_float2(u.x, u.y), g.c[2 * e + 1] = make_float2(u.z, u.w);
+    g.s[2 * e] = make_float2(v.x, v.y), g.s[2 * e + 1] = make_float2(v.z, v.w);
+  }
+  return true;
+}
+// The pairs turned by the angles, or back by them.
+template <bool BACK>
+__device__ __forceinline__ void heads_turn(HeadsRow& x, const HeadsAngles& g) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float2 u = unpack2<BF16>(w[e]);
-    f[2 * e] = u.x, f[2 * e + 1] = u.y;
-  }
-}
-template <bool BF16>
-__device__ __forceinline__ void heads_store(uint16_t* y, const HeadsLane& t, const float* f) {
-  *reinterpret_cast<uint2*>(y + t.c0) = make_uint2(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]));
-  *reinterpret_cast<uint2*>(y + t.c1) = make_uint2(pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
-}
-
-// f's pairs turned by angles (cs, sign * sn): pairs (f[e], f[e + 4]) in halves, (f[2 e], f[2 e + 1]) interleaved.
-__device__ __forceinline__ void heads_turn(float* f, const float4& cs, const float4& sn, float sign, int interleaved) {
-  const float c[4] = {cs.x, cs.y, cs.z, cs.w}, s[4] = {sign * sn.x, sign * sn.y, sign * sn.z, sign * sn.w};
-  if (interleaved) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float a = f[2 * e], b = f[2 * e + 1];
-      f[2 * e] = a * c[e] - b * s[e];
-      f[2 * e + 1] = b * c[e] + a * s[e];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float a = f[e], b = f[e + 4];
-      f[e] = a * c[e] - b * s[e];
-      f[e + 4] = b * c[e] + a * s[e];
-    }
+    const float2 a = x.a[e], b = x.b[e], s = BACK ? neg2(g.s[e]) : g.s[e];
+    x.a[e] = __ffma2_rn(b, neg2(s), __fmul2_rn(a, g.c[e]));
+    x.b[e] = __ffma2_rn(a, s, __fmul2_rn(b, g.c[e]));
   }
 }
 
-template <bool BF16, int D>
-__global__ void __launch_bounds__(kHeadsThreads) coalibi_heads_fwd_kernel(const HeadsParams p) {
-  constexpr int PIECES = D / 8, UNROLL = 3;
-  __shared__ __align__(16) float s_w[2][D];
+// What a CTA goes over: heads [h0, h0 + n) of a kind (0 queries, 1 keys, 2 values), token groups from `group`.
+struct HeadsWork {
+  int kind, h0, n, row0, group, end, index;  // row0: of the heads in the projection; index: of the CTA in its kind
+};
+__device__ __forceinline__ HeadsWork heads_work(const HeadsParams& p) {
+  HeadsWork w;
+  int chunk = blockIdx.x / p.ctas;
+  const int at = blockIdx.x - chunk * p.ctas;
+  w.index = chunk * p.ctas + at;
+  w.kind = 0;
+  if (chunk >= p.chunks[0]) {
+    chunk -= p.chunks[0];
+    w.index -= p.chunks[0] * p.ctas;
+    w.kind = 1;
+    if (chunk >= p.chunks[1]) {
+      chunk -= p.chunks[1];
+      w.kind = 2;
+    }
+  }
+  const int per = p.per[w.kind > 0], H = w.kind == 0 ? p.Hq : p.Hkv;
+  w.h0 = chunk * per;
+  w.n = min(per, H - w.h0);
+  w.row0 = (w.kind == 0 ? 0 : w.kind == 1 ? p.Hq : p.Hq + p.Hkv) + w.h0;
+  w.group = at * p.per_cta;
+  w.end = min(w.group + p.per_cta, p.groups);
+  return w;
+}
+
+template <bool BF16, int D, bool PAIRS>
+__global__ void __launch_bounds__(kHeadsThreads, 3) coalibi_heads_fwd_kernel(const HeadsParams p) {
+  constexpr int LANES = D / 16, SLOTS = kHeadsThreads / LANES;
+  __shared__ __align__(16) float s_w[D];
   grid_dep_wait();
-  const int tid = threadIdx.x, l = tid % PIECES, r0 = tid / PIECES;
-  for (int e = tid; e < 2 * D; e += blockDim.x) s_w[e / D][e % D] = load_weight<BF16>(p.weight[e / D], p.weight_f32, e % D);
+  const int l = threadIdx.x % LANES, slot = threadIdx.x / LANES;
+  const HeadsWork w = heads_work(p);
+  const HeadsLane t = heads_lane<PAIRS>(l, p.rot);
+  if (w.kind < 2) heads_weights<BF16, PAIRS, D>(p, w.kind, s_w);
   __syncthreads();
-  const HeadsLane t = heads_lane(l, p.rot, p.interleaved);
-  const int H = p.Hq + 2 * p.Hkv, Hn = p.Hq + p.Hkv;
-  for (long long tok = blockIdx.x; tok < p.tokens; tok += gridDim.x) {
-    const int b = (int)(tok / p.S), i = (int)(tok - (long long)b * p.S);
-    const uint16_t* x = static_cast<const uint16_t*>(p.qkv) + b * p.xs[0] + i * p.xs[1];
-    const int angle = heads_angle(p, b, i, tid == 0);
-    float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
-    const bool turns = t.turns && angle >= 0;
-    if (turns) {
-      cs = *reinterpret_cast<const float4*>(p.cos + (size_t)angle * (p.rot / 2) + 4 * l);
-      sn = *reinterpret_cast<const float4*>(p.sin + (size_t)angle * (p.rot / 2) + 4 * l);
-    }
-    // (the same passes for all threads: the reductions take whole warps)
-    for (int base = 0; base < H; base += UNROLL * p.rows) {
-      uint2 u0[UNROLL], u1[UNROLL];
-#pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const int row = base + u * p.rows + r0;
-        u0[u] = u1[u] = make_uint2(0u, 0u);
-        if (row < H && r0 < p.rows) {
-          u0[u] = *reinterpret_cast<const uint2*>(x + row * p.xs[2] + t.c0);
-          u1[u] = *reinterpret_cast<const uint2*>(x + row * p.xs[2] + t.c1);
-        }
+  for (int group = w.group; group < w.end; ++group) {
+    const int tok = group * SLOTS + slot;
+    const bool valid = tok < p.tokens;
+    const int b = valid ? tok / p.S : 0, i = valid ? tok - b * p.S : 0;
+    const uint16_t* x = static_cast<const uint16_t*>(p.qkv) + b * p.xs[0] + i * p.xs[1] + w.row0 * p.xs[2];
+    uint16_t* y = static_cast<uint16_t*>(p.out[w.kind]) + b * p.hs[w.kind][0] + w.h0 * p.hs[w.kind][1] + i * p.hs[w.kind][2];
+    const long long xh = p.xs[2], yh = p.hs[w.kind][1];
+    HeadsAngles g;
+    const bool turns = w.kind < 2 && heads_angles(p, t, l, b, i, valid, g);
+    struct Piece {
+      uint4 u0, u1;
+    };
+    auto load = [&](int h) {
+      Piece r{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+      if (valid && h < w.n) {
+        r.u0 = *reinterpret_cast<const uint4*>(x + h * xh + t.c0);
+        r.u1 = *reinterpret_cast<const uint4*>(x + h * xh + t.c1);
       }
+      return r;
+    };
+    Piece now = load(0), next = load(1);
+#pragma unroll 1
+    for (int h = 0; h < w.n; ++h) {
+      const Piece after = load(h + 2);
+      if (w.kind < 2) {
+        HeadsRow f;
+        heads_unpack<BF16, PAIRS>(now.u0, now.u1, f);
+        float2 ss2 = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        if (base + u * p.rows >= H) break;
-        const int row = base + u * p.rows + r0;
-        float f[8];
-        heads_unpack<BF16>(u0[u], u1[u], f);
-        float ss = 0.f;
+        for (int e = 0; e < 4; ++e) ss2 = __ffma2_rn(f.b[e], f.b[e], __ffma2_rn(f.a[e], f.a[e], ss2));
+        float ss = ss2.x + ss2.y;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+        for (int d = 1; d < LANES; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+        const float2 r = splat(rsqrtf(ss * (1.f / D) + p.eps));
 #pragma unroll
-        for (int d = 1; d < PIECES; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-        if (row >= H || r0 >= p.rows) continue;
-        const int kind = row < p.Hq ? 0 : row < Hn ? 1 : 2;
-        const int h = kind == 0 ? row : kind == 1 ? row - p.Hq : row - Hn;
-        uint16_t* y = static_cast<uint16_t*>(p.out[kind]) + b * p.hs[kind][0] + h * p.hs[kind][1] + i * p.hs[kind][2];
-        if (kind == 2) {
-          *reinterpret_cast<uint2*>(y + t.c0) = u0[u];
-          *reinterpret_cast<uint2*>(y + t.c1) = u1[u];
-          continue;
+        for (int e = 0; e < 4; e += 2) {
+          const float4 wa = heads_weight<LANES>(s_w, l, e / 2), wb = heads_weight<LANES>(s_w, l, 2 + e / 2);
+          f.a[e] = __fmul2_rn(__fmul2_rn(f.a[e], r), make_float2(wa.x, wa.y));
+          f.a[e + 1] = __fmul2_rn(__fmul2_rn(f.a[e + 1], r), make_float2(wa.z, wa.w));
+          f.b[e] = __fmul2_rn(__fmul2_rn(f.b[e], r), make_float2(wb.x, wb.y));
+          f.b[e + 1] = __fmul2_rn(__fmul2_rn(f.b[e + 1], r), make_float2(wb.z, wb.w));
         }
-        const float r = rsqrtf(ss * (1.f / D) + p.eps);
-        const float4 w0 = *reinterpret_cast<const float4*>(&s_w[kind][t.c0]), w1 = *reinterpret_cast<const float4*>(&s_w[kind][t.c1]);
-        const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = f[e] * r * w[e];
-        if (turns) heads_turn(f, cs, sn, 1.f, p.interleaved);
-        heads_store<BF16>(y, t, f);
+        if (turns) heads_turn<false>(f, g);
+        heads_pack<BF16, PAIRS>(f, now.u0, now.u1);
       }
+      if (valid) {
+        *reinterpret_cast<uint4*>(y + h * yh + t.c0) = now.u0;
+        *reinterpret_cast<uint4*>(y + h * yh + t.c1) = now.u1;
+      }
+      now = next;
+      next = after;
     }
   }
 }
 
-template <bool BF16, int D>
-__global__ void __launch_bounds__(kHeadsThreads) coalibi_heads_bwd_kernel(const HeadsParams p) {
-  constexpr int PIECES = D / 8, UNROLL = 3;
-  __shared__ __align__(16) float s_w[2][D];
-  __shared__ __align__(16) float s_sum[kHeadsThreads / PIECES][D];
+template <bool BF16, int D, bool PAIRS>
+__global__ void __launch_bounds__(kHeadsThreads, 2) coalibi_heads_bwd_kernel(const HeadsParams p) {
+  constexpr int LANES = D / 16, SLOTS = kHeadsThreads / LANES, UNROLL = 4;
+  __shared__ __align__(16) float s_w[D], s_sum[kHeadsThreads / 32][D];
   grid_dep_wait();
-  const int tid = threadIdx.x, l = tid % PIECES, r0 = tid / PIECES;
-  for (int e = tid; e < 2 * D; e += blockDim.x) s_w[e / D][e % D] = load_weight<BF16>(p.weight[e / D], p.weight_f32, e % D);
+  const int l = threadIdx.x % LANES, slot = threadIdx.x / LANES;
+  const HeadsWork w = heads_work(p);
+  const HeadsLane t = heads_lane<PAIRS>(l, p.rot);
+  const int H = p.Hq + 2 * p.Hkv;
+  if (w.kind < 2) heads_weights<BF16, PAIRS, D>(p, w.kind, s_w);
   __syncthreads();
-  const HeadsLane t = heads_lane(l, p.rot, p.interleaved);
-  const int H = p.Hq + 2 * p.Hkv, Hn = p.Hq + p.Hkv;
-  float dw[2][8];
+  HeadsRow dw;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) dw[0][e] = dw[1][e] = 0.f;
-  for (long long tok = blockIdx.x; tok < p.tokens; tok += gridDim.x) {
-    const int b = (int)(tok / p.S), i = (int)(tok - (long long)b * p.S);
-    const uint16_t* x = static_cast<const uint16_t*>(p.qkv) + b * p.xs[0] + i * p.xs[1];
-    uint16_t* dx = static_cast<uint16_t*>(p.dqkv) + (size_t)tok * H * D;
-    const int angle = heads_angle(p, b, i, tid == 0);
-    float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
-    const bool turns = t.turns && angle >= 0;
-    if (turns) {
-      cs = *reinterpret_cast<const float4*>(p.cos + (size_t)angle * (p.rot / 2) + 4 * l);
-      sn = *reinterpret_cast<const float4*>(p.sin + (size_t)angle * (p.rot / 2) + 4 * l);
-    }
-    for (int base = 0; base < H; base += UNROLL * p.rows) {
-      uint2 u0[UNROLL], u1[UNROLL], g0[UNROLL], g1[UNROLL];
+  for (int e = 0; e < 4; ++e) dw.a[e] = dw.b[e] = make_float2(0.f, 0.f);
+  for (int group = w.group; group < w.end; ++group) {
+    const int tok = group * SLOTS + slot;
+    const bool valid = tok < p.tokens;
+    const int b = valid ? tok / p.S : 0, i = valid ? tok - b * p.S : 0;
+    const uint16_t* x = static_cast<const uint16_t*>(p.qkv) + b * p.xs[0] + i * p.xs[1] + w.row0 * p.xs[2];
+    const uint16_t* dy =
+        static_cast<const uint16_t*>(p.in[w.kind]) + b * p.hs[w.kind][0] + w.h0 * p.hs[w.kind][1] + i * p.hs[w.kind][2];
+    uint16_t* dx = static_cast<uint16_t*>(p.dqkv) + ((size_t)(valid ? tok : 0) * H + w.row0) * D;
+    const long long xh = p.xs[2], yh = p.hs[w.kind][1];
+    if (w.kind == 2) {
+      for (int h = 0; h < w.n; h += UNROLL) {
+        uint4 u0[UNROLL], u1[UNROLL];
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const int row = base + u * p.rows + r0;
-        u0[u] = u1[u] = g0[u] = g1[u] = make_uint2(0u, 0u);
-        if (row < H && r0 < p.rows) {
-          const int kind = row < p.Hq ? 0 : row < Hn ? 1 : 2;
-          const int h = kind == 0 ? row : kind == 1 ? row - p.Hq : row - Hn;
-          const uint16_t* dy =
-              static_cast<const uint16_t*>(p.in[kind]) + b * p.hs[kind][0] + h * p.hs[kind][1] + i * p.hs[kind][2];
-          g0[u] = *reinterpret_cast<const uint2*>(dy + t.c0);
-          g1[u] = *reinterpret_cast<const uint2*>(dy + t.c1);
-          if (kind < 2) {
-            u0[u] = *reinterpret_cast<const uint2*>(x + row * p.xs[2] + t.c0);
-            u1[u] = *reinterpret_cast<const uint2*>(x + row * p.xs[2] + t.c1);
+        for (int u = 0; u < UNROLL; ++u)
+          if (valid && h + u < w.n) {
+            u0[u] = *reinterpret_cast<const uint4*>(dy + (h + u) * yh + t.c0);
+            u1[u] = *reinterpret_cast<const uint4*>(dy + (h + u) * yh + t.c1);
           }
-        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+          if (valid && h + u < w.n) {
+            *reinterpret_cast<uint4*>(dx + (h + u) * D + t.c0) = u0[u];
+            *reinterpret_cast<uint4*>(dx + (h + u) * D + t.c1) = u1[u];
+          }
       }
-#pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        if (base + u * p.rows >= H) break;
-        const int row = base + u * p.rows + r0;
-        const int kind = row < p.Hq ? 0 : 1;  // (a value's x is 0 here, and its sums are not used)
-        float f[8], d[8];
-        heads_unpack<BF16>(u0[u], u1[u], f);
-        heads_unpack<BF16>(g0[u], g1[u], d);
-        if (turns) heads_turn(d, cs, sn, -1.f, p.interleaved);
-        const float4 w0 = *reinterpret_cast<const float4*>(&s_w[kind][t.c0]), w1 = *reinterpret_cast<const float4*>(&s_w[kind][t.c1]);
-        const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-        float ss = 0.f, dot = 0.f, dn[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ss = fmaf(f[e], f[e], ss);
-          dn[e] = d[e] * f[e];
-          dot = fmaf(dn[e], w[e], dot);
-        }
-#pragma unroll
-        for (int s = 1; s < PIECES; s <<= 1) {
-          ss += __shfl_xor_sync(0xffffffffu, ss, s);
-          dot += __shfl_xor_sync(0xffffffffu, dot, s);
-        }
-        if (row >= H || r0 >= p.rows) continue;
-        uint16_t* y = dx + row * D;
-        if (row >= Hn) {
-          *reinterpret_cast<uint2*>(y + t.c0) = g0[u];
-          *reinterpret_cast<uint2*>(y + t.c1) = g1[u];
-          continue;
-        }
-        const float r = rsqrtf(ss * (1.f / D) + p.eps), m = r * r * dot * (1.f / D);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (kind == 0)
-            dw[0][e] = fmaf(dn[e], r, dw[0][e]);
-          else
-            dw[1][e] = fmaf(dn[e], r, dw[1][e]);
-          f[e] = r * (d[e] * w[e] - f[e] * m);
-        }
-        heads_store<BF16>(y, t, f);
+      continue;
+    }
+    HeadsAngles g;
+    const bool turns = heads_angles(p, t, l, b, i, valid, g);
+    struct Piece {
+      uint4 u0, u1, g0, g1;
+    };
+    auto load = [&](int h) {
+      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+      Piece r{zero, zero, zero, zero};
+      if (valid && h < w.n) {
+        r.u0 = *reinterpret_cast<const uint4*>(x + h * xh + t.c0);
+        r.u1 = *reinterpret_cast<const uint4*>(x + h * xh + t.c1);
+        r.g0 = *reinterpret_cast<const uint4*>(dy + h * yh + t.c0);
+        r.g1 = *reinterpret_cast<const uint4*>(dy + h * yh + t.c1);
       }
+      return r;
+    };
+    Piece now = load(0);
+#pragma unroll 1
+    for (int h = 0; h < w.n; ++h) {
+      const Piece next = load(h + 1);
+      HeadsRow f, d;
+      heads_unpack<BF16, PAIRS>(now.u0, now.u1, f);
+      heads_unpack<BF16, PAIRS>(now.g0, now.g1, d);
+      if (turns) heads_turn<true>(d, g);
+      float2 ss2 = make_float2(0.f, 0.f), dot2 = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float4 wa = heads_weight<LANES>(s_w, l, e / 2), wb = heads_weight<LANES>(s_w, l, 2 + e / 2);
+        ss2 = __ffma2_rn(f.b[e], f.b[e], __ffma2_rn(f.a[e], f.a[e], ss2));
+        dot2 = __ffma2_rn(__fmul2_rn(d.a[e], e & 1 ? make_float2(wa.z, wa.w) : make_float2(wa.x, wa.y)), f.a[e], dot2);
+        dot2 = __ffma2_rn(__fmul2_rn(d.b[e], e & 1 ? make_float2(wb.z, wb.w) : make_float2(wb.x, wb.y)), f.b[e], dot2);
+      }
+      float ss = ss2.x + ss2.y, dot = dot2.x + dot2.y;
+#pragma unroll
+      for (int s = 1; s < LANES; s <<= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, s);
+        dot += __shfl_xor_sync(0xffffffffu, dot, s);
+      }
+      const float r = rsqrtf(ss * (1.f / D) + p.eps);
+      const float2 r2 = splat(r), m2 = splat(-(r * r * dot * (1.f / D)));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float4 wa = heads_weight<LANES>(s_w, l, e / 2), wb = heads_weight<LANES>(s_w, l, 2 + e / 2);
+        dw.a[e] = __ffma2_rn(__fmul2_rn(d.a[e], f.a[e]), r2, dw.a[e]);
+        dw.b[e] = __ffma2_rn(__fmul2_rn(d.b[e], f.b[e]), r2, dw.b[e]);
+        d.a[e] = __fmul2_rn(d.a[e], e & 1 ? make_float2(wa.z, wa.w) : make_float2(wa.x, wa.y));
+        d.b[e] = __fmul2_rn(d.b[e], e & 1 ? make_float2(wb.z, wb.w) : make_float2(wb.x, wb.y));
+        f.a[e] = __fmul2_rn(__ffma2_rn(f.a[e], m2, d.a[e]), r2);
+        f.b[e] = __fmul2_rn(__ffma2_rn(f.b[e], m2, d.b[e]), r2);
+      }
+      heads_pack<BF16, PAIRS>(f, now.u0, now.u1);
+      if (valid) {
+        *reinterpret_cast<uint4*>(dx + h * D + t.c0) = now.u0;
+        *reinterpret_cast<uint4*>(dx + h * D + t.c1) = now.u1;
+      }
+      now = next;
     }
   }
-  // ---- the CTA's sums of the weights' gradients, in a fixed order
+  if (w.kind == 2) return;
+  // ---- the CTA's sums of the weight's gradient, in a fixed order: over a warp's tokens, then over the warps
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    __syncthreads();
-    *reinterpret_cast<float4*>(&s_sum[r0][t.c0]) = make_float4(dw[k][0], dw[k][1], dw[k][2], dw[k][3]);
-    *reinterpret_cast<float4*>(&s_sum[r0][t.c1]) = make_float4(dw[k][4], dw[k][5], dw[k][6], dw[k][7]);
-    __syncthreads();
-    for (int c = tid; c < D; c += blockDim.x) {
-      float sum = 0.f;
-      for (int r = 0; r < p.rows; ++r) sum += s_sum[r][c];
-      p.partial[((size_t)blockIdx.x * 2 + k) * D + c] = sum;
+  for (int e = 0; e < 4; ++e)
+#pragma unroll
+    for (int s = LANES; s < 32; s <<= 1) {
+      dw.a[e].x += __shfl_xor_sync(0xffffffffu, dw.a[e].x, s);
+      dw.a[e].y += __shfl_xor_sync(0xffffffffu, dw.a[e].y, s);
+      dw.b[e].x += __shfl_xor_sync(0xffffffffu, dw.b[e].x, s);
+      dw.b[e].y += __shfl_xor_sync(0xffffffffu, dw.b[e].y, s);
     }
+  if (lane < LANES) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int i = 2 * e + j;
+        const int ca = PAIRS ? (i < 4 ? t.c0 + 2 * i : t.c1 + 2 * i - 8) : t.c0 + i, cb = PAIRS ? ca + 1 : t.c1 + i;
+        s_sum[warp][ca] = j ? dw.a[e].y : dw.a[e].x;
+        s_sum[warp][cb] = j ? dw.b[e].y : dw.b[e].x;
+      }
+  }
+  __syncthreads();
+  float* partial = p.partial + ((size_t)w.kind * p.ctas * p.chunks[0] + w.index) * D;  // (keys after all queries)
+  for (int c = threadIdx.x; c < D; c += kHeadsThreads) {
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < kHeadsThreads / 32; ++r) sum += s_sum[r][c];
+    partial[c] = sum;
   }
 }
 
-// The CTAs' sums added up, one warp for a column (grid: 2 D / 8, of 8 warps each).
+// The CTAs' sums added up: a CTA takes 32 columns of a kind (grid: 2 D / 32), its warps every 32nd row.
 template <bool BF16, int D>
-__global__ void __launch_bounds__(256) coalibi_heads_sum_kernel(const HeadsParams p, int n) {
+__global__ void __launch_bounds__(1024) coalibi_heads_sum_kernel(const HeadsParams p) {
+  __shared__ float s_sum[32][33];
   grid_dep_wait();
-  const int lane = threadIdx.x & 31, col = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int kind = blockIdx.x / (D / 32), col = (blockIdx.x % (D / 32)) * 32;
+  const int n = p.ctas * p.chunks[kind];
+  const float* x = p.partial + (size_t)kind * p.ctas * p.chunks[0] * D + col + lane;
   float sum = 0.f;
-  for (int i = lane; i < n; i += 32) sum += p.partial[(size_t)i * 2 * D + col];
+#pragma unroll 8
+  for (int i = warp; i < n; i += 32) sum += x[(size_t)i * D];
+  s_sum[warp][lane] = sum;
+  __syncthreads();
+  sum = s_sum[lane][warp];  // column `warp`, lane by lane
 #pragma unroll
   for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  void* y = p.dweight[col / D];
+  void* y = p.dweight[kind];
   if (lane != 0 || y == nullptr) return;
   if (p.weight_f32)
-    static_cast<float*>(y)[col % D] = sum;
+    static_cast<float*>(y)[col + warp] = sum;
   else
-    static_cast<uint16_t*>(y)[col % D] = (uint16_t)pack2<BF16>(sum, 0.f);
+    static_cast<uint16_t*>(y)[col + warp] = (uint16_t)pack2<BF16>(sum, 0.f);
 }
 
 }  // namespace coalibi

@@ -331,6 +331,7 @@ def test_refusals():
             (ValueError, dict(start=z(3, dt=torch.int32))), (ValueError, dict(positions=z(2, 2, dt=torch.int32))),
             (TypeError, dict(rotary=tab(4, 8))), (ValueError, dict(rotary=(tab(4, 4), tab(4, 4)))), (ValueError, dict(rotary=(tab(4, 40), tab(4, 40)))),
             (ValueError, dict(rotary=(tab(4, 8), tab(5, 8)))), (TypeError, dict(rotary=(tab(4, 8, f16), tab(4, 8, f16)))),
-            (RuntimeError, dict(rotary=(tab(4, 8).requires_grad_(), tab(4, 8))))):
+            (RuntimeError, dict(rotary=(tab(4, 8).requires_grad_(), tab(4, 8)))),
+            (RuntimeError, dict(rotary=(tab(4, 8), tab(4, 8).requires_grad_()), qkv=z(2, 3, 6, 64).requires_grad_()))):
         with pytest.raises(kind):
             norm_rotate_qkv(**{**good, **kw})
