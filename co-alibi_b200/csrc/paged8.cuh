@@ -61,7 +61,7 @@ struct Append8Params : AppendParams {
 };
 
 template <bool BF16, int D, int TURN>
-__global__ void __launch_bounds__(kAppendThreads) coalibi_paged_append8_kernel(const Append8Params p) {
+__global__ void __launch_bounds__(kAppendThreads, D == 128 ? 3 : 4) coalibi_paged_append8_kernel(const Append8Params p) {
   constexpr int PIECES = D / 8;
   grid_dep_wait();
   const int tid = threadIdx.x, half = p.rot / 2;
@@ -141,52 +141,55 @@ __global__ void __launch_bounds__(kAppendThreads) coalibi_paged_append8_kernel(c
   float* scale_at = (key ? p.k_scales + page * p.kss[0] + h * p.kss[1] : p.v_scales + page * p.vss[0] + h * p.vss[1]) +
                     slot / kQuantBlock;
   const float was = lo > 0 ? *scale_at : 0.f;  // the block holds tokens already
-  float f[N][8];
-  float most = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
+  // Row i's values (r its token of the block), rotated where it has angles.  Computed twice, for the block's
+  // largest and for the codes: the rows in float32 would take twice the registers.
+  bool lost = false;  // some token has no angles
+  auto values = [&](int i, int r, float* f) {
     const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float2 u = unpack2<BF16>(w[e]);
-      f[i][2 * e] = u.x, f[i][2 * e + 1] = u.y;
+      f[2 * e] = u.x, f[2 * e + 1] = u.y;
     }
-    const int r = r0 + i * RPW;
-    if (TURN != kTurnNone && key && c < p.rot && r >= lo && r < hi) {
-      const long long tok = t0 + r, at_pos = p.positions != nullptr ? p.positions[(size_t)b * p.S + (tok - start)] : tok;
-      if (at_pos >= 0 && at_pos < p.n_pos) {
-        Angles<TURN> g;
-        g.load(p.cos + (size_t)at_pos * half, p.sin + (size_t)at_pos * half, c, half);
-        // products and their sum rounded one by one: the same codes as plain float32 arithmetic gives
-        if (TURN == kTurnPairs) {
+    if (TURN == kTurnNone || !key || c >= p.rot || r < lo || r >= hi) return;
+    const long long tok = t0 + r, at_pos = p.positions != nullptr ? p.positions[(size_t)b * p.S + (tok - start)] : tok;
+    if (at_pos < 0 || at_pos >= p.n_pos) {
+      lost = true;
+      return;
+    }
+    Angles<TURN> g;
+    g.load(p.cos + (size_t)at_pos * half, p.sin + (size_t)at_pos * half, c, half);
+    // products and their sum rounded one by one: the same codes as plain float32 arithmetic gives
+    if (TURN == kTurnPairs) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float a0 = f[i][2 * e], a1 = f[i][2 * e + 1];
-            f[i][2 * e] = __fsub_rn(__fmul_rn(a0, g.cs[e]), __fmul_rn(a1, g.sn[e]));
-            f[i][2 * e + 1] = __fadd_rn(__fmul_rn(a1, g.cs[e]), __fmul_rn(a0, g.sn[e]));
-          }
-        } else {
-          const uint4 other = *reinterpret_cast<const uint4*>(x + r * xs[2] + (c < half ? half : -half));
-          const uint32_t o[4] = {other.x, other.y, other.z, other.w};
+      for (int e = 0; e < 4; ++e) {
+        const float a0 = f[2 * e], a1 = f[2 * e + 1];
+        f[2 * e] = __fsub_rn(__fmul_rn(a0, g.cs[e]), __fmul_rn(a1, g.sn[e]));
+        f[2 * e + 1] = __fadd_rn(__fmul_rn(a1, g.cs[e]), __fmul_rn(a0, g.sn[e]));
+      }
+    } else {
+      const uint4 other = *reinterpret_cast<const uint4*>(x + r * xs[2] + (c < half ? half : -half));
+      const uint32_t o[4] = {other.x, other.y, other.z, other.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 u = unpack2<BF16>(o[e]);
-            f[i][2 * e] = __fadd_rn(__fmul_rn(f[i][2 * e], g.cs[2 * e % g.N]), __fmul_rn(u.x, g.sn[2 * e % g.N]));
-            f[i][2 * e + 1] =
-                __fadd_rn(__fmul_rn(f[i][2 * e + 1], g.cs[(2 * e + 1) % g.N]), __fmul_rn(u.y, g.sn[(2 * e + 1) % g.N]));
-          }
-        }
-      } else if (c == 0) {
-        report_page(p.status);
+      for (int e = 0; e < 4; ++e) {
+        const float2 u = unpack2<BF16>(o[e]);
+        f[2 * e] = __fadd_rn(__fmul_rn(f[2 * e], g.cs[2 * e % g.N]), __fmul_rn(u.x, g.sn[2 * e % g.N]));
+        f[2 * e + 1] = __fadd_rn(__fmul_rn(f[2 * e + 1], g.cs[(2 * e + 1) % g.N]), __fmul_rn(u.y, g.sn[(2 * e + 1) % g.N]));
       }
     }
+  };
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float f[8];
+    values(i, r0 + i * RPW, f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float a = fabsf(f[i][e]);
-      if (!(a < INFINITY)) f[i][e] = __int_as_float(0x7fc00000);  // an infinity has no code: NaN, not the block's largest
+      const float a = fabsf(f[e]);
       most = fmaxf(most, a < INFINITY ? a : 0.f);
     }
   }
+  if (lost && c == 0) report_page(p.status);
   most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
   const float scale = fmaxf(quant_scale(most), was), inv = 1.f / scale;
   uint8_t* y = static_cast<uint8_t*>(key ? p.k_pages : p.v_pages) +
@@ -217,10 +220,12 @@ __global__ void __launch_bounds__(kAppendThreads) coalibi_paged_append8_kernel(c
   for (int i = 0; i < N; ++i) {
     const int r = r0 + i * RPW;
     if (r >= lo && r < hi) {
+      float f[8];
+      values(i, r, f);
+      // an infinity has no code: NaN, not the block's largest
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[i][e] *= inv;
-      *reinterpret_cast<uint2*>(y + r * ys) =
-          make_uint2(e4m3_from(f[i][0], f[i][1], f[i][2], f[i][3]), e4m3_from(f[i][4], f[i][5], f[i][6], f[i][7]));
+      for (int e = 0; e < 8; ++e) f[e] = fabsf(f[e]) < INFINITY ? f[e] * inv : __int_as_float(0x7fc00000);
+      *reinterpret_cast<uint2*>(y + r * ys) = make_uint2(e4m3_from(f[0], f[1], f[2], f[3]), e4m3_from(f[4], f[5], f[6], f[7]));
     }
   }
   if (lane == 0 && scale != was) *scale_at = scale;
@@ -245,7 +250,7 @@ struct Read8Params {
   int Hkv, S;
   int chunks;  // of kReadRows tokens
   int tiles;   // B * 2 Hkv * chunks
-  int page_size, max_pages, n_pages;
+  int page_size, page_shift, max_pages, n_pages;  // page_shift: log2(page_size), or -1
 };
 
 constexpr int kReadThreads = 256;
@@ -279,7 +284,7 @@ __global__ void __launch_bounds__(kReadThreads) coalibi_paged_read8_kernel(const
     if (pos < 0) continue;
     int page = -1, slot = 0;
     if (pos < p.max_pages * p.page_size) {
-      const int n = pos / p.page_size;
+      const int n = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
       slot = pos - n * p.page_size;
       page = p.page_table[(size_t)b * p.table_stride + n];
     }
@@ -290,6 +295,8 @@ __global__ void __launch_bounds__(kReadThreads) coalibi_paged_read8_kernel(const
     codes[i] = *reinterpret_cast<const uint4*>(pages + page * ps + slot * ss);
     scale[i] = scales[page * cs + slot / kQuantBlock];
   }
+  // Codes times scale, rounded once.  A scale by which no code passes the type's largest needs no clamp; a
+  // power of two within float16's range multiplies there, where the product is rounded once too.
   const float top = BF16 ? 3.38953139e38f : 65504.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -298,16 +305,24 @@ __global__ void __launch_bounds__(kReadThreads) coalibi_paged_read8_kernel(const
     const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
     uint32_t y[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      uint32_t g[2];
-      e4m3_to_f16x4(w[e], g[0], g[1]);
+    for (int e = 0; e < 4; ++e) e4m3_to_f16x4(w[e], y[2 * e], y[2 * e + 1]);
+    if (!BF16 && scale[i] <= 128.f && scale[i] >= 5.9604645e-8f && (__float_as_int(scale[i]) & 0x7fffff) == 0) {
+      const __half2 s = __float2half2_rn(scale[i]);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        float2 u = f16x2_to_float2(g[q]);
-        u.x *= scale[i], u.y *= scale[i];
-        u.x = u.x > top ? top : u.x < -top ? -top : u.x;  // (NaN stays)
-        u.y = u.y > top ? top : u.y < -top ? -top : u.y;
-        y[2 * e + q] = pack2<BF16>(u.x, u.y);
+      for (int e = 0; e < 8; ++e) {
+        const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&y[e]), s);
+        y[e] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    } else {
+      const bool clamps = !(scale[i] <= (BF16 ? 7e35f : 128.f));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float2 u = __fmul2_rn(f16x2_to_float2(y[e]), make_float2(scale[i], scale[i]));
+        if (clamps) {  // (NaN stays)
+          u.x = u.x > top ? top : u.x < -top ? -top : u.x;
+          u.y = u.y > top ? top : u.y < -top ? -top : u.y;
+        }
+        y[e] = pack2<BF16>(u.x, u.y);
       }
     }
     uint4* to = reinterpret_cast<uint4*>(out + (size_t)t * D);
@@ -909,6 +924,124 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
       if (++b < p.B) span = paged_span<L>(p, b);
     }
   }
+}
+
+// Joins the pieces of the items that span runs, as the 16-bit attention's kernel does, but with a CTA for a
+// query row: runs are a warp's here, so a long item comes in dozens of pieces.  A thread takes a piece's
+// statistics, rightmost first, and a warp every fourth piece's O, the first ones on their way beside the statistics.
+constexpr int kJoinThreads = 128;
+
+template <int D, bool BF16, typename L>
+__global__ void __launch_bounds__(kJoinThreads) coalibi_paged8_join_kernel(const PagedAttnParams p) {
+  constexpr int V = D / 32, WARPS = kJoinThreads / 32, EARLY = 8;
+  __shared__ float s_f[kJoinThreads], s_a[WARPS], s_b[WARPS], s_c[WARPS], s_o[WARPS][D];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = p.Hq / p.Hkv, rows = G * p.Sq;
+  const int b = blockIdx.x / p.Hkv, g = blockIdx.x - b * p.Hkv, r = blockIdx.y;
+  grid_dep_wait();
+  const int* head = reinterpret_cast<const int*>(p.ws);
+  const int heads = p.Hkv * p.row_blocks, item = g * p.row_blocks + r / L::ROWS, rr = r % L::ROWS;
+  const int span = head[b + 1] - head[b];
+  const long long quota = head[p.B + 1];
+  const long long start = (long long)head[b] * heads + (long long)item * span;
+  const long long t0 = start + L::COST, t1 = start + span;
+  const int c0 = (int)(t0 / quota), c1 = (int)((t1 - 1) / quota);
+  if (c0 == c1) return;  // finished by the attention kernel
+  const int h = g * G + r / p.Sq, i = r % p.Sq;
+  const float slope2 = load_slope(p.slopes, p.slopes_dtype, h) * kLog2e;
+  const float* recs = p.ws + paged_ws_head(p.B);
+  auto record = [&](int c) { return recs + ((size_t)c * 2 + (t0 < c * quota ? 0 : 1)) * L::RECORD; };
+  float M = -INFINITY, l = 0.f, right = 0.f, acc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = 0.f;
+  for (int top = c1; top >= c0; top -= kJoinThreads) {
+    const int n = min(kJoinThreads, top - c0 + 1);
+    auto o_of = [&](int j, float* u) {
+      const float* y = record(top - j) + 4 * L::ROWS + rr * D + lane * V;
+      if (V == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(y);
+        u[0] = f.x, u[1] = f.y, u[V - 2] = f.z, u[V - 1] = f.w;
+      } else {
+        const float2 f = *reinterpret_cast<const float2*>(y);
+        u[0] = f.x, u[1] = f.y;
+      }
+    };
+    float4 s = make_float4(0.f, -INFINITY, 0.f, 0.f);
+    if (tid < n) s = reinterpret_cast<const float4*>(record(top - tid))[rr];
+    float early[EARLY][V];
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) early[k][v] = 0.f;
+      if (warp + k * WARPS < n) o_of(warp + k * WARPS, early[k]);
+    }
+    float inc = s.x;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const float y = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += y;
+    }
+    if (lane == 31) s_a[warp] = inc;
+    __syncthreads();
+    float before = right;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) before += s_a[w];
+      right += s_a[w];
+    }
+    const float m = s.y == -INFINITY ? -INFINITY : s.y - slope2 * (before + (inc - s.x));
+    float mx = m;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    if (lane == 0) s_b[warp] = mx;
+    __syncthreads();
+    float m_new = M;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) m_new = fmaxf(m_new, s_b[w]);
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float fac = M == -INFINITY ? 0.f : ex2_approx(M - m_use);
+    M = m_new;
+    const float f = ex2_approx(m - m_use);
+    s_f[tid] = f;
+    float lw = f * s.z;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, d);
+    if (lane == 0) s_c[warp] = lw;
+    __syncthreads();
+    l *= fac;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) l += s_c[w];
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] *= fac;
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k) {
+      const float w = s_f[warp + k * WARPS];  // 0 past the last piece
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = fmaf(w, early[k][v], acc[v]);
+    }
+#pragma unroll 4
+    for (int j = warp + EARLY * WARPS; j < n; j += WARPS) {
+      const float w = s_f[j];
+      float u[V];
+      o_of(j, u);
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = fmaf(w, u[v], acc[v]);
+    }
+    __syncthreads();  // s_a, s_b, s_c and s_f are written again
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) s_o[warp][lane * V + v] = acc[v];
+  __syncthreads();
+  if (tid >= D / 2) return;
+  float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    sum.x += s_o[w][2 * tid];
+    sum.y += s_o[w][2 * tid + 1];
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  uint16_t* y = static_cast<uint16_t*>(p.o) + b * p.os[0] + h * p.os[1] + i * p.os[2] + 2 * tid;
+  *reinterpret_cast<uint32_t*>(y) = pack2<BF16>(sum.x * inv, sum.y * inv);
 }
 
 }  // namespace coalibi

@@ -27,6 +27,13 @@ int check_codes(const CoalibiCacheScales* s, const void* k_pages, const void* v_
   return COALIBI_OK;
 }
 
+// log2 of the page size, or -1.
+int page_shift_of(int page_size) {
+  for (int k = 4; k < 31; ++k)
+    if (page_size == 1 << k) return k;
+  return -1;
+}
+
 void copy2(long long* dst, const long long* src) { dst[0] = src[0], dst[1] = src[1]; }
 
 template <bool BF16, int D>
@@ -36,11 +43,22 @@ auto append8_kernel(int turn) {
                               : coalibi_paged_append8_kernel<BF16, D, kTurnHalves>;
 }
 
+template <bool BF16, int D>
+auto queries_kernel(int turn) {
+  return turn == kTurnNone    ? coalibi_paged_append_kernel<BF16, D, kTurnNone>
+         : turn == kTurnPairs ? coalibi_paged_append_kernel<BF16, D, kTurnPairs>
+                              : coalibi_paged_append_kernel<BF16, D, kTurnHalves>;
+}
+
 template <int D, bool BF16, int NT, int RW, int WARPS>
 int launch_attention8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, int sms, cudaStream_t s) {
   static std::atomic<unsigned long long> ready{0};
-  return launch_paged<D, BF16, Paged8Layout<D, NT, RW, WARPS>>(coalibi_paged8_attn_kernel<D, BF16, NT, RW, WARPS>, ready,
-                                                               32 * WARPS, tk, tv, p, sms, s);
+  using L = Paged8Layout<D, NT, RW, WARPS>;
+  const auto join = [&p, s](int rows) {
+    return launch_pdl(coalibi_paged8_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, rows), dim3(kJoinThreads), 0, s,
+                      static_cast<const PagedAttnParams&>(p));
+  };
+  return launch_paged<L>(coalibi_paged8_attn_kernel<D, BF16, NT, RW, WARPS>, join, ready, 32 * WARPS, tk, tv, p, sms, s);
 }
 
 // Four warps to an item where the tables hold little work, else as many as its rows take (as in the
@@ -142,9 +160,19 @@ extern "C" int coalibi_paged_append8(const CoalibiPagedAppendArgs* a, const Coal
   const int turn = a->rot == 0 ? kTurnNone : a->interleaved ? kTurnPairs : kTurnHalves;
   auto kernel = a->D == 128 ? (bf16 ? append8_kernel<true, 128>(turn) : append8_kernel<false, 128>(turn))
                             : (bf16 ? append8_kernel<true, 64>(turn) : append8_kernel<false, 64>(turn));
-  if (const cudaError_t e = launch_pdl(kernel, dim3((unsigned)(p.kv_ctas + q_ctas)), dim3(kAppendThreads), 0,
-                                       static_cast<cudaStream_t>(stream), p);
-      e != cudaSuccess) {
+  // The queries of few tokens go in the same launch; those of many in one of their own (the 16-bit append's kernel
+  // without keys), whose CTAs take a third of the registers.
+  const bool apart = q_ctas > 0 && p.group > 1;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = launch_pdl(kernel, dim3((unsigned)(p.kv_ctas + (apart ? 0 : q_ctas))), dim3(kAppendThreads), 0, s, p);
+  if (e == cudaSuccess && apart) {
+    AppendParams q = p;
+    q.Hkv = 0;
+    auto queries = a->D == 128 ? (bf16 ? queries_kernel<true, 128>(turn) : queries_kernel<false, 128>(turn))
+                               : (bf16 ? queries_kernel<true, 64>(turn) : queries_kernel<false, 64>(turn));
+    e = launch_pdl(queries, dim3((unsigned)q_ctas), dim3(kAppendThreads), 0, s, q);
+  }
+  if (e != cudaSuccess) {
     set_last_error_detail(cudaGetErrorString(e));
     return COALIBI_ERR_LAUNCH;
   }
@@ -187,6 +215,7 @@ extern "C" int coalibi_paged_read8(const CoalibiPagedReadArgs* a, const CoalibiC
   p.page_size = a->page_size;
   p.max_pages = a->max_pages;
   p.n_pages = a->n_pages;
+  p.page_shift = page_shift_of(a->page_size);
   const bool bf16 = a->dtype == COALIBI_BF16;
   auto kernel = a->D == 128 ? (bf16 ? coalibi_paged_read8_kernel<true, 128> : coalibi_paged_read8_kernel<false, 128>)
                             : (bf16 ? coalibi_paged_read8_kernel<true, 64> : coalibi_paged_read8_kernel<false, 64>);
@@ -250,9 +279,7 @@ extern "C" int coalibi_paged_attention8(const CoalibiPagedAttentionArgs* a, cons
   p.slopes_dtype = a->slopes_dtype;
   p.sm_scale = a->sm_scale;
   p.ws = static_cast<float*>(workspace);
-  p.page_shift = -1;
-  for (int k = 4; k < 31; ++k)
-    if (a->page_size == 1 << k) p.page_shift = k;
+  p.page_shift = page_shift_of(a->page_size);
   p.k_scales = sc->k;
   p.v_scales = sc->v;
   copy2(p.kss, sc->k_stride);

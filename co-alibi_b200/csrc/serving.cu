@@ -96,11 +96,19 @@ extern "C" int coalibi_paged_append(const CoalibiPagedAppendArgs* a, void* strea
 namespace coalibi {
 namespace {
 
+template <int D, bool BF16, typename L>
+auto join_launch(const PagedAttnParams& p, cudaStream_t s) {
+  return [&p, s](int rows) {
+    return launch_pdl(coalibi_paged_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, (rows + 3) / 4), dim3(128), 0, s, p);
+  };
+}
+
 template <int D, bool BF16, int RW, int XR, int WARPS>
 int launch_narrow_of(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& p, int sms, cudaStream_t s) {
   static std::atomic<unsigned long long> ready{0};
-  return launch_paged<D, BF16, PagedLayout<D, RW, WARPS>>(coalibi_paged_attn_kernel<D, BF16, RW, XR, WARPS>, ready,
-                                                          32 * WARPS, tk, tv, p, sms, s);
+  using L = PagedLayout<D, RW, WARPS>;
+  return launch_paged<L>(coalibi_paged_attn_kernel<D, BF16, RW, XR, WARPS>, join_launch<D, BF16, L>(p, s), ready, 32 * WARPS,
+                         tk, tv, p, sms, s);
 }
 
 template <int D, bool BF16, int RW, int XR>
@@ -123,7 +131,8 @@ template <int D, bool BF16, bool DUP>
 int launch_wide(const CUtensorMap& tk, const CUtensorMap& tv, PagedAttnParams& p, int sms, cudaStream_t s) {
   static std::atomic<unsigned long long> ready{0};
   using L = WideLayout<D, DUP>;
-  return launch_paged<D, BF16, L>(coalibi_paged_wide_kernel<D, BF16, DUP>, ready, L::THREADS, tk, tv, p, sms, s);
+  return launch_paged<L>(coalibi_paged_wide_kernel<D, BF16, DUP>, join_launch<D, BF16, L>(p, s), ready, L::THREADS, tk, tv, p,
+                         sms, s);
 }
 
 template <int D, bool BF16>

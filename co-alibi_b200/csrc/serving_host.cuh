@@ -61,9 +61,10 @@ int check_cache(int B, int Hkv, int D, int page_size, int max_pages, int n_pages
   return COALIBI_OK;
 }
 
-// The attention kernel of layout L and the kernel that joins its pieces.
-template <int D, bool BF16, typename L, typename K, typename P>
-int launch_paged(K kernel, std::atomic<unsigned long long>& ready, int threads, const CUtensorMap& tk,
+// The attention kernel of layout L and the kernel that joins its pieces (join: launches it, for `rows` query
+// rows that share a kv head).
+template <typename L, typename K, typename P, typename J>
+int launch_paged(K kernel, J join, std::atomic<unsigned long long>& ready, int threads, const CUtensorMap& tk,
                  const CUtensorMap& tv, P& p, int sms, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
   int dev = 0;
@@ -85,9 +86,7 @@ int launch_paged(K kernel, std::atomic<unsigned long long>& ready, int threads, 
   else if (bound < p.n_ctas)
     p.n_ctas = (int)bound;
   if (e == cudaSuccess) e = launch_pdl(kernel, dim3(p.n_ctas), dim3(threads), L::BYTES, s, tk, tv, p);
-  if (e == cudaSuccess && !p.whole)
-    e = launch_pdl(coalibi_paged_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, (rows + 3) / 4), dim3(128), 0, s,
-                   static_cast<const PagedAttnParams&>(p));
+  if (e == cudaSuccess && !p.whole) e = join(rows);
   if (e != cudaSuccess) set_last_error_detail(cudaGetErrorString(e));
   return e == cudaSuccess ? launched("paged attention launch") : COALIBI_ERR_LAUNCH;
 }
