@@ -104,8 +104,9 @@ extern "C" int coalibi_heads_fwd(const CoalibiHeadsArgs* a, void* stream) {
   p.out[1] = a->k;
   p.out[2] = a->v;
   auto kernel = a->interleaved ? heads_fwd_kernel<true>(a) : heads_fwd_kernel<false>(a);
-  return heads_result(
-      launch_pdl(kernel, dim3(heads_grid(p)), dim3(kHeadsThreads), 0, static_cast<cudaStream_t>(stream), p), "heads launch");
+  return heads_result(launch_pdl(kernel, dim3(heads_grid(p)), dim3(kHeadsThreads), HeadsRing<2>::BYTES,
+                                 static_cast<cudaStream_t>(stream), p),
+                      "heads launch");
 }
 
 extern "C" size_t coalibi_heads_bwd_workspace_bytes(int D) {
@@ -132,7 +133,9 @@ extern "C" int coalibi_heads_bwd(const CoalibiHeadsArgs* a, void* workspace, siz
   auto kernel = a->interleaved ? heads_bwd_kernel<true>(a) : heads_bwd_kernel<false>(a);
   auto sum = a->D == 128 ? (bf16 ? coalibi_heads_sum_kernel<true, 128> : coalibi_heads_sum_kernel<false, 128>)
                          : (bf16 ? coalibi_heads_sum_kernel<true, 64> : coalibi_heads_sum_kernel<false, 64>);
-  cudaError_t e = launch_pdl(kernel, dim3(heads_grid(p)), dim3(kHeadsThreads), 0, s, p);
+  constexpr int ring = HeadsRing<4>::BYTES;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring);
+  if (e == cudaSuccess) e = launch_pdl(kernel, dim3(heads_grid(p)), dim3(kHeadsThreads), ring, s, p);
   if (e == cudaSuccess && (a->dq_weight || a->dk_weight)) e = launch_pdl(sum, dim3(2 * a->D / 32), dim3(1024), 0, s, p);
   return heads_result(e, "heads backward launch");
 }

@@ -94,20 +94,33 @@ __device__ __forceinline__ void heads_pack(const HeadsRow& x, uint4& p0, uint4& 
 __device__ __forceinline__ float2 splat(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 neg2(float2 x) { return make_float2(-x.x, -x.y); }
 
-// Where a lane's columns and angles are (row l of D / 16 in a row).
+// Where a lane's two pieces of 8 columns are (lane l of D / 16 in a row): neighbouring lanes' lie side by side, so
+// that a load or store of a row takes whole sectors.  In halves a lane that turns has the two partners of
+// its pairs; interleaved, pairs lie within a piece, and each turns by itself.
 struct HeadsLane {
   int c0, c1;
-  bool turns;
+  int j0, j1;   // first angles of the pairs 0 .. 3 and 4 .. 7
+  bool t0, t1;  // whether these turn
 };
-template <bool PAIRS>
+template <bool PAIRS, int D>
 __device__ __forceinline__ HeadsLane heads_lane(int l, int rot) {
   HeadsLane t;
-  t.turns = 16 * l < rot;
-  const bool halves = t.turns && !PAIRS;
-  t.c0 = halves ? 8 * l : 16 * l;
-  t.c1 = halves ? rot / 2 + 8 * l : 16 * l + 8;
+  if (PAIRS) {
+    t.c0 = 8 * l, t.c1 = D / 2 + 8 * l;
+    t.j0 = t.c0 / 2, t.j1 = t.c1 / 2;
+    t.t0 = t.c0 < rot, t.t1 = t.c1 < rot;
+  } else if (16 * l < rot) {
+    t.c0 = 8 * l, t.c1 = rot / 2 + 8 * l;
+    t.j0 = 8 * l, t.j1 = 8 * l + 4;
+    t.t0 = t.t1 = true;
+  } else {
+    t.c0 = rot / 2 + 8 * l, t.c1 = D / 2 + 8 * l;  // rot + 8 (l - rot / 16), and (D - rot) / 2 after it
+    t.j0 = t.j1 = 0;
+    t.t0 = t.t1 = false;
+  }
   return t;
 }
+
 // The weights of a kind in shared memory, in the order of each lane's pairs: piece e (a's first and last four,
 // b's) of lane l at (e * LANES + l) * 4, so that a load takes every bank once.
 template <bool BF16, bool PAIRS, int D>
@@ -115,7 +128,7 @@ __device__ __forceinline__ void heads_weights(const HeadsParams& p, int kind, fl
   constexpr int LANES = D / 16;
   for (int at = threadIdx.x; at < D; at += kHeadsThreads) {
     const int e = at / (4 * LANES), l = at / 4 % LANES, i = e % 2 * 4 + at % 4;  // pair i, a or b of it
-    const HeadsLane t = heads_lane<PAIRS>(l, p.rot);
+    const HeadsLane t = heads_lane<PAIRS, D>(l, p.rot);
     const int c = PAIRS ? (i < 4 ? t.c0 + 2 * i : t.c1 + 2 * i - 8) + e / 2 : (e < 2 ? t.c0 : t.c1) + i;
     s_w[at] = load_weight<BF16>(p.weight[kind], p.weight_f32, c);
   }
@@ -134,19 +147,24 @@ __device__ __forceinline__ int heads_angle(const HeadsParams& p, int b, int i, b
   if (reports && p.status != nullptr) atomicCAS(p.status, 0, 11 /* COALIBI_ERR_PAGE */);
   return -1;
 }
+// Cosines and sines of a lane's pairs.
 struct HeadsAngles {
   float2 c[4], s[4];
 };
-// Whether the lane turns its pairs; if so, their angles.
+// Whether the lane turns any pair of the row; if so, the angles.
 __device__ __forceinline__ bool heads_angles(const HeadsParams& p, const HeadsLane& t, int l, int b, int i, bool valid, HeadsAngles& g) {
-  if (!valid || !t.turns) return false;
+  if (!valid || !t.t0) return false;  // (t1 only with t0)
   const int row = heads_angle(p, b, i, l == 0);
   if (row < 0) return false;
-  const float4* c = reinterpret_cast<const float4*>(p.cos + (size_t)row * (p.rot / 2) + 8 * l);
-  const float4* s = reinterpret_cast<const float4*>(p.sin + (size_t)row * (p.rot / 2) + 8 * l);
+  const float* c = p.cos + (size_t)row * (p.rot / 2);
+  const float* s = p.sin + (size_t)row * (p.rot / 2);
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const float4 u = c[e], v = s[e];
+    float4 u = make_float4(1.f, 1.f, 1.f, 1.f), v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (e == 0 || t.t1) {
+      u = *reinterpret_cast<const float4*>(c + (e ? t.j1 : t.j0));
+      v = *reinterpret_cast<const float4*>(s + (e ? t.j1 : t.j0));
+    }
     g.c[2 * e] = make_float2(u.x, u.y), g.c[2 * e + 1] = make_float2(u.z, u.w);
     g.s[2 * e] = make_float2(v.x, v.y), g.s[2 * e + 1] = make_float2(v.z, v.w);
   }
@@ -154,9 +172,10 @@ __device__ __forceinline__ bool heads_angles(const HeadsParams& p, const HeadsLa
 }
 // The pairs turned by the angles, or back by them.
 template <bool BACK>
-__device__ __forceinline__ void heads_turn(HeadsRow& x, const HeadsAngles& g) {
+__device__ __forceinline__ void heads_turn(HeadsRow& x, const HeadsAngles& g, const HeadsLane& t) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
+    if (e >= 2 && !t.t1) break;  // (not by 1 and 0: 0 * infinity)
     const float2 a = x.a[e], b = x.b[e], s = BACK ? neg2(g.s[e]) : g.s[e];
     x.a[e] = __ffma2_rn(b, neg2(s), __fmul2_rn(a, g.c[e]));
     x.b[e] = __ffma2_rn(a, s, __fmul2_rn(b, g.c[e]));
@@ -191,43 +210,97 @@ __device__ __forceinline__ HeadsWork heads_work(const HeadsParams& p) {
   return w;
 }
 
+// Rows on their way: a thread's pieces of the next heads, copied to shared memory of its own (no other thread
+// reads them, so nothing but its own copies is waited for).  A ring of registers holds less: the backward took
+// 99 us with one head ahead in registers and no room for more.
+constexpr int kHeadsStages = 4;
+template <int N>  // pieces of a head
+struct HeadsRing {
+  static constexpr int BYTES = kHeadsStages * N * kHeadsThreads * 16;
+  uint32_t base;
+  int fill = 0, drain = 0;
+  __device__ __forceinline__ explicit HeadsRing(void* smem) : base(smem_u32(smem) + threadIdx.x * 16) {}
+  __device__ __forceinline__ void copy(int k, const uint16_t* from, bool valid) const {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + (fill * N + k) * kHeadsThreads * 16), "l"(from),
+                 "r"(valid ? 16 : 0)
+                 : "memory");
+  }
+  __device__ __forceinline__ void issued() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    fill = fill + 1 == kHeadsStages ? 0 : fill + 1;
+  }
+  __device__ __forceinline__ void wait() const {  // for the oldest head
+    asm volatile("cp.async.wait_group %0;" ::"n"(kHeadsStages - 1) : "memory");
+  }
+  __device__ __forceinline__ uint4 read(int k) const {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(base + (drain * N + k) * kHeadsThreads * 16));
+    return v;
+  }
+  __device__ __forceinline__ void taken() { drain = drain + 1 == kHeadsStages ? 0 : drain + 1; }
+};
+
+// A token of the batch for a slot of a group.
+struct HeadsToken {
+  int tok, b, i;
+  bool valid;
+};
+__device__ __forceinline__ HeadsToken heads_token(const HeadsParams& p, long long tok) {
+  HeadsToken t;
+  t.valid = tok < p.tokens;
+  t.tok = t.valid ? (int)tok : 0;
+  t.b = t.tok / p.S;
+  t.i = t.tok - t.b * p.S;
+  return t;
+}
+
 template <bool BF16, int D, bool PAIRS>
-__global__ void __launch_bounds__(kHeadsThreads, 3) coalibi_heads_fwd_kernel(const HeadsParams p) {
+__global__ void __launch_bounds__(kHeadsThreads, 4) coalibi_heads_fwd_kernel(const HeadsParams p) {
   constexpr int LANES = D / 16, SLOTS = kHeadsThreads / LANES;
+  extern __shared__ __align__(16) uint8_t s_ring[];
   __shared__ __align__(16) float s_w[D];
   grid_dep_wait();
   const int l = threadIdx.x % LANES, slot = threadIdx.x / LANES;
   const HeadsWork w = heads_work(p);
-  const HeadsLane t = heads_lane<PAIRS>(l, p.rot);
+  const HeadsLane t = heads_lane<PAIRS, D>(l, p.rot);
+  HeadsRing<2> ring(s_ring);
+  int next_group = w.group, next_h = 0;
+  const uint16_t* x = nullptr;
+  bool next_valid = false;
+  auto issue = [&]() {
+    if (next_group < w.end) {
+      if (next_h == 0) {
+        const HeadsToken k = heads_token(p, (long long)next_group * SLOTS + slot);
+        next_valid = k.valid;
+        x = static_cast<const uint16_t*>(p.qkv) + k.b * p.xs[0] + k.i * p.xs[1] + w.row0 * p.xs[2];
+      }
+      ring.copy(0, x + t.c0, next_valid);
+      ring.copy(1, x + t.c1, next_valid);
+      x += p.xs[2];
+      if (++next_h == w.n) next_h = 0, ++next_group;
+    }
+    ring.issued();
+  };
+#pragma unroll
+  for (int k = 0; k < kHeadsStages - 1; ++k) issue();
   if (w.kind < 2) heads_weights<BF16, PAIRS, D>(p, w.kind, s_w);
   __syncthreads();
   for (int group = w.group; group < w.end; ++group) {
-    const int tok = group * SLOTS + slot;
-    const bool valid = tok < p.tokens;
-    const int b = valid ? tok / p.S : 0, i = valid ? tok - b * p.S : 0;
-    const uint16_t* x = static_cast<const uint16_t*>(p.qkv) + b * p.xs[0] + i * p.xs[1] + w.row0 * p.xs[2];
-    uint16_t* y = static_cast<uint16_t*>(p.out[w.kind]) + b * p.hs[w.kind][0] + w.h0 * p.hs[w.kind][1] + i * p.hs[w.kind][2];
-    const long long xh = p.xs[2], yh = p.hs[w.kind][1];
+    const HeadsToken k = heads_token(p, (long long)group * SLOTS + slot);
+    uint16_t* y = static_cast<uint16_t*>(p.out[w.kind]) + k.b * p.hs[w.kind][0] + w.h0 * p.hs[w.kind][1] + k.i * p.hs[w.kind][2];
     HeadsAngles g;
-    const bool turns = w.kind < 2 && heads_angles(p, t, l, b, i, valid, g);
-    struct Piece {
-      uint4 u0, u1;
-    };
-    auto load = [&](int h) {
-      Piece r{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-      if (valid && h < w.n) {
-        r.u0 = *reinterpret_cast<const uint4*>(x + h * xh + t.c0);
-        r.u1 = *reinterpret_cast<const uint4*>(x + h * xh + t.c1);
-      }
-      return r;
-    };
-    Piece now = load(0), next = load(1);
+    const bool turns = w.kind < 2 && heads_angles(p, t, l, k.b, k.i, k.valid, g);
 #pragma unroll 1
-    for (int h = 0; h < w.n; ++h) {
-      const Piece after = load(h + 2);
+    for (int h = 0; h < w.n; ++h, y += p.hs[w.kind][1]) {
+      issue();
+      ring.wait();
+      uint4 u0 = ring.read(0), u1 = ring.read(1);
+      ring.taken();
       if (w.kind < 2) {
         HeadsRow f;
-        heads_unpack<BF16, PAIRS>(now.u0, now.u1, f);
+        heads_unpack<BF16, PAIRS>(u0, u1, f);
         float2 ss2 = make_float2(0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) ss2 = __ffma2_rn(f.b[e], f.b[e], __ffma2_rn(f.a[e], f.a[e], ss2));
@@ -243,116 +316,106 @@ __global__ void __launch_bounds__(kHeadsThreads, 3) coalibi_heads_fwd_kernel(con
           f.b[e] = __fmul2_rn(__fmul2_rn(f.b[e], r), make_float2(wb.x, wb.y));
           f.b[e + 1] = __fmul2_rn(__fmul2_rn(f.b[e + 1], r), make_float2(wb.z, wb.w));
         }
-        if (turns) heads_turn<false>(f, g);
-        heads_pack<BF16, PAIRS>(f, now.u0, now.u1);
+        if (turns) heads_turn<false>(f, g, t);
+        heads_pack<BF16, PAIRS>(f, u0, u1);
       }
-      if (valid) {
-        *reinterpret_cast<uint4*>(y + h * yh + t.c0) = now.u0;
-        *reinterpret_cast<uint4*>(y + h * yh + t.c1) = now.u1;
+      if (k.valid) {
+        *reinterpret_cast<uint4*>(y + t.c0) = u0;
+        *reinterpret_cast<uint4*>(y + t.c1) = u1;
       }
-      now = next;
-      next = after;
     }
   }
 }
 
 template <bool BF16, int D, bool PAIRS>
 __global__ void __launch_bounds__(kHeadsThreads, 2) coalibi_heads_bwd_kernel(const HeadsParams p) {
-  constexpr int LANES = D / 16, SLOTS = kHeadsThreads / LANES, UNROLL = 4;
+  constexpr int LANES = D / 16, SLOTS = kHeadsThreads / LANES;
+  extern __shared__ __align__(16) uint8_t s_ring[];
   __shared__ __align__(16) float s_w[D], s_sum[kHeadsThreads / 32][D];
   grid_dep_wait();
   const int l = threadIdx.x % LANES, slot = threadIdx.x / LANES;
   const HeadsWork w = heads_work(p);
-  const HeadsLane t = heads_lane<PAIRS>(l, p.rot);
+  const HeadsLane t = heads_lane<PAIRS, D>(l, p.rot);
   const int H = p.Hq + 2 * p.Hkv;
+  HeadsRing<4> ring(s_ring);
+  int next_group = w.group, next_h = 0;
+  const uint16_t *x = nullptr, *dy = nullptr;
+  bool next_valid = false;
+  auto issue = [&]() {
+    if (next_group < w.end) {
+      if (next_h == 0) {
+        const HeadsToken k = heads_token(p, (long long)next_group * SLOTS + slot);
+        next_valid = k.valid;
+        x = static_cast<const uint16_t*>(p.qkv) + k.b * p.xs[0] + k.i * p.xs[1] + w.row0 * p.xs[2];
+        dy = static_cast<const uint16_t*>(p.in[w.kind]) + k.b * p.hs[w.kind][0] + w.h0 * p.hs[w.kind][1] + k.i * p.hs[w.kind][2];
+      }
+      ring.copy(0, dy + t.c0, next_valid);
+      ring.copy(1, dy + t.c1, next_valid);
+      if (w.kind < 2) {
+        ring.copy(2, x + t.c0, next_valid);
+        ring.copy(3, x + t.c1, next_valid);
+      }
+      x += p.xs[2];
+      dy += p.hs[w.kind][1];
+      if (++next_h == w.n) next_h = 0, ++next_group;
+    }
+    ring.issued();
+  };
+#pragma unroll
+  for (int k = 0; k < kHeadsStages - 1; ++k) issue();
   if (w.kind < 2) heads_weights<BF16, PAIRS, D>(p, w.kind, s_w);
   __syncthreads();
   HeadsRow dw;
 #pragma unroll
   for (int e = 0; e < 4; ++e) dw.a[e] = dw.b[e] = make_float2(0.f, 0.f);
   for (int group = w.group; group < w.end; ++group) {
-    const int tok = group * SLOTS + slot;
-    const bool valid = tok < p.tokens;
-    const int b = valid ? tok / p.S : 0, i = valid ? tok - b * p.S : 0;
-    const uint16_t* x = static_cast<const uint16_t*>(p.qkv) + b * p.xs[0] + i * p.xs[1] + w.row0 * p.xs[2];
-    const uint16_t* dy =
-        static_cast<const uint16_t*>(p.in[w.kind]) + b * p.hs[w.kind][0] + w.h0 * p.hs[w.kind][1] + i * p.hs[w.kind][2];
-    uint16_t* dx = static_cast<uint16_t*>(p.dqkv) + ((size_t)(valid ? tok : 0) * H + w.row0) * D;
-    const long long xh = p.xs[2], yh = p.hs[w.kind][1];
-    if (w.kind == 2) {
-      for (int h = 0; h < w.n; h += UNROLL) {
-        uint4 u0[UNROLL], u1[UNROLL];
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-          if (valid && h + u < w.n) {
-            u0[u] = *reinterpret_cast<const uint4*>(dy + (h + u) * yh + t.c0);
-            u1[u] = *reinterpret_cast<const uint4*>(dy + (h + u) * yh + t.c1);
-          }
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-          if (valid && h + u < w.n) {
-            *reinterpret_cast<uint4*>(dx + (h + u) * D + t.c0) = u0[u];
-            *reinterpret_cast<uint4*>(dx + (h + u) * D + t.c1) = u1[u];
-          }
-      }
-      continue;
-    }
+    const HeadsToken k = heads_token(p, (long long)group * SLOTS + slot);
+    uint16_t* dx = static_cast<uint16_t*>(p.dqkv) + ((size_t)k.tok * H + w.row0) * D;
     HeadsAngles g;
-    const bool turns = heads_angles(p, t, l, b, i, valid, g);
-    struct Piece {
-      uint4 u0, u1, g0, g1;
-    };
-    auto load = [&](int h) {
-      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-      Piece r{zero, zero, zero, zero};
-      if (valid && h < w.n) {
-        r.u0 = *reinterpret_cast<const uint4*>(x + h * xh + t.c0);
-        r.u1 = *reinterpret_cast<const uint4*>(x + h * xh + t.c1);
-        r.g0 = *reinterpret_cast<const uint4*>(dy + h * yh + t.c0);
-        r.g1 = *reinterpret_cast<const uint4*>(dy + h * yh + t.c1);
-      }
-      return r;
-    };
-    Piece now = load(0);
+    const bool turns = w.kind < 2 && heads_angles(p, t, l, k.b, k.i, k.valid, g);
 #pragma unroll 1
-    for (int h = 0; h < w.n; ++h) {
-      const Piece next = load(h + 1);
-      HeadsRow f, d;
-      heads_unpack<BF16, PAIRS>(now.u0, now.u1, f);
-      heads_unpack<BF16, PAIRS>(now.g0, now.g1, d);
-      if (turns) heads_turn<true>(d, g);
-      float2 ss2 = make_float2(0.f, 0.f), dot2 = make_float2(0.f, 0.f);
+    for (int h = 0; h < w.n; ++h, dx += D) {
+      issue();
+      ring.wait();
+      uint4 u0 = ring.read(0), u1 = ring.read(1);
+      if (w.kind < 2) {
+        HeadsRow f, d;
+        heads_unpack<BF16, PAIRS>(u0, u1, d);
+        heads_unpack<BF16, PAIRS>(ring.read(2), ring.read(3), f);
+        if (turns) heads_turn<true>(d, g, t);
+        float2 ss2 = make_float2(0.f, 0.f), dot2 = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float4 wa = heads_weight<LANES>(s_w, l, e / 2), wb = heads_weight<LANES>(s_w, l, 2 + e / 2);
-        ss2 = __ffma2_rn(f.b[e], f.b[e], __ffma2_rn(f.a[e], f.a[e], ss2));
-        dot2 = __ffma2_rn(__fmul2_rn(d.a[e], e & 1 ? make_float2(wa.z, wa.w) : make_float2(wa.x, wa.y)), f.a[e], dot2);
-        dot2 = __ffma2_rn(__fmul2_rn(d.b[e], e & 1 ? make_float2(wb.z, wb.w) : make_float2(wb.x, wb.y)), f.b[e], dot2);
-      }
-      float ss = ss2.x + ss2.y, dot = dot2.x + dot2.y;
+        for (int e = 0; e < 4; ++e) {
+          const float4 wa = heads_weight<LANES>(s_w, l, e / 2), wb = heads_weight<LANES>(s_w, l, 2 + e / 2);
+          ss2 = __ffma2_rn(f.b[e], f.b[e], __ffma2_rn(f.a[e], f.a[e], ss2));
+          dot2 = __ffma2_rn(__fmul2_rn(d.a[e], e & 1 ? make_float2(wa.z, wa.w) : make_float2(wa.x, wa.y)), f.a[e], dot2);
+          dot2 = __ffma2_rn(__fmul2_rn(d.b[e], e & 1 ? make_float2(wb.z, wb.w) : make_float2(wb.x, wb.y)), f.b[e], dot2);
+        }
+        float ss = ss2.x + ss2.y, dot = dot2.x + dot2.y;
 #pragma unroll
-      for (int s = 1; s < LANES; s <<= 1) {
-        ss += __shfl_xor_sync(0xffffffffu, ss, s);
-        dot += __shfl_xor_sync(0xffffffffu, dot, s);
-      }
-      const float r = rsqrtf(ss * (1.f / D) + p.eps);
-      const float2 r2 = splat(r), m2 = splat(-(r * r * dot * (1.f / D)));
+        for (int s = 1; s < LANES; s <<= 1) {
+          ss += __shfl_xor_sync(0xffffffffu, ss, s);
+          dot += __shfl_xor_sync(0xffffffffu, dot, s);
+        }
+        const float r = rsqrtf(ss * (1.f / D) + p.eps);
+        const float2 r2 = splat(r), m2 = splat(-(r * r * dot * (1.f / D)));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float4 wa = heads_weight<LANES>(s_w, l, e / 2), wb = heads_weight<LANES>(s_w, l, 2 + e / 2);
-        dw.a[e] = __ffma2_rn(__fmul2_rn(d.a[e], f.a[e]), r2, dw.a[e]);
-        dw.b[e] = __ffma2_rn(__fmul2_rn(d.b[e], f.b[e]), r2, dw.b[e]);
-        d.a[e] = __fmul2_rn(d.a[e], e & 1 ? make_float2(wa.z, wa.w) : make_float2(wa.x, wa.y));
-        d.b[e] = __fmul2_rn(d.b[e], e & 1 ? make_float2(wb.z, wb.w) : make_float2(wb.x, wb.y));
-        f.a[e] = __fmul2_rn(__ffma2_rn(f.a[e], m2, d.a[e]), r2);
-        f.b[e] = __fmul2_rn(__ffma2_rn(f.b[e], m2, d.b[e]), r2);
+        for (int e = 0; e < 4; ++e) {
+          const float4 wa = heads_weight<LANES>(s_w, l, e / 2), wb = heads_weight<LANES>(s_w, l, 2 + e / 2);
+          dw.a[e] = __ffma2_rn(__fmul2_rn(d.a[e], f.a[e]), r2, dw.a[e]);
+          dw.b[e] = __ffma2_rn(__fmul2_rn(d.b[e], f.b[e]), r2, dw.b[e]);
+          d.a[e] = __fmul2_rn(d.a[e], e & 1 ? make_float2(wa.z, wa.w) : make_float2(wa.x, wa.y));
+          d.b[e] = __fmul2_rn(d.b[e], e & 1 ? make_float2(wb.z, wb.w) : make_float2(wb.x, wb.y));
+          f.a[e] = __fmul2_rn(__ffma2_rn(f.a[e], m2, d.a[e]), r2);
+          f.b[e] = __fmul2_rn(__ffma2_rn(f.b[e], m2, d.b[e]), r2);
+        }
+        heads_pack<BF16, PAIRS>(f, u0, u1);
       }
-      heads_pack<BF16, PAIRS>(f, now.u0, now.u1);
-      if (valid) {
-        *reinterpret_cast<uint4*>(dx + h * D + t.c0) = now.u0;
-        *reinterpret_cast<uint4*>(dx + h * D + t.c1) = now.u1;
+      ring.taken();
+      if (k.valid) {
+        *reinterpret_cast<uint4*>(dx + t.c0) = u0;
+        *reinterpret_cast<uint4*>(dx + t.c1) = u1;
       }
-      now = next;
     }
   }
   if (w.kind == 2) return;

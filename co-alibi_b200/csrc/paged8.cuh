@@ -256,6 +256,13 @@ struct Read8Params {
 constexpr int kReadThreads = 256;
 constexpr int kReadRows = 16;  // tokens of a warp
 
+// 32 bytes in one store: a whole sector, where two of 16 bytes would each write half of every one of the warp's.
+__device__ __forceinline__ void store32(void* to, const uint32_t* y) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]),
+               "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7])
+               : "memory");
+}
+
 template <bool BF16, int D>
 __global__ void __launch_bounds__(kReadThreads) coalibi_paged_read8_kernel(const Read8Params p) {
   constexpr int PIECES = D / 16, RPW = 32 / PIECES, N = (kReadRows + RPW - 1) / RPW;
@@ -325,9 +332,7 @@ __global__ void __launch_bounds__(kReadThreads) coalibi_paged_read8_kernel(const
         y[e] = pack2<BF16>(u.x, u.y);
       }
     }
-    uint4* to = reinterpret_cast<uint4*>(out + (size_t)t * D);
-    to[0] = make_uint4(y[0], y[1], y[2], y[3]);
-    to[1] = make_uint4(y[4], y[5], y[6], y[7]);
+    store32(out + (size_t)t * D, y);
   }
 }
 

@@ -187,7 +187,7 @@ extern "C" int coalibi_paged_read8(const CoalibiPagedReadArgs* a, const CoalibiC
                        a->v_page_stride, a->table_stride);
   if (rc) return rc;
   if (a->S <= 0) return COALIBI_ERR_SHAPE;
-  if (!aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->positions, 4)) return COALIBI_ERR_ALIGNMENT;
+  if (!aligned(a->k, 32) || !aligned(a->v, 32) || !aligned(a->positions, 4)) return COALIBI_ERR_ALIGNMENT;
   if ((rc = check_codes(sc, a->k_pages, a->v_pages, a->k_page_stride, a->v_page_stride, a->n_pages, a->Hkv))) return rc;
   Read8Params p{};
   p.chunks = (a->S - 1) / kReadRows + 1;

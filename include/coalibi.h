@@ -314,7 +314,7 @@ typedef struct CoalibiPagedReadArgs {
   const void* v_pages;
   const int* page_table;  /* [B, max_pages] */
   const int* positions;   /* [B, S] contiguous */
-  void* k;                /* [B, Hkv, S, D] contiguous, dtype */
+  void* k;                /* [B, Hkv, S, D] contiguous, dtype; 32-byte aligned */
   void* v;
   int* status;
   long long k_page_stride[3], v_page_stride[3]; /* page, head, slot */

@@ -336,7 +336,7 @@ def test_refusals_of_the_read_entry():
     from co_alibi_attn import _lib
     lib = _lib.load()
     assert lib.coalibi_paged_read8(None, None, None) == 1
-    base = dict(k_pages=16, v_pages=16, page_table=16, positions=16, k=16, v=16, status=None, k_page_stride=(2048, 1024, 64),
+    base = dict(k_pages=16, v_pages=16, page_table=16, positions=16, k=32, v=32, status=None, k_page_stride=(2048, 1024, 64),
                 v_page_stride=(2048, 1024, 64), table_stride=4, B=2, Hkv=2, S=3, D=64, page_size=16, max_pages=4, n_pages=8, dtype=1)
 
     def code(scales=None, **kw):
@@ -351,7 +351,7 @@ def test_refusals_of_the_read_entry():
     for bad in (dict(B=0), dict(S=0), dict(S=-4), dict(page_size=24), dict(max_pages=1 << 28), dict(B=65535, Hkv=65535, S=1 << 20),
                 dict(scales=dict(k_stride=(0, 1)))):
         assert code(**bad) == 4, bad
-    for bad in (dict(k=8), dict(v=18), dict(k_pages=8), dict(positions=18), dict(v_page_stride=(2048, 1032, 64))):
+    for bad in (dict(k=16), dict(v=18), dict(k_pages=8), dict(positions=18), dict(v_page_stride=(2048, 1032, 64))):
         assert code(**bad) == 5, bad
 
 
