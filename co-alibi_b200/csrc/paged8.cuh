@@ -248,13 +248,13 @@ struct Read8Params {
   long long kps[3], vps[3], kss[2], vss[2];
   long long table_stride;
   int Hkv, S;
-  int chunks;  // of kReadRows tokens
-  int tiles;   // B * 2 Hkv * chunks
+  int chunks;  // of the tokens that a CTA takes
+  int per;     // of the 2 Hkv rows of heads that a CTA goes over
   int page_size, page_shift, max_pages, n_pages;  // page_shift: log2(page_size), or -1
 };
 
 constexpr int kReadThreads = 256;
-constexpr int kReadRows = 16;  // tokens of a warp
+constexpr int kReadUnroll = 8;  // heads whose codes a thread has on their way
 
 // 32 bytes in one store: a whole sector, where two of 16 bytes would each write half of every one of the warp's.
 __device__ __forceinline__ void store32(void* to, const uint32_t* y) {
@@ -263,33 +263,17 @@ __device__ __forceinline__ void store32(void* to, const uint32_t* y) {
                : "memory");
 }
 
+// A thread takes 16 columns of a token, looks the token up once and goes over heads.
 template <bool BF16, int D>
-__global__ void __launch_bounds__(kReadThreads) coalibi_paged_read8_kernel(const Read8Params p) {
-  constexpr int PIECES = D / 16, RPW = 32 / PIECES, N = (kReadRows + RPW - 1) / RPW;
+__global__ void __launch_bounds__(kReadThreads, 4) coalibi_paged_read8_kernel(const Read8Params p) {
+  constexpr int PIECES = D / 16, TOKENS = kReadThreads / PIECES;
   grid_dep_wait();
-  const int lane = threadIdx.x & 31;
-  const int tile = (int)blockIdx.x * (kReadThreads / 32) + (threadIdx.x >> 5);
-  if (tile >= p.tiles) return;
-  const int at = tile / p.chunks, chunk = tile - at * p.chunks;
-  const int b = at / (2 * p.Hkv), row = at - b * 2 * p.Hkv;
-  const bool key = row < p.Hkv;
-  const int h = key ? row : row - p.Hkv;
-  const int c = (lane % PIECES) * 16;
-  const uint8_t* pages = static_cast<const uint8_t*>(key ? p.k_pages : p.v_pages) + h * (key ? p.kps[1] : p.vps[1]) + c;
-  const float* scales = (key ? p.k_scales + h * p.kss[1] : p.v_scales + h * p.vss[1]);
-  const long long ps = key ? p.kps[0] : p.vps[0], ss = key ? p.kps[2] : p.vps[2], cs = key ? p.kss[0] : p.vss[0];
-  uint16_t* out = static_cast<uint16_t*>(key ? p.k : p.v) + (((size_t)b * p.Hkv + h) * p.S) * D + c;
-  uint4 codes[N];
-  float scale[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int t = chunk * kReadRows + lane / PIECES + i * RPW;
-    codes[i] = make_uint4(0u, 0u, 0u, 0u);
-    scale[i] = 0.f;
-    if (t >= p.S) continue;
-    const int pos = p.positions[(size_t)b * p.S + t];
-    if (pos < 0) continue;
-    int page = -1, slot = 0;
+  const int b = blockIdx.x / p.chunks, t = (blockIdx.x - b * p.chunks) * TOKENS + threadIdx.x / PIECES;
+  if (t >= p.S) return;
+  const int c = (threadIdx.x % PIECES) * 16;
+  const int pos = p.positions[(size_t)b * p.S + t];
+  int page = -1, slot = 0;
+  if (pos >= 0) {
     if (pos < p.max_pages * p.page_size) {
       const int n = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
       slot = pos - n * p.page_size;
@@ -297,42 +281,61 @@ __global__ void __launch_bounds__(kReadThreads) coalibi_paged_read8_kernel(const
     }
     if (page < 0 || page >= p.n_pages) {
       if (c == 0) report_page(p.status);
-      continue;
+      page = -1;
     }
-    codes[i] = *reinterpret_cast<const uint4*>(pages + page * ps + slot * ss);
-    scale[i] = scales[page * cs + slot / kQuantBlock];
   }
+  const int row0 = blockIdx.y * p.per, row1 = min(row0 + p.per, 2 * p.Hkv);
+  // (pointers of keys and values at head 0)
+  const uint8_t* codes_at[2] = {static_cast<const uint8_t*>(p.k_pages) + page * p.kps[0] + slot * p.kps[2] + c,
+                                static_cast<const uint8_t*>(p.v_pages) + page * p.vps[0] + slot * p.vps[2] + c};
+  const float* scale_at[2] = {p.k_scales + page * p.kss[0] + slot / kQuantBlock, p.v_scales + page * p.vss[0] + slot / kQuantBlock};
+  const size_t to = ((size_t)b * p.Hkv * p.S + t) * D + c, head = (size_t)p.S * D;
   // Codes times scale, rounded once.  A scale by which no code passes the type's largest needs no clamp; a
   // power of two within float16's range multiplies there, where the product is rounded once too.
   const float top = BF16 ? 3.38953139e38f : 65504.f;
+  for (int row = row0; row < row1; row += kReadUnroll) {
+    uint4 codes[kReadUnroll];
+    float scale[kReadUnroll];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int t = chunk * kReadRows + lane / PIECES + i * RPW;
-    if (t >= p.S) continue;
-    const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
-    uint32_t y[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) e4m3_to_f16x4(w[e], y[2 * e], y[2 * e + 1]);
-    if (!BF16 && scale[i] <= 128.f && scale[i] >= 5.9604645e-8f && (__float_as_int(scale[i]) & 0x7fffff) == 0) {
-      const __half2 s = __float2half2_rn(scale[i]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&y[e]), s);
-        y[e] = *reinterpret_cast<const uint32_t*>(&v);
-      }
-    } else {
-      const bool clamps = !(scale[i] <= (BF16 ? 7e35f : 128.f));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float2 u = __fmul2_rn(f16x2_to_float2(y[e]), make_float2(scale[i], scale[i]));
-        if (clamps) {  // (NaN stays)
-          u.x = u.x > top ? top : u.x < -top ? -top : u.x;
-          u.y = u.y > top ? top : u.y < -top ? -top : u.y;
-        }
-        y[e] = pack2<BF16>(u.x, u.y);
+    for (int i = 0; i < kReadUnroll; ++i) {
+      const bool key = row + i < p.Hkv;
+      const int h = key ? row + i : row + i - p.Hkv;
+      codes[i] = make_uint4(0u, 0u, 0u, 0u);
+      scale[i] = 1.f;
+      if (page >= 0 && row + i < row1) {
+        codes[i] = *reinterpret_cast<const uint4*>(key ? codes_at[0] + h * p.kps[1] : codes_at[1] + h * p.vps[1]);
+        scale[i] = key ? scale_at[0][h * p.kss[1]] : scale_at[1][h * p.vss[1]];
       }
     }
-    store32(out + (size_t)t * D, y);
+#pragma unroll
+    for (int i = 0; i < kReadUnroll; ++i) {
+      if (row + i >= row1) break;
+      const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+      uint32_t y[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) e4m3_to_f16x4(w[e], y[2 * e], y[2 * e + 1]);
+      if (!BF16 && scale[i] <= 128.f && scale[i] >= 5.9604645e-8f && (__float_as_int(scale[i]) & 0x7fffff) == 0) {
+        const __half2 s = __float2half2_rn(scale[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&y[e]), s);
+          y[e] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+      } else {
+        const bool clamps = !(scale[i] <= (BF16 ? 7e35f : 128.f));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float2 u = __fmul2_rn(f16x2_to_float2(y[e]), make_float2(scale[i], scale[i]));
+          if (clamps) {  // (NaN stays)
+            u.x = u.x > top ? top : u.x < -top ? -top : u.x;
+            u.y = u.y > top ? top : u.y < -top ? -top : u.y;
+          }
+          y[e] = pack2<BF16>(u.x, u.y);
+        }
+      }
+      const bool key = row + i < p.Hkv;
+      store32(static_cast<uint16_t*>(key ? p.k : p.v) + to + (key ? row + i : row + i - p.Hkv) * head, y);
+    }
   }
 }
 

@@ -190,9 +190,9 @@ extern "C" int coalibi_paged_read8(const CoalibiPagedReadArgs* a, const CoalibiC
   if (!aligned(a->k, 32) || !aligned(a->v, 32) || !aligned(a->positions, 4)) return COALIBI_ERR_ALIGNMENT;
   if ((rc = check_codes(sc, a->k_pages, a->v_pages, a->k_page_stride, a->v_page_stride, a->n_pages, a->Hkv))) return rc;
   Read8Params p{};
-  p.chunks = (a->S - 1) / kReadRows + 1;
-  const long long tiles = (long long)a->B * 2 * a->Hkv * p.chunks;
-  if (tiles > 0x7fffffffLL - 64) return COALIBI_ERR_SHAPE;
+  const int tokens = kReadThreads / (a->D / 16);
+  p.chunks = (a->S - 1) / tokens + 1;
+  if ((long long)a->B * p.chunks > 0x7fffffffLL || a->Hkv > 32767) return COALIBI_ERR_SHAPE;
   CtxGuard guard;
   if ((rc = enter_device(a->k_pages, stream))) return rc;
   p.k_pages = a->k_pages;
@@ -211,7 +211,9 @@ extern "C" int coalibi_paged_read8(const CoalibiPagedReadArgs* a, const CoalibiC
   p.table_stride = a->table_stride;
   p.Hkv = a->Hkv;
   p.S = a->S;
-  p.tiles = (int)tiles;
+  // all heads to a CTA where tokens are plenty, else fewer, so that every SM has some
+  p.per = 2 * a->Hkv;
+  while (p.per > 1 && (long long)a->B * p.chunks * (2 * a->Hkv / p.per) < 2LL * device_sm_count()) p.per = (p.per + 1) / 2;
   p.page_size = a->page_size;
   p.max_pages = a->max_pages;
   p.n_pages = a->n_pages;
@@ -219,8 +221,8 @@ extern "C" int coalibi_paged_read8(const CoalibiPagedReadArgs* a, const CoalibiC
   const bool bf16 = a->dtype == COALIBI_BF16;
   auto kernel = a->D == 128 ? (bf16 ? coalibi_paged_read8_kernel<true, 128> : coalibi_paged_read8_kernel<false, 128>)
                             : (bf16 ? coalibi_paged_read8_kernel<true, 64> : coalibi_paged_read8_kernel<false, 64>);
-  const unsigned ctas = (unsigned)((tiles + kReadThreads / 32 - 1) / (kReadThreads / 32));
-  if (const cudaError_t e = launch_pdl(kernel, dim3(ctas), dim3(kReadThreads), 0, static_cast<cudaStream_t>(stream), p);
+  const dim3 grid((unsigned)(a->B * p.chunks), (2 * a->Hkv + p.per - 1) / p.per);
+  if (const cudaError_t e = launch_pdl(kernel, grid, dim3(kReadThreads), 0, static_cast<cudaStream_t>(stream), p);
       e != cudaSuccess) {
     set_last_error_detail(cudaGetErrorString(e));
     return COALIBI_ERR_LAUNCH;
