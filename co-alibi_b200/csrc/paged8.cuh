@@ -55,31 +55,33 @@ struct Append8Params : AppendParams {
   float* k_scales;
   float* v_scales;
   long long kss[2], vss[2];  // page, head
+  int page_shift;            // log2(page_size), or -1
   int blocks;                // that a request's S tokens may touch
-  int tiles;                 // B * blocks * 2 Hkv
-  int kv_ctas;
+  int chunks;                // of the Hkv heads, one head to a warp
+  int kv_ctas;               // B * blocks * 2 chunks
 };
 
 template <bool BF16, int D, int TURN>
-__global__ void __launch_bounds__(kAppendThreads, D == 128 ? 3 : 4) coalibi_paged_append8_kernel(const Append8Params p) {
+__global__ void __launch_bounds__(kAppendThreads, 4) coalibi_paged_append8_kernel(const Append8Params p) {
   constexpr int PIECES = D / 8;
+  __shared__ __align__(16) float s_angle[TURN == kTurnNone ? 1 : 2][TURN == kTurnNone ? 4 : kQuantBlock * D / 2];
+  __shared__ bool s_turned[kQuantBlock];  // whether a token has angles
   grid_dep_wait();
   const int tid = threadIdx.x, half = p.rot / 2;
   if ((int)blockIdx.x >= p.kv_ctas) {  // ---- queries: a thread keeps its column, as in the 16-bit append
     const long long first = (long long)((int)blockIdx.x - p.kv_ctas) * p.group;
     const int n = (int)min((long long)p.group, p.tokens - first);
-    constexpr int STEP = kAppendThreads / PIECES;
-    const int r0 = tid / PIECES, c = (tid % PIECES) * 8;
+    const int step = blockDim.x / PIECES, r0 = tid / PIECES, c = (tid % PIECES) * 8;
     const int partner = c < half ? half : -half;
     const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
     for (int k = 0; k < n; ++k) {
-      const int b = (int)((first + k) / p.S), i = (int)(first + k - (long long)b * p.S);
+      const int b = (int)(first + k) / p.S, i = (int)(first + k) - b * p.S;
       const bool fresh = i < (p.count != nullptr ? p.count[b] : p.S);
       const uint16_t* x = static_cast<const uint16_t*>(p.q) + b * p.qs[0] + i * p.qs[2] + r0 * p.qs[1] + c;
       uint16_t* y = static_cast<uint16_t*>(p.q_out) + b * p.qos[0] + i * p.qos[2] + r0 * p.qos[1] + c;
-      const long long dx = STEP * p.qs[1], dy = STEP * p.qos[1];
+      const long long dx = step * p.qs[1], dy = step * p.qos[1];
       if (!fresh) {
-        for (int row = r0; row < p.Hq; row += STEP, y += dy) *reinterpret_cast<uint4*>(y) = zero;
+        for (int row = r0; row < p.Hq; row += step, y += dy) *reinterpret_cast<uint4*>(y) = zero;
         continue;
       }
       bool turn = false;
@@ -90,7 +92,7 @@ __global__ void __launch_bounds__(kAppendThreads, D == 128 ? 3 : 4) coalibi_page
         if (turn) g.load(p.cos + (size_t)pos * half, p.sin + (size_t)pos * half, c, half);
       }
 #pragma unroll 2
-      for (int row = r0; row < p.Hq; row += STEP, x += dx, y += dy) {
+      for (int row = r0; row < p.Hq; row += step, x += dx, y += dy) {
         uint4 val = *reinterpret_cast<const uint4*>(x);
         if (turn)
           val = g.template turn<BF16>(val, TURN == kTurnHalves ? *reinterpret_cast<const uint4*>(x + partner) : zero);
@@ -99,133 +101,176 @@ __global__ void __launch_bounds__(kAppendThreads, D == 128 ? 3 : 4) coalibi_page
     }
     return;
   }
-  // ---- keys and values: a warp takes the 16 tokens of a block for one head
+  // ---- keys or values: a warp takes the 16 tokens of a block for one head.  Keys and values, and blocks, are
+  // CTAs of their own, so that the warps of one share the tokens' angles.
   const int lane = tid & 31;
-  const int tile = (int)blockIdx.x * (kAppendThreads / 32) + (tid >> 5);
-  if (tile >= p.tiles) return;
-  const int heads = 2 * p.Hkv, at = tile / heads, row = tile - at * heads;
+  const int at = blockIdx.x / (2 * p.chunks), part = blockIdx.x - at * 2 * p.chunks;
   const int b = at / p.blocks, j = at - b * p.blocks;
-  const bool key = row < p.Hkv;
-  const int h = key ? row : row - p.Hkv;
+  const bool key = part < p.chunks;
+  const int h = (key ? part : part - p.chunks) * (blockDim.x / 32) + (tid >> 5);
   const int start = p.start[b];
   const int fresh = min(p.count != nullptr ? p.count[b] : p.S, p.S);
   if (fresh <= 0) return;
   if (start < 0) {
-    if (lane == 0) report_page(p.status);
+    if (tid == 0) report_page(p.status);
     return;
   }
   const long long t0 = ((long long)(start / kQuantBlock) + j) * kQuantBlock;  // the block's first token
+  // its tokens of this call
   const int lo = (int)max((long long)start - t0, 0ll), hi = (int)min((long long)start + fresh - t0, (long long)kQuantBlock);
   if (lo >= hi) return;
+  constexpr int RPW = 32 / PIECES, N = kQuantBlock / RPW;  // rows of a pass of the warp, passes
+  const int l = lane % PIECES, r0 = lane / PIECES;
+  // A lane's 8 columns: where it turns in halves, 4 and their partners; else neighbours.
+  const bool turns = TURN != kTurnNone && key && 8 * l < p.rot, split = TURN == kTurnHalves && turns;
+  const int ca = split ? 4 * l : 8 * l, cb = split ? half + 4 * l : 8 * l + 4;
+  uint4 raw[N];
+  {
+    const long long* xs = key ? p.ks : p.vs;
+    const uint16_t* x = static_cast<const uint16_t*>(key ? p.k : p.v) + b * xs[0] + h * xs[1] + (t0 - start + r0) * xs[2];
+    const long long step = RPW * xs[2];
+#pragma unroll
+    for (int i = 0; i < N; ++i, x += step) {
+      const int r = r0 + i * RPW;
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (r >= lo && r < hi && h < p.Hkv) {
+        if (split) {
+          const uint2 u = *reinterpret_cast<const uint2*>(x + ca), v = *reinterpret_cast<const uint2*>(x + cb);
+          raw[i] = make_uint4(u.x, u.y, v.x, v.y);
+        } else {
+          raw[i] = *reinterpret_cast<const uint4*>(x + ca);
+        }
+      }
+    }
+  }
   int page = -1, slot = 0;
   if (t0 < (long long)p.max_pages * p.page_size) {
-    const int n = (int)(t0 / p.page_size);
-    slot = (int)(t0 - (long long)n * p.page_size);
+    const int n = p.page_shift >= 0 ? (int)t0 >> p.page_shift : (int)t0 / p.page_size;
+    slot = (int)t0 - n * p.page_size;
     page = p.page_table[(size_t)b * p.table_stride + n];
   }
-  const bool stored = page >= 0 && page < p.n_pages;
-  if (!stored && lane == 0) report_page(p.status);
-  if (!stored) return;
-
-  constexpr int RPW = 32 / PIECES, N = kQuantBlock / RPW;  // rows of a pass of the warp, passes
-  const int c = (lane % PIECES) * 8, r0 = lane / PIECES;
-  const long long* xs = key ? p.ks : p.vs;
-  const uint16_t* x = static_cast<const uint16_t*>(key ? p.k : p.v) + b * xs[0] + h * xs[1] + (t0 - start) * xs[2] + c;
-  uint4 raw[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int r = r0 + i * RPW;
-    raw[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (r >= lo && r < hi) raw[i] = *reinterpret_cast<const uint4*>(x + r * xs[2]);
+  if (TURN != kTurnNone && key) {
+    const int row4 = half / 4;  // pieces of a row
+    for (int e = tid; e < kQuantBlock * row4; e += blockDim.x) {
+      const int r = e / row4, c = (e - r * row4) * 4;
+      if (r < lo || r >= hi) continue;
+      const long long pos = p.positions != nullptr ? p.positions[(size_t)b * p.S + (t0 + r - start)] : t0 + r;
+      const bool has = pos >= 0 && pos < p.n_pos;
+      if (c == 0) s_turned[r] = has;
+      if (has) {
+        *reinterpret_cast<float4*>(&s_angle[0][r * half + c]) = *reinterpret_cast<const float4*>(p.cos + (size_t)pos * half + c);
+        *reinterpret_cast<float4*>(&s_angle[1][r * half + c]) = *reinterpret_cast<const float4*>(p.sin + (size_t)pos * half + c);
+      } else if (c == 0) {
+        report_page(p.status);
+      }
+    }
+    __syncthreads();
+  }
+  if (h >= p.Hkv) return;
+  if (page < 0 || page >= p.n_pages) {
+    if (lane == 0) report_page(p.status);
+    return;
   }
   float* scale_at = (key ? p.k_scales + page * p.kss[0] + h * p.kss[1] : p.v_scales + page * p.vss[0] + h * p.vss[1]) +
                     slot / kQuantBlock;
   const float was = lo > 0 ? *scale_at : 0.f;  // the block holds tokens already
-  // Row i's values (r its token of the block), rotated where it has angles.  Computed twice, for the block's
-  // largest and for the codes: the rows in float32 would take twice the registers.
-  bool lost = false;  // some token has no angles
-  auto values = [&](int i, int r, float* f) {
-    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 u = unpack2<BF16>(w[e]);
-      f[2 * e] = u.x, f[2 * e + 1] = u.y;
-    }
-    if (TURN == kTurnNone || !key || c >= p.rot || r < lo || r >= hi) return;
-    const long long tok = t0 + r, at_pos = p.positions != nullptr ? p.positions[(size_t)b * p.S + (tok - start)] : tok;
-    if (at_pos < 0 || at_pos >= p.n_pos) {
-      lost = true;
-      return;
-    }
-    Angles<TURN> g;
-    g.load(p.cos + (size_t)at_pos * half, p.sin + (size_t)at_pos * half, c, half);
-    // products and their sum rounded one by one: the same codes as plain float32 arithmetic gives
+  // Row i: f[0], f[1] and f[2], f[3] are the a and the b of pairs (a, b); without a rotation, the columns in order.
+  // Computed twice, for the block's largest and for the codes: the rows in float32 would take twice the registers
+  // and leave half the warps.
+  auto values = [&](int i, float2* f) {
+    const float2 w[4] = {unpack2<BF16>(raw[i].x), unpack2<BF16>(raw[i].y), unpack2<BF16>(raw[i].z), unpack2<BF16>(raw[i].w)};
     if (TURN == kTurnPairs) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float a0 = f[2 * e], a1 = f[2 * e + 1];
-        f[2 * e] = __fsub_rn(__fmul_rn(a0, g.cs[e]), __fmul_rn(a1, g.sn[e]));
-        f[2 * e + 1] = __fadd_rn(__fmul_rn(a1, g.cs[e]), __fmul_rn(a0, g.sn[e]));
-      }
+      f[0] = make_float2(w[0].x, w[1].x), f[1] = make_float2(w[2].x, w[3].x);
+      f[2] = make_float2(w[0].y, w[1].y), f[3] = make_float2(w[2].y, w[3].y);
     } else {
-      const uint4 other = *reinterpret_cast<const uint4*>(x + r * xs[2] + (c < half ? half : -half));
-      const uint32_t o[4] = {other.x, other.y, other.z, other.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 u = unpack2<BF16>(o[e]);
-        f[2 * e] = __fadd_rn(__fmul_rn(f[2 * e], g.cs[2 * e % g.N]), __fmul_rn(u.x, g.sn[2 * e % g.N]));
-        f[2 * e + 1] = __fadd_rn(__fmul_rn(f[2 * e + 1], g.cs[(2 * e + 1) % g.N]), __fmul_rn(u.y, g.sn[(2 * e + 1) % g.N]));
-      }
+      for (int e = 0; e < 4; ++e) f[e] = w[e];
+    }
+    const int r = r0 + i * RPW;
+    if (!turns || r < lo || r >= hi || !s_turned[r]) return;
+    const float4 c4 = *reinterpret_cast<const float4*>(&s_angle[0][r * half + 4 * l]);
+    const float4 s4 = *reinterpret_cast<const float4*>(&s_angle[1][r * half + 4 * l]);
+    // products and their sum rounded one by one: the same codes as plain float32 arithmetic gives
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float2 cs = e ? make_float2(c4.z, c4.w) : make_float2(c4.x, c4.y);
+      const float2 sn = e ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y);
+      const float2 u = f[e], v = f[2 + e], vs = __fmul2_rn(v, sn);
+      f[e] = __fadd2_rn(__fmul2_rn(u, cs), make_float2(-vs.x, -vs.y));
+      f[2 + e] = __fadd2_rn(__fmul2_rn(v, cs), __fmul2_rn(u, sn));
     }
   };
+  auto some = [&](int i) { return i * RPW < hi && (i + 1) * RPW > lo; };  // whether row i of any lane is new
   float most = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    float f[8];
-    values(i, r0 + i * RPW, f);
+    if (!some(i)) continue;
+    float2 f[4];
+    values(i, f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = fabsf(f[e]);
-      most = fmaxf(most, a < INFINITY ? a : 0.f);
-    }
+    for (int e = 0; e < 4; ++e) most = fmaxf(most, fmaxf(fabsf(f[e].x), fabsf(f[e].y)));  // (passes over NaN)
   }
-  if (lost && c == 0) report_page(p.status);
-  most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-  const float scale = fmaxf(quant_scale(most), was), inv = 1.f / scale;
-  uint8_t* y = static_cast<uint8_t*>(key ? p.k_pages : p.v_pages) +
-               (key ? page * p.kps[0] + h * p.kps[1] + slot * p.kps[2] : page * p.vps[0] + h * p.vps[1] + slot * p.vps[2]) + c;
-  const long long ys = key ? p.kps[2] : p.vps[2];
-  if (lo > 0 && scale != was) {  // the tokens that the block held: the same values by the new scale
-    const float ratio = was / scale;
+  const bool infinite = __any_sync(0xffffffffu, most == INFINITY);
+  if (infinite) {  // an infinity has no code: NaN, not the block's largest
+    most = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int r = r0 + i * RPW;
-      if (r < lo) {
-        uint2* at_old = reinterpret_cast<uint2*>(y + r * ys);
-        const uint2 u = *at_old;
-        uint32_t g[4];
-        e4m3_to_f16x4(u.x, g[0], g[1]);
-        e4m3_to_f16x4(u.y, g[2], g[3]);
-        float2 v[4];
+      float2 f[4];
+      values(i, f);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = f16x2_to_float2(g[e]);
-          v[e].x *= ratio, v[e].y *= ratio;
-        }
-        *at_old = make_uint2(e4m3_from(v[0].x, v[0].y, v[1].x, v[1].y), e4m3_from(v[2].x, v[2].y, v[3].x, v[3].y));
+      for (int e = 0; e < 4; ++e) {
+        most = fmaxf(most, fabsf(f[e].x) == INFINITY ? 0.f : fabsf(f[e].x));
+        most = fmaxf(most, fabsf(f[e].y) == INFINITY ? 0.f : fabsf(f[e].y));
       }
     }
   }
+  most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+  const float scale = fmaxf(quant_scale(most), was), inv = 1.f / scale;
+  uint8_t* y = static_cast<uint8_t*>(key ? p.k_pages : p.v_pages) +
+               (key ? page * p.kps[0] + h * p.kps[1] + (slot + r0) * p.kps[2] : page * p.vps[0] + h * p.vps[1] + (slot + r0) * p.vps[2]);
+  const long long step = RPW * (key ? p.kps[2] : p.vps[2]);
+  if (lo > 0 && scale != was) {  // the tokens that the block held: the same values by the new scale
+    const float ratio = was / scale;
+    uint8_t* at_old = y + 8 * l;
+#pragma unroll 1
+    for (int r = r0; r < lo; r += RPW, at_old += step) {
+      const uint2 u = *reinterpret_cast<const uint2*>(at_old);
+      uint32_t g[4];
+      e4m3_to_f16x4(u.x, g[0], g[1]);
+      e4m3_to_f16x4(u.y, g[2], g[3]);
+      float2 v[4];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+      for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(f16x2_to_float2(g[e]), make_float2(ratio, ratio));
+      *reinterpret_cast<uint2*>(at_old) =
+          make_uint2(e4m3_from(v[0].x, v[0].y, v[1].x, v[1].y), e4m3_from(v[2].x, v[2].y, v[3].x, v[3].y));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)  // (so that nothing of the first pass is kept for the codes)
+    asm volatile("" : "+r"(raw[i].x), "+r"(raw[i].y), "+r"(raw[i].z), "+r"(raw[i].w));
+#pragma unroll
+  for (int i = 0; i < N; ++i, y += step) {
     const int r = r0 + i * RPW;
-    if (r >= lo && r < hi) {
-      float f[8];
-      values(i, r, f);
-      // an infinity has no code: NaN, not the block's largest
+    if (some(i) && r >= lo && r < hi) {
+      float2 f[4];
+      values(i, f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = fabsf(f[e]) < INFINITY ? f[e] * inv : __int_as_float(0x7fc00000);
-      *reinterpret_cast<uint2*>(y + r * ys) = make_uint2(e4m3_from(f[0], f[1], f[2], f[3]), e4m3_from(f[4], f[5], f[6], f[7]));
+      for (int e = 0; e < 4; ++e) {
+        if (infinite && fabsf(f[e].x) == INFINITY) f[e].x = __int_as_float(0x7fc00000);
+        if (infinite && fabsf(f[e].y) == INFINITY) f[e].y = __int_as_float(0x7fc00000);
+        f[e] = __fmul2_rn(f[e], make_float2(inv, inv));
+      }
+      uint2 codes;
+      if (TURN == kTurnPairs)
+        codes = make_uint2(e4m3_from(f[0].x, f[2].x, f[0].y, f[2].y), e4m3_from(f[1].x, f[3].x, f[1].y, f[3].y));
+      else
+        codes = make_uint2(e4m3_from(f[0].x, f[0].y, f[1].x, f[1].y), e4m3_from(f[2].x, f[2].y, f[3].x, f[3].y));
+      if (split) {
+        *reinterpret_cast<uint32_t*>(y + ca) = codes.x;
+        *reinterpret_cast<uint32_t*>(y + cb) = codes.y;
+      } else {
+        *reinterpret_cast<uint2*>(y + ca) = codes;
+      }
     }
   }
   if (lane == 0 && scale != was) *scale_at = scale;

@@ -113,8 +113,11 @@ extern "C" int coalibi_paged_append8(const CoalibiPagedAppendArgs* a, const Coal
   if ((rc = check_codes(sc, a->k_pages, a->v_pages, a->k_page_stride, a->v_page_stride, a->n_pages, a->Hkv))) return rc;
   Append8Params p{};
   p.blocks = (a->S + kQuantBlock - 2) / kQuantBlock + 1;
-  const long long tiles = (long long)a->B * p.blocks * 2 * a->Hkv;
-  if (tiles > 0x7fffffffLL - 64) return COALIBI_ERR_SHAPE;
+  // a head to a warp, up to eight warps to a CTA
+  p.chunks = (a->Hkv + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
+  const int threads = 32 * ((a->Hkv + p.chunks - 1) / p.chunks);
+  const long long kv_ctas = (long long)a->B * p.blocks * 2 * p.chunks;
+  if (kv_ctas > 0x7fffffffLL) return COALIBI_ERR_SHAPE;
   CtxGuard guard;
   if ((rc = enter_device(a->k_pages, stream))) return rc;
   p.k = a->k;
@@ -151,8 +154,8 @@ extern "C" int coalibi_paged_append8(const CoalibiPagedAppendArgs* a, const Coal
   p.v_scales = sc->v;
   copy2(p.kss, sc->k_stride);
   copy2(p.vss, sc->v_stride);
-  p.tiles = (int)tiles;
-  p.kv_ctas = (int)((tiles + kAppendThreads / 32 - 1) / (kAppendThreads / 32));
+  p.page_shift = page_shift_of(a->page_size);
+  p.kv_ctas = (int)kv_ctas;
   p.group = p.tokens >= 8LL * kAppendGroup * device_sm_count() ? kAppendGroup : 1;
   const long long q_ctas = a->q != nullptr ? (p.tokens + p.group - 1) / p.group : 0;
   if (p.kv_ctas + q_ctas > 0x7fffffffLL) return COALIBI_ERR_SHAPE;
@@ -164,7 +167,7 @@ extern "C" int coalibi_paged_append8(const CoalibiPagedAppendArgs* a, const Coal
   // without keys), whose CTAs take a third of the registers.
   const bool apart = q_ctas > 0 && p.group > 1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_pdl(kernel, dim3((unsigned)(p.kv_ctas + (apart ? 0 : q_ctas))), dim3(kAppendThreads), 0, s, p);
+  cudaError_t e = launch_pdl(kernel, dim3((unsigned)(p.kv_ctas + (apart ? 0 : q_ctas))), dim3(threads), 0, s, p);
   if (e == cudaSuccess && apart) {
     AppendParams q = p;
     q.Hkv = 0;
