@@ -10,8 +10,8 @@ import math
 import torch
 import torch.nn.functional as F
 
-from co_alibi_attn import append_paged_kv, paged_tree_attention, sample_tokens
-from co_alibi_attn.serving import TREE_MAX_SQ, rotary_tables
+from co_alibi_attn import append_paged_kv, paged_tree_attention, read_paged_kv, sample_tokens
+from co_alibi_attn.serving import QUANT_BLOCK, TREE_MAX_SQ, rotary_tables
 
 from .model import rotate_heads
 
@@ -23,15 +23,26 @@ class PagedCache:
     pools [n_pages, H, page_size, D], one page table for all layers, and the lengths.
     ``spare`` further slots take the drafts of a step that starts near the end: a tree's
     slots run ahead of its depths, so they may be needed though few are accepted.  In all a
-    request has ``capacity`` slots, every one with its row of the rotary tables."""
+    request has ``capacity`` slots, every one with its row of the rotary tables.
 
-    def __init__(self, model, batch, max_len, page_size=64, spare=TREE_MAX_SQ):
+    ``kv_dtype``: the model's own (default), or ``torch.float8_e4m3fn`` for half the memory
+    and reads: codes with a scale for each block of 16 tokens and head, ``scales`` of each layer."""
+
+    def __init__(self, model, batch, max_len, page_size=64, spare=TREE_MAX_SQ, kv_dtype=None):
         cfg, weight = model.cfg, model.emb.weight
+        kv_dtype = kv_dtype or weight.dtype
+        if kv_dtype not in (weight.dtype, torch.float8_e4m3fn):
+            raise ValueError(f"the cache holds {weight.dtype} or float8_e4m3fn, got {kv_dtype}")
         per = -(-(max_len + spare) // page_size)
         self.capacity = per * page_size
         shape = (batch * per, cfg.n_head, page_size, cfg.d_model // cfg.n_head)
-        self.k = [torch.empty(shape, dtype=weight.dtype, device=weight.device) for _ in range(cfg.n_layer)]
+        self.k = [torch.empty(shape, dtype=kv_dtype, device=weight.device) for _ in range(cfg.n_layer)]
         self.v = [torch.empty_like(k) for k in self.k]
+        self.dtype = weight.dtype
+        self.scales = None
+        if kv_dtype == torch.float8_e4m3fn:
+            blocks = (*shape[:2], page_size // QUANT_BLOCK)
+            self.scales = [tuple(torch.empty(blocks, device=weight.device) for _ in range(2)) for _ in range(cfg.n_layer)]
         self.table = torch.arange(batch * per, dtype=torch.int32, device=weight.device).view(batch, per)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=weight.device)
         self.rotary = rotary_tables(cfg.rotary_dim, self.capacity, device=weight.device) if cfg.rotary_dim else None
@@ -54,6 +65,23 @@ class PagedCache:
         """The cached rows of tokens at [B, n] of each request: [B, H, n, D]."""
         page, slot = self.where(at)
         return pages[page, :, slot].transpose(1, 2)
+
+    def of(self, layer):
+        """What the operators' calls take of a layer besides its pools, as keywords."""
+        return {} if self.scales is None else {"scales": self.scales[layer]}
+
+    def move(self, at, count):
+        """Appends to each request the first ``count`` [B] of its tokens at [B, n], of every layer."""
+        if self.scales is None:
+            page, slot = self.where(at)
+        else:
+            at = at.clamp(max=self.capacity - 1)
+        for layer, (k, v) in enumerate(zip(self.k, self.v)):
+            if self.scales is None:
+                new = (x[page, :, slot].transpose(1, 2) for x in (k, v))
+            else:
+                new = read_paged_kv(k, v, self.table, at, self.scales[layer], dtype=self.dtype)
+            append_paged_kv(*new, k, v, self.table, self.lens, count=count, **self.of(layer))
 
 
 def _mlp(blk, x):
@@ -81,11 +109,14 @@ def prefill(model, cache, tokens, counts=None):
     if S > cache.capacity and (counts is None or cache.rotary is not None):
         raise ValueError(f"prompts of {S} tokens, but the cache holds {cache.capacity} of each request")
     for layer, blk in enumerate(model.blocks):
-        q, k, v = blk.attn.heads(blk.ln1(x))
-        if cache.rotary is not None:
-            cos, sin = (t[:S] for t in cache.rotary)
-            q, k = rotate_heads(q, cos, sin), rotate_heads(k, cos, sin)
-        append_paged_kv(k, v, cache.k[layer], cache.v[layer], cache.table, cache.lens, count=counts)
+        if model.cfg.qk_norm:
+            q, k, v = blk.attn.normed_heads(blk.ln1(x), cache.rotary)
+        else:
+            q, k, v = blk.attn.heads(blk.ln1(x))
+            if cache.rotary is not None:
+                cos, sin = (t[:S] for t in cache.rotary)
+                q, k = rotate_heads(q, cos, sin), rotate_heads(k, cos, sin)
+        append_paged_kv(k, v, cache.k[layer], cache.v[layer], cache.table, cache.lens, count=counts, **cache.of(layer))
         y = blk.attn.attn_fn(q.contiguous(), k.contiguous(), v.contiguous(), causal=True, bias_max=model.cfg.bias_max)
         x = _mlp(blk, x + blk.attn.proj(y.transpose(1, 2).reshape(B, S, C)))
     if counts is None:
@@ -121,13 +152,17 @@ def _extend(model, cache, tokens, words=None, depths=None, counts=None):
     B, S, C = x.shape
     positions = None if depths is None else cache.lens[:, None] + depths
     for layer, blk in enumerate(model.blocks):
-        q, k, v = blk.attn.heads(blk.ln1(x))
-        where = (cache.k[layer], cache.v[layer], cache.table, cache.lens)
-        if cache.rotary is None:
-            append_paged_kv(k, v, *where, count=counts)
+        where, more = (cache.k[layer], cache.v[layer], cache.table, cache.lens), cache.of(layer)
+        if model.cfg.qk_norm:
+            q, k, v = blk.attn.normed_heads(blk.ln1(x), cache.rotary, cache.lens, positions)
+            append_paged_kv(k, v, *where, count=counts, **more)
         else:
-            q = append_paged_kv(k, v, *where, count=counts, q=q, rotary=cache.rotary, positions=positions)
-        y = paged_tree_attention(q, *where, tree_mask=words, bias_max=model.cfg.bias_max)
+            q, k, v = blk.attn.heads(blk.ln1(x))
+            if cache.rotary is None:
+                append_paged_kv(k, v, *where, count=counts, **more)
+            else:
+                q = append_paged_kv(k, v, *where, count=counts, q=q, rotary=cache.rotary, positions=positions, **more)
+        y = paged_tree_attention(q, *where, tree_mask=words, bias_max=model.cfg.bias_max, **more)
         x = _mlp(blk, x + blk.attn.proj(y.transpose(1, 2).reshape(B, S, C)))
     return x
 
@@ -137,12 +172,12 @@ def _noise(logits, generator):
 
 
 @torch.no_grad()
-def generate(model, prompts, max_new_tokens, counts=None, generator=None, page_size=64, **sampling):
-    """``max_new_tokens`` tokens for each prompt [B, S], [B, max_new_tokens].  ``sampling``:
-    temperature, top_k, top_p and min_p of ``sample_tokens``."""
+def generate(model, prompts, max_new_tokens, counts=None, generator=None, page_size=64, kv_dtype=None, **sampling):
+    """``max_new_tokens`` tokens for each prompt [B, S], [B, max_new_tokens].  ``kv_dtype`` as in
+    ``PagedCache``; ``sampling``: temperature, top_k, top_p and min_p of ``sample_tokens``."""
     if max_new_tokens <= 0:
         return torch.empty(prompts.shape[0], 0, dtype=torch.int64, device=prompts.device)
-    cache = PagedCache(model, prompts.shape[0], prompts.shape[1] + max_new_tokens, page_size, spare=0)
+    cache = PagedCache(model, prompts.shape[0], prompts.shape[1] + max_new_tokens, page_size, spare=0, kv_dtype=kv_dtype)
     logits = prefill(model, cache, prompts, counts)
     out = []
     for _ in range(max_new_tokens):
@@ -209,8 +244,6 @@ def tree_step(model, cache, last, drafts, parents, generator=None, **sampling):
         n += alive[:, 0].int()
     n.masked_fill_(missing[:, 0], 0)
     # the accepted rows move together behind the context; they are rotated already, by their depth
-    page, slot = cache.where(cache.lens[:, None] + path.int())
-    for k, v in zip(cache.k, cache.v):
-        append_paged_kv(*(x[page, :, slot].transpose(1, 2) for x in (k, v)), k, v, cache.table, cache.lens, count=n)
+    cache.move(cache.lens[:, None] + path.int(), n)
     cache.lens += n
     return tokens, n

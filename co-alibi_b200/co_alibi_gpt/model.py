@@ -27,6 +27,7 @@ class GPTConfig:
     bias_max: float = 8.0
     init_std: float = 0.02
     rotary_dim: int = 0  # first elements of each query and key head rotated by position (0: none); a multiple of 16
+    qk_norm: bool = False  # queries and keys normed per head (root mean square, learned weights) before the rotation
 
 
 def rotate_heads(x, cos, sin):
@@ -59,7 +60,7 @@ def _rotary(rotary_dim, seq_len, S, device):
 class CoALiBiSelfAttention(nn.Module):
     """QKV projection, Co-ALiBi causal attention over [B, H, S, D] heads, output projection."""
 
-    def __init__(self, cfg: GPTConfig, attn_fn):
+    def __init__(self, cfg: GPTConfig, attn_fn, heads_fn=None):
         super().__init__()
         assert cfg.d_model % cfg.n_head == 0
         self.n_head = cfg.n_head
@@ -68,6 +69,11 @@ class CoALiBiSelfAttention(nn.Module):
             raise ValueError(f"rotary_dim must be a multiple of 16 up to the head width {self.head_dim}, got {cfg.rotary_dim}")
         self.qkv = nn.Linear(cfg.d_model, 3 * cfg.d_model)
         self.proj = nn.Linear(cfg.d_model, cfg.d_model)
+        self.qk_norm = cfg.qk_norm
+        if cfg.qk_norm:
+            self.q_norm = nn.Parameter(torch.ones(self.head_dim))
+            self.k_norm = nn.Parameter(torch.ones(self.head_dim))
+        self.heads_fn = heads_fn
         self.attn_fn = attn_fn
         self.bias_max = cfg.bias_max
         self.rotary_dim = cfg.rotary_dim
@@ -79,22 +85,33 @@ class CoALiBiSelfAttention(nn.Module):
         qkv = self.qkv(x).view(B, S, 3, self.n_head, self.head_dim)
         return [t.transpose(1, 2) for t in qkv.unbind(dim=2)]
 
+    def normed_heads(self, x, rotary=None, start=None, positions=None):
+        """Queries, keys and values of x [B, S, C] as contiguous [B, H, S, D], queries and keys normed and
+        rotated: what ``heads`` gives where the model has ``qk_norm``."""
+        B, S, _ = x.shape
+        qkv = self.qkv(x).view(B, S, 3 * self.n_head, self.head_dim)
+        return self.heads_fn(qkv, self.n_head, self.n_head, self.q_norm, self.k_norm, rotary=rotary, start=start,
+                             positions=positions)
+
     def forward(self, x):
         B, S, C = x.shape
-        # contiguous: the kernels take row-major heads
-        q, k, v = (t.contiguous() for t in self.heads(x))
-        if self.rotary_dim:
-            cos, sin = _rotary(self.rotary_dim, self.seq_len, S, x.device)
-            q, k = rotate_heads(q, cos, sin), rotate_heads(k, cos, sin)
+        rotary = _rotary(self.rotary_dim, self.seq_len, S, x.device) if self.rotary_dim else None
+        if self.qk_norm:
+            q, k, v = self.normed_heads(x, rotary)
+        else:
+            # contiguous: the kernels take row-major heads
+            q, k, v = (t.contiguous() for t in self.heads(x))
+            if rotary is not None:
+                q, k = rotate_heads(q, *rotary), rotate_heads(k, *rotary)
         y = self.attn_fn(q, k, v, causal=True, bias_max=self.bias_max)
         return self.proj(y.transpose(1, 2).reshape(B, S, C))
 
 
 class Block(nn.Module):
-    def __init__(self, cfg: GPTConfig, attn_fn):
+    def __init__(self, cfg: GPTConfig, attn_fn, heads_fn=None):
         super().__init__()
         self.ln1 = nn.LayerNorm(cfg.d_model)
-        self.attn = CoALiBiSelfAttention(cfg, attn_fn)
+        self.attn = CoALiBiSelfAttention(cfg, attn_fn, heads_fn)
         self.ln2 = nn.LayerNorm(cfg.d_model)
         self.fc = nn.Linear(cfg.d_model, cfg.mlp_ratio * cfg.d_model)
         self.out = nn.Linear(cfg.mlp_ratio * cfg.d_model, cfg.d_model)
@@ -107,28 +124,32 @@ class Block(nn.Module):
 class CoALiBiGPT(nn.Module):
     """``forward(tokens, targets=None)`` -> logits, or the mean cross-entropy when
     targets are given.  ``attn_fn(q, k, v, causal, bias_max)`` defaults to the
-    package's ``co_alibi_attention`` (CUDA only; no other attention is used)."""
+    package's ``co_alibi_attention`` (CUDA only; no other attention is used), and with
+    ``qk_norm`` ``heads_fn`` to its ``norm_rotate_qkv``."""
 
-    def __init__(self, cfg: GPTConfig, attn_fn=None):
+    def __init__(self, cfg: GPTConfig, attn_fn=None, heads_fn=None):
         super().__init__()
         if attn_fn is None:
             from co_alibi_attn import co_alibi_attention
             attn_fn = co_alibi_attention
+        if cfg.qk_norm and heads_fn is None:
+            from co_alibi_attn import norm_rotate_qkv
+            heads_fn = norm_rotate_qkv
         self.cfg = cfg
         self.emb = nn.Embedding(cfg.vocab, cfg.d_model)
-        self.blocks = nn.ModuleList(Block(cfg, attn_fn) for _ in range(cfg.n_layer))
+        self.blocks = nn.ModuleList(Block(cfg, attn_fn, heads_fn) for _ in range(cfg.n_layer))
         self.ln_f = nn.LayerNorm(cfg.d_model)
         self.reset_parameters()
 
     def reset_parameters(self, generator=None):
         """Weights ~ N(0, init_std) (residual output projections scaled by
-        1/sqrt(2 n_layer)), biases 0, LayerNorm affine 1 / 0."""
+        1/sqrt(2 n_layer)), biases 0, LayerNorm affine 1 / 0, the heads' norms 1."""
         std = self.cfg.init_std
         with torch.no_grad():
             for name, p in self.named_parameters():
                 if name.endswith("bias"):
                     p.zero_()
-                elif ".ln" in name or name.startswith("ln_f"):
+                elif ".ln" in name or name.startswith("ln_f") or name.endswith(("q_norm", "k_norm")):
                     p.fill_(1.0)
                 else:
                     s = std / math.sqrt(2 * self.cfg.n_layer) if name.endswith(("proj.weight", "out.weight")) else std

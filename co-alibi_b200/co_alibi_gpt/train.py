@@ -17,12 +17,12 @@ def make_tokens(cfg: GPTConfig, batch: int, seed: int, device=None):
     return t if device is None else t.to(device)
 
 
-def build(cfg: GPTConfig, device, seed=0, dtype=torch.bfloat16, ddp=False, lr=3e-4, attn_fn=None):
+def build(cfg: GPTConfig, device, seed=0, dtype=torch.bfloat16, ddp=False, lr=3e-4, attn_fn=None, heads_fn=None):
     """Model (weights N(0, 0.02) from ``seed``, cast to ``dtype``), optionally
     wrapped in DistributedDataParallel, and its AdamW optimizer.  ``attn_fn``
-    defaults to ``co_alibi_attention``."""
+    defaults to ``co_alibi_attention``, ``heads_fn`` (with ``qk_norm``) to ``norm_rotate_qkv``."""
     device = torch.device(device)
-    model = CoALiBiGPT(cfg, attn_fn)
+    model = CoALiBiGPT(cfg, attn_fn, heads_fn)
     model.reset_parameters(torch.Generator().manual_seed(seed))
     model = model.to(device=device, dtype=dtype)
     if ddp:

@@ -440,6 +440,12 @@ __device__ __forceinline__ float lg2_approx(float x) {
   return y;
 }
 
+// Pairs in scalar arithmetic: packed instructions want both halves in neighbouring registers, and the moves
+// that puts them there cost more than the issue slots they save.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return make_float2(a.x * b.x, a.y * b.y); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); }
+
 template <int D, bool BF16, int NT, int RW, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::CTAS))
     coalibi_paged8_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -709,11 +715,11 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float2 s[4];
-          const float2 f = __fmul2_rn(unit[n], make_float2(k_scale, k_scale));
+          const float2 f = mul2(unit[n], make_float2(k_scale, k_scale));
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            v[n][c] = __fmul2_rn(make_float2(sc[c >> 1][n][2 * (c & 1)], sc[c >> 1][n][2 * (c & 1) + 1]), f);
-            const float2 e = __fadd2_rn(make_float2(ex2_approx(-v[n][c].x), ex2_approx(-v[n][c].y)), make_float2(1.f, 1.f));
+            v[n][c] = mul2(make_float2(sc[c >> 1][n][2 * (c & 1)], sc[c >> 1][n][2 * (c & 1) + 1]), f);
+            const float2 e = add2(make_float2(ex2_approx(-v[n][c].x), ex2_approx(-v[n][c].y)), make_float2(1.f, 1.f));
             s[c] = make_float2(rcp_approx(e.x), rcp_approx(e.y));
             if (MASKED) {
               s[c].x = vis >> (8 * n + c) & 1 ? s[c].x : 0.f;
@@ -721,26 +727,26 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
             }
           }
           // sums of the tiles c and after it; tiles c >= 4 - turn hold the lane's first keys
-          s[2] = __fadd2_rn(s[2], s[3]);
-          s[1] = __fadd2_rn(s[1], s[2]);
-          s[0] = __fadd2_rn(s[0], s[1]);
+          s[2] = add2(s[2], s[3]);
+          s[1] = add2(s[1], s[2]);
+          s[0] = add2(s[0], s[1]);
           float2 inc = s[0];
 #pragma unroll
           for (int d = 4; d <= 16; d <<= 1) {
             const float2 y = make_float2(__shfl_down_sync(0xffffffffu, inc.x, d), __shfl_down_sync(0xffffffffu, inc.y, d));
-            if (lane + d < 32) inc = __fadd2_rn(inc, y);
+            if (lane + d < 32) inc = add2(inc, y);
           }
           const float2 wrapped = turn == 0 ? make_float2(0.f, 0.f) : turn == 1 ? s[3] : turn == 2 ? s[2] : s[1];
           const float2 right = make_float2(inc.x - s[0].x, inc.y - s[0].y);
           const float2 last = make_float2(carry[n].x + (right.x - wrapped.x), carry[n].y + (right.y - wrapped.y));
-          const float2 first = __fadd2_rn(last, s[0]);
+          const float2 first = add2(last, s[0]);
           carry[n].x += __shfl_sync(0xffffffffu, inc.x, tig);
           carry[n].y += __shfl_sync(0xffffffffu, inc.y, tig);
           mx[n] = make_float2(-INFINITY, -INFINITY);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const float2 z = __fadd2_rn(c + turn >= 4 ? first : last, s[c]);
-            v[n][c] = __ffma2_rn(make_float2(-slope2[n].x, -slope2[n].y), z, v[n][c]);
+            const float2 z = add2(c + turn >= 4 ? first : last, s[c]);
+            v[n][c] = fma2(make_float2(-slope2[n].x, -slope2[n].y), z, v[n][c]);
             if (MASKED) {
               v[n][c].x = vis >> (8 * n + c) & 1 ? v[n][c].x : -INFINITY;
               v[n][c].y = vis >> (8 * n + 4 + c) & 1 ? v[n][c].y : -INFINITY;
@@ -786,18 +792,18 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
           float2 l2 = make_float2(0.f, 0.f);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const float2 x = __fadd2_rn(v[n][c], off2);
+            const float2 x = add2(v[n][c], off2);
             float2 w = make_float2(ex2_approx(x.x), ex2_approx(x.y));
             if (MASKED) {  // (a block that nothing of is seen may have any scale)
               w.x = vis >> (8 * n + c) & 1 ? w.x : 0.f;
               w.y = vis >> (8 * n + 4 + c) & 1 ? w.y : 0.f;
             }
-            l2 = __fadd2_rn(l2, w);
+            l2 = add2(l2, w);
             pb[n][c] = pack2<false>(w.x, w.y);
           }
           // the weights themselves: without the block's scale
           if (MASKED && l2.x == 0.f && l2.y == 0.f) continue;
-          l_part[n] = __ffma2_rn(l2, make_float2(iv, iv), l_part[n]);
+          l_part[n] = fma2(l2, make_float2(iv, iv), l_part[n]);
         }
       };
       if (all)
