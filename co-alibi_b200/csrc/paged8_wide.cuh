@@ -1,0 +1,665 @@
+// Attention over a paged cache in 8 bits for many rows per kv head (drafted trees): tcgen05.
+//
+// As the 16-bit cache's kernel for such rows (paged.cuh): 64 or 128 rows are the 128 lanes of TMEM, one row to a
+// thread; two groups of four softmax warps work on keys of their own, 64 to a step; with at most 64 rows
+// (DUP) the rows stand twice, and the two halves of the lanes take the halves of a step, which come from two
+// separate pieces of the item.  The tensor cores take the codes as float16, which holds them exactly, so each group has two
+// warps that turn the codes of a step, as they arrive by TMA, into the swizzled tiles that the MMA reads; K's tile
+// of the step after the next one is made as soon as the scores are out, V's as soon as its product is.
+// Scales enter the scores and the exponents of the weights as in the kernel for few rows (paged8.cuh).
+#pragma once
+
+#include "paged8.cuh"
+
+namespace coalibi {
+
+template <int D, bool DUP>
+struct Wide8Layout {
+  static constexpr int PIECES = DUP ? 4 : 2;       // of an item, per CTA
+  static constexpr int STEP = DUP ? 32 : 64;       // keys of a piece per step
+  static constexpr int UNIT = 128;
+  static constexpr int COST = 10;                  // of starting and finishing an item, in units
+  static constexpr int WHOLE = 1024;               // keys of a table that is not split
+  static constexpr int ROWS = DUP ? 64 : 128;
+  static constexpr int TILE = 64 * D * 2;          // K or V of a step in float16: [D / 64][64 keys][128 bytes]
+  static constexpr int BOX = 64 * 128;
+  static constexpr int CODES = 64 * D;             // K or V of a step as codes: [64 keys][D], swizzled
+  static constexpr int NCODE = 2, NTILE = 2;       // rings of steps
+  static constexpr int GROUP = NTILE * 2 * TILE + NCODE * 2 * CODES;
+  static constexpr int QBYTES = 128 * D * 2;       // [D / 64][128 rows][128 bytes]
+  static constexpr int BYTES = QBYTES + 2 * GROUP + 1024;
+  static constexpr int CTAS = 1;
+  static constexpr int RECORD = ROWS * (4 + D);
+  static constexpr int TM_S = 64, TM_O = 256;      // columns of an S buffer; O of group w at TM_O + w * D
+  static constexpr int THREADS = 512;              // warps 0-7 softmax, 8 and 9 MMAs, 10 and 11 loads, 12-15 tiles
+  // a group's part of the exchange (O in float, then statistics) reuses its rings
+  static_assert(128 * D * 4 + 128 * 16 <= GROUP, "exchange fits the rings");
+};
+
+// Steps whose scales are kept: those of step n are written when K of step n - 2 is a tile, so the scores of step n - 4
+// are out and the softmax warps past step n - 6.
+constexpr int kWide8Meta = 6;
+
+template <int D, bool BF16, bool DUP>
+__global__ void __launch_bounds__(512, 1)
+    coalibi_paged8_wide_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                               const Paged8Params p) {
+  using L = Wide8Layout<D, DUP>;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ uint64_t s_kc[2][2], s_kc_free[2][2], s_vc[2][2], s_vc_free[2][2];  // codes
+  __shared__ uint64_t s_k[2][2], s_k_free[2][2], s_v[2][2], s_v_free[2][2];      // tiles
+  __shared__ uint64_t s_scores[2][2], s_probs[2][2], s_meta[2][4], s_pv[2][2], s_idle[2];
+  // of a step: the scales of its four blocks of 16 keys; which of them were not loaded (bits 0-3), and 16 where some
+  // key of the step is not of the context
+  __shared__ __align__(16) float s_ks[2][kWide8Meta][4];
+  __shared__ __align__(16) float s_vs[2][kWide8Meta][4];
+  __shared__ unsigned char s_gone[2][kWide8Meta];
+  __shared__ __align__(16) union {
+    int pre[128];
+    uint32_t nan[kTreeMaxSq][4];  // columns of a drafted token's V that are NaN
+  } s_u;
+  __shared__ int s_any_nan;
+  __shared__ signed char s_up[128];  // exponents of the powers of two by which the queries' rows are scaled
+  __shared__ int s_warp[4], s_find, s_abort;
+  __shared__ uint32_t s_tmem;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool softmax = warp < 8, issues = warp == 8 || warp == 9, loads = warp == 10 || warp == 11;
+  const int w = softmax ? warp >> 2 : warp < 12 ? warp & 1 : (warp - 12) >> 1;  // group
+  const int G = p.Hq / p.Hkv, rows = G * p.Sq;
+  const int heads = p.Hkv * p.row_blocks;
+  const CtaGuard guard{&s_abort, p.status, kPagedTimeoutNs};
+  if (tid == 0) {
+    for (int g = 0; g < 2; ++g) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_kc[g][i], 1);
+        mbar_init(&s_kc_free[g][i], 64);
+        mbar_init(&s_vc[g][i], 1);
+        mbar_init(&s_vc_free[g][i], 64);
+        mbar_init(&s_k[g][i], 64);
+        mbar_init(&s_k_free[g][i], 1);
+        mbar_init(&s_v[g][i], 64);
+        mbar_init(&s_v_free[g][i], 1);
+        mbar_init(&s_scores[g][i], 1);
+        mbar_init(&s_probs[g][i], 4);
+        mbar_init(&s_pv[g][i], 1);
+      }
+      for (int i = 0; i < 4; ++i) mbar_init(&s_meta[g][i], 1);
+      mbar_init(&s_idle[g], 1);
+    }
+    s_abort = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
+  if (warp == 8) {
+    tmem_alloc(&s_tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  grid_dep_wait();
+
+  unsigned at = 0, stop;
+  int b = 0, span = 1, item = 0, v0 = 0;
+  if (p.whole) {
+    b = blockIdx.x / heads;
+    item = blockIdx.x - b * heads;
+    span = paged_span<L>(p, b);
+    stop = span;
+  } else {
+    int* head = reinterpret_cast<int*>(p.ws);
+    const int per = (p.B + 127) / 128;
+    const unsigned total = (unsigned)paged_prefix<L>(p, s_u.pre, s_warp, per, blockIdx.x == 0 ? head : nullptr) * heads;
+    const unsigned quota = (total + p.n_ctas - 1) / p.n_ctas;
+    if (blockIdx.x == 0 && tid == 0) head[p.B + 1] = (int)quota;
+    at = quota * blockIdx.x;
+    stop = min(total, at + quota);
+    if (at < stop) paged_find<L>(p, s_u.pre, &s_find, per, heads, at, b, span, item, v0);
+    __syncthreads();  // s_u is used otherwise from here on
+  }
+
+  uint8_t* const rings = smem + L::QBYTES + w * L::GROUP;
+  uint8_t* const k_tiles = rings;
+  uint8_t* const v_tiles = rings + L::NTILE * L::TILE;
+  uint8_t* const codes = rings + 2 * L::NTILE * L::TILE;  // [slot][K, V]
+  uint32_t seq = 0;  // steps of this group in earlier items: the barriers' phases go on
+  bool ok = true;
+  while (at < stop) {
+    const int v1 = (int)min((unsigned)span, v0 + (stop - at));
+    const int u0 = max(v0 - L::COST, 0), u1 = v1 - L::COST, units = span - L::COST;
+    if (u1 <= 0) break;
+    const int g = item / p.row_blocks, rb = (item - g * p.row_blocks) * L::ROWS;
+    const int len = p.ctx_lens[b], room = p.max_pages * p.page_size, ctx = min(max(len, 0), room);
+    unsigned long long seen_by_any = 0;
+    if (p.tree_mask == nullptr) {
+      seen_by_any = (2ull << (p.Sq - 1)) - 1;
+    } else {
+      for (int i = lane; i < p.Sq; i += 32) seen_by_any |= (unsigned long long)p.tree_mask[b * p.mask_stride + i];
+#pragma unroll
+      for (int d = 16; d; d >>= 1) seen_by_any |= __shfl_xor_sync(0xffffffffu, seen_by_any, d);
+      if (p.Sq < 64) seen_by_any &= (1ull << p.Sq) - 1;
+    }
+    const int drafts = 64 - __clzll((long long)seen_by_any);
+    if ((len > room || ctx + drafts > room) && tid == 0) report_page(p.status);
+    // the pieces: `sub` keys each, the group's first at piece PIECES / 2 * w
+    const int s_lo = u0 * L::UNIT, s_hi = min(min(u1 * L::UNIT, room), ctx + drafts);
+    const int sub = ((max(s_hi - s_lo, 0) + L::PIECES - 1) / L::PIECES + 15) & ~15;
+    auto piece_lo = [&](int q) { return s_lo + q * sub; };
+    auto piece_hi = [&](int q) { return min(s_hi, s_lo + (q + 1) * sub); };
+    auto piece_steps = [&](int q) { return max(0, (piece_hi(q) - piece_lo(q) + L::STEP - 1) / L::STEP); };
+    const int q0 = L::PIECES / 2 * w;
+    const int nsteps = DUP ? max(piece_steps(q0), piece_steps(q0 + 1)) : piece_steps(q0);
+    // first key of half hf of step n (counted from the right); its piece's ends
+    auto half_base = [&](int n, int hf) {
+      if (DUP) return piece_lo(q0 + hf) + (piece_steps(q0 + hf) - 1 - n) * 32;
+      return piece_lo(q0) + (nsteps - 1 - n) * 64 + 32 * hf;
+    };
+    auto half_hi = [&](int hf) { return piece_hi(DUP ? q0 + hf : q0); };
+    auto half_lo = [&](int hf) { return piece_lo(DUP ? q0 + hf : q0); };
+
+    // ---- loads: step n of the group, by one warp; lane i < 4 looks up the step's block i
+    int k_loaded = 0, v_loaded = 0;
+    auto load = [&](int n) {
+      const uint32_t k = seq + n;
+      const int slot = k % L::NCODE, meta = k % kWide8Meta;
+      int page = -1, at_slot = 0;
+      bool inside = true;  // all keys of the block's half are of the context
+      if (lane < 4) {
+        const int base = half_base(n, lane >> 1), key = base + 16 * (lane & 1);
+        inside = base + 32 <= min(half_hi(lane >> 1), ctx);
+        if (key >= half_lo(lane >> 1) && key < half_hi(lane >> 1)) {
+          const int t = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+          page = p.page_table[(size_t)b * p.table_stride + t];
+          at_slot = key - t * p.page_size;
+          if ((unsigned)page >= (unsigned)p.n_pages) {
+            page = -1;
+            report_page(p.status);
+          }
+        }
+      }
+      float ks = 1.f, vs = 1.f;
+      if (page >= 0) {
+        ks = p.k_scales[page * p.kss[0] + g * p.kss[1] + at_slot / kQuantBlock];
+        vs = p.v_scales[page * p.vss[0] + g * p.vss[1] + at_slot / kQuantBlock];
+      }
+      const int gone = (int)(__ballot_sync(0xffffffffu, lane < 4 && page < 0) & 15u);
+      const bool plain = gone == 0 && __all_sync(0xffffffffu, inside);
+      const uint32_t dst = smem_u32(codes + slot * 2 * L::CODES), bytes = (4 - __popc(gone)) * 16 * D;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_kc_free[w][slot], ((k / L::NCODE) & 1) ^ 1, guard))) return false;
+      if (lane == 0) mbar_expect_tx(&s_kc[w][slot], bytes);
+      __syncwarp();
+      if (page >= 0) tma_load_4d(dst + lane * 16 * D, &tk, &s_kc[w][slot], 0, at_slot, g, page);
+      if (lane < 4) s_ks[w][meta][lane] = ks, s_vs[w][meta][lane] = vs;
+      if (lane == 0) s_gone[w][meta] = (unsigned char)(plain ? 0 : gone | 16);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_kc[w][slot]);  // (the scales are in, too)
+      ++k_loaded;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_vc_free[w][slot], ((k / L::NCODE) & 1) ^ 1, guard))) return false;
+      if (lane == 0) mbar_arrive_expect_tx(&s_vc[w][slot], bytes);
+      __syncwarp();
+      if (page >= 0) tma_load_4d(dst + L::CODES + lane * 16 * D, &tv, &s_vc[w][slot], 0, at_slot, g, page);
+      ++v_loaded;
+      return true;
+    };
+    const int ahead = min(nsteps, L::NCODE);  // the rings are free: these start beside the queries
+    if (loads)
+      for (int n = 0; n < ahead && ok; ++n) ok = load(n);
+    if (softmax) {
+      // ---- the queries, in the K-major 128-byte-swizzled form the MMA reads; bfloat16 ones as float16, scaled by
+      // a power of two that puts a row's largest at 2^14
+      for (int c = tid; c < 128 * (D / 8); c += 256) {
+        const int r = c / (D / 8), ch = c % (D / 8), row = rb + (DUP ? r & 63 : r);
+        uint4 val = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows)
+          val = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + b * p.qs[0] +
+                                                (g * G + row / p.Sq) * p.qs[1] + (row % p.Sq) * p.qs[2] + ch * 8);
+        if (BF16) {
+          uint32_t x[4] = {val.x, val.y, val.z, val.w}, most = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) most = max(most, max(x[e] << 16 & 0x7f800000u, x[e] & 0x7f800000u));
+#pragma unroll
+          for (int d = 1; d < D / 8; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+          const int up = 14 - min(max((int)(most >> 23) - 127, -100), 127);
+          const float by = __int_as_float((up + 127) << 23);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = unpack2<true>(x[e]);
+            x[e] = pack2<false>(f.x * by, f.y * by);
+          }
+          val = make_uint4(x[0], x[1], x[2], x[3]);
+          if (ch == 0) s_up[r] = (signed char)up;
+        }
+        *reinterpret_cast<uint4*>(smem + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = val;
+      }
+      if (tid < kTreeMaxSq) *reinterpret_cast<uint4*>(s_u.nan[tid]) = make_uint4(0u, 0u, 0u, 0u);
+      if (tid == 0) s_any_nan = 0;
+      fence_async_smem();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+
+    if (loads) {
+      for (int n = ahead; n < nsteps && ok; ++n) ok = load(n);
+      // every issued copy lands before the item (and the CTA) ends
+      if (lane == 0)
+        for (int n = 0; n < L::NCODE; ++n) {
+          const uint32_t kk = seq + k_loaded - 1 - n, kv = seq + v_loaded - 1 - n;
+          if (n < k_loaded) mbar_drain(&s_kc[w][kk % L::NCODE], (kk / L::NCODE) & 1, guard.timeout_ns);
+          if (n < v_loaded) mbar_drain(&s_vc[w][kv % L::NCODE], (kv / L::NCODE) & 1, guard.timeout_ns);
+        }
+      __syncwarp();
+    } else if (warp >= 12) {
+      // ---------------------------------------------------------- codes to tiles
+      const int t = (warp - 12 & 1) * 32 + lane;  // of the group's 64 threads
+      constexpr int CH = D / 16;                  // 16-code chunks of a row: a thread takes one, and 512 / 8 or 64 / 4 keys apart
+      const int c = t % CH;
+      // chunk c of key `key` as float16; `zero`: nothing of the row may be used; nan: columns of NaN, taken out
+      auto turn = [&](const uint8_t* from, uint8_t* to, int key, bool zero, bool takes_nan, uint32_t& nan) {
+        const uint32_t phase = D == 128 ? key & 7 : key >> 1 & 3;
+        const uint4 u = *reinterpret_cast<const uint4*>(from + key * D + ((c ^ phase) << 4));
+        uint32_t x[4] = {u.x, u.y, u.z, u.w};
+        if (zero) x[0] = x[1] = x[2] = x[3] = 0u;
+        if (takes_nan) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t bad = __vcmpeq4(x[j] & 0x7f7f7f7fu, 0x7f7f7f7fu);  // a byte of ones each
+            x[j] &= ~bad;
+            nan |= ((bad & 1u) | (bad >> 7 & 2u) | (bad >> 14 & 4u) | (bad >> 21 & 8u)) << (4 * j);
+          }
+        }
+        uint32_t h[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e4m3_to_f16x4(x[j], h[2 * j], h[2 * j + 1]);
+        uint8_t* row = to + (D == 128 ? (c >> 2) * L::BOX : 0) + key * 128;
+        const int c0 = 2 * c & 7;
+        // (the two halves of a row of 128 columns store their pieces in opposite order, so that the eight lanes of
+        // a row hit all phases of the swizzle)
+        const bool swap = D == 128 && c >= 4;
+        const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
+        *reinterpret_cast<uint4*>(row + (((c0 + swap) ^ (key & 7)) << 4)) = swap ? hi : lo;
+        *reinterpret_cast<uint4*>(row + (((c0 + !swap) ^ (key & 7)) << 4)) = swap ? lo : hi;
+      };
+      auto make_k = [&](int n) {
+        const uint32_t k = seq + n;
+        const int slot = k % L::NCODE, tile = k % L::NTILE;
+        ok = mbar_wait(&s_kc[w][slot], (k / L::NCODE) & 1, guard) && mbar_wait(&s_k_free[w][tile], ((k / L::NTILE) & 1) ^ 1, guard);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        if (t == 0) mbar_arrive(&s_meta[w][k & 3]);  // the scales, to the softmax warps
+        uint32_t none = 0;
+#pragma unroll 4
+        for (int key = t / CH; key < 64; key += 64 / CH)
+          turn(codes + slot * 2 * L::CODES, k_tiles + tile * L::TILE, key, false, false, none);
+        fence_async_smem();
+        mbar_arrive(&s_k[w][tile]);
+        mbar_arrive(&s_kc_free[w][slot]);
+      };
+      auto make_v = [&](int n) {
+        const uint32_t k = seq + n;
+        const int slot = k % L::NCODE, tile = k % L::NTILE;
+        ok = mbar_wait(&s_vc[w][slot], (k / L::NCODE) & 1, guard) && mbar_wait(&s_v_free[w][tile], ((k / L::NTILE) & 1) ^ 1, guard);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        const uint8_t* from = codes + slot * 2 * L::CODES + L::CODES;
+        uint8_t* to = v_tiles + tile * L::TILE;
+        const int gone = s_gone[w][k % kWide8Meta];
+        if (gone == 0) {
+          uint32_t none = 0;
+#pragma unroll 4
+          for (int key = t / CH; key < 64; key += 64 / CH) turn(from, to, key, false, false, none);
+        } else {
+          // V rows that no row sees (past the end, of no page, unseen drafts) may hold any code: zeros, 0 * NaN
+          // is not 0.  What is NaN of a drafted token must not reach the rows that do not see it: zeros too, and
+          // the rows that do get their NaN at the end.
+#pragma unroll 1
+          for (int key = t / CH; key < 64; key += 64 / CH) {
+            const int hf = key >> 5, base = half_base(n, hf), pos = base + (key & 31);
+            const bool used = base >= half_lo(hf) && !(gone >> (key >> 4) & 1) && pos < half_hi(hf) &&
+                              (pos < ctx || (seen_by_any >> (pos - ctx) & 1));
+            uint32_t nan = 0;
+            turn(from, to, key, !used, used && pos >= ctx, nan);
+            if (nan != 0) {
+              atomicOr(&s_u.nan[pos - ctx][c >> 1], nan << (16 * (c & 1)));
+              s_any_nan = 1;
+            }
+          }
+        }
+        fence_async_smem();
+        mbar_arrive(&s_v[w][tile]);
+        mbar_arrive(&s_vc_free[w][slot]);
+      };
+      // K(0), K(1), V(0), K(2), V(1), ...: K's tile is free once the scores before the last are out
+      if (nsteps > 0 && ok) make_k(0);
+      for (int n = 0; n < nsteps && ok; ++n) {
+        if (n + 1 < nsteps) make_k(n + 1);
+        if (ok) make_v(n);
+      }
+    } else if (issues) {
+      // ---------------------------------------------------------- MMAs (lane 0 issues)
+      constexpr uint32_t idS = make_idesc_f16(false, 128, 64, false, false);
+      constexpr uint32_t idPV = make_idesc_f16(false, 128, D, false, true);
+      const uint32_t q_addr = smem_u32(smem), k_addr0 = smem_u32(k_tiles), v_addr0 = smem_u32(v_tiles);
+      auto issue_scores = [&](int n) {
+        const uint32_t k = seq + n;
+        const int tile = k % L::NTILE;
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_k[w][tile], (k / L::NTILE) & 1, guard))) return false;
+        if (lane == 0) {
+          tc_fence_after();
+          const uint32_t d = tmem + (2 * w + (k & 1)) * L::TM_S, k_addr = k_addr0 + tile * L::TILE;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_ss(d, make_sdesc_sw128(q_addr + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024),
+                    make_sdesc_sw128(k_addr + (kk >> 2) * L::BOX + (kk & 3) * 32, 16, 1024), idS, kk > 0 ? 1u : 0u);
+          umma_commit(&s_scores[w][k & 1]);
+          umma_commit(&s_k_free[w][tile]);
+        }
+        __syncwarp();
+        return true;
+      };
+      // S(0), S(1), PV(0), S(2), PV(1), ...: S(n + 2) overwrites the buffer that PV(n), issued
+      // before it by this thread, has read P from
+      for (int n = 0; n < 2 && n < nsteps && ok; ++n) ok = issue_scores(n);
+      for (int n = 0; n < nsteps && ok; ++n) {
+        const uint32_t k = seq + n;
+        const int tile = k % L::NTILE;
+        ok = mbar_wait(&s_probs[w][k & 1], (k >> 1) & 1, guard) && mbar_wait(&s_v[w][tile], (k / L::NTILE) & 1, guard);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        if (lane == 0) {
+          tc_fence_after();
+          const uint32_t pa = tmem + (2 * w + (k & 1)) * L::TM_S, v_addr = v_addr0 + tile * L::TILE;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_ts(tmem + L::TM_O + w * D, pa + kk * 8, make_sdesc_sw128(v_addr + kk * 16 * 128, L::BOX, 1024), idPV,
+                    n > 0 || kk > 0 ? 1u : 0u);
+          umma_commit(&s_pv[w][k & 1]);
+          umma_commit(&s_v_free[w][tile]);
+        }
+        __syncwarp();
+        if (n + 2 < nsteps) ok = issue_scores(n + 2);
+      }
+      if (!ok && lane == 0) {  // what was issued must have finished before TMEM is released
+        umma_commit(&s_idle[w]);
+        mbar_drain(&s_idle[w], 0, guard.timeout_ns);
+      }
+      __syncwarp();
+    } else {
+      // ---------------------------------------------------------- softmax: one row to a thread
+      const int t = (warp & 3) * 32 + lane, r = DUP ? t & 63 : t, my_half = t >> 6;
+      const bool rok = rb + r < rows;
+      const float slope2 = load_slope(p.slopes, p.slopes_dtype, g * G + (rok ? rb + r : rb) / p.Sq) * kLog2e;
+      const float c_a = p.sm_scale * kLog2e * (BF16 ? __int_as_float((127 - s_up[t]) << 23) : 1.f);
+      const int row_of = (rok ? rb + r : rb) % p.Sq;
+      const unsigned long long word =
+          p.tree_mask != nullptr ? (unsigned long long)p.tree_mask[b * p.mask_stride + row_of] : (2ull << row_of) - 1;
+      const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+      const uint32_t o_base = lane_base + L::TM_O + w * D;
+      float m = -INFINITY, l = 0.f, carry = 0.f;
+      bool left = false;
+      for (int n = 0; n < nsteps; ++n) {
+        const uint32_t k = seq + n;
+        const int meta = k % kWide8Meta;
+        const uint32_t s_base = lane_base + (2 * w + (k & 1)) * L::TM_S;
+        if (ok) ok = mbar_wait(&s_meta[w][k & 3], (k >> 2) & 1, guard);
+        if (ok) ok = mbar_wait(&s_scores[w][k & 1], (k >> 1) & 1, guard);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          left = true;
+          break;
+        }
+        const int gone = s_gone[w][meta];
+        const bool plain = gone == 0;
+        uint32_t pk[DUP ? 1 : 2][16];
+        float alpha = 1.f;
+        bool rescale = false;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < (DUP ? 1 : 2); ++x) {  // (the right half first)
+          const int hf = DUP ? my_half : 1 - x;
+          uint32_t s[32];
+          __syncwarp();  // (the loads and stores of TMEM take converged warps)
+          tmem_ld32_sync(s_base + 32 * hf, s);
+          uint32_t seen = 0xffffffffu;
+          if (!plain) {
+            const int base = half_base(n, hf), in = min(half_hi(hf), ctx) - base, end = half_hi(hf) - base;
+            const uint32_t context = in >= 32 ? 0xffffffffu : in > 0 ? (1u << in) - 1u : 0u;
+            uint32_t v = context;
+            if (end > in && end > 0) {  // drafted tokens, up to `end`
+              const int d = base - ctx;
+              const uint32_t bits = d >= 0 ? (d < 64 ? (uint32_t)(word >> d) : 0u) : d > -32 ? (uint32_t)word << -d : 0u;
+              v |= bits & (end >= 32 ? 0xffffffffu : (1u << end) - 1u) & ~context;
+            }
+            if (base < half_lo(hf)) v = 0u;  // this piece has ended
+            if (gone >> (2 * hf) & 1) v &= 0xffff0000u;
+            if (gone >> (2 * hf + 1) & 1) v &= 0x0000ffffu;
+            seen = v;
+          }
+          // of the half's two blocks
+          const float2 ks = *reinterpret_cast<const float2*>(&s_ks[w][meta][2 * hf]);
+          const float2 vs = *reinterpret_cast<const float2*>(&s_vs[w][meta][2 * hf]);
+          const float f0 = c_a * ks.x, f1 = c_a * ks.y, lv0 = lg2_approx(vs.x), lv1 = lg2_approx(vs.y);
+          auto scan = [&](auto masked) {
+            constexpr bool MASKED = decltype(masked)::value;
+            // sub-chunks of 8 keys: short chains of additions that overlap
+            float tot[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float run = 0.f;
+              const float f = c < 2 ? f0 : f1;
+#pragma unroll
+              for (int j = 7; j >= 0; --j) {
+                const int e = 8 * c + j;
+                const float y = __uint_as_float(s[e]) * f;
+                float sg = rcp_approx(ex2_approx(-y) + 1.f);
+                if (MASKED) sg = seen >> e & 1 ? sg : 0.f;
+                run += sg;
+                s[e] = __float_as_uint(fmaf(-slope2, run, y));
+              }
+              tot[c] = run;
+            }
+            // sums right of each sub-chunk shift its logits
+            float off[4];
+            off[3] = carry;
+            off[2] = off[3] + tot[3];
+            off[1] = off[2] + tot[2];
+            off[0] = off[1] + tot[1];
+            carry = off[0] + tot[0];
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float sh = -slope2 * off[c];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int e = 8 * c + j;
+                float v = __uint_as_float(s[e]) + sh;
+                if (MASKED) v = seen >> e & 1 ? v : -INFINITY;
+                s[e] = __float_as_uint(v);
+                mx[c >> 1] = fmaxf(mx[c >> 1], v);
+              }
+            }
+            return fmaxf(mx[0] + lv0, mx[1] + lv1);
+          };
+          const float mx = plain ? scan(std::false_type{}) : scan(std::true_type{});
+          // the reference moves only when a contribution passes it by 2^8: weights stay below 256, and
+          // O needs rescaling rarely
+          if (mx > m + 8.f || (m == -INFINITY && mx > -INFINITY)) {
+            const float f = m == -INFINITY ? 0.f : ex2_approx(m - mx);
+            if (m != -INFINITY) {
+              rescale = true;
+              alpha *= f;
+              if (!DUP && x == 1) {  // the right half's weights of this step move too
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  const float2 u = unpack2<false>(pk[0][j]);
+                  pk[0][j] = pack2<false>(u.x * f, u.y * f);
+                }
+              }
+            }
+            l *= f;
+            m = mx;
+          }
+          const float m_use = m == -INFINITY ? 0.f : m;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const float sh = (q ? lv1 : lv0) - m_use;
+            float ls = 0.f;
+#pragma unroll
+            for (int j = 8 * q; j < 8 * q + 8; ++j) {
+              float e0 = ex2_approx(__uint_as_float(s[2 * j]) + sh), e1 = ex2_approx(__uint_as_float(s[2 * j + 1]) + sh);
+              if (!plain) {  // (a block that nothing of is seen may have any scale)
+                e0 = seen >> (2 * j) & 1 ? e0 : 0.f;
+                e1 = seen >> (2 * j + 1) & 1 ? e1 : 0.f;
+              }
+              ls += e0 + e1;
+              pk[DUP ? 0 : x][j] = pack2<false>(e0, e1);
+            }
+            // the weights themselves: without the block's scale
+            if (plain || (seen >> (16 * q) & 0xffffu) != 0) l = fmaf(ls, rcp_approx(q ? vs.y : vs.x), l);
+          }
+        }
+        if (__any_sync(0xffffffffu, rescale)) {
+          // every PV before this step's must have added its part
+          if (n > 0) ok = mbar_wait(&s_pv[w][(k - 1) & 1], ((k - 1) >> 1) & 1, guard);
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok && n > 0) {
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32_sync(o_base + c, o);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+              tmem_st32(o_base + c, o);
+            }
+          }
+        }
+        // ---- P over this step's scores
+        if (!ok) {
+          left = true;
+          break;
+        }
+        __syncwarp();
+        if (DUP) {
+          const uint32_t none[16] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+          tmem_st16(s_base + 16 * my_half, pk[0]);
+          tmem_st16(s_base + 16 * (1 - my_half), none);
+        } else {
+          tmem_st16(s_base + 16, pk[0]);
+          tmem_st16(s_base, pk[DUP ? 0 : 1]);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_probs[w][k & 1]);
+      }
+      // ---- this group's pieces to the exchange: O, swizzled by row, and the statistics
+      // (the last scores imply every PV but the last two, each of which has a barrier of its own: on one barrier
+      // both might complete between two looks at it, and its parity be what it was)
+      for (int n = max(nsteps - 2, 0); n < nsteps && ok && !left; ++n)
+        ok = mbar_wait(&s_pv[w][(seq + n) & 1], ((seq + n) >> 1) & 1, guard);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        tc_fence_after();
+        float* xo = reinterpret_cast<float*>(rings);
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          if (nsteps > 0) {
+            tmem_ld32_sync(o_base + c, o);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = 0u;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const int ch = (c + j) >> 2;
+            *reinterpret_cast<uint4*>(xo + t * D + ((ch ^ (t & (D / 4 - 1))) << 2)) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          }
+        }
+        reinterpret_cast<float4*>(xo + 128 * D)[t] = make_float4(carry, m, l, slope2);
+      }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (*static_cast<volatile int*>(&s_abort) != 0) break;
+
+    // ---- pieces join, right to left
+    const bool whole = u0 == 0 && u1 == units;
+    float* rec = p.ws + paged_ws_head(p.B) + ((size_t)blockIdx.x * 2 + (u0 > 0 ? 0 : 1)) * L::RECORD;
+    const int n_rows = min(L::ROWS, rows - rb);
+    for (int e = tid; e < n_rows * (D / 4); e += L::THREADS) {
+      const int r = e / (D / 4), ch = e % (D / 4);
+      float right = 0.f, M = -INFINITY, wt[L::PIECES];
+#pragma unroll
+      for (int q = L::PIECES - 1; q >= 0; --q) {
+        const int lane_row = DUP ? r + 64 * (q & 1) : r, grp = DUP ? q >> 1 : q;
+        const float* xo = reinterpret_cast<const float*>(smem + L::QBYTES + grp * L::GROUP);
+        const float4 st = reinterpret_cast<const float4*>(xo + 128 * D)[lane_row];
+        wt[q] = st.y == -INFINITY ? -INFINITY : st.y - st.w * right;
+        M = fmaxf(M, wt[q]);
+        right += st.x;
+      }
+      const float m_use = M == -INFINITY ? 0.f : M;
+      float l = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int q = L::PIECES - 1; q >= 0; --q) {
+        const int lane_row = DUP ? r + 64 * (q & 1) : r, grp = DUP ? q >> 1 : q;
+        const float* xo = reinterpret_cast<const float*>(smem + L::QBYTES + grp * L::GROUP);
+        const float f = ex2_approx(wt[q] - m_use);
+        l = fmaf(reinterpret_cast<const float4*>(xo + 128 * D)[lane_row].z, f, l);
+        const float4 v = *reinterpret_cast<const float4*>(xo + lane_row * D + ((ch ^ (lane_row & (D / 4 - 1))) << 2));
+        acc.x = fmaf(v.x, f, acc.x);
+        acc.y = fmaf(v.y, f, acc.y);
+        acc.z = fmaf(v.z, f, acc.z);
+        acc.w = fmaf(v.w, f, acc.w);
+      }
+      if (s_any_nan != 0) {  // a drafted token that the row sees
+        const int row_of = (rb + r) % p.Sq;
+        unsigned long long word =
+            p.tree_mask != nullptr ? (unsigned long long)p.tree_mask[b * p.mask_stride + row_of] : (2ull << row_of) - 1;
+        if (p.Sq < 64) word &= (1ull << p.Sq) - 1;
+        uint32_t bad = 0;
+        for (; word != 0; word &= word - 1) bad |= s_u.nan[__ffsll((long long)word) - 1][ch >> 3] >> (4 * (ch & 7));
+        const float nan = __int_as_float(0x7fc00000);
+        if (bad & 1) acc.x = nan;
+        if (bad & 2) acc.y = nan;
+        if (bad & 4) acc.z = nan;
+        if (bad & 8) acc.w = nan;
+      }
+      if (whole) {
+        const int rr = rb + r;
+        uint16_t* y = static_cast<uint16_t*>(p.o) + b * p.os[0] + (g * G + rr / p.Sq) * p.os[1] + (rr % p.Sq) * p.os[2];
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        *reinterpret_cast<uint2*>(y + 4 * ch) =
+            make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+      } else {
+        if (ch == 0) reinterpret_cast<float4*>(rec)[r] = make_float4(right, M, l, 0.f);
+        *reinterpret_cast<float4*>(rec + 4 * L::ROWS + r * D + 4 * ch) = acc;
+      }
+    }
+    fence_async_smem();  // the exchange before the loads that refill the rings
+    __syncthreads();
+
+    seq += nsteps;
+    at += v1 - v0;
+    v0 = 0;
+    if (++item == heads) {
+      item = 0;
+      if (++b < p.B) span = paged_span<L>(p, b);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace coalibi

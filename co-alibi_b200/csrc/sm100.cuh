@@ -102,6 +102,11 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t by
                : "memory");
 }
 
+// Bytes to come, without an arrival.
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
 // try_wait with an explicit suspend-time hint (ns): returns within about that
 // long even if the phase has not completed, so a polling loop built on it wakes
 // promptly (the default hint can leave a thread asleep for ~1 us after the
