@@ -40,6 +40,8 @@ struct Wide8Layout {
 // are out and the softmax warps past step n - 6.
 constexpr int kWide8Meta = 6;
 
+__device__ __forceinline__ float2 splat2(float x) { return make_float2(x, x); }
+
 template <int D, bool BF16, bool DUP>
 __global__ void __launch_bounds__(512, 1)
     coalibi_paged8_wide_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -254,13 +256,15 @@ __global__ void __launch_bounds__(512, 1)
       __syncwarp();
     } else if (warp >= 12) {
       // ---------------------------------------------------------- codes to tiles
-      const int t = (warp - 12 & 1) * 32 + lane;  // of the group's 64 threads
-      constexpr int CH = D / 16;                  // 16-code chunks of a row: a thread takes one, and 512 / 8 or 64 / 4 keys apart
-      const int c = t % CH;
-      // chunk c of key `key` as float16; `zero`: nothing of the row may be used; nan: columns of NaN, taken out
-      auto turn = [&](const uint8_t* from, uint8_t* to, int key, bool zero, bool takes_nan, uint32_t& nan) {
-        const uint32_t phase = D == 128 ? key & 7 : key >> 1 & 3;
-        const uint4 u = *reinterpret_cast<const uint4*>(from + key * D + ((c ^ phase) << 4));
+      // A thread takes 16 codes at a time, of keys 16 apart.  The eight threads of a pass over shared memory take
+      // chunks 0-3 of a key of even number and 4-7 of the next one (and then the others; with 64 columns, all four of
+      // both), which hit all phases of both swizzles.
+      const int t = (warp & 1) * 32 + lane, odd = t >> 2 & 1, key0 = 2 * (t >> 3) + odd, c0 = D == 128 ? (t & 3) + 4 * odd : t & 3;
+      const uint32_t from0 = key0 * D + ((c0 ^ (D == 128 ? key0 & 7 : key0 >> 1 & 3)) << 4);
+      const uint32_t to0 = (c0 >> 2) * L::BOX + key0 * 128 + (((2 * c0 & 7) ^ (key0 & 7)) << 4);
+      constexpr int OTHER = D / 64;  // chunks of a key that a thread takes
+      auto convert = [&](const uint8_t* from, uint8_t* to, int i, int v, bool zero, bool takes_nan, uint32_t& nan) {
+        const uint4 u = *reinterpret_cast<const uint4*>(from + (from0 ^ (v << 6)) + i * 16 * D);
         uint32_t x[4] = {u.x, u.y, u.z, u.w};
         if (zero) x[0] = x[1] = x[2] = x[3] = 0u;
         if (takes_nan) {
@@ -274,14 +278,16 @@ __global__ void __launch_bounds__(512, 1)
         uint32_t h[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) e4m3_to_f16x4(x[j], h[2 * j], h[2 * j + 1]);
-        uint8_t* row = to + (D == 128 ? (c >> 2) * L::BOX : 0) + key * 128;
-        const int c0 = 2 * c & 7;
-        // (the two halves of a row of 128 columns store their pieces in opposite order, so that the eight lanes of
-        // a row hit all phases of the swizzle)
-        const bool swap = D == 128 && c >= 4;
-        const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-        *reinterpret_cast<uint4*>(row + (((c0 + swap) ^ (key & 7)) << 4)) = swap ? hi : lo;
-        *reinterpret_cast<uint4*>(row + (((c0 + !swap) ^ (key & 7)) << 4)) = swap ? lo : hi;
+        const uint32_t at = (to0 ^ (v * L::BOX)) + i * 2048;
+        *reinterpret_cast<uint4*>(to + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(to + (at ^ 16)) = make_uint4(h[4], h[5], h[6], h[7]);
+      };
+      auto convert_all = [&](const uint8_t* from, uint8_t* to) {
+        uint32_t none = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int v = 0; v < OTHER; ++v) convert(from, to, i, v, false, false, none);
       };
       auto make_k = [&](int n) {
         const uint32_t k = seq + n;
@@ -290,10 +296,7 @@ __global__ void __launch_bounds__(512, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
         if (t == 0) mbar_arrive(&s_meta[w][k & 3]);  // the scales, to the softmax warps
-        uint32_t none = 0;
-#pragma unroll 4
-        for (int key = t / CH; key < 64; key += 64 / CH)
-          turn(codes + slot * 2 * L::CODES, k_tiles + tile * L::TILE, key, false, false, none);
+        convert_all(codes + slot * 2 * L::CODES, k_tiles + tile * L::TILE);
         fence_async_smem();
         mbar_arrive(&s_k[w][tile]);
         mbar_arrive(&s_kc_free[w][slot]);
@@ -308,20 +311,19 @@ __global__ void __launch_bounds__(512, 1)
         uint8_t* to = v_tiles + tile * L::TILE;
         const int gone = s_gone[w][k % kWide8Meta];
         if (gone == 0) {
-          uint32_t none = 0;
-#pragma unroll 4
-          for (int key = t / CH; key < 64; key += 64 / CH) turn(from, to, key, false, false, none);
+          convert_all(from, to);
         } else {
           // V rows that no row sees (past the end, of no page, unseen drafts) may hold any code: zeros, 0 * NaN
           // is not 0.  What is NaN of a drafted token must not reach the rows that do not see it: zeros too, and
           // the rows that do get their NaN at the end.
 #pragma unroll 1
-          for (int key = t / CH; key < 64; key += 64 / CH) {
+          for (int e = 0; e < 4 * OTHER; ++e) {
+            const int i = e / OTHER, v = e % OTHER, key = key0 + 16 * i, c = c0 ^ (4 * v);
             const int hf = key >> 5, base = half_base(n, hf), pos = base + (key & 31);
             const bool used = base >= half_lo(hf) && !(gone >> (key >> 4) & 1) && pos < half_hi(hf) &&
                               (pos < ctx || (seen_by_any >> (pos - ctx) & 1));
             uint32_t nan = 0;
-            turn(from, to, key, !used, used && pos >= ctx, nan);
+            convert(from, to, i, v, !used, used && pos >= ctx, nan);
             if (nan != 0) {
               atomicOr(&s_u.nan[pos - ctx][c >> 1], nan << (16 * (c & 1)));
               s_any_nan = 1;
@@ -441,22 +443,28 @@ __global__ void __launch_bounds__(512, 1)
           const float2 ks = *reinterpret_cast<const float2*>(&s_ks[w][meta][2 * hf]);
           const float2 vs = *reinterpret_cast<const float2*>(&s_vs[w][meta][2 * hf]);
           const float f0 = c_a * ks.x, f1 = c_a * ks.y, lv0 = lg2_approx(vs.x), lv1 = lg2_approx(vs.y);
-          auto scan = [&](auto masked) {
+          auto half = [&](auto masked) {
             constexpr bool MASKED = decltype(masked)::value;
+            auto pair = [&](int j) { return make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])); };
+            auto keep = [&](int j, float2 v) { s[2 * j] = __float_as_uint(v.x), s[2 * j + 1] = __float_as_uint(v.y); };
+            auto mask = [&](int j, float2 v, float none) {
+              return make_float2(seen >> (2 * j) & 1 ? v.x : none, seen >> (2 * j + 1) & 1 ? v.y : none);
+            };
             // sub-chunks of 8 keys: short chains of additions that overlap
             float tot[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               float run = 0.f;
-              const float f = c < 2 ? f0 : f1;
+              const float2 f = splat2(c < 2 ? f0 : f1);
 #pragma unroll
-              for (int j = 7; j >= 0; --j) {
-                const int e = 8 * c + j;
-                const float y = __uint_as_float(s[e]) * f;
-                float sg = rcp_approx(ex2_approx(-y) + 1.f);
-                if (MASKED) sg = seen >> e & 1 ? sg : 0.f;
-                run += sg;
-                s[e] = __float_as_uint(fmaf(-slope2, run, y));
+              for (int j = 4 * c + 3; j >= 4 * c; --j) {
+                const float2 y = __fmul2_rn(pair(j), f);
+                const float2 dn = __fadd2_rn(make_float2(ex2_approx(-y.x), ex2_approx(-y.y)), splat2(1.f));
+                float2 sg = make_float2(rcp_approx(dn.x), rcp_approx(dn.y));
+                if (MASKED) sg = mask(j, sg, 0.f);
+                const float z1 = run + sg.y;
+                run = z1 + sg.x;
+                keep(j, __ffma2_rn(splat2(-slope2), make_float2(run, z1), y));
               }
               tot[c] = run;
             }
@@ -467,58 +475,58 @@ __global__ void __launch_bounds__(512, 1)
             off[1] = off[2] + tot[2];
             off[0] = off[1] + tot[1];
             carry = off[0] + tot[0];
-            float mx[2] = {-INFINITY, -INFINITY};
+            float mx2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              const float sh = -slope2 * off[c];
+              const float2 sh = splat2(-slope2 * off[c]);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int e = 8 * c + j;
-                float v = __uint_as_float(s[e]) + sh;
-                if (MASKED) v = seen >> e & 1 ? v : -INFINITY;
-                s[e] = __float_as_uint(v);
-                mx[c >> 1] = fmaxf(mx[c >> 1], v);
+              for (int j = 4 * c; j < 4 * c + 4; ++j) {
+                float2 v = __fadd2_rn(pair(j), sh);
+                if (MASKED) v = mask(j, v, -INFINITY);
+                keep(j, v);
+                mx2[c >> 1] = fmaxf(mx2[c >> 1], fmaxf(v.x, v.y));
               }
             }
-            return fmaxf(mx[0] + lv0, mx[1] + lv1);
-          };
-          const float mx = plain ? scan(std::false_type{}) : scan(std::true_type{});
-          // the reference moves only when a contribution passes it by 2^8: weights stay below 256, and
-          // O needs rescaling rarely
-          if (mx > m + 8.f || (m == -INFINITY && mx > -INFINITY)) {
-            const float f = m == -INFINITY ? 0.f : ex2_approx(m - mx);
-            if (m != -INFINITY) {
-              rescale = true;
-              alpha *= f;
-              if (!DUP && x == 1) {  // the right half's weights of this step move too
+            const float mx = fmaxf(mx2[0] + lv0, mx2[1] + lv1);
+            // the reference moves only when a contribution passes it by 2^8: weights stay below 256, and
+            // O needs rescaling rarely
+            if (mx > m + 8.f || (m == -INFINITY && mx > -INFINITY)) {
+              const float f = m == -INFINITY ? 0.f : ex2_approx(m - mx);
+              if (m != -INFINITY) {
+                rescale = true;
+                alpha *= f;
+                if (!DUP && x == 1) {  // the right half's weights of this step move too
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                  const float2 u = unpack2<false>(pk[0][j]);
-                  pk[0][j] = pack2<false>(u.x * f, u.y * f);
+                  for (int j = 0; j < 16; ++j) {
+                    const float2 u = unpack2<false>(pk[0][j]);
+                    pk[0][j] = pack2<false>(u.x * f, u.y * f);
+                  }
                 }
               }
+              l *= f;
+              m = mx;
             }
-            l *= f;
-            m = mx;
-          }
-          const float m_use = m == -INFINITY ? 0.f : m;
+            const float m_use = m == -INFINITY ? 0.f : m;
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const float sh = (q ? lv1 : lv0) - m_use;
-            float ls = 0.f;
+            for (int q = 0; q < 2; ++q) {
+              const float2 sh = splat2((q ? lv1 : lv0) - m_use);
+              float2 ls = splat2(0.f);
 #pragma unroll
-            for (int j = 8 * q; j < 8 * q + 8; ++j) {
-              float e0 = ex2_approx(__uint_as_float(s[2 * j]) + sh), e1 = ex2_approx(__uint_as_float(s[2 * j + 1]) + sh);
-              if (!plain) {  // (a block that nothing of is seen may have any scale)
-                e0 = seen >> (2 * j) & 1 ? e0 : 0.f;
-                e1 = seen >> (2 * j + 1) & 1 ? e1 : 0.f;
+              for (int j = 8 * q; j < 8 * q + 8; ++j) {
+                const float2 v = __fadd2_rn(pair(j), sh);
+                float2 e = make_float2(ex2_approx(v.x), ex2_approx(v.y));
+                if (MASKED) e = mask(j, e, 0.f);  // (a block that nothing of is seen may have any scale)
+                ls = __fadd2_rn(ls, e);
+                pk[DUP ? 0 : x][j] = pack2<false>(e.x, e.y);
               }
-              ls += e0 + e1;
-              pk[DUP ? 0 : x][j] = pack2<false>(e0, e1);
+              // the weights themselves: without the block's scale
+              if (!MASKED || (seen >> (16 * q) & 0xffffu) != 0) l = fmaf(ls.x + ls.y, rcp_approx(q ? vs.y : vs.x), l);
             }
-            // the weights themselves: without the block's scale
-            if (plain || (seen >> (16 * q) & 0xffffu) != 0) l = fmaf(ls, rcp_approx(q ? vs.y : vs.x), l);
-          }
+          };
+          if (plain)
+            half(std::false_type{});
+          else
+            half(std::true_type{});
         }
         if (__any_sync(0xffffffffu, rescale)) {
           // every PV before this step's must have added its part
