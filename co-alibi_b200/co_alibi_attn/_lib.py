@@ -152,7 +152,7 @@ def load():
             lib.coalibi_heads_fwd.restype = c_int
             lib.coalibi_heads_bwd.argtypes = [c_void_p, c_void_p, c_size_t, c_void_p]
             lib.coalibi_heads_bwd.restype = c_int
-            lib.coalibi_heads_bwd_workspace_bytes.argtypes = [c_int]
+            lib.coalibi_heads_bwd_workspace_bytes.argtypes = [c_int] * 3
             lib.coalibi_heads_bwd_workspace_bytes.restype = c_size_t
             lib.coalibi_sample.argtypes = [c_void_p, c_void_p]
             lib.coalibi_sample.restype = c_int

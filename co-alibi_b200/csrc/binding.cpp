@@ -432,7 +432,7 @@ Heads heads_of(PyObject* const* a) {
   if (h.B > 0x7fffffff || h.S > 0x7fffffff || h.B * h.S > 0x7fffffff) refuse(PyExc_ValueError, what, "too many tokens");
   const auto device = x.device();
   if (!device.is_cuda()) refuse(PyExc_ValueError, what, "qkv is on ", device.str());
-  h.qkv = aligned_rows(x.detach());
+  h.qkv = rows16(x) ? x : aligned_rows(x.detach());
   strides(h.qkv, p.qkv_stride);
   const char* names[2] = {"q_weight", "k_weight"};
   at::ScalarType type = x.scalar_type();
@@ -444,8 +444,7 @@ Heads heads_of(PyObject* const* a) {
       refuse(PyExc_TypeError, what, "the weights must both be ", c10::toString(x.scalar_type()), " or float32, got ", c10::toString(w.scalar_type()));
     if (w.dim() != 1 || w.size(0) != h.D) refuse(PyExc_ValueError, what, names[i], " must have shape [", h.D, "], got ", shape_of(w));
     on(what, names[i], w, device);
-    h.weight[i] = w.detach().contiguous();
-    if (reinterpret_cast<uintptr_t>(h.weight[i].data_ptr()) & 3) h.weight[i] = h.weight[i].clone();
+    h.weight[i] = w.is_contiguous() && (reinterpret_cast<uintptr_t>(w.data_ptr()) & 3) == 0 ? w : w.detach().clone(at::MemoryFormat::Contiguous);
     type = w.scalar_type();
     seen = true;
   }
@@ -531,7 +530,7 @@ PyObject* heads_bwd(PyObject* const* a) {
   for (int i = 0; i < 2; ++i)
     if (h.weight[i].defined()) dw[i] = h.qkv.numel() > 0 ? at::empty_like(h.weight[i]) : at::zeros_like(h.weight[i]);
   if (h.qkv.numel() > 0) {
-    const size_t bytes = coalibi_heads_bwd_workspace_bytes((int)h.D);
+    const size_t bytes = coalibi_heads_bwd_workspace_bytes((int)h.Hq, (int)h.Hkv, (int)h.D);
     const Tensor ws = at::empty({(int64_t)bytes}, h.qkv.options().dtype(at::kByte));
     p.q = d[0].data_ptr();
     p.k = d[1].data_ptr();

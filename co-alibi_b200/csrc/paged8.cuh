@@ -995,7 +995,7 @@ __global__ void __launch_bounds__(kJoinThreads) coalibi_paged8_join_kernel(const
   constexpr int V = D / 32, WARPS = kJoinThreads / 32, EARLY = 8;
   __shared__ float s_f[kJoinThreads], s_a[WARPS], s_b[WARPS], s_c[WARPS], s_o[WARPS][D];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int G = p.Hq / p.Hkv, rows = G * p.Sq;
+  const int G = p.Hq / p.Hkv;
   const int b = blockIdx.x / p.Hkv, g = blockIdx.x - b * p.Hkv, r = blockIdx.y;
   grid_dep_wait();
   const int* head = reinterpret_cast<const int*>(p.ws);

@@ -360,7 +360,7 @@ typedef struct CoalibiHeadsArgs {
 } CoalibiHeadsArgs;
 
 int coalibi_heads_fwd(const CoalibiHeadsArgs* args, void* stream);
-size_t coalibi_heads_bwd_workspace_bytes(int D);
+size_t coalibi_heads_bwd_workspace_bytes(int Hq, int Hkv, int D);
 int coalibi_heads_bwd(const CoalibiHeadsArgs* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Draw one token for each row of logits.  Tokens are ranked by (logit descending,

@@ -304,8 +304,8 @@ def test_refusals_of_the_c_entries():
                 dict(q_weight=2), dict(start=2)):
         assert codes(**bad) == (5, 5), bad
     assert codes(dqkv=8)[1] == 5 and codes(dk_weight=2)[1] == 5
-    need = lib.coalibi_heads_bwd_workspace_bytes(64)
-    assert need > 0 and lib.coalibi_heads_bwd_workspace_bytes(96) == 0
+    need = lib.coalibi_heads_bwd_workspace_bytes(2, 1, 64)
+    assert need > 0 and lib.coalibi_heads_bwd_workspace_bytes(2, 1, 96) == 0 and lib.coalibi_heads_bwd_workspace_bytes(0, 1, 64) == 0
     assert codes(ws=None)[1] == 8 and codes(ws=264)[1] == 8 and codes(bytes_=need - 1)[1] == 8
 
 
