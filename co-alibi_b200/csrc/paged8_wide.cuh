@@ -1,26 +1,32 @@
 // Attention over a paged cache in 8 bits for many rows per kv head (drafted trees): tcgen05.
 //
-// As the 16-bit cache's kernel for such rows (paged.cuh): 64 or 128 rows are the 128 lanes of TMEM, one row to a
-// thread; two groups of four softmax warps work on keys of their own, 64 to a step; with at most 64 rows
-// (DUP) the rows stand twice, and the two halves of the lanes take the halves of a step, which come from two
-// separate pieces of the item.  The tensor cores take the codes as float16, which holds them exactly, so each group has two
-// warps that turn the codes of a step, as they arrive by TMA, into the swizzled tiles that the MMA reads; K's tile
-// of the step after the next one is made as soon as the scores are out, V's as soon as its product is.
-// Scales enter the scores and the exponents of the weights as in the kernel for few rows (paged8.cuh).
+// As in the 16-bit cache's kernel for such rows (paged.cuh), 64 rows stand twice in the 128 lanes of TMEM; two
+// groups of warps work on keys of their own, 64 to a step, and the two halves of the lanes take the halves of a
+// step, which come from two separate pieces of the item.  More rows go in blocks of 64.
+//
+// The tensor cores take the codes as float16, which holds them exactly, so each group has two warps that turn
+// the codes of a step, as they arrive by TMA, into the swizzled tiles that the MMA reads; K's tile of the step after the next
+// one is made as soon as the scores are out, V's as soon as its product is.  Scales enter the scores and the exponents of the
+// weights as in the kernel for few rows (paged8.cuh).
+//
+// A group has eight softmax warps, 16 rows to each: four lanes share a row, 8 keys of its 32 to a lane.  The tiles' rows
+// are in the order that makes those 8 consecutive keys (column 8 j + 2 q + e is key 8 q + 2 j + e), so that a row's suffix sum is
+// additions in a lane and one scan over four, and a lane's keys have one scale.  With a row to a thread (four warps a group)
+// the 32 keys of a step took a thread 2750 clocks, most of them its own latencies.
 #pragma once
 
 #include "paged8.cuh"
 
 namespace coalibi {
 
-template <int D, bool DUP>
+template <int D>
 struct Wide8Layout {
-  static constexpr int PIECES = DUP ? 4 : 2;       // of an item, per CTA
-  static constexpr int STEP = DUP ? 32 : 64;       // keys of a piece per step
+  static constexpr int PIECES = 4;                 // of an item, per CTA
+  static constexpr int STEP = 32;                  // keys of a piece per step
   static constexpr int UNIT = 128;
   static constexpr int COST = 10;                  // of starting and finishing an item, in units
   static constexpr int WHOLE = 1024;               // keys of a table that is not split
-  static constexpr int ROWS = DUP ? 64 : 128;
+  static constexpr int ROWS = 64;
   static constexpr int TILE = 64 * D * 2;          // K or V of a step in float16: [D / 64][64 keys][128 bytes]
   static constexpr int BOX = 64 * 128;
   static constexpr int CODES = 64 * D;             // K or V of a step as codes: [64 keys][D], swizzled
@@ -31,7 +37,7 @@ struct Wide8Layout {
   static constexpr int CTAS = 1;
   static constexpr int RECORD = ROWS * (4 + D);
   static constexpr int TM_S = 64, TM_O = 256;      // columns of an S buffer; O of group w at TM_O + w * D
-  static constexpr int THREADS = 512;              // warps 0-7 softmax, 8 and 9 MMAs, 10 and 11 loads, 12-15 tiles
+  static constexpr int THREADS = 768;              // warps 0-15 softmax, 16 and 17 MMAs, 18 and 19 loads, 20-23 tiles
   // a group's part of the exchange (O in float, then statistics) reuses its rings
   static_assert(128 * D * 4 + 128 * 16 <= GROUP, "exchange fits the rings");
 };
@@ -40,13 +46,32 @@ struct Wide8Layout {
 // are out and the softmax warps past step n - 6.
 constexpr int kWide8Meta = 6;
 
+// 16 lanes of TMEM and 32 columns: register 4 j + 2 x + e holds row lane / 4 + 8 x, column 8 j + 2 (lane % 4) + e.
+__device__ __forceinline__ void tmem_ld_quads(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : COALIBI_R8(0), COALIBI_R8(8)
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_quads(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      COALIBI_I8(0), COALIBI_I8(8)
+      : "memory");
+}
+// 16 lanes and 16 columns: register 2 j + x holds row lane / 4 + 8 x, column 4 j + lane % 4.
+__device__ __forceinline__ void tmem_st_quads16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), COALIBI_I8(0) : "memory");
+}
 __device__ __forceinline__ float2 splat2(float x) { return make_float2(x, x); }
 
-template <int D, bool BF16, bool DUP>
-__global__ void __launch_bounds__(512, 1)
+template <int D, bool BF16>
+__global__ void __launch_bounds__(768, 1)
     coalibi_paged8_wide_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                                const Paged8Params p) {
-  using L = Wide8Layout<D, DUP>;
+  using L = Wide8Layout<D>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ uint64_t s_kc[2][2], s_kc_free[2][2], s_vc[2][2], s_vc_free[2][2];  // codes
@@ -66,8 +91,8 @@ __global__ void __launch_bounds__(512, 1)
   __shared__ int s_warp[4], s_find, s_abort;
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const bool softmax = warp < 8, issues = warp == 8 || warp == 9, loads = warp == 10 || warp == 11;
-  const int w = softmax ? warp >> 2 : warp < 12 ? warp & 1 : (warp - 12) >> 1;  // group
+  const bool softmax = warp < 16, issues = warp == 16 || warp == 17, loads = warp == 18 || warp == 19;
+  const int w = softmax ? warp >> 3 : warp < 20 ? warp & 1 : (warp - 20) >> 1;  // group
   const int G = p.Hq / p.Hkv, rows = G * p.Sq;
   const int heads = p.Hkv * p.row_blocks;
   const CtaGuard guard{&s_abort, p.status, kPagedTimeoutNs};
@@ -75,15 +100,15 @@ __global__ void __launch_bounds__(512, 1)
     for (int g = 0; g < 2; ++g) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_kc[g][i], 1);
-        mbar_init(&s_kc_free[g][i], 64);
+        mbar_init(&s_kc_free[g][i], 2);
         mbar_init(&s_vc[g][i], 1);
-        mbar_init(&s_vc_free[g][i], 64);
-        mbar_init(&s_k[g][i], 64);
+        mbar_init(&s_vc_free[g][i], 2);
+        mbar_init(&s_k[g][i], 2);
         mbar_init(&s_k_free[g][i], 1);
-        mbar_init(&s_v[g][i], 64);
+        mbar_init(&s_v[g][i], 2);
         mbar_init(&s_v_free[g][i], 1);
         mbar_init(&s_scores[g][i], 1);
-        mbar_init(&s_probs[g][i], 4);
+        mbar_init(&s_probs[g][i], 8);
         mbar_init(&s_pv[g][i], 1);
       }
       for (int i = 0; i < 4; ++i) mbar_init(&s_meta[g][i], 1);
@@ -94,7 +119,7 @@ __global__ void __launch_bounds__(512, 1)
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
   }
-  if (warp == 8) {
+  if (warp == 16) {
     tmem_alloc(&s_tmem, 512);
     tmem_relinquish();
   }
@@ -153,14 +178,11 @@ __global__ void __launch_bounds__(512, 1)
     auto piece_hi = [&](int q) { return min(s_hi, s_lo + (q + 1) * sub); };
     auto piece_steps = [&](int q) { return max(0, (piece_hi(q) - piece_lo(q) + L::STEP - 1) / L::STEP); };
     const int q0 = L::PIECES / 2 * w;
-    const int nsteps = DUP ? max(piece_steps(q0), piece_steps(q0 + 1)) : piece_steps(q0);
+    const int nsteps = max(piece_steps(q0), piece_steps(q0 + 1));
     // first key of half hf of step n (counted from the right); its piece's ends
-    auto half_base = [&](int n, int hf) {
-      if (DUP) return piece_lo(q0 + hf) + (piece_steps(q0 + hf) - 1 - n) * 32;
-      return piece_lo(q0) + (nsteps - 1 - n) * 64 + 32 * hf;
-    };
-    auto half_hi = [&](int hf) { return piece_hi(DUP ? q0 + hf : q0); };
-    auto half_lo = [&](int hf) { return piece_lo(DUP ? q0 + hf : q0); };
+    auto half_base = [&](int n, int hf) { return piece_lo(q0 + hf) + (piece_steps(q0 + hf) - 1 - n) * 32; };
+    auto half_hi = [&](int hf) { return piece_hi(q0 + hf); };
+    auto half_lo = [&](int hf) { return piece_lo(q0 + hf); };
 
     // ---- loads: step n of the group, by one warp; lane i < 4 looks up the step's block i
     int k_loaded = 0, v_loaded = 0;
@@ -212,8 +234,8 @@ __global__ void __launch_bounds__(512, 1)
     if (softmax) {
       // ---- the queries, in the K-major 128-byte-swizzled form the MMA reads; bfloat16 ones as float16, scaled by
       // a power of two that puts a row's largest at 2^14
-      for (int c = tid; c < 128 * (D / 8); c += 256) {
-        const int r = c / (D / 8), ch = c % (D / 8), row = rb + (DUP ? r & 63 : r);
+      for (int c = tid; c < 128 * (D / 8); c += 512) {
+        const int r = c / (D / 8), ch = c % (D / 8), row = rb + (r & 63);
         uint4 val = make_uint4(0u, 0u, 0u, 0u);
         if (row < rows)
           val = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + b * p.qs[0] +
@@ -254,14 +276,15 @@ __global__ void __launch_bounds__(512, 1)
           if (n < v_loaded) mbar_drain(&s_vc[w][kv % L::NCODE], (kv / L::NCODE) & 1, guard.timeout_ns);
         }
       __syncwarp();
-    } else if (warp >= 12) {
+    } else if (warp >= 20) {
       // ---------------------------------------------------------- codes to tiles
       // A thread takes 16 codes at a time, of keys 16 apart.  The eight threads of a pass over shared memory take
       // chunks 0-3 of a key of even number and 4-7 of the next one (and then the others; with 64 columns, all four of
       // both), which hit all phases of both swizzles.
       const int t = (warp & 1) * 32 + lane, odd = t >> 2 & 1, key0 = 2 * (t >> 3) + odd, c0 = D == 128 ? (t & 3) + 4 * odd : t & 3;
       const uint32_t from0 = key0 * D + ((c0 ^ (D == 128 ? key0 & 7 : key0 >> 1 & 3)) << 4);
-      const uint32_t to0 = (c0 >> 2) * L::BOX + key0 * 128 + (((2 * c0 & 7) ^ (key0 & 7)) << 4);
+      const int row0 = 8 * (key0 >> 1 & 3) + 2 * (key0 >> 3) + odd;  // of key0; 16 keys on, 4 rows; 32 keys on, 32
+      const uint32_t to0 = (c0 >> 2) * L::BOX + row0 * 128 + (((2 * c0 & 7) ^ row0 & 7) << 4);
       constexpr int OTHER = D / 64;  // chunks of a key that a thread takes
       auto convert = [&](const uint8_t* from, uint8_t* to, int i, int v, bool zero, bool takes_nan, uint32_t& nan) {
         const uint4 u = *reinterpret_cast<const uint4*>(from + (from0 ^ (v << 6)) + i * 16 * D);
@@ -278,7 +301,7 @@ __global__ void __launch_bounds__(512, 1)
         uint32_t h[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) e4m3_to_f16x4(x[j], h[2 * j], h[2 * j + 1]);
-        const uint32_t at = (to0 ^ (v * L::BOX)) + i * 2048;
+        const uint32_t at = ((to0 ^ (v * L::BOX)) + (i >> 1) * 4096 + (i & 1) * 512) ^ ((i & 1) << 6);
         *reinterpret_cast<uint4*>(to + at) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(to + (at ^ 16)) = make_uint4(h[4], h[5], h[6], h[7]);
       };
@@ -298,8 +321,11 @@ __global__ void __launch_bounds__(512, 1)
         if (t == 0) mbar_arrive(&s_meta[w][k & 3]);  // the scales, to the softmax warps
         convert_all(codes + slot * 2 * L::CODES, k_tiles + tile * L::TILE);
         fence_async_smem();
-        mbar_arrive(&s_k[w][tile]);
-        mbar_arrive(&s_kc_free[w][slot]);
+        __syncwarp();  // (one arrival for the warp: those of its threads would be taken one by one)
+        if (lane == 0) {
+          mbar_arrive(&s_k[w][tile]);
+          mbar_arrive(&s_kc_free[w][slot]);
+        }
       };
       auto make_v = [&](int n) {
         const uint32_t k = seq + n;
@@ -331,8 +357,11 @@ __global__ void __launch_bounds__(512, 1)
           }
         }
         fence_async_smem();
-        mbar_arrive(&s_v[w][tile]);
-        mbar_arrive(&s_vc_free[w][slot]);
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s_v[w][tile]);
+          mbar_arrive(&s_vc_free[w][slot]);
+        }
       };
       // K(0), K(1), V(0), K(2), V(1), ...: K's tile is free once the scores before the last are out
       if (nsteps > 0 && ok) make_k(0);
@@ -389,17 +418,21 @@ __global__ void __launch_bounds__(512, 1)
       }
       __syncwarp();
     } else {
-      // ---------------------------------------------------------- softmax: one row to a thread
-      const int t = (warp & 3) * 32 + lane, r = DUP ? t & 63 : t, my_half = t >> 6;
-      const bool rok = rb + r < rows;
-      const float slope2 = load_slope(p.slopes, p.slopes_dtype, g * G + (rok ? rb + r : rb) / p.Sq) * kLog2e;
-      const float c_a = p.sm_scale * kLog2e * (BF16 ? __int_as_float((127 - s_up[t]) << 23) : 1.f);
-      const int row_of = (rok ? rb + r : rb) % p.Sq;
-      const unsigned long long word =
-          p.tree_mask != nullptr ? (unsigned long long)p.tree_mask[b * p.mask_stride + row_of] : (2ull << row_of) - 1;
-      const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+      // ---------------------------------------------------------- softmax: two rows of 8 keys to a lane
+      const int t0 = (warp & 3) * 32 + (warp >> 2 & 1) * 16, hf = t0 >> 6, q = lane & 3;
+      const uint32_t lane_base = tmem + ((uint32_t)t0 << 16);
       const uint32_t o_base = lane_base + L::TM_O + w * D;
-      float m = -INFINITY, l = 0.f, carry = 0.f;
+      int row_of[2];       // of the request's drafted tokens
+      float slope2[2], c_a[2], m[2], l[2], carry[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int t = t0 + (lane >> 2) + 8 * x, r = rb + (t & 63), rr = r < rows ? r : rb;
+        row_of[x] = rr % p.Sq;
+        slope2[x] = load_slope(p.slopes, p.slopes_dtype, g * G + rr / p.Sq) * kLog2e;
+        c_a[x] = p.sm_scale * kLog2e * (BF16 ? __int_as_float((127 - s_up[t]) << 23) : 1.f);
+        m[x] = -INFINITY;
+        l[x] = carry[x] = 0.f;
+      }
       bool left = false;
       for (int n = 0; n < nsteps; ++n) {
         const uint32_t k = seq + n;
@@ -413,23 +446,25 @@ __global__ void __launch_bounds__(512, 1)
           break;
         }
         const int gone = s_gone[w][meta];
-        const bool plain = gone == 0;
-        uint32_t pk[DUP ? 1 : 2][16];
-        float alpha = 1.f;
+        uint32_t pk[8];
+        float alpha[2] = {1.f, 1.f};
         bool rescale = false;
         tc_fence_after();
+        uint32_t s[16];
+        tmem_ld_quads(s_base + 32 * hf, s);
+        const float k_scale = s_ks[w][meta][2 * hf + (q >> 1)], v_scale = s_vs[w][meta][2 * hf + (q >> 1)];
+        const float lv = lg2_approx(v_scale), iv = rcp_approx(v_scale);
+        uint32_t seen[2] = {0xffu, 0xffu};  // of this lane's 8 keys
+        if (gone != 0) {
+          const int base = half_base(n, hf), in = min(half_hi(hf), ctx) - base, end = half_hi(hf) - base;
+          const uint32_t context = in >= 32 ? 0xffffffffu : in > 0 ? (1u << in) - 1u : 0u;
 #pragma unroll
-        for (int x = 0; x < (DUP ? 1 : 2); ++x) {  // (the right half first)
-          const int hf = DUP ? my_half : 1 - x;
-          uint32_t s[32];
-          __syncwarp();  // (the loads and stores of TMEM take converged warps)
-          tmem_ld32_sync(s_base + 32 * hf, s);
-          uint32_t seen = 0xffffffffu;
-          if (!plain) {
-            const int base = half_base(n, hf), in = min(half_hi(hf), ctx) - base, end = half_hi(hf) - base;
-            const uint32_t context = in >= 32 ? 0xffffffffu : in > 0 ? (1u << in) - 1u : 0u;
+          for (int x = 0; x < 2; ++x) {
             uint32_t v = context;
             if (end > in && end > 0) {  // drafted tokens, up to `end`
+              const unsigned long long word = p.tree_mask != nullptr
+                                                  ? (unsigned long long)p.tree_mask[b * p.mask_stride + row_of[x]]
+                                                  : (2ull << row_of[x]) - 1;
               const int d = base - ctx;
               const uint32_t bits = d >= 0 ? (d < 64 ? (uint32_t)(word >> d) : 0u) : d > -32 ? (uint32_t)word << -d : 0u;
               v |= bits & (end >= 32 ? 0xffffffffu : (1u << end) - 1u) & ~context;
@@ -437,110 +472,101 @@ __global__ void __launch_bounds__(512, 1)
             if (base < half_lo(hf)) v = 0u;  // this piece has ended
             if (gone >> (2 * hf) & 1) v &= 0xffff0000u;
             if (gone >> (2 * hf + 1) & 1) v &= 0x0000ffffu;
-            seen = v;
+            seen[x] = v >> (8 * q) & 0xffu;
           }
-          // of the half's two blocks
-          const float2 ks = *reinterpret_cast<const float2*>(&s_ks[w][meta][2 * hf]);
-          const float2 vs = *reinterpret_cast<const float2*>(&s_vs[w][meta][2 * hf]);
-          const float f0 = c_a * ks.x, f1 = c_a * ks.y, lv0 = lg2_approx(vs.x), lv1 = lg2_approx(vs.y);
-          auto half = [&](auto masked) {
-            constexpr bool MASKED = decltype(masked)::value;
-            auto pair = [&](int j) { return make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])); };
-            auto keep = [&](int j, float2 v) { s[2 * j] = __float_as_uint(v.x), s[2 * j + 1] = __float_as_uint(v.y); };
-            auto mask = [&](int j, float2 v, float none) {
-              return make_float2(seen >> (2 * j) & 1 ? v.x : none, seen >> (2 * j + 1) & 1 ? v.y : none);
-            };
-            // sub-chunks of 8 keys: short chains of additions that overlap
-            float tot[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              float run = 0.f;
-              const float2 f = splat2(c < 2 ? f0 : f1);
-#pragma unroll
-              for (int j = 4 * c + 3; j >= 4 * c; --j) {
-                const float2 y = __fmul2_rn(pair(j), f);
-                const float2 dn = __fadd2_rn(make_float2(ex2_approx(-y.x), ex2_approx(-y.y)), splat2(1.f));
-                float2 sg = make_float2(rcp_approx(dn.x), rcp_approx(dn.y));
-                if (MASKED) sg = mask(j, sg, 0.f);
-                const float z1 = run + sg.y;
-                run = z1 + sg.x;
-                keep(j, __ffma2_rn(splat2(-slope2), make_float2(run, z1), y));
-              }
-              tot[c] = run;
-            }
-            // sums right of each sub-chunk shift its logits
-            float off[4];
-            off[3] = carry;
-            off[2] = off[3] + tot[3];
-            off[1] = off[2] + tot[2];
-            off[0] = off[1] + tot[1];
-            carry = off[0] + tot[0];
-            float mx2[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const float2 sh = splat2(-slope2 * off[c]);
-#pragma unroll
-              for (int j = 4 * c; j < 4 * c + 4; ++j) {
-                float2 v = __fadd2_rn(pair(j), sh);
-                if (MASKED) v = mask(j, v, -INFINITY);
-                keep(j, v);
-                mx2[c >> 1] = fmaxf(mx2[c >> 1], fmaxf(v.x, v.y));
-              }
-            }
-            const float mx = fmaxf(mx2[0] + lv0, mx2[1] + lv1);
-            // the reference moves only when a contribution passes it by 2^8: weights stay below 256, and
-            // O needs rescaling rarely
-            if (mx > m + 8.f || (m == -INFINITY && mx > -INFINITY)) {
-              const float f = m == -INFINITY ? 0.f : ex2_approx(m - mx);
-              if (m != -INFINITY) {
-                rescale = true;
-                alpha *= f;
-                if (!DUP && x == 1) {  // the right half's weights of this step move too
-#pragma unroll
-                  for (int j = 0; j < 16; ++j) {
-                    const float2 u = unpack2<false>(pk[0][j]);
-                    pk[0][j] = pack2<false>(u.x * f, u.y * f);
-                  }
-                }
-              }
-              l *= f;
-              m = mx;
-            }
-            const float m_use = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const float2 sh = splat2((q ? lv1 : lv0) - m_use);
-              float2 ls = splat2(0.f);
-#pragma unroll
-              for (int j = 8 * q; j < 8 * q + 8; ++j) {
-                const float2 v = __fadd2_rn(pair(j), sh);
-                float2 e = make_float2(ex2_approx(v.x), ex2_approx(v.y));
-                if (MASKED) e = mask(j, e, 0.f);  // (a block that nothing of is seen may have any scale)
-                ls = __fadd2_rn(ls, e);
-                pk[DUP ? 0 : x][j] = pack2<false>(e.x, e.y);
-              }
-              // the weights themselves: without the block's scale
-              if (!MASKED || (seen >> (16 * q) & 0xffffu) != 0) l = fmaf(ls.x + ls.y, rcp_approx(q ? vs.y : vs.x), l);
-            }
-          };
-          if (plain)
-            half(std::false_type{});
-          else
-            half(std::true_type{});
         }
+        // pair j of row x: keys 8 q + 2 j and the next one
+        auto pair = [&](int j, int x) { return make_float2(__uint_as_float(s[4 * j + 2 * x]), __uint_as_float(s[4 * j + 2 * x + 1])); };
+        auto keep = [&](int j, int x, float2 v) { s[4 * j + 2 * x] = __float_as_uint(v.x), s[4 * j + 2 * x + 1] = __float_as_uint(v.y); };
+        auto step = [&](auto masked) {
+          constexpr bool MASKED = decltype(masked)::value;
+          auto mask = [&](int j, int x, float2 v, float none) {
+            return make_float2(seen[x] >> (2 * j) & 1 ? v.x : none, seen[x] >> (2 * j + 1) & 1 ? v.y : none);
+          };
+          float tot[2], inc[2], mx[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float run = 0.f;
+            const float2 f = splat2(c_a[x] * k_scale);
+#pragma unroll
+            for (int j = 3; j >= 0; --j) {
+              const float2 y = __fmul2_rn(pair(j, x), f);
+              const float2 dn = __fadd2_rn(make_float2(ex2_approx(-y.x), ex2_approx(-y.y)), splat2(1.f));
+              float2 sg = make_float2(rcp_approx(dn.x), rcp_approx(dn.y));
+              if (MASKED) sg = mask(j, x, sg, 0.f);
+              const float z1 = run + sg.y;
+              run = z1 + sg.x;
+              keep(j, x, __ffma2_rn(splat2(-slope2[x]), make_float2(run, z1), y));
+            }
+            tot[x] = inc[x] = run;
+          }
+#pragma unroll
+          for (int d = 1; d <= 2; ++d)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float y = __shfl_down_sync(0xffffffffu, inc[x], d);
+              if (q + d < 4) inc[x] += y;
+            }
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float2 sh = splat2(-slope2[x] * (carry[x] + (inc[x] - tot[x])));
+            carry[x] += __shfl_sync(0xffffffffu, inc[x], lane & ~3);
+            mx[x] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float2 v = __fadd2_rn(pair(j, x), sh);
+              if (MASKED) v = mask(j, x, v, -INFINITY);
+              keep(j, x, v);
+              mx[x] = fmaxf(mx[x], fmaxf(v.x, v.y));
+            }
+            mx[x] += lv;
+          }
+#pragma unroll
+          for (int d = 1; d <= 2; ++d)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], d));
+          // the reference moves only when a contribution passes it by 2^8: weights stay below 256, and
+          // O needs rescaling rarely
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (mx[x] > m[x] + 8.f || (m[x] == -INFINITY && mx[x] > -INFINITY)) {
+              const float f = m[x] == -INFINITY ? 0.f : ex2_approx(m[x] - mx[x]);
+              rescale |= m[x] != -INFINITY;
+              alpha[x] = m[x] != -INFINITY ? f : 1.f;
+              l[x] *= f;
+              m[x] = mx[x];
+            }
+            const float2 sh = splat2(lv - (m[x] == -INFINITY ? 0.f : m[x]));
+            float2 ls = splat2(0.f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 v = __fadd2_rn(pair(j, x), sh);
+              float2 e = make_float2(ex2_approx(v.x), ex2_approx(v.y));
+              if (MASKED) e = mask(j, x, e, 0.f);  // (a block that nothing of is seen may have any scale)
+              ls = __fadd2_rn(ls, e);
+              pk[2 * j + x] = pack2<false>(e.x, e.y);
+            }
+            // the weights themselves: without the block's scale
+            if (!MASKED || seen[x] != 0) l[x] = fmaf(ls.x + ls.y, iv, l[x]);
+          }
+        };
+        if (gone == 0)
+          step(std::false_type{});
+        else
+          step(std::true_type{});
         if (__any_sync(0xffffffffu, rescale)) {
           // every PV before this step's must have added its part
           if (n > 0) ok = mbar_wait(&s_pv[w][(k - 1) & 1], ((k - 1) >> 1) & 1, guard);
           ok = __all_sync(0xffffffffu, ok);
           if (ok && n > 0) {
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld32_sync(o_base + c, o);
+              uint32_t o[16];
+              tmem_ld_quads(o_base + c, o);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-              tmem_st32(o_base + c, o);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha[j >> 1 & 1]);
+              tmem_st_quads(o_base + c, o);
             }
           }
         }
@@ -549,15 +575,10 @@ __global__ void __launch_bounds__(512, 1)
           left = true;
           break;
         }
-        __syncwarp();
-        if (DUP) {
-          const uint32_t none[16] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-          tmem_st16(s_base + 16 * my_half, pk[0]);
-          tmem_st16(s_base + 16 * (1 - my_half), none);
-        } else {
-          tmem_st16(s_base + 16, pk[0]);
-          tmem_st16(s_base, pk[DUP ? 0 : 1]);
-        }
+        __syncwarp();  // (the loads and stores of TMEM take converged warps)
+        const uint32_t none[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+        tmem_st_quads16(s_base + 16 * hf, pk);
+        tmem_st_quads16(s_base + 16 * (1 - hf), none);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -573,21 +594,26 @@ __global__ void __launch_bounds__(512, 1)
         tc_fence_after();
         float* xo = reinterpret_cast<float*>(rings);
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          if (nsteps > 0) {
-            tmem_ld32_sync(o_base + c, o);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = 0u;
-          }
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const int ch = (c + j) >> 2;
-            *reinterpret_cast<uint4*>(xo + t * D + ((ch ^ (t & (D / 4 - 1))) << 2)) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-          }
+        for (int x = 0; x < 2; ++x) {
+          l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+          l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+          if (q == 0) reinterpret_cast<float4*>(xo + 128 * D)[t0 + (lane >> 2) + 8 * x] = make_float4(carry[x], m[x], l[x], slope2[x]);
         }
-        reinterpret_cast<float4*>(xo + 128 * D)[t] = make_float4(carry, m, l, slope2);
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = 0u;
+          if (nsteps > 0) tmem_ld_quads(o_base + c, o);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int t = t0 + (lane >> 2) + 8 * x, col = c + 8 * j + 2 * q;
+              *reinterpret_cast<uint2*>(xo + t * D + (((col >> 2) ^ (t & (D / 4 - 1))) << 2) + (col & 3)) =
+                  make_uint2(o[4 * j + 2 * x], o[4 * j + 2 * x + 1]);
+            }
+        }
       }
     }
     tc_fence_before();
@@ -604,7 +630,7 @@ __global__ void __launch_bounds__(512, 1)
       float right = 0.f, M = -INFINITY, wt[L::PIECES];
 #pragma unroll
       for (int q = L::PIECES - 1; q >= 0; --q) {
-        const int lane_row = DUP ? r + 64 * (q & 1) : r, grp = DUP ? q >> 1 : q;
+        const int lane_row = r + 64 * (q & 1), grp = q >> 1;
         const float* xo = reinterpret_cast<const float*>(smem + L::QBYTES + grp * L::GROUP);
         const float4 st = reinterpret_cast<const float4*>(xo + 128 * D)[lane_row];
         wt[q] = st.y == -INFINITY ? -INFINITY : st.y - st.w * right;
@@ -616,7 +642,7 @@ __global__ void __launch_bounds__(512, 1)
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int q = L::PIECES - 1; q >= 0; --q) {
-        const int lane_row = DUP ? r + 64 * (q & 1) : r, grp = DUP ? q >> 1 : q;
+        const int lane_row = r + 64 * (q & 1), grp = q >> 1;
         const float* xo = reinterpret_cast<const float*>(smem + L::QBYTES + grp * L::GROUP);
         const float f = ex2_approx(wt[q] - m_use);
         l = fmaf(reinterpret_cast<const float4*>(xo + 128 * D)[lane_row].z, f, l);
@@ -664,7 +690,7 @@ __global__ void __launch_bounds__(512, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

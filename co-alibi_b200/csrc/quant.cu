@@ -72,15 +72,15 @@ int launch_rows8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, 
   return launch_attention8<D, BF16, NT, RW, 4>(tk, tv, p, sms, s);
 }
 
-template <int D, bool BF16, bool DUP>
+template <int D, bool BF16>
 int launch_wide8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, int sms, cudaStream_t s) {
   static std::atomic<unsigned long long> ready{0};
-  using L = Wide8Layout<D, DUP>;
+  using L = Wide8Layout<D>;
   const auto join = [&p, s](int rows) {
     return launch_pdl(coalibi_paged8_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, rows), dim3(kJoinThreads), 0, s,
                       static_cast<const PagedAttnParams&>(p));
   };
-  return launch_paged<L>(coalibi_paged8_wide_kernel<D, BF16, DUP>, join, ready, L::THREADS, tk, tv, p, sms, s);
+  return launch_paged<L>(coalibi_paged8_wide_kernel<D, BF16>, join, ready, L::THREADS, tk, tv, p, sms, s);
 }
 
 template <int D, bool BF16>
@@ -89,8 +89,7 @@ int launch_paged8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p,
   if (rows <= 8) return launch_rows8<D, BF16, 1, 1>(tk, tv, p, sms, s);
   if (rows <= 16) return launch_rows8<D, BF16, 2, 1>(tk, tv, p, sms, s);
   if (rows <= 32) return launch_rows8<D, BF16, 2, 2>(tk, tv, p, sms, s);
-  if (rows <= 64) return launch_wide8<D, BF16, true>(tk, tv, p, sms, s);
-  return launch_wide8<D, BF16, false>(tk, tv, p, sms, s);
+  return launch_wide8<D, BF16>(tk, tv, p, sms, s);
 }
 
 template <int D>
@@ -98,8 +97,7 @@ size_t paged8_ws(int B, int rows) {
   if (rows <= 8) return std::max(paged_ws_bytes<Paged8Layout<D, 1, 1, 1>>(B), paged_ws_bytes<Paged8Layout<D, 1, 1, 4>>(B));
   if (rows <= 16) return std::max(paged_ws_bytes<Paged8Layout<D, 2, 1, 1>>(B), paged_ws_bytes<Paged8Layout<D, 2, 1, 4>>(B));
   if (rows <= 32) return std::max(paged_ws_bytes<Paged8Layout<D, 2, 2, 2>>(B), paged_ws_bytes<Paged8Layout<D, 2, 2, 4>>(B));
-  if (rows <= 64) return paged_ws_bytes<Wide8Layout<D, true>>(B);
-  return paged_ws_bytes<Wide8Layout<D, false>>(B);
+  return paged_ws_bytes<Wide8Layout<D>>(B);
 }
 
 }  // namespace
