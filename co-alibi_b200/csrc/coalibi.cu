@@ -63,10 +63,10 @@ int make_tmap(CUtensorMap* map, const void* base, int D, int rows, int heads, in
 }
 
 // 4-D view (D, slot, head, page) of a page pool of any strides (in elements; that of a
-// dimension of one entry is never used), loaded as boxes of 16 slots: of 64 columns of 16 bits
+// dimension of one entry is never used), loaded as boxes of `slots` slots: of 64 columns of 16 bits
 // with the 128-byte swizzle, or of whole rows of 8-bit codes with the swizzle of their width.
 int make_page_tmap(CUtensorMap* map, const void* base, int D, int page_size, int heads, int pages,
-                   const long long* stride, int dtype) {
+                   const long long* stride, int dtype, int slots) {
   auto fn = encode_fn();
   if (fn == nullptr) {
     snprintf(g_last_error, sizeof(g_last_error), "cuTensorMapEncodeTiled unavailable from the driver");
@@ -77,7 +77,7 @@ int make_page_tmap(CUtensorMap* map, const void* base, int D, int page_size, int
   const cuuint64_t size = codes ? 1 : 2;
   cuuint64_t strides[3];
   for (int i = 0; i < 3; ++i) strides[i] = (dims[i + 1] > 1 ? (cuuint64_t)stride[2 - i] : (cuuint64_t)D) * size;
-  cuuint32_t box[4] = {codes ? (cuuint32_t)D : 64u, 16, 1, 1};
+  cuuint32_t box[4] = {codes ? (cuuint32_t)D : 64u, (cuuint32_t)slots, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = fn(map,
                   codes                   ? CU_TENSOR_MAP_DATA_TYPE_UINT8

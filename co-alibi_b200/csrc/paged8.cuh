@@ -404,6 +404,7 @@ struct Paged8Params : PagedAttnParams {
   const float* k_scales;
   const float* v_scales;
   long long kss[2], vss[2];  // page, head
+  int box;                   // slots of a load: 16, or 32 where a step lies in one page
 };
 
 template <int D, int NT, int RW, int WARPS>
@@ -414,7 +415,7 @@ struct Paged8Layout {
   static constexpr int WHOLE = 512;
   static constexpr int ROWS = 8 * NT * RW;
   static constexpr int TILE = kPagedStep * D;      // K or V of a step: [32 keys][D bytes], swizzled
-  static constexpr int NBUF = KG > 1 ? 3 : (RW == 1 ? 2 : RW == 2 ? 3 : 4) + (D == 64 ? 1 : 0);
+  static constexpr int NBUF = KG > 1 ? 3 : (RW == 1 ? 2 : 3) + (D == 64 ? 1 : 0);
   static constexpr int RING = NBUF * 2 * TILE;     // per key group
   static constexpr int EXCHANGE = KG > 1 ? ROWS * D * 4 : 0;  // of a key group, over its ring
   static constexpr int GROUP = RING > EXCHANGE ? RING : EXCHANGE;
@@ -433,6 +434,13 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
+}
+// The float16 MMA with nothing to add to.
+__device__ __forceinline__ void mma16816_zero(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ float lg2_approx(float x) {
   float y;
@@ -540,21 +548,27 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
     int page_id[2], page_slot[2];  // of the next step to be loaded, per half; id -1: nothing there
     uint32_t gone_q = 0;           // two bits per ring slot: halves that were not loaded
     float ks_q[L::NBUF - 1], vs_q[L::NBUF - 1];  // scales of this lane's block in the steps under way
-    auto lookup = [&](int st) {
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const int key = lo + st * kPagedStep + 16 * f;
-        page_id[f] = -1;
-        page_slot[f] = 0;
-        if (st >= 0 && key < hi) {
-          const int n = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-          page_id[f] = table[n];
-          page_slot[f] = key - n * p.page_size;
-          if ((unsigned)page_id[f] >= (unsigned)p.n_pages) {
-            page_id[f] = -1;
-            report_page(p.status);
-          }
+    auto lookup_half = [&](int key, int f) {
+      page_id[f] = -1;
+      page_slot[f] = 0;
+      if (key >= lo && key < hi) {
+        const int n = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+        page_id[f] = table[n];
+        page_slot[f] = key - n * p.page_size;
+        if ((unsigned)page_id[f] >= (unsigned)p.n_pages) {
+          page_id[f] = -1;
+          report_page(p.status);
         }
+      }
+    };
+    auto lookup = [&](int st) {
+      const int key = lo + st * kPagedStep;
+      lookup_half(key, 0);
+      if (KG == 1 && p.box == 32) {  // (steps begin at multiples of 32 here)
+        page_id[1] = key + 16 < hi ? page_id[0] : -1;
+        page_slot[1] = page_slot[0] + 16;
+      } else {
+        lookup_half(key + 16, 1);
       }
     };
     auto load = [&]() {
@@ -563,12 +577,20 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
       gone_q |= ((page_id[0] < 0 ? 1u : 0u) | (page_id[1] < 0 ? 2u : 0u)) << (2 * slot);
       if (issuer) {
         const uint32_t dst = smem_u32(ring + slot * 2 * L::TILE);
-        mbar_arrive_expect_tx(&full[slot], ((page_id[0] >= 0) + (page_id[1] >= 0)) * L::TILE);
+        if (KG == 1 && p.box == 32) {  // (the second half may lie past the keys: it is loaded, and masked)
+          mbar_arrive_expect_tx(&full[slot], page_id[0] >= 0 ? 2 * L::TILE : 0);
+          if (page_id[0] >= 0) {
+            tma_load_4d(dst, &tk, &full[slot], 0, page_slot[0], g, page_id[0]);
+            tma_load_4d(dst + L::TILE, &tv, &full[slot], 0, page_slot[0], g, page_id[0]);
+          }
+        } else {
+          mbar_arrive_expect_tx(&full[slot], ((page_id[0] >= 0) + (page_id[1] >= 0)) * L::TILE);
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          if (page_id[f] < 0) continue;
-          tma_load_4d(dst + f * 16 * D, &tk, &full[slot], 0, page_slot[f], g, page_id[f]);
-          tma_load_4d(dst + L::TILE + f * 16 * D, &tv, &full[slot], 0, page_slot[f], g, page_id[f]);
+          for (int f = 0; f < 2; ++f) {
+            if (page_id[f] < 0) continue;
+            tma_load_4d(dst + f * 16 * D, &tk, &full[slot], 0, page_slot[f], g, page_id[f]);
+            tma_load_4d(dst + L::TILE + f * 16 * D, &tv, &full[slot], 0, page_slot[f], g, page_id[f]);
+          }
         }
       }
       loads.issue();
@@ -672,10 +694,6 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
       // ---- S^T = K Q^T: rows of tile pair mt, columns of block n
       float sc[2][NT][4];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) sc[mt][n][0] = sc[mt][n][1] = sc[mt][n][2] = sc[mt][n][3] = 0.f;
-#pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         uint32_t w[4], a[2][4];
         ldsm_x4(kt + (off ^ (kk << 4)), w[0], w[1], w[2], w[3]);
@@ -684,7 +702,12 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816<false>(sc[mt][n], a[mt], qb[n][kk][0], qb[n][kk][1]);
+          for (int n = 0; n < NT; ++n) {
+            if (kk == 0)
+              mma16816_zero(sc[mt][n], a[mt], qb[n][kk][0], qb[n][kk][1]);
+            else
+              mma16816<false>(sc[mt][n], a[mt], qb[n][kk][0], qb[n][kk][1]);
+          }
       }
       // ---- which of this lane's 4 keys each of its rows sees: bit 8 n + 4 x + c
       const uint32_t gone = gone_q >> (2 * slot) & 3;

@@ -54,22 +54,28 @@ template <int D, bool BF16, int NT, int RW, int WARPS>
 int launch_attention8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, int sms, cudaStream_t s) {
   static std::atomic<unsigned long long> ready{0};
   using L = Paged8Layout<D, NT, RW, WARPS>;
+  // A CTA joins a row where items come in many pieces, a warp where they come in few.  With a warp / a CTA to a
+  // row: contexts in some 50 pieces 15 / 6 us, a ragged decode batch 7.5 / 4.4, 4096 rows of 2 to 3 pieces (of
+  // the wide kernel) 4.7 / 12.7.
   const auto join = [&p, s](int rows) {
-    return launch_pdl(coalibi_paged8_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, rows), dim3(kJoinThreads), 0, s,
-                      static_cast<const PagedAttnParams&>(p));
+    const PagedAttnParams& a = p;
+    if ((long long)p.n_ctas > 8LL * p.B * p.Hkv * p.row_blocks)
+      return launch_pdl(coalibi_paged8_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, rows), dim3(kJoinThreads), 0, s, a);
+    return launch_pdl(coalibi_paged_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, (rows + 3) / 4), dim3(128), 0, s, a);
   };
   return launch_paged<L>(coalibi_paged8_attn_kernel<D, BF16, NT, RW, WARPS>, join, ready, 32 * WARPS, tk, tv, p, sms, s);
 }
 
 // Four warps to an item where the tables hold little work, else as many as its rows take (as in the
-// 16-bit attention).
+// 16-bit attention).  Items of up to 32 rows.
+bool shares_items(const Paged8Params& p, int sms) {
+  const long long items = (long long)p.B * p.Hkv, width = (long long)p.max_pages * p.page_size;
+  return !(items > 2LL * sms || (width > 512 && items * width > 32768));
+}
 template <int D, bool BF16, int NT, int RW>
 int launch_rows8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, int sms, cudaStream_t s) {
-  const int rows = p.Hq / p.Hkv * p.Sq;
-  const long long items = (long long)p.B * p.Hkv * ((rows + 8 * NT * RW - 1) / (8 * NT * RW));
-  const long long width = (long long)p.max_pages * p.page_size;
-  if (items > 2LL * sms || (width > 512 && items * width > 32768)) return launch_attention8<D, BF16, NT, RW, RW>(tk, tv, p, sms, s);
-  return launch_attention8<D, BF16, NT, RW, 4>(tk, tv, p, sms, s);
+  return shares_items(p, sms) ? launch_attention8<D, BF16, NT, RW, 4>(tk, tv, p, sms, s)
+                              : launch_attention8<D, BF16, NT, RW, RW>(tk, tv, p, sms, s);
 }
 
 template <int D, bool BF16>
@@ -77,7 +83,7 @@ int launch_wide8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, 
   static std::atomic<unsigned long long> ready{0};
   using L = Wide8Layout<D>;
   const auto join = [&p, s](int rows) {
-    return launch_pdl(coalibi_paged8_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, rows), dim3(kJoinThreads), 0, s,
+    return launch_pdl(coalibi_paged_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, (rows + 3) / 4), dim3(128), 0, s,
                       static_cast<const PagedAttnParams&>(p));
   };
   return launch_paged<L>(coalibi_paged8_wide_kernel<D, BF16>, join, ready, L::THREADS, tk, tv, p, sms, s);
@@ -86,6 +92,9 @@ int launch_wide8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, 
 template <int D, bool BF16>
 int launch_paged8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, int sms, cudaStream_t s) {
   const int rows = p.Hq / p.Hkv * p.Sq;
+  // The wide kernel costs the same for 1 to 64 rows.  8 ragged contexts up to 16k keys, narrow / wide: 16 rows 62 /
+  // 67 us, 20 rows 81 / 79, 32 rows 87 / 79; 32 rows of 64 contexts of 200 keys 36 / 65, of 1000 keys 97 / 104;
+  // 32 rows of D = 64 65 / 79.
   if (rows <= 8) return launch_rows8<D, BF16, 1, 1>(tk, tv, p, sms, s);
   if (rows <= 16) return launch_rows8<D, BF16, 2, 1>(tk, tv, p, sms, s);
   if (rows <= 32) return launch_rows8<D, BF16, 2, 2>(tk, tv, p, sms, s);
@@ -303,9 +312,13 @@ extern "C" int coalibi_paged_attention8(const CoalibiPagedAttentionArgs* a, cons
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = a->dtype == COALIBI_BF16;
   const int sms = device_sm_count();
+  // Loads of 32 slots where a warp walks whole steps and no step crosses a page; the 16-slot form
+  // serves the rest (its warps share an item, or pages end within a step).
+  const bool narrow = a->Hq / a->Hkv * a->Sq <= 32;
+  p.box = narrow && a->page_size % 32 == 0 && !shares_items(p, sms) ? 32 : 16;
   CUtensorMap tk, tv;
-  if ((rc = make_page_tmap(&tk, a->k_pages, a->D, a->page_size, a->Hkv, a->n_pages, a->k_page_stride, COALIBI_E4M3))) return rc;
-  if ((rc = make_page_tmap(&tv, a->v_pages, a->D, a->page_size, a->Hkv, a->n_pages, a->v_page_stride, COALIBI_E4M3))) return rc;
+  if ((rc = make_page_tmap(&tk, a->k_pages, a->D, a->page_size, a->Hkv, a->n_pages, a->k_page_stride, COALIBI_E4M3, p.box))) return rc;
+  if ((rc = make_page_tmap(&tv, a->v_pages, a->D, a->page_size, a->Hkv, a->n_pages, a->v_page_stride, COALIBI_E4M3, p.box))) return rc;
   if (a->D == 128) return bf16 ? launch_paged8<128, true>(tk, tv, p, sms, s) : launch_paged8<128, false>(tk, tv, p, sms, s);
   return bf16 ? launch_paged8<64, true>(tk, tv, p, sms, s) : launch_paged8<64, false>(tk, tv, p, sms, s);
 }

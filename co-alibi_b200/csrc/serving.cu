@@ -218,8 +218,8 @@ extern "C" int coalibi_paged_attention(const CoalibiPagedAttentionArgs* a, void*
   const bool bf16 = a->dtype == COALIBI_BF16;
   const int sms = device_sm_count();
   CUtensorMap tk, tv;
-  if ((rc = make_page_tmap(&tk, a->k_pages, a->D, a->page_size, a->Hkv, a->n_pages, a->k_page_stride, a->dtype))) return rc;
-  if ((rc = make_page_tmap(&tv, a->v_pages, a->D, a->page_size, a->Hkv, a->n_pages, a->v_page_stride, a->dtype))) return rc;
+  if ((rc = make_page_tmap(&tk, a->k_pages, a->D, a->page_size, a->Hkv, a->n_pages, a->k_page_stride, a->dtype, 16))) return rc;
+  if ((rc = make_page_tmap(&tv, a->v_pages, a->D, a->page_size, a->Hkv, a->n_pages, a->v_page_stride, a->dtype, 16))) return rc;
   if (a->D == 128) return bf16 ? launch_paged_rows<128, true>(tk, tv, p, sms, s) : launch_paged_rows<128, false>(tk, tv, p, sms, s);
   return bf16 ? launch_paged_rows<64, true>(tk, tv, p, sms, s) : launch_paged_rows<64, false>(tk, tv, p, sms, s);
 }

@@ -16,7 +16,7 @@ namespace coalibi {
 
 void set_last_error_detail(const char* msg);
 int make_page_tmap(CUtensorMap* map, const void* base, int D, int page_size, int heads, int pages,
-                   const long long* stride, int dtype);
+                   const long long* stride, int dtype, int slots);
 
 namespace {
 
