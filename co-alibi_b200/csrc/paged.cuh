@@ -905,7 +905,7 @@ __global__ void __launch_bounds__(384, 1)
   using L = WideLayout<D, DUP>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  __shared__ uint64_t s_full[2][L::NBUF], s_empty[2][L::NBUF], s_scores[2][2], s_probs[2][2], s_pv[2], s_idle[2];
+  __shared__ uint64_t s_full[2][L::NBUF], s_empty[2][L::NBUF], s_scores[2][2], s_probs[2][2], s_pv[2][2], s_idle[2];
   // four bits: 16-key quarters of the step that were not loaded; 16: some key of it is not of the context
   __shared__ int s_gone[2][L::NBUF];
   __shared__ int s_pre[128], s_warp[4], s_find, s_abort;
@@ -925,8 +925,8 @@ __global__ void __launch_bounds__(384, 1)
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_scores[g][i], 1);
         mbar_init(&s_probs[g][i], 4);
+        mbar_init(&s_pv[g][i], 1);
       }
-      mbar_init(&s_pv[g], 1);
       mbar_init(&s_idle[g], 1);
     }
     s_abort = 0;
@@ -1158,7 +1158,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             umma_ts(tmem + L::TM_O + w * D, pa + kk * 8, make_sdesc_sw128(v_addr + kk * 16 * 128, L::BOX, 1024), idPV, 1u);
-          umma_commit(&s_pv[w]);
+          umma_commit(&s_pv[w][k & 1]);
           umma_commit(&s_empty[w][slot]);
         }
         __syncwarp();
@@ -1305,7 +1305,7 @@ __global__ void __launch_bounds__(384, 1)
           }
           if (__any_sync(0xffffffffu, rescale)) {
             // every PV before this step's must have added its part
-            if (k > 0) ok = mbar_wait(&s_pv[w], (k - 1) & 1, guard);
+            if (k > 0) ok = mbar_wait(&s_pv[w][(k - 1) & 1], ((k - 1) >> 1) & 1, guard);
             ok = __all_sync(0xffffffffu, ok);
             if (ok) {
               tc_fence_after();
@@ -1343,7 +1343,7 @@ __global__ void __launch_bounds__(384, 1)
             const bool bad = drafted(n, hf, gone) && not_finite(vt + lane * 128);
             const uint32_t bads = __ballot_sync(0xffffffffu, bad);
             if (bads != 0 && (!DUP || hf == my_half)) {
-              if (k > 0) ok = mbar_wait(&s_pv[w], (k - 1) & 1, guard);
+              if (k > 0) ok = mbar_wait(&s_pv[w][(k - 1) & 1], ((k - 1) >> 1) & 1, guard);
               ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
               tc_fence_after();
@@ -1383,10 +1383,10 @@ __global__ void __launch_bounds__(384, 1)
         if (lane == 0) mbar_arrive(&s_probs[w][k & 1]);
       }
       // ---- this group's pieces to the exchange: O, swizzled by row, and the statistics
-      // (the last scores imply every PV but the last two: a wait on the last one's parity alone would
-      // pass while the one before it is under way)
-      if (!left && nsteps > 1) ok = mbar_wait(&s_pv[w], (seq + nsteps - 2) & 1, guard);
-      if (ok && !left && nsteps > 0) ok = mbar_wait(&s_pv[w], (seq + nsteps - 1) & 1, guard);
+      // (the last scores imply every PV but the last two, each of which has a barrier of its own: on one barrier
+      // both might complete between two looks at it, and its parity be what it was)
+      for (int n = max(nsteps - 2, 0); n < nsteps && ok && !left; ++n)
+        ok = mbar_wait(&s_pv[w][(seq + n) & 1], ((seq + n) >> 1) & 1, guard);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
