@@ -335,3 +335,31 @@ def test_refusals():
             (RuntimeError, dict(rotary=(tab(4, 8), tab(4, 8).requires_grad_()), qkv=z(2, 3, 6, 64).requires_grad_()))):
         with pytest.raises(kind):
             norm_rotate_qkv(**{**good, **kw})
+
+
+@pytest.mark.gpu
+def test_no_eps():
+    """Slots of a CTA without a token add nothing to the weights' gradient; tolerances as above."""
+    import co_alibi_attn
+    B, S, Hq, Hkv, D, dt = 1, 3, 2, 1, 64, f16
+    qkv, weights, grads, _, _, _ = _inputs((B, S, Hq, Hkv, D, dt, f32, 0, False, ""), 21)
+    x, w = qkv.cuda().requires_grad_(), [t.cuda().requires_grad_() for t in weights]
+    got = torch.autograd.grad(co_alibi_attn.norm_rotate_qkv(x, Hq, Hkv, *w, eps=0.0), [x, *w], [t.cuda() for t in grads])
+    x64, w64 = qkv.double().requires_grad_(), [t.double().requires_grad_() for t in weights]
+    want = torch.autograd.grad(qr.heads(x64, Hq, Hkv, *w64, 0.0, None, None, torch.arange(S).expand(B, S), False), [x64, *w64],
+                               [t.double() for t in grads])
+    n = qkv.double() * qkv.double().square().mean(-1, keepdim=True).rsqrt()
+    for i, h in enumerate((slice(0, Hq), slice(Hq, Hq + Hkv))):
+        size = (n[:, :, h] * grads[i].double().transpose(1, 2)).abs().sum((0, 1, 2))
+        assert ((got[1 + i].cpu().double() - want[1 + i]).abs() <= 2.0 ** -18 * size + 2.0 ** -25).all()
+    assert (got[0].cpu().double() - want[0]).norm() <= 2 * ref.U[dt] * want[0].norm()
+
+
+@pytest.mark.gpu
+def test_a_row_of_zeros_with_an_eps_whose_inverse_overflows():
+    import co_alibi_attn
+    x = torch.zeros(1, 2, 3, 64, dtype=bf16, device="cuda", requires_grad=True)
+    q, _, _ = co_alibi_attn.norm_rotate_qkv(x, 1, 1, eps=1e-39)
+    d, = torch.autograd.grad(q, x, torch.full_like(q, 2.0 ** -20))
+    want = 2.0 ** -20 * float(torch.tensor(1e-39, dtype=torch.float32).double()) ** -0.5  # 1 / sqrt(eps): about 2^65
+    assert ((d[:, :, 0].double() - want).abs() <= 2 * ref.U[bf16] * want).all() and (d[:, :, 1:] == 0).all()
