@@ -49,7 +49,18 @@ __device__ __forceinline__ float quant_scale(float most) {
 }
 
 // ---------------------------------------------------------------------------
-// Append.
+// Append.  Of each block of 16 tokens and head, y the new tokens' values (keys turned by their angles, each product
+// and sum rounded to float32 by itself):
+//   s = max(the least 2^k, k >= -100, with max |y| <= 448 2^k; the scale of tokens that the block holds already),
+//   code = e4m3(y / s), and where s grew, old codes = e4m3(old code * (old s / s)).
+//
+// Bound by the bytes where tokens are many (2 read for 1 written) and by the launch where they are few.  A
+// warp has a block of one head, so that the largest value is a reduction of the warp and no block is written by two.  Its
+// 16 rows stay in registers in 16 bits and are turned twice, for the largest and for the codes: in float32 they took
+// twice the registers and half the warps (8 ragged prompts of up to 2000 tokens 62 us, 53 so, as keys, values and blocks also became CTAs of
+// their own, whose warps share the angles).  Queries go on beside them or, where they are many, in a launch of
+// their own.  Of those 53 us (the bytes take 38) the keys and values of 8 heads of 128 take 19 and the queries of 32
+// heads 36, side by side at their ends; one token for each of 256 requests takes 6.3 us.
 // ---------------------------------------------------------------------------
 struct Append8Params : AppendParams {
   float* k_scales;
@@ -277,8 +288,13 @@ __global__ void __launch_bounds__(kAppendThreads, 4) coalibi_paged_append8_kerne
 }
 
 // ---------------------------------------------------------------------------
-// Read back: tokens at given positions of each request in 16 bits.  A value past the type's
-// largest (its code rounded up) is that largest.
+// Read back: tokens at given positions of each request in 16 bits, code times scale, rounded once.  A value past
+// the type's largest (its code rounded up) is that largest.
+//
+// Bound by the bytes (1 read, 2 written).  A thread takes 16 columns of a token, looks the token up once and goes over
+// heads, eight rows of codes on their way; stores of 32 bytes fill whole sectors, where two of 16 left each half
+// written until the next (4 prefixes of 16,384 tokens of 8 heads of 128 84 us, 68 so, 0.90 of
+// the measured copy rate).
 // ---------------------------------------------------------------------------
 struct Read8Params {
   const void* k_pages;
@@ -308,7 +324,6 @@ __device__ __forceinline__ void store32(void* to, const uint32_t* y) {
                : "memory");
 }
 
-// A thread takes 16 columns of a token, looks the token up once and goes over heads.
 template <bool BF16, int D>
 __global__ void __launch_bounds__(kReadThreads, 4) coalibi_paged_read8_kernel(const Read8Params p) {
   constexpr int PIECES = D / 16, TOKENS = kReadThreads / PIECES;
@@ -399,6 +414,12 @@ __global__ void __launch_bounds__(kReadThreads, 4) coalibi_paged_read8_kernel(co
 // ldmatrix bytewise: a 16-byte chunk of 8 keys gives a lane 4 neighbouring codes of a key,
 // which are the two halves of an A fragment when Q's columns are taken in the same order; transposed, it
 // gives 2 keys x 2 columns, and the columns of a pair go to rows g and g + 8 of the tile.
+//
+// What bounds it.  With 4 rows to a kv head, 4 contexts of 65,537 to 131,071 keys take 127 us, 0.99 of the measured copy
+// rate: memory.  16 contexts of up to 8191 keys take 28 us and 4.4 of joining against 20.6 of reading: the starts and
+// ends of the items.  With 16 and 32 rows the instructions bound it (56 and 79 us where 8 rows take 35): a score costs a
+// row the same whatever the codes' width is, so 8 bits gain little over 16 there.
+// 16 or 32 rows are two blocks of columns of a warp, or of two warps that share the ring.
 // ---------------------------------------------------------------------------
 struct Paged8Params : PagedAttnParams {
   const float* k_scales;

@@ -13,6 +13,10 @@
 // are in the order that makes those 8 consecutive keys (column 8 j + 2 q + e is key 8 q + 2 j + e), so that a row's suffix sum is
 // additions in a lane and one scan over four, and a lane's keys have one scale.  With a row to a thread (four warps a group)
 // the 32 keys of a step took a thread 2750 clocks, most of them its own latencies.
+//
+// Neither memory nor the tensor cores bound it but the softmax warps and the chain of a step: 8 trees of 16 tokens over
+// 127 to 16,383 keys (64 rows to a kv head) take 73 us and 5 of joining, where the bytes take 21; twice the rows take
+// 129 in all.  The warp-level products of few rows took 144 for the same trees.
 #pragma once
 
 #include "paged8.cuh"
