@@ -10,9 +10,14 @@
 #include <ATen/ops/zeros_like.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <optional>
+#include <stdexcept>
 #include <string>
 
 #include "coalibi.h"
@@ -159,22 +164,28 @@ void check_cache(const char* what, const Tensor& k, const Tensor& v, const Tenso
 }
 
 // An index tensor of the given shape (one or two dimensions), contiguous.
-Tensor indices(PyObject* o, const char* what, const char* name, at::IntArrayRef shape, at::ScalarType dtype,
+Tensor indices(const Tensor& t, const char* what, const char* name, at::IntArrayRef shape, at::ScalarType dtype,
                c10::Device device) {
-  const Tensor& t = tensor(o, what, name);
   if (t.scalar_type() != dtype)
     refuse(PyExc_TypeError, what, name, " must be ", c10::toString(dtype), ", got ", c10::toString(t.scalar_type()));
   if (t.sizes() != shape) refuse(PyExc_ValueError, what, name, " must have shape ", shape_of(shape), ", got ", shape_of(t));
   on(what, name, t, device);
   return t.contiguous();
 }
+Tensor indices(PyObject* o, const char* what, const char* name, at::IntArrayRef shape, at::ScalarType dtype,
+               c10::Device device) {
+  return indices(tensor(o, what, name), what, name, shape, dtype, device);
+}
 
-// The rotary tables (cos, sin), contiguous and aligned.
-void rotary_of(PyObject* o, const char* what, int64_t D, c10::Device device, Tensor& cos, Tensor& sin) {
+void rotary_of(PyObject* o, const char* what, Tensor& cos, Tensor& sin) {
   if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2)
     refuse(PyExc_TypeError, what, "rotary must be a tuple (cos, sin)");
   cos = tensor(PyTuple_GET_ITEM(o, 0), what, "cos");
   sin = tensor(PyTuple_GET_ITEM(o, 1), what, "sin");
+}
+
+// The rotary tables, made contiguous and aligned.
+void check_rotary(const char* what, int64_t D, c10::Device device, Tensor& cos, Tensor& sin) {
   if (cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat)
     refuse(PyExc_TypeError, what, "the rotary tables must be float32");
   if (cos.dim() != 2 || sin.sizes() != cos.sizes() || cos.size(0) == 0 || cos.size(0) > 0x7fffffff ||
@@ -249,7 +260,8 @@ PyObject* append_paged_kv(PyObject* const* a) {
     p.positions = positions.data_ptr<int>();
   }
   if (a[8] != Py_None) {
-    rotary_of(a[8], what, D, device, cos, sin);
+    rotary_of(a[8], what, cos, sin);
+    check_rotary(what, D, device, cos, sin);
     p.cos = cos.data_ptr<float>();
     p.sin = sin.data_ptr<float>();
     p.n_pos = (int)cos.size(0);
@@ -402,25 +414,26 @@ PyObject* read_paged_kv(PyObject* const* a) {
   return pair;
 }
 
-// What the forward and the backward of the heads take alike, and the tensors it points at.
+// The arguments of the heads' forward; its backward takes them too.
+struct HeadsIn {
+  Tensor qkv, weight[2], cos, sin, start, positions, status;  // undefined: not given
+  int64_t Hq, Hkv;
+  double eps;
+  bool interleaved;
+};
+
+// What a call of the C entries needs, and the tensors it points at.
 struct Heads {
   CoalibiHeadsArgs p{};
   Tensor qkv, weight[2], cos, sin, start, positions;
   int64_t B, S, Hq, Hkv, D;
 };
 
-int64_t whole(PyObject* o) {
-  const long long v = PyLong_AsLongLong(o);
-  if (v == -1 && PyErr_Occurred()) throw Refused{nullptr, ""};
-  return v;
-}
-
-// a: qkv, num_heads, num_kv_heads, q_weight, k_weight, eps, rotary, start, positions, interleaved, status
-Heads heads_of(PyObject* const* a) {
+Heads check_heads(const HeadsIn& a) {
   const char* what = "norm_rotate_qkv";
   Heads h;
-  const Tensor& x = tensor(a[0], what, "qkv");
-  h.Hq = whole(a[1]), h.Hkv = whole(a[2]);
+  const Tensor& x = a.qkv;
+  h.Hq = a.Hq, h.Hkv = a.Hkv;
   if (x.dim() != 4) refuse(PyExc_ValueError, what, "qkv must be [B, S, num_heads + 2 num_kv_heads, D], got ", shape_of(x));
   h.B = x.size(0), h.S = x.size(1), h.D = x.size(3);
   if (h.Hq <= 0 || h.Hkv <= 0 || h.Hq > 65535 || h.Hkv > 65535 || x.size(2) != h.Hq + 2 * h.Hkv)
@@ -438,8 +451,8 @@ Heads heads_of(PyObject* const* a) {
   at::ScalarType type = x.scalar_type();
   bool seen = false;
   for (int i = 0; i < 2; ++i) {
-    if (a[3 + i] == Py_None) continue;
-    const Tensor& w = tensor(a[3 + i], what, names[i]);
+    const Tensor& w = a.weight[i];
+    if (!w.defined()) continue;
     if ((w.scalar_type() != x.scalar_type() && w.scalar_type() != at::kFloat) || (seen && w.scalar_type() != type))
       refuse(PyExc_TypeError, what, "the weights must both be ", c10::toString(x.scalar_type()), " or float32, got ", c10::toString(w.scalar_type()));
     if (w.dim() != 1 || w.size(0) != h.D) refuse(PyExc_ValueError, what, names[i], " must have shape [", h.D, "], got ", shape_of(w));
@@ -451,53 +464,35 @@ Heads heads_of(PyObject* const* a) {
   if (seen && type == at::kFloat) p.weight_dtype = COALIBI_F32;
   p.q_weight = h.weight[0].defined() ? h.weight[0].data_ptr() : nullptr;
   p.k_weight = h.weight[1].defined() ? h.weight[1].data_ptr() : nullptr;
-  const double eps = PyFloat_AsDouble(a[5]);
-  if (eps == -1.0 && PyErr_Occurred()) throw Refused{nullptr, ""};
-  if (!(eps >= 0)) refuse(PyExc_ValueError, what, "eps must not be negative");
-  p.eps = (float)eps;
-  if (a[6] != Py_None) {
-    rotary_of(a[6], what, h.D, device, h.cos, h.sin);
-    no_grad(what, "cos", h.cos), no_grad(what, "sin", h.sin);
+  if (!(a.eps >= 0)) refuse(PyExc_ValueError, what, "eps must not be negative");
+  p.eps = (float)a.eps;
+  if (a.cos.defined()) {
+    h.cos = a.cos, h.sin = a.sin;
+    check_rotary(what, h.D, device, h.cos, h.sin);
     p.cos = h.cos.data_ptr<float>();
     p.sin = h.sin.data_ptr<float>();
     p.n_pos = (int)h.cos.size(0);
     p.rot = 2 * (int)h.cos.size(1);
   }
-  if (a[7] != Py_None) {
-    h.start = indices(a[7], what, "start", {h.B}, at::kInt, device);
+  if (a.start.defined()) {
+    h.start = indices(a.start, what, "start", {h.B}, at::kInt, device);
     p.start = h.start.data_ptr<int>();
   }
-  if (a[8] != Py_None) {
-    h.positions = indices(a[8], what, "positions", {h.B, h.S}, at::kInt, device);
+  if (a.positions.defined()) {
+    h.positions = indices(a.positions, what, "positions", {h.B, h.S}, at::kInt, device);
     p.positions = h.positions.data_ptr<int>();
   }
-  const int truth = PyObject_IsTrue(a[9]);
-  if (truth < 0) throw Refused{nullptr, ""};
-  p.interleaved = truth;
-  p.status = static_cast<int*>(status_ptr(a[10], what));
+  p.interleaved = a.interleaved;
+  p.status = static_cast<int*>(a.status.data_ptr());
   p.qkv = h.qkv.data_ptr();
   p.B = (int)h.B, p.S = (int)h.S, p.Hq = (int)h.Hq, p.Hkv = (int)h.Hkv, p.D = (int)h.D;
   return h;
 }
 
-PyObject* triple(const Tensor& x, const Tensor& y, const Tensor& z) {
-  PyObject* t = PyTuple_New(3);
-  if (t == nullptr) return nullptr;
-  const Tensor* of[3] = {&x, &y, &z};
-  for (int i = 0; i < 3; ++i) {
-    if (of[i]->defined()) {
-      PyTuple_SET_ITEM(t, i, THPVariable_Wrap(*of[i]));
-    } else {
-      Py_INCREF(Py_None);
-      PyTuple_SET_ITEM(t, i, Py_None);
-    }
-  }
-  return t;
-}
+using torch::autograd::variable_list;
 
-// (the eleven of heads_of) -> (q, k, v)
-PyObject* heads_fwd(PyObject* const* a) {
-  Heads h = heads_of(a);
+variable_list heads_forward(const HeadsIn& a) {
+  Heads h = check_heads(a);
   CoalibiHeadsArgs& p = h.p;
   Tensor q = at::empty({h.B, h.Hq, h.S, h.D}, h.qkv.options()), k = at::empty({h.B, h.Hkv, h.S, h.D}, h.qkv.options());
   Tensor v = at::empty_like(k);
@@ -508,30 +503,32 @@ PyObject* heads_fwd(PyObject* const* a) {
     strides(q, p.q_stride), strides(k, p.k_stride), strides(v, p.v_stride);
     check(coalibi_heads_fwd(&p, stream_of(h.qkv.device())), "coalibi_heads_fwd");
   }
-  return triple(q, k, v);
+  return {q, k, v};
 }
 
-// (the eleven of heads_of, dq, dk, dv) -> (dqkv, dq_weight or None, dk_weight or None)
-PyObject* heads_bwd(PyObject* const* a) {
+// (dqkv, the weights' gradients where there are weights)
+variable_list heads_backward(const HeadsIn& a, const variable_list& grads) {
   const char* what = "norm_rotate_qkv's backward";
-  Heads h = heads_of(a);
+  Heads h = check_heads(a);
   CoalibiHeadsArgs& p = h.p;
   Tensor d[3];
   const char* names[3] = {"the gradient of q", "the gradient of k", "the gradient of v"};
   for (int i = 0; i < 3; ++i) {
-    const Tensor& t = tensor(a[11 + i], what, names[i]);
+    const Tensor& t = grads[i];
     const int64_t H = i ? h.Hkv : h.Hq;
     if (t.sizes() != at::IntArrayRef{h.B, H, h.S, h.D} || t.scalar_type() != h.qkv.scalar_type())
       refuse(PyExc_ValueError, what, names[i], " has shape ", shape_of(t), " and type ", c10::toString(t.scalar_type()));
     on(what, names[i], t, h.qkv.device());
-    d[i] = aligned_rows(t.detach());
+    d[i] = rows16(t) ? t : aligned_rows(t.detach());
   }
-  Tensor dqkv = at::empty({h.B, h.S, h.Hq + 2 * h.Hkv, h.D}, h.qkv.options()), dw[2];
+  const auto options = h.qkv.options().requires_grad(false);
+  Tensor dqkv = at::empty({h.B, h.S, h.Hq + 2 * h.Hkv, h.D}, options), dw[2];
   for (int i = 0; i < 2; ++i)
-    if (h.weight[i].defined()) dw[i] = h.qkv.numel() > 0 ? at::empty_like(h.weight[i]) : at::zeros_like(h.weight[i]);
+    if (h.weight[i].defined())
+      dw[i] = h.qkv.numel() > 0 ? at::empty({h.D}, h.weight[i].options().requires_grad(false)) : at::zeros_like(h.weight[i].detach());
   if (h.qkv.numel() > 0) {
     const size_t bytes = coalibi_heads_bwd_workspace_bytes((int)h.Hq, (int)h.Hkv, (int)h.D);
-    const Tensor ws = at::empty({(int64_t)bytes}, h.qkv.options().dtype(at::kByte));
+    const Tensor ws = at::empty({(int64_t)bytes}, options.dtype(at::kByte));
     p.q = d[0].data_ptr();
     p.k = d[1].data_ptr();
     p.v = d[2].data_ptr();
@@ -541,7 +538,78 @@ PyObject* heads_bwd(PyObject* const* a) {
     p.dk_weight = dw[1].defined() ? dw[1].data_ptr() : nullptr;
     check(coalibi_heads_bwd(&p, ws.data_ptr(), bytes, stream_of(h.qkv.device())), "coalibi_heads_bwd");
   }
-  return triple(dqkv, dw[0], dw[1]);
+  return {dqkv, dw[0], dw[1]};
+}
+
+// The heads in a graph.  The backward runs in the engine's thread without the interpreter's lock, so nothing of it
+// is a Python object (through torch.autograd.Function forward and backward of 650 tokens took the host 160 us, 130 so; a
+// single product and its gradient take 50).
+struct HeadsGrad : torch::autograd::Function<HeadsGrad> {
+  using Context = torch::autograd::AutogradContext;
+  using Weight = std::optional<Tensor>;
+
+  static variable_list forward(Context* ctx, const Tensor& qkv, const Weight& q_weight, const Weight& k_weight, const HeadsIn* a) {
+    variable_list out = heads_forward(*a);
+    ctx->save_for_backward({qkv, a->weight[0], a->weight[1], a->cos, a->sin, a->start, a->positions});
+    ctx->saved_data["status"] = a->status;  // (not saved as a variable: it is written to)
+    ctx->saved_data["heads"] = std::vector<int64_t>{a->Hq, a->Hkv, a->interleaved};
+    ctx->saved_data["eps"] = a->eps;
+    return out;
+  }
+
+  static variable_list backward(Context* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const auto heads = ctx->saved_data["heads"].toIntVector();
+    const HeadsIn a{s[0], {s[1], s[2]}, s[3], s[4], s[5], s[6], ctx->saved_data["status"].toTensor(),
+                    heads[0], heads[1], ctx->saved_data["eps"].toDouble(), heads[2] != 0};
+    variable_list d;
+    try {
+      d = heads_backward(a, grads);
+    } catch (const Refused& r) {
+      throw std::runtime_error(r.text);
+    }
+    if (c10::GradMode::is_enabled()) {  // no second derivative: an error where one is asked for
+      for (Tensor& t : d)
+        if (t.defined()) t.set_requires_grad(true);
+      d = (*std::make_shared<torch::autograd::DelayedError>("co_alibi_attn: norm_rotate_qkv has no second derivative", 3))(std::move(d));
+    }
+    return {d[0], d[1], d[2], Tensor()};
+  }
+};
+
+int64_t whole(PyObject* o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw Refused{nullptr, ""};
+  return v;
+}
+
+// (qkv, num_heads, num_kv_heads, q_weight, k_weight, eps, rotary, start, positions, interleaved, status) -> (q, k, v)
+PyObject* norm_rotate_qkv(PyObject* const* a) {
+  const char* what = "norm_rotate_qkv";
+  HeadsIn in;
+  const auto given = [what](PyObject* o, const char* name) { return o == Py_None ? Tensor() : tensor(o, what, name); };
+  in.qkv = tensor(a[0], what, "qkv");
+  in.Hq = whole(a[1]), in.Hkv = whole(a[2]);
+  in.weight[0] = given(a[3], "q_weight"), in.weight[1] = given(a[4], "k_weight");
+  in.eps = PyFloat_AsDouble(a[5]);
+  if (in.eps == -1.0 && PyErr_Occurred()) throw Refused{nullptr, ""};
+  if (a[6] != Py_None) {
+    rotary_of(a[6], what, in.cos, in.sin);
+    no_grad(what, "cos", in.cos), no_grad(what, "sin", in.sin);
+  }
+  in.start = given(a[7], "start"), in.positions = given(a[8], "positions");
+  const int truth = PyObject_IsTrue(a[9]);
+  if (truth < 0) throw Refused{nullptr, ""};
+  in.interleaved = truth;
+  in.status = tensor(a[10], what, "status");
+  bool graph = false;
+  for (const Tensor& t : {in.qkv, in.weight[0], in.weight[1]}) graph |= t.defined() && t.requires_grad();
+  const auto weight = [&in](int i) { return in.weight[i].defined() ? HeadsGrad::Weight(in.weight[i]) : HeadsGrad::Weight(); };
+  const variable_list out = graph && c10::GradMode::is_enabled() ? HeadsGrad::apply(in.qkv, weight(0), weight(1), &in) : heads_forward(in);
+  PyObject* t = PyTuple_New(3);
+  if (t == nullptr) return nullptr;
+  for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(out[i]));
+  return t;
 }
 
 // A sampling parameter: a number, or a tensor [B] (kept alive in `keep`).
@@ -618,6 +686,8 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return F(args);
   } catch (const Refused& r) {
     if (r.type != nullptr) PyErr_SetString(r.type, r.text.c_str());
+  } catch (python_error& e) {  // of a hook on saved tensors
+    e.restore();
   } catch (const c10::Error& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
   } catch (const std::exception& e) {
@@ -631,7 +701,7 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
 #define METHOD(name, n) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(append_paged_kv, 13), METHOD(paged_tree_attention, 10), METHOD(sample_tokens, 6),
-                         METHOD(read_paged_kv, 7), METHOD(heads_fwd, 11), METHOD(heads_bwd, 14),
+                         METHOD(read_paged_kv, 7), METHOD(norm_rotate_qkv, 11),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serving", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

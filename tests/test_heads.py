@@ -11,6 +11,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from tests import _quant_ref as qr
 from tests import _serving_ref as ref
@@ -363,3 +364,35 @@ def test_a_row_of_zeros_with_an_eps_whose_inverse_overflows():
     d, = torch.autograd.grad(q, x, torch.full_like(q, 2.0 ** -20))
     want = 2.0 ** -20 * float(torch.tensor(1e-39, dtype=torch.float32).double()) ** -0.5  # 1 / sqrt(eps): about 2^65
     assert ((d[:, :, 0].double() - want).abs() <= 2 * ref.U[bf16] * want).all() and (d[:, :, 1:] == 0).all()
+
+
+@pytest.mark.gpu
+def test_a_backward_that_cannot_run_raises():
+    """In the engine's own thread: a saved input written to in between, a graph used twice, a second derivative."""
+    import co_alibi_attn
+    qkv, weights, grads, rotary, kw, _ = _inputs((2, 5, 3, 1, 64, f16, f16, 32, False, "start"), 31)
+    x, w = qkv.cuda().requires_grad_(), [t.cuda().requires_grad_() for t in weights]
+    kw, grads = {k: t.cuda() for k, t in kw.items()}, [t.cuda() for t in grads]
+    f = lambda: co_alibi_attn.norm_rotate_qkv(x, 3, 1, *w, rotary=_cuda(rotary), **kw)  # noqa: E731
+    out = f()
+    want = torch.autograd.grad(out, [x, *w], grads)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, x, grads)
+    out = f()
+    kw["start"].add_(1)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, x, grads)
+    kw["start"].sub_(1)
+    out = f()
+    assert co_alibi_attn.device_status(reset=True) == 0  # (resets the status word between the two)
+    first = torch.autograd.grad(out, [x, *w], grads, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, want))
+    with pytest.raises(RuntimeError, match="second derivative"):
+        first[0].float().square().sum().backward()
+    # under saved-tensor hooks, and again with the forward computed anew
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        out = f()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, [x, *w], grads), want))
+    out = torch.utils.checkpoint.checkpoint(lambda *a: co_alibi_attn.norm_rotate_qkv(a[0], 3, 1, *a[1:], rotary=_cuda(rotary), **kw), x, *w,
+                                            use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, [x, *w], grads), want))
