@@ -89,7 +89,9 @@ bool rows16(const Tensor& t) {
          (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
 }
 
-Tensor aligned_rows(const Tensor& t) { return rows16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+// (a call of torch costs a microsecond or more: none where nothing is to be done)
+Tensor aligned_rows(const Tensor& t) { return rows16(t) ? t : t.detach().clone(at::MemoryFormat::Contiguous); }
+Tensor empty_as(const Tensor& t) { return t.is_contiguous() ? at::empty(t.sizes(), t.options()) : at::empty_like(t); }
 
 // The scales of a cache in 8 bits.
 struct Scales {
@@ -241,8 +243,8 @@ PyObject* append_paged_kv(PyObject* const* a) {
       refuse(PyExc_ValueError, what, "q must be [", B, ", Hq, ", S, ", ", D, "], got ", shape_of(q));
     on(what, "q", q, device);
     no_grad(what, "q", q);
-    q = aligned_rows(q.detach());
-    q_out = at::empty_like(q);
+    q = aligned_rows(q);
+    q_out = empty_as(q);
     p.Hq = (int)q.size(1);
     p.q = q.data_ptr();
     p.q_out = q_out.data_ptr();
@@ -342,8 +344,8 @@ PyObject* paged_tree_attention(PyObject* const* a) {
     if (s == -1.0 && PyErr_Occurred()) return nullptr;
     p.sm_scale = (float)s;
   }
-  const Tensor q = aligned_rows(q0.detach()), slopes = slopes0.contiguous();
-  Tensor o = at::empty_like(q);
+  const Tensor q = aligned_rows(q0), slopes = slopes0.contiguous();
+  Tensor o = empty_as(q);
   if (q.numel() > 0) {
     const size_t bytes = (scales.given ? coalibi_paged_attention8_workspace_bytes : coalibi_paged_attention_workspace_bytes)(
         (int)B, (int)Hq, (int)Hkv, (int)Sq, (int)D);
@@ -389,7 +391,7 @@ PyObject* read_paged_kv(PyObject* const* a) {
   const int64_t Hkv = kp.size(1), D = kp.size(3);
   if (S > 0x7fffffff) refuse(PyExc_ValueError, what, "too many tokens");
   const Tensor positions = indices(a[3], what, "positions", {B, S}, at::kInt, device);
-  Tensor k = at::empty({B, Hkv, S, D}, kp.options().dtype(dtype)), v = at::empty_like(k);
+  Tensor k = at::empty({B, Hkv, S, D}, kp.options().dtype(dtype)), v = empty_as(k);
   if (k.numel() > 0) {
     CoalibiPagedReadArgs p{};
     p.k_pages = kp.data_ptr();
@@ -445,7 +447,7 @@ Heads check_heads(const HeadsIn& a) {
   if (h.B > 0x7fffffff || h.S > 0x7fffffff || h.B * h.S > 0x7fffffff) refuse(PyExc_ValueError, what, "too many tokens");
   const auto device = x.device();
   if (!device.is_cuda()) refuse(PyExc_ValueError, what, "qkv is on ", device.str());
-  h.qkv = rows16(x) ? x : aligned_rows(x.detach());
+  h.qkv = aligned_rows(x);
   strides(h.qkv, p.qkv_stride);
   const char* names[2] = {"q_weight", "k_weight"};
   at::ScalarType type = x.scalar_type();
@@ -495,7 +497,7 @@ variable_list heads_forward(const HeadsIn& a) {
   Heads h = check_heads(a);
   CoalibiHeadsArgs& p = h.p;
   Tensor q = at::empty({h.B, h.Hq, h.S, h.D}, h.qkv.options()), k = at::empty({h.B, h.Hkv, h.S, h.D}, h.qkv.options());
-  Tensor v = at::empty_like(k);
+  Tensor v = empty_as(k);
   if (h.qkv.numel() > 0) {
     p.q = q.data_ptr();
     p.k = k.data_ptr();
@@ -519,7 +521,7 @@ variable_list heads_backward(const HeadsIn& a, const variable_list& grads) {
     if (t.sizes() != at::IntArrayRef{h.B, H, h.S, h.D} || t.scalar_type() != h.qkv.scalar_type())
       refuse(PyExc_ValueError, what, names[i], " has shape ", shape_of(t), " and type ", c10::toString(t.scalar_type()));
     on(what, names[i], t, h.qkv.device());
-    d[i] = rows16(t) ? t : aligned_rows(t.detach());
+    d[i] = aligned_rows(t);
   }
   const auto options = h.qkv.options().requires_grad(false);
   Tensor dqkv = at::empty({h.B, h.S, h.Hq + 2 * h.Hkv, h.D}, options), dw[2];
