@@ -5,7 +5,7 @@
 // the functions and their arguments; these take all of them by position.
 #include <Python.h>
 
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros_like.h>
 #include <c10/core/GradMode.h>
@@ -91,7 +91,10 @@ bool rows16(const Tensor& t) {
 
 // (a call of torch costs a microsecond or more: none where nothing is to be done)
 Tensor aligned_rows(const Tensor& t) { return rows16(t) ? t : t.detach().clone(at::MemoryFormat::Contiguous); }
-Tensor empty_as(const Tensor& t) { return t.is_contiguous() ? at::empty(t.sizes(), t.options()) : at::empty_like(t); }
+Tensor empty(at::IntArrayRef sizes, at::ScalarType dtype, c10::Device device) {
+  return at::detail::empty_cuda(sizes, dtype, device, std::nullopt);  // (at::empty without its two dispatches)
+}
+Tensor empty_as(const Tensor& t) { return t.is_contiguous() ? empty(t.sizes(), t.scalar_type(), t.device()) : at::empty_like(t); }
 
 // The scales of a cache in 8 bits.
 struct Scales {
@@ -349,7 +352,7 @@ PyObject* paged_tree_attention(PyObject* const* a) {
   if (q.numel() > 0) {
     const size_t bytes = (scales.given ? coalibi_paged_attention8_workspace_bytes : coalibi_paged_attention_workspace_bytes)(
         (int)B, (int)Hq, (int)Hkv, (int)Sq, (int)D);
-    const Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    const Tensor ws = empty({(int64_t)bytes}, at::kByte, device);
     p.q = q.data_ptr();
     p.o = o.data_ptr();
     p.k_pages = kp.data_ptr();
@@ -391,7 +394,7 @@ PyObject* read_paged_kv(PyObject* const* a) {
   const int64_t Hkv = kp.size(1), D = kp.size(3);
   if (S > 0x7fffffff) refuse(PyExc_ValueError, what, "too many tokens");
   const Tensor positions = indices(a[3], what, "positions", {B, S}, at::kInt, device);
-  Tensor k = at::empty({B, Hkv, S, D}, kp.options().dtype(dtype)), v = empty_as(k);
+  Tensor k = empty({B, Hkv, S, D}, dtype, device), v = empty_as(k);
   if (k.numel() > 0) {
     CoalibiPagedReadArgs p{};
     p.k_pages = kp.data_ptr();
@@ -496,14 +499,16 @@ using torch::autograd::variable_list;
 variable_list heads_forward(const HeadsIn& a) {
   Heads h = check_heads(a);
   CoalibiHeadsArgs& p = h.p;
-  Tensor q = at::empty({h.B, h.Hq, h.S, h.D}, h.qkv.options()), k = at::empty({h.B, h.Hkv, h.S, h.D}, h.qkv.options());
+  const auto device = h.qkv.device();
+  const auto dtype = h.qkv.scalar_type();
+  Tensor q = empty({h.B, h.Hq, h.S, h.D}, dtype, device), k = empty({h.B, h.Hkv, h.S, h.D}, dtype, device);
   Tensor v = empty_as(k);
   if (h.qkv.numel() > 0) {
     p.q = q.data_ptr();
     p.k = k.data_ptr();
     p.v = v.data_ptr();
     strides(q, p.q_stride), strides(k, p.k_stride), strides(v, p.v_stride);
-    check(coalibi_heads_fwd(&p, stream_of(h.qkv.device())), "coalibi_heads_fwd");
+    check(coalibi_heads_fwd(&p, stream_of(device)), "coalibi_heads_fwd");
   }
   return {q, k, v};
 }
@@ -513,6 +518,7 @@ variable_list heads_backward(const HeadsIn& a, const variable_list& grads) {
   const char* what = "norm_rotate_qkv's backward";
   Heads h = check_heads(a);
   CoalibiHeadsArgs& p = h.p;
+  const auto device = h.qkv.device();
   Tensor d[3];
   const char* names[3] = {"the gradient of q", "the gradient of k", "the gradient of v"};
   for (int i = 0; i < 3; ++i) {
@@ -520,17 +526,16 @@ variable_list heads_backward(const HeadsIn& a, const variable_list& grads) {
     const int64_t H = i ? h.Hkv : h.Hq;
     if (t.sizes() != at::IntArrayRef{h.B, H, h.S, h.D} || t.scalar_type() != h.qkv.scalar_type())
       refuse(PyExc_ValueError, what, names[i], " has shape ", shape_of(t), " and type ", c10::toString(t.scalar_type()));
-    on(what, names[i], t, h.qkv.device());
+    on(what, names[i], t, device);
     d[i] = aligned_rows(t);
   }
-  const auto options = h.qkv.options().requires_grad(false);
-  Tensor dqkv = at::empty({h.B, h.S, h.Hq + 2 * h.Hkv, h.D}, options), dw[2];
+  Tensor dqkv = empty({h.B, h.S, h.Hq + 2 * h.Hkv, h.D}, h.qkv.scalar_type(), device), dw[2];
   for (int i = 0; i < 2; ++i)
     if (h.weight[i].defined())
-      dw[i] = h.qkv.numel() > 0 ? at::empty({h.D}, h.weight[i].options().requires_grad(false)) : at::zeros_like(h.weight[i].detach());
+      dw[i] = h.qkv.numel() > 0 ? empty({h.D}, h.weight[i].scalar_type(), device) : at::zeros_like(h.weight[i].detach());
   if (h.qkv.numel() > 0) {
     const size_t bytes = coalibi_heads_bwd_workspace_bytes((int)h.Hq, (int)h.Hkv, (int)h.D);
-    const Tensor ws = at::empty({(int64_t)bytes}, options.dtype(at::kByte));
+    const Tensor ws = empty({(int64_t)bytes}, at::kByte, device);
     p.q = d[0].data_ptr();
     p.k = d[1].data_ptr();
     p.v = d[2].data_ptr();
@@ -538,7 +543,7 @@ variable_list heads_backward(const HeadsIn& a, const variable_list& grads) {
     p.dqkv = dqkv.data_ptr();
     p.dq_weight = dw[0].defined() ? dw[0].data_ptr() : nullptr;
     p.dk_weight = dw[1].defined() ? dw[1].data_ptr() : nullptr;
-    check(coalibi_heads_bwd(&p, ws.data_ptr(), bytes, stream_of(h.qkv.device())), "coalibi_heads_bwd");
+    check(coalibi_heads_bwd(&p, ws.data_ptr(), bytes, stream_of(device)), "coalibi_heads_bwd");
   }
   return {dqkv, dw[0], dw[1]};
 }
@@ -654,8 +659,8 @@ PyObject* sample_tokens(PyObject* const* a) {
     refuse(PyExc_ValueError, what, "the vocabulary must have 1 to 2**21 tokens, got ", V);
   const Tensor logits = logits0.stride(1) == 1 || V == 1 ? logits0.detach() : logits0.detach().contiguous();
   const Tensor noise = noise0.stride(1) == 1 || V == 1 ? noise0.detach() : noise0.detach().contiguous();
-  Tensor tokens = at::empty({B}, logits.options().dtype(at::kLong));
-  Tensor logprobs = at::empty({B}, logits.options().dtype(at::kFloat));
+  Tensor tokens = empty({B}, at::kLong, device);
+  Tensor logprobs = empty({B}, at::kFloat, device);
   Tensor keep[4];
   p.temperature = per_row<float>(a[2], "temperature", B, at::kFloat, device, keep[0], &p.temperature_all);
   p.top_k = per_row<int>(a[3], "top_k", B, at::kInt, device, keep[1], &p.top_k_all);
