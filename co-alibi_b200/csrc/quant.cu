@@ -184,8 +184,9 @@ extern "C" int coalibi_paged_append8(const CoalibiPagedAppendArgs* a, const Coal
   auto kernel = a->D == 128 ? (bf16 ? append8_kernel<true, 128>(turn) : append8_kernel<false, 128>(turn))
                             : (bf16 ? append8_kernel<true, 64>(turn) : append8_kernel<false, 64>(turn));
   // The queries of few tokens go in the same launch; those of many in one of their own (the 16-bit append's kernel
-  // without keys), whose CTAs take a third of the registers.
-  const bool apart = q_ctas > 0 && p.group > 1;
+  // without keys), whose CTAs take half the registers.  8 kv and 32 query heads of 128, together / apart: 1000 tokens
+  // 14 / 17 us, 4000 30 / 32, 8000 51 / 48, 16,000 92 / 81.
+  const bool apart = q_ctas > 0 && p.tokens >= 40LL * device_sm_count();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = launch_pdl(kernel, dim3((unsigned)(p.kv_ctas + (apart ? 0 : q_ctas))), dim3(threads), 0, s, p);
   if (e == cudaSuccess && apart) {
@@ -234,7 +235,9 @@ extern "C" int coalibi_paged_read8(const CoalibiPagedReadArgs* a, const CoalibiC
   p.table_stride = a->table_stride;
   p.Hkv = a->Hkv;
   p.S = a->S;
-  // all heads to a CTA where tokens are plenty, else fewer, so that every SM has some
+  // All heads to a CTA where tokens are plenty, so that they are looked up once, else fewer, so that every SM has
+  // some.  8 heads of 128, all / one to a CTA: 144 tokens 10 / 6 us, 2000 10 / 10 (four to a CTA 8), 16,000 23 / 35,
+  // 65,536 72 / 123.
   p.per = 2 * a->Hkv;
   while (p.per > 1 && (long long)a->B * p.chunks * (2 * a->Hkv / p.per) < 2LL * device_sm_count()) p.per = (p.per + 1) / 2;
   p.page_size = a->page_size;

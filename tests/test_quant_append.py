@@ -399,3 +399,24 @@ def test_refusals():
     versions = [t._version for t in (cache["k_pages"], cache["v_pages"], *cache["scales"])]
     append_paged_kv(**cache, **calls[0][1])
     assert all(t._version > v for t, v in zip((cache["k_pages"], cache["v_pages"], *cache["scales"]), versions))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S", [(1, 1), (3, 801), (3, 1975)])  # a token to a CTA, two, and queries in a launch of their own
+@pytest.mark.parametrize("rot,interleaved", [(0, False), (32, True), (64, False)])
+def test_queries_are_those_of_the_16_bit_append(B, S, rot, interleaved):
+    import co_alibi_attn
+    D, Hkv, Hq, page, dt = 64, 1, 3, 16, bf16
+    q, k, v = (t.cuda() for t in _new(B, Hq, Hkv, S, D, dt, 41))
+    width = -(-S // page)
+    table = torch.arange(B * width, dtype=torch.int32, device="cuda").view(B, width)
+    start, count = torch.zeros(B, dtype=torch.int32, device="cuda"), torch.tensor([S, S // 2, 0][:B], dtype=torch.int32, device="cuda")
+    rotary = tuple(t.cuda() for t in _tables(S, rot)) if rot else None
+    pool = torch.zeros(B * width, Hkv, page, D, dtype=dt, device="cuda")
+    codes = [qr.e4m3(torch.zeros(pool.shape, dtype=torch.uint8, device="cuda")) for _ in range(2)]
+    scales = tuple(torch.ones(B * width, Hkv, 1, device="cuda") for _ in range(2))
+    for more in (dict(rotary=rotary, interleaved=interleaved), dict()):
+        want = co_alibi_attn.append_paged_kv(k, v, pool, pool.clone(), table, start, count=count, q=q if more.get("rotary") else None, **more)
+        got = co_alibi_attn.append_paged_kv(k, v, *codes, table, start, count=count, q=q if more.get("rotary") else None, scales=scales, **more)
+        assert (want is None and got is None) or torch.equal(want, got)
+    assert co_alibi_attn.device_status(reset=True) == 0
