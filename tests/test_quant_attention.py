@@ -300,3 +300,44 @@ def test_refusals_of_the_c_entry():
     assert need > 0 and code(ws=None) == 8 and code(ws=264) == 8 and code(bytes_=need - 1) == 8
     for bad in ((2, 4, 2, 65, 128), (2, 4, 3, 1, 128), (2, 4, 2, 1, 80), (0, 4, 2, 1, 64)):
         assert lib.coalibi_paged_attention8_workspace_bytes(*bad) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [32, 64, 48])  # whole steps of 32 keys in a page, or not
+@pytest.mark.parametrize("form", [f for f in FORMS if f[0] // f[1] * f[2] <= 32], ids=[i for i, f in zip(IDS, FORMS) if f[0] // f[1] * f[2] <= 32])
+def test_stale_halves_of_steps(form, page):
+    """Split items, one step to a load: codes and scales of NaN behind the last token, drafts of NaN that some rows see,
+    pages outside the pool."""
+    import co_alibi_attn
+    Hq, Hkv, Sq, D, dt = form
+    ctx = [0, 3, 16, 17, 31, 32, 47, 100, 480, 1011, 1500, 2222]
+    kc, vc, ks, vs, table = qr.pool([c + Sq for c in ctx], Hkv, D, page, 80)
+    words = [ref.tree(Sq, 81 + b) for b in range(len(ctx))]
+    q, slopes = _q(len(ctx), Hq, Sq, D, dt, 82), _slopes(Hq)(dt)
+    lost = {7: 100 // page - 1, 9: 0, 10: 7, 11: 2222 // page - 1}  # whole pages of the context
+    t2, short, ctx2 = table.clone(), torch.full_like(table, -1), list(ctx)
+    for b in range(len(ctx)):
+        keep = [n for n in range(table.shape[1]) if n != lost.get(b)]
+        if b in lost:
+            t2[b, lost[b]] = -1 if b % 2 else 1 << 30
+            ctx2[b] -= page
+        short[b, :len(keep)] = table[b, keep]
+    want, bound = qr.attention(q, kc, vc, ks, vs, short, ctx2, words, slopes, 1 / math.sqrt(D))
+    t = 1 if Sq < 5 else 4
+    for b, c in enumerate(ctx):
+        vc[table[b, (c + t) // page], :, (c + t) % page, 3:5] = 0xff
+        end = c + Sq
+        last = table[b, (end - 1) // page]
+        if end % page:
+            kc[last, :, end % page:] = vc[last, :, end % page:] = 0x7f
+            ks[last, :, -(-(end % page) // 16):] = vs[last, :, -(-(end % page) // 16):] = math.nan
+    wide = torch.full((len(ctx), -(-16384 // page)), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = t2
+    o = _run(q, kc, vc, ks, vs, wide, ctx, words)
+    assert co_alibi_attn.device_status(reset=True) == 11
+    for b in range(len(ctx)):
+        for i in range(Sq):
+            if words[b][i] >> t & 1:
+                assert o[b, :, i, 3:5].isnan().all(), (b, i)
+                o[b, :, i, 3:5] = want[b, :, i, 3:5].to(o)
+    _check(o, want, bound)
