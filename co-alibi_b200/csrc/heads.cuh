@@ -11,7 +11,7 @@
 // with the token's angles in registers and the kind's weights in shared memory; the sums of a weight's gradient are a
 // lane's own until the end.  With 8 columns to a lane, whose partners another lane had, forward and backward of 32,768
 // tokens of 36 heads of 64 took 320 us, 157 with 16 and 128 with the ring of copies (below), where the bytes
-// take 115; 32,764 tokens of 48 heads of 128 take 316 where the bytes take 306.
+// take 115; 32,764 tokens of 48 heads of 128 take 315 where the bytes take 306.
 #pragma once
 
 #include "sm100.cuh"
