@@ -415,8 +415,9 @@ __global__ void __launch_bounds__(kReadThreads, 4) coalibi_paged_read8_kernel(co
 // which are the two halves of an A fragment when Q's columns are taken in the same order; transposed, it
 // gives 2 keys x 2 columns, and the columns of a pair go to rows g and g + 8 of the tile.
 //
-// What bounds it.  With 4 rows to a kv head, 4 contexts of 65,537 to 131,071 keys take 127 us, 0.99 of the measured copy
-// rate: memory.  16 contexts of up to 8191 keys take 28 us and 4.4 of joining against 20.6 of reading: the starts and
+// What bounds it.  With 4 rows to a kv head, 4 contexts of 65,537 to 131,071 keys take 124 us, all of the measured copy
+// rate: memory (132 with the joining under the power cap, whose clock makes the instructions count).  16 contexts of up
+// to 8191 keys take 28 us and 4.4 of joining against 20.6 of reading: the starts and
 // ends of the items.  With 16 and 32 rows the instructions bound it (56 and 79 us where 8 rows take 35): a score costs a
 // row the same whatever the codes' width is, so 8 bits gain little over 16 there.
 // 16 or 32 rows are two blocks of columns of a warp, or of two warps that share the ring.
@@ -475,7 +476,10 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return make_float2(
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); }
 
-template <int D, bool BF16, int NT, int RW, int WARPS>
+// HALF: at most 4 rows.  The product leaves half of the lanes with columns of no row, so those lanes (tig 2 and 3) take
+// the second rows of the others: a lane has one row of its 4 keys, in .x, and .y is dead.  The long contexts above took
+// 127 us without it, and 143 with the joining under the power cap.
+template <int D, bool BF16, int NT, int RW, int WARPS, bool HALF>
 __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::CTAS))
     coalibi_paged8_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                                const Paged8Params p) {
@@ -491,6 +495,9 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
   __shared__ float4 s_stat[KG > 1 ? KG * L::ROWS : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gq = lane >> 2, tig = lane & 3;
+  static_assert(!HALF || (NT == 1 && RW == 1), "four rows fit one block of columns");
+  const int my_row = HALF ? 2 * (tig & 1) + (tig >> 1) : 2 * tig;  // in a block of columns
+  auto other = [](float x) { return __shfl_xor_sync(0xffffffffu, x, 2); };
   const int rwarp = warp % RW, kg = warp / RW;
   const bool issuer = rwarp == 0 && lane == 0;  // of the group's loads
   const int G = p.Hq / p.Hkv, rows = G * p.Sq;
@@ -675,10 +682,10 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
             const float2 u = unpack2<true>(qb[n][kk][e]);
             qb[n][kk][e] = pack2<false>(u.x * f, u.y * f);
           }
-        unit[n].x *= __shfl_sync(0xffffffffu, down, 8 * tig);
-        unit[n].y *= __shfl_sync(0xffffffffu, down, 8 * tig + 4);
+        unit[n].x *= __shfl_sync(0xffffffffu, down, 4 * my_row);
+        if (!HALF) unit[n].y *= __shfl_sync(0xffffffffu, down, 4 * my_row + 4);
       }
-      const int ra = min(r0 + 8 * n + 2 * tig, rows - 1), rb = min(ra + 1, rows - 1);
+      const int ra = min(r0 + 8 * n + my_row, rows - 1), rb = min(ra + 1, rows - 1);
       slope2[n] = make_float2(load_slope(p.slopes, p.slopes_dtype, g * G + ra / p.Sq) * kLog2e,
                               load_slope(p.slopes, p.slopes_dtype, g * G + rb / p.Sq) * kLog2e);
     }
@@ -737,8 +744,8 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
       if (!all) {
         vis = 0;
 #pragma unroll 1
-        for (int i = 0; i < 2 * NT; ++i) {
-          const int r = r0 + 8 * (i >> 1) + 2 * tig + (i & 1), row = r < rows ? r % p.Sq : 0;
+        for (int i = 0; i < (HALF ? 1 : 2 * NT); ++i) {
+          const int r = r0 + 8 * (i >> 1) + my_row + (i & 1), row = r < rows ? r % p.Sq : 0;
           const unsigned long long word =
               p.tree_mask != nullptr ? (unsigned long long)p.tree_mask[b * p.mask_stride + row] : (2ull << row) - 1;
 #pragma unroll
@@ -762,7 +769,12 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
           const float2 f = mul2(unit[n], make_float2(k_scale, k_scale));
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            v[n][c] = mul2(make_float2(sc[c >> 1][n][2 * (c & 1)], sc[c >> 1][n][2 * (c & 1) + 1]), f);
+            float2 d = make_float2(sc[c >> 1][n][2 * (c & 1)], sc[c >> 1][n][2 * (c & 1) + 1]);
+            if (HALF) {
+              const float y = other(d.y);
+              d = make_float2(tig < 2 ? d.x : y, 0.f);
+            }
+            v[n][c] = mul2(d, f);
             const float2 e = add2(make_float2(ex2_approx(-v[n][c].x), ex2_approx(-v[n][c].y)), make_float2(1.f, 1.f));
             s[c] = make_float2(rcp_approx(e.x), rcp_approx(e.y));
             if (MASKED) {
@@ -777,7 +789,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
           float2 inc = s[0];
 #pragma unroll
           for (int d = 4; d <= 16; d <<= 1) {
-            const float2 y = make_float2(__shfl_down_sync(0xffffffffu, inc.x, d), __shfl_down_sync(0xffffffffu, inc.y, d));
+            const float2 y = make_float2(__shfl_down_sync(0xffffffffu, inc.x, d), HALF ? 0.f : __shfl_down_sync(0xffffffffu, inc.y, d));
             if (lane + d < 32) inc = add2(inc, y);
           }
           const float2 wrapped = turn == 0 ? make_float2(0.f, 0.f) : turn == 1 ? s[3] : turn == 2 ? s[2] : s[1];
@@ -785,7 +797,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
           const float2 last = make_float2(carry[n].x + (right.x - wrapped.x), carry[n].y + (right.y - wrapped.y));
           const float2 first = add2(last, s[0]);
           carry[n].x += __shfl_sync(0xffffffffu, inc.x, tig);
-          carry[n].y += __shfl_sync(0xffffffffu, inc.y, tig);
+          if (!HALF) carry[n].y += __shfl_sync(0xffffffffu, inc.y, tig);
           mx[n] = make_float2(-INFINITY, -INFINITY);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -806,22 +818,22 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             mx[n].x = fmaxf(mx[n].x, __shfl_xor_sync(0xffffffffu, mx[n].x, d));
-            mx[n].y = fmaxf(mx[n].y, __shfl_xor_sync(0xffffffffu, mx[n].y, d));
+            if (!HALF) mx[n].y = fmaxf(mx[n].y, __shfl_xor_sync(0xffffffffu, mx[n].y, d));
           }
         }
         // the newest keys weigh most, so the maximum seldom moves after the first steps
         bool up = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) up |= mx[n].x > m_run[n].x || mx[n].y > m_run[n].y;
+        for (int n = 0; n < NT; ++n) up |= mx[n].x > m_run[n].x || (!HALF && mx[n].y > m_run[n].y);
         if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const float2 m = make_float2(fmaxf(m_run[n].x, mx[n].x), fmaxf(m_run[n].y, mx[n].y));
             const float fx = m_run[n].x == -INFINITY ? 0.f : ex2_approx(m_run[n].x - m.x);
-            const float fy = m_run[n].y == -INFINITY ? 0.f : ex2_approx(m_run[n].y - m.y);
+            const float fy = HALF ? other(fx) : m_run[n].y == -INFINITY ? 0.f : ex2_approx(m_run[n].y - m.y);
             m_run[n] = m;
             l_part[n].x *= fx;
-            l_part[n].y *= fy;
+            if (!HALF) l_part[n].y *= fy;
 #pragma unroll
             for (int dm = 0; dm < KK; ++dm) {
               o[dm][n][0] *= fx, o[dm][n][2] *= fx;
@@ -842,8 +854,20 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
               w.x = vis >> (8 * n + c) & 1 ? w.x : 0.f;
               w.y = vis >> (8 * n + 4 + c) & 1 ? w.y : 0.f;
             }
+            if (HALF) w.y = 0.f;
             l2 = add2(l2, w);
-            pb[n][c] = pack2<false>(w.x, w.y);
+            if (HALF)
+              v[n][c].x = w.x;
+            else
+              pb[n][c] = pack2<false>(w.x, w.y);
+          }
+          if (HALF) {  // both rows of a column pair again
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+              const uint32_t mine = pack2<false>(v[n][c].x, v[n][c + 1].x), theirs = __shfl_xor_sync(0xffffffffu, mine, 2);
+              pb[n][c] = __byte_perm(mine, theirs, 0x5410);
+              pb[n][c + 1] = __byte_perm(mine, theirs, 0x7632);
+            }
           }
           // the weights themselves: without the block's scale
           if (MASKED && l2.x == 0.f && l2.y == 0.f) continue;
@@ -858,6 +882,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
       // them, 0 * NaN is not 0.  A drafted token's V that has codes of NaN must not reach the rows that do not
       // see it either: it is added by hand, then zeroed.
       if (!all) {
+        if (HALF) vis = (vis & 15u) | __shfl_xor_sync(0xffffffffu, vis & 15u, 2) << 4;
         const int key = kb + lane;
         uint8_t* vrow = ring + slot * 2 * L::TILE + L::TILE + lane * D;
         const bool used = !(gone >> (lane >> 4) & 1) && key < hi && (key < ctx || (seen_by_any >> (key - ctx) & 1));
@@ -935,8 +960,9 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
 #pragma unroll
       for (int d = 4; d <= 16; d <<= 1) {
         l_part[n].x += __shfl_xor_sync(0xffffffffu, l_part[n].x, d);
-        l_part[n].y += __shfl_xor_sync(0xffffffffu, l_part[n].y, d);
+        if (!HALF) l_part[n].y += __shfl_xor_sync(0xffffffffu, l_part[n].y, d);
       }
+    if (HALF) carry[0].y = other(carry[0].x), m_run[0].y = other(m_run[0].x), l_part[0].y = other(l_part[0].x), slope2[0].y = other(slope2[0].x);
 
     // ---- the piece's result: the output if the item is whole, else a record
     const bool whole = u0 == 0 && u1 == units;

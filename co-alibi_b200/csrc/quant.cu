@@ -50,7 +50,7 @@ auto queries_kernel(int turn) {
                               : coalibi_paged_append_kernel<BF16, D, kTurnHalves>;
 }
 
-template <int D, bool BF16, int NT, int RW, int WARPS>
+template <int D, bool BF16, int NT, int RW, int WARPS, bool HALF>
 int launch_attention8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, int sms, cudaStream_t s) {
   static std::atomic<unsigned long long> ready{0};
   using L = Paged8Layout<D, NT, RW, WARPS>;
@@ -63,7 +63,7 @@ int launch_attention8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params
       return launch_pdl(coalibi_paged8_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, rows), dim3(kJoinThreads), 0, s, a);
     return launch_pdl(coalibi_paged_join_kernel<D, BF16, L>, dim3(p.B * p.Hkv, (rows + 3) / 4), dim3(128), 0, s, a);
   };
-  return launch_paged<L>(coalibi_paged8_attn_kernel<D, BF16, NT, RW, WARPS>, join, ready, 32 * WARPS, tk, tv, p, sms, s);
+  return launch_paged<L>(coalibi_paged8_attn_kernel<D, BF16, NT, RW, WARPS, HALF>, join, ready, 32 * WARPS, tk, tv, p, sms, s);
 }
 
 // Four warps to an item where the tables hold little work, else as many as its rows take (as in the
@@ -72,10 +72,10 @@ bool shares_items(const Paged8Params& p, int sms) {
   const long long items = (long long)p.B * p.Hkv, width = (long long)p.max_pages * p.page_size;
   return !(items > 2LL * sms || (width > 512 && items * width > 32768));
 }
-template <int D, bool BF16, int NT, int RW>
+template <int D, bool BF16, int NT, int RW, bool HALF = false>
 int launch_rows8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, int sms, cudaStream_t s) {
-  return shares_items(p, sms) ? launch_attention8<D, BF16, NT, RW, 4>(tk, tv, p, sms, s)
-                              : launch_attention8<D, BF16, NT, RW, RW>(tk, tv, p, sms, s);
+  return shares_items(p, sms) ? launch_attention8<D, BF16, NT, RW, 4, HALF>(tk, tv, p, sms, s)
+                              : launch_attention8<D, BF16, NT, RW, RW, HALF>(tk, tv, p, sms, s);
 }
 
 template <int D, bool BF16>
@@ -92,9 +92,11 @@ int launch_wide8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, 
 template <int D, bool BF16>
 int launch_paged8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, int sms, cudaStream_t s) {
   const int rows = p.Hq / p.Hkv * p.Sq;
-  // The wide kernel costs the same for 1 to 64 rows.  8 ragged contexts up to 16k keys, narrow / wide: 16 rows 62 /
+  // Up to 4 rows lanes share what 8 columns leave over (4 rows of long contexts, without / with it: 143 / 132 us; the
+  // shuffles it takes would buy nothing with more rows).  The wide kernel costs the same for 1 to 64 rows.  8 ragged contexts up to 16k keys, narrow / wide: 16 rows 62 /
   // 67 us, 20 rows 81 / 79, 32 rows 87 / 79; 32 rows of 64 contexts of 200 keys 36 / 65, of 1000 keys 97 / 104;
   // 32 rows of D = 64 65 / 79.
+  if (rows <= 4) return launch_rows8<D, BF16, 1, 1, true>(tk, tv, p, sms, s);
   if (rows <= 8) return launch_rows8<D, BF16, 1, 1>(tk, tv, p, sms, s);
   if (rows <= 16) return launch_rows8<D, BF16, 2, 1>(tk, tv, p, sms, s);
   if (rows <= 32) return launch_rows8<D, BF16, 2, 2>(tk, tv, p, sms, s);
