@@ -28,7 +28,8 @@ block of 16 tokens of a page and head.  A value is its code times the scale of i
 value is at most 448 (and at least 2^-100): a code's relative error is at most 2^-4 then, or 2^-10 of the scale, that is
 2^-18 to 2^-17 of the block's largest, for what is smaller.  A block that already holds tokens keeps its scale unless
 a new one is too large for it, and if so the old codes move to the new scale, which changes none but
-those that fall below 2^-6 of it.  Slots behind a request's tokens hold nothing, and those before ``start`` in
+those that fall below 2^-6 of it.  Reading and attention take scales that another program wrote as well: any finite ones, 0
+and negative ones among them (attention's weights of values in blocks below 2^-100 are rounded as those of 2^-100).  Slots behind a request's tokens hold nothing, and those before ``start`` in
 its block hold tokens; as the block's codes may move, no other request writes or reads the block in the same call.
 
 There is no backward: where gradients are enabled, keys, values, queries and pools that

@@ -241,6 +241,7 @@ struct PagedLayout {
   // resident per SM: by shared memory, and by 256 registers a thread
   static constexpr int FIT = 200 * 1024 / BYTES, CTAS = FIT < 256 / THREADS ? FIT : 256 / THREADS;
   static constexpr int RECORD = ROWS * (4 + D);    // floats of one piece: stats, then O
+  static constexpr bool SPREAD_SUMS = false;       // (PieceFactor)
   // the joining of the key groups reuses the ring
   static_assert(16 * RW * D * 4 <= RING, "exchange fits the ring");
 };
@@ -892,6 +893,7 @@ struct WideLayout {
   static constexpr int BYTES = QBYTES + 2 * RING + 1024;
   static constexpr int CTAS = 1;
   static constexpr int RECORD = ROWS * (4 + D);
+  static constexpr bool SPREAD_SUMS = false;
   static constexpr int TM_S = 64, TM_O = 256;      // columns of an S buffer; O of group w at TM_O + w * D
   static constexpr int THREADS = 384;
   // a group's part of the exchange (O in float, then statistics) reuses its ring
@@ -1471,6 +1473,19 @@ __global__ void __launch_bounds__(384, 1)
   }
 }
 
+// The factor 2^a by which a piece with the reference m (a <= 0: m less the largest one) joins others.  In a cache of 8
+// bits the sum of the weights may be up to 2^126 times the piece's largest contribution, so 2^a may flush to 0 where its
+// product with the sum counts: there it is the square of 2^(a / 2).
+template <typename L>
+struct PieceFactor {
+  float half, f;
+  __device__ __forceinline__ explicit PieceFactor(float a) {
+    half = ex2_approx(L::SPREAD_SUMS ? 0.5f * a : a);
+    f = L::SPREAD_SUMS ? half * half : half;
+  }
+  __device__ __forceinline__ float of_sum(float l) const { return L::SPREAD_SUMS ? l * half * half : l * half; }
+};
+
 // Joins the pieces of the items that span runs.  One warp per query row; lanes hold the
 // statistics of up to 32 pieces at a time, rightmost first.
 template <int D, bool BF16, typename L>
@@ -1531,24 +1546,23 @@ __global__ void __launch_bounds__(128) coalibi_paged_join_kernel(const PagedAttn
 #pragma unroll
     for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
     const float m_new = fmaxf(M, mx), m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float fac = M == -INFINITY ? 0.f : ex2_approx(M - m_use);
+    const PieceFactor<L> fac(M == -INFINITY ? -INFINITY : M - m_use), f(m - m_use);
     M = m_new;
-    const float f = ex2_approx(m - m_use);
-    float lw = f * s.z;
+    float lw = f.of_sum(s.z);
 #pragma unroll
     for (int d = 16; d; d >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, d);
-    l = l * fac + lw;
+    l = fac.of_sum(l) + lw;
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] *= fac;
+    for (int v = 0; v < V; ++v) acc[v] *= fac.f;
 #pragma unroll
     for (int j = 0; j < EARLY; ++j) {
-      const float w = __shfl_sync(0xffffffffu, f, j);  // 0 past the last piece
+      const float w = __shfl_sync(0xffffffffu, f.f, j);  // 0 past the last piece
 #pragma unroll
       for (int v = 0; v < V; ++v) acc[v] = fmaf(w, early[j][v], acc[v]);
     }
 #pragma unroll 4
     for (int j = EARLY; j < n; ++j) {
-      const float w = __shfl_sync(0xffffffffu, f, j);
+      const float w = __shfl_sync(0xffffffffu, f.f, j);
       float u[V];
       o_of(j, u);
 #pragma unroll

@@ -19,6 +19,11 @@ namespace coalibi {
 constexpr int kQuantBlock = 16;        // tokens that share a scale
 constexpr float kE4m3Max = 448.f;
 constexpr int kScaleMinExp = -100;     // its inverse is a normal float32 too
+// Scales of V that are 0, negative or far from 1 take the attention's masked steps (below).
+constexpr float kScaleHeldMin = 0x1p-100f, kScaleHeldMax = 0x1p126f;
+__device__ __forceinline__ bool odd_scale(float s) {  // not within [2^-40, 2^40)
+  return __float_as_uint(s) - (87u << 23) >= (80u << 23);
+}
 
 __device__ __forceinline__ uint32_t e4m3_to_f16x2(uint32_t two) {  // the low 16 bits
   uint32_t h;
@@ -407,7 +412,11 @@ __global__ void __launch_bounds__(kReadThreads, 4) coalibi_paged_read8_kernel(co
 // exponent of its weight: the running reference is the largest x_j - slope z_j + log2 c_j, so the largest
 // *contribution* has a weight near 1, whatever the blocks' scales are, and a block whose values are
 // small beside another's is rounded relative to what it adds; the sum of the weights is kept in
-// float32 by the same reference.
+// float32 by the same reference, as sum (w_j c_j) / c_j.
+// A block whose c_j is 0, negative or far from 1 (one of zeros that the append wrote, 2^-100; any that another program
+// wrote) cannot give its weights back by that division.  Its step goes as a masked one, with c~_j = |c_j| held within
+// 2^-100 .. 2^126 in the exponent and the product's weight times c_j / c~_j; what it adds to the sum is (h c~_j^-1/2)^2 with
+// h the root of the weight, which does not flush to 0 where the weight does, and moves to other references by PieceFactor.
 //
 // The keys stand on the rows of the MMA and the queries on its 8 columns (S^T = K Q^T, O^T += V^T P^T):
 // with at most 8 rows that share a key nothing of a product is wasted.  Both operands come out of
@@ -445,6 +454,7 @@ struct Paged8Layout {
   // resident per SM: by shared memory, and by 168 registers a thread
   static constexpr int FIT = 208 * 1024 / BYTES, CTAS = FIT < 384 / THREADS ? FIT : 384 / THREADS;
   static constexpr int RECORD = ROWS * (4 + D);
+  static constexpr bool SPREAD_SUMS = true;
 };
 
 // Order of a step's 32 keys: lane group g (0 .. 7) holds keys 4 g .. 4 g + 3, so a row's suffix sum is
@@ -739,7 +749,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
       }
       // ---- which of this lane's 4 keys each of its rows sees: bit 8 n + 4 x + c
       const uint32_t gone = gone_q >> (2 * slot) & 3;
-      const bool all = kb + kPagedStep <= min(hi, ctx) && gone == 0;
+      const bool all = kb + kPagedStep <= min(hi, ctx) && gone == 0 && !__any_sync(0xffffffffu, odd_scale(v_scale));
       uint32_t vis = 0xffffu;
       if (!all) {
         vis = 0;
@@ -757,10 +767,12 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
       }
       // ---- sigmoids, suffix sums, logits (in log2 units), online softmax; both rows of a column
       // pair as float2
-      const float lv = lg2_approx(v_scale), iv = rcp_approx(v_scale);
       uint32_t pb[NT][4];
       auto softmax = [&](auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
+        const bool odd = MASKED && odd_scale(v_scale);
+        const float held = odd ? fminf(fmaxf(fabsf(v_scale), kScaleHeldMin), kScaleHeldMax) : v_scale;
+        const float lv = lg2_approx(held), iv = rcp_approx(held);
         float2 mx[NT];
         float2 v[NT][4];
 #pragma unroll
@@ -829,11 +841,12 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const float2 m = make_float2(fmaxf(m_run[n].x, mx[n].x), fmaxf(m_run[n].y, mx[n].y));
-            const float fx = m_run[n].x == -INFINITY ? 0.f : ex2_approx(m_run[n].x - m.x);
-            const float fy = HALF ? other(fx) : m_run[n].y == -INFINITY ? 0.f : ex2_approx(m_run[n].y - m.y);
+            const PieceFactor<L> px(m_run[n].x == -INFINITY ? -INFINITY : m_run[n].x - m.x);
+            const PieceFactor<L> py(HALF || m_run[n].y == -INFINITY ? -INFINITY : m_run[n].y - m.y);
+            const float fx = px.f, fy = HALF ? other(fx) : py.f;
             m_run[n] = m;
-            l_part[n].x *= fx;
-            if (!HALF) l_part[n].y *= fy;
+            l_part[n].x = px.of_sum(l_part[n].x);
+            if (!HALF) l_part[n].y = py.of_sum(l_part[n].y);
 #pragma unroll
             for (int dm = 0; dm < KK; ++dm) {
               o[dm][n][0] *= fx, o[dm][n][2] *= fx;
@@ -846,16 +859,25 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
           const float2 off2 = make_float2(lv - (m_run[n].x == -INFINITY ? 0.f : m_run[n].x),
                                           lv - (m_run[n].y == -INFINITY ? 0.f : m_run[n].y));
           float2 l2 = make_float2(0.f, 0.f);
+          const float by = odd ? v_scale * iv : 1.f, root = odd ? ex2_approx(-0.5f * lv) : 1.f;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const float2 x = add2(v[n][c], off2);
-            float2 w = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            float2 w;
+            if (odd) {  // (masked keys: x is -inf, all 0)
+              w = make_float2(ex2_approx(0.5f * x.x), HALF ? 0.f : ex2_approx(0.5f * x.y));
+              const float2 u = mul2(w, make_float2(root, root));
+              l2 = fma2(u, u, l2);
+              w = mul2(mul2(w, w), make_float2(by, by));
+            } else {
+              w = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            }
             if (MASKED) {  // (a block that nothing of is seen may have any scale)
               w.x = vis >> (8 * n + c) & 1 ? w.x : 0.f;
               w.y = vis >> (8 * n + 4 + c) & 1 ? w.y : 0.f;
             }
             if (HALF) w.y = 0.f;
-            l2 = add2(l2, w);
+            if (!odd) l2 = add2(l2, w);
             if (HALF)
               v[n][c].x = w.x;
             else
@@ -870,8 +892,8 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
             }
           }
           // the weights themselves: without the block's scale
-          if (MASKED && l2.x == 0.f && l2.y == 0.f) continue;
-          l_part[n] = fma2(l2, make_float2(iv, iv), l_part[n]);
+          const float un = odd ? 1.f : iv;
+          l_part[n] = fma2(l2, make_float2(un, un), l_part[n]);
         }
       };
       if (all)
@@ -1021,8 +1043,9 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int c = KG - 1; c >= 0; --c) {
-          const float f = ex2_approx(w[c] - m_use);
-          l = fmaf(s_stat[c * L::ROWS + r].z, f, l);
+          const PieceFactor<L> pf(w[c] - m_use);
+          const float f = pf.f;
+          l += pf.of_sum(s_stat[c * L::ROWS + r].z);
           const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + c * L::GROUP) + r * D + d);
           acc.x = fmaf(v.x, f, acc.x);
           acc.y = fmaf(v.y, f, acc.y);
@@ -1128,20 +1151,19 @@ __global__ void __launch_bounds__(kJoinThreads) coalibi_paged8_join_kernel(const
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) m_new = fmaxf(m_new, s_b[w]);
     const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float fac = M == -INFINITY ? 0.f : ex2_approx(M - m_use);
+    const PieceFactor<L> fac(M == -INFINITY ? -INFINITY : M - m_use), f(m - m_use);
     M = m_new;
-    const float f = ex2_approx(m - m_use);
-    s_f[tid] = f;
-    float lw = f * s.z;
+    s_f[tid] = f.f;
+    float lw = f.of_sum(s.z);
 #pragma unroll
     for (int d = 16; d; d >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, d);
     if (lane == 0) s_c[warp] = lw;
     __syncthreads();
-    l *= fac;
+    l = fac.of_sum(l);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) l += s_c[w];
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] *= fac;
+    for (int v = 0; v < V; ++v) acc[v] *= fac.f;
 #pragma unroll
     for (int k = 0; k < EARLY; ++k) {
       const float w = s_f[warp + k * WARPS];  // 0 past the last piece

@@ -40,6 +40,7 @@ struct Wide8Layout {
   static constexpr int BYTES = QBYTES + 2 * GROUP + 1024;
   static constexpr int CTAS = 1;
   static constexpr int RECORD = ROWS * (4 + D);
+  static constexpr bool SPREAD_SUMS = true;
   static constexpr int TM_S = 64, TM_O = 256;      // columns of an S buffer; O of group w at TM_O + w * D
   static constexpr int THREADS = 768;              // warps 0-15 softmax, 16 and 17 MMAs, 18 and 19 loads, 20-23 tiles
   // a group's part of the exchange (O in float, then statistics) reuses its rings
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(768, 1)
   __shared__ uint64_t s_k[2][2], s_k_free[2][2], s_v[2][2], s_v_free[2][2];      // tiles
   __shared__ uint64_t s_scores[2][2], s_probs[2][2], s_meta[2][4], s_pv[2][2], s_idle[2];
   // of a step: the scales of its four blocks of 16 keys; which of them were not loaded (bits 0-3), and 16 where some
-  // key of the step is not of the context
+  // key of the step is not of the context, or a scale of V is one that odd_scale() names
   __shared__ __align__(16) float s_ks[2][kWide8Meta][4];
   __shared__ __align__(16) float s_vs[2][kWide8Meta][4];
   __shared__ unsigned char s_gone[2][kWide8Meta];
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(768, 1)
         vs = p.v_scales[page * p.vss[0] + g * p.vss[1] + at_slot / kQuantBlock];
       }
       const int gone = (int)(__ballot_sync(0xffffffffu, lane < 4 && page < 0) & 15u);
-      const bool plain = gone == 0 && __all_sync(0xffffffffu, inside);
+      const bool plain = gone == 0 && __all_sync(0xffffffffu, inside && !odd_scale(vs));
       const uint32_t dst = smem_u32(codes + slot * 2 * L::CODES), bytes = (4 - __popc(gone)) * 16 * D;
       if (!__all_sync(0xffffffffu, mbar_wait(&s_kc_free[w][slot], ((k / L::NCODE) & 1) ^ 1, guard))) return false;
       if (lane == 0) mbar_expect_tx(&s_kc[w][slot], bytes);
@@ -457,7 +458,8 @@ __global__ void __launch_bounds__(768, 1)
         uint32_t s[16];
         tmem_ld_quads(s_base + 32 * hf, s);
         const float k_scale = s_ks[w][meta][2 * hf + (q >> 1)], v_scale = s_vs[w][meta][2 * hf + (q >> 1)];
-        const float lv = lg2_approx(v_scale), iv = rcp_approx(v_scale);
+        const float held = fminf(fmaxf(fabsf(v_scale), kScaleHeldMin), kScaleHeldMax);  // (v_scale itself, unless odd)
+        const float lv = lg2_approx(held), iv = rcp_approx(held);
         uint32_t seen[2] = {0xffu, 0xffu};  // of this lane's 8 keys
         if (gone != 0) {
           const int base = half_base(n, hf), in = min(half_hi(hf), ctx) - base, end = half_hi(hf) - base;
@@ -534,24 +536,31 @@ __global__ void __launch_bounds__(768, 1)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             if (mx[x] > m[x] + 8.f || (m[x] == -INFINITY && mx[x] > -INFINITY)) {
-              const float f = m[x] == -INFINITY ? 0.f : ex2_approx(m[x] - mx[x]);
+              const PieceFactor<L> f(m[x] - mx[x]);
               rescale |= m[x] != -INFINITY;
-              alpha[x] = m[x] != -INFINITY ? f : 1.f;
-              l[x] *= f;
+              alpha[x] = m[x] != -INFINITY ? f.f : 1.f;
+              l[x] = f.of_sum(l[x]);
               m[x] = mx[x];
             }
-            const float2 sh = splat2(lv - (m[x] == -INFINITY ? 0.f : m[x]));
+            const float ref = m[x] == -INFINITY ? 0.f : m[x];
+            const float2 sh = splat2(lv - ref);
+            const bool odd = MASKED && odd_scale(v_scale);  // (paged8.cuh)
             float2 ls = splat2(0.f);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float2 v = __fadd2_rn(pair(j, x), sh);
               float2 e = make_float2(ex2_approx(v.x), ex2_approx(v.y));
+              if (odd) {  // (exponentials of their own for the sum: the roots, as there, cost the plain steps 1%)
+                const float2 y = pair(j, x);
+                ls = __fadd2_rn(ls, mask(j, x, make_float2(ex2_approx(y.x - ref), ex2_approx(y.y - ref)), 0.f));
+                e = __fmul2_rn(e, splat2(v_scale * iv));
+              }
               if (MASKED) e = mask(j, x, e, 0.f);  // (a block that nothing of is seen may have any scale)
-              ls = __fadd2_rn(ls, e);
+              if (!odd) ls = __fadd2_rn(ls, e);
               pk[2 * j + x] = pack2<false>(e.x, e.y);
             }
             // the weights themselves: without the block's scale
-            if (!MASKED || seen[x] != 0) l[x] = fmaf(ls.x + ls.y, iv, l[x]);
+            l[x] = fmaf(ls.x + ls.y, odd ? 1.f : iv, l[x]);
           }
         };
         if (gone == 0)
@@ -648,8 +657,9 @@ __global__ void __launch_bounds__(768, 1)
       for (int q = L::PIECES - 1; q >= 0; --q) {
         const int lane_row = r + 64 * (q & 1), grp = q >> 1;
         const float* xo = reinterpret_cast<const float*>(smem + L::QBYTES + grp * L::GROUP);
-        const float f = ex2_approx(wt[q] - m_use);
-        l = fmaf(reinterpret_cast<const float4*>(xo + 128 * D)[lane_row].z, f, l);
+        const PieceFactor<L> pf(wt[q] - m_use);
+        const float f = pf.f;
+        l += pf.of_sum(reinterpret_cast<const float4*>(xo + 128 * D)[lane_row].z);
         const float4 v = *reinterpret_cast<const float4*>(xo + lane_row * D + ((ch ^ (lane_row & (D / 4 - 1))) << 2));
         acc.x = fmaf(v.x, f, acc.x);
         acc.y = fmaf(v.y, f, acc.y);

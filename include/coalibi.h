@@ -285,8 +285,9 @@ int coalibi_paged_attention(const CoalibiPagedAttentionArgs* args, void* workspa
                             void* stream);
 
 /* The same cache in 8 bits.  k_pages and v_pages hold e4m3 codes (strides multiples of 16), and each
- * block of 16 tokens of a page and head has a float32 scale, a power of two, at page * stride[0] +
- * head * stride[1] + slot / 16: a value is its code times the scale of its block. */
+ * block of 16 tokens of a page and head has a float32 scale at page * stride[0] + head * stride[1] + slot / 16: a
+ * value is its code times the scale of its block.  The append writes powers of two; reading and attention take
+ * any finite scale. */
 #define COALIBI_QUANT_BLOCK 16
 typedef struct CoalibiCacheScales {
   float* k; /* [n_pages, Hkv, page_size / 16] */
