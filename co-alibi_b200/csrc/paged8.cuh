@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kReadThreads, 4) coalibi_paged_read8_kernel(co
           y[e] = *reinterpret_cast<const uint32_t*>(&v);
         }
       } else {
-        const bool clamps = !(scale[i] <= (BF16 ? 7e35f : 128.f));
+        const bool clamps = !(fabsf(scale[i]) <= (BF16 ? 7e35f : 128.f));
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           float2 u = __fmul2_rn(f16x2_to_float2(y[e]), make_float2(scale[i], scale[i]));

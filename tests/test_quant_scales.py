@@ -60,3 +60,21 @@ def test_keys_of_zero_values_keep_their_weight(form, width):
     slopes, scale = torch.full((Hq,), 0.02), 0.5
     o = _run(q, kc, vc, ks, vs, _widen(table, 4096) if width == "wide" else table, ctx, words, slopes=slopes.cuda(), sm_scale=scale)
     _check(o, *_bounded(q, kc, vc, ks, vs, table, ctx, words, slopes, scale))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [f16, bf16])
+def test_reading_takes_any_scale(dt):
+    """A code times its block's scale, rounded once; past the type's largest, that, of either sign."""
+    import co_alibi_attn
+    Hkv, D, page, n = 3, 64, 48, 200
+    kc, vc, ks, vs, table = qr.pool([n], Hkv, D, page, 94)
+    sizes = torch.tensor([0.0, 1.0, 0.3, 1e-9, 129.0, 7e4, 1e30, 7.1e35, 3e38, 2.0 ** -130])
+    sizes = torch.cat((sizes, -sizes))  # (19 blocks apart: every page and head has others)
+    for i, s in enumerate((ks, vs)):
+        s.copy_(sizes[(torch.arange(s.numel()) * 19 + i) % len(sizes)].view(s.shape))
+    at = torch.arange(n, dtype=torch.int32)[None]
+    got = co_alibi_attn.read_paged_kv(qr.e4m3(kc.cuda()), qr.e4m3(vc.cuda()), table.cuda(), at.cuda(), (ks.cuda(), vs.cuda()), dtype=dt)
+    top = torch.finfo(dt).max
+    for x, c, s in zip(got, (kc, vc), (ks, vs)):
+        assert torch.equal(x[0].cpu(), ref.gather(qr.dequantised(c, s), table, 0, n).clamp(-top, top).to(dt))
