@@ -53,6 +53,22 @@ __device__ __forceinline__ float quant_scale(float most) {
   return __int_as_float((max(e, kScaleMinExp) + 127) << 23);
 }
 
+// For a scale that is no power of two (only another program writes one; a block keeps it where it is large enough): a
+// result in 24 bits towards zero, its last bit set where it is not exact, so that it rounds to a code as the exact one would.
+__device__ __forceinline__ float to_odd(float x, float rest) {  // the exact value is x and something of rest's sign
+  const uint32_t u = __float_as_uint(x), back = ((__float_as_uint(rest) ^ u) >> 31) & 1u;
+  return rest == 0.f ? x : __uint_as_float((u - back) | 1u);
+}
+__device__ __forceinline__ float quotient_to_odd(float y, float s, float inv) {  // s > 0, inv = 1 / s
+  float q = y * inv;
+  q = fmaf(fmaf(-q, s, y), inv, q);
+  return to_odd(q, fmaf(-q, s, y));
+}
+__device__ __forceinline__ float product_to_odd(float a, float b) {
+  const float x = a * b;
+  return to_odd(x, fmaf(a, b, -x));
+}
+
 // ---------------------------------------------------------------------------
 // Append.  Of each block of 16 tokens and head, y the new tokens' values (keys turned by their angles, each product
 // and sum rounded to float32 by itself):
@@ -256,7 +272,10 @@ __global__ void __launch_bounds__(kAppendThreads, 4) coalibi_paged_append8_kerne
       e4m3_to_f16x4(u.y, g[2], g[3]);
       float2 v[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(f16x2_to_float2(g[e]), make_float2(ratio, ratio));
+      for (int e = 0; e < 4; ++e) {
+        const float2 u = f16x2_to_float2(g[e]);
+        v[e] = make_float2(product_to_odd(u.x, ratio), product_to_odd(u.y, ratio));
+      }
       *reinterpret_cast<uint2*>(at_old) =
           make_uint2(e4m3_from(v[0].x, v[0].y, v[1].x, v[1].y), e4m3_from(v[2].x, v[2].y, v[3].x, v[3].y));
     }
@@ -264,31 +283,40 @@ __global__ void __launch_bounds__(kAppendThreads, 4) coalibi_paged_append8_kerne
 #pragma unroll
   for (int i = 0; i < N; ++i)  // (so that nothing of the first pass is kept for the codes)
     asm volatile("" : "+r"(raw[i].x), "+r"(raw[i].y), "+r"(raw[i].z), "+r"(raw[i].w));
+  auto store = [&](auto power_of_two) {
 #pragma unroll
-  for (int i = 0; i < N; ++i, y += step) {
-    const int r = r0 + i * RPW;
-    if (some(i) && r >= lo && r < hi) {
-      float2 f[4];
-      values(i, f);
+    for (int i = 0; i < N; ++i, y += step) {
+      const int r = r0 + i * RPW;
+      if (some(i) && r >= lo && r < hi) {
+        float2 f[4];
+        values(i, f);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (infinite && fabsf(f[e].x) == INFINITY) f[e].x = __int_as_float(0x7fc00000);
-        if (infinite && fabsf(f[e].y) == INFINITY) f[e].y = __int_as_float(0x7fc00000);
-        f[e] = __fmul2_rn(f[e], make_float2(inv, inv));
-      }
-      uint2 codes;
-      if (TURN == kTurnPairs)
-        codes = make_uint2(e4m3_from(f[0].x, f[2].x, f[0].y, f[2].y), e4m3_from(f[1].x, f[3].x, f[1].y, f[3].y));
-      else
-        codes = make_uint2(e4m3_from(f[0].x, f[0].y, f[1].x, f[1].y), e4m3_from(f[2].x, f[2].y, f[3].x, f[3].y));
-      if (split) {
-        *reinterpret_cast<uint32_t*>(y + ca) = codes.x;
-        *reinterpret_cast<uint32_t*>(y + cb) = codes.y;
-      } else {
-        *reinterpret_cast<uint2*>(y + ca) = codes;
+        for (int e = 0; e < 4; ++e) {
+          if (infinite && fabsf(f[e].x) == INFINITY) f[e].x = __int_as_float(0x7fc00000);
+          if (infinite && fabsf(f[e].y) == INFINITY) f[e].y = __int_as_float(0x7fc00000);
+          if (decltype(power_of_two)::value)
+            f[e] = __fmul2_rn(f[e], make_float2(inv, inv));
+          else
+            f[e] = make_float2(quotient_to_odd(f[e].x, scale, inv), quotient_to_odd(f[e].y, scale, inv));
+        }
+        uint2 codes;
+        if (TURN == kTurnPairs)
+          codes = make_uint2(e4m3_from(f[0].x, f[2].x, f[0].y, f[2].y), e4m3_from(f[1].x, f[3].x, f[1].y, f[3].y));
+        else
+          codes = make_uint2(e4m3_from(f[0].x, f[0].y, f[1].x, f[1].y), e4m3_from(f[2].x, f[2].y, f[3].x, f[3].y));
+        if (split) {
+          *reinterpret_cast<uint32_t*>(y + ca) = codes.x;
+          *reinterpret_cast<uint32_t*>(y + cb) = codes.y;
+        } else {
+          *reinterpret_cast<uint2*>(y + ca) = codes;
+        }
       }
     }
-  }
+  };
+  if ((__float_as_uint(scale) & 0x7fffffu) == 0u)
+    store(std::true_type{});
+  else
+    store(std::false_type{});
   if (lane == 0 && scale != was) *scale_at = scale;
 }
 

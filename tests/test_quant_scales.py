@@ -7,6 +7,7 @@ import torch
 
 from tests import _quant_ref as qr
 from tests import _serving_ref as ref
+from tests.test_quant_append import _new, _same, _tables
 from tests.test_quant_attention import FORMS, IDS, _case, _check, _run, _widen
 
 f16, bf16 = torch.float16, torch.bfloat16
@@ -78,3 +79,58 @@ def test_reading_takes_any_scale(dt):
     top = torch.finfo(dt).max
     for x, c, s in zip(got, (kc, vc), (ks, vs)):
         assert torch.equal(x[0].cpu(), ref.gather(qr.dequantised(c, s), table, 0, n).clamp(-top, top).to(dt))
+
+
+@pytest.mark.gpu
+def test_new_tokens_by_a_scale_that_is_no_power_of_two():
+    """A block keeps such a scale where it is large enough, and its new codes are the nearest ones: borders between codes
+    fall to the even one, and what lies off them by less than a float32 quotient tells, to its own side."""
+    import co_alibi_attn
+    D, Hkv = 64, 4
+    border = (qr.GRID[1:] + qr.GRID[:-1])[7:].div(2).float()  # (5 bits each)
+    scales = torch.tensor([k / 32 for k in range(33, 64)] + [0.7, 1 / 3, 3e-5, 1.1e4])
+    S, pages = 15, len(scales)
+    x = torch.empty(pages, Hkv, S, D)
+    for p, s in enumerate(scales):
+        y = (border * s)[border * s < 60000]
+        x[p] = y[torch.arange(x[p].numel()) % len(y)].view(x[p].shape)
+    x = (x * (1 - 2 * (torch.arange(S) % 2))[None, None, :, None])
+    codes = torch.randint(0, 127, (pages, Hkv, 16, D), dtype=torch.uint8, generator=torch.Generator().manual_seed(96))
+    was = scales[:, None, None].expand(pages, Hkv, 1).contiguous()
+    table = torch.arange(pages, dtype=torch.int32)[:, None]
+    for dt in (f16, bf16):  # a border times k / 32 is a float16; the rest are what they round to
+        new = x.to(dt)
+        want = codes.clone(), was.clone()
+        qr.append(new, *want, table, [1] * pages, [S] * pages)
+        kd, vd, ks, vs = qr.e4m3(codes.cuda()), qr.e4m3(codes.cuda()), was.cuda(), was.cuda()
+        co_alibi_attn.append_paged_kv(new.cuda(), new.cuda(), kd, vd, table.cuda(), torch.ones(pages, dtype=torch.int32).cuda(), scales=(ks, vs))
+        assert torch.equal(ks.cpu(), want[1]) and torch.equal(vs.cpu(), want[1])
+        assert _same(kd.view(torch.uint8), want[0]) and _same(vd.view(torch.uint8), want[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,dt,rot", [(64, f16, 0), (128, bf16, 64)])
+def test_old_tokens_move_from_any_scale(D, dt, rot):
+    """Codes under a smaller scale that is no power of two, 0 or negative go to the new one with one rounding of the exact
+    product; larger scales stay, rotated keys among the new ones."""
+    import co_alibi_attn
+    Hkv, S, B = 3, 6, 40
+    g = torch.Generator().manual_seed(97)
+    kc, vc, ks, vs, table = qr.pool([30] * B, Hkv, D, 32, 98)
+    for s in (ks, vs):
+        s.copy_(torch.tensor([1 / 448, 1.5 / 512, 0.0, -0.01, 1e-9, 0.3, 1.75, 1.0, 123.4, 2e-38])[torch.randint(0, 10, s.shape, generator=g)]
+                * (1 + torch.rand(s.shape, generator=g) * (torch.rand(s.shape, generator=g) < 0.5)))
+    start = [5 + b % 17 for b in range(B)]
+    q, k, v = _new(B, 4, Hkv, S, D, dt, 99)
+    rotary, k_in = None, k.double()
+    if rot:
+        cos, sin = _tables(60, rot)
+        at = torch.tensor(start)[:, None] + torch.arange(S)
+        k_in, rotary = qr.rotated32(k, cos[at][:, None], sin[at][:, None], False), (cos.cuda(), sin.cuda())
+    want = [x.clone() for x in (kc, vc, ks, vs)]
+    qr.append(k_in, want[0], want[2], table, start, [S] * B)
+    qr.append(v, want[1], want[3], table, start, [S] * B)
+    kd, vd, ksd, vsd = qr.e4m3(kc.cuda()), qr.e4m3(vc.cuda()), ks.cuda(), vs.cuda()
+    co_alibi_attn.append_paged_kv(k.cuda(), v.cuda(), kd, vd, table.cuda(), torch.tensor(start, dtype=torch.int32).cuda(), rotary=rotary, scales=(ksd, vsd))
+    assert torch.equal(ksd.cpu(), want[2]) and torch.equal(vsd.cpu(), want[3])
+    assert _same(kd.view(torch.uint8), want[0]) and _same(vd.view(torch.uint8), want[1])
