@@ -135,9 +135,10 @@ def read_paged_kv(k_pages, v_pages, page_table, positions, scales, dtype=torch.b
 
     ``positions`` int32 [B, S]: which tokens of each request, in any order, the same one as often
     as asked for; a negative one gives a row of zeros, and so does one without a page, which is
-    reported.  Values are rounded once (bfloat16 holds every one whose scale is a power of two whole);
-    one past the type's largest is that.  What is read and appended again, with a scale not below
-    its block's, gets the same codes."""
+    reported.  Values are rounded once; one past the type's largest is that.  What the append wrote is
+    whole in bfloat16 (up to its largest), and in float16 under scales from 2^-15 to 2^7.  A token that is read whole and
+    appended again has the same values, and under a scale as large as its old one the same codes; a larger scale rounds
+    it like any other."""
     assert k_pages.is_cuda, "Inputs must be CUDA tensors"
     if dtype not in _READ_DTYPES:
         raise TypeError(f"co_alibi_attn: read_paged_kv: dtype must be float16 or bfloat16, got {dtype}")

@@ -38,7 +38,6 @@ class PagedCache:
         shape = (batch * per, cfg.n_head, page_size, cfg.d_model // cfg.n_head)
         self.k = [torch.empty(shape, dtype=kv_dtype, device=weight.device) for _ in range(cfg.n_layer)]
         self.v = [torch.empty_like(k) for k in self.k]
-        self.dtype = weight.dtype
         self.scales = None
         if kv_dtype == torch.float8_e4m3fn:
             blocks = (*shape[:2], page_size // QUANT_BLOCK)
@@ -80,7 +79,8 @@ class PagedCache:
             if self.scales is None:
                 new = (x[page, :, slot].transpose(1, 2) for x in (k, v))
             else:
-                new = read_paged_kv(k, v, self.table, at, self.scales[layer], dtype=self.dtype)
+                # (bfloat16, whatever the model's type: float16 does not hold small codes whole)
+                new = read_paged_kv(k, v, self.table, at, self.scales[layer], dtype=torch.bfloat16)
             append_paged_kv(*new, k, v, self.table, self.lens, count=count, **self.of(layer))
 
 
