@@ -23,7 +23,8 @@ def norm_rotate_qkv(qkv, num_heads, num_kv_heads, q_weight=None, k_weight=None, 
     moved as they are.  Arithmetic is float32, rounded once.
 
     Gradients reach ``qkv`` and the weights (the weights' sums are float32, added in a fixed order: results
-    repeat bit for bit); tables that require one are refused, and there is no second derivative.  A
+    repeat bit for bit); tables that require one are refused, and there is neither a second
+    derivative nor a forward-mode one (tangents are refused).  A
     backward that is captured in a CUDA graph takes leaves (or detached copies) of which no eager graph lives: the leaf's
     accumulation belongs to the stream of the first."""
     assert qkv.is_cuda, "Inputs must be CUDA tensors"

@@ -33,7 +33,7 @@ and negative ones among them (attention's weights of values in blocks below 2^-1
 its block hold tokens; as the block's codes may move, no other request writes or reads the block in the same call.
 
 There is no backward: where gradients are enabled, keys, values, queries and pools that
-require one are refused (call under ``torch.no_grad()``), and log-probabilities of sampled
+require one are refused (call under ``torch.no_grad()``), forward-mode tangents of theirs too, and log-probabilities of sampled
 tokens carry none.  Appending counts as an in-place write of the pools for autograd.
 """
 import torch

@@ -8,6 +8,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros_like.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -64,8 +65,15 @@ void on(const char* what, const char* name, const Tensor& t, c10::Device device)
   if (t.device() != device) refuse(PyExc_ValueError, what, name, " is on ", t.device().str(), ", not ", device.str());
 }
 
+// A result that silently dropped a forward-mode tangent would have a derivative of 0.
+void no_tangent(const char* what, const char* name, const Tensor& t) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined())
+    refuse(PyExc_RuntimeError, what, name, " carries a forward-mode tangent, but there is no forward-mode derivative");
+}
+
 // The operators have no backward: a result that silently dropped its graph would train wrongly.
 void no_grad(const char* what, const char* name, const Tensor& t) {
+  no_tangent(what, name, t);
   if (c10::GradMode::is_enabled() && t.requires_grad())
     refuse(PyExc_RuntimeError, what, name, " requires grad, but there is no backward: call this under torch.no_grad()");
 }
@@ -600,6 +608,9 @@ PyObject* norm_rotate_qkv(PyObject* const* a) {
   in.weight[0] = given(a[3], "q_weight"), in.weight[1] = given(a[4], "k_weight");
   in.eps = PyFloat_AsDouble(a[5]);
   if (in.eps == -1.0 && PyErr_Occurred()) throw Refused{nullptr, ""};
+  no_tangent(what, "qkv", in.qkv);
+  for (int i = 0; i < 2; ++i)
+    if (in.weight[i].defined()) no_tangent(what, i ? "k_weight" : "q_weight", in.weight[i]);
   if (a[6] != Py_None) {
     rotary_of(a[6], what, in.cos, in.sin);
     no_grad(what, "cos", in.cos), no_grad(what, "sin", in.sin);
