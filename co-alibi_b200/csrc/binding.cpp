@@ -399,6 +399,7 @@ PyObject* read_paged_kv(PyObject* const* a) {
   if (kp.dim() == 4 && kp.size(3) != 64 && kp.size(3) != 128) refuse(PyExc_ValueError, what, "head_dim must be 64 or 128, got ", kp.size(3));
   check_cache(what, kp, vp, table, B, kp.dim() == 4 ? kp.size(3) : 0, dtype, device, scales);
   no_grad(what, "k_scales", scales.k), no_grad(what, "v_scales", scales.v);
+  no_grad(what, "k_pages", kp), no_grad(what, "v_pages", vp);
   const int64_t Hkv = kp.size(1), D = kp.size(3);
   if (S > 0x7fffffff) refuse(PyExc_ValueError, what, "too many tokens");
   const Tensor positions = indices(a[3], what, "positions", {B, S}, at::kInt, device);

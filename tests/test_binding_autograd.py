@@ -1,6 +1,6 @@
-"""The operators of the compiled binding have no forward-mode derivative: a dual input is refused, as
-``co_alibi_attention`` refuses it, rather than answered without its tangent.  On the CPU the binding itself, which
-refuses before it looks for a device; on the GPU the calls."""
+"""What the operators of the compiled binding do not differentiate is refused: dual inputs, as ``co_alibi_attention``
+refuses them, rather than answered without their tangent, and pools that require grad.  On the CPU the binding itself,
+which refuses before it looks for a device; on the GPU the calls."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -63,3 +63,24 @@ def test_plain_calls_beside_dual_tensors():
         plain = fwd.unpack_dual(dual).primal
         assert torch.equal(co_alibi_attn.norm_rotate_qkv(plain, 2, 2)[0], co_alibi_attn.norm_rotate_qkv(x.detach(), 2, 2)[0])
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("name", ["k_pages", "v_pages", "k_scales", "v_scales"])
+def test_reading_refuses_what_requires_grad(name, device):
+    """As append and attention do; pools of codes are floating tensors to autograd."""
+    import co_alibi_attn
+    from co_alibi_attn.serving import _native
+    z = lambda *s, dt=torch.int32: torch.zeros(*s, dtype=dt, device=device)  # noqa: E731
+    t = {n: z(3, 2, 16, 64, dt=torch.uint8).view(torch.float8_e4m3fn) for n in ("k_pages", "v_pages")}
+    t.update({n: z(3, 2, 1, dt=torch.float32) for n in ("k_scales", "v_scales")})
+    t[name].requires_grad_()
+    args = t["k_pages"], t["v_pages"], z(2, 1), z(2, 3), (t["k_scales"], t["v_scales"])
+    with pytest.raises(RuntimeError, match="no_grad"):
+        if device == "cuda":
+            co_alibi_attn.read_paged_kv(*args)
+        else:
+            _native().read_paged_kv(*args, True, z(1))
+    if device == "cuda":
+        with torch.no_grad():
+            assert not co_alibi_attn.read_paged_kv(*args)[0].requires_grad
