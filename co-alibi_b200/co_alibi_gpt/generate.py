@@ -151,6 +151,11 @@ def _extend(model, cache, tokens, words=None, depths=None, counts=None):
     x = _embed(model, tokens)
     B, S, C = x.shape
     positions = None if depths is None else cache.lens[:, None] + depths
+    if model.cfg.qk_norm and cache.rotary is not None and counts is not None:
+        # the heads rotate every token: those that counts leaves out by an angle that is there
+        steps = cache.steps[:S]
+        positions = cache.lens[:, None] + steps if positions is None else positions
+        positions = torch.where(steps < counts[:, None], positions, positions.clamp(0, cache.capacity - 1))
     for layer, blk in enumerate(model.blocks):
         where, more = (cache.k[layer], cache.v[layer], cache.table, cache.lens), cache.of(layer)
         if model.cfg.qk_norm:

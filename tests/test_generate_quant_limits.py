@@ -2,7 +2,10 @@
 import pytest
 import torch
 
-from tests.test_generate_quant import E4M3, _cfg, _model
+from tests import _serving_cpu
+from tests import test_generate_limits as limits
+from tests.test_generate_quant import E4M3, _cfg, _model, plain_heads
+from tests.test_gpt import oracle_attention
 from tests.test_quant_append import _tables
 
 
@@ -31,3 +34,71 @@ def test_small_values_of_a_float16_model_move_whole():
     for layer in range(2):
         for got, expect in zip(read(layer, at), want[layer]):
             assert torch.equal(got[0], expect[0]) and torch.equal(got[1, :, :2], expect[1, :, :2])
+
+
+def reporting_heads(qkv, Hq, Hkv, q_weight, k_weight, eps=1e-6, rotary=None, start=None, positions=None):
+    """norm_rotate_qkv in torch operations; a position outside the tables leaves the row as it is and is noted, as the
+    kernel reports it."""
+    plain = plain_heads(qkv, Hq, Hkv, q_weight, k_weight, eps)
+    if rotary is None:
+        return plain
+    at = positions if positions is not None else torch.arange(qkv.shape[1]).expand(qkv.shape[:2]) + (0 if start is None else start[:, None])
+    out = (at < 0) | (at >= rotary[0].shape[0])
+    _serving_cpu.reports.extend(("angle", *w) for w in out.nonzero().tolist())
+    turned = plain_heads(qkv, Hq, Hkv, q_weight, k_weight, eps, rotary, positions=at.masked_fill(out, 0))
+    return tuple(torch.where(out[:, None, :, None], a, b) for a, b in zip(plain[:2], turned[:2])) + (plain[2],)
+
+
+def _normed(device, rotary_dim=0):
+    """Weights by which its first greedy tokens differ from one another, as the tests of drafts take them to."""
+    from co_alibi_gpt import build
+    cfg, kw = _cfg(rotary_dim=rotary_dim, init_std=0.3), dict(dtype=torch.float16)
+    if device == "cpu":
+        kw = dict(dtype=torch.float32, attn_fn=oracle_attention, heads_fn=reporting_heads)
+    model = build(cfg, device, seed=4, **kw)[0].eval()
+    with torch.no_grad():
+        for name, p in model.named_parameters():
+            if name.endswith(("q_norm", "k_norm")):
+                p.fill_(2.0)
+    return model
+
+
+@pytest.mark.parametrize("rotary_dim", [0, 32])
+@pytest.mark.parametrize("device", limits.DEVICES)
+@pytest.mark.parametrize("name", ["test_a_tree_of_siblings_two_tokens_before_the_end", "test_drafts_without_a_slot_are_not_accepted",
+                                  "test_rows_of_a_chunk_past_the_end_have_no_logits", "test_padding_of_minus_one_is_not_looked_up",
+                                  "test_a_model_without_a_token_to_draw_ends_in_minus_one", "test_counts_outside_the_prompt", "test_no_new_tokens",
+                                  "test_a_parent_that_does_not_come_before_its_draft_is_none", "test_an_absent_token_confirms_nothing"])
+def test_limits_of_a_normed_model(name, device, rotary_dim, monkeypatch):
+    test = getattr(limits, name)
+    own = "rotary_dim" in test.__code__.co_varnames[:test.__code__.co_argcount]
+    if name == "test_counts_outside_the_prompt":
+        rotary_dim = 0  # (prompts wider than a cache of rotated keys are refused)
+    monkeypatch.setattr(limits, "_model", lambda device, rotary=None: _normed(device, rotary_dim if rotary is None else rotary))
+    test(device, *((rotary_dim,) if own else ()), monkeypatch)
+
+
+@pytest.mark.parametrize("deep", [False, True])
+@pytest.mark.parametrize("device", limits.DEVICES)
+def test_tokens_that_counts_leaves_out_are_not_reported(device, deep, monkeypatch):
+    """Their positions run past the end of the cache and of the tables; those that enter have their logits."""
+    gen = limits._generate(device, monkeypatch)
+    model = _normed(device, 32)
+    tok = limits._tokens(2, 36, device)
+    cache = gen.PagedCache(model, 2, 32, page_size=16, spare=0)
+    lens = torch.tensor([29, 24], dtype=torch.int32, device=device)
+    gen.prefill(model, cache, tok[:, :30], lens)
+    chunk = torch.stack((tok[0, 29:34], tok[1, 24:29]))
+    steps = torch.arange(5, dtype=torch.int32, device=device)
+    counts = torch.tensor([3, 5], dtype=torch.int32, device=device)
+    words = torch.where(steps < counts[:, None], (2 << steps.long()) - 1, 0)
+    depths = (steps + torch.where(steps < counts[:, None], 0, 1000)).int() if deep else None
+    logits = gen.extend(model, cache, chunk, words, depths, counts)
+    assert limits._status(device) == 0
+    with torch.no_grad():
+        full = model(tok)
+    for got, want in ((logits[0, :3], full[0, 29:32]), (logits[1], full[1, 24:29])):
+        assert (got.float() - want.float()).abs().max() < 0.1
+    # what enters the cache past the tables is reported
+    gen.extend(model, cache, chunk, words, steps.expand(2, 5) + 1000, counts)
+    assert limits._status(device) != 0
