@@ -61,7 +61,10 @@ class PagedCache:
         return self.table.gather(1, (at // size).long()).long(), (at % size).long()
 
     def rows(self, pages, at):
-        """The cached rows of tokens at [B, n] of each request: [B, H, n, D]."""
+        """The cached rows of tokens at [B, n] of each request: [B, H, n, D].  Codes are no rows without their scales:
+        ``read_paged_kv`` gives those of a cache in 8 bits."""
+        if self.scales is not None:
+            raise ValueError("the cache holds 8-bit codes: read_paged_kv gives their values")
         page, slot = self.where(at)
         return pages[page, :, slot].transpose(1, 2)
 

@@ -102,3 +102,13 @@ def test_tokens_that_counts_leaves_out_are_not_reported(device, deep, monkeypatc
     # what enters the cache past the tables is reported
     gen.extend(model, cache, chunk, words, steps.expand(2, 5) + 1000, counts)
     assert limits._status(device) != 0
+
+
+def test_rows_of_codes_are_refused():
+    from co_alibi_gpt.generate import PagedCache
+    model, at = limits._model("cpu"), torch.zeros(2, 3, dtype=torch.int32)
+    cache = PagedCache(model, 2, 20, 16)
+    assert cache.rows(cache.k[0], at).shape == (2, 2, 3, 64)
+    cache = PagedCache(model, 2, 20, 16, kv_dtype=E4M3)
+    with pytest.raises(ValueError):
+        cache.rows(cache.k[0], at)
