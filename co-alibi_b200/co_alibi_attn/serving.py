@@ -26,7 +26,7 @@ too) with ``scales`` = (k_scales, v_scales), float32 [n_pages, Hkv, page_size / 
 block of 16 tokens of a page and head.  A value is its code times the scale of its block.
 ``append_paged_kv`` writes scales that are powers of two, the least by which a block's largest
 value is at most 448 (and at least 2^-100): a code's relative error is at most 2^-4 then, or 2^-10 of the scale, that is
-2^-18 to 2^-17 of the block's largest, for what is smaller.  A block that already holds tokens keeps its scale unless
+less than 2^-17 of the block's largest, for what is smaller.  A block that already holds tokens keeps its scale unless
 a new one is too large for it, and if so the old codes move to the new scale, which changes none but
 those that fall below 2^-6 of it.  Reading and attention take scales that another program wrote as well: any finite ones, 0
 and negative ones among them (attention's weights of values in blocks below 2^-100 are rounded as those of 2^-100).  Slots behind a request's tokens hold nothing, and those before ``start`` in

@@ -223,7 +223,10 @@ def tree_step(model, cache, last, drafts, parents, generator=None, **sampling):
     the cache), ``drafts`` [B, T] and ``parents`` [B, T] as in ``tree_words``.  A token is
     sampled after every row; from row 0 on, a draft that equals its parent's sample is
     accepted, and the first sample that no draft matches ends the step.  That draws from the
-    model's own distribution whatever the drafts are.  Drafts behind the cache's capacity, and
+    model's own distribution whatever the drafts are; over a cache in 8 bits, but for one rounding:
+    drafts share the scale of the block that the context ends in, so a large key or value among
+    them, accepted or not, rounds those in the block that are below 2^-14 of its size to steps of
+    about 2^-17 of it, and the block keeps that scale.  Drafts behind the cache's capacity, and
     tokens below 0, count as none: the step ends before them.
 
     Returns (tokens [B, T + 1], n [B] int32): the first n[b] of tokens[b] are new, the last of
