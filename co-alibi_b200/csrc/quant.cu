@@ -134,7 +134,7 @@ extern "C" int coalibi_paged_append8(const CoalibiPagedAppendArgs* a, const Coal
     return COALIBI_ERR_ALIGNMENT;
   if ((rc = check_codes(sc, a->k_pages, a->v_pages, a->k_page_stride, a->v_page_stride, a->n_pages, a->Hkv))) return rc;
   Append8Params p{};
-  p.blocks = (a->S + kQuantBlock - 2) / kQuantBlock + 1;
+  p.blocks = (int)(((long long)a->S + kQuantBlock - 2) / kQuantBlock) + 1;
   // a head to a warp, up to eight warps to a CTA
   p.chunks = (a->Hkv + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
   const int threads = 32 * ((a->Hkv + p.chunks - 1) / p.chunks);
