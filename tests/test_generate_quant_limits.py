@@ -112,3 +112,82 @@ def test_rows_of_codes_are_refused():
     cache = PagedCache(model, 2, 20, 16, kv_dtype=E4M3)
     with pytest.raises(ValueError):
         cache.rows(cache.k[0], at)
+
+
+def _sampled_path(sampled, drafts, parents, slots):
+    """How many tokens a tree step of greedy samples accepts: the walk from row 0 along drafts with a slot."""
+    n, at = 1, 0
+    while True:
+        next_ = [t for t in range(drafts.shape[0]) if int(parents[t]) == at and t + 1 < slots and int(drafts[t]) == int(sampled[at])]
+        if not next_:
+            return n
+        n, at = n + 1, next_[0] + 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_drafts_at_the_end_of_a_cache_in_8_bits(qk_norm):
+    """A chain of drafts over caches with room for some of them.  What is accepted follows the cache's own samples (the same
+    rows give the same logits again: their scales are there already); a full cache keeps its codes and is reported."""
+    from co_alibi_gpt import generate as gen
+    model = _normed("cuda", 32) if qk_norm else limits._model("cuda", 32)
+    counts = torch.tensor([28, 31, 20], dtype=torch.int32, device="cuda")
+    prompt = limits._tokens(3, 31, "cuda")
+
+    def start():
+        cache = gen.PagedCache(model, 3, 32, page_size=16, spare=0, kv_dtype=E4M3)
+        return cache, gen.prefill(model, cache, prompt, counts).argmax(-1)
+
+    cache, last = start()
+    chain = [last]
+    room = cache.capacity - cache.lens
+    for _ in range(6):  # greedy tokens, one at a time, where there is room
+        chain.append(gen.extend(model, cache, chain[-1][:, None])[:, 0].nan_to_num(nan=-1.0).argmax(-1))
+        cache.lens += 1
+    limits._status("cuda")
+    drafts, parents = torch.stack(chain[1:], 1), torch.arange(6, device="cuda").expand(3, 6)
+    cache, last = start()
+    words, depths = gen.tree_words(torch.where(torch.arange(1, 7, device="cuda") < room[:, None], parents, -1))
+    sampled = gen.extend(model, cache, torch.cat((last[:, None], drafts), 1), words, depths, room).nan_to_num(nan=-1.0).argmax(-1)
+    assert limits._status("cuda") == 0
+    want = [_sampled_path(sampled[b], drafts[b], parents[b], int(room[b])) for b in range(3)]
+    tokens, n = gen.tree_step(model, cache, last, drafts, parents, temperature=0.0)
+    assert limits._status("cuda") == 0 and n.tolist() == want and want[1] == 1 and want[0] >= 2 and want[2] >= 4
+    assert cache.lens.tolist() == [int(c) + m for c, m in zip(counts, want)]
+    for b, m in enumerate(want):
+        assert torch.equal(tokens[b, :m], sampled[b, :m])
+    # full now
+    cache.lens[0] = cache.capacity
+    before = [x.view(torch.uint8)[cache.table[:2].long()].clone() for x in cache.k + cache.v]
+    scales = [s[cache.table[:2].long()].clone() for pair in cache.scales for s in pair]
+    tokens, n = gen.tree_step(model, cache, tokens[:, 0], drafts[:, :1], parents[:, :1], temperature=0.0)
+    assert n.tolist()[:2] == [0, 0] and n[2] >= 1 and (tokens[:2] == -1).all() and limits._status("cuda") != 0
+    assert all(torch.equal(a, x.view(torch.uint8)[cache.table[:2].long()]) for a, x in zip(before, cache.k + cache.v))
+    assert all(torch.equal(a, s[cache.table[:2].long()]) for a, s in zip(scales, (s for pair in cache.scales for s in pair)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["test_a_model_without_a_token_to_draw_ends_in_minus_one", "test_counts_outside_the_prompt", "test_no_new_tokens",
+                                  "test_an_absent_token_confirms_nothing"])
+def test_limits_of_a_cache_in_8_bits(name, monkeypatch):
+    """Those that ask for no more bits than e4m3 has: statuses, lengths, absent tokens, a prompt's own logits."""
+    from co_alibi_gpt import generate as gen
+    real = gen.PagedCache
+    monkeypatch.setattr(gen, "PagedCache", lambda *a, **kw: real(*a, **{**kw, "kv_dtype": E4M3}))
+    getattr(limits, name)("cuda", monkeypatch)
+
+
+@pytest.mark.gpu
+def test_rows_of_a_chunk_past_the_end_of_a_cache_in_8_bits():
+    """Without logits, and reported; the rows that fit have those of a chunk of them alone (two forms of the attention over
+    the same codes: 0.1, as in the other tests of logits)."""
+    from co_alibi_gpt import generate as gen
+    model = limits._model("cuda", 32)
+    tok = limits._tokens(2, 36, "cuda")
+    cache = gen.PagedCache(model, 2, 32, page_size=16, spare=0, kv_dtype=E4M3)
+    gen.prefill(model, cache, tok[:, :30], torch.tensor([30, 25], dtype=torch.int32, device="cuda"))
+    chunk = torch.stack((tok[0, 30:35], tok[1, 25:30]))
+    logits = gen.extend(model, cache, chunk)
+    assert logits[0, 2:].isnan().all() and torch.isfinite(logits[1]).all() and limits._status("cuda") != 0
+    fits = gen.extend(model, cache, chunk[:, :2])
+    assert limits._status("cuda") == 0 and (logits[:, :2].float() - fits.float()).abs().max() < 0.1 and fits.float().abs().max() > 3
