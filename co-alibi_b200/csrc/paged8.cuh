@@ -4,8 +4,8 @@
 //
 // With a power of two for a scale nothing but the exponent moves: a code keeps its three mantissa
 // bits whatever the scale is, so raising a block's scale for a larger token that joins it later
-// leaves the tokens before it as they are (only what falls below 2^-9 of the new scale rounds), and a
-// token that is read back and appended again gets the same code.
+// leaves the tokens before it as they are (only what falls below 2^-6 of the new scale rounds), and a
+// token that is read back whole (in bfloat16) and appended again, under a scale that does not grow, gets the same code.
 #pragma once
 
 #include <cuda_fp16.h>
