@@ -452,10 +452,11 @@ __global__ void __launch_bounds__(kReadThreads, 4) coalibi_paged_read8_kernel(co
 // which are the two halves of an A fragment when Q's columns are taken in the same order; transposed, it
 // gives 2 keys x 2 columns, and the columns of a pair go to rows g and g + 8 of the tile.
 //
-// What bounds it.  With 4 rows to a kv head, 4 contexts of 65,537 to 131,071 keys take 124 us, all of the measured copy
-// rate: memory (132 with the joining under the power cap, whose clock makes the instructions count).  16 contexts of up
-// to 8191 keys take 28 us and 4.4 of joining against 20.6 of reading: the starts and
-// ends of the items.  With 16 and 32 rows the instructions bound it (56 and 79 us where 8 rows take 35): a score costs a
+// What bounds it.  With 4 rows to a kv head, 4 contexts of 65,537 to 131,071 keys take 125 us, 0.98 of the measured copy
+// rate: memory (130 to 138 a pass with 6 of joining, under the power cap, whose clock makes the instructions count).  With
+// 64 columns a score costs the same for half the bytes: 126 us for 92 of reading at 12 heads.  16 contexts of up
+// to 8191 keys take 28 us and 4.5 of joining against 20.5 of reading: the starts and
+// ends of the items.  With 16 and 32 rows the instructions bound it (56 and 73 us where 8 rows take 31): a score costs a
 // row the same whatever the codes' width is, so 8 bits gain little over 16 there.
 // 16 or 32 rows are two blocks of columns of a warp, or of two warps that share the ring.
 // ---------------------------------------------------------------------------
@@ -516,7 +517,7 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return ma
 
 // HALF: at most 4 rows.  The product leaves half of the lanes with columns of no row, so those lanes (tig 2 and 3) take
 // the second rows of the others: a lane has one row of its 4 keys, in .x, and .y is dead.  The long contexts above took
-// 127 us without it, and 143 with the joining under the power cap.
+// 127 us without it.
 template <int D, bool BF16, int NT, int RW, int WARPS, bool HALF>
 __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::CTAS))
     coalibi_paged8_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -984,7 +985,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
         group_sync();
       }
       // ---- O^T += V^T P^T.  P goes to float16 (half an ulp of each weight, which averages out over the
-      // keys; the sum takes them unrounded), and from the accumulators' layout to the operand's by a transpose.
+      // keys, and nothing of one below 2^-25 of the largest contribution; the sum takes them unrounded), and from the accumulators' layout to the operand's by a transpose.
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll

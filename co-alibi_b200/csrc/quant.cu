@@ -92,10 +92,10 @@ int launch_wide8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, 
 template <int D, bool BF16>
 int launch_paged8(const CUtensorMap& tk, const CUtensorMap& tv, Paged8Params& p, int sms, cudaStream_t s) {
   const int rows = p.Hq / p.Hkv * p.Sq;
-  // Up to 4 rows lanes share what 8 columns leave over (4 rows of long contexts, without / with it: 143 / 132 us; the
-  // shuffles it takes would buy nothing with more rows).  The wide kernel costs the same for 1 to 64 rows.  8 ragged contexts up to 16k keys, narrow / wide: 16 rows 62 /
-  // 67 us, 20 rows 81 / 79, 32 rows 87 / 79; 32 rows of 64 contexts of 200 keys 36 / 65, of 1000 keys 97 / 104;
-  // 32 rows of D = 64 65 / 79.
+  // Up to 4 rows lanes share what 8 columns leave over (4 rows of long contexts, without / with it: 127 / 124 us of kernel;
+  // the shuffles it takes would buy nothing with more rows).  The wide kernel costs the same for 1 to 64 rows.  8 ragged
+  // contexts up to 16k keys, narrow / wide: 16 rows 55 / 70 us, 20 rows 73 / 71, 32 rows 78 / 71 (bfloat16 81 / 71); 32 rows
+  // of 64 contexts of 200 keys 27 / 58, of 1000 keys 89 / 98; 32 rows of D = 64 56 / 65.
   if (rows <= 4) return launch_rows8<D, BF16, 1, 1, true>(tk, tv, p, sms, s);
   if (rows <= 8) return launch_rows8<D, BF16, 1, 1>(tk, tv, p, sms, s);
   if (rows <= 16) return launch_rows8<D, BF16, 2, 1>(tk, tv, p, sms, s);
