@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ uint64_t s_full[KG * L::NBUF];
   __shared__ int s_abort;
-  __shared__ volatile int s_fail[KG];
+  __shared__ volatile int s_fail[KG], s_plain[KG][2];
   __shared__ int s_pre[128], s_warp[4], s_find;
   __shared__ float4 s_stat[KG > 1 ? KG * L::ROWS : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -743,11 +743,22 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
 
     for (int st = nsteps - 1; st >= 0; --st) {
       if (ok && !mbar_wait(&full[loads.drain], loads.phase, guard)) s_fail[kg] = st + 1;
+      // Whether every key is of the context and every scale plain.  One warp decides for the group, which meets again in
+      // the other steps: were a page or scale written to meanwhile, its warps might disagree and wait for each other.
+      auto plain = [&]() {
+        return lo + (st + 1) * kPagedStep <= min(hi, ctx) && (gone_q >> (2 * loads.drain) & 3) == 0 &&
+               !__any_sync(0xffffffffu, odd_scale(vs_q[0]));
+      };
+      if (RW > 1 && rwarp == 0) {
+        const bool mine = plain();
+        if (lane == 0) s_plain[kg][st & 1] = mine;
+      }
       group_sync();  // all are done with step st + 1, whose slot is loaded next
       // the same for the group's warps, which meet again in the masked steps: a wait of this step or
       // of one before it ran out (one that a faster warp already meets in the next step counts there)
       ok = s_fail[kg] <= st;
       if (!ok) continue;
+      const bool all = RW > 1 ? s_plain[kg][st & 1] != 0 : plain();
       const int slot = loads.drain;
       loads.landed();
       const float k_scale = ks_q[0], v_scale = vs_q[0];
@@ -778,7 +789,6 @@ __global__ void __launch_bounds__(32 * WARPS, (Paged8Layout<D, NT, RW, WARPS>::C
       }
       // ---- which of this lane's 4 keys each of its rows sees: bit 8 n + 4 x + c
       const uint32_t gone = gone_q >> (2 * slot) & 3;
-      const bool all = kb + kPagedStep <= min(hi, ctx) && gone == 0 && !__any_sync(0xffffffffu, odd_scale(v_scale));
       uint32_t vis = 0xffffu;
       if (!all) {
         vis = 0;
